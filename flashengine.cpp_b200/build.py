@@ -33,9 +33,11 @@ NVCC_FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC,-O2", "-Xpt
 CXX_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-Wall", "-Wextra"]
 
 KV_SOURCES = ["fe_kv_ops.cu", "fe_attn.cu", "fe_decode.cu", "fe_prefill_tc.cu", "fe_rope_accept.cu",
-              "fe_plan_device.cu", "fe_attn_plan.cpp", "fe_kv_fork.cpp"]
+              "fe_plan_device.cu", "fe_kv8_ops.cu", "fe_kv8_decode.cu", "fe_kv8_rows.cu",
+              "fe_attn_plan.cpp", "fe_kv_fork.cpp"]
 SHIM_SOURCES = ["fe_native_cuda_shim.cpp"]
-HEADERS = ["fe_common.cuh", "fe_attn_common.cuh", "fe_attn_plan.h", "fe_tcgen05.cuh"]
+HEADERS = ["fe_common.cuh", "fe_attn_common.cuh", "fe_attn_plan.h", "fe_tcgen05.cuh",
+           "fe_kv8_common.cuh", "fe_kv8_attn.h"]
 
 
 def nvcc() -> str:

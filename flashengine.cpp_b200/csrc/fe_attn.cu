@@ -13,6 +13,8 @@
 //    split-K decode kernel (fe_decode.cu); multi-row items (chunked prefill,
 //    speculative verify) go to the tcgen05/TMEM kernel (fe_prefill_tc.cu).
 //    Tensor maps of the K and V pools are encoded once per pool address.
+//  * fe_kv8_plan_create / fe_kv8_attn_run: the same plan and lists over the
+//    8-bit cache (fe_kv8_decode.cu, fe_kv8_rows.cu).
 #include <cstdlib>
 #include <cstring>
 #include <mutex>
@@ -20,6 +22,7 @@
 #include <string>
 
 #include "fe_attn_common.cuh"
+#include "fe_kv8_attn.h"
 #include "fe_plan_device.h"
 
 namespace fe {
@@ -126,6 +129,43 @@ int encode_decode_map(CUtensorMap* map, const void* pool, int dtype, int hkv, in
   return encode_3d(map, pool, dtype, dims, strides, box);
 }
 
+int encode_codes(CUtensorMap* map, const void* codes, int rank, const cuuint64_t* dims,
+                 const cuuint64_t* strides, const cuuint32_t* box) {
+  EncodeTiledFn fn = get_encode_fn();
+  if (!fn) return fail(FE_ERR_CUDA, "cuTensorMapEncodeTiled unavailable from the driver");
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, rank, const_cast<void*>(codes), dims,
+                        strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(FE_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult " + std::to_string(r));
+  return FE_OK;
+}
+
+// 8-bit decode kernel: codes as [hkv*dim/128][cache_slots][128], a box = the
+// 16 slots of a tile x 128 codes of all `heads` heads' boxes (a contiguous
+// block of the page), landing 128 dims at a time, 16 swizzled rows each.
+int encode_kv8_decode_map(CUtensorMap* map, const void* codes, int hkv, int dim, int heads,
+                          int64_t cache_slots) {
+  const cuuint64_t dims[3] = {128, cuuint64_t(cache_slots), cuuint64_t(hkv) * (dim / 128)};
+  const cuuint64_t strides[2] = {cuuint64_t(hkv) * dim, 128};
+  const cuuint32_t box[3] = {128, kTileTokens, cuuint32_t(heads * (dim / 128))};
+  return encode_codes(map, codes, 3, dims, strides, box);
+}
+
+// 8-bit row kernel: codes as [cache_slots/8][hkv*dim/128][8][128]; a box = a
+// 16-token piece of one KV head, landing as [8-slot group][box][8 rows of
+// 128 B].
+int encode_kv8_rows_map(CUtensorMap* map, const void* codes, int hkv, int dim,
+                        int64_t cache_slots) {
+  const cuuint64_t boxes = cuuint64_t(dim / 128);
+  const cuuint64_t dims[4] = {128, 8, cuuint64_t(hkv) * boxes, cuuint64_t(cache_slots / 8)};
+  const cuuint64_t strides[3] = {cuuint64_t(hkv) * dim, 128, cuuint64_t(hkv) * dim * 8};
+  const cuuint32_t box[4] = {128, 8, cuuint32_t(boxes), 2};
+  return encode_codes(map, codes, 4, dims, strides, box);
+}
+
 }  // namespace
 }  // namespace fe
 
@@ -135,6 +175,7 @@ struct fe_attn_plan {
   PlanConfig cfg{};
   int dtype = 0;
   bool host_only = false;
+  bool kv8 = false;  // made by fe_kv8_plan_create: serves fe_kv8_attn_run only
   int device = -1;
   // device workspaces
   uint8_t* d_meta = nullptr;
@@ -202,7 +243,7 @@ int gcd8(int hkv) {
 }
 
 PlanConfig make_config(int hq, int hkv, int dim, int page, int max_batch, int max_pages,
-                       int num_blocks, int grid_cap, int dec_grid_cap) {
+                       int num_blocks, int grid_cap, int dec_grid_cap, bool kv8) {
   PlanConfig c{};
   c.hq = hq;
   c.hkv = hkv;
@@ -218,6 +259,8 @@ PlanConfig make_config(int hq, int hkv, int dim, int page, int max_batch, int ma
   c.dec_heads = dim == kWideHeadDim ? (hkv % 2 == 0 ? 2 : 1) : gcd8(hkv);
   c.row_group_blocks = 8;  // 128 packed rows per tcgen05 work item
   c.row_split = false;      // the tcgen05 kernel walks an item's whole key range
+  c.cut_rows = dim == kWideHeadDim || kv8;
+  c.elem_bytes = kv8 ? 1 : 2;
   int64_t items = int64_t(max_batch) * hkv * 64;
   if (items < 8192) items = 8192;
   if (items > (1 << 20)) items = 1 << 20;
@@ -235,6 +278,7 @@ PlanConfig make_config(int hq, int hkv, int dim, int page, int max_batch, int ma
   c.hbm_gbs = 5800.f;
   c.dec_fixed_us = 10.f;
   c.row_piece_us = dim == kWideHeadDim ? 0.4f : 0.2f;
+  if (kv8) c.row_piece_us *= 0.6f;  // the 8-bit row kernel's measured rate
   return c;
 }
 
@@ -262,10 +306,10 @@ void destroy(fe_attn_plan* p) {
 
 }  // namespace
 
-extern "C" {
+namespace {
 
-int fe_attn_plan_create(int hq, int hkv, int dim, int page, int max_batch, int max_pages,
-                        int dtype, int num_blocks, fe_attn_plan** plan_out) {
+int create_plan(int hq, int hkv, int dim, int page, int max_batch, int max_pages, int dtype,
+                int num_blocks, bool kv8, fe_attn_plan** plan_out) {
   if (!plan_out) return fail(FE_ERR_INVALID_ARGUMENT, "fe_attn_plan_create: plan_out is null");
   *plan_out = nullptr;
   int rc = check_shape(hq, hkv, dim, page, max_batch, max_pages, dtype, num_blocks);
@@ -279,8 +323,9 @@ int fe_attn_plan_create(int hq, int hkv, int dim, int page, int max_batch, int m
     return fail(FE_ERR_NO_DEVICE, "fe_attn_plan_create: needs an sm_100 (B200) device");
   auto* p = new (std::nothrow) fe_attn_plan();
   if (!p) return fail(FE_ERR_INVALID_ARGUMENT, "fe_attn_plan_create: out of host memory");
-  p->cfg = make_config(hq, hkv, dim, page, max_batch, max_pages, num_blocks, sms, sms);
+  p->cfg = make_config(hq, hkv, dim, page, max_batch, max_pages, num_blocks, sms, sms, kv8);
   p->dtype = dtype;
+  p->kv8 = kv8;
   p->device = dev;
   p->meta_cap = meta_capacity(p->cfg);
   cudaError_t e = cudaMalloc(&p->d_meta, p->meta_cap);
@@ -305,10 +350,8 @@ int fe_attn_plan_create(int hq, int hkv, int dim, int page, int max_batch, int m
   return FE_OK;
 }
 
-// Test hook: a plan with no device state, for exercising the planner on a
-// host without a GPU. fe_attn_plan_prepare() then only builds the work list.
-int fe_attn_plan_create_host(int hq, int hkv, int dim, int page, int max_batch, int max_pages,
-                             int dtype, int num_blocks, int grid_cap, fe_attn_plan** plan_out) {
+int create_host_plan(int hq, int hkv, int dim, int page, int max_batch, int max_pages, int dtype,
+                     int num_blocks, int grid_cap, bool kv8, fe_attn_plan** plan_out) {
   if (!plan_out) return fail(FE_ERR_INVALID_ARGUMENT, "plan_out is null");
   *plan_out = nullptr;
   int rc = check_shape(hq, hkv, dim, page, max_batch, max_pages, dtype, num_blocks);
@@ -317,12 +360,40 @@ int fe_attn_plan_create_host(int hq, int hkv, int dim, int page, int max_batch, 
   auto* p = new (std::nothrow) fe_attn_plan();
   if (!p) return fail(FE_ERR_INVALID_ARGUMENT, "out of host memory");
   p->cfg = make_config(hq, hkv, dim, page, max_batch, max_pages, num_blocks, grid_cap,
-                       std::max(1, grid_cap / 2));
+                       std::max(1, grid_cap / 2), kv8);
   p->dtype = dtype;
+  p->kv8 = kv8;
   p->host_only = true;
   p->meta_cap = meta_capacity(p->cfg);
   *plan_out = p;
   return FE_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int fe_attn_plan_create(int hq, int hkv, int dim, int page, int max_batch, int max_pages,
+                        int dtype, int num_blocks, fe_attn_plan** plan_out) {
+  return create_plan(hq, hkv, dim, page, max_batch, max_pages, dtype, num_blocks, false, plan_out);
+}
+
+int fe_kv8_plan_create(int hq, int hkv, int dim, int page, int max_batch, int max_pages, int dtype,
+                       int num_blocks, fe_attn_plan** plan_out) {
+  return create_plan(hq, hkv, dim, page, max_batch, max_pages, dtype, num_blocks, true, plan_out);
+}
+
+// Test hook: a plan with no device state, for exercising the planner on a
+// host without a GPU. fe_attn_plan_prepare() then only builds the work list.
+int fe_attn_plan_create_host(int hq, int hkv, int dim, int page, int max_batch, int max_pages,
+                             int dtype, int num_blocks, int grid_cap, fe_attn_plan** plan_out) {
+  return create_host_plan(hq, hkv, dim, page, max_batch, max_pages, dtype, num_blocks, grid_cap,
+                          false, plan_out);
+}
+int fe_kv8_plan_create_host(int hq, int hkv, int dim, int page, int max_batch, int max_pages,
+                            int dtype, int num_blocks, int grid_cap, fe_attn_plan** plan_out) {
+  return create_host_plan(hq, hkv, dim, page, max_batch, max_pages, dtype, num_blocks, grid_cap,
+                          true, plan_out);
 }
 
 int fe_attn_plan_destroy(fe_attn_plan* plan) {
@@ -482,6 +553,99 @@ int fe_attn_plan_debug_device_meta(const fe_attn_plan* p, void* dst, int64_t cap
   return FE_OK;
 }
 
+}  // extern "C"
+
+namespace {
+
+template <typename T>
+AttnArgs<T> attn_args(const fe_attn_plan* p, const void* q, void* out, int view, int q_map_rows) {
+  return AttnArgs<T>{p->d_meta, static_cast<const T*>(q), static_cast<T*>(out), p->d_partials,
+                     p->d_counters, device_error_word(), p->cfg.hq, p->cfg.hq / p->cfg.hkv,
+                     p->cfg.page, view, 1.4426950408889634f / sqrtf(float(p->cfg.dim)),
+                     q_map_rows};
+}
+
+// Launch the prepared lists' kernels and the merges of their split units.
+// `args`: the AttnArgs of the plan's dtype; dec / rows launch the two kernels
+// on a stream.
+template <typename Dec, typename Rows>
+int launch_lists(fe_attn_plan* p, int view, int grid_rows, int grid_dec, const void* args,
+                 cudaStream_t s, Dec dec, Rows rows) {
+  MetaHeader h;
+  std::memcpy(&h, p->last.meta.data(), sizeof(h));
+  const int dim = p->cfg.dim;
+  // split units of the decode list are merged by a second, dependent kernel
+  int grid_merge = 0;
+  if (grid_dec > 0) grid_merge = p->fixed_grid ? p->cfg.dec_grid_cap : h.n_groups[2];
+  // Merge CTAs per split unit: one warp per record row, 32 rows per CTA. The
+  // host plan knows its units' rows; a graph plan (fixed launch geometry) or
+  // a device-built plan takes the bound: H heads x 16 packed rows for the
+  // decode list, 128 rows for a row list.
+  auto merge_y = [&](int list) {
+    const int bound = list == 2 ? p->cfg.dec_heads * kRowBlock : 128;
+    const int n = (p->fixed_grid || p->device_planned) ? bound : p->last.split_rows[list];
+    return std::max(1, (n + 31) / 32);
+  };
+  // split pieces of the row list (where its key ranges are cut across CTAs)
+  // are merged by the merge kernel over that list
+  const int grid_row_merge =
+      !p->cfg.cut_rows || grid_rows == 0 ? 0
+                                         : (p->fixed_grid ? p->cfg.grid_cap : h.n_groups[view]);
+  // A mixed step planned side by side (the two lists' grids sum to the SMs)
+  // forks: the row kernel runs on the plan's side stream while the decode
+  // kernel and its merge run on `stream`, which then waits for the side.
+  // They read the same q and pools and write disjoint output rows and split
+  // records.
+  const bool fork = grid_dec > 0 && grid_rows > 0 && !p->fixed_grid && p->last.concurrent;
+  cudaStream_t rs = s;
+  if (fork) {
+    FE_CUDA_TRY(cudaEventRecord(p->fork_ev, s));
+    FE_CUDA_TRY(cudaStreamWaitEvent(p->side, p->fork_ev, 0));
+    rs = p->side;
+  }
+  auto launch_all = [&]() -> int {
+    // Side by side, a merge waits for its kernel's grid to complete before
+    // it takes an SM (a programmatic dependent would sit on SMs the other
+    // kernel needs while it waits).
+    if (grid_rows > 0 && fork) {
+      int rc = rows(rs);
+      if (rc == FE_OK)
+        rc = decode_merge_launch(p->dtype, dim, view, args, grid_row_merge, merge_y(view), rs,
+                                 false);
+      if (rc != FE_OK) return rc;
+    }
+    if (grid_dec > 0) {
+      int rc = dec(s);
+      if (rc == FE_OK)
+        rc = decode_merge_launch(p->dtype, dim, 2, args, grid_merge, merge_y(2), s, !fork);
+      if (rc != FE_OK) return rc;
+    }
+    if (grid_rows > 0 && !fork) {
+      int rc = rows(s);
+      if (rc == FE_OK)
+        rc = decode_merge_launch(p->dtype, dim, view, args, grid_row_merge, merge_y(view), s,
+                                 true);
+      return rc;
+    }
+    return FE_OK;
+  };
+  const int rc = launch_all();
+  if (fork) {
+    // join even after a failed launch, so `stream` never runs ahead of the side
+    cudaError_t e1 = cudaEventRecord(p->join_ev, p->side);
+    cudaError_t e2 = cudaStreamWaitEvent(s, p->join_ev, 0);
+    if (rc == FE_OK && e1 != cudaSuccess) return cuda_fail(e1, "fe_attn_run: join record");
+    if (rc == FE_OK && e2 != cudaSuccess) return cuda_fail(e2, "fe_attn_run: join wait");
+  }
+  if (rc != FE_OK) return rc;
+  FE_CUDA_TRY(cudaGetLastError());
+  return FE_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
 int fe_attn_run(fe_attn_plan* p, const void* q, const void* k_pool, const void* v_pool, void* out,
                 int causal, void* stream) {
   return fe_attn_run_lists(p, q, k_pool, v_pool, out, causal, FE_ATTN_LISTS_ALL, stream);
@@ -491,6 +655,8 @@ int fe_attn_run_lists(fe_attn_plan* p, const void* q, const void* k_pool, const 
                       void* out, int causal, int lists, void* stream) {
   if (!p) return fail(FE_ERR_INVALID_ARGUMENT, "fe_attn_run: plan is null");
   if (p->host_only) return fail(FE_ERR_INVALID_ARGUMENT, "fe_attn_run: host-only plan");
+  if (p->kv8)
+    return fail(FE_ERR_INVALID_ARGUMENT, "fe_attn_run: a plan of fe_kv8_plan_create");
   if (!p->prepared) return fail(FE_ERR_INVALID_ARGUMENT, "fe_attn_run: plan not prepared");
   const int view = causal ? 1 : 0;
   // A plan prepared for graph capture launches both kernels at full width
@@ -508,7 +674,6 @@ int fe_attn_run_lists(fe_attn_plan* p, const void* q, const void* k_pool, const 
   const int64_t cache_slots = int64_t(p->cfg.num_blocks + 1) * p->cfg.page;
   const int H = p->cfg.dec_heads;
   const int dim = p->cfg.dim;
-  const bool wide = dim == kWideHeadDim;
   if (k_pool != p->kmap_ptr) {
     int rc = encode_pool_map(&p->kmap, k_pool, p->dtype, p->cfg.hkv, dim, cache_slots);
     if (rc != FE_OK) return rc;
@@ -531,97 +696,80 @@ int fe_attn_run_lists(fe_attn_plan* p, const void* q, const void* k_pool, const 
   }
   MetaHeader h;
   std::memcpy(&h, p->last.meta.data(), sizeof(h));
-  // split units of the decode list are merged by a second, dependent kernel
-  int grid_merge = 0;
-  if (grid_dec > 0) grid_merge = p->fixed_grid ? p->cfg.dec_grid_cap : h.n_groups[2];
-  // Merge CTAs per split unit: one warp per record row, 32 rows per CTA. The
-  // host plan knows its units' rows; a graph plan (fixed launch geometry) or
-  // a device-built plan takes the bound: H heads x 16 packed rows for the
-  // decode list, 128 rows for a row list.
-  auto merge_y = [&](int list) {
-    const int bound = list == 2 ? p->cfg.dec_heads * kRowBlock : 128;
-    const int rows = (p->fixed_grid || p->device_planned) ? bound : p->last.split_rows[list];
-    return std::max(1, (rows + 31) / 32);
-  };
   // the row kernel's Q tiles come from a tensor map over this call's q
   // (the prepared step's query rows, which a graph plan keeps fixed)
   CUtensorMap qmap;
   std::memset(&qmap, 0, sizeof(qmap));  // unused when G does not divide 128
   int q_map_rows = 0;
-  if (grid_rows > 0 && 128 % (p->cfg.hq / p->cfg.hkv) == 0 && h.rows > 0) {
-    int rc = encode_q_map(&qmap, q, p->dtype, p->cfg.hq, dim, h.rows, p->cfg.hq / p->cfg.hkv);
+  const int G = p->cfg.hq / p->cfg.hkv;
+  if (grid_rows > 0 && 128 % G == 0 && h.rows > 0) {
+    int rc = encode_q_map(&qmap, q, p->dtype, p->cfg.hq, dim, h.rows, G);
     if (rc != FE_OK) return rc;
     q_map_rows = h.rows;
   }
-  // split pieces of the row list (head_dim 256 steps with few row items)
-  // are merged by the merge kernel over that list
-  const int grid_row_merge =
-      !wide || grid_rows == 0 ? 0 : (p->fixed_grid ? p->cfg.grid_cap : h.n_groups[view]);
-  const float scale_log2 = 1.4426950408889634f / sqrtf(float(dim));
-  auto s = static_cast<cudaStream_t>(stream);
-  const int G = p->cfg.hq / p->cfg.hkv;
   const CUtensorMap& kd = p->per_head_tma ? p->kmap : p->kmap_dec;
   const CUtensorMap& vd = p->per_head_tma ? p->vmap : p->vmap_dec;
-  // A mixed step planned side by side (the two lists' grids sum to the SMs)
-  // forks: the row kernel runs on the plan's side stream while the decode
-  // kernel and its merge run on `stream`, which then waits for the side.
-  // They read the same q and pools and write disjoint output rows and split
-  // records.
-  const bool fork = grid_dec > 0 && grid_rows > 0 && !p->fixed_grid && p->last.concurrent;
-  cudaStream_t rs = s;
-  if (fork) {
-    FE_CUDA_TRY(cudaEventRecord(p->fork_ev, s));
-    FE_CUDA_TRY(cudaStreamWaitEvent(p->side, p->fork_ev, 0));
-    rs = p->side;
-  }
-  auto launch_all = [&](const auto& a) -> int {
-    // Side by side, a merge waits for its kernel's grid to complete before
-    // it takes an SM (a programmatic dependent would sit on SMs the other
-    // kernel needs while it waits).
-    if (grid_rows > 0 && fork) {
-      int rc = prefill_tc_launch(p->dtype, dim, p->kmap_tc, p->vmap_tc, qmap, &a, grid_rows, rs);
-      if (rc == FE_OK)
-        rc = decode_merge_launch(p->dtype, dim, view, &a, grid_row_merge, merge_y(view), rs,
-                                 false);
-      if (rc != FE_OK) return rc;
-    }
-    if (grid_dec > 0) {
-      int rc = decode_launch(p->dtype, dim, H, kd, vd, p->per_head_tma, &a, grid_dec, s);
-      if (rc == FE_OK)
-        rc = decode_merge_launch(p->dtype, dim, 2, &a, grid_merge, merge_y(2), s, !fork);
-      if (rc != FE_OK) return rc;
-    }
-    if (grid_rows > 0 && !fork) {
-      int rc = prefill_tc_launch(p->dtype, dim, p->kmap_tc, p->vmap_tc, qmap, &a, grid_rows, s);
-      if (rc == FE_OK)
-        rc = decode_merge_launch(p->dtype, dim, view, &a, grid_row_merge, merge_y(view), s, true);
-      return rc;
-    }
-    return FE_OK;
+  auto run = [&](const auto& a) -> int {
+    return launch_lists(
+        p, view, grid_rows, grid_dec, &a, static_cast<cudaStream_t>(stream),
+        [&](cudaStream_t s) {
+          return decode_launch(p->dtype, dim, H, kd, vd, p->per_head_tma, &a, grid_dec, s);
+        },
+        [&](cudaStream_t s) {
+          return prefill_tc_launch(p->dtype, dim, p->kmap_tc, p->vmap_tc, qmap, &a, grid_rows, s);
+        });
   };
-  int rc;
-  if (p->dtype == FE_DTYPE_BF16) {
-    AttnArgs<__nv_bfloat16> a{p->d_meta, static_cast<const __nv_bfloat16*>(q),
-                              static_cast<__nv_bfloat16*>(out), p->d_partials, p->d_counters,
-                              device_error_word(), p->cfg.hq, G, p->cfg.page, view, scale_log2,
-                              q_map_rows};
-    rc = launch_all(a);
-  } else {
-    AttnArgs<__half> a{p->d_meta, static_cast<const __half*>(q), static_cast<__half*>(out),
-                       p->d_partials, p->d_counters, device_error_word(), p->cfg.hq, G,
-                       p->cfg.page, view, scale_log2, q_map_rows};
-    rc = launch_all(a);
+  if (p->dtype == FE_DTYPE_BF16)
+    return run(attn_args<__nv_bfloat16>(p, q, out, view, q_map_rows));
+  return run(attn_args<__half>(p, q, out, view, q_map_rows));
+}
+
+// fe_attn_run over the 8-bit cache. Its tensor maps are encoded by each call
+// (host work of a few microseconds at most, overlapped with the GPU).
+int fe_kv8_attn_run(fe_attn_plan* p, const void* q, const uint8_t* k_codes, const uint8_t* v_codes,
+                    const uint8_t* k_exp, const uint8_t* v_exp, void* out, int causal,
+                    void* stream) {
+  if (!p) return fail(FE_ERR_INVALID_ARGUMENT, "fe_kv8_attn_run: plan is null");
+  if (p->host_only) return fail(FE_ERR_INVALID_ARGUMENT, "fe_kv8_attn_run: host-only plan");
+  if (!p->kv8)
+    return fail(FE_ERR_INVALID_ARGUMENT, "fe_kv8_attn_run: needs a plan of fe_kv8_plan_create");
+  if (!p->prepared) return fail(FE_ERR_INVALID_ARGUMENT, "fe_kv8_attn_run: plan not prepared");
+  const int view = causal ? 1 : 0;
+  const int grid_rows = p->fixed_grid ? p->cfg.grid_cap : p->grid_view[view];
+  const int grid_dec = p->fixed_grid ? p->cfg.dec_grid_cap : p->grid_view[2];
+  if (grid_rows == 0 && grid_dec == 0) return FE_OK;
+  if (!q || !k_codes || !v_codes || !k_exp || !v_exp || !out)
+    return fail(FE_ERR_INVALID_ARGUMENT, "fe_kv8_attn_run: null pointer");
+  if (!aligned16(q) || !aligned16(k_codes) || !aligned16(v_codes) || !aligned16(out))
+    return fail(FE_ERR_INVALID_ARGUMENT, "fe_kv8_attn_run: buffers must be 16-byte aligned");
+  const int H = p->cfg.dec_heads, dim = p->cfg.dim, hkv = p->cfg.hkv;
+  if (reinterpret_cast<uintptr_t>(k_exp) % H || reinterpret_cast<uintptr_t>(v_exp) % H)
+    return fail(FE_ERR_INVALID_ARGUMENT,
+                "fe_kv8_attn_run: exponents must be aligned to gcd(hkv, 8) bytes");
+  const int64_t cache_slots = int64_t(p->cfg.num_blocks + 1) * p->cfg.page;
+  CUtensorMap kd, vd, kr, vr;
+  if (grid_dec > 0) {
+    int rc = encode_kv8_decode_map(&kd, k_codes, hkv, dim, H, cache_slots);
+    if (rc == FE_OK) rc = encode_kv8_decode_map(&vd, v_codes, hkv, dim, H, cache_slots);
+    if (rc != FE_OK) return rc;
   }
-  if (fork) {
-    // join even after a failed launch, so `stream` never runs ahead of the side
-    cudaError_t e1 = cudaEventRecord(p->join_ev, p->side);
-    cudaError_t e2 = cudaStreamWaitEvent(s, p->join_ev, 0);
-    if (rc == FE_OK && e1 != cudaSuccess) return cuda_fail(e1, "fe_attn_run: join record");
-    if (rc == FE_OK && e2 != cudaSuccess) return cuda_fail(e2, "fe_attn_run: join wait");
+  if (grid_rows > 0) {
+    int rc = encode_kv8_rows_map(&kr, k_codes, hkv, dim, cache_slots);
+    if (rc == FE_OK) rc = encode_kv8_rows_map(&vr, v_codes, hkv, dim, cache_slots);
+    if (rc != FE_OK) return rc;
   }
-  if (rc != FE_OK) return rc;
-  FE_CUDA_TRY(cudaGetLastError());
-  return FE_OK;
+  auto run = [&](const auto& a) -> int {
+    return launch_lists(
+        p, view, grid_rows, grid_dec, &a.a, static_cast<cudaStream_t>(stream),
+        [&](cudaStream_t s) {
+          return kv8_decode_launch(p->dtype, dim, H, kd, vd, &a, grid_dec, s);
+        },
+        [&](cudaStream_t s) { return kv8_rows_launch(p->dtype, dim, kr, vr, &a, grid_rows, s); });
+  };
+  if (p->dtype == FE_DTYPE_BF16)
+    return run(Kv8Args<__nv_bfloat16>{attn_args<__nv_bfloat16>(p, q, out, view, 0), k_exp, v_exp,
+                                      hkv});
+  return run(Kv8Args<__half>{attn_args<__half>(p, q, out, view, 0), k_exp, v_exp, hkv});
 }
 
 int fe_attn_plan_get_info(const fe_attn_plan* p, fe_attn_plan_info* info) {

@@ -347,7 +347,7 @@ int build_plan(const PlanConfig& cfg, const int32_t* qo, const int32_t* kv, cons
   if (!fixed_grid && !key_units.empty() && !row_units_causal.empty()) {
     double dec_bytes = 0, pieces = 0, max_pieces = 0;
     for (const auto& u : key_units)
-      dec_bytes += double(u.tiles) * kTileTokens * cfg.dec_heads * cfg.dim * 4.0;
+      dec_bytes += double(u.tiles) * kTileTokens * cfg.dec_heads * cfg.dim * (2.0 * cfg.elem_bytes);
     for (const auto* list : {&row_units_full, &row_units_causal}) {
       double total = 0;
       for (const auto& u : *list) {
@@ -369,8 +369,8 @@ int build_plan(const PlanConfig& cfg, const int32_t* qo, const int32_t* kv, cons
   View views[3];
   {
     int rc;
-    if (cfg.dim == kWideHeadDim) {
-      // head_dim 256 row lists are cut exactly like the decode list: the
+    if (cfg.cut_rows) {
+      // row lists of head_dim 256 and of the 8-bit cache are cut exactly like the decode list: the
       // tcgen05 kernel's time per key tile hardly depends on how many of an
       // item's 128 rows are valid, so equal tile counts per CTA balance it,
       // at the price of up to one split unit per CTA boundary (pieces of at
@@ -380,7 +380,7 @@ int build_plan(const PlanConfig& cfg, const int32_t* qo, const int32_t* kv, cons
       rc = build_cut_view(cfg, row_units_causal, row_cap, kWideMinChunk, fixed_grid, views[1],
                           err);
     } else {
-      // head_dim 128 keeps whole items (cfg.row_split), longest first onto
+      // head_dim 128 over the 16-bit cache keeps whole items (cfg.row_split), longest first onto
       // the least-loaded CTA
       const int row_min_chunk = cfg.row_split ? 16 : (1 << 29);
       rc = build_view(cfg, row_units_full, row_cap, 4, row_min_chunk, fixed_grid, views[0], err);

@@ -81,6 +81,8 @@ struct PlanConfig {
   int dec_heads;              // KV heads per decode item: gcd(hkv, 8)
   int row_group_blocks;       // 16-row blocks per row-mode item (8 = one 128-row tcgen05 tile)
   bool row_split;             // row-mode key ranges may be split across CTAs
+  bool cut_rows;              // row lists are cut exactly, as the decode list (head_dim 256, 8-bit)
+  int elem_bytes;             // bytes of a cached element
   int max_items;              // work-item capacity
   int64_t partial_capacity;   // floats in the split-K workspace
   int max_groups;             // split-counter capacity

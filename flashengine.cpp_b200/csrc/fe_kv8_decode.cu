@@ -1,0 +1,633 @@
+// Paged decode attention over the 8-bit KV cache (sm_100a): sequences whose
+// query rows x GQA group fit one 16-row block. No counterpart in the
+// reference, whose pools are 16-bit; semantics as fe_attn_run (the arithmetic
+// of Cambridgebit/FlashEngine.cpp src/portable_gpu_ops.cpp:39-44) over the
+// cache's values code * 2^exponent.
+//
+// Mathematics. With s(t) the score in base-2 units, 2^v(t) the V scale of the
+// token's block and m a running maximum of s + v (not of s), the kernel keeps
+//   w(t) = 2^(s(t) + v(t) - m),  O = sum w(t) code_v(t),  l = sum w(t) 2^-v(t)
+// and the output is O / l: V's scales cost one addition per 16 tokens, K's one
+// factor per 16 tokens, and the codes feed the tensor core as they lie in the
+// cache. The other operand of each product is split into 8-bit parts:
+//  * a query row into two e4m3 parts (high part and residual, 8 to 9
+//    significant bits: exactly a bf16 where its magnitude is within 2^11 of
+//    the row's largest, and an error of 2^-19 of that below);
+//  * a weight into three e5m2 parts (9 bits). e5m2 and not e4m3, for the
+//    range: weights are kept up to 2^15, so they keep their bits down to
+//    2^-26 of the largest. Two e4m3 parts reach 2^-18, and a long context whose
+//    first token takes most of the softmax would lose its other tokens.
+//    The first two parts are cut, not rounded (a half's upper byte is its
+//    value cut to e5m2), the last is rounded.
+// Products on mma.m16n8k32 (fp32 accumulation): measured on a B200 one takes
+// 5 clocks a warp and SM quarter against 8 for the 16-bit m16n8k16, so the
+// parts cost about what one 16-bit product does, and no code is converted.
+//
+// B200 design, as fe_decode.cu: bound by HBM traffic. One persistent CTA per
+// SM with 8 consumer warps and a producer warp; an item is (sequence, group
+// of H KV heads, range of 16-token tiles), a step is two tiles (32 tokens, the
+// K of one PV product) of all H heads, fetched with one TMA box per tile for
+// K and one for V into a ring of 128-192 KiB. The tiles' scale exponents are
+// gathered by the producer's lanes a batch ahead and travel with the stage.
+#include <mutex>
+
+#include "fe_attn_common.cuh"
+#include "fe_kv8_attn.h"
+#include "fe_kv8_common.cuh"
+
+namespace fe {
+namespace {
+
+constexpr int kConsumers = 8;
+constexpr int kThreads = (kConsumers + 1) * 32;
+constexpr int kStepTiles = 2;
+constexpr int kStepTokens = kStepTiles * kTileTokens;
+constexpr int kBoxBytes = kTileTokens * 128;  // 16 rows x 128 codes
+constexpr float kWeightBits = 15.f;           // weights are kept times 2^15 (a half holds 2^16)
+
+// Warps of a CTA: group = (head, half of the packed rows), kWh = 8 / groups
+// warps of a group take steps j, j + kWh, ...; the stage count is a multiple
+// of kWh, so a stage's previous user among them is the warp itself and a
+// parity wait can never be a phase ahead.
+template <int H, int D>
+struct Cfg {
+  static constexpr int kBoxes = D / 128;
+  static constexpr int kTileBytes = H * D * kTileTokens;        // one of K or V
+  static constexpr int kStageBytes = 2 * kStepTiles * kTileBytes;
+  static constexpr int kStages = (D == 128 && H == 8) ? 3 : (128 * 1024) / kStageBytes;
+  static constexpr int kNT = D == 128 ? 2 : 1;                  // most 8-row column tiles a warp
+  static constexpr int kSlotFloats = 8 * kNT * (D + 4);
+  static constexpr int kCombBytes = H == 8 ? 0 : (kConsumers / 2) * kSlotFloats * 4;
+  static constexpr int kExpOff = kStages * kStageBytes + kCombBytes;
+  static constexpr int kExpBytes = 2 * kStepTiles * 8;          // [tile][K|V][8 heads]
+  static constexpr int kBarOff = kExpOff + kStages * kExpBytes;
+  static constexpr int kSmem = 1024 + kBarOff + 2 * kStages * 8 + 16;
+  static_assert(kSmem <= 232448, "shared memory budget");
+  static_assert(H == 8 || kStages % (kConsumers / H) == 0, "see above");
+};
+
+__device__ __forceinline__ void mma_e4m3(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                         uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void mma_e4m3_e5m2(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                              uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e5m2.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t hsub2(uint32_t a, uint32_t b) {
+  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&a),
+                            *reinterpret_cast<const __half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// 8*NT packed rows (columns of the products) of one KV head of D dims.
+// Fragment layout: the tokens of a tile are the M side of S^T = K Q^T, dims
+// the M side of O^T = V^T W^T. O row i of m-tile mt is dim 16 mt + 2 i (i < 8)
+// or 16 mt + 2 (i - 8) + 1: the byte pairs that a transposed 16-bit load of
+// 8-bit V delivers.
+template <typename T, int NT, int D>
+struct State {
+  static constexpr int kKS = D / 32;  // k-steps of S^T
+  static constexpr int kMT = D / 16;  // m-tiles of O^T
+  uint32_t qh[NT][kKS][2], ql[NT][kKS][2];
+  float f[NT][2];  // base-2 score units per raw product, per column of this lane
+  int lim[NT][2];
+  int lim_min;
+  float m[NT][2], l[NT][2];
+  float o[NT][kMT][4];
+
+  __device__ __forceinline__ void init(const T* q, int hq, const SeqInfo& si, int head0, int G,
+                                       bool causal, float scale_log2, int key_end, int lane,
+                                       int col0) {
+    const int r8 = lane >> 2, cq = lane & 3;
+    const int P = si.qrows * G;
+    const int length = min(si.length, key_end);
+    lim_min = length;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int p = col0 + nt * 8 + r8;
+      const T* qp = p < P ? q + (static_cast<int64_t>(si.q_row0 + p / G) * hq + head0 + p % G) * D
+                          : nullptr;
+      uint2 raw[kKS][2];
+      float amax = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < kKS; ++ks)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          raw[ks][x] = make_uint2(0u, 0u);
+          if (qp) raw[ks][x] = __ldg(reinterpret_cast<const uint2*>(qp + ks * 32 + x * 16 + 4 * cq));
+          const float2 a = unpack2<T>(raw[ks][x].x), b = unpack2<T>(raw[ks][x].y);
+          const float v[4] = {fabsf(a.x), fabsf(a.y), fabsf(b.x), fabsf(b.y)};
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (v[e] < INFINITY) amax = fmaxf(amax, v[e]);
+        }
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+      const int e = kv8_query_exp(amax);
+      const float up = exp_scale(254 - e);
+#pragma unroll
+      for (int ks = 0; ks < kKS; ++ks)
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+          kv8_split_query<T>(raw[ks][x], up, qh[nt][ks][x], ql[nt][ks][x]);
+      const float mine = exp_scale(e) * scale_log2;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        f[nt][c] = __shfl_sync(0xffffffffu, mine, (2 * cq + c) * 4);
+        const int pc = col0 + nt * 8 + 2 * cq + c;
+        lim[nt][c] = (causal && pc < P)
+                         ? min(length, si.length - si.qrows + pc / G + 1) : length;
+        lim_min = min(lim_min, lim[nt][c]);
+        m[nt][c] = -INFINITY;
+        l[nt][c] = 0.f;
+      }
+#pragma unroll
+      for (int mt = 0; mt < kMT; ++mt)
+        o[nt][mt][0] = o[nt][mt][1] = o[nt][mt][2] = o[nt][mt][3] = 0.f;
+    }
+  }
+
+  // One step: the 32 tokens from `tbase` on; ka, va: shared addresses of this
+  // head's boxes of the first tile, the second tile's `tile_bytes` further;
+  // ke, ve: the two tiles' scale exponents (clamped, biased); `length`: keys
+  // of the item.
+  __device__ __forceinline__ void step(uint32_t ka, uint32_t va, uint32_t tile_bytes,
+                                       const int (&ke)[2], const int (&ve)[2], int tbase,
+                                       int length, int lane) {
+    const int r8 = lane >> 2, cq = lane & 3, mi = lane >> 3, li = lane & 7;
+    // ---- S^T = K Q^T
+    float s[2][NT][4];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) s[u][nt][0] = s[u][nt][1] = s[u][nt][2] = s[u][nt][3] = 0.f;
+      const uint32_t row = ka + u * tile_bytes + (li + ((mi & 1) << 3)) * 128;
+#pragma unroll
+      for (int ks = 0; ks < kKS; ++ks) {
+        const int c = 2 * ks + (mi >> 1);  // 16-code chunk of the row, 8 per box
+        uint32_t af[4];
+        ldmatrix_x4(row + (c >> 3) * kBoxBytes + (((c & 7) ^ li) << 4), af[0], af[1], af[2],
+                    af[3]);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          mma_e4m3(s[u][nt], af, qh[nt][ks][0], qh[nt][ks][1]);
+          mma_e4m3(s[u][nt], af, ql[nt][ks][0], ql[nt][ks][1]);
+        }
+      }
+    }
+    // ---- hide keys past each column's limit
+    if (tbase + kStepTokens > lim_min) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (tbase + u * kTileTokens + r8 + (e >> 1) * 8 >= lim[nt][e & 1])
+              s[u][nt][e] = -INFINITY;
+    }
+    // ---- weights: columns are held by the 8 lanes with the same lane % 4
+    const float kf[2] = {exp_scale(ke[0]), exp_scale(ke[1])};
+    const float vf[2] = {float(ve[0] - 127), float(ve[1] - 127)};
+    const float vi[2] = {exp_scale(254 - ve[0]), exp_scale(254 - ve[1])};
+    uint32_t bw[3][NT][2];  // parts of W^T
+    float al[NT][2];
+    bool moved = false;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float mx = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          mx = fmaxf(mx, fmaf(fmaxf(s[u][nt][c], s[u][nt][2 + c]), kf[u] * f[nt][c], vf[u]));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+        const float mn = fmaxf(m[nt][c], mx);
+        const float base = mn == -INFINITY ? 0.f : mn;
+        moved |= mn > m[nt][c];
+        al[nt][c] = fast_exp2(m[nt][c] - base);
+        m[nt][c] = mn;
+        float add = 0.f;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const float ft = kf[u] * f[nt][c], off = vf[u] + kWeightBits - base;
+          const float w0 = fast_exp2(fmaf(s[u][nt][c], ft, off));
+          const float w1 = fast_exp2(fmaf(s[u][nt][2 + c], ft, off));
+          s[u][nt][c] = w0;
+          s[u][nt][2 + c] = w1;
+          add = fmaf(w0 + w1, vi[u], add);
+        }
+        l[nt][c] = fmaf(l[nt][c], al[nt][c], add);
+      }
+    if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int mt = 0; mt < kMT; ++mt) {
+          o[nt][mt][0] *= al[nt][0];
+          o[nt][mt][1] *= al[nt][1];
+          o[nt][mt][2] *= al[nt][0];
+          o[nt][mt][3] *= al[nt][1];
+        }
+    }
+    // ---- W^T as B fragments. A 16-bit element holds the codes of tokens r8
+    // (low) and r8 + 8 of one column; transposed, a lane has column lane / 4
+    // and tokens 2cq, 2cq + 8, 2cq + 1, 2cq + 9 of the tile, lowest byte first.
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const uint32_t w0 = pack2<__half>(s[u][nt][0], s[u][nt][2]);
+        const uint32_t w1 = pack2<__half>(s[u][nt][1], s[u][nt][3]);
+        const uint32_t r0 = hsub2(w0, w0 & 0xff00ff00u), r1 = hsub2(w1, w1 & 0xff00ff00u);
+        const uint32_t t0 = hsub2(r0, r0 & 0xff00ff00u), t1 = hsub2(r1, r1 & 0xff00ff00u);
+        bw[0][nt][u] = movmatrix_trans(__byte_perm(w0, w1, 0x7531));
+        bw[1][nt][u] = movmatrix_trans(__byte_perm(r0, r1, 0x7531));
+        bw[2][nt][u] = movmatrix_trans(e5m2x2_h2(t0) | e5m2x2_h2(t1) << 16);
+      }
+    // ---- codes of V rows past the end are zeroed (anything may lie there,
+    // and 0 * NaN would poison O)
+    uint32_t vm[2] = {0xffffffffu, 0xffffffffu};
+    if (tbase + kStepTokens > length) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int t = tbase + u * kTileTokens + 2 * cq;
+        vm[u] = (t < length ? 0xffu : 0u) | (t + 8 < length ? 0xff00u : 0u) |
+                (t + 1 < length ? 0xff0000u : 0u) | (t + 9 < length ? 0xff000000u : 0u);
+      }
+    }
+    // ---- O^T += V^T W^T
+    const uint32_t row = va + (mi >> 1) * tile_bytes + (li + ((mi & 1) << 3)) * 128;
+#pragma unroll
+    for (int mt = 0; mt < kMT; ++mt) {
+      uint32_t x0, y0, x1, y1;  // tokens 0-7 and 8-15 of either tile, dims 16 mt ..
+      ldmatrix_x4_trans(row + (mt >> 3) * kBoxBytes + (((mt & 7) ^ li) << 4), x0, y0, x1, y1);
+      uint32_t a[4];
+      a[0] = __byte_perm(x0, y0, 0x6240) & vm[0];
+      a[1] = __byte_perm(x0, y0, 0x7351) & vm[0];
+      a[2] = __byte_perm(x1, y1, 0x6240) & vm[1];
+      a[3] = __byte_perm(x1, y1, 0x7351) & vm[1];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int x = 0; x < 3; ++x) mma_e4m3_e5m2(o[nt][mt], a, bw[x][nt][0], bw[x][nt][1]);
+    }
+  }
+
+  __device__ __forceinline__ void reduce_l() {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], 4);
+        l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], 8);
+        l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], 16);
+      }
+  }
+
+  // (O, m, l) of every column as merge rows of D + 4 floats; a column's dims
+  // in order.
+  __device__ __forceinline__ void stash(float* rows, int lane) const {
+    const int r8 = lane >> 2, cq = lane & 3;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float* row = rows + (nt * 8 + 2 * cq + c) * (D + 4);
+#pragma unroll
+        for (int mt = 0; mt < kMT; ++mt)
+          *reinterpret_cast<float2*>(row + 16 * mt + 2 * r8) =
+              make_float2(o[nt][mt][c], o[nt][mt][2 + c]);
+        if (r8 == 0) {
+          row[D] = m[nt][c];
+          row[D + 1] = l[nt][c];
+        }
+      }
+  }
+  __device__ __forceinline__ void absorb(const float* rows, int lane) {
+    const int r8 = lane >> 2, cq = lane & 3;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const float* row = rows + (nt * 8 + 2 * cq + c) * (D + 4);
+        const float mo = row[D], lo = row[D + 1];
+        const float mn = fmaxf(m[nt][c], mo);
+        const float base = mn == -INFINITY ? 0.f : mn;
+        const float as = fast_exp2(m[nt][c] - base), ao = fast_exp2(mo - base);
+        m[nt][c] = mn;
+        l[nt][c] = l[nt][c] * as + lo * ao;
+#pragma unroll
+        for (int mt = 0; mt < kMT; ++mt) {
+          const float2 x = *reinterpret_cast<const float2*>(row + 16 * mt + 2 * r8);
+          o[nt][mt][c] = o[nt][mt][c] * as + x.x * ao;
+          o[nt][mt][2 + c] = o[nt][mt][2 + c] * as + x.y * ao;
+        }
+      }
+  }
+};
+
+template <typename T, int H, int D, int NT>
+__device__ __forceinline__ void run_item(const Kv8Args<T>& ka, const WorkItem& wi,
+                                         const SeqInfo& si, int halves, uint8_t* stages,
+                                         const uint8_t* exps, uint64_t* full, uint64_t* empty,
+                                         volatile int* flags, float* comb, int w, int lane,
+                                         uint32_t& g, bool& aborted) {
+  using C = Cfg<H, D>;
+  const AttnArgs<T>& a = ka.a;
+  const int G = a.G;
+  const int P = si.qrows * G;
+  const int groups = H * halves;
+  const int kwh = kConsumers / groups;
+  const int grp = w % groups, sub = w / groups;
+  const int hh = grp % H, col0 = (grp / H) * 8;
+  const int head0 = (wi.kvh + hh) * G;
+  const int key_end = wi.kt1 * kTileTokens;
+  State<T, NT, D> st;
+  st.init(a.q, a.hq, si, head0, G, a.view == 1, a.scale_log2, key_end, lane, col0);
+  const int length = min(si.length, key_end);
+
+  const int nsteps = (wi.kt1 - wi.kt0 + kStepTiles - 1) / kStepTiles;
+  for (int j = sub; j < nsteps; j += kwh) {
+    const uint32_t gg = g + j;
+    const int s = gg % C::kStages;
+    if (aborted || flags[0] || !wait_bounded(&full[s], (gg / C::kStages) & 1u, flags)) {
+      aborted = true;
+      break;
+    }
+    const uint8_t* ex = exps + s * C::kExpBytes + hh;
+    const int ke[2] = {exp_clamp(ex[0]), exp_clamp(ex[16])};
+    const int ve[2] = {exp_clamp(ex[8]), exp_clamp(ex[24])};
+    // stage: K tile 0, K tile 1, V tile 0, V tile 1, each [head][box][16 rows]
+    const uint32_t base = smem_u32(stages + s * C::kStageBytes) + hh * C::kBoxes * kBoxBytes;
+    st.step(base, base + kStepTiles * C::kTileBytes, C::kTileBytes, ke, ve,
+            (wi.kt0 + j * kStepTiles) * kTileTokens, length, lane);
+    __syncwarp();
+    if (lane == 0) mbar_arrive_cnt(&empty[s], kwh);
+  }
+  g += nsteps;
+  st.reduce_l();
+
+  if constexpr (H < 8) {
+    // fold the group's states pairwise: round `step` leaves warps 0..step-1
+    constexpr int kSlot = C::kSlotFloats;
+    for (int step = kwh >> 1; step >= 1; step >>= 1) {
+      if (sub >= step && sub < 2 * step)
+        st.stash(comb + ((sub - step) * groups + grp) * kSlot, lane);
+      named_barrier_sync(1, kConsumers * 32);
+      if (sub < step) st.absorb(comb + (sub * groups + grp) * kSlot, lane);
+      named_barrier_sync(1, kConsumers * 32);
+    }
+  }
+  if (sub != 0 || aborted) return;
+
+  const int r8 = lane >> 2, cq = lane & 3;
+  const int R = H * P;  // rows of the item's record: head-major, then packed row
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int p = col0 + nt * 8 + 2 * cq + c;
+      if (p >= P) continue;
+      if (wi.group < 0) {
+        const float inv = 1.f / st.l[nt][c];
+        T* dst = a.out + (static_cast<int64_t>(si.q_row0 + p / G) * a.hq + head0 + p % G) * D;
+#pragma unroll
+        for (int mt = 0; mt < D / 16; ++mt)
+          *reinterpret_cast<uint32_t*>(dst + 16 * mt + 2 * r8) =
+              pack2<T>(st.o[nt][mt][c] * inv, st.o[nt][mt][2 + c] * inv);
+      } else {
+        float* rec = a.partials + wi.part;
+        float* row = rec + (hh * P + p) * D;
+#pragma unroll
+        for (int mt = 0; mt < D / 16; ++mt)
+          *reinterpret_cast<float2*>(row + 16 * mt + 2 * r8) =
+              make_float2(st.o[nt][mt][c], st.o[nt][mt][2 + c]);
+        if (r8 == 0) {
+          rec[R * D + hh * P + p] = st.m[nt][c];
+          rec[R * (D + 1) + hh * P + p] = st.l[nt][c];
+        }
+      }
+    }
+}
+
+template <typename T, int H, int D>
+__global__ void __launch_bounds__(kThreads, 1)
+    kv8_decode_kernel(const __grid_constant__ CUtensorMap kmap,
+                      const __grid_constant__ CUtensorMap vmap, const Kv8Args<T> ka) {
+  using C = Cfg<H, D>;
+  const AttnArgs<T>& a = ka.a;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~uintptr_t(1023));
+  uint8_t* stages = smem;
+  float* comb = reinterpret_cast<float*>(smem + C::kStages * C::kStageBytes);
+  uint8_t* exps = smem + C::kExpOff;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kBarOff);
+  uint64_t* empty = full + C::kStages;
+  volatile int* flags = reinterpret_cast<volatile int*>(empty + C::kStages);
+
+  pdl_trigger();  // the merge kernel may be scheduled; it waits for this grid
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const MetaHeader* hdr = reinterpret_cast<const MetaHeader*>(a.meta);
+  constexpr int kList = 2;  // decode work list
+  if (static_cast<int>(blockIdx.x) >= hdr->grid[kList]) return;
+  const int32_t* cta_off = reinterpret_cast<const int32_t*>(a.meta + hdr->cta_off_off[kList]);
+  const WorkItem* items = reinterpret_cast<const WorkItem*>(a.meta + hdr->items_off[kList]);
+  const SeqInfo* seqs = reinterpret_cast<const SeqInfo*>(a.meta + hdr->seqs_off);
+  const int32_t* pages = reinterpret_cast<const int32_t*>(a.meta + hdr->pages_off);
+  const int it0 = cta_off[blockIdx.x], it1 = cta_off[blockIdx.x + 1];
+  if (it0 >= it1) return;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], kConsumers);
+    }
+    flags[0] = 0;
+    fence_barrier_init();
+  }
+  __syncthreads();
+
+  if (warp == kConsumers) {
+    // ------------------------------------------------------------ producer
+    if (lane == 0) {
+      prefetch_tensormap(&kmap);
+      prefetch_tensormap(&vmap);
+    }
+    // A lane looks after one tile of a batch of 32: its first slot (from the
+    // page list, asked for two batches ahead) and the H + H exponents of its
+    // block (one batch ahead).
+    auto tile_slot = [&](const WorkItem& w, const SeqInfo& si, int j) -> int {
+      if (j >= w.kt1) return 0;
+      const int t0 = j * kTileTokens;
+      return __ldg(pages + si.page_off + t0 / a.page) * a.page + (t0 % a.page);
+    };
+    struct Exps {
+      uint64_t k, v;
+    };
+    auto tile_exps = [&](const WorkItem& w, int slot) -> Exps {
+      const int64_t at = int64_t(slot / kKv8Block) * ka.hkv + w.kvh;
+      Exps e;
+      if constexpr (H == 8) {
+        e.k = *reinterpret_cast<const uint64_t*>(ka.k_exp + at);
+        e.v = *reinterpret_cast<const uint64_t*>(ka.v_exp + at);
+      } else if constexpr (H == 4) {
+        e.k = *reinterpret_cast<const uint32_t*>(ka.k_exp + at);
+        e.v = *reinterpret_cast<const uint32_t*>(ka.v_exp + at);
+      } else if constexpr (H == 2) {
+        e.k = *reinterpret_cast<const uint16_t*>(ka.k_exp + at);
+        e.v = *reinterpret_cast<const uint16_t*>(ka.v_exp + at);
+      } else {
+        e.k = ka.k_exp[at];
+        e.v = ka.v_exp[at];
+      }
+      return e;
+    };
+    // page ids are the plan's metadata, fetched before waiting for the kernel
+    // that owns the pools
+    const WorkItem w0 = items[it0];
+    const SeqInfo si0 = seqs[w0.seq];
+    const int first = tile_slot(w0, si0, w0.kt0 + lane);
+    const int second = tile_slot(w0, si0, w0.kt0 + 32 + lane);
+    pdl_wait();
+    uint32_t g = 0;
+    bool ok = true;
+    for (int it = it0; it < it1 && ok; ++it) {
+      const WorkItem w = items[it];
+      const SeqInfo si = seqs[w.seq];
+      const int box = w.kvh * C::kBoxes;
+      int nxt = it == it0 ? first : tile_slot(w, si, w.kt0 + lane);
+      int nxt2 = it == it0 ? second : tile_slot(w, si, w.kt0 + 32 + lane);
+      Exps enxt = tile_exps(w, nxt);
+      for (int j0 = w.kt0; j0 < w.kt1 && ok; j0 += 32) {
+        const int n = min(32, w.kt1 - j0);
+        const int slot = nxt;
+        const Exps e = enxt;
+        nxt = nxt2;
+        enxt = tile_exps(w, nxt);
+        nxt2 = tile_slot(w, si, j0 + 64 + lane);
+        for (int jj = 0; jj < n; jj += kStepTiles) {
+          const int s0 = __shfl_sync(0xffffffffu, slot, jj);
+          const int s1 = __shfl_sync(0xffffffffu, slot, jj + 1);
+          const int s = g % C::kStages;
+          int good = 1;
+          if (lane == 0 && (flags[0] || !wait_bounded(&empty[s], ((g / C::kStages) & 1u) ^ 1u, flags)))
+            good = 0;
+          good = __shfl_sync(0xffffffffu, good, 0);
+          if (!good) {
+            ok = false;
+            break;
+          }
+          if ((lane & ~1) == jj) {
+            uint64_t* dst = reinterpret_cast<uint64_t*>(exps + s * C::kExpBytes + (lane & 1) * 16);
+            dst[0] = e.k;
+            dst[1] = e.v;
+          }
+          __syncwarp();
+          if (lane == 0) {
+            const int tiles = min(kStepTiles, n - jj);
+            mbar_arrive_expect_tx(&full[s], tiles * 2 * C::kTileBytes);
+            uint8_t* st = stages + s * C::kStageBytes;
+            tma_load_3d(st, &kmap, &full[s], 0, s0, box);
+            if (tiles == 2) tma_load_3d(st + C::kTileBytes, &kmap, &full[s], 0, s1, box);
+            st += kStepTiles * C::kTileBytes;
+            tma_load_3d(st, &vmap, &full[s], 0, s0, box);
+            if (tiles == 2) tma_load_3d(st + C::kTileBytes, &vmap, &full[s], 0, s1, box);
+          }
+          ++g;
+        }
+      }
+    }
+    if (!ok && lane == 0) {
+      raise_device_error(a.err, FE_DEVERR_TIMEOUT);
+      flags[0] = 1;
+      const uint32_t pending = g < C::kStages ? g : C::kStages;
+      for (uint32_t k = 1; k <= pending; ++k) {
+        const uint32_t gg = g - k;
+        volatile int never = 0;
+        (void)wait_bounded(&full[gg % C::kStages], (gg / C::kStages) & 1u, &never);
+      }
+    }
+    return;
+  }
+
+  // -------------------------------------------------------------- consumers
+  pdl_wait();  // q and the split workspace belong to earlier kernels until here
+  uint32_t g = 0;
+  bool aborted = false;
+  for (int it = it0; it < it1; ++it) {
+    const WorkItem wi = items[it];
+    const SeqInfo si = seqs[wi.seq];
+    const bool many = si.qrows * a.G > 8;
+    if constexpr (D == 128) {
+      if (many)
+        run_item<T, H, D, 2>(ka, wi, si, 1, stages, exps, full, empty, flags, comb, warp, lane, g,
+                             aborted);
+      else
+        run_item<T, H, D, 1>(ka, wi, si, 1, stages, exps, full, empty, flags, comb, warp, lane, g,
+                             aborted);
+    } else {
+      // 256 dims leave registers for 8 packed rows a warp: more are two groups
+      run_item<T, H, D, 1>(ka, wi, si, many ? 2 : 1, stages, exps, full, empty, flags, comb, warp,
+                           lane, g, aborted);
+    }
+  }
+  if (aborted && lane == 0) raise_device_error(a.err, FE_DEVERR_TIMEOUT);
+}
+
+template <typename T, int H, int D>
+int launch(const CUtensorMap& kmap, const CUtensorMap& vmap, const Kv8Args<T>& args, int grid,
+           cudaStream_t stream) {
+  using C = Cfg<H, D>;
+  static std::once_flag once;
+  static cudaError_t attr_err = cudaSuccess;
+  std::call_once(once, [] {
+    attr_err = cudaFuncSetAttribute(kv8_decode_kernel<T, H, D>,
+                                    cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+  });
+  if (attr_err != cudaSuccess) return cuda_fail(attr_err, "kv8_decode_kernel attribute");
+  FE_CUDA_TRY(launch_pdl(kv8_decode_kernel<T, H, D>, dim3(grid), dim3(kThreads), C::kSmem, stream,
+                         kmap, vmap, args));
+  return FE_OK;
+}
+
+template <typename T>
+int dispatch(int dim, int heads, const CUtensorMap& kmap, const CUtensorMap& vmap,
+             const Kv8Args<T>& a, int grid, cudaStream_t stream) {
+  if (dim == kWideHeadDim)
+    return heads == 2 ? launch<T, 2, kWideHeadDim>(kmap, vmap, a, grid, stream)
+                      : launch<T, 1, kWideHeadDim>(kmap, vmap, a, grid, stream);
+  switch (heads) {
+    case 8: return launch<T, 8, kHeadDim>(kmap, vmap, a, grid, stream);
+    case 4: return launch<T, 4, kHeadDim>(kmap, vmap, a, grid, stream);
+    case 2: return launch<T, 2, kHeadDim>(kmap, vmap, a, grid, stream);
+    default: return launch<T, 1, kHeadDim>(kmap, vmap, a, grid, stream);
+  }
+}
+
+}  // namespace
+
+int kv8_decode_launch(int dtype, int dim, int heads, const CUtensorMap& kmap,
+                      const CUtensorMap& vmap, const void* args, int grid, cudaStream_t stream) {
+  if (dtype == FE_DTYPE_BF16)
+    return dispatch(dim, heads, kmap, vmap, *static_cast<const Kv8Args<__nv_bfloat16>*>(args),
+                    grid, stream);
+  return dispatch(dim, heads, kmap, vmap, *static_cast<const Kv8Args<__half>*>(args), grid,
+                  stream);
+}
+
+}  // namespace fe

@@ -4,7 +4,9 @@
   (``lib/libfe_kv_b200.so``; no fallback when it is missing).
 * :mod:`fekv.ops`       the reference's ``fe::cuda`` operator interface
   (``create_plan``/``prepare_plan``/``attention``/``store``/``rope``/
-  ``accept``) plus the fused ``rope_append`` and block copy.
+  ``accept``) plus the fused ``rope_append`` and block copy, and the
+  8-bit cache (``Kv8Pool``, ``append_kv8``, ``Kv8Plan``, ``gather_kv8``,
+  ``copy_blocks_kv8``).
 * :mod:`fekv.metadata`  the per-step slot mapping / page tables of
   ``CudaModel::prepare``.
 * :mod:`fekv.workloads` seeded synthetic configs C1..C5.
@@ -12,6 +14,7 @@
 from . import metadata, workloads  # noqa: F401
 from ._lib import (FE_DTYPE_BF16, FE_DTYPE_F16, FeError, LIB_PATH, SHIM_PATH,  # noqa: F401
                    load)
-from .ops import (AttentionPlan, HostPlan, accept, attention, clear_pages,  # noqa: F401
-                  copy_blocks, create_plan, destroy_plan, device_errors, fork_copies, gather,
+from .ops import (AttentionPlan, HostKv8Plan, HostPlan, Kv8Plan, Kv8Pool,  # noqa: F401
+                  accept, append_kv8, attention, clear_pages, copy_blocks,
+                  copy_blocks_kv8, create_plan, destroy_plan, device_errors, fork_copies, gather, gather_kv8,
                   paged_decode_noalloc, prepare_plan, rope, rope_append, store)

@@ -34,6 +34,7 @@ FE_DEVERR_POS_RANGE = 0x20
 FE_DEVERR_PLAN = 0x40
 
 FE_MAX_LAYERS = 128
+FE_KV8_BLOCK = 16
 
 FE_ATTN_LISTS_DECODE = 1
 FE_ATTN_LISTS_ROWS = 2
@@ -65,6 +66,12 @@ SIGNATURES = {
     "fe_step_prepare_device": (_I, [_P, _P, _I, _P, _I, _I, _P, _P, _P]),
     "fe_attn_plan_debug_device_meta": (_I, [_P, _P, _I64, _P]),
     "fe_paged_decode_noalloc": (_I, [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P]),
+    "fe_kv8_append": (_I, [_P] * 11 + [_I] * 7 + [_I64, _P]),
+    "fe_kv8_gather": (_I, [_P] * 7 + [_I] * 6 + [_I64, _P]),
+    "fe_kv8_copy_blocks": (_I, [_P] * 4 + [_I] + [_P] * 3 + [_I] * 5 + [_P]),
+    "fe_kv8_plan_create": (_I, [_I, _I, _I, _I, _I, _I, _I, _I, ctypes.POINTER(_P)]),
+    "fe_kv8_plan_create_host": (_I, [_I, _I, _I, _I, _I, _I, _I, _I, _I, ctypes.POINTER(_P)]),
+    "fe_kv8_attn_run": (_I, [_P] * 7 + [_I, _P]),
     "fe_rope": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P]),
     "fe_rope_append": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I64,
                             _P]),

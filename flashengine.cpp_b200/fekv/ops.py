@@ -216,13 +216,15 @@ class AttentionPlan:
     """Owns an fe_attn_plan. `prepare` takes host metadata (as
     fe::cuda::prepare_plan); `attention` takes device tensors."""
 
+    _create = "fe_attn_plan_create"
+
     def __init__(self, hq, hkv, dim, page, max_batch, max_pages, bf16, blocks):
         self.lib = _lib.load()
         h = _P()
         dtype = FE_DTYPE_BF16 if bf16 else FE_DTYPE_F16
-        check(self.lib.fe_attn_plan_create(int(hq), int(hkv), int(dim), int(page), int(max_batch),
-                                           int(max_pages), dtype, int(blocks), ctypes.byref(h)),
-              "create_plan")
+        check(getattr(self.lib, self._create)(int(hq), int(hkv), int(dim), int(page),
+                                              int(max_batch), int(max_pages), dtype, int(blocks),
+                                              ctypes.byref(h)), "create_plan")
         self.handle = h
         self.hq, self.hkv, self.dim, self.page = hq, hkv, dim, page
         self.bf16, self.blocks = bool(bf16), blocks
@@ -307,6 +309,163 @@ class AttentionPlan:
             pass
 
 
+# ---------------------------------------------------------------------------
+# 8-bit KV cache (no reference counterpart)
+# ---------------------------------------------------------------------------
+
+class Kv8Pool:
+    """One layer's K or V in 8 bits: `codes` [cache_slots, hkv, dim] in
+    float8_e4m3fn and `exps` uint8 [cache_slots / 16, hkv], the biased
+    exponents of the scales of 16 slots (value = code * 2 ** (exp - 127)).
+    Both contiguous CUDA tensors on one device; they may be slices of larger
+    tensors that hold all layers."""
+
+    __slots__ = ("codes", "exps")
+
+    def __init__(self, codes, exps):
+        torch = _torch()
+        for name, t, dt, nd in (("codes", codes, torch.float8_e4m3fn, 3),
+                                ("exps", exps, torch.uint8, 2)):
+            if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype == dt and
+                    t.dim() == nd and t.is_contiguous()):
+                raise ValueError(f"{name}: expected a contiguous {nd}-d {dt} CUDA tensor")
+        if codes.shape[0] % _lib.FE_KV8_BLOCK or \
+                tuple(exps.shape) != (codes.shape[0] // _lib.FE_KV8_BLOCK, codes.shape[1]):
+            raise ValueError(f"exps {tuple(exps.shape)} do not fit codes {tuple(codes.shape)}: "
+                             "one row per 16 slots")
+        if exps.device != codes.device:
+            raise ValueError("codes and exps are on different devices")
+        self.codes, self.exps = codes, exps
+
+    @classmethod
+    def empty(cls, num_blocks, page, hkv, dim, device="cuda"):
+        """A zeroed pool of num_blocks pages and the padding page."""
+        torch = _torch()
+        slots = (int(num_blocks) + 1) * int(page)
+        codes = torch.zeros(slots, hkv, dim, dtype=torch.uint8, device=device)
+        exps = torch.full((slots // _lib.FE_KV8_BLOCK, hkv), 127, dtype=torch.uint8, device=device)
+        return cls(codes.view(torch.float8_e4m3fn), exps)
+
+    @property
+    def cache_slots(self):
+        return int(self.codes.shape[0])
+
+
+def _kv8_pair(kpool, vpool):
+    if kpool.codes.shape != vpool.codes.shape:
+        raise ValueError("the K and V pools differ in shape")
+
+
+def _kv8_rows(name, t, like, heads=None):
+    torch = _torch()
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.is_contiguous() and t.dim() == 3):
+        raise ValueError(f"{name}: expected a contiguous CUDA tensor [rows, heads, dim]")
+    if t.dtype != like.dtype or t.shape[0] != like.shape[0] or t.shape[2] != like.shape[2] or \
+            (heads is not None and t.shape[1] != heads):
+        raise ValueError(f"{name}: {t.dtype} {tuple(t.shape)} does not fit "
+                         f"{like.dtype} {tuple(like.shape)}")
+
+
+def append_kv8(q, k, v, kpool, vpool, slots, pos=None, cache=None, q_out=None, stream=None):
+    """rope_append into 8-bit pools, one launch: q [rows, hq, dim] rotated into
+    `q_out` (default: in place; q may be None), k [rows, hkv, dim] rotated and
+    v quantised into `kpool` / `vpool` through `slots` (int64 [rows]). pos int64
+    [rows] and cache fp32 [max_positions, rotary_dim] as in rope(); cache None
+    rotates nothing. Rows of one 16-slot block must be adjacent and in order."""
+    lib = _lib.load()
+    torch = _torch()
+    _kv8_pair(kpool, vpool)
+    _kv8_rows("k", k, k, int(kpool.codes.shape[1]))
+    _kv8_rows("v", v, k, int(k.shape[1]))
+    rows, hkv, dim = (int(x) for x in k.shape)
+    if dim != kpool.codes.shape[2]:
+        raise ValueError(f"k: head_dim {dim}, the pools have {int(kpool.codes.shape[2])}")
+    hq = 0
+    if q is not None:
+        q_out = q if q_out is None else q_out
+        _kv8_rows("q", q, k)
+        _kv8_rows("q_out", q_out, q, int(q.shape[1]))
+        hq = int(q.shape[1])
+    index = [("slots", slots)] + ([("pos", pos)] if cache is not None else [])
+    for name, t in index:
+        if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype == torch.int64 and
+                t.is_contiguous() and t.numel() == rows):
+            raise ValueError(f"{name}: expected a contiguous int64 CUDA tensor of {rows}")
+    rot = most = 0
+    if cache is not None:
+        if not (cache.is_cuda and cache.dtype == torch.float32 and cache.is_contiguous() and
+                cache.dim() == 2):
+            raise ValueError("cache: expected a contiguous fp32 CUDA tensor "
+                             "[max_positions, rotary_dim]")
+        most, rot = (int(x) for x in cache.shape)
+    check(lib.fe_kv8_append(_ptr(q) if hq else None, _ptr(q_out) if hq else None, _ptr(k), _ptr(v),
+                            _ptr(kpool.codes), _ptr(vpool.codes), _ptr(kpool.exps),
+                            _ptr(vpool.exps), _ptr(slots), _ptr(pos) if rot else None,
+                            _ptr(cache) if rot else None, rows, hq, hkv, dim, rot, most,
+                            dtype_code(k), kpool.cache_slots, _stream(stream)), "append_kv8")
+
+
+def gather_kv8(pool, out, kv, pages, last, row_offset, max_len, page, stream=None):
+    """Whole sequences' values from an 8-bit pool into rows of `out` [rows,
+    hkv, dim] (16-bit), metadata as gather(): int32 CUDA tensors."""
+    lib = _lib.load()
+    for t in (kv, pages, last, row_offset):
+        _require_device_i32(t)
+    hkv, dim = int(pool.codes.shape[1]), int(pool.codes.shape[2])
+    if not out.is_contiguous() or out.numel() % (hkv * dim):
+        raise ValueError("out: expected a contiguous tensor [rows, hkv, dim]")
+    check(lib.fe_kv8_gather(_ptr(pool.codes), _ptr(pool.exps), _ptr(out), _ptr(kv), _ptr(pages),
+                            _ptr(last), _ptr(row_offset), int(kv.shape[0]) - 1, int(max_len),
+                            int(page), hkv, dim, dtype_code(out), pool.cache_slots,
+                            _stream(stream)), "gather_kv8")
+
+
+def copy_blocks_kv8(k_pools, v_pools, src, dst, ntok, page, stream=None):
+    """copy_blocks for 8-bit pools (lists of Kv8Pool, one per layer): codes
+    and scales. src/dst/ntok: int32 CUDA tensors."""
+    lib = _lib.load()
+    n = len(k_pools)
+    if n != len(v_pools):
+        raise ValueError("k_pools and v_pools differ in length")
+    for t in (src, dst, ntok):
+        _require_device_i32(t)
+    if n == 0:
+        return
+    shape = k_pools[0].codes.shape
+    for p in (*k_pools, *v_pools):
+        if p.codes.shape != shape:
+            raise ValueError("the layers' pools differ in shape")
+    arr = lambda ts: (_P * n)(*[t.data_ptr() for t in ts])  # noqa: E731
+    check(lib.fe_kv8_copy_blocks(arr([p.codes for p in k_pools]), arr([p.codes for p in v_pools]),
+                                 arr([p.exps for p in k_pools]), arr([p.exps for p in v_pools]), n,
+                                 _ptr(src), _ptr(dst), _ptr(ntok), int(src.shape[0]), int(page),
+                                 int(shape[1]), int(shape[2]), int(shape[0]) // int(page),
+                                 _stream(stream)), "copy_blocks_kv8")
+
+
+class Kv8Plan(AttentionPlan):
+    """An attention plan over 8-bit pools: prepared like any other plan;
+    `attention` takes Kv8Pools. bf16: the dtype of q and out."""
+
+    _create = "fe_kv8_plan_create"
+
+    def attention(self, q, kpool, vpool, out, causal=True, stream=None):
+        torch = _torch()
+        _kv8_pair(kpool, vpool)
+        want = ((int(self.blocks) + 1) * int(self.page), self.hkv, self.dim)
+        if tuple(kpool.codes.shape) != want:
+            raise ValueError(f"pools of shape {tuple(kpool.codes.shape)}, the plan is for {want}")
+        dt = torch.bfloat16 if self.bf16 else torch.float16
+        for name, t in (("q", q), ("out", out)):
+            if not (t.is_cuda and t.is_contiguous() and t.dtype == dt and
+                    tuple(t.shape[-2:]) == (self.hq, self.dim)):
+                raise ValueError(f"{name}: expected a contiguous {dt} CUDA tensor [rows, "
+                                 f"{self.hq}, {self.dim}]")
+        check(self.lib.fe_kv8_attn_run(self.handle, _ptr(q), _ptr(kpool.codes), _ptr(vpool.codes),
+                                       _ptr(kpool.exps), _ptr(vpool.exps), _ptr(out),
+                                       int(bool(causal)), _stream(stream)), "attention")
+
+
 def create_plan(hq, hkv, dim, page, max_batch, max_pages, bf16, blocks) -> AttentionPlan:
     return AttentionPlan(hq, hkv, dim, page, max_batch, max_pages, bf16, blocks)
 
@@ -380,13 +539,15 @@ class HostPlan:
     """fe_attn_plan_create_host: validates metadata and builds the work list
     on the host for `grid_cap` CTAs, without touching a GPU."""
 
+    _create = "fe_attn_plan_create_host"
+
     def __init__(self, hq, hkv, dim, page, max_batch, max_pages, bf16, blocks, grid_cap=296):
         self.lib = _lib.load()
         h = _P()
         dtype = FE_DTYPE_BF16 if bf16 else FE_DTYPE_F16
-        check(self.lib.fe_attn_plan_create_host(int(hq), int(hkv), int(dim), int(page),
-                                                int(max_batch), int(max_pages), dtype, int(blocks),
-                                                int(grid_cap), ctypes.byref(h)), "create_host")
+        check(getattr(self.lib, self._create)(int(hq), int(hkv), int(dim), int(page),
+                                              int(max_batch), int(max_pages), dtype, int(blocks),
+                                              int(grid_cap), ctypes.byref(h)), "create_host")
         self.handle = h
         self.G = hq // hkv
 
@@ -415,6 +576,13 @@ class HostPlan:
             pass
 
 
-__all__ = ["store", "copy_blocks", "paged_decode_noalloc", "clear_pages", "gather", "device_errors", "AttentionPlan",
+class HostKv8Plan(HostPlan):
+    """HostPlan with the lists of a Kv8Plan."""
+
+    _create = "fe_kv8_plan_create_host"
+
+
+__all__ = ["Kv8Pool", "Kv8Plan", "HostKv8Plan", "append_kv8", "gather_kv8", "copy_blocks_kv8",
+           "store", "copy_blocks", "paged_decode_noalloc", "clear_pages", "gather", "device_errors", "AttentionPlan",
            "create_plan", "destroy_plan", "prepare_plan", "attention", "HostPlan", "FeError",
            "dtype_code", "ITEM_DTYPE", "GROUP_DTYPE", "SEQ_DTYPE", "parse_meta"]

@@ -261,6 +261,93 @@ int fe_paged_decode_noalloc(const void* q, const void* k_pool, const void* v_poo
                             int dtype, void* stream);
 
 /* ------------------------------------------------------------------------
+ * 8-bit KV cache (no reference counterpart: the reference's pools are
+ * 16-bit, src/cuda_model.cpp:60). Keys and values are e4m3 codes
+ * [cache_slots, hkv, dim] with one power-of-two scale per block of
+ * FE_KV8_BLOCK consecutive slots and KV head, stored as its biased exponent,
+ * uint8 [cache_slots / FE_KV8_BLOCK, hkv]:
+ *   value = code * 2^(exponent - 127).
+ * Half the bytes of a 16-bit pool (and 1/16 byte per 128 for the scales), so
+ * half the attention traffic and twice the tokens; slots, block tables, page
+ * lists and plans are as for the 16-bit pools. page is a multiple of 16.
+ *
+ * What a cache holds is set by fe_kv8_append: exponents within 2^-32 .. 2^64
+ * (bytes 95 .. 191; the attention and gather operators read a byte outside
+ * as the nearest of these, so pages never written to are harmless beyond a
+ * sequence's end), codes of magnitude up to 448, NaN where the input was
+ * NaN.
+ * ------------------------------------------------------------------------ */
+#define FE_KV8_BLOCK 16
+
+/* Rotation, quantisation and append in one launch. q [rows, hq, dim] is
+ * rotated into q_out (which may be q; hq may be 0) exactly as by fe_rope; k is
+ * rotated the same way, in fp32 and not rounded before it is quantised; v is
+ * taken as it is. rotary_dim = 0 rotates nothing (pos and cache may be NULL; q
+ * is copied).
+ * A RUN is a sequence of adjacent rows (skipped ones aside) whose slots lie in
+ * one block, in increasing order. Per KV head, and for K and V apart, a run's scale is the smallest
+ * power of two s with |x| <= 448 s for its largest finite magnitude |x|, no
+ * smaller than the block's present scale when the run does not begin at the
+ * block's first slot: the tokens before it are kept, and their codes are
+ * rounded to the new scale when it grew (exact but for codes that become
+ * subnormal). Tokens of the block after the run are not kept: an append at
+ * slot n leaves slots n + 1 .. of its block undefined (they hold rejected
+ * drafts at most; the next append overwrites them). Codes are rounded to
+ * nearest even; infinities saturate, NaN stays NaN.
+ * A call has at most one run in a block (every step's slot mapping does: a
+ * sequence's rows are adjacent and in order): two would race for its scale,
+ * and that block's contents are then unspecified.
+ *   slots: int64 [rows]; < 0: skipped; >= cache_slots: skipped,
+ *          FE_DEVERR_SLOT_RANGE. pos: int64 [rows]; outside [0,
+ *          max_positions): the row's k, v and q are skipped,
+ *          FE_DEVERR_POS_RANGE.
+ * dim 128 or 256; rotary_dim a multiple of 8; cache_slots a multiple of 16;
+ * q, k, v and codes 8-byte aligned, the cos / sin cache 16-byte aligned. */
+int fe_kv8_append(const void* q, void* q_out, const void* k, const void* v, uint8_t* k_codes,
+                  uint8_t* v_codes, uint8_t* k_exp, uint8_t* v_exp, const int64_t* slots,
+                  const int64_t* pos, const float* cache, int rows, int hq, int hkv, int dim,
+                  int rotary_dim, int max_positions, int dtype, int64_t cache_slots,
+                  void* stream);
+
+/* fe_kv_gather from an 8-bit pool: the values, rounded to the 16-bit `dtype`
+ * (bf16 holds every one exactly). A page id that reaches past cache_slots
+ * leaves its token unwritten and raises FE_DEVERR_PAGE_RANGE. max_len bounds
+ * the launch only: longer sequences are covered by striding. */
+int fe_kv8_gather(const uint8_t* codes, const uint8_t* exps, void* out, const int32_t* kv,
+                  const int32_t* pages, const int32_t* last, const int32_t* row_offset, int batch,
+                  int max_len, int page, int hkv, int dim, int dtype, int64_t cache_slots,
+                  void* stream);
+
+/* fe_kv_copy_blocks for 8-bit pools: token rows [0, ntok[c]) of page src[c]
+ * onto page dst[c], and the scales of the blocks they lie in, in every layer's
+ * K and V pool (HOST arrays of num_layers device pointers). Works on the lists
+ * of fe_kv_fork_copies. */
+int fe_kv8_copy_blocks(void* const* k_codes, void* const* v_codes, void* const* k_exps,
+                       void* const* v_exps, int num_layers, const int32_t* src,
+                       const int32_t* dst, const int32_t* ntok, int num_copies, int page, int hkv,
+                       int dim, int num_pages_total, void* stream);
+
+/* Attention over 8-bit pools. A plan of fe_kv8_plan_create is prepared by the
+ * same calls as any other (fe_attn_plan_prepare, _prepare_device,
+ * fe_step_prepare_device), serves fe_kv8_attn_run only, and is destroyed by
+ * fe_attn_plan_destroy; dtype is that of q and out. Its row lists are cut
+ * across CTAs by keys as its decode list is.
+ * fe_kv8_attn_run is fe_attn_run over the values of the codes: the same masks
+ * (every query row sees at least one key: a prepared sequence has no fewer
+ * keys than query rows), scale 1/sqrt(dim), fp32 softmax and accumulation,
+ * output rounded to nearest even. Queries enter the product as two e4m3 parts
+ * (8 to 9 significant bits: bf16's own), softmax weights as three e5m2 parts
+ * (decode rows, 9 bits) or f16 (multi-row sequences), both over a range of
+ * 2^26 and more below the row's largest. A query row that holds an
+ * infinity or NaN gives NaN. Exponent arrays are aligned to gcd(hkv, 8) bytes
+ * (2 at most for dim 256), all other buffers to 16. */
+int fe_kv8_plan_create(int hq, int hkv, int dim, int page, int max_batch, int max_pages, int dtype,
+                       int num_blocks, fe_attn_plan** plan_out);
+int fe_kv8_attn_run(fe_attn_plan* plan, const void* q, const uint8_t* k_codes,
+                    const uint8_t* v_codes, const uint8_t* k_exp, const uint8_t* v_exp, void* out,
+                    int causal, void* stream);
+
+/* ------------------------------------------------------------------------
  * Device-side step preparation (no reference counterpart: replaces the host
  * loops of CudaModel::prepare, src/cuda_model.cpp:131-142, and the host
  * planning plus pageable H2D copies of prepare_plan,
@@ -317,6 +404,8 @@ int fe_attn_plan_get_info(const fe_attn_plan* plan, fe_attn_plan_info* info);
  * and builds the work list, for `grid_cap` persistent CTAs. */
 int fe_attn_plan_create_host(int hq, int hkv, int dim, int page, int max_batch, int max_pages,
                              int dtype, int num_blocks, int grid_cap, fe_attn_plan** plan_out);
+int fe_kv8_plan_create_host(int hq, int hkv, int dim, int page, int max_batch, int max_pages,
+                            int dtype, int num_blocks, int grid_cap, fe_attn_plan** plan_out);
 /* Copy the packed work-list metadata of the last prepare into `dst` (at most
  * `cap` bytes); *bytes receives its full size. Layout: fe_attn_plan.h. */
 int fe_attn_plan_debug_meta(const fe_attn_plan* plan, void* dst, int64_t cap, int64_t* bytes);
