@@ -8,20 +8,15 @@
 // token's block and m a running maximum of s + v (not of s), the kernel keeps
 //   w(t) = 2^(s(t) + v(t) - m),  O = sum w(t) code_v(t),  l = sum w(t) 2^-v(t)
 // and the output is O / l: V's scales cost one addition per 16 tokens, K's one
-// factor per 16 tokens, and the codes feed the tensor core as they lie in the
-// cache. The other operand of each product is split into 8-bit parts:
-//  * a query row into two e4m3 parts (high part and residual, 8 to 9
-//    significant bits: exactly a bf16 where its magnitude is within 2^11 of
-//    the row's largest, and an error of 2^-19 of that below);
-//  * a weight into three e5m2 parts (9 bits). e5m2 and not e4m3, for the
-//    range: weights are kept up to 2^15, so they keep their bits down to
-//    2^-26 of the largest. Two e4m3 parts reach 2^-18, and a long context whose
-//    first token takes most of the softmax would lose its other tokens.
-//    The first two parts are cut, not rounded (a half's upper byte is its
-//    value cut to e5m2), the last is rounded.
-// Products on mma.m16n8k32 (fp32 accumulation): measured on a B200 one takes
-// 5 clocks a warp and SM quarter against 8 for the 16-bit m16n8k16, so the
-// parts cost about what one 16-bit product does, and no code is converted.
+// factor per 16 tokens. Both products run on mma.m16n8k16 in f16 with fp32
+// accumulation: the codes become halves, exactly, in registers (one conversion
+// for two codes); queries are halves times a power of two per row (f16 as they
+// are, bf16 exactly down to 2^-29 of the row's largest); weights are halves
+// times 2^15, so that they keep 11 bits down to 2^-29 of the largest.
+// mma.m16n8k32 on the codes themselves, with the other operand in two or three
+// 8-bit parts, was built and measured first: on a B200 one takes 21 to 29
+// clocks a warp and SM quarter when its operands change (the 16-bit one 10), a
+// step of this kernel 3200 clocks, and it was bound by them and not by HBM.
 //
 // B200 design, as fe_decode.cu: bound by HBM traffic. One persistent CTA per
 // SM with 8 consumer warps and a producer warp; an item is (sequence, group
@@ -30,6 +25,7 @@
 // K and one for V into a ring of 128-192 KiB. The tiles' scale exponents are
 // gathered by the producer's lanes a batch ahead and travel with the stage.
 #include <mutex>
+#include <type_traits>
 
 #include "fe_attn_common.cuh"
 #include "fe_kv8_attn.h"
@@ -66,40 +62,17 @@ struct Cfg {
   static_assert(H == 8 || kStages % (kConsumers / H) == 0, "see above");
 };
 
-__device__ __forceinline__ void mma_e4m3(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
-                                         uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-      "{%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-__device__ __forceinline__ void mma_e4m3_e5m2(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
-                                              uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e5m2.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-      "{%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-__device__ __forceinline__ uint32_t hsub2(uint32_t a, uint32_t b) {
-  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&a),
-                            *reinterpret_cast<const __half2*>(&b));
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
-
 // 8*NT packed rows (columns of the products) of one KV head of D dims.
 // Fragment layout: the tokens of a tile are the M side of S^T = K Q^T, dims
-// the M side of O^T = V^T W^T. O row i of m-tile mt is dim 16 mt + 2 i (i < 8)
-// or 16 mt + 2 (i - 8) + 1: the byte pairs that a transposed 16-bit load of
-// 8-bit V delivers.
+// the M side of O^T = V^T W^T. A 32-bit word of K holds dims 4cq .. 4cq + 3 of
+// a 16-dim chunk (cq = lane % 4); its halves are k elements 2cq, 2cq + 1 and
+// 2cq + 8, 2cq + 9 of a product over that chunk, and Q's words are picked to
+// match. O row i of m-tile mt is dim 16 mt + 2 i (i < 8) or 16 mt + 2 (i - 8)
+// + 1: the byte pairs that a transposed 16-bit load of 8-bit V delivers.
 template <typename T, int NT, int D>
 struct State {
-  static constexpr int kKS = D / 32;  // k-steps of S^T
-  static constexpr int kMT = D / 16;  // m-tiles of O^T
-  uint32_t qh[NT][kKS][2], ql[NT][kKS][2];
+  static constexpr int kMT = D / 16;  // 16-dim chunks: k-steps of S^T, m-tiles of O^T
+  uint32_t qf[NT][kMT][2];
   float f[NT][2];  // base-2 score units per raw product, per column of this lane
   int lim[NT][2];
   int lim_min;
@@ -118,30 +91,39 @@ struct State {
       const int p = col0 + nt * 8 + r8;
       const T* qp = p < P ? q + (static_cast<int64_t>(si.q_row0 + p / G) * hq + head0 + p % G) * D
                           : nullptr;
-      uint2 raw[kKS][2];
-      float amax = 0.f;
 #pragma unroll
-      for (int ks = 0; ks < kKS; ++ks)
+      for (int c = 0; c < kMT; ++c) {
+        uint2 raw = make_uint2(0u, 0u);
+        if (qp) raw = __ldg(reinterpret_cast<const uint2*>(qp + 16 * c + 4 * cq));
+        qf[nt][c][0] = raw.x;
+        qf[nt][c][1] = raw.y;
+      }
+      float mine = scale_log2;
+      if constexpr (!std::is_same<T, __half>::value) {
+        // into f16's range: the row's largest magnitude to [2^14, 2^15)
+        float amax = 0.f;
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          raw[ks][x] = make_uint2(0u, 0u);
-          if (qp) raw[ks][x] = __ldg(reinterpret_cast<const uint2*>(qp + ks * 32 + x * 16 + 4 * cq));
-          const float2 a = unpack2<T>(raw[ks][x].x), b = unpack2<T>(raw[ks][x].y);
-          const float v[4] = {fabsf(a.x), fabsf(a.y), fabsf(b.x), fabsf(b.y)};
+        for (int c = 0; c < kMT; ++c)
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (v[e] < INFINITY) amax = fmaxf(amax, v[e]);
-        }
-      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-      const int e = kv8_query_exp(amax);
-      const float up = exp_scale(254 - e);
+          for (int x = 0; x < 2; ++x) {
+            const float2 v = unpack2<T>(qf[nt][c][x]);
+            if (fabsf(v.x) < INFINITY) amax = fmaxf(amax, fabsf(v.x));
+            if (fabsf(v.y) < INFINITY) amax = fmaxf(amax, fabsf(v.y));
+          }
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+        // (at least 2^-60: products of smaller rows stay normal numbers)
+        const int e = max((__float_as_int(amax) >> 23) - 14, 67);
+        const float up = exp_scale(254 - e);
 #pragma unroll
-      for (int ks = 0; ks < kKS; ++ks)
+        for (int c = 0; c < kMT; ++c)
 #pragma unroll
-        for (int x = 0; x < 2; ++x)
-          kv8_split_query<T>(raw[ks][x], up, qh[nt][ks][x], ql[nt][ks][x]);
-      const float mine = exp_scale(e) * scale_log2;
+          for (int x = 0; x < 2; ++x) {
+            const float2 v = unpack2<T>(qf[nt][c][x]);
+            qf[nt][c][x] = pack2<__half>(v.x * up, v.y * up);
+          }
+        mine *= exp_scale(e);
+      }
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         f[nt][c] = __shfl_sync(0xffffffffu, mine, (2 * cq + c) * 4);
@@ -166,25 +148,31 @@ struct State {
                                        const int (&ke)[2], const int (&ve)[2], int tbase,
                                        int length, int lane) {
     const int r8 = lane >> 2, cq = lane & 3, mi = lane >> 3, li = lane & 7;
-    // ---- S^T = K Q^T
+    // ---- S^T = K Q^T, the two tiles' products alternating
     float s[2][NT][4];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
+    for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) s[u][nt][0] = s[u][nt][1] = s[u][nt][2] = s[u][nt][3] = 0.f;
-      const uint32_t row = ka + u * tile_bytes + (li + ((mi & 1) << 3)) * 128;
+    const uint32_t krow = ka + (li + ((mi & 1) << 3)) * 128;
 #pragma unroll
-      for (int ks = 0; ks < kKS; ++ks) {
-        const int c = 2 * ks + (mi >> 1);  // 16-code chunk of the row, 8 per box
-        uint32_t af[4];
-        ldmatrix_x4(row + (c >> 3) * kBoxBytes + (((c & 7) ^ li) << 4), af[0], af[1], af[2],
-                    af[3]);
+    for (int c2 = 0; c2 < kMT / 2; ++c2) {
+      const int c = 2 * c2 + (mi >> 1);  // 16-code chunk of the row, 8 per box
+      const uint32_t at = krow + (c >> 3) * kBoxBytes + (((c & 7) ^ li) << 4);
+      uint32_t w[2][4];  // tokens r8, r8 + 8 of chunk 2 c2, then of chunk 2 c2 + 1
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          mma_e4m3(s[u][nt], af, qh[nt][ks][0], qh[nt][ks][1]);
-          mma_e4m3(s[u][nt], af, ql[nt][ks][0], ql[nt][ks][1]);
+      for (int u = 0; u < 2; ++u)
+        ldmatrix_x4(at + u * tile_bytes, w[u][0], w[u][1], w[u][2], w[u][3]);
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const uint32_t af[4] = {e4m3x2_to_h2(w[u][2 * x]), e4m3x2_to_h2(w[u][2 * x + 1]),
+                                  e4m3x2_hi_to_h2(w[u][2 * x]), e4m3x2_hi_to_h2(w[u][2 * x + 1])};
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+            mma_16816<__half>(s[u][nt], af, qf[nt][2 * c2 + x][0], qf[nt][2 * c2 + x][1]);
         }
-      }
     }
     // ---- hide keys past each column's limit
     if (tbase + kStepTokens > lim_min) {
@@ -201,7 +189,6 @@ struct State {
     const float kf[2] = {exp_scale(ke[0]), exp_scale(ke[1])};
     const float vf[2] = {float(ve[0] - 127), float(ve[1] - 127)};
     const float vi[2] = {exp_scale(254 - ve[0]), exp_scale(254 - ve[1])};
-    uint32_t bw[3][NT][2];  // parts of W^T
     float al[NT][2];
     bool moved = false;
 #pragma unroll
@@ -243,47 +230,55 @@ struct State {
           o[nt][mt][3] *= al[nt][1];
         }
     }
-    // ---- W^T as B fragments. A 16-bit element holds the codes of tokens r8
-    // (low) and r8 + 8 of one column; transposed, a lane has column lane / 4
-    // and tokens 2cq, 2cq + 8, 2cq + 1, 2cq + 9 of the tile, lowest byte first.
+    // ---- W^T as B fragments
+    uint32_t bw[2][NT][2];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const uint32_t w0 = pack2<__half>(s[u][nt][0], s[u][nt][2]);
-        const uint32_t w1 = pack2<__half>(s[u][nt][1], s[u][nt][3]);
-        const uint32_t r0 = hsub2(w0, w0 & 0xff00ff00u), r1 = hsub2(w1, w1 & 0xff00ff00u);
-        const uint32_t t0 = hsub2(r0, r0 & 0xff00ff00u), t1 = hsub2(r1, r1 & 0xff00ff00u);
-        bw[0][nt][u] = movmatrix_trans(__byte_perm(w0, w1, 0x7531));
-        bw[1][nt][u] = movmatrix_trans(__byte_perm(r0, r1, 0x7531));
-        bw[2][nt][u] = movmatrix_trans(e5m2x2_h2(t0) | e5m2x2_h2(t1) << 16);
-      }
-    // ---- codes of V rows past the end are zeroed (anything may lie there,
-    // and 0 * NaN would poison O)
-    uint32_t vm[2] = {0xffffffffu, 0xffffffffu};
-    if (tbase + kStepTokens > length) {
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int t = tbase + u * kTileTokens + 2 * cq;
-        vm[u] = (t < length ? 0xffu : 0u) | (t + 8 < length ? 0xff00u : 0u) |
-                (t + 1 < length ? 0xff0000u : 0u) | (t + 9 < length ? 0xff000000u : 0u);
-      }
-    }
-    // ---- O^T += V^T W^T
-    const uint32_t row = va + (mi >> 1) * tile_bytes + (li + ((mi & 1) << 3)) * 128;
-#pragma unroll
-    for (int mt = 0; mt < kMT; ++mt) {
-      uint32_t x0, y0, x1, y1;  // tokens 0-7 and 8-15 of either tile, dims 16 mt ..
-      ldmatrix_x4_trans(row + (mt >> 3) * kBoxBytes + (((mt & 7) ^ li) << 4), x0, y0, x1, y1);
-      uint32_t a[4];
-      a[0] = __byte_perm(x0, y0, 0x6240) & vm[0];
-      a[1] = __byte_perm(x0, y0, 0x7351) & vm[0];
-      a[2] = __byte_perm(x1, y1, 0x6240) & vm[1];
-      a[3] = __byte_perm(x1, y1, 0x7351) & vm[1];
+    for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int x = 0; x < 3; ++x) mma_e4m3_e5m2(o[nt][mt], a, bw[x][nt][0], bw[x][nt][1]);
+        for (int x = 0; x < 2; ++x)
+          bw[u][nt][x] = movmatrix_trans(pack2<__half>(s[u][nt][2 * x], s[u][nt][2 * x + 1]));
+    // ---- codes of V rows past the end are zeroed (anything may lie there,
+    // and 0 * NaN would poison O): bytes of tokens 2cq and 2cq + 1, twice
+    uint32_t vm[2][2] = {{0xffffffffu, 0xffffffffu}, {0xffffffffu, 0xffffffffu}};
+    if (tbase + kStepTokens > length) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const int t = tbase + u * kTileTokens + 8 * x + 2 * cq;
+          vm[u][x] = (t < length ? 0x00ff00ffu : 0u) | (t + 1 < length ? 0xff00ff00u : 0u);
+        }
+    }
+    // ---- O^T += V^T W^T, two m-tiles at a time
+    const uint32_t vrow = va + (mi >> 1) * tile_bytes + (li + ((mi & 1) << 3)) * 128;
+#pragma unroll
+    for (int m0 = 0; m0 < kMT; m0 += 2) {
+      uint32_t a[2][2][4];  // [m-tile][tile]
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int mt = m0 + i;
+        uint32_t w[2][2];  // [tile][tokens 0-7, 8-15], dims 16 mt ..
+        ldmatrix_x4_trans(vrow + (mt >> 3) * kBoxBytes + (((mt & 7) ^ li) << 4), w[0][0], w[0][1],
+                          w[1][0], w[1][1]);
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            // both tokens of the even dim, then both of the odd dim
+            const uint32_t y = __byte_perm(w[u][x], 0, 0x3120) & vm[u][x];
+            a[i][u][2 * x] = e4m3x2_to_h2(y);
+            a[i][u][2 * x + 1] = e4m3x2_hi_to_h2(y);
+          }
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+            mma_16816<__half>(o[nt][m0 + i], a[i][u], bw[u][nt][0], bw[u][nt][1]);
     }
   }
 
