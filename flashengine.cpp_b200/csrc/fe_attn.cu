@@ -261,6 +261,9 @@ PlanConfig make_config(int hq, int hkv, int dim, int page, int max_batch, int ma
   c.row_split = false;      // the tcgen05 kernel walks an item's whole key range
   c.cut_rows = dim == kWideHeadDim || kv8;
   c.elem_bytes = kv8 ? 1 : 2;
+  // a step of the 8-bit decode kernel is two tiles: two steps, where a short
+  // batch leaves SMs idle, cost less than four in a row and their merge
+  c.dec_min_tiles = kv8 ? 4 : 8;
   int64_t items = int64_t(max_batch) * hkv * 64;
   if (items < 8192) items = 8192;
   if (items > (1 << 20)) items = 1 << 20;
@@ -471,6 +474,7 @@ int prepare_on_device(fe_attn_plan* p, DevPlanArgs& a, int batch, int rows, void
   a.dec_heads = c.dec_heads;
   a.grid_cap = c.grid_cap;
   a.dec_grid_cap = c.dec_grid_cap;
+  a.dec_min_tiles = c.dec_min_tiles;
   a.max_items = c.max_items;
   a.max_groups = c.max_groups;
   a.partial_capacity = c.partial_capacity;

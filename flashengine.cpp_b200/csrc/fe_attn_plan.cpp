@@ -388,7 +388,7 @@ int build_plan(const PlanConfig& cfg, const int32_t* qo, const int32_t* kv, cons
       rc = build_view(cfg, row_units_causal, row_cap, 4, row_min_chunk, fixed_grid, views[1], err);
     }
     if (rc != FE_OK) return rc;
-    rc = build_cut_view(cfg, key_units, dec_cap, 8, fixed_grid, views[2], err);
+    rc = build_cut_view(cfg, key_units, dec_cap, cfg.dec_min_tiles, fixed_grid, views[2], err);
     if (rc != FE_OK) return rc;
   }
   // Both kernels of one run share the split workspace and counters: offset

@@ -83,6 +83,7 @@ struct PlanConfig {
   bool row_split;             // row-mode key ranges may be split across CTAs
   bool cut_rows;              // row lists are cut exactly, as the decode list (head_dim 256, 8-bit)
   int elem_bytes;             // bytes of a cached element
+  int dec_min_tiles;          // fewest key tiles per CTA of the decode list, while CTAs are left
   int max_items;              // work-item capacity
   int64_t partial_capacity;   // floats in the split-K workspace
   int max_groups;             // split-counter capacity

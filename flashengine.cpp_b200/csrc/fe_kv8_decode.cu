@@ -492,29 +492,40 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       return e;
     };
-    // page ids are the plan's metadata, fetched before waiting for the kernel
-    // that owns the pools
-    const WorkItem w0 = items[it0];
-    const SeqInfo si0 = seqs[w0.seq];
-    const int first = tile_slot(w0, si0, w0.kt0 + lane);
-    const int second = tile_slot(w0, si0, w0.kt0 + 32 + lane);
+    // The first two batches' slots of an item, and its first batch's exponents,
+    // are asked for while the item before it streams (they are four dependent
+    // loads). Page ids are the plan's metadata: the first item's are fetched
+    // before waiting for the kernel that owns the pools.
+    struct Head {
+      WorkItem w;
+      SeqInfo si;
+      int slot, slot2;
+      Exps e;
+    };
+    Head cur, next;
+    auto head_slots = [&](int it, Head& h) {
+      h.w = items[it];
+      h.si = seqs[h.w.seq];
+      h.slot = tile_slot(h.w, h.si, h.w.kt0 + lane);
+      h.slot2 = tile_slot(h.w, h.si, h.w.kt0 + 32 + lane);
+    };
+    head_slots(it0, next);
     pdl_wait();
+    next.e = tile_exps(next.w, next.slot);
     uint32_t g = 0;
     bool ok = true;
     for (int it = it0; it < it1 && ok; ++it) {
-      const WorkItem w = items[it];
-      const SeqInfo si = seqs[w.seq];
-      const int box = w.kvh * C::kBoxes;
-      int nxt = it == it0 ? first : tile_slot(w, si, w.kt0 + lane);
-      int nxt2 = it == it0 ? second : tile_slot(w, si, w.kt0 + 32 + lane);
-      Exps enxt = tile_exps(w, nxt);
-      for (int j0 = w.kt0; j0 < w.kt1 && ok; j0 += 32) {
-        const int n = min(32, w.kt1 - j0);
-        const int slot = nxt;
-        const Exps e = enxt;
-        nxt = nxt2;
-        enxt = tile_exps(w, nxt);
-        nxt2 = tile_slot(w, si, j0 + 64 + lane);
+      cur = next;
+      const int box = cur.w.kvh * C::kBoxes;
+      // steps of this item to issue before looking at the next one
+      int before = min(C::kStages, (cur.w.kt1 - cur.w.kt0 + kStepTiles - 1) / kStepTiles);
+      for (int j0 = cur.w.kt0; j0 < cur.w.kt1 && ok; j0 += 32) {
+        const int n = min(32, cur.w.kt1 - j0);
+        const int slot = cur.slot;
+        const Exps e = cur.e;
+        cur.slot = cur.slot2;
+        cur.e = tile_exps(cur.w, cur.slot);
+        cur.slot2 = tile_slot(cur.w, cur.si, j0 + 64 + lane);
         for (int jj = 0; jj < n; jj += kStepTiles) {
           const int s0 = __shfl_sync(0xffffffffu, slot, jj);
           const int s1 = __shfl_sync(0xffffffffu, slot, jj + 1);
@@ -544,6 +555,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (tiles == 2) tma_load_3d(st + C::kTileBytes, &vmap, &full[s], 0, s1, box);
           }
           ++g;
+          if (--before == 0 && it + 1 < it1) {
+            head_slots(it + 1, next);
+            next.e = tile_exps(next.w, next.slot);
+          }
         }
       }
     }
@@ -564,9 +579,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   pdl_wait();  // q and the split workspace belong to earlier kernels until here
   uint32_t g = 0;
   bool aborted = false;
+  WorkItem wi_next = items[it0];
+  SeqInfo si_next = seqs[wi_next.seq];
   for (int it = it0; it < it1; ++it) {
-    const WorkItem wi = items[it];
-    const SeqInfo si = seqs[wi.seq];
+    const WorkItem wi = wi_next;
+    const SeqInfo si = si_next;
+    if (it + 1 < it1) {  // in flight while this item runs
+      wi_next = items[it + 1];
+      si_next = seqs[wi_next.seq];
+    }
     const bool many = si.qrows * a.G > 8;
     if constexpr (D == 128) {
       if (many)

@@ -4,6 +4,7 @@
 // reference, whose pools are 16-bit (src/cuda_model.cpp:60); slot semantics,
 // rotation and roundings follow fe_kv_append / fe_rope.
 #include <cstring>
+#include <mutex>
 #include <string>
 
 #include "fe_kv8_common.cuh"
@@ -15,32 +16,70 @@ constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kQHeads = 4;  // query heads per thread of an append
 
-__device__ __forceinline__ float2 to_float2(uint32_t v, __half) {
-  return __half22float2(*reinterpret_cast<__half2*>(&v));
-}
-__device__ __forceinline__ float2 to_float2(uint32_t v, __nv_bfloat16) {
-  return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&v));
+// Four values as two fp32 pairs.
+struct Quad {
+  float2 x, y;
+};
+
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 ra, rb, rd;\n\t"
+      "mov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\t"
+      "mul.rn.f32x2 rd, ra, rb;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
 }
 
-// Four rotation pairs a[i], b[i] in fp32, each product and sum rounded
-// separately as fe_rope does.
-__device__ __forceinline__ void rotate4(float* a, float* b, const float (&c)[4],
-                                        const float (&s)[4]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float x = a[i], y = b[i];
-    a[i] = __fsub_rn(__fmul_rn(x, c[i]), __fmul_rn(y, s[i]));
-    b[i] = __fadd_rn(__fmul_rn(y, c[i]), __fmul_rn(x, s[i]));
-  }
+// A rotation pair in fp32, each product and sum rounded separately as fe_rope
+// does (the packed fp32 instructions were not: ptxas fused them).
+__device__ __forceinline__ void rotate1(float& a, float& b, float c, float s) {
+  const float x = a;
+  a = __fsub_rn(__fmul_rn(x, c), __fmul_rn(b, s));
+  b = __fadd_rn(__fmul_rn(b, c), __fmul_rn(x, s));
+}
+__device__ __forceinline__ void rotate4(Quad& a, Quad& b, const float* cos, const float* sin) {
+  const float4 c = *reinterpret_cast<const float4*>(cos);
+  const float4 s = *reinterpret_cast<const float4*>(sin);
+  rotate1(a.x.x, b.x.x, c.x, s.x);
+  rotate1(a.x.y, b.x.y, c.y, s.y);
+  rotate1(a.y.x, b.y.x, c.z, s.z);
+  rotate1(a.y.y, b.y.y, c.w, s.w);
 }
 
 template <typename T>
-__device__ __forceinline__ void unpack4(float* x, uint2 v) {
-  const float2 a = to_float2(v.x, T()), b = to_float2(v.y, T());
-  x[0] = a.x;
-  x[1] = a.y;
-  x[2] = b.x;
-  x[3] = b.y;
+__device__ __forceinline__ Quad unpack4(uint2 v) {
+  return Quad{unpack2<T>(v.x), unpack2<T>(v.y)};
+}
+
+__device__ __forceinline__ float max4(float m, const Quad& q) {
+  return fmaxf(fmaxf(fmaxf(m, fabsf(q.x.x)), fmaxf(fabsf(q.x.y), fabsf(q.y.x))), fabsf(q.y.y));
+}
+// The same over finite values only.
+__device__ __forceinline__ float max4_finite(float m, const Quad& q) {
+  const float v[4] = {fabsf(q.x.x), fabsf(q.x.y), fabsf(q.y.x), fabsf(q.y.y)};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (v[i] < INFINITY) m = fmaxf(m, v[i]);
+  return m;
+}
+
+__device__ __forceinline__ uint32_t codes4(const Quad& q, float inv) {
+  const float2 s = make_float2(inv, inv);
+  const float2 x = mul2(q.x, s), y = mul2(q.y, s);
+  return e4m3x2(x.x, x.y) | e4m3x2(y.x, y.y) << 16;
+}
+
+// Packed 16-bit maximum of magnitudes (a NaN is passed over).
+__device__ __forceinline__ uint32_t max_abs2(uint32_t m, uint32_t v, __half) {
+  const __half2 r = __hmax2(*reinterpret_cast<__half2*>(&m),
+                            __habs2(*reinterpret_cast<__half2*>(&v)));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t max_abs2(uint32_t m, uint32_t v, __nv_bfloat16) {
+  const __nv_bfloat162 r = __hmax2(*reinterpret_cast<__nv_bfloat162*>(&m),
+                                   __habs2(*reinterpret_cast<__nv_bfloat162*>(&v)));
+  return *reinterpret_cast<const uint32_t*>(&r);
 }
 
 // Biased exponent of the smallest power of two s with amax <= 448 s (448 is
@@ -63,7 +102,7 @@ struct AppendArgs {
   const int64_t* pos;   // null when nothing is rotated
   const float* cache;
   int rows, hq, hkv, rot, max_positions;
-  int64_t cache_slots;
+  int64_t cache_slots;  // below 2^31
   int kv_blocks;        // blocks of the kv part; the rest rotate queries
   unsigned int* err;
 };
@@ -71,42 +110,223 @@ struct AppendArgs {
 // ---------------------------------------------------------------------------
 // Append. Work of the kv part: a RUN, the adjacent rows whose slots lie in one
 // scale block in increasing order (rows that are skipped do not end it), for
-// one KV head of K or of V, is one warp's: it holds the (rotated) values in
-// fp32 registers, takes their largest finite magnitude, joins it with the
-// block's old exponent when earlier tokens are kept, and writes the codes;
-// when the scale grows, the kept tokens' codes are rounded to the new one. So
-// every (block, head) has one writer per call and nothing is atomic.
+// one KV head, is one warp's: it takes the largest finite magnitude of the
+// (rotated) values of K, and of V, joins each with the block's old exponent
+// when earlier tokens are kept, and writes the codes; when a scale grows, the
+// kept tokens' codes are rounded to the new one. So every (block, head) has
+// one writer per call and nothing is atomic.
 //
 // A warp looks at a window of W rows for run starts (W = 1: a decode step
-// gives each row its own warp; W = 16: a prompt's rows, whose runs are mostly
-// whole blocks, are covered by one warp per 16 rows instead of 16 warps of
-// which 15 find nothing). The 32 lanes read the slots of rows w - 1 .. w + 30:
-// the row before the window, the window, and what its last run can reach;
-// only among skipped rows does a run need more (the two loops over rows).
+// gives each row its own warps; W = 16: a prompt's rows, whose runs are mostly
+// whole blocks, are covered by one warp per 16 rows and head instead of 16
+// warps of which 15 find nothing). The 32 lanes read the slots of rows w - 1
+// .. w + 30: the row before the window, the window, and what its last run can
+// reach; only among skipped rows does a run need more (the two loops over
+// rows). All of a run's K and V rows (8 KiB at head_dim 128) are in flight to
+// shared memory before the first is used.
 //
 // The query part rotates q into q_out, a thread per (row, kQHeads heads, 4 + 4
 // dims): the heads share the row's cos / sin.
 // Both parts are bound by memory traffic on prompts and by a chain of three
 // loads (slot and position, row and cos / sin, store) on decode steps.
 // ---------------------------------------------------------------------------
+
+// The m-th row of a run: rows are adjacent and slots consecutive (dense), or
+// lane m holds its row, its token of the block and its position.
+struct Run {
+  bool dense;
+  int row0, len, kept, blk;
+  int row_m, off_m, pos_m;
+};
+
+// A warp's staged rows of one head, [16][D]. Rows wait in shared memory and
+// not in registers: the loops over them stay loops, and 24 warps an SM fit.
+template <int D>
+struct Stage {
+  static constexpr int kBytes = kKv8Block * D * 2;
+  static constexpr int kUnits = D / 8;     // a unit is 4 + 4 dims of a row
+  static constexpr int kRows = 256 / D;    // rows per pass of a warp
+};
+
+template <int D>
+__device__ __forceinline__ void stage_rows(uint8_t* to, const void* from, int hkv, int h,
+                                           const Run& run, int lane) {
+  using S = Stage<D>;
+  const int sub = lane / S::kUnits, c = lane % S::kUnits;  // 16 bytes of a row
+  const uint8_t* base = static_cast<const uint8_t*>(from) + (int64_t(h) * D + 8 * c) * 2;
+  for (int i = 0; i < run.len; i += S::kRows) {
+    const int t = i + sub;
+    const int row = run.dense ? run.row0 + t : __shfl_sync(0xffffffffu, run.row_m, t & 31);
+    if (t < run.len)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                       smem_u32(to + t * (D * 2) + 16 * c)),
+                   "l"(base + int64_t(row) * hkv * (D * 2))
+                   : "memory");
+  }
+}
+
+// Quantise the staged rows into block run.blk of one head. kRot: `rot` dims
+// are rotated (the lanes that `turn`). kFull: a whole block of adjacent rows,
+// as most of a prompt's are, without the checks of the others (a third of the
+// instructions, which are what bounds the kv part). Values are formed twice,
+// for the maximum and for the codes.
+template <typename T, int D, bool kRot, bool kFull>
+__device__ __forceinline__ void quantise_rows(const uint8_t* stage, const Run& run,
+                                              const float* cache, int rot, int e0, int e1,
+                                              bool turn, uint8_t* codes, uint8_t* exps, int old,
+                                              int hkv, int h, int lane) {
+  using S = Stage<D>;
+  constexpr int kRows = S::kRows, kStep = kFull ? 4 : 1;
+  const int sub = lane / S::kUnits, u = lane % S::kUnits;
+  const int len = kFull ? kKv8Block : run.len;
+  const uint8_t* from = stage + sub * (D * 2);
+  auto raw = [&](int i, uint2& lo, uint2& hi) {
+    lo = *reinterpret_cast<const uint2*>(from + i * (D * 2) + 2 * e0);
+    hi = *reinterpret_cast<const uint2*>(from + i * (D * 2) + 2 * e1);
+  };
+  auto values = [&](int i, Quad& a, Quad& b) {
+    uint2 lo, hi;
+    raw(i, lo, hi);
+    a = unpack4<T>(lo);
+    b = unpack4<T>(hi);
+    if (kRot) {
+      const int p = __shfl_sync(0xffffffffu, run.pos_m, (i + sub) & 31);
+      if (turn && (kFull || i + sub < len)) {
+        const float* at = cache + int64_t(p) * rot + e0;
+        rotate4(a, b, at, at + rot / 2);
+      }
+    }
+  };
+  float amax = 0.f;
+  if (kRot) {
+#pragma unroll kStep
+    for (int i = 0; i < len; i += kRows) {
+      Quad a, b;
+      values(i, a, b);
+      if (kFull || i + sub < len) amax = max4(max4(amax, a), b);
+    }
+  } else {
+    uint32_t m = 0;
+#pragma unroll kStep
+    for (int i = 0; i < len; i += kRows) {
+      uint2 lo, hi;
+      raw(i, lo, hi);
+      if (kFull || i + sub < len)
+        m = max_abs2(max_abs2(max_abs2(max_abs2(m, lo.x, T()), lo.y, T()), hi.x, T()), hi.y, T());
+    }
+    const float2 f = unpack2<T>(m);
+    amax = fmaxf(f.x, f.y);
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  if (amax == INFINITY) {  // infinities saturate: once more without them
+    amax = 0.f;
+#pragma unroll 1
+    for (int i = 0; i < len; i += kRows) {
+      Quad a, b;
+      values(i, a, b);
+      if (i + sub < len) amax = max4_finite(max4_finite(amax, a), b);
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  }
+  int e = needed_exp(amax);
+  if (run.kept) e = min(max(e, old), kKv8MaxExp);
+  const float inv = exp_scale(254 - e);
+  const int64_t tok = int64_t(hkv) * D;  // bytes from one token to the next
+  uint8_t* block = codes + int64_t(run.blk) * kKv8Block * tok + h * D;
+  if (kFull) {
+    uint8_t* dst = block + sub * tok;
+#pragma unroll kStep
+    for (int i = 0; i < len; i += kRows, dst += kRows * tok) {
+      Quad a, b;
+      values(i, a, b);
+      *reinterpret_cast<uint32_t*>(dst + e0) = codes4(a, inv);
+      *reinterpret_cast<uint32_t*>(dst + e1) = codes4(b, inv);
+    }
+  } else {
+#pragma unroll 1
+    for (int i = 0; i < len; i += kRows) {
+      const int t = i + sub;
+      const int off = run.dense ? run.kept + t : __shfl_sync(0xffffffffu, run.off_m, t & 31);
+      Quad a, b;
+      values(i, a, b);
+      if (t < len) {
+        uint8_t* dst = block + off * tok;
+        *reinterpret_cast<uint32_t*>(dst + e0) = codes4(a, inv);
+        *reinterpret_cast<uint32_t*>(dst + e1) = codes4(b, inv);
+      }
+    }
+  }
+  if (run.kept && e > old) {
+    // the kept tokens move to the larger scale: 8 codes per lane and pass
+    const float down = exp_scale(max(old - e + 127, 1));
+    for (int t = sub; t < run.kept; t += kRows) {
+      uint2* w = reinterpret_cast<uint2*>(block + t * tok) + u;
+      uint2 c = *w;
+      uint32_t* cw = &c.x;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float2 a = unpack2<__half>(e4m3x2_to_h2(cw[j]));
+        const float2 b = unpack2<__half>(e4m3x2_hi_to_h2(cw[j]));
+        cw[j] = e4m3x2(a.x * down, a.y * down) | e4m3x2(b.x * down, b.y * down) << 16;
+      }
+      *w = c;
+    }
+  }
+  if (lane == 0 && (!run.kept || e != old))
+    exps[int64_t(run.blk) * hkv + h] = static_cast<uint8_t>(e);
+}
+
+template <typename T, int D, bool kFull>
+__device__ __forceinline__ void append_run(const AppendArgs& a, const Run& run, int h,
+                                           uint8_t* stage, int lane) {
+  using S = Stage<D>;
+  stage_rows<D>(stage, a.k, a.hkv, h, run, lane);
+  asm volatile("cp.async.commit_group;" ::: "memory");
+  stage_rows<D>(stage + S::kBytes, a.v, a.hkv, h, run, lane);
+  asm volatile("cp.async.commit_group;" ::: "memory");
+  const int rot_units = a.rot / 8;
+  const int u = lane % S::kUnits;
+  const bool turn = u < rot_units;
+  const int e0 = turn ? 4 * u : a.rot + 8 * (u - rot_units), e1 = e0 + (turn ? a.rot / 2 : 4);
+  int old_k = 0, old_v = 0;
+  if (run.kept) {
+    old_k = a.k_exp[int64_t(run.blk) * a.hkv + h];
+    old_v = a.v_exp[int64_t(run.blk) * a.hkv + h];
+  }
+  asm volatile("cp.async.wait_group 1;" ::: "memory");
+  __syncwarp();
+  if (a.pos)
+    quantise_rows<T, D, true, kFull>(stage, run, a.cache, a.rot, e0, e1, turn, a.k_codes, a.k_exp,
+                                     old_k, a.hkv, h, lane);
+  else
+    quantise_rows<T, D, false, kFull>(stage, run, nullptr, 0, e0, e1, false, a.k_codes, a.k_exp,
+                                      old_k, a.hkv, h, lane);
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  __syncwarp();
+  quantise_rows<T, D, false, kFull>(stage + S::kBytes, run, nullptr, 0, e0, e1, false, a.v_codes,
+                                    a.v_exp, old_v, a.hkv, h, lane);
+  __syncwarp();  // the stage may be refilled
+}
+
 template <typename T, int D, int W>
-__global__ void __launch_bounds__(kThreads, D == 128 ? 3 : 2) kv8_append_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(kThreads, D == 128 ? 3 : 1) kv8_append_kernel(const AppendArgs a) {
+  extern __shared__ __align__(16) uint8_t smem[];
   pdl_trigger();
   pdl_wait();  // q, k, v come from, and the pools are read by, earlier kernels
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int r = a.rot / 2;
-  const int rot_units = a.rot / 8;
   constexpr int kUnits = D / 8;  // a unit is 4 + 4 dims of a head
   if (static_cast<int>(blockIdx.x) >= a.kv_blocks) {
     // ------------------------------------------------------------- queries
-    const int groups = (a.hq + kQHeads - 1) / kQHeads;
-    const int64_t per_row = int64_t(groups) * kUnits;
-    const int64_t total = a.rows * per_row;
-    const int64_t step = int64_t(gridDim.x - a.kv_blocks) * kThreads;
-    for (int64_t i = int64_t(blockIdx.x - a.kv_blocks) * kThreads + threadIdx.x; i < total;
-         i += step) {
+    const int r = a.rot / 2, rot_units = a.rot / 8;
+    const int per_row = (a.hq + kQHeads - 1) / kQHeads * kUnits;
+    const int64_t total = int64_t(a.rows) * per_row;
+    const int64_t i =
+        int64_t(blockIdx.x - a.kv_blocks) * kThreads + threadIdx.x;
+    if (i < total) {
       const int row = static_cast<int>(i / per_row);
-      const int rem = static_cast<int>(i - row * per_row);
+      const int rem = static_cast<int>(i - int64_t(row) * per_row);
       const int u = rem % kUnits, h0 = rem / kUnits * kQHeads;
       const bool turn = u < rot_units;
       const int e0 = turn ? 4 * u : a.rot + 8 * (u - rot_units), e1 = turn ? e0 + r : e0 + 4;
@@ -120,29 +340,23 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? 3 : 2) kv8_append_kernel(
           lo[h] = *reinterpret_cast<const uint2*>(src + h * D + e0);
           hi[h] = *reinterpret_cast<const uint2*>(src + h * D + e1);
         }
-      float cs[4], sn[4];
+      const float* cs = nullptr;
       if (a.pos) {
         const int64_t p = a.pos[row];
         if (p < 0 || p >= a.max_positions) {
           if (rem == 0) raise_device_error(a.err, FE_DEVERR_POS_RANGE);
-          continue;
+          return;
         }
-        if (turn) {
-          const float* at = a.cache + p * a.rot + e0;
-          *reinterpret_cast<float4*>(cs) = *reinterpret_cast<const float4*>(at);
-          *reinterpret_cast<float4*>(sn) = *reinterpret_cast<const float4*>(at + r);
-        }
+        if (turn) cs = a.cache + p * a.rot + e0;
       }
 #pragma unroll
       for (int h = 0; h < kQHeads; ++h)
         if (h0 + h < a.hq) {
-          if (turn && a.pos) {
-            float x[4], y[4];
-            unpack4<T>(x, lo[h]);
-            unpack4<T>(y, hi[h]);
-            rotate4(x, y, cs, sn);
-            lo[h] = make_uint2(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]));
-            hi[h] = make_uint2(pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3]));
+          if (cs) {
+            Quad x = unpack4<T>(lo[h]), y = unpack4<T>(hi[h]);
+            rotate4(x, y, cs, cs + r);
+            lo[h] = make_uint2(pack2<T>(x.x.x, x.x.y), pack2<T>(x.y.x, x.y.y));
+            hi[h] = make_uint2(pack2<T>(y.x.x, y.x.y), pack2<T>(y.y.x, y.y.y));
           }
           *reinterpret_cast<uint2*>(dst + h * D + e0) = lo[h];
           *reinterpret_cast<uint2*>(dst + h * D + e1) = hi[h];
@@ -151,48 +365,44 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? 3 : 2) kv8_append_kernel(
     return;
   }
   // -------------------------------------------------------------- keys, values
-  const int64_t job = int64_t(blockIdx.x) * kWarps + warp;
-  const int jobs_per_window = 2 * a.hkv;
-  const int64_t window = job / jobs_per_window;
-  const int which = static_cast<int>(job - window * jobs_per_window);
-  const int64_t w0 = window * W;
-  if (w0 >= a.rows) return;
-  const bool is_v = which >= a.hkv;
-  const int h = is_v ? which - a.hkv : which;
-  uint8_t* codes = is_v ? a.v_codes : a.k_codes;
-  uint8_t* exps = is_v ? a.v_exp : a.k_exp;
-  const T* src = static_cast<const T*>(is_v ? a.v : a.k);
-  const bool turning = !is_v && a.pos != nullptr;
+  // `lanes_h` warps share a window's heads; a block has 8 / lanes_h windows
+  const int lanes_h = min(a.hkv, kWarps), windows = kWarps / lanes_h;
+  if (warp >= windows * lanes_h) return;
+  const int64_t w0l = (int64_t(blockIdx.x) * windows + warp / lanes_h) * W;
+  if (w0l >= a.rows) return;
+  const int w0 = static_cast<int>(w0l);
+  const int h0 = warp % lanes_h;
 
   // slot of a row, or -1 where it is skipped
-  auto slot_of = [&](int64_t row, int64_t& p, unsigned& bad) -> int64_t {
+  auto slot_of = [&](int row, int& p, unsigned& bad) -> int {
     const int64_t s = a.slots[row];
     if (s < 0) return -1;
     if (s >= a.cache_slots) bad |= FE_DEVERR_SLOT_RANGE;
     if (a.pos) {
-      p = a.pos[row];
-      if (p < 0 || p >= a.max_positions) bad |= FE_DEVERR_POS_RANGE;
+      const int64_t q = a.pos[row];
+      if (q < 0 || q >= a.max_positions) bad |= FE_DEVERR_POS_RANGE;
+      p = static_cast<int>(q);
     }
-    return bad ? -1 : s;
+    return bad ? -1 : static_cast<int>(s);
   };
-  const int64_t my = w0 - 1 + lane;  // this lane's row
-  int64_t slot = -1, p = 0;
+  const int my = w0 - 1 + lane;  // this lane's row
+  int slot = -1, p = 0;
   unsigned bad = 0;
   if (my >= 0 && my < a.rows) slot = slot_of(my, p, bad);
-  if (which == 0 && bad && lane >= 1 && lane <= W) raise_device_error(a.err, bad);
+  if (h0 == 0 && bad && lane >= 1 && lane <= W) raise_device_error(a.err, bad);
   const unsigned good = __ballot_sync(0xffffffffu, slot >= 0);
   const unsigned below = good & ((1u << lane) - 1u);
-  int64_t prev = __shfl_sync(0xffffffffu, slot, below ? 31 - __clz(below) : 0);
+  int prev = __shfl_sync(0xffffffffu, slot, below ? 31 - __clz(below) : 0);
   if (!below) prev = -1;
   const int lowest = __ffs(good) - 1;
   if (lowest >= 1 && lowest <= W)  // the row before is skipped: look further back
-    for (int64_t c = w0 - 2; c >= 0; c -= 32) {
+    for (int c = w0 - 2; c >= 0; c -= 32) {
       unsigned bits = 0;
-      int64_t q = 0;
-      const int64_t s = c >= lane ? slot_of(c - lane, q, bits) : -1;
+      int q = 0;
+      const int s = c >= lane ? slot_of(c - lane, q, bits) : -1;
       const unsigned any = __ballot_sync(0xffffffffu, s >= 0);
       if (any) {
-        const int64_t near = __shfl_sync(0xffffffffu, s, __ffs(any) - 1);
+        const int near = __shfl_sync(0xffffffffu, s, __ffs(any) - 1);
         if (lane == lowest) prev = near;
         break;
       }
@@ -202,130 +412,54 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? 3 : 2) kv8_append_kernel(
   const unsigned heads = __ballot_sync(0xffffffffu, slot >= 0 && !joins);
   unsigned starts = heads & static_cast<unsigned>(((uint64_t(1) << W) - 1) << 1);
 
-  constexpr int kRows = 256 / D;               // rows per pass of the warp
-  constexpr int kPasses = kKv8Block / kRows;
-  const int sub = lane / kUnits, u = lane % kUnits;
-  const bool turn = u < rot_units;
-  const int e0 = turn ? 4 * u : a.rot + 8 * (u - rot_units), e1 = turn ? e0 + r : e0 + 4;
   while (starts) {
     const int b = __ffs(starts) - 1;
     starts &= starts - 1;
-    // the run's rows: lane m < len has row and slot of the m-th
+    // the run's rows: lane m < len has row, slot and position of the m-th
     const unsigned next = heads & ~((2u << b) - 1u);
     unsigned members = good & ~((1u << b) - 1u);
     if (next) members &= (1u << (__ffs(next) - 1)) - 1u;
-    int len = __popc(members);
-    const bool dense = (members >> b) == (len == 32 ? ~0u : (1u << len) - 1u);
-    const int at = dense ? (b + lane) & 31 : static_cast<int>(__fns(members, 0, lane + 1)) & 31;
-    int64_t row_m = w0 - 1 + at, slot_m = __shfl_sync(0xffffffffu, slot, at),
-            pos_m = __shfl_sync(0xffffffffu, p, at);
-    int64_t last = __shfl_sync(0xffffffffu, slot_m, len - 1);
-    if (!next) {  // skipped rows may have pushed the run past the lanes
-      bool more = true;
-      for (int64_t c = w0 + 31; more && c < a.rows && last % kKv8Block != kKv8Block - 1; c += 32) {
-        unsigned bits = 0;
-        int64_t q = 0;
-        const int64_t s = c + lane < a.rows ? slot_of(c + lane, q, bits) : -1;
-        for (unsigned g = __ballot_sync(0xffffffffu, s >= 0); g && more; g &= g - 1) {
-          const int l = __ffs(g) - 1;
-          const int64_t sl = __shfl_sync(0xffffffffu, s, l), ql = __shfl_sync(0xffffffffu, q, l);
-          more = sl / kKv8Block == last / kKv8Block && sl > last;
-          if (!more) break;
-          if (lane == len) {
-            row_m = c + l;
-            slot_m = sl;
-            pos_m = ql;
-          }
-          ++len;
-          last = sl;
+    Run run;
+    run.len = __popc(members);
+    const bool adjacent = (members >> b) == (1u << run.len) - 1u;  // b >= 1: len < 32
+    const int at = adjacent ? (b + lane) & 31 : static_cast<int>(__fns(members, 0, lane + 1)) & 31;
+    run.row0 = w0 - 1 + b;
+    run.row_m = w0 - 1 + at;
+    int slot_m = __shfl_sync(0xffffffffu, slot, at);
+    run.pos_m = __shfl_sync(0xffffffffu, p, at);
+    int last = __shfl_sync(0xffffffffu, slot_m, run.len - 1);
+    bool more = !next;  // skipped rows may have pushed the run past the lanes
+    for (int c = w0 + 31; more && c < a.rows && last % kKv8Block != kKv8Block - 1; c += 32) {
+      unsigned bits = 0;
+      int q = 0;
+      const int s = c + lane < a.rows ? slot_of(c + lane, q, bits) : -1;
+      for (unsigned g = __ballot_sync(0xffffffffu, s >= 0); g; g &= g - 1) {
+        const int l = __ffs(g) - 1;
+        const int sl = __shfl_sync(0xffffffffu, s, l), ql = __shfl_sync(0xffffffffu, q, l);
+        more = sl / kKv8Block == last / kKv8Block && sl > last;
+        if (!more) break;
+        if (lane == run.len) {
+          run.row_m = c + l;
+          slot_m = sl;
+          run.pos_m = ql;
         }
+        ++run.len;
+        last = sl;
       }
     }
-    const int64_t blk = last / kKv8Block;
-    const int off_m = static_cast<int>(slot_m % kKv8Block);
-    const int kept = __shfl_sync(0xffffffffu, off_m, 0);
-    const int old = kept ? exps[blk * a.hkv + h] : 0;
-    // all rows of the run in flight, then the rotation and the maximum
-    uint2 lo[kPasses], hi[kPasses];
-#pragma unroll
-    for (int i = 0; i < kPasses; ++i) {
-      const int t = i * kRows + sub;
-      const int64_t rt = __shfl_sync(0xffffffffu, row_m, t & 31);
-      if (t < len) {
-        const T* row = src + (rt * a.hkv + h) * D;
-        lo[i] = *reinterpret_cast<const uint2*>(row + e0);
-        hi[i] = *reinterpret_cast<const uint2*>(row + e1);
-      }
+    run.blk = last / kKv8Block;
+    run.off_m = slot_m % kKv8Block;
+    run.kept = __shfl_sync(0xffffffffu, run.off_m, 0);
+    const int last_row = __shfl_sync(0xffffffffu, run.row_m, run.len - 1);
+    run.dense = last_row - run.row0 == run.len - 1 &&
+                last % kKv8Block - run.kept == run.len - 1;
+    uint8_t* stage = smem + warp * 2 * Stage<D>::kBytes;
+    for (int h = h0; h < a.hkv; h += lanes_h) {
+      if (W > 1 && run.dense && run.len == kKv8Block)
+        append_run<T, D, true>(a, run, h, stage, lane);
+      else
+        append_run<T, D, false>(a, run, h, stage, lane);
     }
-    // (the second time for the codes: rotating again costs less than keeping
-    // the fp32 values, 64 registers a lane, would in warps per SM)
-    auto turned = [&](int i, float (&x)[8]) {
-      const int64_t pt = __shfl_sync(0xffffffffu, pos_m, (i * kRows + sub) & 31);
-      if (i * kRows + sub < len) {
-        unpack4<T>(x, lo[i]);
-        unpack4<T>(x + 4, hi[i]);
-        if (turning && turn) {
-          const float* at = a.cache + pt * a.rot + e0;
-          float cs[4], sn[4];
-          *reinterpret_cast<float4*>(cs) = *reinterpret_cast<const float4*>(at);
-          *reinterpret_cast<float4*>(sn) = *reinterpret_cast<const float4*>(at + r);
-          rotate4(x, x + 4, cs, sn);
-        }
-      }
-    };
-    float amax = 0.f;
-#pragma unroll
-    for (int i = 0; i < kPasses; ++i) {
-      if (i * kRows >= len) break;
-      float x[8];
-      turned(i, x);
-      if (i * kRows + sub < len) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float m = fabsf(x[e]);
-          if (m < INFINITY) amax = fmaxf(amax, m);  // infinities saturate, NaN stays
-        }
-      }
-    }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    int e = needed_exp(amax);
-    if (kept) e = min(max(e, old), kKv8MaxExp);
-    const float inv = exp_scale(254 - e);
-    uint8_t* block = codes + (blk * kKv8Block * a.hkv + h) * D;
-    const int64_t tok = int64_t(a.hkv) * D;  // bytes from one token to the next
-#pragma unroll
-    for (int i = 0; i < kPasses; ++i) {
-      if (i * kRows >= len) break;
-      const int t = i * kRows + sub;
-      const int off = __shfl_sync(0xffffffffu, off_m, t & 31);
-      float x[8];
-      turned(i, x);
-      if (t < len) {
-        uint8_t* dst = block + off * tok;
-        const uint32_t c0 = e4m3x2(x[0] * inv, x[1] * inv) | e4m3x2(x[2] * inv, x[3] * inv) << 16;
-        const uint32_t c1 = e4m3x2(x[4] * inv, x[5] * inv) | e4m3x2(x[6] * inv, x[7] * inv) << 16;
-        *reinterpret_cast<uint32_t*>(dst + e0) = c0;
-        *reinterpret_cast<uint32_t*>(dst + e1) = c1;
-      }
-    }
-    if (kept && e > old) {
-      // the kept tokens move to the larger scale: 8 codes per lane and pass
-      const float down = exp_scale(max(old - e + 127, 1));
-      for (int t = sub; t < kept; t += kRows) {
-        uint2* w = reinterpret_cast<uint2*>(block + t * tok) + u;
-        uint2 c = *w;
-        uint32_t* cw = &c.x;
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const uint32_t l = e4m3x2_to_h2(cw[j]), g = e4m3x2_hi_to_h2(cw[j]);
-          const float2 fl = unpack2<__half>(l), fg = unpack2<__half>(g);
-          cw[j] = e4m3x2(fl.x * down, fl.y * down) | e4m3x2(fg.x * down, fg.y * down) << 16;
-        }
-        *w = c;
-      }
-    }
-    if (lane == 0 && (!kept || e != old)) exps[blk * a.hkv + h] = static_cast<uint8_t>(e);
   }
 }
 
@@ -446,20 +580,28 @@ __global__ void __launch_bounds__(kThreads)
 
 template <typename T, int D>
 int launch_append(AppendArgs& a, cudaStream_t stream) {
-  // One warp per row and head up to 64 Ki of them, a warp per 16 rows beyond (prompts).
-  const bool wide = int64_t(a.rows) * 2 * a.hkv > 65536;
+  // A warp per row and head up to 64 Ki of them, a warp per 16 rows beyond.
+  const bool wide = int64_t(a.rows) * a.hkv > 32768;
   const int64_t windows = wide ? (int64_t(a.rows) + 15) / 16 : a.rows;
-  const int64_t kvb = (windows * 2 * a.hkv + kWarps - 1) / kWarps;
-  int64_t qb = (int64_t(a.rows) * ((a.hq + kQHeads - 1) / kQHeads) * (D / 8) + kThreads - 1) /
+  const int per_block = a.hkv < kWarps ? kWarps / a.hkv : 1;
+  const int64_t kvb = (windows + per_block - 1) / per_block;
+  const int64_t qb = (int64_t(a.rows) * ((a.hq + kQHeads - 1) / kQHeads) * (D / 8) + kThreads - 1) /
                kThreads;
-  if (qb > 148 * 64) qb = 148 * 64;
   if (kvb > INT32_MAX - qb) return fail(FE_ERR_CAPACITY, "fe_kv8_append: too many rows");
   a.kv_blocks = static_cast<int>(kvb);
   const dim3 grid(static_cast<unsigned>(kvb + qb));
-  if (wide)
-    FE_CUDA_TRY(launch_pdl(kv8_append_kernel<T, D, 16>, grid, dim3(kThreads), 0, stream, a));
-  else
-    FE_CUDA_TRY(launch_pdl(kv8_append_kernel<T, D, 1>, grid, dim3(kThreads), 0, stream, a));
+  constexpr int kSmem = kWarps * 2 * Stage<D>::kBytes;
+  static std::once_flag once;
+  static cudaError_t attr_err = cudaSuccess;
+  std::call_once(once, [] {
+    for (auto kernel : {kv8_append_kernel<T, D, 16>, kv8_append_kernel<T, D, 1>})
+      if (attr_err == cudaSuccess)
+        attr_err =
+            cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  });
+  if (attr_err != cudaSuccess) return cuda_fail(attr_err, "kv8_append_kernel attribute");
+  FE_CUDA_TRY(launch_pdl(wide ? kv8_append_kernel<T, D, 16> : kv8_append_kernel<T, D, 1>, grid,
+                         dim3(kThreads), kSmem, stream, a));
   return FE_OK;
 }
 
@@ -488,14 +630,16 @@ int fe_kv8_append(const void* q, void* q_out, const void* k, const void* v, uint
                 "fe_kv8_append: rotary_dim must be a multiple of 8, at most head_dim");
   if (rotary_dim > 0 && max_positions <= 0)
     return fail(FE_ERR_INVALID_ARGUMENT, "fe_kv8_append: max_positions <= 0");
+  if (cache_slots > INT32_MAX)
+    return fail(FE_ERR_CAPACITY, "fe_kv8_append: cache_slots above 2^31");
   if (rows == 0) return FE_OK;
   if (!k || !v || !k_codes || !v_codes || !k_exp || !v_exp || !slots ||
       (hq > 0 && (!q || !q_out)) || (rotary_dim > 0 && (!pos || !cache)))
     return fail(FE_ERR_INVALID_ARGUMENT, "fe_kv8_append: null pointer");
-  if (!aligned8(k) || !aligned8(v) || !aligned8(q) || !aligned8(q_out) || !aligned8(k_codes) ||
+  if (!aligned16(k) || !aligned16(v) || !aligned8(q) || !aligned8(q_out) || !aligned8(k_codes) ||
       !aligned8(v_codes) || !aligned16(cache))
     return fail(FE_ERR_INVALID_ARGUMENT,
-                "fe_kv8_append: q, k, v and codes must be 8-byte, the cache 16-byte aligned");
+                "fe_kv8_append: k, v and the cache must be 16-byte, q and codes 8-byte aligned");
   AppendArgs a{q, q_out, k, v, k_codes, v_codes, k_exp, v_exp, slots,
                rotary_dim > 0 ? pos : nullptr, cache, rows, hq, hkv, rotary_dim, max_positions,
                cache_slots, 0, device_error_word()};

@@ -273,11 +273,11 @@ __global__ void __launch_bounds__(kPlanThreads, 1) plan_device_kernel(const DevP
     const int64_t T = scan_range(
         B, [&](int b) -> int64_t { return int64_t(n_dec(b)) * cdiv(seq_len(b), kTileTokens); },
         [&](int b, int64_t ex) { p_tiles[b] = ex; }, wsum);
-    // decode cut: ncta CTAs of `per` tiles (at least 8 tiles per CTA), as
+    // decode cut: ncta CTAs of `per` tiles (at least dec_min_tiles tiles per CTA), as
     // build_cut_view
     int64_t per = 1, ncta = 0;
     if (T > 0) {
-      ncta = T / 8 < 1 ? 1 : T / 8;
+      ncta = T / a.dec_min_tiles < 1 ? 1 : T / a.dec_min_tiles;
       if (ncta > a.dec_grid_cap) ncta = a.dec_grid_cap;
       per = cdiv(T, ncta);
       ncta = cdiv(T, per);

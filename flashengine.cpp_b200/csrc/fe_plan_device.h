@@ -27,7 +27,7 @@ struct DevPlanArgs {
   int batch, rows;
   // plan configuration and capacities
   int hq, hkv, dim, page, max_batch, max_pages, num_blocks, dec_heads, grid_cap, dec_grid_cap;
-  int max_items, max_groups;
+  int max_items, max_groups, dec_min_tiles;
   int64_t partial_capacity, meta_cap;
   // outputs: the packed work lists (fe_attn_plan.h layout), split counters
   uint8_t* meta;

@@ -9,6 +9,7 @@ a failing call raises (the reference throws std::runtime_error).
 """
 from __future__ import annotations
 
+import array
 import ctypes
 
 import numpy as np
@@ -55,7 +56,7 @@ def _host_i32(a) -> np.ndarray:
 
 def _require_device_i32(t):
     torch = _torch()
-    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype == torch.int32 and
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype is torch.int32 and
             t.is_contiguous()):
         raise ValueError("expected a contiguous int32 CUDA tensor")
 
@@ -318,9 +319,10 @@ class Kv8Pool:
     float8_e4m3fn and `exps` uint8 [cache_slots / 16, hkv], the biased
     exponents of the scales of 16 slots (value = code * 2 ** (exp - 127)).
     Both contiguous CUDA tensors on one device; they may be slices of larger
-    tensors that hold all layers."""
+    tensors that hold all layers. A pool is made once and keeps its tensors,
+    so what a call needs of them (shape, addresses) is read here."""
 
-    __slots__ = ("codes", "exps")
+    __slots__ = ("codes", "exps", "shape", "device", "codes_ptr", "exps_ptr")
 
     def __init__(self, codes, exps):
         torch = _torch()
@@ -336,6 +338,8 @@ class Kv8Pool:
         if exps.device != codes.device:
             raise ValueError("codes and exps are on different devices")
         self.codes, self.exps = codes, exps
+        self.shape, self.device = tuple(codes.shape), codes.device
+        self.codes_ptr, self.exps_ptr = codes.data_ptr(), exps.data_ptr()
 
     @classmethod
     def empty(cls, num_blocks, page, hkv, dim, device="cuda"):
@@ -348,22 +352,27 @@ class Kv8Pool:
 
     @property
     def cache_slots(self):
-        return int(self.codes.shape[0])
+        return self.shape[0]
 
 
-def _kv8_pair(kpool, vpool):
-    if kpool.codes.shape != vpool.codes.shape:
-        raise ValueError("the K and V pools differ in shape")
+# These calls are short enough on the GPU that a decode step is bound by the
+# host; their checks read each tensor attribute once and pass plain integers.
+
+def _kv8_stream(stream):
+    if stream is None:
+        c = _torch()._C
+        return c._cuda_getCurrentRawStream(c._cuda_getDevice())
+    return stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
 
 
-def _kv8_rows(name, t, like, heads=None):
-    torch = _torch()
-    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.is_contiguous() and t.dim() == 3):
-        raise ValueError(f"{name}: expected a contiguous CUDA tensor [rows, heads, dim]")
-    if t.dtype != like.dtype or t.shape[0] != like.shape[0] or t.shape[2] != like.shape[2] or \
-            (heads is not None and t.shape[1] != heads):
-        raise ValueError(f"{name}: {t.dtype} {tuple(t.shape)} does not fit "
-                         f"{like.dtype} {tuple(like.shape)}")
+def _kv8_rows(name, t, dtype, shape):
+    """Address of a contiguous CUDA tensor of this dtype and shape."""
+    if t is None:
+        raise ValueError(f"{name} is missing")
+    if t.dtype is not dtype or t.shape != shape or not t.is_cuda or not t.is_contiguous():
+        raise ValueError(f"{name}: expected a contiguous {dtype} CUDA tensor {tuple(shape)}, got "
+                         f"{t.dtype} {tuple(t.shape)} {tuple(t.stride())} on {t.device}")
+    return t.data_ptr()
 
 
 def append_kv8(q, k, v, kpool, vpool, slots, pos=None, cache=None, q_out=None, stream=None):
@@ -372,58 +381,50 @@ def append_kv8(q, k, v, kpool, vpool, slots, pos=None, cache=None, q_out=None, s
     v quantised into `kpool` / `vpool` through `slots` (int64 [rows]). pos int64
     [rows] and cache fp32 [max_positions, rotary_dim] as in rope(); cache None
     rotates nothing. Rows of one 16-slot block must be adjacent and in order."""
-    lib = _lib.load()
     torch = _torch()
-    _kv8_pair(kpool, vpool)
-    _kv8_rows("k", k, k, int(kpool.codes.shape[1]))
-    _kv8_rows("v", v, k, int(k.shape[1]))
-    rows, hkv, dim = (int(x) for x in k.shape)
-    if dim != kpool.codes.shape[2]:
-        raise ValueError(f"k: head_dim {dim}, the pools have {int(kpool.codes.shape[2])}")
+    shape, dt = k.shape, k.dtype
+    if len(shape) != 3 or kpool.shape != vpool.shape or shape[1:] != kpool.shape[1:]:
+        raise ValueError(f"k {tuple(shape)} and pools {kpool.shape}, {vpool.shape} do not fit")
+    rows, hkv, dim = shape
+    kp, vp = _kv8_rows("k", k, dt, shape), _kv8_rows("v", v, dt, shape)
     hq = 0
+    qp = op = None
     if q is not None:
-        q_out = q if q_out is None else q_out
-        _kv8_rows("q", q, k)
-        _kv8_rows("q_out", q_out, q, int(q.shape[1]))
-        hq = int(q.shape[1])
-    index = [("slots", slots)] + ([("pos", pos)] if cache is not None else [])
-    for name, t in index:
-        if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype == torch.int64 and
-                t.is_contiguous() and t.numel() == rows):
-            raise ValueError(f"{name}: expected a contiguous int64 CUDA tensor of {rows}")
+        qs = q.shape
+        hq = qs[1] if len(qs) == 3 else -1
+        qp = _kv8_rows("q", q, dt, (rows, hq, dim))
+        op = qp if q_out is None else _kv8_rows("q_out", q_out, dt, (rows, hq, dim))
+    sp = _kv8_rows("slots", slots, torch.int64, (rows,))
     rot = most = 0
+    pp = cp = None
     if cache is not None:
-        if not (cache.is_cuda and cache.dtype == torch.float32 and cache.is_contiguous() and
-                cache.dim() == 2):
-            raise ValueError("cache: expected a contiguous fp32 CUDA tensor "
-                             "[max_positions, rotary_dim]")
-        most, rot = (int(x) for x in cache.shape)
-    check(lib.fe_kv8_append(_ptr(q) if hq else None, _ptr(q_out) if hq else None, _ptr(k), _ptr(v),
-                            _ptr(kpool.codes), _ptr(vpool.codes), _ptr(kpool.exps),
-                            _ptr(vpool.exps), _ptr(slots), _ptr(pos) if rot else None,
-                            _ptr(cache) if rot else None, rows, hq, hkv, dim, rot, most,
-                            dtype_code(k), kpool.cache_slots, _stream(stream)), "append_kv8")
+        most, rot = cache.shape
+        if rot:
+            pp = _kv8_rows("pos", pos, torch.int64, (rows,))
+            cp = _kv8_rows("cache", cache, torch.float32, (most, rot))
+    check(_lib.load().fe_kv8_append(qp, op, kp, vp, kpool.codes_ptr, vpool.codes_ptr,
+                                    kpool.exps_ptr, vpool.exps_ptr, sp, pp, cp, rows, hq, hkv, dim,
+                                    rot, most, dtype_code(k), kpool.shape[0],
+                                    _kv8_stream(stream)), "append_kv8")
 
 
 def gather_kv8(pool, out, kv, pages, last, row_offset, max_len, page, stream=None):
     """Whole sequences' values from an 8-bit pool into rows of `out` [rows,
     hkv, dim] (16-bit), metadata as gather(): int32 CUDA tensors."""
-    lib = _lib.load()
     for t in (kv, pages, last, row_offset):
         _require_device_i32(t)
-    hkv, dim = int(pool.codes.shape[1]), int(pool.codes.shape[2])
-    if not out.is_contiguous() or out.numel() % (hkv * dim):
-        raise ValueError("out: expected a contiguous tensor [rows, hkv, dim]")
-    check(lib.fe_kv8_gather(_ptr(pool.codes), _ptr(pool.exps), _ptr(out), _ptr(kv), _ptr(pages),
-                            _ptr(last), _ptr(row_offset), int(kv.shape[0]) - 1, int(max_len),
-                            int(page), hkv, dim, dtype_code(out), pool.cache_slots,
-                            _stream(stream)), "gather_kv8")
+    _, hkv, dim = pool.shape
+    if not out.is_contiguous() or not out.is_cuda or out.numel() % (hkv * dim):
+        raise ValueError("out: expected a contiguous CUDA tensor [rows, hkv, dim]")
+    check(_lib.load().fe_kv8_gather(pool.codes_ptr, pool.exps_ptr, out.data_ptr(), kv.data_ptr(),
+                                    pages.data_ptr(), last.data_ptr(), row_offset.data_ptr(),
+                                    kv.shape[0] - 1, max_len, page, hkv, dim, dtype_code(out),
+                                    pool.shape[0], _kv8_stream(stream)), "gather_kv8")
 
 
 def copy_blocks_kv8(k_pools, v_pools, src, dst, ntok, page, stream=None):
     """copy_blocks for 8-bit pools (lists of Kv8Pool, one per layer): codes
     and scales. src/dst/ntok: int32 CUDA tensors."""
-    lib = _lib.load()
     n = len(k_pools)
     if n != len(v_pools):
         raise ValueError("k_pools and v_pools differ in length")
@@ -431,16 +432,18 @@ def copy_blocks_kv8(k_pools, v_pools, src, dst, ntok, page, stream=None):
         _require_device_i32(t)
     if n == 0:
         return
-    shape = k_pools[0].codes.shape
-    for p in (*k_pools, *v_pools):
-        if p.codes.shape != shape:
-            raise ValueError("the layers' pools differ in shape")
-    arr = lambda ts: (_P * n)(*[t.data_ptr() for t in ts])  # noqa: E731
-    check(lib.fe_kv8_copy_blocks(arr([p.codes for p in k_pools]), arr([p.codes for p in v_pools]),
-                                 arr([p.exps for p in k_pools]), arr([p.exps for p in v_pools]), n,
-                                 _ptr(src), _ptr(dst), _ptr(ntok), int(src.shape[0]), int(page),
-                                 int(shape[1]), int(shape[2]), int(shape[0]) // int(page),
-                                 _stream(stream)), "copy_blocks_kv8")
+    shape = k_pools[0].shape
+    for side in (k_pools, v_pools):
+        for p in side:
+            if p.shape != shape:
+                raise ValueError("the layers' pools differ in shape")
+    arrays = [array.array("Q", ptrs) for ptrs in
+              ([p.codes_ptr for p in k_pools], [p.codes_ptr for p in v_pools],
+               [p.exps_ptr for p in k_pools], [p.exps_ptr for p in v_pools])]
+    check(_lib.load().fe_kv8_copy_blocks(*[a.buffer_info()[0] for a in arrays], n, src.data_ptr(),
+                                         dst.data_ptr(), ntok.data_ptr(), src.shape[0], page,
+                                         shape[1], shape[2], shape[0] // page,
+                                         _kv8_stream(stream)), "copy_blocks_kv8")
 
 
 class Kv8Plan(AttentionPlan):
@@ -449,21 +452,21 @@ class Kv8Plan(AttentionPlan):
 
     _create = "fe_kv8_plan_create"
 
-    def attention(self, q, kpool, vpool, out, causal=True, stream=None):
+    def __init__(self, hq, hkv, dim, page, max_batch, max_pages, bf16, blocks):
+        super().__init__(hq, hkv, dim, page, max_batch, max_pages, bf16, blocks)
         torch = _torch()
-        _kv8_pair(kpool, vpool)
-        want = ((int(self.blocks) + 1) * int(self.page), self.hkv, self.dim)
-        if tuple(kpool.codes.shape) != want:
-            raise ValueError(f"pools of shape {tuple(kpool.codes.shape)}, the plan is for {want}")
-        dt = torch.bfloat16 if self.bf16 else torch.float16
-        for name, t in (("q", q), ("out", out)):
-            if not (t.is_cuda and t.is_contiguous() and t.dtype == dt and
-                    tuple(t.shape[-2:]) == (self.hq, self.dim)):
-                raise ValueError(f"{name}: expected a contiguous {dt} CUDA tensor [rows, "
-                                 f"{self.hq}, {self.dim}]")
-        check(self.lib.fe_kv8_attn_run(self.handle, _ptr(q), _ptr(kpool.codes), _ptr(vpool.codes),
-                                       _ptr(kpool.exps), _ptr(vpool.exps), _ptr(out),
-                                       int(bool(causal)), _stream(stream)), "attention")
+        self.pool_shape = ((int(blocks) + 1) * int(page), int(hkv), int(dim))
+        self.dtype = torch.bfloat16 if bf16 else torch.float16
+
+    def attention(self, q, kpool, vpool, out, causal=True, stream=None):
+        if kpool.shape != self.pool_shape or vpool.shape != self.pool_shape:
+            raise ValueError(f"pools of shape {kpool.shape}, {vpool.shape}: the plan is for "
+                             f"{self.pool_shape}")
+        shape = (q.shape[0], self.hq, self.dim)
+        check(self.lib.fe_kv8_attn_run(self.handle, _kv8_rows("q", q, self.dtype, shape),
+                                       kpool.codes_ptr, vpool.codes_ptr, kpool.exps_ptr,
+                                       vpool.exps_ptr, _kv8_rows("out", out, self.dtype, shape),
+                                       1 if causal else 0, _kv8_stream(stream)), "attention")
 
 
 def create_plan(hq, hkv, dim, page, max_batch, max_pages, bf16, blocks) -> AttentionPlan:

@@ -301,8 +301,9 @@ int fe_paged_decode_noalloc(const void* q, const void* k_pool, const void* v_poo
  *          FE_DEVERR_SLOT_RANGE. pos: int64 [rows]; outside [0,
  *          max_positions): the row's k, v and q are skipped,
  *          FE_DEVERR_POS_RANGE.
- * dim 128 or 256; rotary_dim a multiple of 8; cache_slots a multiple of 16;
- * q, k, v and codes 8-byte aligned, the cos / sin cache 16-byte aligned. */
+ * dim 128 or 256; rotary_dim a multiple of 8; cache_slots a multiple of 16,
+ * below 2^31; k, v and the cos / sin cache 16-byte, q and codes 8-byte
+ * aligned. */
 int fe_kv8_append(const void* q, void* q_out, const void* k, const void* v, uint8_t* k_codes,
                   uint8_t* v_codes, uint8_t* k_exp, uint8_t* v_exp, const int64_t* slots,
                   const int64_t* pos, const float* cache, int rows, int hq, int hkv, int dim,
