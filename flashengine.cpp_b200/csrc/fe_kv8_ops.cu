@@ -470,7 +470,7 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? 3 : 1) kv8_append_kernel(
 constexpr int kGatherTok = 4;
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 4)
     kv8_gather_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ exps,
                       T* __restrict__ out, const int32_t* __restrict__ kv,
                       const int32_t* __restrict__ pages, const int32_t* __restrict__ last,
@@ -487,14 +487,17 @@ __global__ void __launch_bounds__(kThreads)
   const int chunks = hkv * dim / 16;
   const int step = gridDim.x * kWarps * kGatherTok;
   for (int t0 = (blockIdx.x * kWarps + (threadIdx.x >> 5)) * kGatherTok; t0 < len; t0 += step) {
-    int64_t slot[kGatherTok];
+    int slot[kGatherTok];  // below 2^31, -1: nothing to do
 #pragma unroll
     for (int i = 0; i < kGatherTok; ++i) {
       const int t = t0 + i;
-      slot[i] = t < len ? int64_t(__ldg(pages + p0 + t / page)) * page + t % page : -1;
-      if (t < len && (slot[i] < 0 || slot[i] >= cache_slots)) {
-        if (lane == 0) raise_device_error(err, FE_DEVERR_PAGE_RANGE);
-        slot[i] = -1;
+      slot[i] = -1;
+      if (t < len) {
+        const int64_t s = int64_t(__ldg(pages + p0 + t / page)) * page + t % page;
+        if (s >= 0 && s < cache_slots)
+          slot[i] = static_cast<int>(s);
+        else if (lane == 0)
+          raise_device_error(err, FE_DEVERR_PAGE_RANGE);
       }
     }
     for (int c = lane; c < chunks; c += 32) {
@@ -504,8 +507,8 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
       for (int i = 0; i < kGatherTok; ++i)
         if (slot[i] >= 0) {
-          v[i] = __ldg(reinterpret_cast<const uint4*>(codes) + slot[i] * chunks + c);
-          e[i] = __ldg(exps + slot[i] / kKv8Block * hkv + h);
+          v[i] = __ldg(reinterpret_cast<const uint4*>(codes) + int64_t(slot[i]) * chunks + c);
+          e[i] = __ldg(exps + int64_t(slot[i] / kKv8Block) * hkv + h);
         }
 #pragma unroll
       for (int i = 0; i < kGatherTok; ++i)
@@ -515,10 +518,11 @@ __global__ void __launch_bounds__(kThreads)
           uint32_t o[8];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const float2 lo = unpack2<__half>(e4m3x2_to_h2(w[j]));
-            const float2 hi = unpack2<__half>(e4m3x2_hi_to_h2(w[j]));
-            o[2 * j] = pack2<T>(lo.x * s, lo.y * s);
-            o[2 * j + 1] = pack2<T>(hi.x * s, hi.y * s);
+            const float2 s2 = make_float2(s, s);
+            const float2 lo = mul2(unpack2<__half>(e4m3x2_to_h2(w[j])), s2);
+            const float2 hi = mul2(unpack2<__half>(e4m3x2_hi_to_h2(w[j])), s2);
+            o[2 * j] = pack2<T>(lo.x, lo.y);
+            o[2 * j + 1] = pack2<T>(hi.x, hi.y);
           }
           uint4* dst = reinterpret_cast<uint4*>(out + (orow + t0 + i) * (int64_t(chunks) * 16)) +
                        2 * c;
@@ -580,8 +584,8 @@ __global__ void __launch_bounds__(kThreads)
 
 template <typename T, int D>
 int launch_append(AppendArgs& a, cudaStream_t stream) {
-  // A warp per row and head up to 64 Ki of them, a warp per 16 rows beyond.
-  const bool wide = int64_t(a.rows) * a.hkv > 32768;
+  // A warp per row and head up to 8 Ki of them, a warp per 16 rows beyond.
+  const bool wide = int64_t(a.rows) * a.hkv > 8192;
   const int64_t windows = wide ? (int64_t(a.rows) + 15) / 16 : a.rows;
   const int per_block = a.hkv < kWarps ? kWarps / a.hkv : 1;
   const int64_t kvb = (windows + per_block - 1) / per_block;
@@ -662,6 +666,8 @@ int fe_kv8_gather(const uint8_t* codes, const uint8_t* exps, void* out, const in
     return fail(FE_ERR_UNSUPPORTED, "fe_kv8_gather: head_dim must be a multiple of 16");
   if (batch == 0 || max_len == 0) return FE_OK;
   if (batch > 65535) return fail(FE_ERR_CAPACITY, "fe_kv8_gather: at most 65535 sequences");
+  if (cache_slots > INT32_MAX)
+    return fail(FE_ERR_CAPACITY, "fe_kv8_gather: cache_slots above 2^31");
   if (!codes || !exps || !out || !kv || !pages || !last || !row_offset)
     return fail(FE_ERR_INVALID_ARGUMENT, "fe_kv8_gather: null pointer");
   if (!aligned16(codes) || !aligned16(out))
