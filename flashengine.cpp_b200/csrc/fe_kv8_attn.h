@@ -1,6 +1,6 @@
 // Launch interface of the attention kernels over the 8-bit KV cache, shared by
 // the plan (fe_attn.cu) and the two kernels (fe_kv8_decode.cu, fe_kv8_rows.cu),
-// and the conversion of a query row to e4m3 parts, which both use.
+// and the row kernel's conversion of a query row to e4m3 parts.
 #pragma once
 
 #include "fe_attn_common.cuh"
@@ -28,18 +28,27 @@ __device__ __forceinline__ int kv8_query_exp(float amax) {
   return min(max(((__float_as_int(amax) + 0x1fffff) >> 23) - 8, 67), 247);
 }
 
-// Four query elements times `up` as e4m3 codes and the codes of what those
-// leave. Infinities become NaN: a row that holds one has no defined softmax.
-template <typename T>
-__device__ __forceinline__ void kv8_split_query(uint2 raw, float up, uint32_t& hi, uint32_t& lo) {
+// Four query elements times `up` as e4m3 codes, part by part: each holds the
+// rounding of what the parts before it leave (exact in fp32). Infinities
+// become NaN: a row that holds one has no defined softmax.
+template <typename T, int kParts>
+__device__ __forceinline__ void kv8_split_query(uint2 raw, float up, uint32_t (&part)[kParts]) {
   const float2 a = unpack2<T>(raw.x), b = unpack2<T>(raw.y);
   float x[4] = {a.x, a.y, b.x, b.y};
 #pragma unroll
   for (int i = 0; i < 4; ++i) x[i] = (fabsf(x[i]) == INFINITY ? NAN : x[i]) * up;
-  const uint32_t h0 = e4m3x2(x[0], x[1]), h1 = e4m3x2(x[2], x[3]);
-  const float2 r0 = unpack2<__half>(e4m3x2_to_h2(h0)), r1 = unpack2<__half>(e4m3x2_to_h2(h1));
-  hi = h0 | h1 << 16;
-  lo = e4m3x2(x[0] - r0.x, x[1] - r0.y) | e4m3x2(x[2] - r1.x, x[3] - r1.y) << 16;
+#pragma unroll
+  for (int k = 0; k < kParts; ++k) {
+    const uint32_t c0 = e4m3x2(x[0], x[1]), c1 = e4m3x2(x[2], x[3]);
+    part[k] = c0 | c1 << 16;
+    if (k + 1 < kParts) {
+      const float2 r0 = unpack2<__half>(e4m3x2_to_h2(c0)), r1 = unpack2<__half>(e4m3x2_to_h2(c1));
+      x[0] -= r0.x;
+      x[1] -= r0.y;
+      x[2] -= r1.x;
+      x[3] -= r1.y;
+    }
+  }
 }
 
 }  // namespace fe

@@ -7,35 +7,38 @@
 // V scale of the key's block, the weights are w = 2^(s + v - m) with m the
 // running maximum of s + v, O = sum w code_v, l = sum w 2^-v, out = O / l.
 //  * S = Q K^T runs on tcgen05 kind::f8f6f4 with the K codes as they lie in
-//    the cache and each query row as two e4m3 parts (high part and residual)
-//    scaled by a power of two: two fp8 products take the tensor core the time
-//    of one 16-bit product, and K needs no conversion.
+//    the cache and each query row scaled by a power of two and split into e4m3
+//    parts, each the rounding of what the ones before leave: two for bf16 (8 to
+//    9 bits: a bf16 exactly where it is within 2^11 of the row's largest) and
+//    three for f16 (its 11 bits). An fp8 product takes the tensor core half the
+//    time of a 16-bit one, and K needs no conversion.
 //  * O = W V runs on kind::f16 with the weights in f16 (11 bits, kept between
-//    2^-9 and 2^15 around the running maximum, so that the codes' 4 bits
-//    dominate the error) and V's codes converted to f16, exactly, by a
-//    warpgroup. Splitting the weights into two e4m3 parts instead would feed V
-//    raw, but costs five conversions a pair of weights (about 14 clocks of a
-//    warp) in the softmax warps, which are what bounds this kernel, against
-//    the one that f16 takes; converting V costs the spare warpgroup about 250
-//    clocks a tile.
+//    2^-9 and 2^15 around the running maximum) and V's codes converted to f16,
+//    exactly, by a warpgroup. Splitting the weights into e4m3 parts instead
+//    would feed V raw, but costs five conversions a pair of weights in the
+//    softmax warps, which are what bounds this kernel, against the one that f16
+//    takes.
 //
 // One persistent CTA per SM, sixteen warps. An item is 128 packed query rows
 // (row p = query row p / G, head kvh*G + p % G) of one sequence and KV head
 // against a range of keys, in tiles of 128 keys (64 for head_dim 256).
-//  warps 0-7   softmax, as in fe_prefill_tc.cu: a thread per packed row, the
-//              two groups take half a tile's keys each, trade maxima through
-//              shared memory and keep one O, rescaled lazily in TMEM.
+//  warps 0-7   softmax, two groups of four warps, a thread per packed row; the
+//              groups take alternate tiles, so that one's exponentials run
+//              while the other loads scores, finds its maximum or waits. The
+//              running maximum passes from tile to tile through shared memory;
+//              there is one O, rescaled in TMEM when the maximum has grown by
+//              2^8. Each group keeps the sum of its own tiles' weights.
 //  warp 8/11   producers of K (with the tiles' scale exponents) and of V.
 //  warp 9      issues S into one of three TMEM slots; owns TMEM.
-//  warp 10     issues O += W V once both groups wrote their half of W over
-//              the slot.
+//  warp 10     issues O += W V once the tile's group wrote W over the slot.
 //  warps 12-15 convert: V tiles to f16 (rows past the end become zeros, so
 //              nothing that lies there reaches O), and the next item's query
-//              rows to their two parts.
-// The softmax warps take 184 registers, the others 72 (setmaxnreg: 256 x 184 +
-// 256 x 72 = the launch's 512 x 128). All hand-offs are mbarriers; every wait
-// is bounded.
+//              rows to their parts.
+// The softmax warps take 200 registers (a row's 128 scores stay in them), the
+// others 56 (setmaxnreg: 256 x 200 + 256 x 56 = the launch's 512 x 128). All
+// hand-offs are mbarriers; every wait is bounded.
 #include <mutex>
+#include <type_traits>
 
 #include "fe_attn_common.cuh"
 #include "fe_kv8_attn.h"
@@ -48,26 +51,28 @@ namespace {
 constexpr int kThreads = 16 * 32;
 constexpr int kKWarp = 8, kSWarp = 9, kPvWarp = 10, kVWarp = 11, kConvWarp = 12;
 constexpr int kSlots = 3;      // S / W slots in TMEM
-constexpr int kKStages = 3;    // raw K tiles
-constexpr int kV8Stages = 2;   // raw V tiles
 constexpr int kV16Stages = 2;  // V tiles in f16
 constexpr int kExpRing = 8;    // tiles of scale factors; K runs at most 6 ahead
 constexpr uint32_t kTmemCols = 512;
 constexpr float kRescale = 8.f;  // O is rescaled when the maximum grew by 2^8
 constexpr float kBias = 7.f;     // weights are kept times 2^7: at most 2^15
 
-template <int D>
+template <typename T, int D>
 struct Cfg {
+  static constexpr bool kHalf = std::is_same<T, __half>::value;
   static constexpr int kM = 128;
   static constexpr int kN = D == 128 ? 128 : 64;       // keys per tile
-  static constexpr int kHalfN = kN / 2;
-  static constexpr int kPieces = kN / kTileTokens;
-  static constexpr int kHalfBlocks = kPieces / 2;      // scale blocks of a group's half
+  static constexpr int kPieces = kN / kTileTokens;     // = scale blocks of a tile
   static constexpr int kBoxes = D / 128;               // 128-code boxes per row
+  static constexpr int kParts = kHalf ? 3 : 2;         // e4m3 parts of a query
   static constexpr int kQBox = kM * 128;               // 128 rows x 128 codes
   static constexpr int kQPart = kBoxes * kQBox;
-  static constexpr int kQBytes = 2 * kQPart;
-  static constexpr int kQBufs = D == 128 ? 2 : 1;
+  static constexpr int kQBytes = kParts * kQPart;
+  // Raw V waits longest (for its load, then for the conversion): four stages
+  // where they fit. One query buffer: the next item's rows are converted while
+  // the softmax finishes the last tiles, whose S no longer needs it.
+  static constexpr int kKStages = D == 256 && kHalf ? 2 : 3;
+  static constexpr int kV8Stages = D == 128 ? (kHalf ? 3 : 4) : (kHalf ? 1 : 2);
   // raw tiles: [8-key group][box][8 rows x 128 B]; f16 V: [8-key group][64-dim
   // box][8 rows x 128 B]; all in 128-byte swizzle
   static constexpr int kPiece8 = kTileTokens * D;
@@ -75,19 +80,19 @@ struct Cfg {
   static constexpr int kTile8 = kN * D;
   static constexpr int kGroup16 = 16 * D;
   static constexpr int kTile16 = 2 * kTile8;
-  static constexpr int kOffK = kQBufs * kQBytes;
+  static constexpr int kOffK = kQBytes;
   static constexpr int kOffV8 = kOffK + kKStages * kTile8;
   static constexpr int kOffV16 = kOffV8 + kV8Stages * kTile8;
-  static constexpr int kOffMax = kOffV16 + kV16Stages * kTile16;  // [tile parity][group][row]
-  static constexpr int kOffSum = kOffMax + 2 * 2 * kM * 4;        // [item parity][group][row]
-  static constexpr int kOffRow = kOffSum + 2 * 2 * kM * 4;        // [Q buffer][row] score factors
-  static constexpr int kOffExp = kOffRow + 2 * kM * 4;            // [ring][8] float4
+  static constexpr int kOffMax = kOffV16 + kV16Stages * kTile16;  // [tile parity][row]
+  static constexpr int kOffSum = kOffMax + 2 * kM * 4;            // [item parity][group][row]
+  static constexpr int kOffRow = kOffSum + 2 * 2 * kM * 4;        // [row] score factors
+  static constexpr int kOffExp = kOffRow + kM * 4;            // [ring][8] float4
   static constexpr int kOffBar = kOffExp + kExpRing * 8 * 16;
-  static constexpr int kNumBars = 2 + 2 + 1 + 1 + 2 * kKStages + 2 * kV8Stages + 2 * kV16Stages +
-                                  kSlots + kSlots + 2 * kSlots + kExpRing + 8 + 1;
+  static constexpr int kNumBars = 1 + 1 + 1 + 1 + 2 * kKStages + 2 * kV8Stages + 2 * kV16Stages +
+                                  kSlots + kSlots + kSlots + kExpRing + 8 + 1;
   static constexpr int kSmem = kOffBar + kNumBars * 8 + 32;
   static constexpr uint32_t kOCol = D == 128 ? kSlots * kN : 256;
-  static constexpr int kGroupDims = D / 2;  // O dims a softmax group rescales and stores
+  static constexpr int kGroupDims = D / 2;  // O dims a softmax group stores
   static_assert(kSmem <= 232448, "shared memory budget");
   static_assert(kSlots * kN <= int(kOCol) && kOCol + D <= 512, "TMEM budget");
 };
@@ -143,14 +148,15 @@ template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1)
     kv8_rows_kernel(const __grid_constant__ CUtensorMap kmap,
                     const __grid_constant__ CUtensorMap vmap, const Kv8Args<T> ka) {
-  using C = Cfg<D>;
-  constexpr int kM = C::kM, kN = C::kN, kHalfN = C::kHalfN, kPieces = C::kPieces;
+  using C = Cfg<T, D>;
+  constexpr int kM = C::kM, kN = C::kN, kPieces = C::kPieces;
+  constexpr int kKStages = C::kKStages, kV8Stages = C::kV8Stages;
   const AttnArgs<T>& a = ka.a;
   extern __shared__ __align__(16) uint8_t smem[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
-  uint64_t* q_full = bars;                        // [buffer] both parts written
-  uint64_t* q_empty = q_full + 2;                 // [buffer] S done, row factors read
-  uint64_t* o_free = q_empty + 2;
+  uint64_t* q_full = bars;                        // an item's query parts written
+  uint64_t* q_empty = q_full + 1;                 // its S done, its row factors read
+  uint64_t* o_free = q_empty + 1;
   uint64_t* l_done = o_free + 1;
   uint64_t* k_full = l_done + 1;
   uint64_t* k_empty = k_full + kKStages;
@@ -160,9 +166,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* v16_empty = v16_full + kV16Stages;
   uint64_t* s_full = v16_empty + kV16Stages;      // [slot] S written
   uint64_t* s_free = s_full + kSlots;             // [slot] the PV that read it is done
-  uint64_t* p_full = s_free + kSlots;             // [slot*2 + group] W written
-  uint64_t* e_full = p_full + 2 * kSlots;         // [ring] scale factors written
-  uint64_t* max_bar = e_full + kExpRing;          // [tile parity*4 + quad]
+  uint64_t* p_full = s_free + kSlots;             // [slot] W written
+  uint64_t* e_full = p_full + kSlots;             // [ring] scale factors written
+  uint64_t* max_bar = e_full + kExpRing;          // [tile parity*4 + quad] maxima published
   uint64_t* drain = max_bar + 8;                  // every MMA issued is done
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + C::kNumBars);
   volatile int* flags = reinterpret_cast<volatile int*>(tmem_slot + 2);
@@ -188,10 +194,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 
   if (threadIdx.x == 0) {
-    for (int b = 0; b < 2; ++b) {
-      mbar_init(&q_full[b], 4);   // one arrival per converter warp
-      mbar_init(&q_empty[b], 9);  // the S issuer's commit, the softmax warps
-    }
+    mbar_init(q_full, 4);   // one arrival per converter warp
+    mbar_init(q_empty, 9);  // the S issuer's commit, the softmax warps
     mbar_init(o_free, 256);
     mbar_init(l_done, 256);
     for (int s = 0; s < kKStages; ++s) {
@@ -209,10 +213,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int s = 0; s < kSlots; ++s) {
       mbar_init(&s_full[s], 1);
       mbar_init(&s_free[s], 1);
+      mbar_init(&p_full[s], 4);
     }
-    for (int b = 0; b < 2 * kSlots; ++b) mbar_init(&p_full[b], 4);
     for (int b = 0; b < kExpRing; ++b) mbar_init(&e_full[b], 1);
-    for (int b = 0; b < 8; ++b) mbar_init(&max_bar[b], 64);
+    for (int b = 0; b < 8; ++b) mbar_init(&max_bar[b], 1);
     mbar_init(drain, 2);
     flags[0] = 0;
     flags[1] = 0;
@@ -231,7 +235,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   pdl_wait();
 
   if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == kKWarp || warp == kVWarp) {
       // ---------------------------------------------------------- producers
       const bool is_v = warp == kVWarp;
@@ -327,9 +331,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const WorkItem w = items[it];
           const int ntiles = (w.kt1 - w.kt0 + kPieces - 1) / kPieces;
           if (warp == kSWarp) {
-            const int qb = unit % C::kQBufs;
-            if (!wait_or_abort(&q_full[qb], (unit / C::kQBufs) & 1u, flags, aborted)) break;
-            const uint64_t q_desc = q_desc0 + uint64_t((qb * C::kQBytes) >> 4);
+            if (!wait_or_abort(q_full, unit & 1u, flags, aborted)) break;
             for (int t = 0; t < ntiles && !aborted; ++t, ++n) {
               const int slot = n % kSlots;
               const uint32_t st = n % kKStages;
@@ -338,19 +340,19 @@ __global__ void __launch_bounds__(kThreads, 1)
               tc::fence_after_sync();
               const uint64_t k_desc = k_desc0 + uint64_t((st * C::kTile8) >> 4);
 #pragma unroll
-              for (int part = 0; part < 2; ++part)
+              for (int part = 0; part < C::kParts; ++part)
 #pragma unroll
                 for (int kk = 0; kk < D / 32; ++kk) {
                   const int box = kk >> 2, ko = (kk & 3) * 32;
                   mma_f8_ss(tmem + slot * kN,
-                            q_desc + uint64_t((part * C::kQPart + box * C::kQBox + ko) >> 4),
+                            q_desc0 + uint64_t((part * C::kQPart + box * C::kQBox + ko) >> 4),
                             k_desc + uint64_t((box * 1024 + ko) >> 4), idesc_s,
                             part + kk > 0 ? 1u : 0u);
                 }
               tc::commit(&s_full[slot]);
               tc::commit(&k_empty[st]);
             }
-            if (!aborted) tc::commit(&q_empty[qb]);
+            if (!aborted) tc::commit(q_empty);
           } else {
             for (int t = 0; t < ntiles && !aborted; ++t, ++n) {
               const int slot = n % kSlots;
@@ -360,14 +362,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                   !wait_or_abort(o_free, (unit - 1) & 1, flags, aborted))
                 break;
               if (!wait_or_abort(&v16_full[st], (n / kV16Stages) & 1u, flags, aborted)) break;
-              if (!wait_or_abort(&p_full[slot * 2], (n / kSlots) & 1u, flags, aborted)) break;
-              if (!wait_or_abort(&p_full[slot * 2 + 1], (n / kSlots) & 1u, flags, aborted)) break;
+              if (!wait_or_abort(&p_full[slot], (n / kSlots) & 1u, flags, aborted)) break;
               tc::fence_after_sync();
               const uint64_t v_desc = v_desc0 + uint64_t((st * C::kTile16) >> 4);
 #pragma unroll
               for (int kk = 0; kk < kN / 16; ++kk) {
-                const int gi = kk / (kHalfN / 16), kg = kk % (kHalfN / 16);
-                tc::mma_f16_ts(tmem + C::kOCol, tmem + slot * kN + gi * kHalfN + kg * 8,
+                tc::mma_f16_ts(tmem + C::kOCol, tmem + slot * kN + kk * 8,
                                v_desc + uint64_t((kk * 2 * C::kGroup16) >> 4), idesc_o,
                                t + kk > 0 ? 1u : 0u);
               }
@@ -384,95 +384,131 @@ __global__ void __launch_bounds__(kThreads, 1)
       // ---------------------------------------------------------- converters
       const int tid = threadIdx.x - kConvWarp * 32;
       const int G = a.G;
-      // Query rows of item `u` (the CTA's u-th): a thread per packed row, its
-      // scale from the row's largest magnitude, two parts, the row's factor
-      // from products to base-2 scores.
-      auto convert_q = [&](int u) {
-        if (it0 + u >= it1) return;
-        const int qb = u % C::kQBufs;
-        if (!wait_warp(&q_empty[qb], ((u / C::kQBufs) & 1u) ^ 1u, flags, aborted)) return;
+      // Query rows of item `u` (the CTA's u-th): D / 16 lanes a row, 16
+      // elements each. fetch_q copies the 16-bit rows into the buffer (zeros
+      // past the sequence), 16-byte chunk k of row r to position k % 8 (swizzled)
+      // of box k / 8; convert_q replaces a row by its parts in place (the row
+      // takes as many bytes as two of them), and sets the row's factor from
+      // products to base-2 scores.
+      constexpr int kLanes = D / 16, kStep = 32 / kLanes;
+      const int qc = lane % kLanes;  // 16 elements, or codes of a part
+      const int q_r0 = (warp - kConvWarp) * 32 + lane / kLanes;
+      const int q_odd = (qc >> 2) & 1;  // odd boxes second chunk first: no bank conflicts
+      auto q_at = [&](int r, int k) {
+        return smem + (k >> 3) * C::kQBox + (r >> 3) * 1024 + (r & 7) * 128 +
+               (((k & 7) ^ (r & 7)) << 4);
+      };
+      auto fetch_q = [&](int u) {
         const WorkItem w = items[it0 + u];
         const SeqInfo si = seqs[w.seq];
-        const int p = w.rb0 * kRowBlock + tid;
-        const bool valid = p < si.qrows * G;
-        const uint4* src = reinterpret_cast<const uint4*>(
-            a.q + (valid ? (static_cast<int64_t>(si.q_row0 + p / G) * a.hq + w.kvh * G + p % G) * D
-                         : 0));
-        float amax = 0.f;
-        if (valid) {
-#pragma unroll 4
-          for (int c = 0; c < D / 8; ++c) {
-            const uint4 v = __ldg(src + c);
-            const uint32_t x[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float2 f = unpack2<T>(x[e]);
-              if (fabsf(f.x) < INFINITY) amax = fmaxf(amax, fabsf(f.x));
-              if (fabsf(f.y) < INFINITY) amax = fmaxf(amax, fabsf(f.y));
-            }
-          }
-        }
-        const int e = kv8_query_exp(amax);
-        const float up = exp_scale(254 - e);
-        row_f[qb * kM + tid] = exp_scale(e) * a.scale_log2;
-        uint8_t* dst = smem + qb * C::kQBytes + (tid >> 3) * 1024 + (tid & 7) * 128;
 #pragma unroll 2
-        for (int c = 0; c < D / 16; ++c) {  // 16 codes
-          uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
-          if (valid) {
-            const uint4 x = __ldg(src + 2 * c), y = __ldg(src + 2 * c + 1);
-            kv8_split_query<T>(make_uint2(x.x, x.y), up, hi.x, lo.x);
-            kv8_split_query<T>(make_uint2(x.z, x.w), up, hi.y, lo.y);
-            kv8_split_query<T>(make_uint2(y.x, y.y), up, hi.z, lo.z);
-            kv8_split_query<T>(make_uint2(y.z, y.w), up, hi.w, lo.w);
+        for (int r = q_r0; r < (q_r0 | 31) + 1; r += kStep) {
+          const int p = w.rb0 * kRowBlock + r;
+          const bool valid = p < si.qrows * G;
+          const int row = valid ? p / G : 0, head = valid ? p - row * G : 0;
+          const T* src =
+              a.q + (static_cast<int64_t>(si.q_row0 + row) * a.hq + w.kvh * G + head) * D + 16 * qc;
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                             smem_u32(q_at(r, 2 * qc + x))),
+                         "l"(src + 8 * x), "r"(valid ? 16 : 0)
+                         : "memory");
+        }
+      };
+      auto convert_q = [&]() {
+        asm volatile("cp.async.wait_all;" ::: "memory");
+#pragma unroll 2
+        for (int r = q_r0; r < (q_r0 | 31) + 1; r += kStep) {
+          uint4 x = *reinterpret_cast<const uint4*>(q_at(r, 2 * qc + q_odd));
+          uint4 y = *reinterpret_cast<const uint4*>(q_at(r, 2 * qc + 1 - q_odd));
+          if (q_odd) {
+            const uint4 z = x;
+            x = y;
+            y = z;
           }
-          uint8_t* at = dst + (c >> 3) * C::kQBox + (((c & 7) ^ (tid & 7)) << 4);
-          *reinterpret_cast<uint4*>(at) = hi;
-          *reinterpret_cast<uint4*>(at + C::kQPart) = lo;
+          const uint32_t v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+          float amax = 0.f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float2 f = unpack2<T>(v[e]);
+            if (fabsf(f.x) < INFINITY) amax = fmaxf(amax, fabsf(f.x));
+            if (fabsf(f.y) < INFINITY) amax = fmaxf(amax, fabsf(f.y));
+          }
+#pragma unroll
+          for (int o = kLanes / 2; o; o >>= 1)
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+          const int e = kv8_query_exp(amax);
+          const float up = exp_scale(254 - e);
+          if (qc == 0) row_f[r] = exp_scale(e) * a.scale_log2;
+          uint32_t part[C::kParts][4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint32_t four[C::kParts];
+            kv8_split_query<T, C::kParts>(make_uint2(v[2 * i], v[2 * i + 1]), up, four);
+#pragma unroll
+            for (int k = 0; k < C::kParts; ++k) part[k][i] = four[k];
+          }
+          __syncwarp();  // every lane of the row has read its elements
+#pragma unroll
+          for (int k = 0; k < C::kParts; ++k)
+            *reinterpret_cast<uint4*>(q_at(r, qc) + k * C::kQPart) =
+                make_uint4(part[k][0], part[k][1], part[k][2], part[k][3]);
         }
         tc::fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&q_full[qb]);
+        if (lane == 0) mbar_arrive(q_full);
       };
-      convert_q(0);
+      // A thread's part of a V tile: chunk vc (16 codes) of rows vr, vr +
+      // kRowStep, ..., whose addresses are constants apart. Codes 16 vc ..
+      // become chunks 2 vc and 2 vc + 1 of the f16 rows (64-dim box vc / 4);
+      // threads of odd boxes store their second chunk first, so that the
+      // eight threads of a row use all banks.
+      constexpr int kRowChunks = D / 16, kRowStep = 128 / kRowChunks, kPer = kN / kRowStep;
+      constexpr int kFromStep = kRowStep * D, kToStep = kRowStep * D * 2;
+      static_assert(kRowStep % 8 == 0, "whole 8-key groups between a thread's rows");
+      const int vc = tid % kRowChunks, vr = tid / kRowChunks;
+      const bool odd = (vc >> 2) & 1;
+      const uint8_t* v_from = smem + C::kOffV8 + (vr >> 3) * C::kGroup8 + (vc >> 3) * 1024 +
+                              (vr & 7) * 128 + (((vc & 7) ^ (vr & 7)) << 4);
+      uint8_t* v_to =
+          smem + C::kOffV16 + (vr >> 3) * C::kGroup16 + (vc >> 2) * 1024 + (vr & 7) * 128;
+      const int at0 = ((((2 * vc) & 7) + odd) ^ (vr & 7)) << 4;
+      const int at1 = ((((2 * vc) & 7) + 1 - odd) ^ (vr & 7)) << 4;
+      fetch_q(0);
+      convert_q();
       uint32_t n = 0;
       for (int u = 0; it0 + u < it1 && !aborted; ++u) {
         const WorkItem w = items[it0 + u];
         const SeqInfo si = seqs[w.seq];
         const int npieces = w.kt1 - w.kt0;
         const int ntiles = (npieces + kPieces - 1) / kPieces;
-        // the next item's queries: after the item's second tile where a second
-        // buffer takes them, else after its last (the buffer is then waiting
-        // for S of tiles whose V is converted)
-        const int q_after = C::kQBufs == 2 ? min(1, ntiles - 1) : ntiles - 1;
+        bool fetched = it0 + u + 1 >= it1;  // nothing to fetch
         for (int t = 0; t < ntiles; ++t, ++n) {
           const uint32_t s8 = n % kV8Stages, s16 = n % kV16Stages;
           if (!wait_warp(&v8_full[s8], (n / kV8Stages) & 1u, flags, aborted)) break;
           if (!wait_warp(&v16_empty[s16], ((n / kV16Stages) & 1u) ^ 1u, flags, aborted)) break;
-          const uint8_t* from = smem + C::kOffV8 + s8 * C::kTile8;
-          uint8_t* to = smem + C::kOffV16 + s16 * C::kTile16;
           const int valid = min(si.length - (w.kt0 + kPieces * t) * kTileTokens,
                                 (npieces - kPieces * t) * kTileTokens);
-          constexpr int kRowChunks = D / 16;
-          constexpr int kPer = kN * kRowChunks / 128;
+          const uint8_t* from = v_from + s8 * C::kTile8;
+          uint8_t* to = v_to + s16 * C::kTile16;
+          if (valid >= kN) {
 #pragma unroll 4
-          for (int k = 0; k < kPer; ++k) {
-            const int i = tid + k * 128;
-            const int c = i % kRowChunks, r = i / kRowChunks;
-            uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
-            if (r < valid)
-              codes_to_h2(*reinterpret_cast<const uint4*>(
-                              from + (r >> 3) * C::kGroup8 + (c >> 3) * 1024 + (r & 7) * 128 +
-                              (((c & 7) ^ (r & 7)) << 4)),
-                          lo, hi);
-            // dims 16c .. 16c + 15: chunks 2c and 2c + 1 of 64-dim box c / 4.
-            // Lanes of odd boxes store their second chunk first, so that the
-            // eight lanes of a row use all banks.
-            uint8_t* at = to + (r >> 3) * C::kGroup16 + (c >> 2) * 1024 + (r & 7) * 128;
-            const int odd = (c >> 2) & 1;
-            const int ch = (2 * c) & 7;
-            *reinterpret_cast<uint4*>(at + (((ch + odd) ^ (r & 7)) << 4)) = odd ? hi : lo;
-            *reinterpret_cast<uint4*>(at + (((ch + 1 - odd) ^ (r & 7)) << 4)) = odd ? lo : hi;
+            for (int k = 0; k < kPer; ++k) {
+              uint4 lo, hi;
+              codes_to_h2(*reinterpret_cast<const uint4*>(from + k * kFromStep), lo, hi);
+              *reinterpret_cast<uint4*>(to + at0 + k * kToStep) = odd ? hi : lo;
+              *reinterpret_cast<uint4*>(to + at1 + k * kToStep) = odd ? lo : hi;
+            }
+          } else {
+#pragma unroll 1
+            for (int k = 0; k < kPer; ++k) {
+              uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
+              if (vr + k * kRowStep < valid)
+                codes_to_h2(*reinterpret_cast<const uint4*>(from + k * kFromStep), lo, hi);
+              *reinterpret_cast<uint4*>(to + at0 + k * kToStep) = odd ? hi : lo;
+              *reinterpret_cast<uint4*>(to + at1 + k * kToStep) = odd ? lo : hi;
+            }
           }
           tc::fence_proxy_async_smem();
           __syncwarp();
@@ -480,15 +516,27 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_arrive(&v8_empty[s8]);
             mbar_arrive(&v16_full[s16]);
           }
-          if (t == q_after) convert_q(u + 1);
+          // the next item's queries, once the item's last S has read these
+          if (!fetched && t + kSlots >= ntiles &&
+              __all_sync(0xffffffffu, mbar_try_wait_short(q_empty, u & 1u))) {
+            fetch_q(u + 1);
+            fetched = true;
+          }
+        }
+        if (it0 + u + 1 < it1) {
+          if (!fetched) {
+            if (!wait_warp(q_empty, u & 1u, flags, aborted)) break;
+            fetch_q(u + 1);
+          }
+          convert_q();
         }
       }
       if (aborted && lane == 0) raise_device_error(a.err, FE_DEVERR_TIMEOUT);
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
     // ------------------------------------------------ softmax and epilogue
-    constexpr int kGD = C::kGroupDims, kHB = C::kHalfBlocks;
+    constexpr int kGD = C::kGroupDims;
     const int gi = warp >= 4 ? 1 : 0;
     const int quad = warp & 3;
     const int r = quad * 32 + lane;  // packed row = TMEM lane
@@ -496,7 +544,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t o_dims = lane_addr + C::kOCol + gi * kGD;
     const int G = a.G;
     const bool causal = view == 1;
-    uint32_t n = 0;  // tiles processed
+    uint32_t n0 = 0;  // the item's first tile
     int unit = 0;
     for (int it = it0; it < it1 && !aborted; ++it, ++unit) {
       const WorkItem w = items[it];
@@ -509,91 +557,85 @@ __global__ void __launch_bounds__(kThreads, 1)
       // keys this row sees in this item
       int lim = (causal && row_valid) ? si.length - si.qrows + p / G + 1 : si.length;
       lim = min(lim, w.kt1 * kTileTokens);
-      const int qb = unit % C::kQBufs;
-      if (!wait_warp(&q_full[qb], (unit / C::kQBufs) & 1u, flags, aborted)) break;
-      const float rf = row_f[qb * kM + r];
+      if (!wait_warp(q_full, unit & 1u, flags, aborted)) break;
+      const float rf = row_f[r];
       __syncwarp();
-      if (lane == 0) mbar_arrive(&q_empty[qb]);
+      if (lane == 0) mbar_arrive(q_empty);
+      // the maximum this group's weight sum l refers to
       float m_used = -INFINITY, l = 0.f;
-      for (int j = 0; j < ntiles; ++j, ++n) {
+      for (int j = (gi ^ n0) & 1; j < ntiles; j += 2) {
+        const uint32_t n = n0 + j;
         const int slot = n % kSlots;
-        const uint32_t half_addr = lane_addr + slot * kN + gi * kHalfN;
+        const uint32_t s_addr = lane_addr + slot * kN;
+        const float4* fac = ring + (n % kExpRing) * 8;
         if (!wait_warp(&e_full[n % kExpRing], (n / kExpRing) & 1u, flags, aborted)) break;
-        float kf[kHB], vf[kHB], vi[kHB];
-#pragma unroll
-        for (int b = 0; b < kHB; ++b) {
-          const float4 x = ring[(n % kExpRing) * 8 + gi * kHB + b];
-          kf[b] = x.x * rf;
-          vf[b] = x.y;
-          vi[b] = x.z;
-        }
         if (!wait_warp(&s_full[slot], (n / kSlots) & 1u, flags, aborted)) break;
         tc::fence_after_sync();
-        const int tkey = (w.kt0 + kPieces * j) * kTileTokens + gi * kHalfN;
-        float s[kHalfN];
+        const int tkey = (w.kt0 + kPieces * j) * kTileTokens;
+        float s[kN];
 #pragma unroll
-        for (int c = 0; c < kHalfN; c += 32)
-          tc::ld_32x32b_x32(half_addr + c, *reinterpret_cast<uint32_t(*)[32]>(&s[c]));
+        for (int c = 0; c < kN; c += 32)
+          tc::ld_32x32b_x32(s_addr + c, *reinterpret_cast<uint32_t(*)[32]>(&s[c]));
         tc::wait_ld();
-        if (tkey + kHalfN > lim) {
+        if (tkey + kN > lim) {
 #pragma unroll
-          for (int c = 0; c < kHalfN; ++c)
+          for (int c = 0; c < kN; ++c)
             if (tkey + c >= lim) s[c] = -INFINITY;
         }
         float mx = -INFINITY;
 #pragma unroll
-        for (int b = 0; b < kHB; ++b) {
+        for (int b = 0; b < kPieces; ++b) {
           const float* x = s + 16 * b;
+          const float4 f = fac[b];
           const float m0 = fmax3(x[0], x[1], x[2]), m1 = fmax3(x[3], x[4], x[5]),
                       m2 = fmax3(x[6], x[7], x[8]), m3 = fmax3(x[9], x[10], x[11]),
                       m4 = fmax3(x[12], x[13], x[14]);
-          const float mb = fmax3(fmax3(m0, m1, m2), fmax3(m3, m4, x[15]), -INFINITY);
-          mx = fmaxf(mx, fmaf(mb, kf[b], vf[b]));
+          mx = fmaxf(mx, fmaf(fmaxf(fmax3(m0, m1, m2), fmax3(m3, m4, x[15])), f.x * rf, f.y));
         }
-        {
-          // trade maxima with the other warp of these rows; the buffer of a
-          // tile parity is rewritten only after the partner passed the
-          // exchange of the tile in between
-          const int b = n & 1;
-          float* xm = xmax + b * 2 * kM;
-          xm[gi * kM + r] = mx;
-          mbar_arrive(&max_bar[b * 4 + quad]);
-          if (!wait_warp(&max_bar[b * 4 + quad], (n >> 1) & 1u, flags, aborted)) break;
-          mx = fmaxf(mx, xm[(gi ^ 1) * kM + r]);
+        // the maximum so far comes from the tile before and goes to the next;
+        // it moves only when it grows by more than 2^8 (or from nothing)
+        float m_prev = -INFINITY;
+        if (j > 0) {
+          if (!wait_warp(&max_bar[((n - 1) & 1) * 4 + quad], ((n - 1) >> 1) & 1u, flags, aborted))
+            break;
+          m_prev = xmax[((n - 1) & 1) * kM + r];
         }
-        const float m_new = fmaxf(m_used, mx);
-        // both groups see the same maxima and take the same decisions
-        const bool grow = m_new > m_used + kRescale;
-        if (__any_sync(0xffffffffu, grow)) {
-          const float alpha = grow ? fast_exp2(m_used - m_new) : 1.f;
-          if (j > 0) {
-            // wait for the last PV into O, then rescale this group's dims
-            if (!wait_warp(&s_free[(n - 1) % kSlots], ((n - 1) / kSlots) & 1u, flags, aborted))
-              break;
-            tc::fence_after_sync();
+        const float m_top = fmaxf(m_prev, mx);
+        const bool grow = m_top > m_prev + kRescale;
+        const float m_now = grow ? m_top : m_prev;
+        xmax[(n & 1) * kM + r] = m_now;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&max_bar[(n & 1) * 4 + quad]);
+        if (m_now != m_used) {
+          l *= fast_exp2(m_used - m_now);
+          m_used = m_now;
+        }
+        if (j > 0 && __any_sync(0xffffffffu, grow)) {
+          // wait for the last PV into O, then rescale it
+          const float alpha = grow ? fast_exp2(m_prev - m_now) : 1.f;
+          if (!wait_warp(&s_free[(n - 1) % kSlots], ((n - 1) / kSlots) & 1u, flags, aborted))
+            break;
+          tc::fence_after_sync();
+#pragma unroll 1
+          for (int c2 = 0; c2 < D / 16; ++c2) {
+            uint32_t ov[16];
+            tc::ld_32x32b_x16(lane_addr + C::kOCol + c2 * 16, ov);
+            tc::wait_ld();
 #pragma unroll
-            for (int c2 = 0; c2 < kGD / 32; ++c2) {
-              float ov[32];
-              tc::ld_32x32b_x32(o_dims + c2 * 32, *reinterpret_cast<uint32_t(*)[32]>(&ov[0]));
-              tc::wait_ld();
-#pragma unroll
-              for (int c = 0; c < 32; ++c) ov[c] *= alpha;
-              tc::st_32x32b_x32(o_dims + c2 * 32, *reinterpret_cast<uint32_t(*)[32]>(&ov[0]));
-            }
+            for (int c = 0; c < 16; ++c) ov[c] = __float_as_uint(__uint_as_float(ov[c]) * alpha);
+            tc::st_32x32b_x16(lane_addr + C::kOCol + c2 * 16, ov);
           }
-          l *= alpha;
-          if (grow) m_used = m_new;
         }
-        const float m_sub = (m_used == -INFINITY ? 0.f : m_used) - kBias;
+        const float m_sub = (m_now == -INFINITY ? 0.f : m_now) - kBias;
 #pragma unroll
-        for (int h = 0; h < kHalfN / 32; ++h) {
+        for (int h = 0; h < kN / 32; ++h) {
           uint32_t pk[16];
 #pragma unroll
           for (int b2 = 0; b2 < 2; ++b2) {
             const int b = 2 * h + b2;
-            const float2 sc2 = make_float2(kf[b], kf[b]);
-            const float off = vf[b] - m_sub;
-            const float2 off2 = make_float2(off, off);
+            const float4 f = fac[b];
+            const float fs = f.x * rf, off = f.y - m_sub;
+            const float2 sc2 = make_float2(fs, fs), off2 = make_float2(off, off);
             float2 sum0 = make_float2(0.f, 0.f), sum1 = sum0;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
@@ -606,20 +648,23 @@ __global__ void __launch_bounds__(kThreads, 1)
                 sum0 = add2(sum0, pp);
               pk[8 * b2 + e] = pack2<__half>(pp.x, pp.y);
             }
-            l = fmaf((sum0.x + sum0.y) + (sum1.x + sum1.y), vi[b], l);
+            l = fmaf((sum0.x + sum0.y) + (sum1.x + sum1.y), f.z, l);
           }
-          tc::st_32x32b_x16(half_addr + 16 * h, pk);
+          tc::st_32x32b_x16(s_addr + 16 * h, pk);
         }
         tc::wait_st();
         tc::fence_before_sync();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[slot * 2 + gi]);
+        if (lane == 0) mbar_arrive(&p_full[slot]);
       }
       if (aborted) break;
-      // the item's last PV
-      if (ntiles > 0 &&
-          !wait_warp(&s_free[(n - 1) % kSlots], ((n - 1) / kSlots) & 1u, flags, aborted))
-        break;
+      // the last tile's maximum is the item's; its PV is the item's last
+      const uint32_t nl = n0 + ntiles - 1;
+      n0 += ntiles;
+      if (!wait_warp(&max_bar[(nl & 1) * 4 + quad], (nl >> 1) & 1u, flags, aborted)) break;
+      const float m_item = xmax[(nl & 1) * kM + r];
+      if (m_used != m_item) l *= fast_exp2(m_used - m_item);
+      if (!wait_warp(&s_free[nl % kSlots], (nl / kSlots) & 1u, flags, aborted)) break;
       float* xs = xsum + (unit & 1) * 2 * kM;
       xs[gi * kM + r] = l;
       mbar_arrive(l_done);
@@ -635,7 +680,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                  D + gi * kGD
                    : nullptr;
       if (split && row_valid && gi == 0) {
-        rec[rows_rec * D + r] = m_used;
+        rec[rows_rec * D + r] = m_item;
         rec[rows_rec * (D + 1) + r] = lsum;
       }
 #pragma unroll
@@ -683,11 +728,12 @@ int launch(const CUtensorMap& kmap, const CUtensorMap& vmap, const Kv8Args<T>& a
   static cudaError_t attr_err = cudaSuccess;
   std::call_once(once, [] {
     attr_err = cudaFuncSetAttribute(kv8_rows_kernel<T, D>,
-                                    cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::kSmem);
+                                    cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<T, D>::kSmem);
   });
   if (attr_err != cudaSuccess) return cuda_fail(attr_err, "kv8_rows_kernel attribute");
-  FE_CUDA_TRY(launch_pdl(kv8_rows_kernel<T, D>, dim3(grid), dim3(kThreads), Cfg<D>::kSmem, stream,
-                         kmap, vmap, args));
+  constexpr int kSmem = Cfg<T, D>::kSmem;
+  FE_CUDA_TRY(launch_pdl(kv8_rows_kernel<T, D>, dim3(grid), dim3(kThreads), kSmem, stream, kmap,
+                         vmap, args));
   return FE_OK;
 }
 
