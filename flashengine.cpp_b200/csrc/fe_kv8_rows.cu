@@ -34,9 +34,7 @@
 //  warps 12-15 convert: V tiles to f16 (rows past the end become zeros, so
 //              nothing that lies there reaches O), and the next item's query
 //              rows to their parts.
-// The softmax warps take 200 registers (a row's 128 scores stay in them), the
-// others 56 (setmaxnreg: 256 x 200 + 256 x 56 = the launch's 512 x 128). All
-// hand-offs are mbarriers; every wait is bounded.
+// All hand-offs are mbarriers; every wait is bounded.
 #include <mutex>
 #include <type_traits>
 
@@ -235,7 +233,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   pdl_wait();
 
   if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == kKWarp || warp == kVWarp) {
       // ---------------------------------------------------------- producers
       const bool is_v = warp == kVWarp;
@@ -251,9 +248,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         const SeqInfo si = seqs[w.seq];
         const int npieces = w.kt1 - w.kt0;
         const int ntiles = (npieces + kPieces - 1) / kPieces;
-        // Slot of 16-token piece i; the lanes hold 32 pieces and ask for the
-        // next 32 before they are needed. The K producer also holds its
-        // pieces' K and V exponents.
+        // Slot of 16-token piece i. A lane looks after one piece of a batch of
+        // 32: its slot is asked for two batches ahead; in the K producer, the K
+        // and V exponents of its block one batch ahead.
         auto piece_slot = [&](int i) -> int {
           if (i >= npieces) return -1;
           const int t0 = (w.kt0 + i) * kTileTokens;
@@ -264,21 +261,19 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int64_t at = int64_t(slot / kKv8Block) * ka.hkv + w.kvh;
           return ka.k_exp[at] | ka.v_exp[at] << 8;
         };
-        int cur = piece_slot(lane), nxt = piece_slot(32 + lane);
-        int ecur = piece_exps(cur), enxt = piece_exps(nxt);
+        int cur = 0, nxt = piece_slot(lane), nxt2 = piece_slot(32 + lane);
+        int ecur = 0, enxt = piece_exps(nxt);
         for (int j = 0; j < ntiles && !aborted; ++j, ++g) {
           const int pb = (kPieces * j) & 31;
-          if (j > 0 && pb == 0) {
+          if (pb == 0) {
             cur = nxt;
             ecur = enxt;
-            nxt = piece_slot(kPieces * j + 32 + lane);
+            nxt = nxt2;
             enxt = piece_exps(nxt);
+            nxt2 = piece_slot(kPieces * j + 64 + lane);
           }
           const int pieces = min(kPieces, npieces - kPieces * j);
           const uint32_t st = g % stages;
-          int sl[kPieces];
-#pragma unroll
-          for (int u = 0; u < kPieces; ++u) sl[u] = __shfl_sync(0xffffffffu, cur, pb + u);
           int good = 1;
           if (lane == 0 && !wait_or_abort(&empty[st], ((g / stages) & 1u) ^ 1u, flags, aborted))
             good = 0;
@@ -286,27 +281,21 @@ __global__ void __launch_bounds__(kThreads, 1)
             aborted = true;
             break;
           }
-          if (!is_v) {
+          const int mine = lane - pb;  // this lane's piece of the tile
+          if (!is_v && mine >= 0 && mine < kPieces) {
             // this tile's factors (the softmax is done with the tile kExpRing
             // back: the S three tiles back has completed, which waited for
             // the PV of the tile six back)
-            if (lane >= pb && lane < pb + kPieces) {
-              const int ke = exp_clamp(ecur & 0xff), ve = exp_clamp(ecur >> 8);
-              ring[(g % kExpRing) * 8 + lane - pb] =
-                  make_float4(exp_scale(ke), float(ve - 127), exp_scale(254 - ve), 0.f);
-            }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&e_full[g % kExpRing]);
+            const int ke = exp_clamp(ecur & 0xff), ve = exp_clamp(ecur >> 8);
+            ring[(g % kExpRing) * 8 + mine] =
+                make_float4(exp_scale(ke), float(ve - 127), exp_scale(254 - ve), 0.f);
           }
-          if (lane == 0) {
-            mbar_arrive_expect_tx(&full[st], pieces * C::kPiece8);
-            uint8_t* dst = region + st * C::kTile8;
-#pragma unroll
-            for (int u = 0; u < kPieces; ++u)
-              if (u < pieces)
-                tma_load_4d(dst + u * C::kPiece8, map, &full[st], 0, 0, w.kvh * C::kBoxes,
-                            sl[u] >> 3);
-          }
+          if (lane == 0) mbar_arrive_expect_tx(&full[st], pieces * C::kPiece8);
+          __syncwarp();
+          if (!is_v && lane == 0) mbar_arrive(&e_full[g % kExpRing]);
+          if (mine >= 0 && mine < pieces)
+            tma_load_4d(region + st * C::kTile8 + mine * C::kPiece8, map, &full[st], 0, 0,
+                        w.kvh * C::kBoxes, cur >> 3);
         }
       }
       if (lane == 0) {
@@ -534,7 +523,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (aborted && lane == 0) raise_device_error(a.err, FE_DEVERR_TIMEOUT);
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
     // ------------------------------------------------ softmax and epilogue
     constexpr int kGD = C::kGroupDims;
     const int gi = warp >= 4 ? 1 : 0;
@@ -572,25 +560,39 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!wait_warp(&s_full[slot], (n / kSlots) & 1u, flags, aborted)) break;
         tc::fence_after_sync();
         const int tkey = (w.kt0 + kPieces * j) * kTileTokens;
-        float s[kN];
-#pragma unroll
-        for (int c = 0; c < kN; c += 32)
-          tc::ld_32x32b_x32(s_addr + c, *reinterpret_cast<uint32_t(*)[32]>(&s[c]));
-        tc::wait_ld();
-        if (tkey + kN > lim) {
-#pragma unroll
-          for (int c = 0; c < kN; ++c)
-            if (tkey + c >= lim) s[c] = -INFINITY;
-        }
+        // Scores pass twice through registers, 64 keys at a time: for the
+        // maximum, and for the weights. (All 128 at once need 200 registers
+        // and twice the code; the instruction fetch of the kernel's eight kinds
+        // of warps then bounds it.)
         float mx = -INFINITY;
+#pragma unroll 1
+        for (int h = 0; h < kN; h += 64) {
+          float s[64];
 #pragma unroll
-        for (int b = 0; b < kPieces; ++b) {
-          const float* x = s + 16 * b;
-          const float4 f = fac[b];
-          const float m0 = fmax3(x[0], x[1], x[2]), m1 = fmax3(x[3], x[4], x[5]),
-                      m2 = fmax3(x[6], x[7], x[8]), m3 = fmax3(x[9], x[10], x[11]),
-                      m4 = fmax3(x[12], x[13], x[14]);
-          mx = fmaxf(mx, fmaf(fmaxf(fmax3(m0, m1, m2), fmax3(m3, m4, x[15])), f.x * rf, f.y));
+          for (int c = 0; c < 64; c += 32)
+            tc::ld_32x32b_x32(s_addr + h + c, *reinterpret_cast<uint32_t(*)[32]>(&s[c]));
+          tc::wait_ld();
+          if (tkey + h + 64 > lim) {
+            // hidden keys become -inf, in TMEM too
+#pragma unroll
+            for (int c = 0; c < 64; ++c)
+              if (tkey + h + c >= lim) s[c] = -INFINITY;
+          }
+          if (__any_sync(0xffffffffu, tkey + h + 64 > lim)) {
+#pragma unroll
+            for (int c = 0; c < 64; c += 32)
+              tc::st_32x32b_x32(s_addr + h + c, *reinterpret_cast<uint32_t(*)[32]>(&s[c]));
+            tc::wait_st();
+          }
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {
+            const float* x = s + 16 * b;
+            const float4 f = fac[h / 16 + b];
+            const float m0 = fmax3(x[0], x[1], x[2]), m1 = fmax3(x[3], x[4], x[5]),
+                        m2 = fmax3(x[6], x[7], x[8]), m3 = fmax3(x[9], x[10], x[11]),
+                        m4 = fmax3(x[12], x[13], x[14]);
+            mx = fmaxf(mx, fmaf(fmaxf(fmax3(m0, m1, m2), fmax3(m3, m4, x[15])), f.x * rf, f.y));
+          }
         }
         // the maximum so far comes from the tile before and goes to the next;
         // it moves only when it grows by more than 2^8 (or from nothing)
@@ -627,30 +629,39 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         const float m_sub = (m_now == -INFINITY ? 0.f : m_now) - kBias;
+#pragma unroll 1
+        for (int h = 0; h < kN; h += 64) {
+          float s[64];
 #pragma unroll
-        for (int h = 0; h < kN / 32; ++h) {
-          uint32_t pk[16];
+          for (int c = 0; c < 64; c += 32)
+            tc::ld_32x32b_x32(s_addr + h + c, *reinterpret_cast<uint32_t(*)[32]>(&s[c]));
+          tc::wait_ld();
 #pragma unroll
-          for (int b2 = 0; b2 < 2; ++b2) {
-            const int b = 2 * h + b2;
-            const float4 f = fac[b];
-            const float fs = f.x * rf, off = f.y - m_sub;
-            const float2 sc2 = make_float2(fs, fs), off2 = make_float2(off, off);
-            float2 sum0 = make_float2(0.f, 0.f), sum1 = sum0;
+          for (int h2 = 0; h2 < 2; ++h2) {
+            uint32_t pk[16];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const float2 x =
-                  fma2(make_float2(s[16 * b + 2 * e], s[16 * b + 2 * e + 1]), sc2, off2);
-              const float2 pp = make_float2(fast_exp2(x.x), fast_exp2(x.y));
-              if (e & 1)
-                sum1 = add2(sum1, pp);
-              else
-                sum0 = add2(sum0, pp);
-              pk[8 * b2 + e] = pack2<__half>(pp.x, pp.y);
+            for (int b2 = 0; b2 < 2; ++b2) {
+              const int b = 2 * h2 + b2;
+              const float4 f = fac[h / 16 + b];
+              const float fs = f.x * rf, off = f.y - m_sub;
+              const float2 sc2 = make_float2(fs, fs), off2 = make_float2(off, off);
+              float2 sum0 = make_float2(0.f, 0.f), sum1 = sum0;
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                const float2 x =
+                    fma2(make_float2(s[16 * b + 2 * e], s[16 * b + 2 * e + 1]), sc2, off2);
+                const float2 pp = make_float2(fast_exp2(x.x), fast_exp2(x.y));
+                if (e & 1)
+                  sum1 = add2(sum1, pp);
+                else
+                  sum0 = add2(sum0, pp);
+                pk[8 * b2 + e] = pack2<__half>(pp.x, pp.y);
+              }
+              l = fmaf((sum0.x + sum0.y) + (sum1.x + sum1.y), f.z, l);
             }
-            l = fmaf((sum0.x + sum0.y) + (sum1.x + sum1.y), f.z, l);
+            // (weights of 64 keys take the columns of 32: never ones still to be read)
+            tc::st_32x32b_x16(s_addr + h / 2 + 16 * h2, pk);
           }
-          tc::st_32x32b_x16(s_addr + 16 * h, pk);
         }
         tc::wait_st();
         tc::fence_before_sync();
