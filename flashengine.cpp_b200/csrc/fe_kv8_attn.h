@@ -29,24 +29,19 @@ __device__ __forceinline__ int kv8_query_exp(float amax) {
 }
 
 // Four query elements times `up` as e4m3 codes, part by part: each holds the
-// rounding of what the parts before it leave (exact in fp32). Infinities
-// become NaN: a row that holds one has no defined softmax.
+// rounding of what the parts before it leave (exact in fp32).
 template <typename T, int kParts>
-__device__ __forceinline__ void kv8_split_query(uint2 raw, float up, uint32_t (&part)[kParts]) {
-  const float2 a = unpack2<T>(raw.x), b = unpack2<T>(raw.y);
-  float x[4] = {a.x, a.y, b.x, b.y};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) x[i] = (fabsf(x[i]) == INFINITY ? NAN : x[i]) * up;
+__device__ __forceinline__ void kv8_split_query(uint32_t v0, uint32_t v1, float up,
+                                                uint32_t (&part)[kParts]) {
+  const float2 up2 = make_float2(up, up);
+  float2 x = mul2(unpack2<T>(v0), up2), y = mul2(unpack2<T>(v1), up2);
 #pragma unroll
   for (int k = 0; k < kParts; ++k) {
-    const uint32_t c0 = e4m3x2(x[0], x[1]), c1 = e4m3x2(x[2], x[3]);
+    const uint32_t c0 = e4m3x2(x.x, x.y), c1 = e4m3x2(y.x, y.y);
     part[k] = c0 | c1 << 16;
     if (k + 1 < kParts) {
-      const float2 r0 = unpack2<__half>(e4m3x2_to_h2(c0)), r1 = unpack2<__half>(e4m3x2_to_h2(c1));
-      x[0] -= r0.x;
-      x[1] -= r0.y;
-      x[2] -= r1.x;
-      x[3] -= r1.y;
+      x = sub2(x, unpack2<__half>(e4m3x2_to_h2(c0)));
+      y = sub2(y, unpack2<__half>(e4m3x2_to_h2(c1)));
     }
   }
 }

@@ -58,4 +58,26 @@ __device__ __forceinline__ float exp_scale(int e) { return __int_as_float(e << 2
 // so that bytes of blocks no token was written to stay finite.
 __device__ __forceinline__ int exp_clamp(int e) { return min(max(e, kKv8MinExp), kKv8MaxExp); }
 
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 ra, rb, rd;\n\t"
+      "mov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\t"
+      "mul.rn.f32x2 rd, ra, rb;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
+// Packed 16-bit maximum of magnitudes (a NaN is passed over).
+__device__ __forceinline__ uint32_t max_abs2(uint32_t m, uint32_t v, __half) {
+  const __half2 r = __hmax2(*reinterpret_cast<__half2*>(&m),
+                            __habs2(*reinterpret_cast<__half2*>(&v)));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t max_abs2(uint32_t m, uint32_t v, __nv_bfloat16) {
+  const __nv_bfloat162 r = __hmax2(*reinterpret_cast<__nv_bfloat162*>(&m),
+                                   __habs2(*reinterpret_cast<__nv_bfloat162*>(&v)));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
 }  // namespace fe

@@ -21,16 +21,6 @@ struct Quad {
   float2 x, y;
 };
 
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  float2 d;
-  asm("{\n\t.reg .b64 ra, rb, rd;\n\t"
-      "mov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\t"
-      "mul.rn.f32x2 rd, ra, rb;\n\tmov.b64 {%0, %1}, rd;\n\t}"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return d;
-}
-
 // A rotation pair in fp32, each product and sum rounded separately as fe_rope
 // does (the packed fp32 instructions were not: ptxas fused them).
 __device__ __forceinline__ void rotate1(float& a, float& b, float c, float s) {
@@ -68,18 +58,6 @@ __device__ __forceinline__ uint32_t codes4(const Quad& q, float inv) {
   const float2 s = make_float2(inv, inv);
   const float2 x = mul2(q.x, s), y = mul2(q.y, s);
   return e4m3x2(x.x, x.y) | e4m3x2(y.x, y.y) << 16;
-}
-
-// Packed 16-bit maximum of magnitudes (a NaN is passed over).
-__device__ __forceinline__ uint32_t max_abs2(uint32_t m, uint32_t v, __half) {
-  const __half2 r = __hmax2(*reinterpret_cast<__half2*>(&m),
-                            __habs2(*reinterpret_cast<__half2*>(&v)));
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
-__device__ __forceinline__ uint32_t max_abs2(uint32_t m, uint32_t v, __nv_bfloat16) {
-  const __nv_bfloat162 r = __hmax2(*reinterpret_cast<__nv_bfloat162*>(&m),
-                                   __habs2(*reinterpret_cast<__nv_bfloat162*>(&v)));
-  return *reinterpret_cast<const uint32_t*>(&r);
 }
 
 // Biased exponent of the smallest power of two s with amax <= 448 s (448 is

@@ -105,26 +105,10 @@ __device__ __forceinline__ void mma_f8_ss(uint32_t d, uint64_t a, uint64_t b, ui
       : "memory");
 }
 
-// wait_bounded_short, inlined: a call would keep ptxas from giving the two
-// halves of the kernel their own register counts.
-__device__ __forceinline__ bool wait_bounded_inl(uint64_t* bar, uint32_t parity,
-                                                 volatile int* abort_flag) {
-  if (mbar_try_wait_short(bar, parity)) return true;
-  const uint64_t t0 = global_ns();
-  for (;;) {
-    if (mbar_try_wait_short(bar, parity)) return true;
-    if (*abort_flag) return false;
-    if (global_ns() - t0 > kWaitLimitNs) {
-      *abort_flag = 1;
-      return false;
-    }
-  }
-}
-
 __device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, volatile int* flags,
                                               bool& aborted) {
   if (aborted) return false;
-  if (!wait_bounded_inl(bar, parity, flags)) aborted = true;
+  if (!wait_bounded_short(bar, parity, flags)) aborted = true;
   return !aborted;
 }
 __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, volatile int* flags,
@@ -302,7 +286,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (aborted) raise_device_error(a.err, FE_DEVERR_TIMEOUT);
         // the last load into each stage has landed before the CTA may exit
         for (uint32_t t = g > stages ? g - stages : 0; t < g; ++t)
-          wait_bounded_inl(&full[t % stages], (t / stages) & 1u, flags + 1);
+          wait_bounded_short(&full[t % stages], (t / stages) & 1u, flags + 1);
       }
     } else if (warp == kSWarp || warp == kPvWarp) {
       // -------------------------------------------------------- MMA issuers
@@ -367,7 +351,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (aborted) raise_device_error(a.err, FE_DEVERR_TIMEOUT);
         tc::commit(drain);
-        wait_bounded_inl(drain, 0, flags + 1);
+        wait_bounded_short(drain, 0, flags + 1);
       }
     } else {
       // ---------------------------------------------------------- converters
@@ -384,8 +368,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int q_r0 = (warp - kConvWarp) * 32 + lane / kLanes;
       const int q_odd = (qc >> 2) & 1;  // odd boxes second chunk first: no bank conflicts
       auto q_at = [&](int r, int k) {
-        return smem + (k >> 3) * C::kQBox + (r >> 3) * 1024 + (r & 7) * 128 +
-               (((k & 7) ^ (r & 7)) << 4);
+        return smem + (k >> 3) * C::kQBox + (r >> 3) * 1024 +
+               (r & 7) * 128 + (((k & 7) ^ (r & 7)) << 4);
       };
       auto fetch_q = [&](int u) {
         const WorkItem w = items[it0 + u];
@@ -417,24 +401,23 @@ __global__ void __launch_bounds__(kThreads, 1)
             y = z;
           }
           const uint32_t v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-          float amax = 0.f;
+          uint32_t m2 = 0;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float2 f = unpack2<T>(v[e]);
-            if (fabsf(f.x) < INFINITY) amax = fmaxf(amax, fabsf(f.x));
-            if (fabsf(f.y) < INFINITY) amax = fmaxf(amax, fabsf(f.y));
-          }
+          for (int e = 0; e < 8; ++e) m2 = max_abs2(m2, v[e], T());
+          const float2 mf = unpack2<T>(m2);
+          float amax = fmaxf(mf.x, mf.y);
 #pragma unroll
           for (int o = kLanes / 2; o; o >>= 1)
             amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
           const int e = kv8_query_exp(amax);
-          const float up = exp_scale(254 - e);
+          // a row that holds an infinity has no defined softmax
+          const float up = amax == INFINITY ? NAN : exp_scale(254 - e);
           if (qc == 0) row_f[r] = exp_scale(e) * a.scale_log2;
           uint32_t part[C::kParts][4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             uint32_t four[C::kParts];
-            kv8_split_query<T, C::kParts>(make_uint2(v[2 * i], v[2 * i + 1]), up, four);
+            kv8_split_query<T, C::kParts>(v[2 * i], v[2 * i + 1], up, four);
 #pragma unroll
             for (int k = 0; k < C::kParts; ++k) part[k][i] = four[k];
           }
@@ -472,7 +455,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         const SeqInfo si = seqs[w.seq];
         const int npieces = w.kt1 - w.kt0;
         const int ntiles = (npieces + kPieces - 1) / kPieces;
-        bool fetched = it0 + u + 1 >= it1;  // nothing to fetch
+        // the next item's queries: fetched as soon as the last S has read this
+        // item's, converted a tile later, or when this item's V is done
+        enum { kWanted, kFetched, kDone } next = it0 + u + 1 < it1 ? kWanted : kDone;
         for (int t = 0; t < ntiles; ++t, ++n) {
           const uint32_t s8 = n % kV8Stages, s16 = n % kV16Stages;
           if (!wait_warp(&v8_full[s8], (n / kV8Stages) & 1u, flags, aborted)) break;
@@ -505,20 +490,20 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_arrive(&v8_empty[s8]);
             mbar_arrive(&v16_full[s16]);
           }
-          // the next item's queries, once the item's last S has read these
-          if (!fetched && t + kSlots >= ntiles &&
-              __all_sync(0xffffffffu, mbar_try_wait_short(q_empty, u & 1u))) {
+          if (next == kFetched) {
+            convert_q();
+            next = kDone;
+          } else if (next == kWanted && __all_sync(0xffffffffu, mbar_test(q_empty, u & 1u))) {
             fetch_q(u + 1);
-            fetched = true;
+            next = kFetched;
           }
         }
-        if (it0 + u + 1 < it1) {
-          if (!fetched) {
-            if (!wait_warp(q_empty, u & 1u, flags, aborted)) break;
-            fetch_q(u + 1);
-          }
-          convert_q();
+        if (aborted) break;
+        if (next == kWanted) {
+          if (!wait_warp(q_empty, u & 1u, flags, aborted)) break;
+          fetch_q(u + 1);
         }
+        if (next != kDone) convert_q();
       }
       if (aborted && lane == 0) raise_device_error(a.err, FE_DEVERR_TIMEOUT);
     }
