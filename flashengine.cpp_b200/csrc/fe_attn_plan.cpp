@@ -227,6 +227,114 @@ int build_cut_view(const PlanConfig& cfg, const std::vector<Unit>& units, int gr
   return FE_OK;
 }
 
+// Row lists of the 8-bit cache. The kernel's time for an item is its key tiles
+// (of cfg.row_tile 16-key pieces) plus a fixed cost worth cfg.row_item_tiles of
+// them (queries, first scores, epilogue), so a cut by tiles alone gives the
+// CTAs of a step's many short items far more time than the others (a mixed
+// step took 314 us where this cut takes a third). The units are laid end to end
+// and cut into at most grid_cap pieces of equal cost, at whole tiles; a unit is
+// cut only into pieces of at least cfg.row_item_tiles tiles.
+int build_cost_view(const PlanConfig& cfg, const std::vector<Unit>& units, int grid_cap_in,
+                    bool fixed_grid, View& v, std::string& err) {
+  v = View{};
+  if (units.empty()) return FE_OK;
+  const int64_t ov = cfg.row_item_tiles;
+  const int grid_cap = std::max(1, grid_cap_in);
+  auto big = [&](const Unit& u) -> int64_t { return ceil_div(u.tiles, cfg.row_tile); };
+  // Cut for CTAs of cost `budget`; emit(unit, first tile, tiles, cta). Returns
+  // the CTAs used.
+  auto cut = [&](int64_t budget, auto&& emit) -> int64_t {
+    int64_t cta = 0, room = budget;
+    for (size_t i = 0; i < units.size(); ++i) {
+      int64_t at = 0, left = big(units[i]);
+      while (left > 0) {
+        int64_t take = std::min(left, room - ov);
+        if (take < left) {  // a piece: both sides long enough, or none here
+          if (left - take < ov) take = left - ov;
+          if (take < ov) take = 0;
+        }
+        if (take <= 0) {
+          if (room == budget) take = left;  // does not fit an empty CTA: whole
+          else {
+            ++cta;
+            room = budget;
+            continue;
+          }
+        }
+        emit(i, at, take, cta);
+        at += take;
+        left -= take;
+        room -= take + ov;
+      }
+    }
+    return cta + 1;
+  };
+  int64_t total = 0, most = 0;
+  for (const auto& u : units) {
+    total += big(u) + ov;
+    most = std::max(most, big(u) + ov);
+  }
+  // (below 2 ov no unit can be cut, and every budget would do)
+  int64_t lo = std::max<int64_t>(2 * ov, (total + grid_cap - 1) / grid_cap), hi = total + most;
+  auto none = [](size_t, int64_t, int64_t, int64_t) {};
+  while (lo < hi) {
+    const int64_t mid = (lo + hi) / 2;
+    if (cut(mid, none) <= grid_cap)
+      hi = mid;
+    else
+      lo = mid + 1;
+  }
+  std::vector<int> pieces(units.size(), 0);
+  cut(lo, [&](size_t i, int64_t, int64_t, int64_t) { ++pieces[i]; });
+  std::vector<int> group_of(units.size(), -1), part_of(units.size(), -1);
+  for (size_t i = 0; i < units.size(); ++i) {
+    if (pieces[i] < 2) continue;
+    const Unit& u = units[i];
+    const int rec = partial_rec_floats(u.rows, cfg.dim);
+    group_of[i] = static_cast<int>(v.groups.size());
+    part_of[i] = static_cast<int>(v.partial_floats);
+    v.groups.push_back(SplitGroup{pieces[i], part_of[i], rec, u.rows, u.seq, u.kvh,
+                                  u.rb0 * kRowBlock, u.rows});
+    v.partial_floats += int64_t(rec) * pieces[i];
+    ++v.split_units;
+  }
+  int64_t last_cta = -1;
+  cut(lo, [&](size_t i, int64_t at, int64_t take, int64_t cta) {
+    const Unit& u = units[i];
+    for (; last_cta < cta; ++last_cta) v.cta_off.push_back(static_cast<int32_t>(v.items.size()));
+    WorkItem it;
+    it.seq = u.seq;
+    it.kvh = static_cast<int16_t>(u.kvh);
+    it.key_mode = 0;
+    it.rb0 = u.rb0;
+    it.nrb = u.nrb;
+    it.kt0 = static_cast<int32_t>(at * cfg.row_tile);
+    it.kt1 = static_cast<int32_t>(std::min<int64_t>(u.tiles, (at + take) * cfg.row_tile));
+    it.group = group_of[i];
+    it.part = -1;
+    if (group_of[i] >= 0) {
+      it.part = part_of[i];
+      part_of[i] += partial_rec_floats(u.rows, cfg.dim);
+    }
+    v.items.push_back(it);
+    ++v.prefill_items;
+  });
+  v.cta_off.push_back(static_cast<int32_t>(v.items.size()));
+  v.grid = static_cast<int>(v.cta_off.size()) - 1;
+  v.chunk = static_cast<int>(lo * cfg.row_tile);
+  if (static_cast<int>(v.items.size()) > cfg.max_items ||
+      v.partial_floats > cfg.partial_capacity ||
+      static_cast<int>(v.groups.size()) > cfg.max_groups) {
+    err = "attention work exceeds the plan's item / split-workspace capacity";
+    return FE_ERR_CAPACITY;
+  }
+  while (fixed_grid && v.grid < grid_cap) {  // graph mode launches grid_cap CTAs
+    v.cta_off.push_back(static_cast<int32_t>(v.items.size()));
+    ++v.grid;
+  }
+  return FE_OK;
+}
+
 }  // namespace
 
 int concurrent_decode_ctas(const PlanConfig& cfg, int sms, double dec_bytes, double row_pieces,
@@ -369,8 +477,12 @@ int build_plan(const PlanConfig& cfg, const int32_t* qo, const int32_t* kv, cons
   View views[3];
   {
     int rc;
-    if (cfg.cut_rows) {
-      // row lists of head_dim 256 and of the 8-bit cache are cut exactly like the decode list: the
+    if (cfg.row_item_tiles > 0) {
+      rc = build_cost_view(cfg, row_units_full, row_cap, fixed_grid, views[0], err);
+      if (rc != FE_OK) return rc;
+      rc = build_cost_view(cfg, row_units_causal, row_cap, fixed_grid, views[1], err);
+    } else if (cfg.cut_rows) {
+      // head_dim 256 row lists are cut exactly like the decode list: the
       // tcgen05 kernel's time per key tile hardly depends on how many of an
       // item's 128 rows are valid, so equal tile counts per CTA balance it,
       // at the price of up to one split unit per CTA boundary (pieces of at

@@ -81,7 +81,9 @@ struct PlanConfig {
   int dec_heads;              // KV heads per decode item: gcd(hkv, 8)
   int row_group_blocks;       // 16-row blocks per row-mode item (8 = one 128-row tcgen05 tile)
   bool row_split;             // row-mode key ranges may be split across CTAs
-  bool cut_rows;              // row lists are cut exactly, as the decode list (head_dim 256, 8-bit)
+  bool cut_rows;              // row items' key ranges are cut across CTAs (head_dim 256, 8-bit)
+  int row_tile;               // 8-bit row lists: 16-key pieces per tile of the kernel,
+  int row_item_tiles;         // and an item's fixed cost in tiles (0: cut by keys alone)
   int elem_bytes;             // bytes of a cached element
   int dec_min_tiles;          // fewest key tiles per CTA of the decode list, while CTAs are left
   int max_items;              // work-item capacity
