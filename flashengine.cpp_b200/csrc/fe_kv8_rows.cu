@@ -66,11 +66,14 @@ struct Cfg {
   static constexpr int kQBox = kM * 128;               // 128 rows x 128 codes
   static constexpr int kQPart = kBoxes * kQBox;
   static constexpr int kQBytes = kParts * kQPart;
-  // Raw V waits longest (for its load, then for the conversion): four stages
-  // where they fit. One query buffer: the next item's rows are converted while
-  // the softmax finishes the last tiles, whose S no longer needs it.
-  static constexpr int kKStages = D == 256 && kHalf ? 2 : 3;
-  static constexpr int kV8Stages = D == 128 ? (kHalf ? 3 : 4) : (kHalf ? 1 : 2);
+  // What the 208 KiB of operands hold: two f16 V tiles, the query parts (twice
+  // for bf16 with 128 dims: the next item's rows are converted while this
+  // one's tiles run; with one buffer, while the softmax finishes the last
+  // tiles, whose S no longer needs it) and raw tiles, of which V's wait longer
+  // (for their load, then for the conversion).
+  static constexpr int kQBufs = D == 128 && !kHalf ? 2 : 1;
+  static constexpr int kKStages = D == 128 ? (kHalf ? 3 : 2) : (kHalf ? 2 : 3);
+  static constexpr int kV8Stages = D == 128 ? 3 : (kHalf ? 1 : 2);
   // raw tiles: [8-key group][box][8 rows x 128 B]; f16 V: [8-key group][64-dim
   // box][8 rows x 128 B]; all in 128-byte swizzle
   static constexpr int kPiece8 = kTileTokens * D;
@@ -78,15 +81,15 @@ struct Cfg {
   static constexpr int kTile8 = kN * D;
   static constexpr int kGroup16 = 16 * D;
   static constexpr int kTile16 = 2 * kTile8;
-  static constexpr int kOffK = kQBytes;
+  static constexpr int kOffK = kQBufs * kQBytes;
   static constexpr int kOffV8 = kOffK + kKStages * kTile8;
   static constexpr int kOffV16 = kOffV8 + kV8Stages * kTile8;
   static constexpr int kOffMax = kOffV16 + kV16Stages * kTile16;  // [tile parity][row]
   static constexpr int kOffSum = kOffMax + 2 * kM * 4;            // [item parity][group][row]
-  static constexpr int kOffRow = kOffSum + 2 * 2 * kM * 4;        // [row] score factors
-  static constexpr int kOffExp = kOffRow + kM * 4;            // [ring][8] float4
+  static constexpr int kOffRow = kOffSum + 2 * 2 * kM * 4;        // [Q buffer][row] score factors
+  static constexpr int kOffExp = kOffRow + 2 * kM * 4;            // [ring][8] float4
   static constexpr int kOffBar = kOffExp + kExpRing * 8 * 16;
-  static constexpr int kNumBars = 1 + 1 + 1 + 1 + 2 * kKStages + 2 * kV8Stages + 2 * kV16Stages +
+  static constexpr int kNumBars = 2 + 2 + 1 + 1 + 2 * kKStages + 2 * kV8Stages + 2 * kV16Stages +
                                   kSlots + kSlots + kSlots + kExpRing + 8 + 1;
   static constexpr int kSmem = kOffBar + kNumBars * 8 + 32;
   static constexpr uint32_t kOCol = D == 128 ? kSlots * kN : 256;
@@ -136,9 +139,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   const AttnArgs<T>& a = ka.a;
   extern __shared__ __align__(16) uint8_t smem[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
-  uint64_t* q_full = bars;                        // an item's query parts written
-  uint64_t* q_empty = q_full + 1;                 // its S done, its row factors read
-  uint64_t* o_free = q_empty + 1;
+  uint64_t* q_full = bars;                        // [buffer] an item's query parts written
+  uint64_t* q_empty = q_full + 2;                 // [buffer] its S done, its row factors read
+  uint64_t* o_free = q_empty + 2;
   uint64_t* l_done = o_free + 1;
   uint64_t* k_full = l_done + 1;
   uint64_t* k_empty = k_full + kKStages;
@@ -176,8 +179,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 
   if (threadIdx.x == 0) {
-    mbar_init(q_full, 4);   // one arrival per converter warp
-    mbar_init(q_empty, 9);  // the S issuer's commit, the softmax warps
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&q_full[b], 4);   // one arrival per converter warp
+      mbar_init(&q_empty[b], 9);  // the S issuer's commit, the softmax warps
+    }
     mbar_init(o_free, 256);
     mbar_init(l_done, 256);
     for (int s = 0; s < kKStages; ++s) {
@@ -304,7 +309,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           const WorkItem w = items[it];
           const int ntiles = (w.kt1 - w.kt0 + kPieces - 1) / kPieces;
           if (warp == kSWarp) {
-            if (!wait_or_abort(q_full, unit & 1u, flags, aborted)) break;
+            const int qb = unit % C::kQBufs;
+            if (!wait_or_abort(&q_full[qb], (unit / C::kQBufs) & 1u, flags, aborted)) break;
+            const uint64_t q_desc = q_desc0 + uint64_t((qb * C::kQBytes) >> 4);
             for (int t = 0; t < ntiles && !aborted; ++t, ++n) {
               const int slot = n % kSlots;
               const uint32_t st = n % kKStages;
@@ -318,14 +325,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int kk = 0; kk < D / 32; ++kk) {
                   const int box = kk >> 2, ko = (kk & 3) * 32;
                   mma_f8_ss(tmem + slot * kN,
-                            q_desc0 + uint64_t((part * C::kQPart + box * C::kQBox + ko) >> 4),
+                            q_desc + uint64_t((part * C::kQPart + box * C::kQBox + ko) >> 4),
                             k_desc + uint64_t((box * 1024 + ko) >> 4), idesc_s,
                             part + kk > 0 ? 1u : 0u);
                 }
               tc::commit(&s_full[slot]);
               tc::commit(&k_empty[st]);
             }
-            if (!aborted) tc::commit(q_empty);
+            if (!aborted) tc::commit(&q_empty[qb]);
           } else {
             for (int t = 0; t < ntiles && !aborted; ++t, ++n) {
               const int slot = n % kSlots;
@@ -367,8 +374,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int qc = lane % kLanes;  // 16 elements, or codes of a part
       const int q_r0 = (warp - kConvWarp) * 32 + lane / kLanes;
       const int q_odd = (qc >> 2) & 1;  // odd boxes second chunk first: no bank conflicts
-      auto q_at = [&](int r, int k) {
-        return smem + (k >> 3) * C::kQBox + (r >> 3) * 1024 +
+      auto q_at = [&](int u, int r, int k) {
+        return smem + (u % C::kQBufs) * C::kQBytes + (k >> 3) * C::kQBox + (r >> 3) * 1024 +
                (r & 7) * 128 + (((k & 7) ^ (r & 7)) << 4);
       };
       auto fetch_q = [&](int u) {
@@ -384,17 +391,17 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int x = 0; x < 2; ++x)
             asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
-                             smem_u32(q_at(r, 2 * qc + x))),
+                             smem_u32(q_at(u, r, 2 * qc + x))),
                          "l"(src + 8 * x), "r"(valid ? 16 : 0)
                          : "memory");
         }
       };
-      auto convert_q = [&]() {
+      auto convert_q = [&](int u) {
         asm volatile("cp.async.wait_all;" ::: "memory");
 #pragma unroll 2
         for (int r = q_r0; r < (q_r0 | 31) + 1; r += kStep) {
-          uint4 x = *reinterpret_cast<const uint4*>(q_at(r, 2 * qc + q_odd));
-          uint4 y = *reinterpret_cast<const uint4*>(q_at(r, 2 * qc + 1 - q_odd));
+          uint4 x = *reinterpret_cast<const uint4*>(q_at(u, r, 2 * qc + q_odd));
+          uint4 y = *reinterpret_cast<const uint4*>(q_at(u, r, 2 * qc + 1 - q_odd));
           if (q_odd) {
             const uint4 z = x;
             x = y;
@@ -412,7 +419,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int e = kv8_query_exp(amax);
           // a row that holds an infinity has no defined softmax
           const float up = amax == INFINITY ? NAN : exp_scale(254 - e);
-          if (qc == 0) row_f[r] = exp_scale(e) * a.scale_log2;
+          if (qc == 0) row_f[(u % C::kQBufs) * kM + r] = exp_scale(e) * a.scale_log2;
           uint32_t part[C::kParts][4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -424,12 +431,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           __syncwarp();  // every lane of the row has read its elements
 #pragma unroll
           for (int k = 0; k < C::kParts; ++k)
-            *reinterpret_cast<uint4*>(q_at(r, qc) + k * C::kQPart) =
+            *reinterpret_cast<uint4*>(q_at(u, r, qc) + k * C::kQPart) =
                 make_uint4(part[k][0], part[k][1], part[k][2], part[k][3]);
         }
         tc::fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(q_full);
+        if (lane == 0) mbar_arrive(&q_full[u % C::kQBufs]);
       };
       // A thread's part of a V tile: chunk vc (16 codes) of rows vr, vr +
       // kRowStep, ..., whose addresses are constants apart. Codes 16 vc ..
@@ -448,15 +455,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int at0 = ((((2 * vc) & 7) + odd) ^ (vr & 7)) << 4;
       const int at1 = ((((2 * vc) & 7) + 1 - odd) ^ (vr & 7)) << 4;
       fetch_q(0);
-      convert_q();
+      convert_q(0);
       uint32_t n = 0;
       for (int u = 0; it0 + u < it1 && !aborted; ++u) {
         const WorkItem w = items[it0 + u];
         const SeqInfo si = seqs[w.seq];
         const int npieces = w.kt1 - w.kt0;
         const int ntiles = (npieces + kPieces - 1) / kPieces;
-        // the next item's queries: fetched as soon as the last S has read this
-        // item's, converted a tile later, or when this item's V is done
+        // the next item's queries: fetched as soon as their buffer is free,
+        // converted a tile later, or when this item's V is done
         enum { kWanted, kFetched, kDone } next = it0 + u + 1 < it1 ? kWanted : kDone;
         for (int t = 0; t < ntiles; ++t, ++n) {
           const uint32_t s8 = n % kV8Stages, s16 = n % kV16Stages;
@@ -491,19 +498,22 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_arrive(&v16_full[s16]);
           }
           if (next == kFetched) {
-            convert_q();
+            convert_q(u + 1);
             next = kDone;
-          } else if (next == kWanted && __all_sync(0xffffffffu, mbar_test(q_empty, u & 1u))) {
+          } else if (next == kWanted && __all_sync(0xffffffffu, mbar_test(&q_empty[(u + 1) % C::kQBufs],
+                                                   (((u + 1) / C::kQBufs) & 1u) ^ 1u))) {
             fetch_q(u + 1);
             next = kFetched;
           }
         }
         if (aborted) break;
         if (next == kWanted) {
-          if (!wait_warp(q_empty, u & 1u, flags, aborted)) break;
+          if (!wait_warp(&q_empty[(u + 1) % C::kQBufs], (((u + 1) / C::kQBufs) & 1u) ^ 1u, flags,
+                         aborted))
+            break;
           fetch_q(u + 1);
         }
-        if (next != kDone) convert_q();
+        if (next != kDone) convert_q(u + 1);
       }
       if (aborted && lane == 0) raise_device_error(a.err, FE_DEVERR_TIMEOUT);
     }
@@ -530,10 +540,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       // keys this row sees in this item
       int lim = (causal && row_valid) ? si.length - si.qrows + p / G + 1 : si.length;
       lim = min(lim, w.kt1 * kTileTokens);
-      if (!wait_warp(q_full, unit & 1u, flags, aborted)) break;
-      const float rf = row_f[r];
+      const int qb = unit % C::kQBufs;
+      if (!wait_warp(&q_full[qb], (unit / C::kQBufs) & 1u, flags, aborted)) break;
+      const float rf = row_f[qb * kM + r];
       __syncwarp();
-      if (lane == 0) mbar_arrive(q_empty);
+      if (lane == 0) mbar_arrive(&q_empty[qb]);
       // the maximum this group's weight sum l refers to
       float m_used = -INFINITY, l = 0.f;
       for (int j = (gi ^ n0) & 1; j < ntiles; j += 2) {
