@@ -19,7 +19,7 @@
 //    softmax warps, which are what bounds this kernel, against the one that f16
 //    takes.
 //
-// One persistent CTA per SM, sixteen warps. An item is 128 packed query rows
+// One persistent CTA per SM, twenty warps. An item is 128 packed query rows
 // (row p = query row p / G, head kvh*G + p % G) of one sequence and KV head
 // against a range of keys, in tiles of 128 keys (64 for head_dim 256).
 //  warps 0-7   softmax, two groups of four warps, a thread per packed row; the
@@ -31,9 +31,9 @@
 //  warp 8/11   producers of K (with the tiles' scale exponents) and of V.
 //  warp 9      issues S into one of three TMEM slots; owns TMEM.
 //  warp 10     issues O += W V once the tile's group wrote W over the slot.
-//  warps 12-15 convert: V tiles to f16 (rows past the end become zeros, so
-//              nothing that lies there reaches O), and the next item's query
-//              rows to their parts.
+//  warps 12-15 convert V tiles to f16 (rows past the end become zeros, so
+//              nothing that lies there reaches O).
+//  warps 16-19 split the next items' query rows into their parts.
 // All hand-offs are mbarriers; every wait is bounded.
 #include <mutex>
 #include <type_traits>
@@ -46,8 +46,9 @@
 namespace fe {
 namespace {
 
-constexpr int kThreads = 16 * 32;
-constexpr int kKWarp = 8, kSWarp = 9, kPvWarp = 10, kVWarp = 11, kConvWarp = 12;
+constexpr int kThreads = 20 * 32;
+constexpr int kKWarp = 8, kSWarp = 9, kPvWarp = 10, kVWarp = 11, kConvWarp = 12,
+              kQWarp = 16;
 constexpr int kSlots = 3;      // S / W slots in TMEM
 constexpr int kV16Stages = 2;  // V tiles in f16
 constexpr int kExpRing = 8;    // tiles of scale factors; K runs at most 6 ahead
@@ -360,34 +361,38 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc::commit(drain);
         wait_bounded_short(drain, 0, flags + 1);
       }
-    } else {
-      // ---------------------------------------------------------- converters
-      const int tid = threadIdx.x - kConvWarp * 32;
-      const int G = a.G;
-      // Query rows of item `u` (the CTA's u-th): D / 16 lanes a row, 16
-      // elements each. fetch_q copies the 16-bit rows into the buffer (zeros
-      // past the sequence), 16-byte chunk k of row r to position k % 8 (swizzled)
-      // of box k / 8; convert_q replaces a row by its parts in place (the row
+    } else if (warp >= kQWarp) {
+      // ------------------------------------------------------ query conversion
+      // Rows of the CTA's u-th item: D / 16 lanes a row, 16 elements each.
+      // fetch_q copies the 16-bit rows into the item's buffer (zeros past the
+      // sequence), 16-byte chunk k of row r to position k % 8 (swizzled) of
+      // box k / 8; convert_q replaces a row by its parts in place (the row
       // takes as many bytes as two of them), and sets the row's factor from
       // products to base-2 scores.
+      const int G = a.G, nitems = it1 - it0;
       constexpr int kLanes = D / 16, kStep = 32 / kLanes;
       const int qc = lane % kLanes;  // 16 elements, or codes of a part
-      const int q_r0 = (warp - kConvWarp) * 32 + lane / kLanes;
+      const int q_r0 = (warp - kQWarp) * 32 + lane / kLanes;
       const int q_odd = (qc >> 2) & 1;  // odd boxes second chunk first: no bank conflicts
+      const int step_row = kStep / G, step_head = kStep % G;
       auto q_at = [&](int u, int r, int k) {
         return smem + (u % C::kQBufs) * C::kQBytes + (k >> 3) * C::kQBox + (r >> 3) * 1024 +
                (r & 7) * 128 + (((k & 7) ^ (r & 7)) << 4);
       };
-      auto fetch_q = [&](int u) {
-        const WorkItem w = items[it0 + u];
-        const SeqInfo si = seqs[w.seq];
+      auto fetch_q = [&](int u, const WorkItem& w, const SeqInfo& si) {
+        int row = (w.rb0 * kRowBlock + q_r0) / G, head = (w.rb0 * kRowBlock + q_r0) % G;
+        const T* base =
+            a.q + (static_cast<int64_t>(si.q_row0) * a.hq + w.kvh * G) * D + 16 * qc;
 #pragma unroll 2
         for (int r = q_r0; r < (q_r0 | 31) + 1; r += kStep) {
-          const int p = w.rb0 * kRowBlock + r;
-          const bool valid = p < si.qrows * G;
-          const int row = valid ? p / G : 0, head = valid ? p - row * G : 0;
-          const T* src =
-              a.q + (static_cast<int64_t>(si.q_row0 + row) * a.hq + w.kvh * G + head) * D + 16 * qc;
+          const bool valid = row < si.qrows;
+          const T* src = valid ? base + (static_cast<int64_t>(row) * a.hq + head) * D : a.q;
+          row += step_row;
+          head += step_head;
+          if (head >= G) {
+            head -= G;
+            ++row;
+          }
 #pragma unroll
           for (int x = 0; x < 2; ++x)
             asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
@@ -438,6 +443,21 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&q_full[u % C::kQBufs]);
       };
+      WorkItem w = items[it0];
+      SeqInfo si = seqs[w.seq];
+      for (int u = 0; u < nitems && !aborted; ++u) {
+        if (!wait_warp(&q_empty[u % C::kQBufs], ((u / C::kQBufs) & 1u) ^ 1u, flags, aborted)) break;
+        fetch_q(u, w, si);
+        if (u + 1 < nitems) {  // in flight with this item's rows
+          w = items[it0 + u + 1];
+          si = seqs[w.seq];
+        }
+        convert_q(u);
+      }
+      if (aborted && lane == 0) raise_device_error(a.err, FE_DEVERR_TIMEOUT);
+    } else {
+      // ---------------------------------------------------------- V conversion
+      const int tid = threadIdx.x - kConvWarp * 32;
       // A thread's part of a V tile: chunk vc (16 codes) of rows vr, vr +
       // kRowStep, ..., whose addresses are constants apart. Codes 16 vc ..
       // become chunks 2 vc and 2 vc + 1 of the f16 rows (64-dim box vc / 4);
@@ -454,17 +474,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           smem + C::kOffV16 + (vr >> 3) * C::kGroup16 + (vc >> 2) * 1024 + (vr & 7) * 128;
       const int at0 = ((((2 * vc) & 7) + odd) ^ (vr & 7)) << 4;
       const int at1 = ((((2 * vc) & 7) + 1 - odd) ^ (vr & 7)) << 4;
-      fetch_q(0);
-      convert_q(0);
       uint32_t n = 0;
       for (int u = 0; it0 + u < it1 && !aborted; ++u) {
         const WorkItem w = items[it0 + u];
         const SeqInfo si = seqs[w.seq];
         const int npieces = w.kt1 - w.kt0;
         const int ntiles = (npieces + kPieces - 1) / kPieces;
-        // the next item's queries: fetched as soon as their buffer is free,
-        // converted a tile later, or when this item's V is done
-        enum { kWanted, kFetched, kDone } next = it0 + u + 1 < it1 ? kWanted : kDone;
         for (int t = 0; t < ntiles; ++t, ++n) {
           const uint32_t s8 = n % kV8Stages, s16 = n % kV16Stages;
           if (!wait_warp(&v8_full[s8], (n / kV8Stages) & 1u, flags, aborted)) break;
@@ -497,23 +512,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_arrive(&v8_empty[s8]);
             mbar_arrive(&v16_full[s16]);
           }
-          if (next == kFetched) {
-            convert_q(u + 1);
-            next = kDone;
-          } else if (next == kWanted && __all_sync(0xffffffffu, mbar_test(&q_empty[(u + 1) % C::kQBufs],
-                                                   (((u + 1) / C::kQBufs) & 1u) ^ 1u))) {
-            fetch_q(u + 1);
-            next = kFetched;
-          }
         }
-        if (aborted) break;
-        if (next == kWanted) {
-          if (!wait_warp(&q_empty[(u + 1) % C::kQBufs], (((u + 1) / C::kQBufs) & 1u) ^ 1u, flags,
-                         aborted))
-            break;
-          fetch_q(u + 1);
-        }
-        if (next != kDone) convert_q(u + 1);
       }
       if (aborted && lane == 0) raise_device_error(a.err, FE_DEVERR_TIMEOUT);
     }
@@ -556,32 +555,25 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!wait_warp(&s_full[slot], (n / kSlots) & 1u, flags, aborted)) break;
         tc::fence_after_sync();
         const int tkey = (w.kt0 + kPieces * j) * kTileTokens;
-        // Scores pass twice through registers, 64 keys at a time: for the
+        // Scores pass twice through registers, 32 keys at a time: for the
         // maximum, and for the weights. (All 128 at once need 200 registers
-        // and twice the code; the instruction fetch of the kernel's eight kinds
-        // of warps then bounds it.)
+        // and four times the code; the instruction fetch of the kernel's many
+        // kinds of warps then bounds it.)
         float mx = -INFINITY;
 #pragma unroll 1
-        for (int h = 0; h < kN; h += 64) {
-          float s[64];
-#pragma unroll
-          for (int c = 0; c < 64; c += 32)
-            tc::ld_32x32b_x32(s_addr + h + c, *reinterpret_cast<uint32_t(*)[32]>(&s[c]));
+        for (int h = 0; h < kN; h += 32) {
+          float s[32];
+          tc::ld_32x32b_x32(s_addr + h, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
           tc::wait_ld();
-          if (tkey + h + 64 > lim) {
+          if (__any_sync(0xffffffffu, tkey + h + 32 > lim)) {
             // hidden keys become -inf, in TMEM too
 #pragma unroll
-            for (int c = 0; c < 64; ++c)
+            for (int c = 0; c < 32; ++c)
               if (tkey + h + c >= lim) s[c] = -INFINITY;
-          }
-          if (__any_sync(0xffffffffu, tkey + h + 64 > lim)) {
-#pragma unroll
-            for (int c = 0; c < 64; c += 32)
-              tc::st_32x32b_x32(s_addr + h + c, *reinterpret_cast<uint32_t(*)[32]>(&s[c]));
-            tc::wait_st();
+            tc::st_32x32b_x32(s_addr + h, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
           }
 #pragma unroll
-          for (int b = 0; b < 4; ++b) {
+          for (int b = 0; b < 2; ++b) {
             const float* x = s + 16 * b;
             const float4 f = fac[h / 16 + b];
             const float m0 = fmax3(x[0], x[1], x[2]), m1 = fmax3(x[3], x[4], x[5]),
@@ -590,6 +582,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             mx = fmaxf(mx, fmaf(fmaxf(fmax3(m0, m1, m2), fmax3(m3, m4, x[15])), f.x * rf, f.y));
           }
         }
+        tc::wait_st();
         // the maximum so far comes from the tile before and goes to the next;
         // it moves only when it grows by more than 2^8 (or from nothing)
         float m_prev = -INFINITY;
@@ -626,38 +619,32 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         const float m_sub = (m_now == -INFINITY ? 0.f : m_now) - kBias;
 #pragma unroll 1
-        for (int h = 0; h < kN; h += 64) {
-          float s[64];
-#pragma unroll
-          for (int c = 0; c < 64; c += 32)
-            tc::ld_32x32b_x32(s_addr + h + c, *reinterpret_cast<uint32_t(*)[32]>(&s[c]));
+        for (int h = 0; h < kN; h += 32) {
+          float s[32];
+          tc::ld_32x32b_x32(s_addr + h, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
           tc::wait_ld();
+          uint32_t pk[16];
 #pragma unroll
-          for (int h2 = 0; h2 < 2; ++h2) {
-            uint32_t pk[16];
+          for (int b = 0; b < 2; ++b) {
+            const float4 f = fac[h / 16 + b];
+            const float fs = f.x * rf, off = f.y - m_sub;
+            const float2 sc2 = make_float2(fs, fs), off2 = make_float2(off, off);
+            float2 sum0 = make_float2(0.f, 0.f), sum1 = sum0;
 #pragma unroll
-            for (int b2 = 0; b2 < 2; ++b2) {
-              const int b = 2 * h2 + b2;
-              const float4 f = fac[h / 16 + b];
-              const float fs = f.x * rf, off = f.y - m_sub;
-              const float2 sc2 = make_float2(fs, fs), off2 = make_float2(off, off);
-              float2 sum0 = make_float2(0.f, 0.f), sum1 = sum0;
-#pragma unroll
-              for (int e = 0; e < 8; ++e) {
-                const float2 x =
-                    fma2(make_float2(s[16 * b + 2 * e], s[16 * b + 2 * e + 1]), sc2, off2);
-                const float2 pp = make_float2(fast_exp2(x.x), fast_exp2(x.y));
-                if (e & 1)
-                  sum1 = add2(sum1, pp);
-                else
-                  sum0 = add2(sum0, pp);
-                pk[8 * b2 + e] = pack2<__half>(pp.x, pp.y);
-              }
-              l = fmaf((sum0.x + sum0.y) + (sum1.x + sum1.y), f.z, l);
+            for (int e = 0; e < 8; ++e) {
+              const float2 x =
+                  fma2(make_float2(s[16 * b + 2 * e], s[16 * b + 2 * e + 1]), sc2, off2);
+              const float2 pp = make_float2(fast_exp2(x.x), fast_exp2(x.y));
+              if (e & 1)
+                sum1 = add2(sum1, pp);
+              else
+                sum0 = add2(sum0, pp);
+              pk[8 * b + e] = pack2<__half>(pp.x, pp.y);
             }
-            // (weights of 64 keys take the columns of 32: never ones still to be read)
-            tc::st_32x32b_x16(s_addr + h / 2 + 16 * h2, pk);
+            l = fmaf((sum0.x + sum0.y) + (sum1.x + sum1.y), f.z, l);
           }
+          // (weights of 32 keys take 16 columns: never ones still to be read)
+          tc::st_32x32b_x16(s_addr + h / 2, pk);
         }
         tc::wait_st();
         tc::fence_before_sync();
