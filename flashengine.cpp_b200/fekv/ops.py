@@ -20,10 +20,16 @@ from ._lib import FE_DTYPE_BF16, FE_DTYPE_F16, FeError, check
 _P = ctypes.c_void_p
 
 
-def _torch():
-    import torch
+_TORCH = None
 
-    return torch
+
+def _torch():
+    global _TORCH
+    if _TORCH is None:
+        import torch
+
+        _TORCH = torch
+    return _TORCH
 
 
 def _ptr(t):
@@ -369,10 +375,10 @@ def _kv8_rows(name, t, dtype, shape):
     """Address of a contiguous CUDA tensor of this dtype and shape."""
     if t is None:
         raise ValueError(f"{name} is missing")
-    if t.dtype is not dtype or t.shape != shape or not t.is_cuda or not t.is_contiguous():
-        raise ValueError(f"{name}: expected a contiguous {dtype} CUDA tensor {tuple(shape)}, got "
-                         f"{t.dtype} {tuple(t.shape)} {tuple(t.stride())} on {t.device}")
-    return t.data_ptr()
+    if t.dtype is dtype and t.shape == shape and t.is_cuda and t.is_contiguous():
+        return t.data_ptr()
+    raise ValueError(f"{name}: expected a contiguous {dtype} CUDA tensor {tuple(shape)}, got "
+                     f"{t.dtype} {tuple(t.shape)} {tuple(t.stride())} on {t.device}")
 
 
 def append_kv8(q, k, v, kpool, vpool, slots, pos=None, cache=None, q_out=None, stream=None):
@@ -383,29 +389,39 @@ def append_kv8(q, k, v, kpool, vpool, slots, pos=None, cache=None, q_out=None, s
     rotates nothing. Rows of one 16-slot block must be adjacent and in order."""
     torch = _torch()
     shape, dt = k.shape, k.dtype
-    if len(shape) != 3 or kpool.shape != vpool.shape or shape[1:] != kpool.shape[1:]:
-        raise ValueError(f"k {tuple(shape)} and pools {kpool.shape}, {vpool.shape} do not fit")
+    pool = kpool.shape
+    if len(shape) != 3 or pool != vpool.shape or shape[1:] != pool[1:]:
+        raise ValueError(f"k {tuple(shape)} and pools {pool}, {vpool.shape} do not fit")
     rows, hkv, dim = shape
-    kp, vp = _kv8_rows("k", k, dt, shape), _kv8_rows("v", v, dt, shape)
-    hq = 0
-    qp = op = None
+    if dt is torch.bfloat16:
+        code = FE_DTYPE_BF16
+    elif dt is torch.float16:
+        code = FE_DTYPE_F16
+    else:
+        raise ValueError(f"k: expected float16 or bfloat16, got {dt}")
+    if not (k.is_cuda and k.is_contiguous()):
+        raise ValueError("k: expected a contiguous CUDA tensor")
+    vp = _kv8_rows("v", v, dt, shape)
+    hq = rot = most = 0
+    qp = op = pp = cp = None
     if q is not None:
         qs = q.shape
         hq = qs[1] if len(qs) == 3 else -1
-        qp = _kv8_rows("q", q, dt, (rows, hq, dim))
-        op = qp if q_out is None else _kv8_rows("q_out", q_out, dt, (rows, hq, dim))
+        qp = op = _kv8_rows("q", q, dt, (rows, hq, dim))
+        if q_out is not None:
+            op = _kv8_rows("q_out", q_out, dt, qs)
     sp = _kv8_rows("slots", slots, torch.int64, (rows,))
-    rot = most = 0
-    pp = cp = None
     if cache is not None:
-        most, rot = cache.shape
+        cs = cache.shape
+        most, rot = cs
         if rot:
             pp = _kv8_rows("pos", pos, torch.int64, (rows,))
-            cp = _kv8_rows("cache", cache, torch.float32, (most, rot))
-    check(_lib.load().fe_kv8_append(qp, op, kp, vp, kpool.codes_ptr, vpool.codes_ptr,
-                                    kpool.exps_ptr, vpool.exps_ptr, sp, pp, cp, rows, hq, hkv, dim,
-                                    rot, most, dtype_code(k), kpool.shape[0],
-                                    _kv8_stream(stream)), "append_kv8")
+            cp = _kv8_rows("cache", cache, torch.float32, cs)
+    rc = _lib.load().fe_kv8_append(qp, op, k.data_ptr(), vp, kpool.codes_ptr, vpool.codes_ptr,
+                                   kpool.exps_ptr, vpool.exps_ptr, sp, pp, cp, rows, hq, hkv, dim,
+                                   rot, most, code, pool[0], _kv8_stream(stream))
+    if rc:
+        check(rc, "append_kv8")
 
 
 def gather_kv8(pool, out, kv, pages, last, row_offset, max_len, page, stream=None):
@@ -433,13 +449,11 @@ def copy_blocks_kv8(k_pools, v_pools, src, dst, ntok, page, stream=None):
     if n == 0:
         return
     shape = k_pools[0].shape
-    for side in (k_pools, v_pools):
-        for p in side:
-            if p.shape != shape:
-                raise ValueError("the layers' pools differ in shape")
-    arrays = [array.array("Q", ptrs) for ptrs in
-              ([p.codes_ptr for p in k_pools], [p.codes_ptr for p in v_pools],
-               [p.exps_ptr for p in k_pools], [p.exps_ptr for p in v_pools])]
+    ptrs = [[p.codes_ptr for p in side if p.shape == shape] for side in (k_pools, v_pools)] + \
+        [[p.exps_ptr for p in side] for side in (k_pools, v_pools)]
+    if len(ptrs[0]) != n or len(ptrs[1]) != n:
+        raise ValueError("the layers' pools differ in shape")
+    arrays = [array.array("Q", p) for p in ptrs]
     check(_lib.load().fe_kv8_copy_blocks(*[a.buffer_info()[0] for a in arrays], n, src.data_ptr(),
                                          dst.data_ptr(), ntok.data_ptr(), src.shape[0], page,
                                          shape[1], shape[2], shape[0] // page,
