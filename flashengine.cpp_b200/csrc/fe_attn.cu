@@ -584,20 +584,28 @@ int launch_lists(fe_attn_plan* p, int view, int grid_rows, int grid_dec, const v
   // split units of the decode list are merged by a second, dependent kernel
   int grid_merge = 0;
   if (grid_dec > 0) grid_merge = p->fixed_grid ? p->cfg.dec_grid_cap : h.n_groups[2];
-  // Merge CTAs per split unit: one warp per record row, 32 rows per CTA. The
-  // host plan knows its units' rows; a graph plan (fixed launch geometry) or
-  // a device-built plan takes the bound: H heads x 16 packed rows for the
-  // decode list, 128 rows for a row list.
-  auto merge_y = [&](int list) {
-    const int bound = list == 2 ? p->cfg.dec_heads * kRowBlock : 128;
-    const int n = (p->fixed_grid || p->device_planned) ? bound : p->last.split_rows[list];
-    return std::max(1, (n + 31) / 32);
-  };
   // split pieces of the row list (where its key ranges are cut across CTAs)
   // are merged by the merge kernel over that list
   const int grid_row_merge =
       !p->cfg.cut_rows || grid_rows == 0 ? 0
                                          : (p->fixed_grid ? p->cfg.grid_cap : h.n_groups[view]);
+  // Rows of a split unit's record: the host plan knows its units' rows; a
+  // graph plan (fixed launch geometry) or a device-built plan takes the bound:
+  // H heads x 16 packed rows for the decode list, 128 rows for a row list.
+  auto merge = [&](int list, int units, cudaStream_t on, bool pdl) -> int {
+    const bool bound = p->fixed_grid || p->device_planned;
+    const int rows =
+        bound ? (list == 2 ? p->cfg.dec_heads * kRowBlock : 128) : p->last.split_rows[list];
+    if (!p->kv8)  // one warp per record row, 32 rows per CTA
+      return decode_merge_launch(p->dtype, dim, list, args, units, std::max(1, (rows + 31) / 32),
+                                 on, pdl);
+    // pieces of a unit: under a fixed geometry what an even cut gives
+    const int even = list == 2 ? p->cfg.dec_grid_cap * p->cfg.dec_heads /
+                                     (p->cfg.hkv * std::max(1, h.batch)) + 1
+                               : 1;
+    return kv8_merge_launch(p->dtype, dim, list, args, units, std::max(1, rows),
+                            bound ? even : p->last.split_pieces[list], on, pdl);
+  };
   // A mixed step planned side by side (the two lists' grids sum to the SMs)
   // forks: the row kernel runs on the plan's side stream while the decode
   // kernel and its merge run on `stream`, which then waits for the side.
@@ -616,22 +624,17 @@ int launch_lists(fe_attn_plan* p, int view, int grid_rows, int grid_dec, const v
     // kernel needs while it waits).
     if (grid_rows > 0 && fork) {
       int rc = rows(rs);
-      if (rc == FE_OK)
-        rc = decode_merge_launch(p->dtype, dim, view, args, grid_row_merge, merge_y(view), rs,
-                                 false);
+      if (rc == FE_OK) rc = merge(view, grid_row_merge, rs, false);
       if (rc != FE_OK) return rc;
     }
     if (grid_dec > 0) {
       int rc = dec(s);
-      if (rc == FE_OK)
-        rc = decode_merge_launch(p->dtype, dim, 2, args, grid_merge, merge_y(2), s, !fork);
+      if (rc == FE_OK) rc = merge(2, grid_merge, s, !fork);
       if (rc != FE_OK) return rc;
     }
     if (grid_rows > 0 && !fork) {
       int rc = rows(s);
-      if (rc == FE_OK)
-        rc = decode_merge_launch(p->dtype, dim, view, args, grid_row_merge, merge_y(view), s,
-                                 true);
+      if (rc == FE_OK) rc = merge(view, grid_row_merge, s, true);
       return rc;
     }
     return FE_OK;

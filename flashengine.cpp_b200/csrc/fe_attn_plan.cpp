@@ -232,8 +232,9 @@ int build_cut_view(const PlanConfig& cfg, const std::vector<Unit>& units, int gr
 // them (queries, first scores, epilogue), so a cut by tiles alone gives the
 // CTAs of a step's many short items far more time than the others (a mixed
 // step took 314 us where this cut takes a third). The units are laid end to end
-// and cut into at most grid_cap pieces of equal cost, at whole tiles; a unit is
-// cut only into pieces of at least cfg.row_item_tiles tiles.
+// and cut into at most grid_cap pieces of equal cost, at whole tiles, in pieces
+// of at least kMinPiece tiles.
+constexpr int64_t kMinPiece = 4;
 int build_cost_view(const PlanConfig& cfg, const std::vector<Unit>& units, int grid_cap_in,
                     bool fixed_grid, View& v, std::string& err) {
   v = View{};
@@ -250,8 +251,8 @@ int build_cost_view(const PlanConfig& cfg, const std::vector<Unit>& units, int g
       while (left > 0) {
         int64_t take = std::min(left, room - ov);
         if (take < left) {  // a piece: both sides long enough, or none here
-          if (left - take < ov) take = left - ov;
-          if (take < ov) take = 0;
+          if (left - take < kMinPiece) take = left - kMinPiece;
+          if (take < kMinPiece) take = 0;
         }
         if (take <= 0) {
           if (room == budget) take = left;  // does not fit an empty CTA: whole
@@ -274,8 +275,8 @@ int build_cost_view(const PlanConfig& cfg, const std::vector<Unit>& units, int g
     total += big(u) + ov;
     most = std::max(most, big(u) + ov);
   }
-  // (below 2 ov no unit can be cut, and every budget would do)
-  int64_t lo = std::max<int64_t>(2 * ov, (total + grid_cap - 1) / grid_cap), hi = total + most;
+  // (below ov + kMinPiece no unit can be cut, and every budget would do)
+  int64_t lo = std::max<int64_t>(ov + kMinPiece, (total + grid_cap - 1) / grid_cap), hi = total + most;
   auto none = [](size_t, int64_t, int64_t, int64_t) {};
   while (lo < hi) {
     const int64_t mid = (lo + hi) / 2;
@@ -592,7 +593,10 @@ int build_plan(const PlanConfig& cfg, const int32_t* qo, const int32_t* kv, cons
   out.partial_floats = row_floats + views[2].partial_floats;
   for (int c = 0; c < 3; ++c)
     for (const auto& gi : views[c].groups)
-      if (gi.nsplit > 1) out.split_rows[c] = std::max(out.split_rows[c], gi.rows);
+      if (gi.nsplit > 1) {
+        out.split_rows[c] = std::max(out.split_rows[c], gi.rows);
+        out.split_pieces[c] = std::max(out.split_pieces[c], gi.nsplit);
+      }
   return FE_OK;
 }
 

@@ -104,6 +104,7 @@ struct PlanResult {
   int chunk_tiles = 0;
   int grid[3] = {0, 0, 0};    // CTAs per work list (0 = nothing to launch)
   int split_rows[3] = {0, 0, 0};  // most rows in one split unit's records, per list
+  int split_pieces[3] = {0, 0, 0};  // and most records of one unit
   int64_t kv_tokens = 0, partial_floats = 0;
   bool concurrent = false;  // decode and row kernels run side by side (grids sum to the SMs)
 };

@@ -635,7 +635,171 @@ int dispatch(int dim, int heads, const CUtensorMap& kmap, const CUtensorMap& vma
   }
 }
 
+// ---------------------------------------------------------------------------
+// Merge of split units' records (O[rows][D], m[rows], l[rows], as in
+// fe_decode.cu): out = sum 2^(m_i - M) O_i / sum 2^(m_i - M) l_i.
+// `per_row` warps of a block share a row, each taking every per_row-th piece
+// with up to eight O vectors in flight, and join through shared memory: one
+// long sequence has a record per CTA, and a warp that walked 128 of them alone
+// took longer than the attention (38 us for one sequence of 8192 keys against
+// 13). gridDim.x blocks stride over the units, gridDim.y over a unit's rows.
+// ---------------------------------------------------------------------------
+constexpr int kMergeWarps = 8;
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kMergeWarps * 32)
+    kv8_merge_kernel(const AttnArgs<T> a, int list, int per_row) {
+  constexpr int kV = D / 128;  // float4 per lane
+  __shared__ float4 part[kMergeWarps][32 * kV];
+  __shared__ float2 stat[kMergeWarps];
+  pdl_trigger();
+  // the metadata is older than the kernel that wrote the records
+  const MetaHeader* hdr = reinterpret_cast<const MetaHeader*>(a.meta);
+  const int n = hdr->n_groups[list];
+  const SplitGroup* groups = reinterpret_cast<const SplitGroup*>(a.meta + hdr->groups_off[list]);
+  const SeqInfo* seqs = reinterpret_cast<const SeqInfo*>(a.meta + hdr->seqs_off);
+  SplitGroup g{};
+  SeqInfo si{};
+  if (static_cast<int>(blockIdx.x) < n) {
+    g = groups[blockIdx.x];
+    if (g.nsplit >= 2) si = seqs[g.seq];
+  }
+  pdl_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int sub = warp % per_row, rows = kMergeWarps / per_row;
+  for (int u = blockIdx.x; u < n; u += gridDim.x) {
+    if (u != static_cast<int>(blockIdx.x)) {
+      g = groups[u];
+      if (g.nsplit >= 2) si = seqs[g.seq];
+    }
+    if (g.nsplit < 2) continue;  // placeholder ids of the row lists
+    const int rph = g.rows_per_head > 0 ? g.rows_per_head : si.qrows * a.G;
+    for (int r0 = blockIdx.y * rows; r0 < g.rows; r0 += gridDim.y * rows) {
+      const int r = r0 + warp / per_row;
+      float M = -INFINITY, L = 0.f;
+      float4 acc[kV];
+#pragma unroll
+      for (int v = 0; v < kV; ++v) acc[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (r < g.rows) {
+        const float* base = a.partials + g.part0;
+        // the warp's pieces, 32 at a time: sub, sub + per_row, ..
+        for (int s0 = sub; s0 < g.nsplit; s0 += 32 * per_row) {
+          const int s = s0 + lane * per_row;
+          float m = -INFINITY, l = 0.f;
+          if (s < g.nsplit) {
+            const float* rec = base + int64_t(s) * g.rec_floats;
+            m = __ldcg(rec + g.rows * D + r);
+            l = __ldcg(rec + g.rows * (D + 1) + r);
+          }
+          float top = m;
+#pragma unroll
+          for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+          const float M_new = fmaxf(M, top);
+          const float ref = M_new == -INFINITY ? 0.f : M_new;
+          const float old = fast_exp2(M - ref);  // 0 from nothing
+          const float w = fast_exp2(m - ref);
+          float lw = l * w;
+#pragma unroll
+          for (int o = 16; o; o >>= 1) lw += __shfl_xor_sync(0xffffffffu, lw, o);
+          L = fmaf(L, old, lw);
+          M = M_new;
+#pragma unroll
+          for (int v = 0; v < kV; ++v) {
+            acc[v].x *= old;
+            acc[v].y *= old;
+            acc[v].z *= old;
+            acc[v].w *= old;
+          }
+          const int count = min(32, (g.nsplit - s0 + per_row - 1) / per_row);
+#pragma unroll 8
+          for (int j = 0; j < count; ++j) {
+            const float* rec = base + int64_t(s0 + j * per_row) * g.rec_floats;
+            const float wj = __shfl_sync(0xffffffffu, w, j);
+#pragma unroll
+            for (int v = 0; v < kV; ++v) {
+              const float4 x =
+                  __ldcg(reinterpret_cast<const float4*>(rec + r * D + v * 128 + lane * 4));
+              acc[v].x = fmaf(x.x, wj, acc[v].x);
+              acc[v].y = fmaf(x.y, wj, acc[v].y);
+              acc[v].z = fmaf(x.z, wj, acc[v].z);
+              acc[v].w = fmaf(x.w, wj, acc[v].w);
+            }
+          }
+        }
+      }
+      if (per_row > 1) {
+#pragma unroll
+        for (int v = 0; v < kV; ++v) part[warp][v * 32 + lane] = acc[v];
+        if (lane == 0) stat[warp] = make_float2(M, L);
+        __syncthreads();
+        if (sub == 0) {
+          float top = M;
+          for (int k = 1; k < per_row; ++k) top = fmaxf(top, stat[warp + k].x);
+          const float ref = top == -INFINITY ? 0.f : top;
+          float w = fast_exp2(M - ref);
+          L *= w;
+#pragma unroll
+          for (int v = 0; v < kV; ++v)
+            acc[v] = make_float4(acc[v].x * w, acc[v].y * w, acc[v].z * w, acc[v].w * w);
+          for (int k = 1; k < per_row; ++k) {
+            w = fast_exp2(stat[warp + k].x - ref);
+            L = fmaf(stat[warp + k].y, w, L);
+#pragma unroll
+            for (int v = 0; v < kV; ++v) {
+              const float4 x = part[warp + k][v * 32 + lane];
+              acc[v].x = fmaf(x.x, w, acc[v].x);
+              acc[v].y = fmaf(x.y, w, acc[v].y);
+              acc[v].z = fmaf(x.z, w, acc[v].z);
+              acc[v].w = fmaf(x.w, w, acc[v].w);
+            }
+          }
+        }
+        __syncthreads();
+      }
+      if (sub == 0 && r < g.rows) {
+        const float inv = 1.f / L;
+        const int p = g.row0 + r % rph;
+        T* dst = a.out + (static_cast<int64_t>(si.q_row0 + p / a.G) * a.hq +
+                          (g.kvh + r / rph) * a.G + p % a.G) * D + lane * 4;
+#pragma unroll
+        for (int v = 0; v < kV; ++v)
+          store4<T>(dst + v * 128, acc[v].x * inv, acc[v].y * inv, acc[v].z * inv,
+                    acc[v].w * inv);
+      }
+    }
+  }
+}
+
+template <typename T>
+int merge_launch(int dim, int list, const AttnArgs<T>& a, int units, int rows, int pieces,
+                 cudaStream_t stream, bool pdl) {
+  // eight pieces a warp, where that leaves the GPU's warps enough rows
+  int per_row = 1;
+  while (per_row < kMergeWarps && pieces > 8 * per_row) per_row *= 2;
+  const int per_block = kMergeWarps / per_row;
+  const dim3 grid(units, (rows + per_block - 1) / per_block);
+  auto kernel = dim == kWideHeadDim ? kv8_merge_kernel<T, kWideHeadDim>
+                                    : kv8_merge_kernel<T, kHeadDim>;
+  if (pdl) {
+    FE_CUDA_TRY(launch_pdl(kernel, grid, dim3(kMergeWarps * 32), 0, stream, a, list, per_row));
+  } else {
+    kernel<<<grid, kMergeWarps * 32, 0, stream>>>(a, list, per_row);
+    FE_CUDA_TRY(cudaGetLastError());
+  }
+  return FE_OK;
+}
+
 }  // namespace
+
+int kv8_merge_launch(int dtype, int dim, int list, const void* args, int units, int rows,
+                     int pieces, cudaStream_t stream, bool pdl) {
+  if (units <= 0) return FE_OK;
+  if (dtype == FE_DTYPE_BF16)
+    return merge_launch(dim, list, *static_cast<const AttnArgs<__nv_bfloat16>*>(args), units, rows,
+                        pieces, stream, pdl);
+  return merge_launch(dim, list, *static_cast<const AttnArgs<__half>*>(args), units, rows, pieces,
+                      stream, pdl);
+}
 
 int kv8_decode_launch(int dtype, int dim, int heads, const CUtensorMap& kmap,
                       const CUtensorMap& vmap, const void* args, int grid, cudaStream_t stream) {

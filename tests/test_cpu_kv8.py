@@ -129,7 +129,7 @@ def test_attention_refusals():
 
 def test_row_lists_are_cut_and_cover_every_key():
     """Every (sequence, KV head, 128-row group) has its keys covered once, in
-    pieces of at least 16 tiles a CTA, and the pieces' records do not overlap."""
+    pieces at whole tiles, and the pieces' records do not overlap."""
     plan = fekv.HostKv8Plan(16, 4, 128, 16, 4, 600, True, 2000, grid_cap=296)
     lens, rows = [9000, 40, 700], [20, 40, 1]
     need = [-(-n // 16) for n in lens]
