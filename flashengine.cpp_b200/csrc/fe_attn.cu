@@ -261,7 +261,7 @@ PlanConfig make_config(int hq, int hkv, int dim, int page, int max_batch, int ma
   c.row_split = false;      // the tcgen05 kernel walks an item's whole key range
   c.cut_rows = dim == kWideHeadDim || kv8;
   c.elem_bytes = kv8 ? 1 : 2;
-  // (measured: 1.35 us a tile of 128 keys, 5.7 us an item beyond its tiles)
+  // (measured: 1.35 us a tile of the row kernel, 5 us an item beyond its tiles)
   c.row_tile = dim == kWideHeadDim ? 4 : 8;
   c.row_item_tiles = kv8 ? 4 : 0;
   // a step of the 8-bit decode kernel is two tiles: two steps, where a short
@@ -284,7 +284,13 @@ PlanConfig make_config(int hq, int hkv, int dim, int page, int max_batch, int ma
   c.hbm_gbs = 5800.f;
   c.dec_fixed_us = 10.f;
   c.row_piece_us = dim == kWideHeadDim ? 0.4f : 0.2f;
-  if (kv8) c.row_piece_us *= 0.6f;  // the 8-bit row kernel's measured rate
+  if (kv8) {
+    // the 8-bit kernels: 1.35 us a tile; with 50 GB/s per decode SM four mixed
+    // steps took 81, 48, 152 and 66 us, with 42 and 60: 82-88, 48-50, 161-190,
+    // 67-69
+    c.row_piece_us = 1.35f / c.row_tile;
+    c.dec_sm_gbs = 50.f;
+  }
   return c;
 }
 

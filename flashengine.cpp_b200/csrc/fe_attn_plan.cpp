@@ -460,6 +460,10 @@ int build_plan(const PlanConfig& cfg, const int32_t* qo, const int32_t* kv, cons
     for (const auto* list : {&row_units_full, &row_units_causal}) {
       double total = 0;
       for (const auto& u : *list) {
+        if (cfg.row_item_tiles > 0) {  // with the items' fixed part; no unit need stay whole
+          total += double(ceil_div(u.tiles, cfg.row_tile) + cfg.row_item_tiles) * cfg.row_tile;
+          continue;
+        }
         total += u.tiles;
         max_pieces = std::max(max_pieces, double(u.tiles));
       }

@@ -73,8 +73,8 @@ struct Cfg {
   // tiles, whose S no longer needs it) and raw tiles, of which V's wait longer
   // (for their load, then for the conversion).
   static constexpr int kQBufs = D == 128 && !kHalf ? 2 : 1;
-  static constexpr int kKStages = D == 128 ? (kHalf ? 3 : 2) : (kHalf ? 2 : 3);
-  static constexpr int kV8Stages = D == 128 ? 3 : (kHalf ? 1 : 2);
+  static constexpr int kKStages = D == 128 ? 3 : (kHalf ? 2 : 3);
+  static constexpr int kV8Stages = D == 128 ? (kHalf ? 3 : 2) : (kHalf ? 1 : 2);
   // raw tiles: [8-key group][box][8 rows x 128 B]; f16 V: [8-key group][64-dim
   // box][8 rows x 128 B]; all in 128-byte swizzle
   static constexpr int kPiece8 = kTileTokens * D;
