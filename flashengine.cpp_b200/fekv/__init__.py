@@ -12,8 +12,8 @@
 * :mod:`fekv.workloads` seeded synthetic configs C1..C5.
 """
 from . import metadata, workloads  # noqa: F401
-from ._lib import (FE_DTYPE_BF16, FE_DTYPE_F16, FeError, LIB_PATH, SHIM_PATH,  # noqa: F401
-                   load)
+from ._lib import (FE_DTYPE_BF16, FE_DTYPE_F16, FE_KV8_BLOCK as KV8_BLOCK,  # noqa: F401
+                   FeError, LIB_PATH, SHIM_PATH, load)
 from .ops import (AttentionPlan, HostKv8Plan, HostPlan, Kv8Plan, Kv8Pool,  # noqa: F401
                   accept, append_kv8, attention, clear_pages, copy_blocks,
                   copy_blocks_kv8, create_plan, destroy_plan, device_errors, fork_copies, gather, gather_kv8,
