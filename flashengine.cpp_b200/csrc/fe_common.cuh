@@ -113,6 +113,13 @@ __device__ __forceinline__ void mbar_arrive_expect_tx(uint64_t* bar, uint32_t by
                : "memory");
 }
 
+// Bytes that copies will bring to the current phase, without an arrival.
+__device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
+  asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)),
+               "r"(bytes)
+               : "memory");
+}
+
 // One poll of a phase; the hardware may suspend the thread for up to
 // `suspend_ns` while the phase is incomplete instead of returning at once.
 __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity,

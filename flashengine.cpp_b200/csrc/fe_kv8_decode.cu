@@ -538,15 +538,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             ok = false;
             break;
           }
-          if ((lane & ~1) == jj) {
-            uint64_t* dst = reinterpret_cast<uint64_t*>(exps + s * C::kExpBytes + (lane & 1) * 16);
-            dst[0] = e.k;
-            dst[1] = e.v;
-          }
-          __syncwarp();
+          // the loads first: the exponents of an item's first batch may still
+          // be on their way
           if (lane == 0) {
             const int tiles = min(kStepTiles, n - jj);
-            mbar_arrive_expect_tx(&full[s], tiles * 2 * C::kTileBytes);
+            mbar_expect_tx(&full[s], tiles * 2 * C::kTileBytes);
             uint8_t* st = stages + s * C::kStageBytes;
             tma_load_3d(st, &kmap, &full[s], 0, s0, box);
             if (tiles == 2) tma_load_3d(st + C::kTileBytes, &kmap, &full[s], 0, s1, box);
@@ -554,6 +550,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             tma_load_3d(st, &vmap, &full[s], 0, s0, box);
             if (tiles == 2) tma_load_3d(st + C::kTileBytes, &vmap, &full[s], 0, s1, box);
           }
+          if ((lane & ~1) == jj) {
+            uint64_t* dst = reinterpret_cast<uint64_t*>(exps + s * C::kExpBytes + (lane & 1) * 16);
+            dst[0] = e.k;
+            dst[1] = e.v;
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&full[s]);
           ++g;
           if (--before == 0 && it + 1 < it1) {
             head_slots(it + 1, next);
@@ -691,6 +694,18 @@ __global__ void __launch_bounds__(kMergeWarps * 32)
             m = __ldcg(rec + g.rows * D + r);
             l = __ldcg(rec + g.rows * (D + 1) + r);
           }
+          // the first O vectors are in flight with them
+          constexpr int kPre = 8 / kV;
+          const int count = min(32, (g.nsplit - s0 + per_row - 1) / per_row);
+          float4 pre[kPre][kV];
+#pragma unroll
+          for (int j = 0; j < kPre; ++j)
+            if (j < count) {
+              const float* rec = base + int64_t(s0 + j * per_row) * g.rec_floats;
+#pragma unroll
+              for (int v = 0; v < kV; ++v)
+                pre[j][v] = __ldcg(reinterpret_cast<const float4*>(rec + r * D + v * 128 + lane * 4));
+            }
           float top = m;
 #pragma unroll
           for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -710,20 +725,28 @@ __global__ void __launch_bounds__(kMergeWarps * 32)
             acc[v].z *= old;
             acc[v].w *= old;
           }
-          const int count = min(32, (g.nsplit - s0 + per_row - 1) / per_row);
-#pragma unroll 8
-          for (int j = 0; j < count; ++j) {
-            const float* rec = base + int64_t(s0 + j * per_row) * g.rec_floats;
-            const float wj = __shfl_sync(0xffffffffu, w, j);
+          auto add = [&](const float4 (&x)[kV], float wj) {
 #pragma unroll
             for (int v = 0; v < kV; ++v) {
-              const float4 x =
-                  __ldcg(reinterpret_cast<const float4*>(rec + r * D + v * 128 + lane * 4));
-              acc[v].x = fmaf(x.x, wj, acc[v].x);
-              acc[v].y = fmaf(x.y, wj, acc[v].y);
-              acc[v].z = fmaf(x.z, wj, acc[v].z);
-              acc[v].w = fmaf(x.w, wj, acc[v].w);
+              acc[v].x = fmaf(x[v].x, wj, acc[v].x);
+              acc[v].y = fmaf(x[v].y, wj, acc[v].y);
+              acc[v].z = fmaf(x[v].z, wj, acc[v].z);
+              acc[v].w = fmaf(x[v].w, wj, acc[v].w);
             }
+          };
+#pragma unroll
+          for (int j = 0; j < kPre; ++j) {
+            const float wj = __shfl_sync(0xffffffffu, w, j);
+            if (j < count) add(pre[j], wj);
+          }
+#pragma unroll 4
+          for (int j = kPre; j < count; ++j) {
+            const float* rec = base + int64_t(s0 + j * per_row) * g.rec_floats;
+            float4 x[kV];
+#pragma unroll
+            for (int v = 0; v < kV; ++v)
+              x[v] = __ldcg(reinterpret_cast<const float4*>(rec + r * D + v * 128 + lane * 4));
+            add(x, __shfl_sync(0xffffffffu, w, j));
           }
         }
       }
