@@ -29,12 +29,6 @@ __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
   return r;
 }
-// Two e5m2 codes from a packed half pair.
-__device__ __forceinline__ uint32_t e5m2x2_h2(uint32_t h2) {
-  uint16_t r;
-  asm("cvt.rn.satfinite.e5m2x2.f16x2 %0, %1;" : "=h"(r) : "r"(h2));
-  return r;
-}
 // Two codes (the low 16 bits of `c`) as a half pair; every e4m3 value is a
 // half exactly.
 __device__ __forceinline__ uint32_t e4m3x2_to_h2(uint32_t c) {

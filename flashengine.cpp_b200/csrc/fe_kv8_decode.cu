@@ -23,7 +23,15 @@
 // of H KV heads, range of 16-token tiles), a step is two tiles (32 tokens, the
 // K of one PV product) of all H heads, fetched with one TMA box per tile for
 // K and one for V into a ring of 128-192 KiB. The tiles' scale exponents are
-// gathered by the producer's lanes a batch ahead and travel with the stage.
+// gathered by the producer's lanes a batch ahead and travel with the stage; a
+// stage's loads go out before its exponents are stored, so that an item's
+// first do not wait for them (64 sequences of 512 to 4096 keys: 47.0 -> 45.7
+// us).
+// Measured on a B200 with 8 KV heads of 128 dims, merge included: 64 bf16
+// sequences of 2 to 32 Ki keys, 64 query heads, 220 us = 6.4 TB/s (0.98 of a
+// device-to-device copy's rate); of 512 to 4096 keys, 32 heads, 45.7 us = 4.8
+// TB/s (the rest: launch, first loads, the merge and the cut's ends); 4
+// sequences of up to 1000 keys, 9.6 us (a chain of dependent latencies).
 #include <mutex>
 #include <type_traits>
 
@@ -644,8 +652,8 @@ int dispatch(int dim, int heads, const CUtensorMap& kmap, const CUtensorMap& vma
 // `per_row` warps of a block share a row, each taking every per_row-th piece
 // with up to eight O vectors in flight, and join through shared memory: one
 // long sequence has a record per CTA, and a warp that walked 128 of them alone
-// took longer than the attention (38 us for one sequence of 8192 keys against
-// 13). gridDim.x blocks stride over the units, gridDim.y over a unit's rows.
+// took longer than the attention (one sequence of 8192 keys: 38 us in all, so
+// 10.3). gridDim.x blocks stride over the units, gridDim.y over a unit's rows.
 // ---------------------------------------------------------------------------
 constexpr int kMergeWarps = 8;
 

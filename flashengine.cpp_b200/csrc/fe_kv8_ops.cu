@@ -82,6 +82,7 @@ struct AppendArgs {
   int rows, hq, hkv, rot, max_positions;
   int64_t cache_slots;  // below 2^31
   int kv_blocks;        // blocks of the kv part; the rest rotate queries
+  bool apart;           // its blocks take K and V in turn
   unsigned int* err;
 };
 
@@ -97,7 +98,8 @@ struct AppendArgs {
 // A warp looks at a window of W rows for run starts (W = 1: a decode step
 // gives each row its own warps; W = 16: a prompt's rows, whose runs are mostly
 // whole blocks, are covered by one warp per 16 rows and head instead of 16
-// warps of which 15 find nothing). The 32 lanes read the slots of rows w - 1
+// warps of which 15 find nothing); a small step takes K and V by warps of
+// their own. The 32 lanes read the slots of rows w - 1
 // .. w + 30: the row before the window, the window, and what its last run can
 // reach; only among skipped rows does a run need more (the two loops over
 // rows). All of a run's K and V rows (8 KiB at head_dim 128) are in flight to
@@ -107,6 +109,12 @@ struct AppendArgs {
 // dims): the heads share the row's cos / sin.
 // Both parts are bound by memory traffic on prompts and by a chain of three
 // loads (slot and position, row and cos / sin, store) on decode steps.
+// Measured on a B200, bf16, 32 query and 8 KV heads of 128 dims, all rotated:
+// 64 Ki rows of 16 prompts 286 us = 5.3 TB/s (0.81 of a device-to-device copy's
+// rate; 402 us with rows in registers and runs found by a warp a row); 64 rows
+// of 64 sequences 3.5 us, 4 rows 3.2 us. Query and KV blocks in turn instead of
+// one after the other, and KV rows held in fp32 registers, measured 305 and 342
+// us against 301 and 290.
 // ---------------------------------------------------------------------------
 
 // The m-th row of a run: rows are adjacent and slots consecutive (dense), or
@@ -256,13 +264,15 @@ __device__ __forceinline__ void quantise_rows(const uint8_t* stage, const Run& r
     exps[int64_t(run.blk) * hkv + h] = static_cast<uint8_t>(e);
 }
 
+// do_k, do_v: one of them or both are this warp's.
 template <typename T, int D, bool kFull>
-__device__ __forceinline__ void append_run(const AppendArgs& a, const Run& run, int h,
-                                           uint8_t* stage, int lane) {
+__device__ __forceinline__ void append_run(const AppendArgs& a, const Run& run, int h, bool do_k,
+                                           bool do_v, uint8_t* stage, int lane) {
   using S = Stage<D>;
-  stage_rows<D>(stage, a.k, a.hkv, h, run, lane);
+  uint8_t* stage_v = stage + (do_k ? S::kBytes : 0);
+  if (do_k) stage_rows<D>(stage, a.k, a.hkv, h, run, lane);
   asm volatile("cp.async.commit_group;" ::: "memory");
-  stage_rows<D>(stage + S::kBytes, a.v, a.hkv, h, run, lane);
+  if (do_v) stage_rows<D>(stage_v, a.v, a.hkv, h, run, lane);
   asm volatile("cp.async.commit_group;" ::: "memory");
   const int rot_units = a.rot / 8;
   const int u = lane % S::kUnits;
@@ -273,18 +283,22 @@ __device__ __forceinline__ void append_run(const AppendArgs& a, const Run& run, 
     old_k = a.k_exp[int64_t(run.blk) * a.hkv + h];
     old_v = a.v_exp[int64_t(run.blk) * a.hkv + h];
   }
-  asm volatile("cp.async.wait_group 1;" ::: "memory");
-  __syncwarp();
-  if (a.pos)
-    quantise_rows<T, D, true, kFull>(stage, run, a.cache, a.rot, e0, e1, turn, a.k_codes, a.k_exp,
-                                     old_k, a.hkv, h, lane);
-  else
-    quantise_rows<T, D, false, kFull>(stage, run, nullptr, 0, e0, e1, false, a.k_codes, a.k_exp,
-                                      old_k, a.hkv, h, lane);
-  asm volatile("cp.async.wait_group 0;" ::: "memory");
-  __syncwarp();
-  quantise_rows<T, D, false, kFull>(stage + S::kBytes, run, nullptr, 0, e0, e1, false, a.v_codes,
-                                    a.v_exp, old_v, a.hkv, h, lane);
+  if (do_k) {
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    __syncwarp();
+    if (a.pos)
+      quantise_rows<T, D, true, kFull>(stage, run, a.cache, a.rot, e0, e1, turn, a.k_codes,
+                                       a.k_exp, old_k, a.hkv, h, lane);
+    else
+      quantise_rows<T, D, false, kFull>(stage, run, nullptr, 0, e0, e1, false, a.k_codes, a.k_exp,
+                                        old_k, a.hkv, h, lane);
+  }
+  if (do_v) {
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncwarp();
+    quantise_rows<T, D, false, kFull>(stage_v, run, nullptr, 0, e0, e1, false, a.v_codes, a.v_exp,
+                                      old_v, a.hkv, h, lane);
+  }
   __syncwarp();  // the stage may be refilled
 }
 
@@ -346,7 +360,9 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? 3 : 1) kv8_append_kernel(
   // `lanes_h` warps share a window's heads; a block has 8 / lanes_h windows
   const int lanes_h = min(a.hkv, kWarps), windows = kWarps / lanes_h;
   if (warp >= windows * lanes_h) return;
-  const int64_t w0l = (int64_t(blockIdx.x) * windows + warp / lanes_h) * W;
+  const bool apart = W == 1 && a.apart;
+  const bool do_k = !apart || !(blockIdx.x & 1), do_v = !apart || (blockIdx.x & 1);
+  const int64_t w0l = (int64_t(apart ? blockIdx.x / 2 : blockIdx.x) * windows + warp / lanes_h) * W;
   if (w0l >= a.rows) return;
   const int w0 = static_cast<int>(w0l);
   const int h0 = warp % lanes_h;
@@ -367,7 +383,7 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? 3 : 1) kv8_append_kernel(
   int slot = -1, p = 0;
   unsigned bad = 0;
   if (my >= 0 && my < a.rows) slot = slot_of(my, p, bad);
-  if (h0 == 0 && bad && lane >= 1 && lane <= W) raise_device_error(a.err, bad);
+  if (h0 == 0 && do_k && bad && lane >= 1 && lane <= W) raise_device_error(a.err, bad);
   const unsigned good = __ballot_sync(0xffffffffu, slot >= 0);
   const unsigned below = good & ((1u << lane) - 1u);
   int prev = __shfl_sync(0xffffffffu, slot, below ? 31 - __clz(below) : 0);
@@ -431,19 +447,23 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? 3 : 1) kv8_append_kernel(
     const int last_row = __shfl_sync(0xffffffffu, run.row_m, run.len - 1);
     run.dense = last_row - run.row0 == run.len - 1 &&
                 last % kKv8Block - run.kept == run.len - 1;
-    uint8_t* stage = smem + warp * 2 * Stage<D>::kBytes;
+    uint8_t* stage = smem + warp * (apart ? 1 : 2) * Stage<D>::kBytes;
     for (int h = h0; h < a.hkv; h += lanes_h) {
       if (W > 1 && run.dense && run.len == kKv8Block)
-        append_run<T, D, true>(a, run, h, stage, lane);
+        append_run<T, D, true>(a, run, h, do_k, do_v, stage, lane);
       else
-        append_run<T, D, false>(a, run, h, stage, lane);
+        append_run<T, D, false>(a, run, h, do_k, do_v, stage, lane);
     }
   }
 }
 
 // ---------------------------------------------------------------------------
 // Gather: blockIdx.y = sequence; a warp takes kTok tokens, every lane's
-// 16-code chunks of them in flight together. Bound by memory traffic.
+// 16-code chunks of them in flight together. Bound by memory traffic: 64
+// sequences of 512 to 4096 tokens, 8 heads of 128 dims to bf16, 71.9 us = 5.4
+// TB/s (0.82 of a device-to-device copy's rate, whose reads and writes are
+// equal parts; here two thirds are writes). Four blocks an SM against three,
+// by registers: 72 against 85 us.
 // ---------------------------------------------------------------------------
 constexpr int kGatherTok = 4;
 
@@ -515,7 +535,8 @@ __global__ void __launch_bounds__(kThreads, 4)
 // Block copy: blockIdx.y = copy, blockIdx.z = layer * 2 + (K|V). A page's
 // first ntok tokens are one contiguous range of codes; their scales are the
 // first ceil(ntok / 16) rows of the page's scales (a partly copied block
-// keeps its source's scale).
+// keeps its source's scale). Bound by memory traffic, once it outlasts the
+// launch: 64 pages in 48 layers with 4 heads of 128 dims 14.8 us = 3.9 TB/s.
 // ---------------------------------------------------------------------------
 struct Kv8Table {
   uint8_t* codes[2 * FE_MAX_LAYERS];
@@ -562,11 +583,18 @@ __global__ void __launch_bounds__(kThreads)
 
 template <typename T, int D>
 int launch_append(AppendArgs& a, cudaStream_t stream) {
-  // A warp per row and head up to 8 Ki of them, a warp per 16 rows beyond.
-  const bool wide = int64_t(a.rows) * a.hkv > 8192;
+  // Up to 2 Ki (row, head) pairs two warps each, one for K and one for V; up to
+  // 8 Ki one; a warp per 16 rows and head beyond. us on a B200 with 8 heads:
+  //   sequences x rows   64x1   16x16  512x1  16x61  1024x1  16x125  16x1021
+  //   two warps           3.5    7.9    8.5   12.7    15.5    25.5    173
+  //   one warp            3.9   10.3    7.5   13.3    11.7    20.2    124
+  //   a warp per 16 rows 32.5   12.2   35.4   15.2    37.1    18.3     76
+  const int64_t pairs = int64_t(a.rows) * a.hkv;
+  const bool wide = pairs > 8192;
+  a.apart = pairs <= 2048;
   const int64_t windows = wide ? (int64_t(a.rows) + 15) / 16 : a.rows;
   const int per_block = a.hkv < kWarps ? kWarps / a.hkv : 1;
-  const int64_t kvb = (windows + per_block - 1) / per_block;
+  const int64_t kvb = (windows + per_block - 1) / per_block * (a.apart ? 2 : 1);
   const int64_t qb = (int64_t(a.rows) * ((a.hq + kQHeads - 1) / kQHeads) * (D / 8) + kThreads - 1) /
                kThreads;
   if (kvb > INT32_MAX - qb) return fail(FE_ERR_CAPACITY, "fe_kv8_append: too many rows");
@@ -583,7 +611,7 @@ int launch_append(AppendArgs& a, cudaStream_t stream) {
   });
   if (attr_err != cudaSuccess) return cuda_fail(attr_err, "kv8_append_kernel attribute");
   FE_CUDA_TRY(launch_pdl(wide ? kv8_append_kernel<T, D, 16> : kv8_append_kernel<T, D, 1>, grid,
-                         dim3(kThreads), kSmem, stream, a));
+                         dim3(kThreads), a.apart ? kSmem / 2 : kSmem, stream, a));
   return FE_OK;
 }
 
@@ -624,7 +652,7 @@ int fe_kv8_append(const void* q, void* q_out, const void* k, const void* v, uint
                 "fe_kv8_append: k, v and the cache must be 16-byte, q and codes 8-byte aligned");
   AppendArgs a{q, q_out, k, v, k_codes, v_codes, k_exp, v_exp, slots,
                rotary_dim > 0 ? pos : nullptr, cache, rows, hq, hkv, rotary_dim, max_positions,
-               cache_slots, 0, device_error_word()};
+               cache_slots, 0, false, device_error_word()};
   auto s = static_cast<cudaStream_t>(stream);
   if (dtype == FE_DTYPE_BF16)
     return dim == 128 ? launch_append<__nv_bfloat16, 128>(a, s)

@@ -285,12 +285,12 @@ int fe_paged_decode_noalloc(const void* q, const void* k_pool, const void* v_poo
  * taken as it is. rotary_dim = 0 rotates nothing (pos and cache may be NULL; q
  * is copied).
  * A RUN is a sequence of adjacent rows (skipped ones aside) whose slots lie in
- * one block, in increasing order. Per KV head, and for K and V apart, a run's scale is the smallest
- * power of two s with |x| <= 448 s for its largest finite magnitude |x|, no
- * smaller than the block's present scale when the run does not begin at the
- * block's first slot: the tokens before it are kept, and their codes are
- * rounded to the new scale when it grew (exact but for codes that become
- * subnormal). Tokens of the block after the run are not kept: an append at
+ * one block, in increasing order. Per KV head, and for K and V apart, a run's
+ * scale is the smallest power of two s with |x| <= 448 s for its largest
+ * finite magnitude |x|, no smaller than the block's present scale when the run
+ * does not begin at the block's first slot: the tokens before it are kept, and
+ * their codes are rounded to the new scale when it grew (exact but for codes
+ * that become subnormal). Tokens of the block after the run are not kept: an append at
  * slot n leaves slots n + 1 .. of its block undefined (they hold rejected
  * drafts at most; the next append overwrites them). Codes are rounded to
  * nearest even; infinities saturate, NaN stays NaN.
@@ -331,17 +331,22 @@ int fe_kv8_copy_blocks(void* const* k_codes, void* const* v_codes, void* const* 
 /* Attention over 8-bit pools. A plan of fe_kv8_plan_create is prepared by the
  * same calls as any other (fe_attn_plan_prepare, _prepare_device,
  * fe_step_prepare_device), serves fe_kv8_attn_run only, and is destroyed by
- * fe_attn_plan_destroy; dtype is that of q and out. Its row lists are cut
- * across CTAs by keys as its decode list is.
+ * fe_attn_plan_destroy; dtype is that of q and out. The host's prepare cuts
+ * the lists of both kernels across CTAs by keys and by their measured costs.
  * fe_kv8_attn_run is fe_attn_run over the values of the codes: the same masks
  * (every query row sees at least one key: a prepared sequence has no fewer
  * keys than query rows), scale 1/sqrt(dim), fp32 softmax and accumulation,
- * output rounded to nearest even. Queries enter the product as two e4m3 parts
- * (8 to 9 significant bits: bf16's own), softmax weights as three e5m2 parts
- * (decode rows, 9 bits) or f16 (multi-row sequences), both over a range of
- * 2^26 and more below the row's largest. A query row that holds an
- * infinity or NaN gives NaN. Exponent arrays are aligned to gcd(hkv, 8) bytes
- * (2 at most for dim 256), all other buffers to 16. */
+ * output rounded to nearest even. Queries enter the product as they are
+ * (sequences of up to 16 packed rows, rows x hq / hkv: f16, and bf16 down to
+ * 2^-29 of the row's largest) or in two (bf16) or three (f16) e4m3 parts
+ * (more packed rows: 8 to 9 bits, bf16's own, and 11, f16's), softmax weights
+ * as f16 over a range of 2^26 and more below the row's largest.
+ * A query row that holds an infinity or NaN gives NaN. NaN in a key reaches
+ * the rows that see it. NaN in a value reaches its dim of the rows that see it
+ * and may reach that dim of the sequence's rows it is masked from (weight 0
+ * times NaN, as in fe_attn_run); nothing past a sequence's end reaches any
+ * row. Exponent arrays are aligned to gcd(hkv, 8) bytes (2 at most for dim
+ * 256), all other buffers to 16. */
 int fe_kv8_plan_create(int hq, int hkv, int dim, int page, int max_batch, int max_pages, int dtype,
                        int num_blocks, fe_attn_plan** plan_out);
 int fe_kv8_attn_run(fe_attn_plan* plan, const void* q, const uint8_t* k_codes,

@@ -97,10 +97,10 @@ def attention(q: np.ndarray, kval: np.ndarray, vval: np.ndarray, md, hq, hkv, pa
     are never touched). Returns (out, bound): the elementwise bound on the
     kernels' error, from their roundings:
       * a query element: 2^-9 of it for f16, nothing for bf16, and 2^-19 of the
-        row's largest (the residual part's subnormals); the score moves by at
+        row's largest (the last part's subnormals; no kernel rounds more); the score moves by at
         most eps = scale * sum |dq k|, the weights by e^(+-eps), so the output
         by (e^(2 eps) - 1) sum p |v|;
-      * a weight: 2^-9 + 2^-12 of it (three e5m2 parts of a half), its
+      * a weight: 2^-9 + 2^-12 of it (no kernel rounds more: halves), its
         exponential 2^-14 (score up to some hundreds in fp32, exp2 in
         hardware) on the weight and again on the sum, and 2^-31 of the
         largest weight per key (underflow);
