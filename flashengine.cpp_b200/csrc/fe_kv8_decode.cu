@@ -652,8 +652,8 @@ int dispatch(int dim, int heads, const CUtensorMap& kmap, const CUtensorMap& vma
 // `per_row` warps of a block share a row, each taking every per_row-th piece
 // with up to eight O vectors in flight, and join through shared memory: one
 // long sequence has a record per CTA, and a warp that walked 128 of them alone
-// took longer than the attention (one sequence of 8192 keys: 38 us in all, so
-// 10.3). gridDim.x blocks stride over the units, gridDim.y over a unit's rows.
+// took longer than the attention. gridDim.x blocks stride over the units,
+// gridDim.y over a unit's rows.
 // ---------------------------------------------------------------------------
 constexpr int kMergeWarps = 8;
 
@@ -804,7 +804,10 @@ __global__ void __launch_bounds__(kMergeWarps * 32)
 template <typename T>
 int merge_launch(int dim, int list, const AttnArgs<T>& a, int units, int rows, int pieces,
                  cudaStream_t stream, bool pdl) {
-  // eight pieces a warp, where that leaves the GPU's warps enough rows
+  // One warp a row up to eight pieces, then as many as leave each about eight.
+  // Whole calls in us on a B200 with always one, this rule, always eight:
+  // a sequence of 8192 keys 22.0, 10.2, 10.2; 64 of 512 to 4096 keys 45.6,
+  // 45.6, 60.1; a 1024-row chunk over 8192 keys 159.6, 159.8, 262.5.
   int per_row = 1;
   while (per_row < kMergeWarps && pieces > 8 * per_row) per_row *= 2;
   const int per_block = kMergeWarps / per_row;
