@@ -129,6 +129,10 @@ int encode_decode_map(CUtensorMap* map, const void* pool, int dtype, int hkv, in
   return encode_3d(map, pool, dtype, dims, strides, box);
 }
 
+// A head's row of 128 codes is one cache line: fetching the next head's line
+// with it (256-byte promotion) brought lines that were gone again before that
+// head's item came: 37 blocks of 32 rows over 8192 keys, 4 KV heads, 195 us
+// against 181.
 int encode_codes(CUtensorMap* map, const void* codes, int rank, const cuuint64_t* dims,
                  const cuuint64_t* strides, const cuuint32_t* box) {
   EncodeTiledFn fn = get_encode_fn();
@@ -136,7 +140,7 @@ int encode_codes(CUtensorMap* map, const void* codes, int rank, const cuuint64_t
   const cuuint32_t estr[4] = {1, 1, 1, 1};
   const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, rank, const_cast<void*>(codes), dims,
                         strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)
     return fail(FE_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult " + std::to_string(r));
