@@ -265,7 +265,10 @@ PlanConfig make_config(int hq, int hkv, int dim, int page, int max_batch, int ma
   c.row_split = false;      // the tcgen05 kernel walks an item's whole key range
   c.cut_rows = dim == kWideHeadDim || kv8;
   c.elem_bytes = kv8 ? 1 : 2;
-  // (measured: 1.35 us a tile of the row kernel, 5 us an item beyond its tiles)
+  // (measured: 1.3 us a tile of the row kernel, 2.5 us an item beyond its tiles
+  // and its share of the merge; with 4, 3, 2, 1 tiles an item a mixed step of
+  // 4 x 512 rows beside 60 takes 81, 84, 98, 124 us, 128 blocks of 16 rows 114,
+  // 114, 116, 117)
   c.row_tile = dim == kWideHeadDim ? 4 : 8;
   c.row_item_tiles = kv8 ? 4 : 0;
   // a step of the 8-bit decode kernel is two tiles: two steps, where a short

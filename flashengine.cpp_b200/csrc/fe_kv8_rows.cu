@@ -27,24 +27,28 @@
 //              while the other loads scores, finds its maximum or waits. The
 //              running maximum passes from tile to tile through shared memory;
 //              there is one O, rescaled in TMEM when the maximum has grown by
-//              2^8. Each group keeps the sum of its own tiles' weights.
+//              2^8. Each group keeps the sum of its own tiles' weights, and
+//              goes on to the next item's tiles while this one is stored.
 //  warp 8/11   producers of K (with the tiles' scale exponents) and of V.
 //  warp 9      issues S into one of three TMEM slots; owns TMEM.
 //  warp 10     issues O += W V once the tile's group wrote W over the slot.
 //  warps 12-15 convert V tiles to f16 (rows past the end become zeros, so
 //              nothing that lies there reaches O).
-//  warps 16-19 split the next items' query rows into their parts.
+//  warps 16-19 split the next items' query rows into their parts and store the
+//              items' outputs (by the softmax warps, between items, 120 us
+//              against 114 below, and 79 against 68 for 148 blocks of 32 rows
+//              over 512 keys).
 // All hand-offs are mbarriers; every wait is bounded.
 //
 // Measured on a B200: 128 blocks of 16 bf16 rows, 32 query heads over 4 KV
-// heads of 128 dims, 2064 to 2560 keys each, no mask: 119 us, 650 TFLOP/s and
-// 2.8 TB/s (twice that many bytes in a 16-bit cache). About 1.35 us for a tile
-// of 128 keys and 5 us for an item beside its tiles. Neither the tensor pipe
-// (38 % busy) nor the exponentials (39 %) nor the issue slots (49 %) bound it:
+// heads of 128 dims, 2064 to 2560 keys each, no mask: 114 us, 675 TFLOP/s and
+// 2.9 TB/s (twice that many bytes in a 16-bit cache). About 1.3 us for a tile
+// of 128 keys and 2.5 us for an item beside its tiles. Neither the tensor pipe
+// (40 % busy) nor the exponentials (40 %) nor the issue slots (50 %) bound it:
 // leaving out the exponentials, V's loads, its conversion or one part of the
-// queries each saves 2 to 11 %. What bounds it is the ring S -> softmax -> PV
+// queries each saved 2 to 11 %. What bounds it is the ring S -> softmax -> PV
 // -> S of dependent steps and the hand-offs between them.
-// Built, measured and not kept (the same case): V loaded by the converting
+// Built, measured and not kept (the same case, at 118 to 129 us): V loaded by the converting
 // warps two tiles ahead, 215 us (the fence for the asynchronous proxy waits
 // for the loads in flight); V stages of half a tile, 155; all 128 scores in
 // registers with the S slot freed early, 152; S and W in separate TMEM halves
@@ -101,7 +105,7 @@ struct Cfg {
   static constexpr int kOffV8 = kOffK + kKStages * kTile8;
   static constexpr int kOffV16 = kOffV8 + kV8Stages * kTile8;
   static constexpr int kOffMax = kOffV16 + kV16Stages * kTile16;  // [tile parity][row]
-  static constexpr int kOffSum = kOffMax + 2 * kM * 4;            // [item parity][group][row]
+  static constexpr int kOffSum = kOffMax + 2 * kM * 4;            // [sum|maximum][group][row]
   static constexpr int kOffRow = kOffSum + 2 * 2 * kM * 4;        // [Q buffer][row] score factors
   static constexpr int kOffExp = kOffRow + 2 * kM * 4;            // [ring][8] float4
   static constexpr int kOffBar = kOffExp + kExpRing * 8 * 16;
@@ -109,7 +113,6 @@ struct Cfg {
                                   kSlots + kSlots + kSlots + kExpRing + 8 + 1;
   static constexpr int kSmem = kOffBar + kNumBars * 8 + 32;
   static constexpr uint32_t kOCol = D == 128 ? kSlots * kN : 256;
-  static constexpr int kGroupDims = D / 2;  // O dims a softmax group stores
   static_assert(kSmem <= 232448, "shared memory budget");
   static_assert(kSlots * kN <= int(kOCol) && kOCol + D <= 512, "TMEM budget");
 };
@@ -199,8 +202,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&q_full[b], 4);   // one arrival per converter warp
       mbar_init(&q_empty[b], 9);  // the S issuer's commit, the softmax warps
     }
-    mbar_init(o_free, 256);
-    mbar_init(l_done, 256);
+    mbar_init(o_free, 128);  // the storing warps
+    mbar_init(l_done, 8);    // the softmax warps
     for (int s = 0; s < kKStages; ++s) {
       mbar_init(&k_full[s], 1);
       mbar_init(&k_empty[s], 1);
@@ -353,7 +356,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int t = 0; t < ntiles && !aborted; ++t, ++n) {
               const int slot = n % kSlots;
               const uint32_t st = n % kV16Stages;
-              // O is free once both groups stored the last item's output
+              // O is free once the last item's output is stored
               if (t == 0 && unit > 0 &&
                   !wait_or_abort(o_free, (unit - 1) & 1, flags, aborted))
                 break;
@@ -377,7 +380,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         wait_bounded_short(drain, 0, flags + 1);
       }
     } else if (warp >= kQWarp) {
-      // ------------------------------------------------------ query conversion
+      // --------------------------------------------- query conversion, output
       // Rows of the CTA's u-th item: D / 16 lanes a row, 16 elements each.
       // fetch_q copies the 16-bit rows into the item's buffer (zeros past the
       // sequence), 16-byte chunk k of row r to position k % 8 (swizzled) of
@@ -458,16 +461,82 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&q_full[u % C::kQBufs]);
       };
+      // Output of the CTA's u-th item, once its last PV is done: the next
+      // item's tiles are on their way in the other warps meanwhile.
+      uint32_t n_end = 0;  // tiles of the items stored
+      auto store_o = [&](int u) {
+        const WorkItem w = items[it0 + u];
+        const SeqInfo si = seqs[w.seq];
+        n_end += (w.kt1 - w.kt0 + kPieces - 1) / kPieces;
+        const uint32_t nl = n_end - 1;
+        const int quad = warp - kQWarp, r = quad * 32 + lane;
+        const int P = si.qrows * G, p = w.rb0 * kRowBlock + r;
+        const bool row_valid = p < P, split = w.part >= 0;
+        const int rows_rec = min(P, w.rb0 * kRowBlock + kM) - w.rb0 * kRowBlock;
+        float* rec = split ? a.partials + w.part : nullptr;
+        T* dst = row_valid && !split
+                     ? a.out + (static_cast<int64_t>(si.q_row0 + p / G) * a.hq + w.kvh * G +
+                                p % G) * D
+                     : nullptr;
+        if (!wait_warp(l_done, u & 1, flags, aborted)) return;
+        // (the last tile's S waited for the slot's PV before)
+        if (!wait_warp(&s_free[nl % kSlots], (nl / kSlots) & 1u, flags, aborted)) return;
+        tc::fence_after_sync();
+        // the group of the last tile has the item's maximum
+        const float* sums = xsum + r;
+        const float* maxs = xsum + 2 * kM + r;
+        const int own = (nl & 1) * kM, other = kM - own;
+        const float m_item = maxs[own], m_other = maxs[other];
+        float l_other = sums[other];
+        if (m_other != m_item) l_other *= fast_exp2(m_other - m_item);
+        const float lsum = sums[own] + l_other;
+        const float inv = 1.f / lsum;
+        if (split && row_valid) {
+          rec[rows_rec * D + r] = m_item;
+          rec[rows_rec * (D + 1) + r] = lsum;
+        }
+        const uint32_t o_addr = tmem + (uint32_t(quad * 32) << 16) + C::kOCol;
+#pragma unroll 2
+        for (int c2 = 0; c2 < D / 32; ++c2) {
+          float o[32];
+          tc::ld_32x32b_x32(o_addr + c2 * 32, *reinterpret_cast<uint32_t(*)[32]>(&o[0]));
+          tc::wait_ld();
+          if (dst) {
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+              uint4 pk;
+              pk.x = pack2<T>(o[8 * v + 0] * inv, o[8 * v + 1] * inv);
+              pk.y = pack2<T>(o[8 * v + 2] * inv, o[8 * v + 3] * inv);
+              pk.z = pack2<T>(o[8 * v + 4] * inv, o[8 * v + 5] * inv);
+              pk.w = pack2<T>(o[8 * v + 6] * inv, o[8 * v + 7] * inv);
+              *reinterpret_cast<uint4*>(dst + c2 * 32 + 8 * v) = pk;
+            }
+          } else if (split && row_valid) {
+            float* row = rec + r * D + c2 * 32;
+#pragma unroll
+            for (int v = 0; v < 8; ++v)
+              *reinterpret_cast<float4*>(row + 4 * v) =
+                  make_float4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
+          }
+        }
+        // O and this item's sums have been read: the next item may reuse them
+        tc::fence_before_sync();
+        mbar_arrive(o_free);
+      };
       WorkItem w = items[it0];
       SeqInfo si = seqs[w.seq];
-      for (int u = 0; u < nitems && !aborted; ++u) {
-        if (!wait_warp(&q_empty[u % C::kQBufs], ((u / C::kQBufs) & 1u) ^ 1u, flags, aborted)) break;
-        fetch_q(u, w, si);
-        if (u + 1 < nitems) {  // in flight with this item's rows
-          w = items[it0 + u + 1];
-          si = seqs[w.seq];
+      for (int u = 0; u <= nitems && !aborted; ++u) {
+        if (u < nitems) {
+          if (!wait_warp(&q_empty[u % C::kQBufs], ((u / C::kQBufs) & 1u) ^ 1u, flags, aborted))
+            break;
+          fetch_q(u, w, si);
+          if (u + 1 < nitems) {  // in flight with this item's rows
+            w = items[it0 + u + 1];
+            si = seqs[w.seq];
+          }
+          convert_q(u);
         }
-        convert_q(u);
+        if (u > 0) store_o(u - 1);
       }
       if (aborted && lane == 0) raise_device_error(a.err, FE_DEVERR_TIMEOUT);
     } else {
@@ -532,13 +601,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (aborted && lane == 0) raise_device_error(a.err, FE_DEVERR_TIMEOUT);
     }
   } else {
-    // ------------------------------------------------ softmax and epilogue
-    constexpr int kGD = C::kGroupDims;
+    // ------------------------------------------------------------- softmax
     const int gi = warp >= 4 ? 1 : 0;
     const int quad = warp & 3;
     const int r = quad * 32 + lane;  // packed row = TMEM lane
     const uint32_t lane_addr = tmem + (uint32_t(quad * 32) << 16);
-    const uint32_t o_dims = lane_addr + C::kOCol + gi * kGD;
     const int G = a.G;
     const bool causal = view == 1;
     uint32_t n0 = 0;  // the item's first tile
@@ -600,11 +667,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc::wait_st();
         // the maximum so far comes from the tile before and goes to the next;
         // it moves only when it grows by more than 2^8 (or from nothing)
+        // (an item's first tile only waits, so that the group of the tile before
+        // has read what this one overwrites)
         float m_prev = -INFINITY;
-        if (j > 0) {
+        if (n > 0) {
           if (!wait_warp(&max_bar[((n - 1) & 1) * 4 + quad], ((n - 1) >> 1) & 1u, flags, aborted))
             break;
-          m_prev = xmax[((n - 1) & 1) * kM + r];
+          if (j > 0) m_prev = xmax[((n - 1) & 1) * kM + r];
         }
         const float m_top = fmaxf(m_prev, mx);
         const bool grow = m_top > m_prev + kRescale;
@@ -667,57 +736,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) mbar_arrive(&p_full[slot]);
       }
       if (aborted) break;
-      // the last tile's maximum is the item's; its PV is the item's last
-      const uint32_t nl = n0 + ntiles - 1;
       n0 += ntiles;
-      if (!wait_warp(&max_bar[(nl & 1) * 4 + quad], (nl >> 1) & 1u, flags, aborted)) break;
-      const float m_item = xmax[(nl & 1) * kM + r];
-      if (m_used != m_item) l *= fast_exp2(m_used - m_item);
-      if (!wait_warp(&s_free[nl % kSlots], (nl / kSlots) & 1u, flags, aborted)) break;
-      float* xs = xsum + (unit & 1) * 2 * kM;
-      xs[gi * kM + r] = l;
-      mbar_arrive(l_done);
-      if (!wait_warp(l_done, unit & 1, flags, aborted)) break;
-      tc::fence_after_sync();
-      const float lsum = l + xs[(gi ^ 1) * kM + r];
-      const float inv = 1.f / lsum;
-      const bool split = w.part >= 0;
-      const int rows_rec = min(P, w.rb0 * kRowBlock + kM) - w.rb0 * kRowBlock;
-      float* rec = split ? a.partials + w.part : nullptr;
-      T* dst = row_valid && !split
-                   ? a.out + (static_cast<int64_t>(si.q_row0 + p / G) * a.hq + w.kvh * G + p % G) *
-                                 D + gi * kGD
-                   : nullptr;
-      if (split && row_valid && gi == 0) {
-        rec[rows_rec * D + r] = m_item;
-        rec[rows_rec * (D + 1) + r] = lsum;
-      }
-#pragma unroll
-      for (int c2 = 0; c2 < kGD / 32; ++c2) {
-        float o[32];
-        tc::ld_32x32b_x32(o_dims + c2 * 32, *reinterpret_cast<uint32_t(*)[32]>(&o[0]));
-        tc::wait_ld();
-        if (dst) {
-#pragma unroll
-          for (int v = 0; v < 4; ++v) {
-            uint4 pk;
-            pk.x = pack2<T>(o[8 * v + 0] * inv, o[8 * v + 1] * inv);
-            pk.y = pack2<T>(o[8 * v + 2] * inv, o[8 * v + 3] * inv);
-            pk.z = pack2<T>(o[8 * v + 4] * inv, o[8 * v + 5] * inv);
-            pk.w = pack2<T>(o[8 * v + 6] * inv, o[8 * v + 7] * inv);
-            *reinterpret_cast<uint4*>(dst + c2 * 32 + 8 * v) = pk;
-          }
-        } else if (split && row_valid) {
-          float* row = rec + r * D + gi * kGD + c2 * 32;
-#pragma unroll
-          for (int v = 0; v < 8; ++v)
-            *reinterpret_cast<float4*>(row + 4 * v) =
-                make_float4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
-        }
-      }
-      // O and this item's sums have been read: the next item may reuse them
-      tc::fence_before_sync();
-      mbar_arrive(o_free);
+      // this group's sum and the maximum it refers to, once the item before is
+      // stored
+      if (unit > 0 && !wait_warp(o_free, (unit - 1) & 1, flags, aborted)) break;
+      xsum[gi * kM + r] = l;
+      xsum[(2 + gi) * kM + r] = m_used;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(l_done);
     }
     if (aborted && lane == 0) raise_device_error(a.err, FE_DEVERR_TIMEOUT);
   }
