@@ -45,16 +45,19 @@
 // 3.0 TB/s (twice that many bytes in a 16-bit cache). About 1.3 us for a tile
 // of 128 keys and 2.5 us for an item beside its tiles. Neither the tensor pipe
 // (40 % busy) nor the exponentials (40 %) nor the issue slots (50 %) bound it:
-// leaving out the exponentials, V's loads, its conversion or one part of the
-// queries each saved 2 to 11 %. What bounds it is the ring S -> softmax -> PV
-// -> S of dependent steps and the hand-offs between them.
-// Built, measured and not kept (the same case, at 118 to 129 us): V loaded by the converting
-// warps two tiles ahead, 215 us (the fence for the asynchronous proxy waits
-// for the loads in flight); V stages of half a tile, 155; all 128 scores in
-// registers with the S slot freed early, 152; S and W in separate TMEM halves
-// in turn, 122 to 126; scores loaded 16 keys ahead in either pass or both, 2 to
-// 5 % slower; three softmax groups, outputs staged through shared
-// memory, items' descriptions in shared memory: no change.
+// without the exponentials 107 us, without 7/8 of the PV products 110, with one
+// part of the queries 112, without all three 102. Nor do the loads: a third V
+// stage and a fourth K stage in place of the second query buffer change
+// nothing on long items. What bounds it is the ring S -> softmax -> PV -> S of
+// dependent steps over three TMEM slots, which take all columns beside O.
+// Built, measured and not kept (the same case, at 112 to 129 us): V loaded by
+// the converting warps two tiles ahead, 215 us (the fence for the asynchronous
+// proxy waits for the loads in flight); V stages of half a tile, 155; all 128
+// scores in registers with the S slot freed early, 152; S and W in separate
+// TMEM halves in turn, 122 to 126; scores loaded 16 keys ahead in either pass
+// or both, 2 to 5 % slower; one pass over the scores with the maximum of the
+// group's tile before (and corrections where it is exceeded), three softmax
+// groups, items' descriptions in shared memory: no change.
 #include <mutex>
 #include <type_traits>
 
