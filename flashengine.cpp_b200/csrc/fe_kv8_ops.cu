@@ -479,7 +479,13 @@ __global__ void __launch_bounds__(kThreads, 4)
   const int b = blockIdx.y;
   const int p0 = __ldg(kv + b), p1 = __ldg(kv + b + 1);
   if (p1 <= p0) return;
-  const int len = (p1 - p0 - 1) * page + __ldg(last + b);
+  const int tail = __ldg(last + b);
+  const int64_t tokens = int64_t(p1 - p0 - 1) * page + tail;
+  if (tail < 1 || tail > page || tokens > INT32_MAX / 2) {
+    if (threadIdx.x == 0 && blockIdx.x == 0) raise_device_error(err, FE_DEVERR_PAGE_RANGE);
+    return;
+  }
+  const int len = static_cast<int>(tokens);
   const int64_t orow = __ldg(row_offset + b);
   const int lane = threadIdx.x & 31;
   const int chunks = hkv * dim / 16;

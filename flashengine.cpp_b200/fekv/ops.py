@@ -429,6 +429,8 @@ def gather_kv8(pool, out, kv, pages, last, row_offset, max_len, page, stream=Non
     hkv, dim] (16-bit), metadata as gather(): int32 CUDA tensors."""
     for t in (kv, pages, last, row_offset):
         _require_device_i32(t)
+    if not last.shape == row_offset.shape == (kv.shape[0] - 1,):
+        raise ValueError("last and row_offset must have one entry per sequence, kv one more")
     _, hkv, dim = pool.shape
     if not out.is_contiguous() or not out.is_cuda or out.numel() % (hkv * dim):
         raise ValueError("out: expected a contiguous CUDA tensor [rows, hkv, dim]")
@@ -446,6 +448,8 @@ def copy_blocks_kv8(k_pools, v_pools, src, dst, ntok, page, stream=None):
         raise ValueError("k_pools and v_pools differ in length")
     for t in (src, dst, ntok):
         _require_device_i32(t)
+    if not src.shape == dst.shape == ntok.shape:
+        raise ValueError("src, dst and ntok differ in length")
     if n == 0:
         return
     shape = k_pools[0].shape
@@ -471,12 +475,28 @@ class Kv8Plan(AttentionPlan):
         torch = _torch()
         self.pool_shape = ((int(blocks) + 1) * int(page), int(hkv), int(dim))
         self.dtype = torch.bfloat16 if bf16 else torch.float16
+        self.rows = 0  # query rows of the last prepare
+
+    def prepare(self, qo, kv, pages, last, batch=None, rows=None, graph=False, stream=None):
+        super().prepare(qo, kv, pages, last, batch, rows, graph, stream)
+        self.rows = int(qo[len(kv) - 1 if batch is None else batch])
+
+    def prepare_device(self, qo, kv, pages, last, batch, rows, stream=None):
+        super().prepare_device(qo, kv, pages, last, batch, rows, stream)
+        self.rows = int(rows)
+
+    def step_prepare_device(self, block_tables, starts, rows_per_seq, slots, positions,
+                            stream=None):
+        super().step_prepare_device(block_tables, starts, rows_per_seq, slots, positions, stream)
+        self.rows = int(block_tables.shape[0]) * int(rows_per_seq)
 
     def attention(self, q, kpool, vpool, out, causal=True, stream=None):
         if kpool.shape != self.pool_shape or vpool.shape != self.pool_shape:
             raise ValueError(f"pools of shape {kpool.shape}, {vpool.shape}: the plan is for "
                              f"{self.pool_shape}")
         shape = (q.shape[0], self.hq, self.dim)
+        if shape[0] < self.rows:
+            raise ValueError(f"q has {shape[0]} rows, the plan was prepared for {self.rows}")
         check(self.lib.fe_kv8_attn_run(self.handle, _kv8_rows("q", q, self.dtype, shape),
                                        kpool.codes_ptr, vpool.codes_ptr, kpool.exps_ptr,
                                        vpool.exps_ptr, _kv8_rows("out", out, self.dtype, shape),

@@ -312,8 +312,8 @@ int fe_kv8_append(const void* q, void* q_out, const void* k, const void* v, uint
 
 /* fe_kv_gather from an 8-bit pool: the values, rounded to the 16-bit `dtype`
  * (bf16 holds every one exactly). A page id that reaches past cache_slots
- * leaves its token unwritten and raises FE_DEVERR_PAGE_RANGE. max_len bounds
- * the launch only: longer sequences are covered by striding. */
+ * leaves its token unwritten and raises FE_DEVERR_PAGE_RANGE, a `last` outside
+ * [1, page] its sequence. max_len bounds the launch only: longer sequences are covered by striding. */
 int fe_kv8_gather(const uint8_t* codes, const uint8_t* exps, void* out, const int32_t* kv,
                   const int32_t* pages, const int32_t* last, const int32_t* row_offset, int batch,
                   int max_len, int page, int hkv, int dim, int dtype, int64_t cache_slots,

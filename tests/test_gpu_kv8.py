@@ -257,6 +257,16 @@ def test_gather_bad_page_is_skipped():
     assert fekv.device_errors() == _lib.FE_DEVERR_PAGE_RANGE
 
 
+def test_gather_bad_last_skips_its_sequence():
+    pool = fekv.Kv8Pool.empty(7, 16, 2, 128)
+    out = torch.full((6 * 16, 2, 128), 5.0, device="cuda", dtype=torch.float16)
+    i32 = lambda *a: torch.tensor(a, dtype=torch.int32, device="cuda")  # noqa: E731
+    fekv.gather_kv8(pool, out, i32(0, 2, 4, 4, 6), i32(0, 1, 2, 3, 4, 5), i32(17, 16, 9, 0),
+                    i32(0, 32, 0, 64), 32, 16)
+    assert (out[:32] == 5).all() and (out[32:64] == 0).all() and (out[64:] == 5).all()
+    assert fekv.device_errors() == _lib.FE_DEVERR_PAGE_RANGE
+
+
 @pytest.mark.parametrize("hkv,dim,page,layers", [(8, 128, 16, 1), (3, 128, 48, 5), (2, 256, 32, 3)])
 def test_copy_blocks(hkv, dim, page, layers):
     rng = np.random.default_rng(page)
@@ -637,3 +647,28 @@ def test_python_refusals():
         with pytest.raises(ValueError):
             f()
     plan.close()
+
+
+def test_refusals_of_short_arrays():
+    pool = fekv.Kv8Pool.empty(8, 16, 4, 128)
+    i32 = lambda *a: torch.tensor(a, dtype=torch.int32, device="cuda")  # noqa: E731
+    out = torch.zeros(16, 4, 128, dtype=torch.bfloat16, device="cuda")
+    q = torch.zeros(5, 8, 128, dtype=torch.bfloat16, device="cuda")
+    for prepare in ("host", "device"):
+        plan = fekv.Kv8Plan(8, 4, 128, 16, 2, 4, True, 8)
+        meta = ([0, 4, 5], [0, 1, 2], [2, 3], [5, 16])
+        if prepare == "host":
+            plan.prepare(*meta)
+        else:
+            plan.prepare_device(*(i32(*m) for m in meta), 2, 5)
+        with pytest.raises(ValueError):
+            plan.attention(q[:4], pool, pool, q[:4])
+        plan.attention(q, pool, pool, torch.empty_like(q))
+        plan.close()
+    for f in (lambda: fekv.gather_kv8(pool, out, i32(0, 1), i32(2), i32(5, 6), i32(0), 16, 16),
+              lambda: fekv.gather_kv8(pool, out, i32(0, 1), i32(2), i32(5), i32(0, 0), 16, 16),
+              lambda: fekv.copy_blocks_kv8([pool], [pool], i32(1, 2), i32(3), i32(4, 4), 16),
+              lambda: fekv.copy_blocks_kv8([pool], [pool], i32(1), i32(3), i32(), 16)):
+        with pytest.raises(ValueError):
+            f()
+    assert fekv.device_errors() == 0
