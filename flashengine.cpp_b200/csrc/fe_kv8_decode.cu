@@ -447,13 +447,21 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const MetaHeader* hdr = reinterpret_cast<const MetaHeader*>(a.meta);
   constexpr int kList = 2;  // decode work list
-  if (static_cast<int>(blockIdx.x) >= hdr->grid[kList]) return;
+  // A CTA without work waits as well: a grid that ended before the one it
+  // follows would let the next one start beside that.
+  if (static_cast<int>(blockIdx.x) >= hdr->grid[kList]) {
+    pdl_wait();
+    return;
+  }
   const int32_t* cta_off = reinterpret_cast<const int32_t*>(a.meta + hdr->cta_off_off[kList]);
   const WorkItem* items = reinterpret_cast<const WorkItem*>(a.meta + hdr->items_off[kList]);
   const SeqInfo* seqs = reinterpret_cast<const SeqInfo*>(a.meta + hdr->seqs_off);
   const int32_t* pages = reinterpret_cast<const int32_t*>(a.meta + hdr->pages_off);
   const int it0 = cta_off[blockIdx.x], it1 = cta_off[blockIdx.x + 1];
-  if (it0 >= it1) return;
+  if (it0 >= it1) {
+    pdl_wait();
+    return;
+  }
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kStages; ++s) {
