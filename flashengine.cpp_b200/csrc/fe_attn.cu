@@ -612,12 +612,17 @@ int launch_lists(fe_attn_plan* p, int view, int grid_rows, int grid_dec, const v
     if (!p->kv8)  // one warp per record row, 32 rows per CTA
       return decode_merge_launch(p->dtype, dim, list, args, units, std::max(1, (rows + 31) / 32),
                                  on, pdl);
-    // pieces of a unit: under a fixed geometry what an even cut gives
+    // Pieces of a unit: under a fixed geometry what an even cut gives. Its grid
+    // is mostly empty blocks, so it is bounded and strides over the rows:
+    // replayed decode steps of 4 short sequences take 33 us with a block for
+    // every possible row, 17, 16, 17, 21 with 16, 8, 4, 2 blocks an SM; of 64
+    // sequences 55, then 56, 52, 51, 52; of one of 8192 keys 19, 21, 29, 46.
     const int even = list == 2 ? p->cfg.dec_grid_cap * p->cfg.dec_heads /
                                      (p->cfg.hkv * std::max(1, h.batch)) + 1
                                : 1;
     return kv8_merge_launch(p->dtype, dim, list, args, units, std::max(1, rows),
-                            bound ? even : p->last.split_pieces[list], on, pdl);
+                            bound ? even : p->last.split_pieces[list],
+                            bound ? 8 * p->cfg.grid_cap : INT32_MAX, on, pdl);
   };
   // A mixed step planned side by side (the two lists' grids sum to the SMs)
   // forks: the row kernel runs on the plan's side stream while the decode

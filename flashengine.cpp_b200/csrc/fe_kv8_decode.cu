@@ -32,6 +32,7 @@
 // device-to-device copy's rate); of 512 to 4096 keys, 32 heads, 45.7 us = 4.8
 // TB/s (the rest: launch, first loads, the merge and the cut's ends); 4
 // sequences of up to 1000 keys, 9.6 us (a chain of dependent latencies).
+#include <algorithm>
 #include <mutex>
 #include <type_traits>
 
@@ -811,7 +812,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32)
 
 template <typename T>
 int merge_launch(int dim, int list, const AttnArgs<T>& a, int units, int rows, int pieces,
-                 cudaStream_t stream, bool pdl) {
+                 int max_blocks, cudaStream_t stream, bool pdl) {
   // One warp a row up to eight pieces, then as many as leave each about eight.
   // Whole calls in us on a B200 with always one, this rule, always eight:
   // a sequence of 8192 keys 22.0, 10.2, 10.2; 64 of 512 to 4096 keys 45.6,
@@ -819,7 +820,8 @@ int merge_launch(int dim, int list, const AttnArgs<T>& a, int units, int rows, i
   int per_row = 1;
   while (per_row < kMergeWarps && pieces > 8 * per_row) per_row *= 2;
   const int per_block = kMergeWarps / per_row;
-  const dim3 grid(units, (rows + per_block - 1) / per_block);
+  const dim3 grid(units, std::min((rows + per_block - 1) / per_block,
+                                  std::max(1, max_blocks / units)));
   auto kernel = dim == kWideHeadDim ? kv8_merge_kernel<T, kWideHeadDim>
                                     : kv8_merge_kernel<T, kHeadDim>;
   if (pdl) {
@@ -834,13 +836,13 @@ int merge_launch(int dim, int list, const AttnArgs<T>& a, int units, int rows, i
 }  // namespace
 
 int kv8_merge_launch(int dtype, int dim, int list, const void* args, int units, int rows,
-                     int pieces, cudaStream_t stream, bool pdl) {
+                     int pieces, int max_blocks, cudaStream_t stream, bool pdl) {
   if (units <= 0) return FE_OK;
   if (dtype == FE_DTYPE_BF16)
     return merge_launch(dim, list, *static_cast<const AttnArgs<__nv_bfloat16>*>(args), units, rows,
-                        pieces, stream, pdl);
+                        pieces, max_blocks, stream, pdl);
   return merge_launch(dim, list, *static_cast<const AttnArgs<__half>*>(args), units, rows, pieces,
-                      stream, pdl);
+                      max_blocks, stream, pdl);
 }
 
 int kv8_decode_launch(int dtype, int dim, int heads, const CUtensorMap& kmap,
