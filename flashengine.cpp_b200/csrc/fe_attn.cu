@@ -292,9 +292,11 @@ PlanConfig make_config(int hq, int hkv, int dim, int page, int max_batch, int ma
   c.dec_fixed_us = 10.f;
   c.row_piece_us = dim == kWideHeadDim ? 0.4f : 0.2f;
   if (kv8) {
-    // the 8-bit kernels: 1.35 us a tile; with 50 GB/s per decode SM four mixed
-    // steps took 81, 48, 152 and 66 us, with 42 and 60: 82-88, 48-50, 161-190,
-    // 67-69
+    // the 8-bit kernels: 1.35 us a tile, item costs aside. Steps of 4 x 512 rows
+    // beside 60, 2 x 200 beside 38, 2 x 1024 beside 32 and 4 x 256 beside 128
+    // take 79, 46, 190 and 112 us with 50 GB/s per decode SM, 79, 46, 217, 118
+    // with 45 and 82, 48, 194, 110 with 55; with 1.2 us a tile 78, 46, 191, 120,
+    // with 1.5 84, 48, 201, 111.
     c.row_piece_us = 1.35f / c.row_tile;
     c.dec_sm_gbs = 50.f;
   }
