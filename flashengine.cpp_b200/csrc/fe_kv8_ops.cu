@@ -98,8 +98,8 @@ struct AppendArgs {
 // A warp looks at a window of W rows for run starts (W = 1: a decode step
 // gives each row its own warps; W = 16: a prompt's rows, whose runs are mostly
 // whole blocks, are covered by one warp per 16 rows and head instead of 16
-// warps of which 15 find nothing); a small step takes K and V by warps of
-// their own. The 32 lanes read the slots of rows w - 1
+// warps of which 15 find nothing; W = 4 between them); a small step takes K and
+// V by warps of their own. The 32 lanes read the slots of rows w - 1
 // .. w + 30: the row before the window, the window, and what its last run can
 // reach; only among skipped rows does a run need more (the two loops over
 // rows). All of a run's K and V rows (8 KiB at head_dim 128) are in flight to
@@ -590,15 +590,18 @@ __global__ void __launch_bounds__(kThreads)
 template <typename T, int D>
 int launch_append(AppendArgs& a, cudaStream_t stream) {
   // Up to 2 Ki (row, head) pairs two warps each, one for K and one for V; up to
-  // 8 Ki one; a warp per 16 rows and head beyond. us on a B200 with 8 heads:
-  //   sequences x rows   64x1   16x16  512x1  16x61  1024x1  16x125  16x1021
-  //   two warps           3.5    7.9    8.5   12.7    15.5    25.5    173
-  //   one warp            3.9   10.3    7.5   13.3    11.7    20.2    124
-  //   a warp per 16 rows 32.5   12.2   35.4   15.2    37.1    18.3     76
+  // 8 Ki one; a warp per 4 rows and head up to 32 Ki, per 16 beyond. us on a
+  // B200 with 8 heads:
+  //   sequences x rows  64x1 16x16 512x1 16x61 1024x1 16x125 2048x1 16x253 16x1021
+  //   two warps          3.5   7.9   8.5  12.7   15.5   25.5     37     45     173
+  //   one warp           3.9  10.3   7.5  13.3   11.7   20.2     27     32     124
+  //   per 4 rows         9.7  12.2  12.3  12.5   12.9   15.7     26     22      80
+  //   per 16 rows       32.5  12.2  35.4  15.2   37.1   18.3     47     22      76
+  // (8 rows: 64 Ki rows of 16 prompts 297 against 289.)
   const int64_t pairs = int64_t(a.rows) * a.hkv;
-  const bool wide = pairs > 8192;
+  const int w = pairs > 32768 ? 16 : pairs > 8192 ? 4 : 1;
   a.apart = pairs <= 2048;
-  const int64_t windows = wide ? (int64_t(a.rows) + 15) / 16 : a.rows;
+  const int64_t windows = (int64_t(a.rows) + w - 1) / w;
   const int per_block = a.hkv < kWarps ? kWarps / a.hkv : 1;
   const int64_t kvb = (windows + per_block - 1) / per_block * (a.apart ? 2 : 1);
   const int64_t qb = (int64_t(a.rows) * ((a.hq + kQHeads - 1) / kQHeads) * (D / 8) + kThreads - 1) /
@@ -610,14 +613,17 @@ int launch_append(AppendArgs& a, cudaStream_t stream) {
   static std::once_flag once;
   static cudaError_t attr_err = cudaSuccess;
   std::call_once(once, [] {
-    for (auto kernel : {kv8_append_kernel<T, D, 16>, kv8_append_kernel<T, D, 1>})
+    for (auto kernel : {kv8_append_kernel<T, D, 16>, kv8_append_kernel<T, D, 4>,
+                        kv8_append_kernel<T, D, 1>})
       if (attr_err == cudaSuccess)
         attr_err =
             cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   });
   if (attr_err != cudaSuccess) return cuda_fail(attr_err, "kv8_append_kernel attribute");
-  FE_CUDA_TRY(launch_pdl(wide ? kv8_append_kernel<T, D, 16> : kv8_append_kernel<T, D, 1>, grid,
-                         dim3(kThreads), a.apart ? kSmem / 2 : kSmem, stream, a));
+  auto kernel = w == 16  ? kv8_append_kernel<T, D, 16>
+                : w == 4 ? kv8_append_kernel<T, D, 4>
+                         : kv8_append_kernel<T, D, 1>;
+  FE_CUDA_TRY(launch_pdl(kernel, grid, dim3(kThreads), a.apart ? kSmem / 2 : kSmem, stream, a));
   return FE_OK;
 }
 

@@ -174,6 +174,24 @@ def test_append_runs_go_on_past_skipped_rows(gap):
     assert fekv.device_errors() == 0
 
 
+@pytest.mark.parametrize("gap", [0, 1, 2, 5, 33])
+def test_append_windows_of_four_rows(gap):
+    """Rows enough for 4-row windows, few enough not for 16-row ones: blocks
+    begun anywhere, and blocks with skipped rows inside."""
+    rng = np.random.default_rng(40 + gap)
+    counts = [700, 1, 16, 17, 400, 3, 1, 900]
+    starts = [9, 15, 0, 3, 16, 14, 31, 5]
+    slots, pos = step_slots(rng, 16, starts, counts, 200)
+    slots = np.insert(slots, 300, [-1] * gap)
+    slots = np.insert(slots, 1000, [-1] * gap)
+    pos = np.insert(np.insert(pos, 300, [0] * gap), 1000, [0] * gap)
+    k = half(rng.standard_normal((len(slots), 8, 128)) *
+             np.exp2(rng.integers(-3, 4, (len(slots), 1, 1))), True)
+    pools = [random_pool(rng, 200 * 16, 8, 128) for _ in range(2)]
+    run_append(rng, k, k[::-1].copy(), slots, pos, rope_cache(1000, 128), pools, True, 2)
+    assert fekv.device_errors() == 0
+
+
 def test_append_special_values():
     """Zeros, infinities, NaN, subnormals, the largest finite numbers, and
     magnitudes at the edge of a scale (448, 1.75 * 2^n, and just above)."""
