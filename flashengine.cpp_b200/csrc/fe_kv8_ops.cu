@@ -217,7 +217,10 @@ __device__ __forceinline__ void quantise_rows(const uint8_t* stage, const Run& r
     for (int o = 16; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
   }
   int e = needed_exp(amax);
-  if (run.kept) e = min(max(e, old), kKv8MaxExp);
+  // the kept tokens' scale as every reader takes it: a byte outside the limits
+  // is the nearest within
+  const int was = exp_clamp(old);
+  if (run.kept) e = max(e, was);
   const float inv = exp_scale(254 - e);
   const int64_t tok = int64_t(hkv) * D;  // bytes from one token to the next
   uint8_t* block = codes + int64_t(run.blk) * kKv8Block * tok + h * D;
@@ -244,9 +247,9 @@ __device__ __forceinline__ void quantise_rows(const uint8_t* stage, const Run& r
       }
     }
   }
-  if (run.kept && e > old) {
+  if (run.kept && e > was) {
     // the kept tokens move to the larger scale: 8 codes per lane and pass
-    const float down = exp_scale(max(old - e + 127, 1));
+    const float down = exp_scale(was - e + 127);
     for (int t = sub; t < run.kept; t += kRows) {
       uint2* w = reinterpret_cast<uint2*>(block + t * tok) + u;
       uint2 c = *w;

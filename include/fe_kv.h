@@ -272,10 +272,10 @@ int fe_paged_decode_noalloc(const void* q, const void* k_pool, const void* v_poo
  * lists and plans are as for the 16-bit pools. page is a multiple of 16.
  *
  * What a cache holds is set by fe_kv8_append: exponents within 2^-32 .. 2^64
- * (bytes 95 .. 191; the attention and gather operators read a byte outside
- * as the nearest of these, so pages never written to are harmless beyond a
- * sequence's end), codes of magnitude up to 448, NaN where the input was
- * NaN.
+ * (bytes 95 .. 191; attention, gather and an append that keeps a block's
+ * tokens read a byte outside as the nearest of these, so pages never written to
+ * are harmless beyond a sequence's end), codes of magnitude up to 448, NaN
+ * where the input was NaN.
  * ------------------------------------------------------------------------ */
 #define FE_KV8_BLOCK 16
 

@@ -1,0 +1,55 @@
+"""Forms of the 8-bit cache's operators that test_gpu_kv8.py does not reach,
+against the same restatement in 64 bits (kv8_ref.py)."""
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+import fekv
+import kv8_ref as ref
+from test_gpu_kv8 import codes_of, dev, exps_of, half, pool_of, random_pool
+
+pytestmark = pytest.mark.gpu
+
+DT = {True: torch.bfloat16, False: torch.float16}
+
+
+# ---------------------------------------------------------------------------
+# append
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("byte", [0, 60, 94, 95, 191, 192, 255])
+@pytest.mark.parametrize("hkv,dim,rows", [(8, 128, 1), (3, 256, 1), (8, 128, 1100), (8, 128, 4200)])
+def test_append_reads_scales_outside_the_limits_as_every_reader_does(byte, hkv, dim, rows):
+    """A scale byte outside the limits reads as the nearest within (attention
+    and gather): an append that keeps tokens keeps those values, whichever way
+    its own scale compares, and leaves a byte within the limits."""
+    rng = np.random.default_rng(byte)
+    lead = [(5, -14), (9, -40), (15, 60)]  # (tokens kept, exponent of the new ones)
+    slots = [16 * (i + 1) + kept for i, (kept, _) in enumerate(lead)]
+    slots += list(range(64, 64 + rows - 1))
+    cs = (64 + rows + 31) // 16 * 16
+    codes, exps = random_pool(rng, cs, hkv, dim)
+    exps[:4] = byte
+    k = half(rng.standard_normal((len(slots), hkv, dim)), True)
+    for i, (_, e) in enumerate(lead):
+        k[i] *= 2.0 ** e
+    before = ref.values(codes, exps)
+    kp, vp = pool_of(codes, exps), pool_of(codes, exps)
+    kd = dev(k, torch.bfloat16)
+    fekv.append_kv8(None, kd, kd, kp, vp, dev(np.asarray(slots, np.int64)))
+    for pool in (kp, vp):
+        got_c, got_e = codes_of(pool), exps_of(pool)
+        got = ref.values(got_c, got_e)
+        for i, (kept, _) in enumerate(lead):
+            blk = i + 1
+            e = got_e[blk].astype(int) - 127
+            assert ((e >= ref.MIN_E) & (e <= ref.MAX_E)).all()
+            for h in range(hkv):
+                s = 2.0 ** e[h]
+                want = ref.decode_e4m3(ref.encode_e4m3(before[16 * blk:16 * blk + kept, h] / s)) * s
+                assert np.array_equal(got[16 * blk:16 * blk + kept, h], want)
+                need = max(ref.needed(float(np.abs(k[i, h].astype(np.float64)).max())),
+                           min(max(byte - 127, ref.MIN_E), ref.MAX_E))
+                assert e[h] == need
+    assert fekv.device_errors() == 0
