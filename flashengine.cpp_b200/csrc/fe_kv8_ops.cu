@@ -681,8 +681,9 @@ int fe_kv8_gather(const uint8_t* codes, const uint8_t* exps, void* out, const in
                   void* stream) {
   if (!valid_dtype(dtype)) return fail(FE_ERR_INVALID_ARGUMENT, "fe_kv8_gather: bad dtype");
   if (batch < 0 || max_len < 0 || page <= 0 || page % kKv8Block != 0 || hkv <= 0 || dim <= 0 ||
-      cache_slots <= 0)
-    return fail(FE_ERR_INVALID_ARGUMENT, "fe_kv8_gather: bad sizes (page a multiple of 16)");
+      cache_slots <= 0 || cache_slots % kKv8Block != 0)
+    return fail(FE_ERR_INVALID_ARGUMENT,
+                "fe_kv8_gather: bad sizes (page and cache_slots multiples of 16)");
   if (dim % 16 != 0 || int64_t(hkv) * dim > INT32_MAX / 2)
     return fail(FE_ERR_UNSUPPORTED, "fe_kv8_gather: head_dim must be a multiple of 16");
   if (batch == 0 || max_len == 0) return FE_OK;
