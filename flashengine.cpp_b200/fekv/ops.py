@@ -326,9 +326,9 @@ class Kv8Pool:
     exponents of the scales of 16 slots (value = code * 2 ** (exp - 127)).
     Both contiguous CUDA tensors on one device; they may be slices of larger
     tensors that hold all layers. A pool is made once and keeps its tensors,
-    so what a call needs of them (shape, addresses) is read here."""
+    so what a call needs of them (shape, device, addresses) is read here."""
 
-    __slots__ = ("codes", "exps", "shape", "device", "codes_ptr", "exps_ptr")
+    __slots__ = ("codes", "exps", "shape", "device", "index", "codes_ptr", "exps_ptr")
 
     def __init__(self, codes, exps):
         torch = _torch()
@@ -341,10 +341,11 @@ class Kv8Pool:
                 tuple(exps.shape) != (codes.shape[0] // _lib.FE_KV8_BLOCK, codes.shape[1]):
             raise ValueError(f"exps {tuple(exps.shape)} do not fit codes {tuple(codes.shape)}: "
                              "one row per 16 slots")
-        if exps.device != codes.device:
+        if exps.get_device() != codes.get_device():
             raise ValueError("codes and exps are on different devices")
         self.codes, self.exps = codes, exps
         self.shape, self.device = tuple(codes.shape), codes.device
+        self.index = codes.get_device()
         self.codes_ptr, self.exps_ptr = codes.data_ptr(), exps.data_ptr()
 
     @classmethod
@@ -363,22 +364,39 @@ class Kv8Pool:
 
 # These calls are short enough on the GPU that a decode step is bound by the
 # host; their checks read each tensor attribute once and pass plain integers.
+# Kernels run on the current device: what they are given has to be there.
 
-def _kv8_stream(stream):
+def _kv8_device():
+    return _torch()._C._cuda_getDevice()
+
+
+def _kv8_stream(stream, device):
     if stream is None:
-        c = _torch()._C
-        return c._cuda_getCurrentRawStream(c._cuda_getDevice())
+        return _torch()._C._cuda_getCurrentRawStream(device)
     return stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
 
 
-def _kv8_rows(name, t, dtype, shape):
-    """Address of a contiguous CUDA tensor of this dtype and shape."""
+def _kv8_rows(name, t, dtype, shape, device):
+    """Address of a contiguous tensor of this dtype and shape on CUDA device
+    `device`."""
     if t is None:
         raise ValueError(f"{name} is missing")
-    if t.dtype is dtype and t.shape == shape and t.is_cuda and t.is_contiguous():
+    if t.dtype is dtype and t.shape == shape and t.get_device() == device and t.is_contiguous():
         return t.data_ptr()
-    raise ValueError(f"{name}: expected a contiguous {dtype} CUDA tensor {tuple(shape)}, got "
-                     f"{t.dtype} {tuple(t.shape)} {tuple(t.stride())} on {t.device}")
+    raise ValueError(f"{name}: expected a contiguous {dtype} tensor {tuple(shape)} on the current "
+                     f"device (cuda:{device}), got {t.dtype} {tuple(t.shape)} {tuple(t.stride())} "
+                     f"on {t.device}")
+
+
+def _kv8_here(device, pools=(), lists=()):
+    """Pools and int32 lists of a call on CUDA device `device`."""
+    for p in pools:
+        if p.index != device:
+            raise ValueError(f"a pool is on {p.device}, the current device is cuda:{device}")
+    for t in lists:
+        _require_device_i32(t)
+        if t.get_device() != device:
+            raise ValueError(f"a list is on {t.device}, the current device is cuda:{device}")
 
 
 def append_kv8(q, k, v, kpool, vpool, slots, pos=None, cache=None, q_out=None, stream=None):
@@ -399,27 +417,29 @@ def append_kv8(q, k, v, kpool, vpool, slots, pos=None, cache=None, q_out=None, s
         code = FE_DTYPE_F16
     else:
         raise ValueError(f"k: expected float16 or bfloat16, got {dt}")
-    if not (k.is_cuda and k.is_contiguous()):
-        raise ValueError("k: expected a contiguous CUDA tensor")
-    vp = _kv8_rows("v", v, dt, shape)
+    device = _kv8_device()
+    if kpool.index != device or vpool.index != device:
+        _kv8_here(device, (kpool, vpool))
+    kp = _kv8_rows("k", k, dt, shape, device)
+    vp = _kv8_rows("v", v, dt, shape, device)
     hq = rot = most = 0
     qp = op = pp = cp = None
     if q is not None:
         qs = q.shape
         hq = qs[1] if len(qs) == 3 else -1
-        qp = op = _kv8_rows("q", q, dt, (rows, hq, dim))
+        qp = op = _kv8_rows("q", q, dt, (rows, hq, dim), device)
         if q_out is not None:
-            op = _kv8_rows("q_out", q_out, dt, qs)
-    sp = _kv8_rows("slots", slots, torch.int64, (rows,))
+            op = _kv8_rows("q_out", q_out, dt, qs, device)
+    sp = _kv8_rows("slots", slots, torch.int64, (rows,), device)
     if cache is not None:
         cs = cache.shape
         most, rot = cs
         if rot:
-            pp = _kv8_rows("pos", pos, torch.int64, (rows,))
-            cp = _kv8_rows("cache", cache, torch.float32, cs)
-    rc = _lib.load().fe_kv8_append(qp, op, k.data_ptr(), vp, kpool.codes_ptr, vpool.codes_ptr,
+            pp = _kv8_rows("pos", pos, torch.int64, (rows,), device)
+            cp = _kv8_rows("cache", cache, torch.float32, cs, device)
+    rc = _lib.load().fe_kv8_append(qp, op, kp, vp, kpool.codes_ptr, vpool.codes_ptr,
                                    kpool.exps_ptr, vpool.exps_ptr, sp, pp, cp, rows, hq, hkv, dim,
-                                   rot, most, code, pool[0], _kv8_stream(stream))
+                                   rot, most, code, pool[0], _kv8_stream(stream, device))
     if rc:
         check(rc, "append_kv8")
 
@@ -427,17 +447,18 @@ def append_kv8(q, k, v, kpool, vpool, slots, pos=None, cache=None, q_out=None, s
 def gather_kv8(pool, out, kv, pages, last, row_offset, max_len, page, stream=None):
     """Whole sequences' values from an 8-bit pool into rows of `out` [rows,
     hkv, dim] (16-bit), metadata as gather(): int32 CUDA tensors."""
-    for t in (kv, pages, last, row_offset):
-        _require_device_i32(t)
+    device = _kv8_device()
+    _kv8_here(device, (pool,), (kv, pages, last, row_offset))
     if not last.shape == row_offset.shape == (kv.shape[0] - 1,):
         raise ValueError("last and row_offset must have one entry per sequence, kv one more")
     _, hkv, dim = pool.shape
-    if not out.is_contiguous() or not out.is_cuda or out.numel() % (hkv * dim):
-        raise ValueError("out: expected a contiguous CUDA tensor [rows, hkv, dim]")
+    if not out.is_contiguous() or out.get_device() != device or out.numel() % (hkv * dim):
+        raise ValueError("out: expected a contiguous tensor [rows, hkv, dim] on the current device "
+                         f"(cuda:{device})")
     check(_lib.load().fe_kv8_gather(pool.codes_ptr, pool.exps_ptr, out.data_ptr(), kv.data_ptr(),
                                     pages.data_ptr(), last.data_ptr(), row_offset.data_ptr(),
                                     kv.shape[0] - 1, max_len, page, hkv, dim, dtype_code(out),
-                                    pool.shape[0], _kv8_stream(stream)), "gather_kv8")
+                                    pool.shape[0], _kv8_stream(stream, device)), "gather_kv8")
 
 
 def copy_blocks_kv8(k_pools, v_pools, src, dst, ntok, page, stream=None):
@@ -446,22 +467,24 @@ def copy_blocks_kv8(k_pools, v_pools, src, dst, ntok, page, stream=None):
     n = len(k_pools)
     if n != len(v_pools):
         raise ValueError("k_pools and v_pools differ in length")
-    for t in (src, dst, ntok):
-        _require_device_i32(t)
+    device = _kv8_device()
+    _kv8_here(device, lists=(src, dst, ntok))
     if not src.shape == dst.shape == ntok.shape:
         raise ValueError("src, dst and ntok differ in length")
     if n == 0:
         return
     shape = k_pools[0].shape
-    ptrs = [[p.codes_ptr for p in side if p.shape == shape] for side in (k_pools, v_pools)] + \
+    ptrs = [[p.codes_ptr for p in side if p.index == device and p.shape == shape]
+            for side in (k_pools, v_pools)] + \
         [[p.exps_ptr for p in side] for side in (k_pools, v_pools)]
     if len(ptrs[0]) != n or len(ptrs[1]) != n:
+        _kv8_here(device, (*k_pools, *v_pools))
         raise ValueError("the layers' pools differ in shape")
     arrays = [array.array("Q", p) for p in ptrs]
     check(_lib.load().fe_kv8_copy_blocks(*[a.buffer_info()[0] for a in arrays], n, src.data_ptr(),
                                          dst.data_ptr(), ntok.data_ptr(), src.shape[0], page,
                                          shape[1], shape[2], shape[0] // page,
-                                         _kv8_stream(stream)), "copy_blocks_kv8")
+                                         _kv8_stream(stream, device)), "copy_blocks_kv8")
 
 
 class Kv8Plan(AttentionPlan):
@@ -476,6 +499,7 @@ class Kv8Plan(AttentionPlan):
         self.pool_shape = ((int(blocks) + 1) * int(page), int(hkv), int(dim))
         self.dtype = torch.bfloat16 if bf16 else torch.float16
         self.rows = 0  # query rows of the last prepare
+        self.index = _kv8_device()
 
     def prepare(self, qo, kv, pages, last, batch=None, rows=None, graph=False, stream=None):
         super().prepare(qo, kv, pages, last, batch, rows, graph, stream)
@@ -497,10 +521,18 @@ class Kv8Plan(AttentionPlan):
         shape = (q.shape[0], self.hq, self.dim)
         if shape[0] < self.rows:
             raise ValueError(f"q has {shape[0]} rows, the plan was prepared for {self.rows}")
-        check(self.lib.fe_kv8_attn_run(self.handle, _kv8_rows("q", q, self.dtype, shape),
+        device = _kv8_device()
+        if self.index != device:
+            raise ValueError(f"the plan is for cuda:{self.index}, the current device is "
+                             f"cuda:{device}")
+        if kpool.index != device or vpool.index != device:
+            _kv8_here(device, (kpool, vpool))
+        check(self.lib.fe_kv8_attn_run(self.handle, _kv8_rows("q", q, self.dtype, shape, device),
                                        kpool.codes_ptr, vpool.codes_ptr, kpool.exps_ptr,
-                                       vpool.exps_ptr, _kv8_rows("out", out, self.dtype, shape),
-                                       1 if causal else 0, _kv8_stream(stream)), "attention")
+                                       vpool.exps_ptr,
+                                       _kv8_rows("out", out, self.dtype, shape, device),
+                                       1 if causal else 0, _kv8_stream(stream, device)),
+              "attention")
 
 
 def create_plan(hq, hkv, dim, page, max_batch, max_pages, bf16, blocks) -> AttentionPlan:

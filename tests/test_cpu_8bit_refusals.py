@@ -12,3 +12,102 @@ def test_gather_refuses_slots_without_a_scale_of_their_own(cs):
     """One scale row per 16 slots: a pool's last slots would read past them."""
     assert fekv.load().fe_kv8_gather(*gather_args(cs=cs)) == _lib.FE_ERR_INVALID_ARGUMENT
     assert b"cache_slots" in fekv.load().fe_last_error()
+
+
+# ---------------------------------------------------------------------------
+# tensors that are not on the current device
+# ---------------------------------------------------------------------------
+
+torch = pytest.importorskip("torch")
+
+
+class Placed(torch.Tensor):
+    """A CPU tensor that says it is on CUDA device `where`."""
+
+    is_cuda = True
+
+    def get_device(self):
+        return self.where
+
+
+def placed(t, where):
+    t = t.as_subclass(Placed)
+    t.where = where
+    return t
+
+
+class Calls:
+    """Stands in for the library: every call succeeds and is counted."""
+
+    def __init__(self):
+        self.count = 0
+
+    def __getattr__(self, name):
+        def call(*args):
+            self.count += 1
+            return 0
+
+        return call
+
+
+@pytest.fixture
+def lib(monkeypatch):
+    from fekv import ops
+
+    calls = Calls()
+    monkeypatch.setattr(ops._lib, "load", lambda: calls)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda d: 0, raising=False)
+    return calls
+
+
+def pool(where):
+    return fekv.Kv8Pool(placed(torch.zeros(48, 2, 128, dtype=torch.float8_e4m3fn), where),
+                        placed(torch.zeros(3, 2, dtype=torch.uint8), where))
+
+
+def append_call(**at):
+    where = lambda name: at.get(name, 0)  # noqa: E731
+    t = lambda name, *shape, dtype=torch.bfloat16: placed(  # noqa: E731
+        torch.zeros(*shape, dtype=dtype), where(name))
+    fekv.append_kv8(t("q", 3, 4, 128), t("k", 3, 2, 128), t("v", 3, 2, 128), pool(where("kpool")),
+                    pool(where("vpool")), t("slots", 3, dtype=torch.int64),
+                    t("pos", 3, dtype=torch.int64), t("cache", 8, 64, dtype=torch.float32),
+                    q_out=t("q_out", 3, 4, 128))
+
+
+def gather_call(**at):
+    t = lambda name, *v: placed(torch.tensor(v, dtype=torch.int32), at.get(name, 0))  # noqa: E731
+    out = placed(torch.zeros(16, 2, 128, dtype=torch.bfloat16), at.get("out", 0))
+    fekv.gather_kv8(pool(at.get("pool", 0)), out, t("kv", 0, 1), t("pages", 1), t("last", 5),
+                    t("offset", 0), 5, 16)
+
+
+def copy_call(**at):
+    t = lambda name: placed(torch.zeros(1, dtype=torch.int32), at.get(name, 0))  # noqa: E731
+    fekv.copy_blocks_kv8([pool(0), pool(at.get("kpool", 0))], [pool(at.get("vpool", 0)), pool(0)],
+                         t("src"), t("dst"), t("ntok"), 16)
+
+
+def attention_call(**at):
+    plan = fekv.Kv8Plan.__new__(fekv.Kv8Plan)
+    plan.lib, plan.handle, plan.rows = fekv.ops._lib.load(), None, 3
+    plan.hq, plan.dim, plan.pool_shape, plan.dtype = 4, 128, (48, 2, 128), torch.bfloat16
+    plan.index = at.get("plan", 0)
+    t = lambda name: placed(torch.zeros(3, 4, 128, dtype=torch.bfloat16), at.get(name, 0))  # noqa: E731
+    plan.attention(t("q"), pool(at.get("kpool", 0)), pool(at.get("vpool", 0)), t("out"))
+
+
+@pytest.mark.parametrize("call,names", [
+    (append_call, "q k v kpool vpool slots pos cache q_out"),
+    (gather_call, "pool out kv pages last offset"),
+    (copy_call, "kpool vpool src dst ntok"),
+    (attention_call, "plan q kpool vpool out")])
+def test_what_is_on_another_device_is_refused(lib, call, names):
+    call()  # all on the current device
+    count = lib.count
+    for name in names.split():
+        for where in (1, -1):
+            with pytest.raises(ValueError, match="current device|contiguous"):
+                call(**{name: where})
+    assert lib.count == count  # nothing was launched
