@@ -487,6 +487,13 @@ def copy_blocks_kv8(k_pools, v_pools, src, dst, ntok, page, stream=None):
                                          _kv8_stream(stream, device)), "copy_blocks_kv8")
 
 
+def _kv8_metadata(qo, kv, last, batch):
+    """The lengths that a prepare of `batch` sequences reads."""
+    if batch < 0 or qo.shape[0] <= batch or kv.shape[0] <= batch or last.shape[0] < batch:
+        raise ValueError(f"{batch} sequences need {batch + 1} entries of qo and kv and {batch} of "
+                         f"last, got {qo.shape[0]}, {kv.shape[0]} and {last.shape[0]}")
+
+
 class Kv8Plan(AttentionPlan):
     """An attention plan over 8-bit pools: prepared like any other plan;
     `attention` takes Kv8Pools. bf16: the dtype of q and out."""
@@ -501,16 +508,38 @@ class Kv8Plan(AttentionPlan):
         self.rows = 0  # query rows of the last prepare
         self.index = _kv8_device()
 
+    def _device(self):
+        """The current device, which has to be the plan's."""
+        device = _kv8_device()
+        if self.index != device:
+            raise ValueError(f"the plan is for cuda:{self.index}, the current device is "
+                             f"cuda:{device}")
+        return device
+
     def prepare(self, qo, kv, pages, last, batch=None, rows=None, graph=False, stream=None):
+        self._device()
+        qo, kv, pages, last = _host_i32(qo), _host_i32(kv), _host_i32(pages), _host_i32(last)
+        batch = kv.shape[0] - 1 if batch is None else int(batch)
+        _kv8_metadata(qo, kv, last, batch)
+        if pages.shape[0] < kv[batch]:
+            raise ValueError(f"{pages.shape[0]} pages, kv counts {kv[batch]}")
         super().prepare(qo, kv, pages, last, batch, rows, graph, stream)
-        self.rows = int(qo[len(kv) - 1 if batch is None else batch])
+        self.rows = int(qo[batch])
 
     def prepare_device(self, qo, kv, pages, last, batch, rows, stream=None):
+        _kv8_here(self._device(), lists=(qo, kv, pages, last))
+        _kv8_metadata(qo, kv, last, int(batch))
         super().prepare_device(qo, kv, pages, last, batch, rows, stream)
         self.rows = int(rows)
 
     def step_prepare_device(self, block_tables, starts, rows_per_seq, slots, positions,
                             stream=None):
+        device = self._device()
+        _kv8_here(device, lists=(block_tables, starts))
+        for t in (slots, positions):
+            if t.get_device() != device or not t.is_contiguous():
+                raise ValueError("slots / positions: contiguous int64 tensors on the current "
+                                 f"device (cuda:{device})")
         super().step_prepare_device(block_tables, starts, rows_per_seq, slots, positions, stream)
         self.rows = int(block_tables.shape[0]) * int(rows_per_seq)
 
@@ -521,10 +550,7 @@ class Kv8Plan(AttentionPlan):
         shape = (q.shape[0], self.hq, self.dim)
         if shape[0] < self.rows:
             raise ValueError(f"q has {shape[0]} rows, the plan was prepared for {self.rows}")
-        device = _kv8_device()
-        if self.index != device:
-            raise ValueError(f"the plan is for cuda:{self.index}, the current device is "
-                             f"cuda:{device}")
+        device = self._device()
         if kpool.index != device or vpool.index != device:
             _kv8_here(device, (kpool, vpool))
         check(self.lib.fe_kv8_attn_run(self.handle, _kv8_rows("q", q, self.dtype, shape, device),

@@ -89,11 +89,16 @@ def copy_call(**at):
                          t("src"), t("dst"), t("ntok"), 16)
 
 
-def attention_call(**at):
+def bare_plan(index=0):
     plan = fekv.Kv8Plan.__new__(fekv.Kv8Plan)
     plan.lib, plan.handle, plan.rows = fekv.ops._lib.load(), None, 3
     plan.hq, plan.dim, plan.pool_shape, plan.dtype = 4, 128, (48, 2, 128), torch.bfloat16
-    plan.index = at.get("plan", 0)
+    plan.index = index
+    return plan
+
+
+def attention_call(**at):
+    plan = bare_plan(at.get("plan", 0))
     t = lambda name: placed(torch.zeros(3, 4, 128, dtype=torch.bfloat16), at.get(name, 0))  # noqa: E731
     plan.attention(t("q"), pool(at.get("kpool", 0)), pool(at.get("vpool", 0)), t("out"))
 
@@ -111,3 +116,59 @@ def test_what_is_on_another_device_is_refused(lib, call, names):
             with pytest.raises(ValueError, match="current device|contiguous"):
                 call(**{name: where})
     assert lib.count == count  # nothing was launched
+
+
+# ---------------------------------------------------------------------------
+# metadata shorter than a prepare reads
+# ---------------------------------------------------------------------------
+
+META = dict(qo=(0, 2, 3, 3), kv=(0, 2, 3, 4), pages=(5, 1, 2, 7), last=(16, 3, 1))
+
+
+def host_prepare(batch=None, **kw):
+    m = {**META, **kw}
+    bare_plan(m.pop("plan", 0)).prepare(m["qo"], m["kv"], m["pages"], m["last"], batch, stream=0)
+
+
+def device_prepare(batch=3, where=None, plan=0, **kw):
+    m = {n: placed(torch.tensor(v, dtype=torch.int32), int(n == where))
+         for n, v in {**META, **kw}.items()}
+    bare_plan(plan).prepare_device(m["qo"], m["kv"], m["pages"], m["last"], batch, 3, stream=0)
+
+
+def step_prepare(plan=0, where=None, slots=None):
+    t = {n: placed(torch.zeros(*shape, dtype=dt), int(n == where))
+         for n, shape, dt in (("tables", (3, 4), torch.int32), ("starts", (3,), torch.int32),
+                              ("slots", (6,), torch.int64), ("positions", (6,), torch.int64))}
+    bare_plan(plan).step_prepare_device(t["tables"], t["starts"], 2,
+                                        t["slots"] if slots is None else slots, t["positions"],
+                                        stream=0)
+
+
+@pytest.mark.parametrize("prepare,wrong", [
+    (host_prepare, dict(qo=(0, 2, 3))), (host_prepare, dict(last=(16, 3))),
+    (host_prepare, dict(pages=(5, 1, 2))), (host_prepare, dict(batch=4)),
+    (host_prepare, dict(batch=-1)), (host_prepare, dict(plan=1)),
+    (device_prepare, dict(qo=(0, 2, 3))), (device_prepare, dict(kv=(0, 2, 3))),
+    (device_prepare, dict(last=(16, 3))), (device_prepare, dict(batch=4)),
+    (device_prepare, dict(batch=-1)), (device_prepare, dict(plan=1)),
+    *((device_prepare, dict(where=n)) for n in META),
+    *((step_prepare, dict(where=n)) for n in ("tables", "starts", "slots", "positions")),
+    (step_prepare, dict(plan=1)),
+    (step_prepare, dict(slots=placed(torch.zeros(1, dtype=torch.int64), 0))),
+    (step_prepare, "strided")])
+def test_prepares_refuse_what_they_would_read_or_write_past(lib, prepare, wrong):
+    if wrong == "strided":
+        wrong = dict(slots=placed(torch.zeros(1, dtype=torch.int64).expand(6), 0))
+    prepare()
+    count = lib.count
+    with pytest.raises(ValueError):
+        prepare(**wrong)
+    assert lib.count == count
+
+
+def test_a_prepare_of_part_of_the_metadata_is_taken(lib):
+    host_prepare(batch=2)
+    device_prepare(batch=2)
+    host_prepare(pages=(5, 1, 2, 7, 9))
+    assert lib.count == 3
