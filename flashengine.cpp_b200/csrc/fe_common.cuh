@@ -151,19 +151,6 @@ __device__ __forceinline__ bool mbar_try_wait_short(uint64_t* bar, uint32_t pari
   return ok != 0;
 }
 
-// Whether a phase has completed, without waiting.
-__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-
 // 3-D tiled TMA load global -> shared (this CTA's own shared memory only),
 // completion signalled on `bar` via complete_tx.
 __device__ __forceinline__ void tma_load_3d(void* smem_dst, const CUtensorMap* map, uint64_t* bar,
