@@ -476,20 +476,22 @@ __global__ void __launch_bounds__(kThreads, 4)
                       T* __restrict__ out, const int32_t* __restrict__ kv,
                       const int32_t* __restrict__ pages, const int32_t* __restrict__ last,
                       const int32_t* __restrict__ row_offset, int page, int hkv, int dim,
-                      int64_t cache_slots, unsigned int* err) {
+                      int64_t cache_slots, int64_t out_rows, int num_pages, unsigned int* err) {
   pdl_trigger();
   pdl_wait();
   const int b = blockIdx.y;
   const int p0 = __ldg(kv + b), p1 = __ldg(kv + b + 1);
   if (p1 <= p0) return;
   const int tail = __ldg(last + b);
-  const int64_t tokens = int64_t(p1 - p0 - 1) * page + tail;
-  if (tail < 1 || tail > page || tokens > INT32_MAX / 2) {
+  const int64_t orow = __ldg(row_offset + b);
+  const int64_t tokens = (int64_t(p1) - p0 - 1) * page + tail;
+  // its pages within the list, its rows within `out`
+  if (tail < 1 || tail > page || tokens > INT32_MAX / 2 || p0 < 0 || p1 > num_pages || orow < 0 ||
+      tokens > out_rows - orow) {
     if (threadIdx.x == 0 && blockIdx.x == 0) raise_device_error(err, FE_DEVERR_PAGE_RANGE);
     return;
   }
   const int len = static_cast<int>(tokens);
-  const int64_t orow = __ldg(row_offset + b);
   const int lane = threadIdx.x & 31;
   const int chunks = hkv * dim / 16;
   const int step = gridDim.x * kWarps * kGatherTok;
@@ -679,9 +681,18 @@ int fe_kv8_gather(const uint8_t* codes, const uint8_t* exps, void* out, const in
                   const int32_t* pages, const int32_t* last, const int32_t* row_offset, int batch,
                   int max_len, int page, int hkv, int dim, int dtype, int64_t cache_slots,
                   void* stream) {
+  return fe_kv8_gather_within(codes, exps, out, INT64_MAX, kv, pages, INT32_MAX, last, row_offset,
+                              batch, max_len, page, hkv, dim, dtype, cache_slots, stream);
+}
+
+int fe_kv8_gather_within(const uint8_t* codes, const uint8_t* exps, void* out, int64_t out_rows,
+                         const int32_t* kv, const int32_t* pages, int num_pages,
+                         const int32_t* last, const int32_t* row_offset, int batch, int max_len,
+                         int page, int hkv, int dim, int dtype, int64_t cache_slots,
+                         void* stream) {
   if (!valid_dtype(dtype)) return fail(FE_ERR_INVALID_ARGUMENT, "fe_kv8_gather: bad dtype");
   if (batch < 0 || max_len < 0 || page <= 0 || page % kKv8Block != 0 || hkv <= 0 || dim <= 0 ||
-      cache_slots <= 0 || cache_slots % kKv8Block != 0)
+      cache_slots <= 0 || cache_slots % kKv8Block != 0 || out_rows < 0 || num_pages < 0)
     return fail(FE_ERR_INVALID_ARGUMENT,
                 "fe_kv8_gather: bad sizes (page and cache_slots multiples of 16)");
   if (dim % 16 != 0 || int64_t(hkv) * dim > INT32_MAX / 2)
@@ -702,11 +713,12 @@ int fe_kv8_gather(const uint8_t* codes, const uint8_t* exps, void* out, const in
   if (dtype == FE_DTYPE_BF16)
     FE_CUDA_TRY(launch_pdl(kv8_gather_kernel<__nv_bfloat16>, grid, dim3(kThreads), 0, s, codes,
                            exps, static_cast<__nv_bfloat16*>(out), kv, pages, last, row_offset,
-                           page, hkv, dim, cache_slots, device_error_word()));
+                           page, hkv, dim, cache_slots, out_rows, num_pages,
+                           device_error_word()));
   else
     FE_CUDA_TRY(launch_pdl(kv8_gather_kernel<__half>, grid, dim3(kThreads), 0, s, codes, exps,
                            static_cast<__half*>(out), kv, pages, last, row_offset, page, hkv, dim,
-                           cache_slots, device_error_word()));
+                           cache_slots, out_rows, num_pages, device_error_word()));
   return FE_OK;
 }
 

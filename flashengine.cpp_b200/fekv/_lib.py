@@ -68,6 +68,8 @@ SIGNATURES = {
     "fe_paged_decode_noalloc": (_I, [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P]),
     "fe_kv8_append": (_I, [_P] * 11 + [_I] * 7 + [_I64, _P]),
     "fe_kv8_gather": (_I, [_P] * 7 + [_I] * 6 + [_I64, _P]),
+    "fe_kv8_gather_within": (_I, [_P] * 3 + [_I64] + [_P] * 2 + [_I] + [_P] * 2 + [_I] * 6 +
+                             [_I64, _P]),
     "fe_kv8_copy_blocks": (_I, [_P] * 4 + [_I] + [_P] * 3 + [_I] * 5 + [_P]),
     "fe_kv8_plan_create": (_I, [_I, _I, _I, _I, _I, _I, _I, _I, ctypes.POINTER(_P)]),
     "fe_kv8_plan_create_host": (_I, [_I, _I, _I, _I, _I, _I, _I, _I, _I, ctypes.POINTER(_P)]),

@@ -446,7 +446,9 @@ def append_kv8(q, k, v, kpool, vpool, slots, pos=None, cache=None, q_out=None, s
 
 def gather_kv8(pool, out, kv, pages, last, row_offset, max_len, page, stream=None):
     """Whole sequences' values from an 8-bit pool into rows of `out` [rows,
-    hkv, dim] (16-bit), metadata as gather(): int32 CUDA tensors."""
+    hkv, dim] (16-bit), metadata as gather(): int32 CUDA tensors. A sequence
+    whose rows reach past `out`, or whose pages past `pages`, is skipped and
+    flagged (device_errors)."""
     device = _kv8_device()
     _kv8_here(device, (pool,), (kv, pages, last, row_offset))
     if not last.shape == row_offset.shape == (kv.shape[0] - 1,):
@@ -455,10 +457,12 @@ def gather_kv8(pool, out, kv, pages, last, row_offset, max_len, page, stream=Non
     if not out.is_contiguous() or out.get_device() != device or out.numel() % (hkv * dim):
         raise ValueError("out: expected a contiguous tensor [rows, hkv, dim] on the current device "
                          f"(cuda:{device})")
-    check(_lib.load().fe_kv8_gather(pool.codes_ptr, pool.exps_ptr, out.data_ptr(), kv.data_ptr(),
-                                    pages.data_ptr(), last.data_ptr(), row_offset.data_ptr(),
-                                    kv.shape[0] - 1, max_len, page, hkv, dim, dtype_code(out),
-                                    pool.shape[0], _kv8_stream(stream, device)), "gather_kv8")
+    check(_lib.load().fe_kv8_gather_within(pool.codes_ptr, pool.exps_ptr, out.data_ptr(),
+                                           out.numel() // (hkv * dim), kv.data_ptr(),
+                                           pages.data_ptr(), pages.shape[0], last.data_ptr(),
+                                           row_offset.data_ptr(), kv.shape[0] - 1, max_len, page,
+                                           hkv, dim, dtype_code(out), pool.shape[0],
+                                           _kv8_stream(stream, device)), "gather_kv8")
 
 
 def copy_blocks_kv8(k_pools, v_pools, src, dst, ntok, page, stream=None):

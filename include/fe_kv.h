@@ -313,15 +313,21 @@ int fe_kv8_append(const void* q, void* q_out, const void* k, const void* v, uint
 /* fe_kv_gather from an 8-bit pool: the values, rounded to the 16-bit `dtype`
  * (bf16 holds every one exactly). A page id that reaches past cache_slots
  * leaves its token unwritten and raises FE_DEVERR_PAGE_RANGE, a `last` outside
- * [1, page] its sequence. cache_slots is a multiple of 16. max_len sizes the
- * launch: longer sequences are covered by striding, 0 gathers nothing. Neither
- * the rows of `out` nor the entries of `pages` are known to the call: rows
- * row_offset[b] .. + length of sequence b have to lie in `out`, and kv[batch]
- * page ids in `pages`. */
+ * [1, page] or a negative list entry its sequence. cache_slots is a multiple of
+ * 16. max_len sizes the launch: longer sequences are covered by striding, 0
+ * gathers nothing. Neither the rows of `out` nor the entries of `pages` are
+ * known to fe_kv8_gather: rows row_offset[b] .. + length of sequence b have to
+ * lie in `out`, and kv[batch] page ids in `pages`. fe_kv8_gather_within is told
+ * both, and skips a sequence that reaches past either (FE_DEVERR_PAGE_RANGE). */
 int fe_kv8_gather(const uint8_t* codes, const uint8_t* exps, void* out, const int32_t* kv,
                   const int32_t* pages, const int32_t* last, const int32_t* row_offset, int batch,
                   int max_len, int page, int hkv, int dim, int dtype, int64_t cache_slots,
                   void* stream);
+int fe_kv8_gather_within(const uint8_t* codes, const uint8_t* exps, void* out, int64_t out_rows,
+                         const int32_t* kv, const int32_t* pages, int num_pages,
+                         const int32_t* last, const int32_t* row_offset, int batch, int max_len,
+                         int page, int hkv, int dim, int dtype, int64_t cache_slots,
+                         void* stream);
 
 /* fe_kv_copy_blocks for 8-bit pools: token rows [0, ntok[c]) of page src[c]
  * onto page dst[c], and the scales of the blocks they lie in, in every layer's

@@ -14,6 +14,14 @@ def test_gather_refuses_slots_without_a_scale_of_their_own(cs):
     assert b"cache_slots" in fekv.load().fe_last_error()
 
 
+@pytest.mark.parametrize("out_rows,num_pages,status", [
+    (-1, 1, _lib.FE_ERR_INVALID_ARGUMENT), (4, -1, _lib.FE_ERR_INVALID_ARGUMENT)])
+def test_gather_refuses_negative_sizes(out_rows, num_pages, status):
+    codes, exps, out, kv, pages, *rest = gather_args()
+    assert fekv.load().fe_kv8_gather_within(codes, exps, out, out_rows, kv, pages, num_pages,
+                                            *rest) == status
+
+
 # ---------------------------------------------------------------------------
 # tensors that are not on the current device
 # ---------------------------------------------------------------------------

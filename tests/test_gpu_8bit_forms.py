@@ -7,6 +7,7 @@ torch = pytest.importorskip("torch")
 
 import fekv
 import kv8_ref as ref
+from fekv import _lib
 from test_gpu_kv8 import codes_of, dev, exps_of, half, pool_of, random_pool
 
 pytestmark = pytest.mark.gpu
@@ -53,3 +54,35 @@ def test_append_reads_scales_outside_the_limits_as_every_reader_does(byte, hkv, 
                            min(max(byte - 127, ref.MIN_E), ref.MAX_E))
                 assert e[h] == need
     assert fekv.device_errors() == 0
+
+
+# ---------------------------------------------------------------------------
+# gather
+# ---------------------------------------------------------------------------
+
+def i32(*a):
+    return torch.tensor(a, dtype=torch.int32, device="cuda")
+
+
+@pytest.mark.parametrize("kv,pages,offset", [
+    ((0, 2, 4, 6), range(6), (0, 32, 65)),       # the last sequence: one row past `out`
+    ((0, 2, 4, 6), range(6), (0, 32, 2 ** 30)),
+    ((0, 2, 4, 6), range(6), (0, 32, -1)),
+    ((0, 2, 4, 7), range(6), (0, 32, 64)),       # one page past the list
+    ((0, 2, 4, 2 ** 24), range(6), (0, 32, 64)),
+    ((-2, 2, 4, 6), range(6), (64, 32, 0))])     # the first sequence: before the list
+def test_gather_stays_within_its_arrays(kv, pages, offset):
+    """A sequence whose rows reach past `out`, or whose pages past the list,
+    is skipped and flagged; the others are gathered, nothing else is written."""
+    rng = np.random.default_rng(2)
+    codes, exps = random_pool(rng, 8 * 16, 2, 128)
+    buf = torch.full((200, 2, 128), 5.0, device="cuda", dtype=torch.float16)
+    fekv.gather_kv8(pool_of(codes, exps), buf[50:146], i32(*kv), i32(*pages), i32(16, 16, 16),
+                    i32(*offset), 32, 16)
+    got = buf.float().cpu().numpy()
+    want = np.full(got.shape, 5.0)
+    val = ref.values(codes, exps)
+    for b in (1, 2) if kv[0] < 0 else (0, 1):
+        want[50 + offset[b]:82 + offset[b]] = val[16 * kv[b]:16 * kv[b] + 32]
+    assert np.array_equal(got, half(want, False))
+    assert fekv.device_errors() == _lib.FE_DEVERR_PAGE_RANGE
