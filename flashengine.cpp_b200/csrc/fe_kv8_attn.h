@@ -20,7 +20,8 @@ int kv8_decode_launch(int dtype, int dim, int heads, const CUtensorMap& kmap,
                       const CUtensorMap& vmap, const void* args, int grid, cudaStream_t stream);
 // Merge the split units of a work list: `units` of them (an upper bound under a
 // fixed launch geometry) of at most `rows` record rows; `pieces`: records of the
-// most split unit, or an estimate; at most about `max_blocks` blocks.
+// most split unit, or an estimate (it sizes the grid only); at most about
+// `max_blocks` blocks.
 int kv8_merge_launch(int dtype, int dim, int list, const void* args, int units, int rows,
                      int pieces, int max_blocks, cudaStream_t stream, bool pdl);
 int kv8_rows_launch(int dtype, int dim, const CUtensorMap& kmap, const CUtensorMap& vmap,

@@ -661,14 +661,26 @@ int dispatch(int dim, int heads, const CUtensorMap& kmap, const CUtensorMap& vma
 // `per_row` warps of a block share a row, each taking every per_row-th piece
 // with up to eight O vectors in flight, and join through shared memory: one
 // long sequence has a record per CTA, and a warp that walked 128 of them alone
-// took longer than the attention. gridDim.x blocks stride over the units,
-// gridDim.y over a unit's rows.
+// took longer than the attention. per_row follows from the unit's pieces alone,
+// not from the launch, so that the sums' order, and with it the bits, are the
+// same for a plan of the host and one of the device with the same cuts.
+// gridDim.x blocks stride over the units, gridDim.y over a unit's rows.
 // ---------------------------------------------------------------------------
 constexpr int kMergeWarps = 8;
 
+// One warp a row up to eight pieces, then as many as leave each about eight.
+// Whole calls in us on a B200 with always one, this rule, always eight:
+// a sequence of 8192 keys 22.0, 10.2, 10.2; 64 of 512 to 4096 keys 45.6,
+// 45.6, 60.1; a 1024-row chunk over 8192 keys 159.6, 159.8, 262.5.
+__host__ __device__ __forceinline__ int merge_warps_per_row(int pieces) {
+  int n = 1;
+  while (n < kMergeWarps && pieces > 8 * n) n *= 2;
+  return n;
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kMergeWarps * 32)
-    kv8_merge_kernel(const AttnArgs<T> a, int list, int per_row) {
+    kv8_merge_kernel(const AttnArgs<T> a, int list) {
   constexpr int kV = D / 128;  // float4 per lane
   __shared__ float4 part[kMergeWarps][32 * kV];
   __shared__ float2 stat[kMergeWarps];
@@ -686,16 +698,17 @@ __global__ void __launch_bounds__(kMergeWarps * 32)
   }
   pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int sub = warp % per_row, rows = kMergeWarps / per_row;
   for (int u = blockIdx.x; u < n; u += gridDim.x) {
     if (u != static_cast<int>(blockIdx.x)) {
       g = groups[u];
       if (g.nsplit >= 2) si = seqs[g.seq];
     }
     if (g.nsplit < 2) continue;  // placeholder ids of the row lists
+    const int per_row = merge_warps_per_row(g.nsplit);
+    const int sub = warp & (per_row - 1), rows = kMergeWarps / per_row;
     const int rph = g.rows_per_head > 0 ? g.rows_per_head : si.qrows * a.G;
     for (int r0 = blockIdx.y * rows; r0 < g.rows; r0 += gridDim.y * rows) {
-      const int r = r0 + warp / per_row;
+      const int r = r0 + (warp - sub) / per_row;
       float M = -INFINITY, L = 0.f;
       float4 acc[kV];
 #pragma unroll
@@ -813,21 +826,16 @@ __global__ void __launch_bounds__(kMergeWarps * 32)
 template <typename T>
 int merge_launch(int dim, int list, const AttnArgs<T>& a, int units, int rows, int pieces,
                  int max_blocks, cudaStream_t stream, bool pdl) {
-  // One warp a row up to eight pieces, then as many as leave each about eight.
-  // Whole calls in us on a B200 with always one, this rule, always eight:
-  // a sequence of 8192 keys 22.0, 10.2, 10.2; 64 of 512 to 4096 keys 45.6,
-  // 45.6, 60.1; a 1024-row chunk over 8192 keys 159.6, 159.8, 262.5.
-  int per_row = 1;
-  while (per_row < kMergeWarps && pieces > 8 * per_row) per_row *= 2;
-  const int per_block = kMergeWarps / per_row;
+  // blocks for the rows of the most split unit
+  const int per_block = kMergeWarps / merge_warps_per_row(pieces);
   const dim3 grid(units, std::min((rows + per_block - 1) / per_block,
                                   std::max(1, max_blocks / units)));
   auto kernel = dim == kWideHeadDim ? kv8_merge_kernel<T, kWideHeadDim>
                                     : kv8_merge_kernel<T, kHeadDim>;
   if (pdl) {
-    FE_CUDA_TRY(launch_pdl(kernel, grid, dim3(kMergeWarps * 32), 0, stream, a, list, per_row));
+    FE_CUDA_TRY(launch_pdl(kernel, grid, dim3(kMergeWarps * 32), 0, stream, a, list));
   } else {
-    kernel<<<grid, kMergeWarps * 32, 0, stream>>>(a, list, per_row);
+    kernel<<<grid, kMergeWarps * 32, 0, stream>>>(a, list);
     FE_CUDA_TRY(cudaGetLastError());
   }
   return FE_OK;

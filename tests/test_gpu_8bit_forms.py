@@ -6,9 +6,10 @@ import pytest
 torch = pytest.importorskip("torch")
 
 import fekv
+import kv8_bounds as bounds
 import kv8_ref as ref
 from fekv import _lib
-from test_gpu_kv8 import codes_of, dev, exps_of, half, pool_of, random_pool
+from test_gpu_kv8 import Step, codes_of, dev, exps_of, half, pool_of, random_pool
 
 pytestmark = pytest.mark.gpu
 
@@ -86,3 +87,32 @@ def test_gather_stays_within_its_arrays(kv, pages, offset):
         want[50 + offset[b]:82 + offset[b]] = val[16 * kv[b]:16 * kv[b] + 32]
     assert np.array_equal(got, half(want, False))
     assert fekv.device_errors() == _lib.FE_DEVERR_PAGE_RANGE
+
+
+# ---------------------------------------------------------------------------
+# attention, within the bound of each rounding that the kernels make
+# ---------------------------------------------------------------------------
+
+def check(st, causal, got=None):
+    got = st.run(causal) if got is None else got
+    want, bound = bounds.attention(st.q, *st.pools, st.md, st.hq, st.hkv, st.page, causal, st.bf16)
+    over = np.abs(got - want) / bound
+    assert np.isfinite(got).all()
+    assert over.max() <= 1, (over.max(), np.unravel_index(over.argmax(), over.shape))
+
+
+# ---------------------------------------------------------------------------
+# plans: prepared on the device, for replay
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("rows", [1, 3, 40])
+@pytest.mark.parametrize("hkv", [4, 3])
+@pytest.mark.parametrize("bf16", [True, False])
+def test_device_prepare_at_256_dims(rows, hkv, bf16):
+    rng = np.random.default_rng(24)
+    st = Step(rng, 4 * hkv, hkv, 256, 16, [900, 64, 333, 41], [rows] * 4, bf16)
+    host, device = st.run(True), st.run(True, st.plan(device=True))
+    if rows * 4 <= 16:
+        assert np.array_equal(host, device)  # the same cuts
+    check(st, True, device)
+    check(st, False, st.run(False, st.plan(device=True)))
