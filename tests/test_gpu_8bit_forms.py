@@ -9,7 +9,9 @@ import fekv
 import kv8_bounds as bounds
 import kv8_ref as ref
 from fekv import _lib
-from test_gpu_kv8 import Step, codes_of, dev, exps_of, half, pool_of, random_pool
+from fekv.metadata import build_step_metadata
+from test_gpu_kv8 import (HEADS, Step, codes_of, dev, exps_of, half, pool_of, random_pool,
+                          rope_cache, run_append, step_slots)
 
 pytestmark = pytest.mark.gpu
 
@@ -57,6 +59,30 @@ def test_append_reads_scales_outside_the_limits_as_every_reader_does(byte, hkv, 
     assert fekv.device_errors() == 0
 
 
+# Rows times heads choose the append's form: up to 2 Ki pairs K and V have warps
+# of their own, up to 8 Ki they share one, then windows of 4 rows, from 32 Ki 16.
+@pytest.mark.parametrize("bf16", [True, False])
+@pytest.mark.parametrize("hkv,dim,rot,rows", [
+    (8, 128, 128, 150), (8, 128, 64, 600), (8, 128, 128, 900), (8, 128, 128, 1500),
+    (8, 128, 0, 4300), (8, 128, 128, 4300), (4, 256, 256, 300), (4, 256, 64, 900),
+    (4, 256, 128, 2600), (4, 256, 0, 2600), (4, 256, 256, 8400), (3, 128, 128, 1100)])
+def test_append_forms(bf16, hkv, dim, rot, rows):
+    """Each form in both types and at both widths: blocks begun anywhere, kept
+    tokens whose scale grows, skipped rows inside a block, whole blocks."""
+    rng = np.random.default_rng(rows + dim + bf16)
+    counts = [1, rows // 2, 16, 17, 1, 3, rows - rows // 2]
+    starts = [9, 5, 0, 3, 15, 14, 31]
+    slots, pos = step_slots(rng, 16, starts, counts, rows // 16 + 40)
+    for at, gap in ((40, 3), (60, 1), (100, 20)):
+        slots, pos = (np.insert(a, at, [x] * gap) for a, x in ((slots, -1), (pos, 0)))
+    k = half(rng.standard_normal((len(slots), hkv, dim)) *
+             np.exp2(rng.integers(-4, 5, (len(slots), 1, 1))), bf16)
+    pools = [random_pool(rng, (rows // 16 + 41) * 16, hkv, dim) for _ in range(2)]
+    cache = rope_cache(int(pos.max()) + 1, rot) if rot else None
+    run_append(rng, k, k[::-1].copy(), slots, pos, cache, pools, bf16, 3)
+    assert fekv.device_errors() == 0
+
+
 # ---------------------------------------------------------------------------
 # gather
 # ---------------------------------------------------------------------------
@@ -101,6 +127,121 @@ def check(st, causal, got=None):
     assert over.max() <= 1, (over.max(), np.unravel_index(over.argmax(), over.shape))
 
 
+@pytest.mark.parametrize("bf16", [True, False])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("hq,hkv,dim,page", HEADS)
+def test_multi_row(hq, hkv, dim, page, causal, bf16):
+    """Verify blocks, chunks that start a sequence, chunks over a prefix, rows
+    and keys that end inside a tile, decode rows beside them."""
+    rng = np.random.default_rng(hq * hkv + dim + 7)
+    lens = [2, 16, 40, 129, 300, 64, 140, 1, 33, 128, 700]
+    rows = [2, 16, 5, 129, 17, 64, 40, 1, 1, 127, 1]
+    check(Step(rng, hq, hkv, dim, page, lens, rows, bf16), causal)
+
+
+@pytest.mark.parametrize("rows", [1, 20])
+@pytest.mark.parametrize("dim", [128, 256])
+@pytest.mark.parametrize("bf16", [True, False])
+def test_every_part_of_a_query_counts(bf16, dim, rows):
+    """Scores that come from the queries' last bits alone: all else cancels."""
+    rng = np.random.default_rng(rows + dim)
+    st = Step(rng, 8, 4, dim, 16, [300, 40, 77], [rows] * 3, bf16)
+    st.q = half(bounds.cancelling_queries(rng, 3 * rows, 8, dim, bf16), bf16)
+    bounds.even_keys(rng, *st.pools[0], dim, bf16)
+    st.pools[0][0][~st.used] = 0x7F
+    check(st, True)
+    check(st, False)
+
+
+@pytest.mark.parametrize("dim", [128, 256])
+@pytest.mark.parametrize("bf16", [True, False])
+def test_long_sequences_are_cut(dim, bf16):
+    """Few rows, many keys: the row items' keys are cut across CTAs and joined."""
+    rng = np.random.default_rng(dim + 1)
+    st = Step(rng, 8, 2, dim, 16, [6000, 3001], [9, 30], bf16)
+    p = st.plan()
+    assert p.info()["split_sequences"] > 0
+    check(st, True, st.run(True, p))
+    check(st, False)
+
+
+@pytest.mark.parametrize("rows,dim", [(1, 128), (1, 256), (24, 128), (24, 256)])
+@pytest.mark.parametrize("bf16", [True, False])
+def test_block_scales_far_apart(rows, dim, bf16):
+    """V scales that differ by 2^40 between blocks, blocks of zeros, and K
+    scales that differ by 2^6."""
+    rng = np.random.default_rng(rows + dim + 1)
+    st = Step(rng, 8, 2, dim, 16, [700, 300], [rows, rows], bf16)
+    (kc, ke), (vc, ve) = st.pools
+    ve[:] = 127 + rng.integers(-30, 3, ve.shape)
+    ke[:] = 127 + rng.integers(-13, -6, ke.shape)
+    zero = rng.random(ve.shape) < 0.3
+    vc.reshape(-1, 16, *vc.shape[1:])[zero.nonzero()[0], :, zero.nonzero()[1]] = 0
+    ve[zero] = 127 - 32
+    check(st, True)
+    check(st, False)
+
+
+@pytest.mark.parametrize("rows,dim", [(1, 128), (40, 128), (40, 256)])
+@pytest.mark.parametrize("bf16", [True, False])
+def test_queries_of_any_size(rows, dim, bf16):
+    """Zero rows, tiny rows (f16: subnormal), large ones, rows with an outlier;
+    rows that hold NaN or infinity give NaN and touch no other."""
+    rng = np.random.default_rng(rows + dim)
+    st = Step(rng, 8, 2, dim, 16, [200, 77], [rows, rows], bf16)
+    st.q[0, 0] = 0
+    st.q[0, 1] *= 1e-30 if bf16 else 1e-6
+    st.q[0, 2, 5] *= 1000
+    st.q[0, 3] *= 2.0 ** 5
+    st.q[0, 4, 77] = 3e4
+    st.q = half(st.q, bf16)
+    for causal in (True, False):
+        check(st, causal)
+    clean = st.run(True)
+    st.q[-1, 0, 3] = np.nan
+    st.q[-1, 5, 100] = np.inf
+    st.q[0, 7, 0] = -np.inf
+    got = st.run(True)
+    for r, h in ((-1, 0), (-1, 5), (0, 7)):
+        assert np.isnan(got[r, h]).all()
+        got[r, h] = clean[r, h]
+    assert np.array_equal(got, clean)
+
+
+@pytest.mark.parametrize("bf16", [True, False])
+@pytest.mark.parametrize("dim", [128, 256])
+def test_nan_past_a_chunks_limit_stays_out_of_earlier_rows(dim, bf16):
+    """A NaN in a chunk's last key: hidden from every row but the last, whose
+    heads of that KV head it reaches."""
+    rng = np.random.default_rng(dim)
+    st = Step(rng, 8, 4, dim, 16, [190], [40], bf16)
+    clean = st.run(True)
+    st.pools[0][0][int(st.md.pages[189 // 16]) * 16 + 189 % 16, 2, 9] = 0x7F
+    got = st.run(True)
+    assert np.isnan(got[-1, 4:6]).all()
+    got[-1, 4:6] = clean[-1, 4:6]
+    assert np.array_equal(got, clean)
+
+
+@pytest.mark.parametrize("bf16", [True, False])
+def test_a_call_repeats_its_bits(bf16):
+    """Nothing depends on the order in which CTAs or warps run."""
+    rng = np.random.default_rng(21)
+    lens = [600] * 3 + [5000] + [int(x) for x in rng.integers(900, 1600, 30)]
+    st = Step(rng, 16, 4, 128, 16, lens, [300] * 3 + [20] + [1] * 30, bf16)
+    plan = st.plan()
+    pools = [pool_of(*p) for p in st.pools]
+    qd = dev(st.q, DT[bf16])
+    outs = [torch.full_like(qd, 9.0) for _ in range(12)]
+    for o in outs:
+        plan.attention(qd, *pools, o, True)
+    torch.cuda.synchronize()
+    for o in outs[1:]:
+        assert torch.equal(o, outs[0])
+    check(st, True, outs[0].double().cpu().numpy())
+    plan.close()
+
+
 # ---------------------------------------------------------------------------
 # plans: prepared on the device, for replay
 # ---------------------------------------------------------------------------
@@ -116,3 +257,99 @@ def test_device_prepare_at_256_dims(rows, hkv, bf16):
         assert np.array_equal(host, device)  # the same cuts
     check(st, True, device)
     check(st, False, st.run(False, st.plan(device=True)))
+
+
+@pytest.mark.parametrize("dim", [128, 256])
+@pytest.mark.parametrize("causal", [True, False])
+def test_a_device_prepared_long_block(dim, causal):
+    """One block of 32 rows over thousands of keys, its items whole."""
+    st = Step(np.random.default_rng(26), 8, 2, dim, 16, [5003], [32], True)
+    check(st, causal, st.run(causal, st.plan(device=True)))
+
+
+@pytest.mark.parametrize("dim", [128, 256])
+@pytest.mark.parametrize("bf16", [True, False])
+def test_a_host_plan_for_replay(dim, bf16):
+    """prepare(graph=True): one captured call serves steps of the same batch and
+    rows, decode rows, blocks and chunks, few keys and many."""
+    rng = np.random.default_rng(dim)
+    rows = [1, 30, 1, 5, 100]
+    steps = [Step(rng, 8, 2, dim, 16, lens, rows, bf16, blocks=900)
+             for lens in ([40, 33, 1, 7, 150], [3000, 4000, 17, 900, 100], [1, 30, 800, 5, 2100])]
+    plan = fekv.Kv8Plan(8, 2, dim, 16, len(rows), 300, bf16, 900)
+    q = dev(steps[0].q, DT[bf16])
+    out = torch.zeros_like(q)
+    pools = [pool_of(*p) for p in steps[0].pools]
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        for i, st in enumerate(steps):
+            md = st.md
+            plan.prepare(md.qo, md.kv, md.pages, md.last, graph=True)
+            q.copy_(dev(st.q, DT[bf16]))
+            for pool, (codes, exps) in zip(pools, st.pools):
+                pool.codes.view(torch.uint8).copy_(dev(codes))
+                pool.exps.copy_(dev(exps))
+            if i == 0:
+                plan.attention(q, *pools, out, True)
+                side.synchronize()
+                with torch.cuda.graph(graph, stream=side):
+                    plan.attention(q, *pools, out, True)
+            out.fill_(9.0)
+            graph.replay()
+            side.synchronize()
+            check(st, True, out.double().cpu().numpy())
+    assert fekv.device_errors() == 0
+    plan.close()
+
+
+@pytest.mark.parametrize("dim", [128, 256])
+@pytest.mark.parametrize("bf16", [True, False])
+def test_a_step_of_blocks_replays_from_a_graph(dim, bf16):
+    """Device-side prepare, append and attention of 20 packed rows a sequence
+    captured once, a padding entry among them; replayed with other starts,
+    tables and contents."""
+    rng = np.random.default_rng(25)
+    hq, hkv, page, batch, rows = 8, 2, 16, 4, 5
+    blocks = 100
+    tables = torch.zeros(batch, 20, dtype=torch.int32, device="cuda")
+    starts = torch.zeros(batch, dtype=torch.int32, device="cuda")
+    slots = torch.zeros(batch * rows, dtype=torch.int64, device="cuda")
+    pos = torch.zeros_like(slots)
+    q = torch.zeros(batch * rows, hq, dim, dtype=DT[bf16], device="cuda")
+    k = torch.zeros(batch * rows, hkv, dim, dtype=DT[bf16], device="cuda")
+    v = torch.zeros_like(k)
+    qr, out = torch.zeros_like(q), torch.zeros_like(q)
+    rope = dev(rope_cache(320, 128))
+    pools = [pool_of(*random_pool(rng, (blocks + 1) * page, hkv, dim)) for _ in range(2)]
+    plan = fekv.Kv8Plan(hq, hkv, dim, page, batch, 20, bf16, blocks)
+
+    def step():
+        plan.step_prepare_device(tables, starts, rows, slots, pos)
+        fekv.append_kv8(q, k, v, *pools, slots, pos, rope, q_out=qr)
+        plan.attention(qr, *pools, out, True)
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        tables.copy_(dev(rng.permutation(blocks)[:batch * 20].reshape(batch, 20).astype(np.int32)))
+        step()
+        side.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            step()
+        for first in ([5, 300, 31, 0], [10, 305, 36, 5], [100, 7, -1, 250]):
+            starts.copy_(dev(np.asarray(first, np.int32)))
+            for t in (q, k, v):
+                t.copy_(torch.randn(t.shape, device="cuda"))
+            graph.replay()
+            side.synchronize()
+            live = [b for b in range(batch) if first[b] >= 0]
+            at = np.concatenate([np.arange(b * rows, (b + 1) * rows) for b in live])
+            md = build_step_metadata([tables[b].cpu().numpy() for b in live],
+                                     [first[b] for b in live], [rows] * len(live), page)
+            assert np.array_equal(slots.cpu().numpy()[at], md.slots)
+            want, bound = bounds.attention(qr.double().cpu().numpy()[at],
+                                           *[(codes_of(p), exps_of(p)) for p in pools], md, hq,
+                                           hkv, page, True, bf16)
+            assert (np.abs(out.double().cpu().numpy()[at] - want) <= bound).all()
+    assert fekv.device_errors() == 0
+    plan.close()
