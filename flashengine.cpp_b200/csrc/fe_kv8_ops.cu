@@ -483,15 +483,20 @@ __global__ void __launch_bounds__(kThreads, 4)
   const int p0 = __ldg(kv + b), p1 = __ldg(kv + b + 1);
   if (p1 <= p0) return;
   const int tail = __ldg(last + b);
-  const int64_t orow = __ldg(row_offset + b);
-  const int64_t tokens = (int64_t(p1) - p0 - 1) * page + tail;
-  // its pages within the list, its rows within `out`
-  if (tail < 1 || tail > page || tokens > INT32_MAX / 2 || p0 < 0 || p1 > num_pages || orow < 0 ||
-      tokens > out_rows - orow) {
-    if (threadIdx.x == 0 && blockIdx.x == 0) raise_device_error(err, FE_DEVERR_PAGE_RANGE);
-    return;
+  const int off = __ldg(row_offset + b);
+  int len;
+  {
+    const int64_t tokens = (int64_t(p1) - p0 - 1) * page + tail;
+    // its pages within the list, its rows within `out`
+    const bool bad = tail < 1 || tail > page || tokens > INT32_MAX / 2 || p0 < 0 ||
+                     p1 > num_pages || off < 0 || tokens > out_rows - off;
+    if (bad) {
+      if (threadIdx.x == 0 && blockIdx.x == 0) raise_device_error(err, FE_DEVERR_PAGE_RANGE);
+      return;
+    }
+    len = static_cast<int>(tokens);
   }
-  const int len = static_cast<int>(tokens);
+  const int64_t orow = off;
   const int lane = threadIdx.x & 31;
   const int chunks = hkv * dim / 16;
   const int step = gridDim.x * kWarps * kGatherTok;

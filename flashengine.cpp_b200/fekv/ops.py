@@ -388,15 +388,22 @@ def _kv8_rows(name, t, dtype, shape, device):
                      f"on {t.device}")
 
 
-def _kv8_here(device, pools=(), lists=()):
-    """Pools and int32 lists of a call on CUDA device `device`."""
+def _kv8_pools(device, *pools):
+    """Pools of a call on CUDA device `device`."""
     for p in pools:
         if p.index != device:
             raise ValueError(f"a pool is on {p.device}, the current device is cuda:{device}")
+
+
+def _kv8_lists(device, *lists):
+    """Contiguous int32 tensors on CUDA device `device`."""
+    torch = _torch()
+    tensor, i32 = torch.Tensor, torch.int32
     for t in lists:
-        _require_device_i32(t)
-        if t.get_device() != device:
-            raise ValueError(f"a list is on {t.device}, the current device is cuda:{device}")
+        if not (isinstance(t, tensor) and t.dtype is i32 and t.get_device() == device and
+                t.is_contiguous()):
+            raise ValueError("expected a contiguous int32 tensor on the current device "
+                             f"(cuda:{device})")
 
 
 def append_kv8(q, k, v, kpool, vpool, slots, pos=None, cache=None, q_out=None, stream=None):
@@ -419,8 +426,9 @@ def append_kv8(q, k, v, kpool, vpool, slots, pos=None, cache=None, q_out=None, s
         raise ValueError(f"k: expected float16 or bfloat16, got {dt}")
     device = _kv8_device()
     if kpool.index != device or vpool.index != device:
-        _kv8_here(device, (kpool, vpool))
-    kp = _kv8_rows("k", k, dt, shape, device)
+        _kv8_pools(device, kpool, vpool)
+    if k.get_device() != device or not k.is_contiguous():
+        raise ValueError(f"k: expected a contiguous tensor on the current device (cuda:{device})")
     vp = _kv8_rows("v", v, dt, shape, device)
     hq = rot = most = 0
     qp = op = pp = cp = None
@@ -437,7 +445,7 @@ def append_kv8(q, k, v, kpool, vpool, slots, pos=None, cache=None, q_out=None, s
         if rot:
             pp = _kv8_rows("pos", pos, torch.int64, (rows,), device)
             cp = _kv8_rows("cache", cache, torch.float32, cs, device)
-    rc = _lib.load().fe_kv8_append(qp, op, kp, vp, kpool.codes_ptr, vpool.codes_ptr,
+    rc = _lib.load().fe_kv8_append(qp, op, k.data_ptr(), vp, kpool.codes_ptr, vpool.codes_ptr,
                                    kpool.exps_ptr, vpool.exps_ptr, sp, pp, cp, rows, hq, hkv, dim,
                                    rot, most, code, pool[0], _kv8_stream(stream, device))
     if rc:
@@ -450,18 +458,20 @@ def gather_kv8(pool, out, kv, pages, last, row_offset, max_len, page, stream=Non
     whose rows reach past `out`, or whose pages past `pages`, is skipped and
     flagged (device_errors)."""
     device = _kv8_device()
-    _kv8_here(device, (pool,), (kv, pages, last, row_offset))
-    if not last.shape == row_offset.shape == (kv.shape[0] - 1,):
+    _kv8_pools(device, pool)
+    _kv8_lists(device, kv, pages, last, row_offset)
+    batch = last.numel()
+    if not last.shape == row_offset.shape == (batch,) or kv.shape != (batch + 1,):
         raise ValueError("last and row_offset must have one entry per sequence, kv one more")
-    _, hkv, dim = pool.shape
-    if not out.is_contiguous() or out.get_device() != device or out.numel() % (hkv * dim):
+    slots, hkv, dim = pool.shape
+    rows, odd = divmod(out.numel(), hkv * dim)
+    if odd or out.get_device() != device or not out.is_contiguous():
         raise ValueError("out: expected a contiguous tensor [rows, hkv, dim] on the current device "
                          f"(cuda:{device})")
     check(_lib.load().fe_kv8_gather_within(pool.codes_ptr, pool.exps_ptr, out.data_ptr(),
-                                           out.numel() // (hkv * dim), kv.data_ptr(),
-                                           pages.data_ptr(), pages.shape[0], last.data_ptr(),
-                                           row_offset.data_ptr(), kv.shape[0] - 1, max_len, page,
-                                           hkv, dim, dtype_code(out), pool.shape[0],
+                                           rows, kv.data_ptr(), pages.data_ptr(), pages.numel(),
+                                           last.data_ptr(), row_offset.data_ptr(), batch, max_len,
+                                           page, hkv, dim, dtype_code(out), slots,
                                            _kv8_stream(stream, device)), "gather_kv8")
 
 
@@ -472,7 +482,7 @@ def copy_blocks_kv8(k_pools, v_pools, src, dst, ntok, page, stream=None):
     if n != len(v_pools):
         raise ValueError("k_pools and v_pools differ in length")
     device = _kv8_device()
-    _kv8_here(device, lists=(src, dst, ntok))
+    _kv8_lists(device, src, dst, ntok)
     if not src.shape == dst.shape == ntok.shape:
         raise ValueError("src, dst and ntok differ in length")
     if n == 0:
@@ -482,7 +492,7 @@ def copy_blocks_kv8(k_pools, v_pools, src, dst, ntok, page, stream=None):
             for side in (k_pools, v_pools)] + \
         [[p.exps_ptr for p in side] for side in (k_pools, v_pools)]
     if len(ptrs[0]) != n or len(ptrs[1]) != n:
-        _kv8_here(device, (*k_pools, *v_pools))
+        _kv8_pools(device, *k_pools, *v_pools)
         raise ValueError("the layers' pools differ in shape")
     arrays = [array.array("Q", p) for p in ptrs]
     check(_lib.load().fe_kv8_copy_blocks(*[a.buffer_info()[0] for a in arrays], n, src.data_ptr(),
@@ -531,7 +541,7 @@ class Kv8Plan(AttentionPlan):
         self.rows = int(qo[batch])
 
     def prepare_device(self, qo, kv, pages, last, batch, rows, stream=None):
-        _kv8_here(self._device(), lists=(qo, kv, pages, last))
+        _kv8_lists(self._device(), qo, kv, pages, last)
         _kv8_metadata(qo, kv, last, int(batch))
         super().prepare_device(qo, kv, pages, last, batch, rows, stream)
         self.rows = int(rows)
@@ -539,7 +549,7 @@ class Kv8Plan(AttentionPlan):
     def step_prepare_device(self, block_tables, starts, rows_per_seq, slots, positions,
                             stream=None):
         device = self._device()
-        _kv8_here(device, lists=(block_tables, starts))
+        _kv8_lists(device, block_tables, starts)
         for t in (slots, positions):
             if t.get_device() != device or not t.is_contiguous():
                 raise ValueError("slots / positions: contiguous int64 tensors on the current "
@@ -556,7 +566,7 @@ class Kv8Plan(AttentionPlan):
             raise ValueError(f"q has {shape[0]} rows, the plan was prepared for {self.rows}")
         device = self._device()
         if kpool.index != device or vpool.index != device:
-            _kv8_here(device, (kpool, vpool))
+            _kv8_pools(device, kpool, vpool)
         check(self.lib.fe_kv8_attn_run(self.handle, _kv8_rows("q", q, self.dtype, shape, device),
                                        kpool.codes_ptr, vpool.codes_ptr, kpool.exps_ptr,
                                        vpool.exps_ptr,
