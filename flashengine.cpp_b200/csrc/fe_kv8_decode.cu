@@ -672,11 +672,10 @@ constexpr int kMergeWarps = 8;
 // Whole calls in us on a B200 with always one, this rule, always eight:
 // a sequence of 8192 keys 22.0, 10.2, 10.2; 64 of 512 to 4096 keys 45.6,
 // 45.6, 60.1; a 1024-row chunk over 8192 keys 159.6, 159.8, 262.5.
-__host__ __device__ __forceinline__ int merge_warps_per_row(int pieces) {
-  int n = 1;
-  while (n < kMergeWarps && pieces > 8 * n) n *= 2;
-  return n;
+__host__ __device__ __forceinline__ int merge_log2_warps(int pieces) {
+  return (pieces > 8) + (pieces > 16) + (pieces > 32);
 }
+static_assert(kMergeWarps == 8, "merge_log2_warps");
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kMergeWarps * 32)
@@ -696,19 +695,23 @@ __global__ void __launch_bounds__(kMergeWarps * 32)
     g = groups[blockIdx.x];
     if (g.nsplit >= 2) si = seqs[g.seq];
   }
-  pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int lg = merge_log2_warps(g.nsplit), per_row = 1 << lg;
+  int sub = warp & (per_row - 1), rows = kMergeWarps >> lg;
+  pdl_wait();
   for (int u = blockIdx.x; u < n; u += gridDim.x) {
     if (u != static_cast<int>(blockIdx.x)) {
       g = groups[u];
       if (g.nsplit >= 2) si = seqs[g.seq];
+      lg = merge_log2_warps(g.nsplit);
+      per_row = 1 << lg;
+      sub = warp & (per_row - 1);
+      rows = kMergeWarps >> lg;
     }
     if (g.nsplit < 2) continue;  // placeholder ids of the row lists
-    const int per_row = merge_warps_per_row(g.nsplit);
-    const int sub = warp & (per_row - 1), rows = kMergeWarps / per_row;
     const int rph = g.rows_per_head > 0 ? g.rows_per_head : si.qrows * a.G;
     for (int r0 = blockIdx.y * rows; r0 < g.rows; r0 += gridDim.y * rows) {
-      const int r = r0 + (warp - sub) / per_row;
+      const int r = r0 + (warp >> lg);
       float M = -INFINITY, L = 0.f;
       float4 acc[kV];
 #pragma unroll
@@ -726,7 +729,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32)
           }
           // the first O vectors are in flight with them
           constexpr int kPre = 8 / kV;
-          const int count = min(32, (g.nsplit - s0 + per_row - 1) / per_row);
+          const int count = min(32, (g.nsplit - s0 + per_row - 1) >> lg);
           float4 pre[kPre][kV];
 #pragma unroll
           for (int j = 0; j < kPre; ++j)
@@ -827,7 +830,7 @@ template <typename T>
 int merge_launch(int dim, int list, const AttnArgs<T>& a, int units, int rows, int pieces,
                  int max_blocks, cudaStream_t stream, bool pdl) {
   // blocks for the rows of the most split unit
-  const int per_block = kMergeWarps / merge_warps_per_row(pieces);
+  const int per_block = kMergeWarps >> merge_log2_warps(pieces);
   const dim3 grid(units, std::min((rows + per_block - 1) / per_block,
                                   std::max(1, max_blocks / units)));
   auto kernel = dim == kWideHeadDim ? kv8_merge_kernel<T, kWideHeadDim>
