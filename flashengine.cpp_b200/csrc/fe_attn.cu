@@ -616,9 +616,9 @@ int launch_lists(fe_attn_plan* p, int view, int grid_rows, int grid_dec, const v
                                  on, pdl);
     // Pieces of a unit: under a fixed geometry what an even cut gives. Its grid
     // is mostly empty blocks, so it is bounded and strides over the rows:
-    // replayed decode steps of 4 short sequences take 33 us with a block for
-    // every possible row, 17, 16, 17, 21 with 16, 8, 4, 2 blocks an SM; of 64
-    // sequences 55, then 56, 52, 51, 52; of one of 8192 keys 19, 21, 29, 46.
+    // replayed decode steps of 4 short sequences take 32 us with a block for
+    // every possible row, 15, 13, 12, 11 with 16, 8, 4, 2 blocks an SM; of 64
+    // sequences 56, then 55, 52, 52, 53; of one of 8192 keys 31, 18, 21, 28, 45.
     const int even = list == 2 ? p->cfg.dec_grid_cap * p->cfg.dec_heads /
                                      (p->cfg.hkv * std::max(1, h.batch)) + 1
                                : 1;

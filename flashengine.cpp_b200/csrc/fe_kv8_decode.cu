@@ -18,6 +18,14 @@
 // clocks a warp and SM quarter when its operands change (the 16-bit one 10), a
 // step of this kernel 3200 clocks, and it was bound by them and not by HBM.
 //
+// Roundings. A weight's 11 bits are fewer than the about 16 that the kernels
+// over the 16-bit cache keep (a half and its residual): its share of the
+// output moves by at most 2^-11, where a code of V holds its value to 2^-4 and
+// an output in f16 is rounded to 2^-11 itself, and a second half would cost
+// every PV product again. m refers to weight times V scale, so the 11 bits are
+// there for weights down to 2^-29 of the row's largest such product, fewer
+// below, none under 2^-40; l sums the unrounded weights in fp32.
+//
 // B200 design, as fe_decode.cu: bound by HBM traffic. One persistent CTA per
 // SM with 8 consumer warps and a producer warp; an item is (sequence, group
 // of H KV heads, range of 16-token tiles), a step is two tiles (32 tokens, the
@@ -29,9 +37,12 @@
 // us).
 // Measured on a B200 with 8 KV heads of 128 dims, merge included: 64 bf16
 // sequences of 2 to 32 Ki keys, 64 query heads, 220 us = 6.4 TB/s (0.98 of a
-// device-to-device copy's rate); of 512 to 4096 keys, 32 heads, 45.7 us = 4.8
+// device-to-device copy's rate); of 512 to 4096 keys, 32 heads, 45.2 us = 4.9
 // TB/s (the rest: launch, first loads, the merge and the cut's ends); 4
-// sequences of up to 1000 keys, 9.6 us (a chain of dependent latencies).
+// sequences of up to 1000 keys, 9.5 us (a chain of dependent latencies). Two KV
+// heads of 256 dims, 16 heads, 512 to 4096 keys: 33 us = 3.4 TB/s.
+// Nine warps leave 168 registers a thread, of which ptxas spills 108 to 116
+// bytes at 128 dims, 72 at 256.
 #include <algorithm>
 #include <mutex>
 #include <type_traits>
@@ -670,8 +681,8 @@ constexpr int kMergeWarps = 8;
 
 // One warp a row up to eight pieces, then as many as leave each about eight.
 // Whole calls in us on a B200 with always one, this rule, always eight:
-// a sequence of 8192 keys 22.0, 10.2, 10.2; 64 of 512 to 4096 keys 45.6,
-// 45.6, 60.1; a 1024-row chunk over 8192 keys 159.6, 159.8, 262.5.
+// a sequence of 8192 keys 21.8, 9.9, 11.0; 64 of 512 to 4096 keys 45.7,
+// 45.4, 52.6; a 1024-row chunk over 8192 keys 156.6, 156.3, 203.5.
 __host__ __device__ __forceinline__ int merge_log2_warps(int pieces) {
   return (pieces > 8) + (pieces > 16) + (pieces > 32);
 }

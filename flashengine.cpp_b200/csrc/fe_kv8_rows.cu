@@ -8,13 +8,18 @@
 // running maximum of s + v, O = sum w code_v, l = sum w 2^-v, out = O / l.
 //  * S = Q K^T runs on tcgen05 kind::f8f6f4 with the K codes as they lie in
 //    the cache and each query row scaled by a power of two and split into e4m3
-//    parts, each the rounding of what the ones before leave: two for bf16 (8 to
-//    9 bits: a bf16 exactly where it is within 2^11 of the row's largest) and
-//    three for f16 (its 11 bits). An fp8 product takes the tensor core half the
-//    time of a 16-bit one, and K needs no conversion.
-//  * O = W V runs on kind::f16 with the weights in f16 (11 bits, kept between
-//    2^-9 and 2^15 around the running maximum) and V's codes converted to f16,
-//    exactly, by a warpgroup. Splitting the weights into e4m3 parts instead
+//    parts, each the rounding of what the ones before leave: two for bf16,
+//    three for f16. They hold an element exactly down to 2^-9 (bf16) or 2^-6
+//    (f16) of the row's largest, and smaller ones to 2^-17.8 of the largest:
+//    the last part's subnormals end there. An fp8 product takes the tensor core
+//    half the time of a 16-bit one, and K needs no conversion.
+//  * O = W V runs on kind::f16 with the weights in f16 and V's codes converted
+//    to f16, exactly, by a warpgroup. A weight is kept times 2^7 relative to a
+//    running maximum (of s + v) that moves once it is exceeded by 2^8, so the
+//    row's largest is stored between 2^7 and 2^15: 11 bits for weights down to
+//    2^-21 of it at least, fewer below, none under 2^-32. (The kernels over the
+//    16-bit cache keep a half and its residual, about 16 bits; a code of V holds
+//    its value to 2^-4.) Splitting the weights into e4m3 parts instead
 //    would feed V raw, but costs five conversions a pair of weights in the
 //    softmax warps, which are what bounds this kernel, against the one that f16
 //    takes.

@@ -24,13 +24,14 @@
 //    to end and cut into equal contiguous pieces, one per CTA. Every cut is a
 //    function of prefix sums, so the device list is the host's item for item
 //    (the same split points, hence bit-identical outputs);
-//  - the row lists (prefill / verify units, never split: head_dim 256 plans
-//    too, where the host planner may split them) sort the units by
+//  - the row lists (prefill / verify units, never split: head_dim 256 and 8-bit
+//    plans too, where the host planner may split them) sort the units by
 //    cost, longest first (a bitonic sort in shared memory, up to
 //    kMaxRowUnits units), and deal them to the CTAs in a snake order (0, 1,
 //    ..., n-1, n-1, ..., 0, ...), which needs only each unit's rank instead
 //    of the host's sequential least-loaded choice. Each item is computed whole
-//    by one CTA either way, so outputs do not depend on the assignment.
+//    by one CTA (on the host's lists too, where they are not split), so outputs
+//    do not depend on the assignment.
 // The plan is graph-mode: both attention kernels run at full width and CTAs
 // without work exit. Invalid metadata or exceeded capacity empties the plan
 // (every list has zero items) and raises FE_DEVERR_PLAN.

@@ -294,6 +294,9 @@ int fe_paged_decode_noalloc(const void* q, const void* k_pool, const void* v_poo
  * slot n leaves slots n + 1 .. of its block undefined (they hold rejected
  * drafts at most; the next append overwrites them). Codes are rounded to
  * nearest even; infinities saturate, NaN stays NaN.
+ * A block's scale falls only when its first slot is written again: a rejected
+ * draft that was far larger than the accepted tokens of its block leaves them
+ * at the scale that it needed, with the bits that were left to them there.
  * A call has at most one run in a block (every step's slot mapping does: a
  * sequence's rows are adjacent and in order): two would race for its scale,
  * and that block's contents are then unspecified.
@@ -343,14 +346,22 @@ int fe_kv8_copy_blocks(void* const* k_codes, void* const* v_codes, void* const* 
  * fe_step_prepare_device), serves fe_kv8_attn_run only, and is destroyed by
  * fe_attn_plan_destroy; dtype is that of q and out. The host's prepare cuts
  * the lists of both kernels across CTAs by keys and by their measured costs.
+ * The device's prepares cut the decode list alike (the same bits), and deal the
+ * items of more packed rows whole: few long blocks take longer by them (one of
+ * 32 rows over 8192 keys with 4 KV heads 88 us, 19 by the host's lists, 28 by
+ * those with graph = 1).
  * fe_kv8_attn_run is fe_attn_run over the values of the codes: the same masks
  * (every query row sees at least one key: a prepared sequence has no fewer
  * keys than query rows), scale 1/sqrt(dim), fp32 softmax and accumulation,
- * output rounded to nearest even. Queries enter the product as they are
- * (sequences of up to 16 packed rows, rows x hq / hkv: f16, and bf16 down to
- * 2^-29 of the row's largest) or in two (bf16) or three (f16) e4m3 parts
- * (more packed rows: 8 to 9 bits, bf16's own, and 11, f16's), softmax weights
- * as f16 over a range of 2^26 and more below the row's largest.
+ * output rounded to nearest even. Queries of sequences of up to 16 packed rows
+ * (rows x hq / hkv) enter the product as they are (f16, and bf16 down to 2^-29
+ * of the row's largest element); with more packed rows in two (bf16) or three
+ * (f16) e4m3 parts, which hold an element exactly down to 2^-9 (bf16) or 2^-6
+ * (f16) of the row's largest, and smaller ones to 2^-17.8 of the largest.
+ * Softmax weights enter the second product as f16, fewer bits than the about 16
+ * of fe_attn_run: 11 down to 2^-29 (up to 16 packed rows) or 2^-21 (more) of
+ * the row's largest weight times V scale, fewer below, none under 2^-40 or
+ * 2^-32; their sum is over the unrounded weights.
  * A query row that holds an infinity or NaN gives NaN. NaN in a key reaches
  * the rows that see it. NaN in a value reaches its dim of the rows that see it
  * and may reach that dim of the sequence's rows it is masked from (weight 0
