@@ -36,12 +36,12 @@
 // first do not wait for them (64 sequences of 512 to 4096 keys: 47.0 -> 45.7
 // us).
 // Measured on a B200 with 8 KV heads of 128 dims, merge included: 64 bf16
-// sequences of 2 to 32 Ki keys, 64 query heads, 220 us = 6.4 TB/s (0.98 of a
-// device-to-device copy's rate); of 512 to 4096 keys, 32 heads, 45.2 us = 4.9
+// sequences of 2 to 32 Ki keys, 64 query heads, 219 us = 6.4 TB/s (0.98 of a
+// device-to-device copy's rate); of 512 to 4096 keys, 32 heads, 44.7 us = 4.9
 // TB/s (the rest: launch, first loads, the merge and the cut's ends); 4
 // sequences of up to 1000 keys, 9.5 us (a chain of dependent latencies). Two KV
 // heads of 256 dims, 16 heads, 512 to 4096 keys: 33 us = 3.4 TB/s.
-// Nine warps leave 168 registers a thread, of which ptxas spills 108 to 116
+// Nine warps leave 168 registers a thread, of which ptxas spills 96 to 112
 // bytes at 128 dims, 72 at 256.
 #include <algorithm>
 #include <mutex>
@@ -60,6 +60,7 @@ constexpr int kStepTiles = 2;
 constexpr int kStepTokens = kStepTiles * kTileTokens;
 constexpr int kBoxBytes = kTileTokens * 128;  // 16 rows x 128 codes
 constexpr float kWeightBits = 15.f;           // weights are kept times 2^15 (a half holds 2^16)
+constexpr float kFar = 1 << 20;               // maxima of a unit of 2^-3 and more
 
 // Warps of a CTA: group = (head, half of the packed rows), kWh = 8 / groups
 // warps of a group take steps j, j + kWh, ...; the stage count is a multiple
@@ -228,11 +229,25 @@ struct State {
         al[nt][c] = fast_exp2(m[nt][c] - base);
         m[nt][c] = mn;
         float add = 0.f;
+        // s + v rounded as in the maximum, and the difference taken then: at the
+        // largest score it is 0 whatever the scores' size (one fma with v - base
+        // would leave that sum's rounding, beyond a half's range from |s| = 2^23
+        // on). At 256 dims only where it is needed: there the two additions take
+        // 64 sequences of 512 to 4096 keys from 32.6 to 33.6 us, at 128 from 45.2
+        // to 44.7.
+        const bool apart = D == 128 || __any_sync(0xffffffffu, fabsf(base) > kFar);
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           const float ft = kf[u] * f[nt][c], off = vf[u] + kWeightBits - base;
-          const float w0 = fast_exp2(fmaf(s[u][nt][c], ft, off));
-          const float w1 = fast_exp2(fmaf(s[u][nt][2 + c], ft, off));
+          float x0, x1;
+          if (apart) {
+            x0 = fmaf(s[u][nt][c], ft, vf[u]) - base + kWeightBits;
+            x1 = fmaf(s[u][nt][2 + c], ft, vf[u]) - base + kWeightBits;
+          } else {
+            x0 = fmaf(s[u][nt][c], ft, off);
+            x1 = fmaf(s[u][nt][2 + c], ft, off);
+          }
+          const float w0 = fast_exp2(x0), w1 = fast_exp2(x1);
           s[u][nt][c] = w0;
           s[u][nt][2 + c] = w1;
           add = fmaf(w0 + w1, vi[u], add);

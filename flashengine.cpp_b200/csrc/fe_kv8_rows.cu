@@ -84,6 +84,7 @@ constexpr int kExpRing = 8;    // tiles of scale factors; K runs at most 6 ahead
 constexpr uint32_t kTmemCols = 512;
 constexpr float kRescale = 8.f;  // O is rescaled when the maximum grew by 2^8
 constexpr float kBias = 7.f;     // weights are kept times 2^7: at most 2^15
+constexpr float kFar = 1 << 20;  // maxima beyond (unit 2^-3 and more) are subtracted apart
 
 template <typename T, int D>
 struct Cfg {
@@ -721,34 +722,61 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc::st_32x32b_x16(lane_addr + C::kOCol + c2 * 16, ov);
           }
         }
-        const float m_sub = (m_now == -INFINITY ? 0.f : m_now) - kBias;
+        const float m_ref = m_now == -INFINITY ? 0.f : m_now, m_sub = m_ref - kBias;
+        // Scores so large that one fma with the maximum would leave a rounding
+        // beyond a half's range (from |s| = 2^23 on): s + v rounded as in the
+        // maximum, and the difference taken then. In a loop of its own, as small
+        // as it gets: shared with the one below it cost 2 % of a call.
+        if (__builtin_expect(__any_sync(0xffffffffu, fabsf(m_ref) > kFar), 0)) {
 #pragma unroll 1
-        for (int h = 0; h < kN; h += 32) {
-          float s[32];
-          tc::ld_32x32b_x32(s_addr + h, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
-          tc::wait_ld();
-          uint32_t pk[16];
+          for (int h = 0; h < kN; h += 16) {
+            uint32_t s[16], pk[8];
+            tc::ld_32x32b_x16(s_addr + h, s);
+            tc::wait_ld();
+            const float4 f = fac[h / 16];
+            const float fs = f.x * rf;
+            float sum = 0.f;
 #pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            const float4 f = fac[h / 16 + b];
-            const float fs = f.x * rf, off = f.y - m_sub;
-            const float2 sc2 = make_float2(fs, fs), off2 = make_float2(off, off);
-            float2 sum0 = make_float2(0.f, 0.f), sum1 = sum0;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const float2 x =
-                  fma2(make_float2(s[16 * b + 2 * e], s[16 * b + 2 * e + 1]), sc2, off2);
-              const float2 pp = make_float2(fast_exp2(x.x), fast_exp2(x.y));
-              if (e & 1)
-                sum1 = add2(sum1, pp);
-              else
-                sum0 = add2(sum0, pp);
-              pk[8 * b + e] = pack2<__half>(pp.x, pp.y);
+            for (int e = 0; e < 16; ++e) {
+              const float w = fast_exp2(fmaf(__uint_as_float(s[e]), fs, f.y) - m_ref + kBias);
+              sum += w;
+              s[e] = __float_as_uint(w);
             }
-            l = fmaf((sum0.x + sum0.y) + (sum1.x + sum1.y), f.z, l);
+            l = fmaf(sum, f.z, l);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              pk[e] = pack2<__half>(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1]));
+            tc::st_32x32b_x8(s_addr + h / 2, pk);
           }
-          // (weights of 32 keys take 16 columns: never ones still to be read)
-          tc::st_32x32b_x16(s_addr + h / 2, pk);
+        } else {
+#pragma unroll 1
+          for (int h = 0; h < kN; h += 32) {
+            float s[32];
+            tc::ld_32x32b_x32(s_addr + h, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
+            tc::wait_ld();
+            uint32_t pk[16];
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+              const float4 f = fac[h / 16 + b];
+              const float fs = f.x * rf, off = f.y - m_sub;
+              const float2 sc2 = make_float2(fs, fs), off2 = make_float2(off, off);
+              float2 sum0 = make_float2(0.f, 0.f), sum1 = sum0;
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                const float2 x =
+                    fma2(make_float2(s[16 * b + 2 * e], s[16 * b + 2 * e + 1]), sc2, off2);
+                const float2 pp = make_float2(fast_exp2(x.x), fast_exp2(x.y));
+                if (e & 1)
+                  sum1 = add2(sum1, pp);
+                else
+                  sum0 = add2(sum0, pp);
+                pk[8 * b + e] = pack2<__half>(pp.x, pp.y);
+              }
+              l = fmaf((sum0.x + sum0.y) + (sum1.x + sum1.y), f.z, l);
+            }
+            // (weights of 32 keys take 16 columns: never ones still to be read)
+            tc::st_32x32b_x16(s_addr + h / 2, pk);
+          }
         }
         tc::wait_st();
         tc::fence_before_sync();

@@ -208,6 +208,53 @@ def test_queries_of_any_size(rows, dim, bf16):
     assert np.array_equal(got, clean)
 
 
+def half_ulp(x, bf16):
+    mant, low = (7, -126) if bf16 else (10, -14)
+    return np.exp2(np.floor(np.log2(np.maximum(x, 2.0 ** low))) - mant - 1)
+
+
+@pytest.mark.parametrize("rows,dim", [(1, 128), (1, 256), (3, 256), (40, 128), (40, 256)])
+@pytest.mark.parametrize("bf16", [True, False])
+@pytest.mark.parametrize("size", [1e4, 1e6, 3e6, 1e7, 1e9, 1e13])
+def test_scores_of_any_size(size, bf16, rows, dim):
+    """Scores far apart in fp32: one key above all others by an eighth of its
+    score is the whole output, keys of one score share it evenly, however large
+    the scores, of either sign."""
+    rng = np.random.default_rng(rows + dim)
+    for sign in (1.0, -1.0):
+        st = Step(rng, 8, 2, dim, 16, [700, 41, 130], [rows] * 3, bf16)
+        (kc, ke), (vc, ve) = st.pools
+        st.q[:] = sign
+        e = int(np.floor(np.log2(size / dim ** 0.5 / 14)))
+        ke[:] = 127 + e
+        kc[st.used] = ref.encode_e4m3(rng.integers(8, 13, (int(st.used.sum()), 2)) * 1.0)[..., None]
+        first = [int(st.md.pages[p]) * 16 for p in st.md.kv[:-1]]
+        kc[first] = ref.encode_e4m3(np.array(14.0 if sign > 0 else 6.0))
+        got = st.run(True)
+        for b, at in enumerate(first):
+            want = np.repeat(ref.values(vc, ve)[at], 4, 0)  # [hq, dim]
+            # the weight's rounding to a half, the quotient's, the result's
+            near = np.abs(want) * (2.0 ** -11 + 2.0 ** -22)
+            near = near + half_ulp(np.abs(want) + near, bf16)
+            assert (np.abs(got[b * rows:(b + 1) * rows] - want) <= near).all()
+        # one score for all keys, one scale for all values
+        kc[st.used] = ref.encode_e4m3(np.array(11.0))
+        ve[:] = 127 - 7
+        got = st.run(True)
+        want, mass = np.zeros(got.shape), np.zeros(got.shape)
+        val = ref.values(vc, ve)
+        for b, n in enumerate((700, 41, 130)):
+            t = np.arange(n)
+            slots = st.md.pages[st.md.kv[b]:st.md.kv[b + 1]][t // 16] * 16 + t % 16
+            for i in range(rows):
+                v = val[slots[:n - rows + i + 1]]
+                want[b * rows + i] = np.repeat(v.mean(0), 4, 0)
+                mass[b * rows + i] = np.repeat(np.abs(v).mean(0), 4, 0)
+        # sums in fp32 over 700 keys and the quotient, weights as halves, the result
+        bound = (701 * 2.0 ** -23 + 2.0 ** -11) * mass
+        assert (np.abs(got - want) <= bound + half_ulp(np.abs(want) + bound, bf16)).all()
+
+
 @pytest.mark.parametrize("bf16", [True, False])
 @pytest.mark.parametrize("dim", [128, 256])
 def test_nan_past_a_chunks_limit_stays_out_of_earlier_rows(dim, bf16):
