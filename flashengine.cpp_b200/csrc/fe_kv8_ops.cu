@@ -115,7 +115,7 @@ struct AppendArgs {
 // of 64 sequences 3.5 us, 4 rows 3.2 us. Query and KV blocks in turn instead of
 // one after the other, and KV rows held in fp32 registers, measured 305 and 342
 // us against 301 and 290. 64 Ki rows of 16 query and 2 KV heads of 256 dims:
-// 492 us = 2.7 TB/s, 0.42 of the copy's rate (a warp's stage of 16 KiB leaves
+// 484 us = 2.8 TB/s, 0.42 of the copy's rate (a warp's stage of 16 KiB leaves
 // one block an SM, and the query part is launched with it).
 // ---------------------------------------------------------------------------
 
@@ -465,7 +465,7 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? 3 : 1) kv8_append_kernel(
 // ---------------------------------------------------------------------------
 // Gather: blockIdx.y = sequence; a warp takes kTok tokens, every lane's
 // 16-code chunks of them in flight together. Bound by memory traffic: 64
-// sequences of 512 to 4096 tokens, 8 heads of 128 dims to bf16, 68.6 us = 5.6
+// sequences of 512 to 4096 tokens, 8 heads of 128 dims to bf16, 68.4 us = 5.6
 // TB/s (0.86 of a device-to-device copy's rate, whose reads and writes are
 // equal parts; here two thirds are writes). Four blocks an SM against three,
 // by registers: 72 against 85 us.
