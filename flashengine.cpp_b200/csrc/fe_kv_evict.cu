@@ -1,0 +1,380 @@
+// Eviction from the paged cache by accumulated attention weight: selection of
+// the tokens to keep, per sequence and KV head, and their compaction to the
+// front of the sequence. No counterpart in the reference, whose cache drops
+// whole sequences only (Cambridgebit/FlashEngine.cpp src/scheduler.cpp:6-29).
+//
+// Both kernels take device metadata (a captured graph replays them for later
+// steps) and check what they read of it: a sequence or token that reaches past
+// its lists or the pool is skipped and flagged.
+#include <algorithm>
+#include <mutex>
+#include <string>
+
+#include "fe_common.cuh"
+
+namespace fe {
+namespace {
+
+constexpr int kSelThreads = 512;
+constexpr int kSelWarps = kSelThreads / 32;
+constexpr int kBins = 2048;
+constexpr int kSelKeys = 48 << 10;  // keys that fit in shared memory beside the histogram
+
+// A score as an unsigned number of the same order; NaN below everything.
+__device__ __forceinline__ uint32_t ordered(float x) {
+  if (x != x) return 0;
+  const uint32_t b = __float_as_uint(x == 0.f ? 0.f : x);  // -0 and +0 tie
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+
+struct SeqTable {
+  const int32_t* kv;
+  const int32_t* pages;
+  const int32_t* last;
+  int num_pages, page;
+  int64_t cache_slots;
+};
+
+// Pages [p0, p1) and length of sequence b; false when they reach past the
+// list or are no sequence.
+__device__ __forceinline__ bool sequence(const SeqTable& t, int b, int& p0, int& n) {
+  p0 = __ldg(t.kv + b);
+  const int p1 = __ldg(t.kv + b + 1), ln = __ldg(t.last + b);
+  n = 0;
+  if (p0 < 0 || p1 <= p0 || p1 > t.num_pages || ln < 1 || ln > t.page) return false;
+  const int64_t len = static_cast<int64_t>(p1 - p0 - 1) * t.page + ln;
+  if (len > INT32_MAX) return false;
+  n = static_cast<int>(len);
+  return true;
+}
+
+// Slot of token t of the sequence at p0, -1 for a page outside the pool.
+__device__ __forceinline__ int64_t slot_of(const SeqTable& s, int p0, int t) {
+  const int pg = __ldg(s.pages + p0 + t / s.page);
+  const int64_t first = static_cast<int64_t>(pg) * s.page;
+  return pg < 0 || first + s.page > s.cache_slots ? -1 : first + t % s.page;
+}
+
+// Exclusive sum over the block of one value a thread; `total` for everyone.
+__device__ __forceinline__ int block_scan(int v, int* warp_sums, int& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();  // the last call's sums have been read
+  if (lane == 31) warp_sums[warp] = x;
+  __syncthreads();
+  int before = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < kSelWarps; ++w) {
+    const int s = warp_sums[w];
+    before += w < warp ? s : 0;
+    total += s;
+  }
+  return before + x - v;
+}
+
+// One CTA per (sequence, KV head). The `want` best of the tokens between sink
+// and the recent ones are found by a radix select over their ordered scores
+// (11, 11 and 10 bits: histogram, then the bin in which the want-th lies),
+// which gives the threshold and how many of the tokens equal to it are kept,
+// the lowest indexes first; then the kept tokens are written in order.
+// The keys of a sequence of up to `room` tokens stay in shared memory between
+// the passes; a longer one's scores are read again by each.
+__global__ void __launch_bounds__(kSelThreads)
+    select_kernel(const float* __restrict__ scores, const SeqTable table,
+                  int32_t* __restrict__ kept, int hkv, int budget, int sink, int recent, int room,
+                  unsigned int* err) {
+  extern __shared__ uint32_t keys[];
+  __shared__ int hist[kBins];
+  __shared__ int warp_sums[kSelWarps];
+  __shared__ int found[2];
+  pdl_trigger();
+  pdl_wait();  // the scores come from, and the lists may come from, earlier kernels
+  const int b = blockIdx.x / hkv, h = blockIdx.x % hkv;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int32_t* out = kept + static_cast<int64_t>(blockIdx.x) * budget;
+  int p0, n;
+  if (!sequence(table, b, p0, n)) {
+    if (tid == 0 && h == 0) raise_device_error(err, FE_DEVERR_PAGE_RANGE);
+    for (int i = tid; i < budget; i += kSelThreads) out[i] = -1;
+    return;
+  }
+  if (n <= budget) {
+    for (int i = tid; i < budget; i += kSelThreads) out[i] = i < n ? i : -1;
+    return;
+  }
+  const int end = n - recent, want = budget - sink - recent;
+  for (int i = tid; i < sink; i += kSelThreads) out[i] = i;
+  for (int i = tid; i < recent; i += kSelThreads) out[budget - recent + i] = end + i;
+  if (want == 0) return;
+  const float* sc = scores + static_cast<int64_t>(h) * table.cache_slots;
+  auto load = [&](int t) -> uint32_t {
+    const int64_t slot = slot_of(table, p0, t);
+    if (slot < 0) {
+      raise_device_error(err, FE_DEVERR_PAGE_RANGE);
+      return 0;
+    }
+    return ordered(__ldg(sc + slot));
+  };
+  const bool cached = n <= room;
+  if (cached)
+    for (int t = sink + tid; t < end; t += kSelThreads) keys[t] = load(t);
+  auto key = [&](int t) -> uint32_t { return cached ? keys[t] : load(t); };
+  // ---- the want-th largest key: `prefix` holds its bits above `shift`
+  uint32_t prefix = 0;
+  int left = want;  // of the keys that begin with prefix
+#pragma unroll 1
+  for (int pass = 0; pass < 3; ++pass) {
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+    const int bits = pass == 2 ? 10 : 11;
+    for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0;
+    __syncthreads();
+    const uint32_t mask = pass == 0 ? 0u : ~0u << (shift + bits);
+    for (int t = sink + tid; t < end; t += kSelThreads) {
+      const uint32_t x = key(t);
+      if ((x & mask) == prefix) atomicAdd(&hist[(x >> shift) & ((1u << bits) - 1)], 1);
+    }
+    __syncthreads();
+    // bins from the largest down, a few a thread
+    constexpr int kPer = kBins / kSelThreads;
+    int mine[kPer], sum = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      mine[i] = hist[kBins - 1 - (tid * kPer + i)];
+      sum += mine[i];
+    }
+    int total;
+    int above = block_scan(sum, warp_sums, total);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      if (above < left && left <= above + mine[i]) {
+        found[0] = kBins - 1 - (tid * kPer + i);
+        found[1] = left - above;
+      }
+      above += mine[i];
+    }
+    __syncthreads();
+    prefix |= static_cast<uint32_t>(found[0]) << shift;
+    left = found[1];
+    __syncthreads();
+  }
+  // ---- kept tokens in order: a warp owns a stretch of the tokens
+  const int span = end - sink;
+  const int per = ((span + kSelWarps - 1) / kSelWarps + 31) / 32 * 32;
+  const int t0 = min(end, sink + warp * per), t1 = min(end, t0 + per);
+  int gt = 0, eq = 0;
+  for (int t = t0 + lane; t < t1; t += 32) {
+    const uint32_t x = key(t);
+    gt += x > prefix;
+    eq += x == prefix;
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    gt += __shfl_xor_sync(0xffffffffu, gt, o);
+    eq += __shfl_xor_sync(0xffffffffu, eq, o);
+  }
+  int total;
+  int gt0 = block_scan(lane == 0 ? gt : 0, warp_sums, total);
+  int eq0 = block_scan(lane == 0 ? eq : 0, warp_sums, total);
+  gt0 = __shfl_sync(0xffffffffu, gt0, 0);
+  eq0 = __shfl_sync(0xffffffffu, eq0, 0);
+  const uint32_t below = (1u << lane) - 1;
+  for (int tb = t0; tb < t1; tb += 32) {
+    const int t = tb + lane;
+    const uint32_t x = t < t1 ? key(t) : 0;
+    const uint32_t mg = __ballot_sync(0xffffffffu, t < t1 && x > prefix);
+    const uint32_t me = __ballot_sync(0xffffffffu, t < t1 && x == prefix);
+    const int g = gt0 + __popc(mg & below), e = eq0 + __popc(me & below);
+    const bool keep = (mg >> lane & 1) || ((me >> lane & 1) && e < left);
+    if (keep) out[sink + g + min(e, left)] = t;
+    gt0 += __popc(mg);
+    eq0 += __popc(me);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// compaction: for every sequence and KV head, the K and V rows and the score
+// of token kept[j] move to token j. A CTA walks the list of one (sequence,
+// head) in order, for one slice of the row's 16-byte chunks (slices give one
+// sequence's move more CTAs). Each step moves kMoveRows tokens: all of them are
+// read before any is written, and the sources of later steps lie at or past
+// their own index (kept[j] >= j, checked), which no earlier step writes; so the
+// move works in place.
+// ---------------------------------------------------------------------------
+constexpr int kMoveThreads = 256;
+constexpr int kMoveUnroll = 4;
+
+struct MoveArgs {
+  uint4* k;
+  uint4* v;
+  float* scores;
+  const int32_t* kept;
+  SeqTable src, dst;
+  int in_place;
+  int hkv, budget, chunks;  // chunks: 16-byte chunks of a K (or V) row
+  int slice;                // chunks of a CTA's slice, of K and of V each
+  unsigned int* err;
+};
+
+__global__ void __launch_bounds__(kMoveThreads) compact_kernel(const MoveArgs a) {
+  pdl_trigger();
+  pdl_wait();
+  const int b = blockIdx.x / a.hkv, h = blockIdx.x % a.hkv;
+  const int lanes = 2 * a.slice;  // threads of a token
+  const int row = threadIdx.x / lanes, c = threadIdx.x % lanes;
+  const int rows = kMoveThreads / lanes;
+  const bool idle = row >= rows;  // threads left over where lanes does not divide the block
+  const bool is_v = c >= a.slice;
+  const int chunk = blockIdx.y * a.slice + (is_v ? c - a.slice : c);
+  const bool first = blockIdx.y == 0 && c == 0;
+  uint4* pool = is_v ? a.v : a.k;
+  float* sc = a.scores ? a.scores + static_cast<int64_t>(h) * a.src.cache_slots : nullptr;
+  int p0, n, d0, dn;
+  bool good = sequence(a.src, b, p0, n);
+  if (a.in_place) {
+    d0 = p0;
+    dn = n;
+  } else {
+    d0 = __ldg(a.dst.kv + b);
+    const int d1 = __ldg(a.dst.kv + b + 1);
+    good &= d0 >= 0 && d1 >= d0 && d1 <= a.dst.num_pages;
+    dn = good ? static_cast<int>(min(static_cast<int64_t>(d1 - d0) * a.src.page,
+                                     static_cast<int64_t>(INT32_MAX)))
+              : 0;
+  }
+  if (!good) {
+    if (threadIdx.x == 0 && h == 0 && blockIdx.y == 0)
+      raise_device_error(a.err, FE_DEVERR_PAGE_RANGE);
+    return;
+  }
+  const int32_t* kept = a.kept + static_cast<int64_t>(blockIdx.x) * a.budget;
+  for (int j0 = 0; j0 < a.budget; j0 += rows * kMoveUnroll) {
+    int64_t to[kMoveUnroll];
+    uint4 x[kMoveUnroll];
+    float s[kMoveUnroll];
+#pragma unroll
+    for (int u = 0; u < kMoveUnroll; ++u) {
+      const int j = j0 + u * rows + row;
+      to[u] = -1;
+      const int t = !idle && j < a.budget ? __ldg(kept + j) : -1;
+      if (t < 0 || (a.in_place && t == j)) continue;
+      int64_t from = -1;
+      if (t < n && j < dn && (!a.in_place || t > j)) {
+        from = slot_of(a.src, p0, t);
+        to[u] = slot_of(a.in_place ? a.src : a.dst, d0, j);
+      }
+      if (from < 0 || to[u] < 0) {
+        if (first) raise_device_error(a.err, FE_DEVERR_PAGE_RANGE);
+        to[u] = -1;
+        continue;
+      }
+      x[u] = pool[(from * a.hkv + h) * a.chunks + chunk];
+      if (first && sc) s[u] = sc[from];
+    }
+    __syncthreads();  // everything of this step has been read
+#pragma unroll
+    for (int u = 0; u < kMoveUnroll; ++u) {
+      if (to[u] < 0) continue;
+      pool[(to[u] * a.hkv + h) * a.chunks + chunk] = x[u];
+      if (first && sc) sc[to[u]] = s[u];
+    }
+  }
+}
+
+int check_lists(const char* what, const int32_t* kv, const int32_t* pages, const int32_t* last,
+                int num_pages, int batch, int hkv, int page, int budget, int64_t cache_slots) {
+  const std::string name = what;
+  if (batch < 0 || hkv <= 0 || budget < 0 || num_pages < 0)
+    return fail(FE_ERR_INVALID_ARGUMENT, name + ": sizes out of range");
+  if (page <= 0 || page % 16 != 0)
+    return fail(FE_ERR_UNSUPPORTED, name + ": page must be a multiple of 16");
+  if (cache_slots <= 0 || cache_slots % page != 0 || cache_slots >= INT32_MAX)
+    return fail(FE_ERR_INVALID_ARGUMENT,
+                name + ": cache_slots must be whole pages, below 2^31");
+  if (int64_t(batch) * hkv > INT32_MAX)
+    return fail(FE_ERR_CAPACITY, name + ": batch x hkv too large");
+  if (batch > 0 && budget > 0 && (!kv || !pages || !last))
+    return fail(FE_ERR_INVALID_ARGUMENT, name + ": null pointer");
+  return FE_OK;
+}
+
+}  // namespace
+}  // namespace fe
+
+using namespace fe;
+
+extern "C" {
+
+int fe_kv_select(const float* scores, const int32_t* kv, const int32_t* pages, int num_pages,
+                 const int32_t* last, int32_t* kept, int batch, int max_len, int hkv, int page,
+                 int budget, int sink, int recent, int64_t cache_slots, void* stream) {
+  int rc = check_lists("fe_kv_select", kv, pages, last, num_pages, batch, hkv, page, budget,
+                       cache_slots);
+  if (rc != FE_OK) return rc;
+  if (sink < 0 || recent < 0 || int64_t(sink) + recent > budget)
+    return fail(FE_ERR_INVALID_ARGUMENT,
+                "fe_kv_select: sink and recent must be non-negative and fit the budget");
+  if (max_len < 0) return fail(FE_ERR_INVALID_ARGUMENT, "fe_kv_select: max_len < 0");
+  if (batch == 0 || budget == 0) return FE_OK;
+  if (!scores || !kept) return fail(FE_ERR_INVALID_ARGUMENT, "fe_kv_select: null pointer");
+  const SeqTable table{kv, pages, last, num_pages, page, cache_slots};
+  auto s = static_cast<cudaStream_t>(stream);
+  const int room = max_len <= kSelKeys ? max_len : 0;
+  static std::once_flag once;
+  static cudaError_t attr = cudaSuccess;
+  std::call_once(once, [] {
+    attr = cudaFuncSetAttribute(select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                kSelKeys * 4);
+  });
+  if (attr != cudaSuccess) return cuda_fail(attr, "fe_kv_select: shared memory attribute");
+  FE_CUDA_TRY(launch_pdl(select_kernel, dim3(batch * hkv), dim3(kSelThreads),
+                         sizeof(uint32_t) * room, s, scores, table, kept, hkv, budget, sink,
+                         recent, room, device_error_word()));
+  return FE_OK;
+}
+
+int fe_kv_compact(void* k_pool, void* v_pool, float* scores, const int32_t* kept,
+                  const int32_t* kv, const int32_t* pages, int num_pages, const int32_t* last,
+                  const int32_t* dst_kv, const int32_t* dst_pages, int num_dst_pages, int batch,
+                  int hkv, int dim, int page, int budget, int dtype, int64_t cache_slots,
+                  void* stream) {
+  if (!valid_dtype(dtype)) return fail(FE_ERR_INVALID_ARGUMENT, "fe_kv_compact: bad dtype");
+  int rc = check_lists("fe_kv_compact", kv, pages, last, num_pages, batch, hkv, page, budget,
+                       cache_slots);
+  if (rc != FE_OK) return rc;
+  if (dim <= 0 || dim % 8 != 0 || dim > 512)
+    return fail(FE_ERR_UNSUPPORTED, "fe_kv_compact: dim must be a multiple of 8, at most 512");
+  if ((dst_kv == nullptr) != (dst_pages == nullptr) || num_dst_pages < 0)
+    return fail(FE_ERR_INVALID_ARGUMENT, "fe_kv_compact: dst_kv and dst_pages go together");
+  if (batch == 0 || budget == 0) return FE_OK;
+  if (!k_pool || !v_pool || !kept)
+    return fail(FE_ERR_INVALID_ARGUMENT, "fe_kv_compact: null pointer");
+  if (!aligned16(k_pool) || !aligned16(v_pool))
+    return fail(FE_ERR_INVALID_ARGUMENT, "fe_kv_compact: pools must be 16-byte aligned");
+  MoveArgs a{};
+  a.k = static_cast<uint4*>(k_pool);
+  a.v = static_cast<uint4*>(v_pool);
+  a.scores = scores;
+  a.kept = kept;
+  a.src = SeqTable{kv, pages, last, num_pages, page, cache_slots};
+  a.dst = SeqTable{dst_kv, dst_pages, nullptr, num_dst_pages, page, cache_slots};
+  a.in_place = dst_kv == nullptr;
+  a.hkv = hkv;
+  a.budget = budget;
+  a.chunks = dim / 8;
+  a.err = device_error_word();
+  // slices of whole 32-byte sectors while there are fewer CTAs than SMs take
+  const int64_t lists = int64_t(batch) * hkv;
+  a.slice = a.chunks;
+  while (a.slice % 4 == 0 && lists * (a.chunks / a.slice) < 512) a.slice /= 2;
+  FE_CUDA_TRY(launch_pdl(compact_kernel, dim3(static_cast<unsigned>(lists), a.chunks / a.slice),
+                         dim3(kMoveThreads), 0, static_cast<cudaStream_t>(stream), a));
+  return FE_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,339 @@
+// Rotary embedding with several position axes (time, height and width of an
+// image's or video's patches), alone and fused with the K/V append. No
+// counterpart in the reference, whose rope has one position a row
+// (Cambridgebit/FlashEngine.cpp src/cuda_kernels.cu:19-23).
+//
+// Pair j of a head, (x[j], x[j + r]) with r = rotary_dim / 2, turns by the
+// cos / sin of cache row pos[axis(j)][row], column j: the rotation of fe_rope,
+// with a cache row of its own for each pair's axis and the same roundings, so
+// that equal positions on all axes give fe_rope's bits.
+//
+// HBM-bound: 4 bytes of q and 8 of k and v per element (in and out) and one
+// cos / sin row a token.
+#include <string>
+
+#include "fe_rope_common.cuh"
+
+namespace fe {
+namespace {
+
+constexpr int kMaxAxes = FE_MAX_AXES;
+constexpr int kMaxPairs = 256;
+constexpr int kAxesThreads = 256;
+
+// Axis of each pair, a kernel argument (the caller's list lives on the host).
+struct __align__(16) AxisMap {
+  uint8_t axis[kMaxPairs];
+};
+
+struct AxesArgs {
+  const int64_t* slots;
+  const int64_t* pos;  // [axes][rows]
+  const float* cache;
+  unsigned int* err;
+  int64_t cache_slots;
+  int rows, axes, hq, hkv, dim, rot, max_positions;
+};
+
+// The row's position on each axis; false (and flagged by `who`) when one lies
+// outside the cache.
+__device__ __forceinline__ bool row_positions(const AxesArgs& a, int row, int (&p)[kMaxAxes],
+                                              bool who) {
+  bool good = true;
+#pragma unroll
+  for (int x = 0; x < kMaxAxes; ++x) {
+    const int64_t v = x < a.axes ? __ldg(a.pos + static_cast<int64_t>(x) * a.rows + row) : 0;
+    good &= v >= 0 && v < a.max_positions;
+    p[x] = static_cast<int>(v);
+  }
+  if (!good && who) raise_device_error(a.err, FE_DEVERR_POS_RANGE);
+  return good;
+}
+
+__device__ __forceinline__ int pick(const int (&p)[kMaxAxes], int axis) {
+  return axis == 0 ? p[0] : axis == 1 ? p[1] : axis == 2 ? p[2] : p[3];
+}
+
+// Any dim and rotary_dim that are multiples of 4: a thread owns two adjacent
+// pairs (or four unrotated dims) of a head, as in fe_rope's plain form.
+template <typename T>
+__global__ void __launch_bounds__(kAxesThreads)
+    rope_axes_kernel(T* __restrict__ q, const T* k, const T* __restrict__ v, T* k_out,
+                     T* __restrict__ kc, T* __restrict__ vc, const AxesArgs a, const AxisMap map) {
+  using V = typename Pair2<T>::V;
+  pdl_trigger();
+  pdl_wait();  // q, k, v come from, and the pools are read by, earlier kernels
+  const int per_head = a.dim / 4, heads = a.hq + a.hkv;
+  const int64_t idx = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+  if (idx >= static_cast<int64_t>(a.rows) * heads * per_head) return;
+  const int jp = static_cast<int>(idx % per_head);
+  const int head = static_cast<int>((idx / per_head) % heads);
+  const int row = static_cast<int>(idx / (static_cast<int64_t>(per_head) * heads));
+  int p[kMaxAxes];
+  if (!row_positions(a, row, p, jp == 0 && head == 0)) return;
+  const bool rotating = jp < a.rot / 4;
+  const int i0 = rotating ? jp : (a.rot + 4 * (jp - a.rot / 4)) / 2;
+  const int i1 = rotating ? (a.rot / 2 + 2 * jp) / 2 : i0 + 1;
+  float2 c = make_float2(0.f, 0.f), s = c;
+  if (rotating) {
+    const int j = 2 * jp, r = a.rot / 2;
+    const float* c0 = a.cache + static_cast<int64_t>(pick(p, map.axis[j])) * a.rot + j;
+    const float* c1 = a.cache + static_cast<int64_t>(pick(p, map.axis[j + 1])) * a.rot + j + 1;
+    c = make_float2(__ldg(c0), __ldg(c1));
+    s = make_float2(__ldg(c0 + r), __ldg(c1 + r));
+  }
+  if (head < a.hq) {
+    if (!rotating) return;  // q's unrotated dims stay as they are
+    V* base = reinterpret_cast<V*>(q + (static_cast<int64_t>(row) * a.hq + head) * a.dim);
+    V lo = base[i0], hi = base[i1];
+    rotate<T>(lo, hi, c, s);
+    base[i0] = lo;
+    base[i1] = hi;
+    return;
+  }
+  const int h = head - a.hq;
+  const int64_t off = (static_cast<int64_t>(row) * a.hkv + h) * a.dim;
+  const V* kb = reinterpret_cast<const V*>(k + off);
+  V lo = kb[i0], hi = kb[i1];
+  if (rotating) rotate<T>(lo, hi, c, s);
+  if (k_out && (rotating || k_out != k)) {
+    V* ko = reinterpret_cast<V*>(k_out + off);
+    ko[i0] = lo;
+    ko[i1] = hi;
+  }
+  if (!kc) return;
+  const int64_t slot = __ldg(a.slots + row);
+  if (slot < 0) return;
+  if (slot >= a.cache_slots) {
+    if (jp == 0 && h == 0) raise_device_error(a.err, FE_DEVERR_SLOT_RANGE);
+    return;
+  }
+  const int64_t dst = (slot * a.hkv + h) * a.dim;
+  V* kd = reinterpret_cast<V*>(kc + dst);
+  kd[i0] = lo;
+  kd[i1] = hi;
+  const V* vb = reinterpret_cast<const V*>(v + off);
+  V* vd = reinterpret_cast<V*>(vc + dst);
+  vd[i0] = vb[i0];
+  vd[i1] = vb[i1];
+}
+
+// 16-byte form, for rotary_dim a multiple of 16, dim a multiple of 8 and
+// 16-byte aligned buffers. A head is `units` units: unit u < rot/16 owns the
+// eight pairs 8u .. 8u+7 (two 16-byte chunks), the others an unrotated chunk.
+// A thread keeps its unit and walks the heads hl, hl + hl_count, ... two at a
+// time, so that a row's cos / sin are read once for all of its heads.
+// kWhole: the eight pairs of every unit turn by one axis (sections that are
+// multiples of 8), and their cos / sin are whole vectors.
+template <typename T, bool kWhole>
+__global__ void __launch_bounds__(kAxesThreads)
+    rope_axes_vec_kernel(T* __restrict__ q, const T* k, const T* __restrict__ v, T* k_out,
+                         T* __restrict__ kc, T* __restrict__ vc, const AxesArgs a,
+                         const AxisMap map, int units, int hl_count) {
+  using V = typename Pair2<T>::V;
+  union Chunk {
+    uint4 u;
+    V v[4];
+  };
+  pdl_trigger();
+  pdl_wait();  // q, k, v come from, and the pools are read by, earlier kernels
+  const int heads = a.hq + a.hkv;
+  const int hl = threadIdx.x / units, u = threadIdx.x - hl * units;
+  if (hl >= hl_count) return;
+  const int rot_units = a.rot / 16, r = a.rot / 2;
+  const bool rotating = u < rot_units;
+  const int e0 = rotating ? 8 * u : a.rot + 8 * (u - rot_units);
+  const int e1 = e0 + r;  // the partners (rotating)
+  const int first = blockIdx.x * hl_count + hl, step = gridDim.x * hl_count;
+  for (int row = blockIdx.y; row < a.rows; row += gridDim.y) {
+    float2 c[4], s[4];
+    bool known = false, good = true;
+    int64_t slot = -1;
+    for (int h0 = first; h0 < heads; h0 += 2 * step) {
+      // every load that does not depend on the position first
+      Chunk lo[2], hi[2], vlo[2], vhi[2];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int head = h0 + x * step;
+        if (head >= heads || (head < a.hq && !rotating)) continue;
+        const T* src = head < a.hq ? q + (static_cast<int64_t>(row) * a.hq + head) * a.dim
+                                   : k + (static_cast<int64_t>(row) * a.hkv + head - a.hq) * a.dim;
+        lo[x].u = *reinterpret_cast<const uint4*>(src + e0);
+        if (rotating) hi[x].u = *reinterpret_cast<const uint4*>(src + e1);
+        if (head >= a.hq && kc) {
+          const T* vs = v + (static_cast<int64_t>(row) * a.hkv + head - a.hq) * a.dim;
+          vlo[x].u = *reinterpret_cast<const uint4*>(vs + e0);
+          if (rotating) vhi[x].u = *reinterpret_cast<const uint4*>(vs + e1);
+        }
+      }
+      if (!known) {
+        known = true;
+        if (kc) slot = __ldg(a.slots + row);
+        int p[kMaxAxes];
+        good = row_positions(a, row, p, threadIdx.x == 0 && blockIdx.x == 0);
+        if (slot >= a.cache_slots) {
+          if (threadIdx.x == 0 && blockIdx.x == 0 && good)
+            raise_device_error(a.err, FE_DEVERR_SLOT_RANGE);
+          slot = -1;
+        }
+        if (good && rotating) {
+          if constexpr (kWhole) {
+            const float* base =
+                a.cache + static_cast<int64_t>(pick(p, map.axis[8 * u])) * a.rot + 8 * u;
+            const float4* cp = reinterpret_cast<const float4*>(base);
+            const float4* sp = reinterpret_cast<const float4*>(base + r);
+            const float4 c0 = __ldg(cp), c1 = __ldg(cp + 1), s0 = __ldg(sp), s1 = __ldg(sp + 1);
+            c[0] = make_float2(c0.x, c0.y);
+            c[1] = make_float2(c0.z, c0.w);
+            c[2] = make_float2(c1.x, c1.y);
+            c[3] = make_float2(c1.z, c1.w);
+            s[0] = make_float2(s0.x, s0.y);
+            s[1] = make_float2(s0.z, s0.w);
+            s[2] = make_float2(s1.x, s1.y);
+            s[3] = make_float2(s1.z, s1.w);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int j = 8 * u + 2 * i;
+              const float* c0 = a.cache + static_cast<int64_t>(pick(p, map.axis[j])) * a.rot + j;
+              const float* c1 =
+                  a.cache + static_cast<int64_t>(pick(p, map.axis[j + 1])) * a.rot + j + 1;
+              c[i] = make_float2(__ldg(c0), __ldg(c1));
+              s[i] = make_float2(__ldg(c0 + r), __ldg(c1 + r));
+            }
+          }
+        }
+      }
+      if (!good) break;
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int head = h0 + x * step;
+        if (head >= heads || (head < a.hq && !rotating)) continue;
+        if (rotating)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) rotate<T>(lo[x].v[i], hi[x].v[i], c[i], s[i]);
+        if (head < a.hq) {
+          T* dst = q + (static_cast<int64_t>(row) * a.hq + head) * a.dim;
+          *reinterpret_cast<uint4*>(dst + e0) = lo[x].u;
+          *reinterpret_cast<uint4*>(dst + e1) = hi[x].u;
+          continue;
+        }
+        const int h = head - a.hq;
+        const int64_t off = (static_cast<int64_t>(row) * a.hkv + h) * a.dim;
+        if (k_out && (rotating || k_out != k)) {
+          *reinterpret_cast<uint4*>(k_out + off + e0) = lo[x].u;
+          if (rotating) *reinterpret_cast<uint4*>(k_out + off + e1) = hi[x].u;
+        }
+        if (!kc || slot < 0) continue;
+        const int64_t dst = (slot * a.hkv + h) * a.dim;
+        *reinterpret_cast<uint4*>(kc + dst + e0) = lo[x].u;
+        *reinterpret_cast<uint4*>(vc + dst + e0) = vlo[x].u;
+        if (rotating) {
+          *reinterpret_cast<uint4*>(kc + dst + e1) = hi[x].u;
+          *reinterpret_cast<uint4*>(vc + dst + e1) = vhi[x].u;
+        }
+      }
+    }
+  }
+}
+
+template <typename T>
+int launch_axes(void* q, const void* k, const void* v, void* k_out, void* kc, void* vc,
+                const AxesArgs& a, const AxisMap& map, cudaStream_t stream) {
+  T* tq = static_cast<T*>(q);
+  const T* tk = static_cast<const T*>(k);
+  const T* tv = static_cast<const T*>(v);
+  T *to = static_cast<T*>(k_out), *tkc = static_cast<T*>(kc), *tvc = static_cast<T*>(vc);
+  const int heads = a.hq + a.hkv;
+  const int units = a.rot / 16 + (a.dim - a.rot) / 8;
+  if (a.rot % 16 == 0 && a.dim % 8 == 0 && aligned16(q) && aligned16(k) && aligned16(v) &&
+      aligned16(k_out) && aligned16(kc) && aligned16(vc) && aligned16(a.cache) &&
+      units <= kAxesThreads) {
+    bool whole = true;
+    for (int j = 0; j < a.rot / 2; ++j) whole &= map.axis[j] == map.axis[j & ~7];
+    // heads of a row over as few blocks as fit, evenly
+    const int most = kAxesThreads / units;
+    const int passes = (heads + most - 1) / most;
+    const int hl = (heads + passes - 1) / passes;
+    const int threads = (hl * units + 31) / 32 * 32;
+    const dim3 grid(a.rows < 1024 ? passes : (passes + 1) / 2, a.rows < 65535 ? a.rows : 65535);
+    auto kernel = whole ? rope_axes_vec_kernel<T, true> : rope_axes_vec_kernel<T, false>;
+    FE_CUDA_TRY(launch_pdl(kernel, grid, dim3(threads), 0, stream, tq, tk, tv, to, tkc, tvc, a,
+                           map, units, hl));
+    return FE_OK;
+  }
+  const int64_t total = static_cast<int64_t>(a.rows) * heads * (a.dim / 4);
+  const int64_t blocks = (total + kAxesThreads - 1) / kAxesThreads;
+  if (blocks > INT32_MAX) return fail(FE_ERR_CAPACITY, "fe_rope_axes: too many rows");
+  FE_CUDA_TRY(launch_pdl(rope_axes_kernel<T>, dim3(static_cast<int>(blocks)), dim3(kAxesThreads),
+                         0, stream, tq, tk, tv, to, tkc, tvc, a, map));
+  return FE_OK;
+}
+
+int run_axes(const char* what, void* q, const void* k, const void* v, void* k_out, void* k_pool,
+             void* v_pool, const int64_t* slots, const int64_t* pos, int axes,
+             const uint8_t* pair_axis, const float* cache, int rows, int hq, int hkv, int dim,
+             int rot, int max_positions, int dtype, int64_t cache_slots, bool append,
+             void* stream) {
+  const std::string name = what;
+  if (!valid_dtype(dtype)) return fail(FE_ERR_INVALID_ARGUMENT, name + ": bad dtype");
+  if (rows < 0 || hq < 0 || hkv <= 0 || dim <= 0 || max_positions <= 0)
+    return fail(FE_ERR_INVALID_ARGUMENT, name + ": sizes out of range");
+  if (axes < 1 || axes > kMaxAxes)
+    return fail(FE_ERR_UNSUPPORTED, name + ": 1 to 4 axes");
+  if (dim % 4 != 0 || rot < 0 || rot > dim || rot % 4 != 0 || rot > 2 * kMaxPairs)
+    return fail(FE_ERR_UNSUPPORTED, name + ": dim and rotary_dim must be multiples of 4, "
+                                           "rotary_dim <= dim and <= 512");
+  if (rot > 0 && !pair_axis) return fail(FE_ERR_INVALID_ARGUMENT, name + ": pair_axis is null");
+  AxisMap map{};
+  for (int j = 0; j < rot / 2; ++j) {
+    if (pair_axis[j] >= axes)
+      return fail(FE_ERR_INVALID_ARGUMENT, name + ": a pair's axis is not below `axes`");
+    map.axis[j] = pair_axis[j];
+  }
+  if (rows == 0) return FE_OK;
+  if (!k || !pos || (rot > 0 && !cache) || (hq > 0 && !q))
+    return fail(FE_ERR_INVALID_ARGUMENT, name + ": null pointer");
+  if (append && (!v || !k_pool || !v_pool || !slots))
+    return fail(FE_ERR_INVALID_ARGUMENT, name + ": null pointer");
+  if (append && cache_slots <= 0)
+    return fail(FE_ERR_INVALID_ARGUMENT, name + ": cache_slots <= 0");
+  for (const void* p : {static_cast<const void*>(q), k, v, static_cast<const void*>(k_out),
+                        static_cast<const void*>(k_pool), static_cast<const void*>(v_pool),
+                        static_cast<const void*>(cache)})
+    if (reinterpret_cast<uintptr_t>(p) & 3u)
+      return fail(FE_ERR_INVALID_ARGUMENT, name + ": buffers must be 4-byte aligned");
+  const AxesArgs a{slots, pos, cache, device_error_word(), cache_slots, rows, axes, hq, hkv, dim,
+                   rot, max_positions};
+  auto s = static_cast<cudaStream_t>(stream);
+  if (dtype == FE_DTYPE_BF16)
+    return launch_axes<__nv_bfloat16>(q, k, v, k_out, k_pool, v_pool, a, map, s);
+  return launch_axes<__half>(q, k, v, k_out, k_pool, v_pool, a, map, s);
+}
+
+}  // namespace
+}  // namespace fe
+
+using namespace fe;
+
+extern "C" {
+
+int fe_rope_axes(void* q, void* k, const int64_t* pos, int axes, const uint8_t* pair_axis,
+                 const float* cache, int rows, int hq, int hkv, int dim, int rotary_dim,
+                 int max_positions, int dtype, void* stream) {
+  return run_axes("fe_rope_axes", q, k, nullptr, k, nullptr, nullptr, nullptr, pos, axes,
+                  pair_axis, cache, rows, hq, hkv, dim, rotary_dim, max_positions, dtype, 0, false,
+                  stream);
+}
+
+int fe_rope_axes_append(void* q, const void* k, const void* v, void* k_out, void* k_pool,
+                        void* v_pool, const int64_t* slots, const int64_t* pos, int axes,
+                        const uint8_t* pair_axis, const float* cache, int rows, int hq, int hkv,
+                        int dim, int rotary_dim, int max_positions, int dtype,
+                        int64_t cache_slots, void* stream) {
+  return run_axes("fe_rope_axes_append", q, k, v, k_out, k_pool, v_pool, slots, pos, axes,
+                  pair_axis, cache, rows, hq, hkv, dim, rotary_dim, max_positions, dtype,
+                  cache_slots, true, stream);
+}
+
+}  // extern "C"

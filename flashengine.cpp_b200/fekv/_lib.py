@@ -35,6 +35,7 @@ FE_DEVERR_PLAN = 0x40
 
 FE_MAX_LAYERS = 128
 FE_KV8_BLOCK = 16
+FE_MAX_AXES = 4
 
 FE_ATTN_LISTS_DECODE = 1
 FE_ATTN_LISTS_ROWS = 2
@@ -78,6 +79,10 @@ SIGNATURES = {
     "fe_rope_append": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I64,
                             _P]),
     "fe_accept": (_I, [_P, _P, _P, _I, _I, _P]),
+    "fe_rope_axes": (_I, [_P, _P, _P, _I, _P, _P] + [_I] * 7 + [_P]),
+    "fe_rope_axes_append": (_I, [_P] * 8 + [_I, _P, _P] + [_I] * 7 + [_I64, _P]),
+    "fe_kv_select": (_I, [_P] * 3 + [_I] + [_P] * 2 + [_I] * 7 + [_I64, _P]),
+    "fe_kv_compact": (_I, [_P] * 6 + [_I] + [_P] * 3 + [_I] * 7 + [_I64, _P]),
 }
 
 

@@ -575,6 +575,184 @@ class Kv8Plan(AttentionPlan):
               "attention")
 
 
+# ---------------------------------------------------------------------------
+# Long shared prompts: rotary positions with several axes, and eviction by
+# accumulated attention weight (no reference counterpart). Checks as for the
+# 8-bit calls: each tensor attribute is read once.
+# ---------------------------------------------------------------------------
+
+def _code(name, dt):
+    torch = _torch()
+    if dt is torch.bfloat16:
+        return FE_DTYPE_BF16
+    if dt is torch.float16:
+        return FE_DTYPE_F16
+    raise ValueError(f"{name}: expected float16 or bfloat16, got {dt}")
+
+
+def _pool16(name, t, dtype, width, device):
+    """Address and slots of a 16-bit pool [cache_slots, ...] of `width`
+    elements a slot on CUDA device `device`."""
+    slots, odd = divmod(t.numel(), width)
+    if odd or not slots or t.shape[0] != slots or t.dtype is not dtype or \
+            t.get_device() != device or not t.is_contiguous():
+        raise ValueError(f"{name}: expected a contiguous {dtype} pool of {width} elements a slot on "
+                         f"the current device (cuda:{device}), got {t.dtype} {tuple(t.shape)} on "
+                         f"{t.device}")
+    return t.data_ptr(), slots
+
+
+def rope_sections(sections, interleaved=False):
+    """The axis of each rotary pair, for rope_axes: sections[a] pairs turn by
+    axis a. In order (all pairs of axis 0, then those of axis 1, ...), or
+    `interleaved`: pair j belongs to axis j % axes while that axis has pairs
+    left, else to axis 0."""
+    sections = [int(n) for n in sections]
+    if not 1 <= len(sections) <= _lib.FE_MAX_AXES or min(sections) < 0:
+        raise ValueError(f"sections {sections}: 1 to {_lib.FE_MAX_AXES} axes of pairs")
+    if not interleaved:
+        return bytes(a for a, n in enumerate(sections) for _ in range(n))
+    axes = len(sections)
+    out = bytes(j % axes if j // axes < sections[j % axes] else 0 for j in range(sum(sections)))
+    if [out.count(a) for a in range(axes)] != sections:
+        raise ValueError(f"sections {sections} cannot take turns: axis 0 is not the longest")
+    return out
+
+
+def _axes_args(k, pos, cache, pair_axis, device):
+    """What the two calls share: shape, dtype code, positions, cache."""
+    torch = _torch()
+    if k.dim() != 3 or cache.dim() != 2 or pos.dim() != 2:
+        raise ValueError("expected k [rows, hkv, dim], cache [max_positions, rotary_dim] and pos "
+                         "[axes, rows]")
+    rows, hkv, dim = k.shape
+    axes = pos.shape[0]
+    most, rot = cache.shape
+    if not isinstance(pair_axis, bytes) or 2 * len(pair_axis) != rot:
+        raise ValueError(f"pair_axis: expected {rot // 2} bytes, one for each pair "
+                         "(rope_sections)")
+    if k.get_device() != device or not k.is_contiguous():
+        raise ValueError(f"k: expected a contiguous tensor on the current device (cuda:{device})")
+    pp = _kv8_rows("pos", pos, torch.int64, (axes, rows), device)
+    cp = _kv8_rows("cache", cache, torch.float32, (most, rot), device)
+    return rows, hkv, dim, axes, rot, most, pp, cp, _code("k", k.dtype)
+
+
+def rope_axes(q, k, pos, cache, pair_axis, stream=None):
+    """rope() with several position axes: pos int64 [axes, rows], pair_axis the
+    axis of each rotary pair (rope_sections). q [rows, hq, dim] (or None) and k
+    [rows, hkv, dim] are rotated in place."""
+    device = _kv8_device()
+    rows, hkv, dim, axes, rot, most, pp, cp, code = _axes_args(k, pos, cache, pair_axis, device)
+    hq, qp = 0, None
+    if q is not None:
+        hq = q.shape[1] if q.dim() == 3 else -1
+        qp = _kv8_rows("q", q, k.dtype, (rows, hq, dim), device)
+    rc = _lib.load().fe_rope_axes(qp, k.data_ptr(), pp, axes, pair_axis, cp, rows, hq, hkv, dim,
+                                  rot, most, code, _kv8_stream(stream, device))
+    if rc:
+        check(rc, "rope_axes")
+
+
+def rope_axes_append(q, k, v, kc, vc, slots, pos, cache, pair_axis, k_out=None, stream=None):
+    """rope_append() with several position axes (see rope_axes): q rotated in
+    place, rotated k and v written to the pools [cache_slots, hkv, dim] through
+    `slots`; the rotated keys also go to `k_out` when given (it may be `k`)."""
+    torch = _torch()
+    device = _kv8_device()
+    rows, hkv, dim, axes, rot, most, pp, cp, code = _axes_args(k, pos, cache, pair_axis, device)
+    dt, shape = k.dtype, k.shape
+    hq, qp = 0, None
+    if q is not None:
+        hq = q.shape[1] if q.dim() == 3 else -1
+        qp = _kv8_rows("q", q, dt, (rows, hq, dim), device)
+    vp = _kv8_rows("v", v, dt, shape, device)
+    op = None if k_out is None else _kv8_rows("k_out", k_out, dt, shape, device)
+    sp = _kv8_rows("slots", slots, torch.int64, (rows,), device)
+    kcp, cache_slots = _pool16("kc", kc, dt, hkv * dim, device)
+    vcp, v_slots = _pool16("vc", vc, dt, hkv * dim, device)
+    if v_slots != cache_slots:
+        raise ValueError(f"kc has {cache_slots} slots, vc {v_slots}")
+    rc = _lib.load().fe_rope_axes_append(qp, k.data_ptr(), vp, op, kcp, vcp, sp, pp, axes,
+                                         pair_axis, cp, rows, hq, hkv, dim, rot, most, code,
+                                         cache_slots, _kv8_stream(stream, device))
+    if rc:
+        check(rc, "rope_axes_append")
+
+
+def _score_pool(scores, device):
+    """Address and shape of a score pool fp32 [hkv, cache_slots]."""
+    if scores.dim() != 2:
+        raise ValueError(f"scores: expected [hkv, cache_slots], got {tuple(scores.shape)}")
+    return _kv8_rows("scores", scores, _torch().float32, scores.shape, device), scores.shape
+
+
+def select_tokens(scores, kv, pages, last, kept, page, max_len, sink=0, recent=0, stream=None):
+    """The tokens that each sequence and KV head keeps, into `kept` (int32
+    [batch, hkv, budget]): ascending, -1 past the last. The first `sink` and the
+    last `recent` tokens stay, of the others those with the highest `scores`
+    (fp32 [hkv, cache_slots]), `budget` in all; ties go to the lowest index. kv
+    [batch+1], pages and last [batch]: int32 CUDA tensors as in gather();
+    max_len sizes the launch."""
+    device = _kv8_device()
+    sp, (hkv, slots) = _score_pool(scores, device)
+    _kv8_lists(device, kv, pages, last)
+    batch = last.numel()
+    if last.shape != (batch,) or kv.shape != (batch + 1,):
+        raise ValueError("last must have one entry per sequence, kv one more")
+    if kept.dim() != 3:
+        raise ValueError(f"kept: expected [batch, hkv, budget], got {tuple(kept.shape)}")
+    budget = kept.shape[2]
+    kp = _kv8_rows("kept", kept, _torch().int32, (batch, hkv, budget), device)
+    rc = _lib.load().fe_kv_select(sp, kv.data_ptr(), pages.data_ptr(), pages.numel(),
+                                  last.data_ptr(), kp, batch, max_len, hkv, page, budget, sink,
+                                  recent, slots, _kv8_stream(stream, device))
+    if rc:
+        check(rc, "select_tokens")
+
+
+def compact_tokens(k_pool, v_pool, scores, kept, kv, pages, last, page, dst_kv=None,
+                   dst_pages=None, stream=None):
+    """Move the kept tokens (int32 [batch, hkv, budget], as select_tokens writes
+    them) of each sequence and KV head to its front: rows of the pools
+    [cache_slots, hkv, dim] and of `scores` (fp32 [hkv, cache_slots] or None).
+    In place, or to the pages dst_pages[dst_kv[b]:dst_kv[b + 1]], which are none
+    of the sources'. The sequence then has as many tokens as were kept:
+    min(length, budget). kv, pages, last, dst_*: int32 CUDA tensors."""
+    torch = _torch()
+    device = _kv8_device()
+    if k_pool.dim() != 3 or k_pool.shape != v_pool.shape:
+        raise ValueError(f"pools {tuple(k_pool.shape)}, {tuple(v_pool.shape)}: expected two of "
+                         "[cache_slots, hkv, dim]")
+    slots, hkv, dim = k_pool.shape
+    kp, _ = _pool16("k_pool", k_pool, k_pool.dtype, hkv * dim, device)
+    vp, _ = _pool16("v_pool", v_pool, k_pool.dtype, hkv * dim, device)
+    sp = None
+    if scores is not None:
+        sp = _kv8_rows("scores", scores, torch.float32, (hkv, slots), device)
+    _kv8_lists(device, kv, pages, last)
+    batch = last.numel()
+    if last.shape != (batch,) or kv.shape != (batch + 1,):
+        raise ValueError("last must have one entry per sequence, kv one more")
+    if kept.dim() != 3:
+        raise ValueError(f"kept: expected [batch, hkv, budget], got {tuple(kept.shape)}")
+    budget = kept.shape[2]
+    lp = _kv8_rows("kept", kept, torch.int32, (batch, hkv, budget), device)
+    dk = dp = None
+    count = 0
+    if dst_kv is not None or dst_pages is not None:
+        _kv8_lists(device, dst_kv, dst_pages)
+        if dst_kv.shape != (batch + 1,):
+            raise ValueError("dst_kv must have one entry more than there are sequences")
+        dk, dp, count = dst_kv.data_ptr(), dst_pages.data_ptr(), dst_pages.numel()
+    rc = _lib.load().fe_kv_compact(kp, vp, sp, lp, kv.data_ptr(), pages.data_ptr(),
+                                   pages.numel(), last.data_ptr(), dk, dp, count, batch, hkv, dim,
+                                   page, budget, _code("k_pool", k_pool.dtype), slots,
+                                   _kv8_stream(stream, device))
+    if rc:
+        check(rc, "compact_tokens")
+
+
 def create_plan(hq, hkv, dim, page, max_batch, max_pages, bf16, blocks) -> AttentionPlan:
     return AttentionPlan(hq, hkv, dim, page, max_batch, max_pages, bf16, blocks)
 
@@ -691,7 +869,8 @@ class HostKv8Plan(HostPlan):
     _create = "fe_kv8_plan_create_host"
 
 
-__all__ = ["Kv8Pool", "Kv8Plan", "HostKv8Plan", "append_kv8", "gather_kv8", "copy_blocks_kv8",
+__all__ = ["rope_sections", "rope_axes", "rope_axes_append", "select_tokens", "compact_tokens",
+           "Kv8Pool", "Kv8Plan", "HostKv8Plan", "append_kv8", "gather_kv8", "copy_blocks_kv8",
            "store", "copy_blocks", "paged_decode_noalloc", "clear_pages", "gather", "device_errors", "AttentionPlan",
            "create_plan", "destroy_plan", "prepare_plan", "attention", "HostPlan", "FeError",
            "dtype_code", "ITEM_DTYPE", "GROUP_DTYPE", "SEQ_DTYPE", "parse_meta"]

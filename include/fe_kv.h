@@ -134,6 +134,44 @@ int fe_kv_gather(const void* pool, void* out, const int32_t* kv, const int32_t* 
                  int width, int dtype, void* stream);
 
 /* ------------------------------------------------------------------------
+ * Eviction from the paged cache by accumulated attention weight (no reference
+ * counterpart). Scores are fp32 [hkv, cache_slots], one for each cached token
+ * and KV head, as fe_scored_attn_run accumulates them. Both calls take DEVICE
+ * metadata: kv [batch+1], pages [num_pages] (kv[batch] of them are used) and
+ * last [batch] as in fe_attn_plan_prepare. A sequence that reaches past the
+ * page list, or a page past the pool, is skipped (its kept entries are -1) and
+ * raises FE_DEVERR_PAGE_RANGE.
+ *
+ * fe_kv_select: the tokens to keep, int32 kept [batch, hkv, budget], ascending.
+ * Of a sequence of more than `budget` tokens each KV head keeps the first `sink`,
+ * the last `recent`, and of the others those with the highest scores, `budget`
+ * in all; of equal scores (-0 and +0 are equal) the lowest token indexes win,
+ * NaN is below every number. A shorter sequence keeps all of its tokens, and -1
+ * fills the rest. max_len sizes the launch: sequences of up to max_len tokens
+ * (and up to 49152) are read once, longer ones several times. A page that lies
+ * outside the pool counts as NaN.
+ *
+ * fe_kv_compact: for each KV head, the K and V row and (scores not NULL) the
+ * score of token kept[b, h, j] become those of token j of the sequence, for
+ * every j before the first -1. With dst_kv / dst_pages NULL in place: kept[b, h,
+ * j] >= j has to hold (an ascending list's does), and the sequence goes on with
+ * as many tokens as were kept; what its slots past them held is unspecified.
+ * Otherwise the tokens go to the pages dst_pages[dst_kv[b] ..], none of which
+ * may be among the source pages of any sequence of the call: the source keeps
+ * its tokens. A page that is written belongs to one sequence. Entries that break
+ * these bounds are skipped and raise FE_DEVERR_PAGE_RANGE. dim a multiple of 8,
+ * at most 512; pools 16-byte aligned; cache_slots whole pages.
+ * ------------------------------------------------------------------------ */
+int fe_kv_select(const float* scores, const int32_t* kv, const int32_t* pages, int num_pages,
+                 const int32_t* last, int32_t* kept, int batch, int max_len, int hkv, int page,
+                 int budget, int sink, int recent, int64_t cache_slots, void* stream);
+int fe_kv_compact(void* k_pool, void* v_pool, float* scores, const int32_t* kept,
+                  const int32_t* kv, const int32_t* pages, int num_pages, const int32_t* last,
+                  const int32_t* dst_kv, const int32_t* dst_pages, int num_dst_pages, int batch,
+                  int hkv, int dim, int page, int budget, int dtype, int64_t cache_slots,
+                  void* stream);
+
+/* ------------------------------------------------------------------------
  * Rotary embedding. Replaces fe::cuda::rope (include/fe/native_cuda.hpp:13;
  * src/cuda_kernels.cu:19-23 rope_kernel and :33 its launcher), bit-exact:
  * with r = rotary_dim / 2, for each head and pair (j, j + r), j < r, with
@@ -163,6 +201,27 @@ int fe_rope_append(void* q, const void* k, const void* v, void* k_out, void* k_p
                    void* v_pool, const int64_t* slots, const int64_t* pos, const float* cache,
                    int rows, int hq, int hkv, int dim, int rotary_dim, int max_positions,
                    int dtype, int64_t cache_slots, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Rotary embedding with several position axes (no reference counterpart:
+ * its rope has one position a row). As fe_rope and fe_rope_append, but pair j
+ * of a head, (x[j], x[j + rotary_dim/2]), turns by the cache row of its own
+ * axis: pos is int64 [axes, rows], and pair_axis[j] (HOST, rotary_dim/2 bytes,
+ * read by the call) names the axis of pair j, e.g. time, height and width of an
+ * image's patches, in sections or taking turns. Equal positions on all axes
+ * give fe_rope's bits. A row with a position outside [0, max_positions) on any
+ * axis is skipped (rotation and append) and raises FE_DEVERR_POS_RANGE.
+ * axes 1 .. 4, rotary_dim <= 512; else as fe_rope.
+ * ------------------------------------------------------------------------ */
+#define FE_MAX_AXES 4
+int fe_rope_axes(void* q, void* k, const int64_t* pos, int axes, const uint8_t* pair_axis,
+                 const float* cache, int rows, int hq, int hkv, int dim, int rotary_dim,
+                 int max_positions, int dtype, void* stream);
+int fe_rope_axes_append(void* q, const void* k, const void* v, void* k_out, void* k_pool,
+                        void* v_pool, const int64_t* slots, const int64_t* pos, int axes,
+                        const uint8_t* pair_axis, const float* cache, int rows, int hq, int hkv,
+                        int dim, int rotary_dim, int max_positions, int dtype,
+                        int64_t cache_slots, void* stream);
 
 /* ------------------------------------------------------------------------
  * Greedy speculative acceptance. Replaces fe::cuda::accept
