@@ -24,6 +24,7 @@
 #include "fe_attn_common.cuh"
 #include "fe_kv8_attn.h"
 #include "fe_plan_device.h"
+#include "fe_tensor_maps.h"
 
 namespace fe {
 
@@ -80,6 +81,8 @@ int encode_3d(CUtensorMap* map, const void* pool, int dtype, const cuuint64_t di
   return encode_nd(map, pool, dtype, 3, dims, strides, box);
 }
 
+}  // namespace
+
 // tcgen05 row kernel: pool viewed as [cache_slots/8][hkv*dim/64][8][64]
 // (slot groups of 8, 64-dim boxes, slots within the group, 64 elements);
 // box = 2 groups x dim/64 boxes x 8 slots x 64 elements, so one TMA copies a
@@ -128,6 +131,8 @@ int encode_decode_map(CUtensorMap* map, const void* pool, int dtype, int hkv, in
   const cuuint32_t box[3] = {64, kTileTokens, cuuint32_t(heads * (dim / 64))};
   return encode_3d(map, pool, dtype, dims, strides, box);
 }
+
+namespace {
 
 // A head's row of 128 codes is one cache line: fetching the next head's line
 // with it (256-byte promotion) brought lines that were gone again before that

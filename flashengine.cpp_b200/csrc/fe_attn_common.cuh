@@ -29,6 +29,7 @@ struct AttnArgs {
   int hq, G, page, view;
   float scale_log2;
   int q_map_rows;  // query rows the row kernel's Q tensor map covers (0: none)
+  float* sink;     // scored plans: where the decode kernel stores raw scores
 };
 
 __device__ __forceinline__ uint64_t global_ns() {
@@ -151,8 +152,12 @@ struct KeyState {
   }
 
   // One 16-token tile starting at token `tbase` of a sequence of `length` keys.
+  // kSink: the scaled scores (base 2, -inf where masked) are also stored to
+  // sink[key * stride + column], for this state's columns below `cols`.
+  template <bool kSink = false>
   __device__ __forceinline__ void tile(const TileAddr& t, int tbase, int length, float scale_log2,
-                                       int lane) {
+                                       int lane, float* sink = nullptr, int stride = 0,
+                                       int cols = 0) {
     const int r8 = lane >> 2, cq = lane & 3, mi = lane >> 3, li = lane & 7;
     // ---- S^T = K Q^T
     float sc[NT][4];
@@ -178,6 +183,18 @@ struct KeyState {
           if (t0 >= lim[nt][e]) sc[nt][e] = -INFINITY;
           if (t1 >= lim[nt][e]) sc[nt][2 + e] = -INFINITY;
         }
+    }
+    if constexpr (kSink) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const int col = nt * 8 + 2 * cq;
+        if (col < cols) {
+          *reinterpret_cast<float2*>(sink + r8 * stride + col) =
+              make_float2(sc[nt][0] * scale_log2, sc[nt][1] * scale_log2);
+          *reinterpret_cast<float2*>(sink + (r8 + 8) * stride + col) =
+              make_float2(sc[nt][2] * scale_log2, sc[nt][3] * scale_log2);
+        }
+      }
     }
     // ---- online softmax per column; the 8 lanes sharing lane%4 hold a column
     float al[NT][2];

@@ -8,25 +8,10 @@
 #include <utility>
 
 #include "fe_kv.h"
+#include "fe_plan_lists.h"
 
 namespace fe {
 namespace {
-
-struct Unit {
-  int seq, kvh, key_mode, rb0, nrb, tiles, rows;
-};
-
-inline int ceil_div(int64_t a, int64_t b) { return static_cast<int>((a + b - 1) / b); }
-
-inline size_t align16(size_t n) { return (n + 15) & ~size_t(15); }
-
-struct View {
-  std::vector<int32_t> cta_off;
-  std::vector<WorkItem> items;
-  std::vector<SplitGroup> groups;
-  int grid = 0, chunk = 0, decode_items = 0, prefill_items = 0, split_units = 0;
-  int64_t partial_floats = 0;
-};
 
 // Split every unit's key range into balanced chunks and assign the items to
 // CTAs, longest first onto the least-loaded CTA.
@@ -125,6 +110,8 @@ int build_view(const PlanConfig& cfg, const std::vector<Unit>& units, int grid_c
   return FE_OK;
 }
 
+}  // namespace
+
 // Decode lists (and head_dim 256 row lists) cost in proportion to key
 // tiles, so they are balanced exactly: the units' tile ranges are laid end to
 // end and cut into `grid` equal contiguous pieces, one per CTA. A unit cut
@@ -162,7 +149,7 @@ int build_cut_view(const PlanConfig& cfg, const std::vector<Unit>& units, int gr
   // pass 2: emit items CTA by CTA
   std::vector<int> group_of(units.size(), -1), part0_of(units.size(), -1), next_split(units.size(), 0);
   for (size_t i = 0; i < units.size(); ++i) {
-    if (pieces[i] > 1) {
+    if (pieces[i] > 1 || units[i].record) {
       const Unit& u = units[i];
       const int rec = partial_rec_floats(u.rows, cfg.dim);
       group_of[i] = static_cast<int>(v.groups.size());
@@ -176,6 +163,7 @@ int build_cut_view(const PlanConfig& cfg, const std::vector<Unit>& units, int gr
       ++v.split_units;
     }
   }
+  v.unit_group = group_of;
   v.cta_off.clear();
   int64_t room = per;
   int cta = 0;
@@ -234,9 +222,9 @@ int build_cut_view(const PlanConfig& cfg, const std::vector<Unit>& units, int gr
 // step took 314 us where this cut takes a third). The units are laid end to end
 // and cut into at most grid_cap pieces of equal cost, at whole tiles, in pieces
 // of at least kMinPiece tiles.
-constexpr int64_t kMinPiece = 4;
 int build_cost_view(const PlanConfig& cfg, const std::vector<Unit>& units, int grid_cap_in,
                     bool fixed_grid, View& v, std::string& err) {
+  constexpr int64_t kMinPiece = 4;
   v = View{};
   if (units.empty()) return FE_OK;
   const int64_t ov = cfg.row_item_tiles;
@@ -289,7 +277,7 @@ int build_cost_view(const PlanConfig& cfg, const std::vector<Unit>& units, int g
   cut(lo, [&](size_t i, int64_t, int64_t, int64_t) { ++pieces[i]; });
   std::vector<int> group_of(units.size(), -1), part_of(units.size(), -1);
   for (size_t i = 0; i < units.size(); ++i) {
-    if (pieces[i] < 2) continue;
+    if (pieces[i] < 2 && !units[i].record) continue;
     const Unit& u = units[i];
     const int rec = partial_rec_floats(u.rows, cfg.dim);
     group_of[i] = static_cast<int>(v.groups.size());
@@ -299,6 +287,7 @@ int build_cost_view(const PlanConfig& cfg, const std::vector<Unit>& units, int g
     v.partial_floats += int64_t(rec) * pieces[i];
     ++v.split_units;
   }
+  v.unit_group = group_of;
   int64_t last_cta = -1;
   cut(lo, [&](size_t i, int64_t at, int64_t take, int64_t cta) {
     const Unit& u = units[i];
@@ -306,7 +295,7 @@ int build_cost_view(const PlanConfig& cfg, const std::vector<Unit>& units, int g
     WorkItem it;
     it.seq = u.seq;
     it.kvh = static_cast<int16_t>(u.kvh);
-    it.key_mode = 0;
+    it.key_mode = static_cast<int16_t>(u.key_mode);
     it.rb0 = u.rb0;
     it.nrb = u.nrb;
     it.kt0 = static_cast<int32_t>(at * cfg.row_tile);
@@ -336,8 +325,6 @@ int build_cost_view(const PlanConfig& cfg, const std::vector<Unit>& units, int g
   return FE_OK;
 }
 
-}  // namespace
-
 int concurrent_decode_ctas(const PlanConfig& cfg, int sms, double dec_bytes, double row_pieces,
                            double max_row_pieces) {
   if (!cfg.concurrent || sms < 2 || dec_bytes <= 0 || row_pieces <= 0) return 0;
@@ -361,10 +348,10 @@ int concurrent_decode_ctas(const PlanConfig& cfg, int sms, double dec_bytes, dou
   return best_t < 0.92 * serial ? best : 0;
 }
 
-int build_plan(const PlanConfig& cfg, const int32_t* qo, const int32_t* kv, const int32_t* pages,
-               const int32_t* last, int batch, int rows, bool fixed_grid, PlanResult& out,
-               std::string& err) {
-  out = PlanResult{};
+// The step's metadata as sequences, after the checks that every prepare makes.
+int read_step(const PlanConfig& cfg, const int32_t* qo, const int32_t* kv, const int32_t* pages,
+              const int32_t* last, int batch, int rows, std::vector<SeqInfo>& seqs,
+              std::string& err) {
   if (batch < 0 || rows < 0) {
     err = "batch and rows must be non-negative";
     return FE_ERR_INVALID_ARGUMENT;
@@ -386,15 +373,12 @@ int build_plan(const PlanConfig& cfg, const int32_t* qo, const int32_t* kv, cons
     err = "qo[batch] must equal rows";
     return FE_ERR_INVALID_ARGUMENT;
   }
-  const int G = cfg.hq / cfg.hkv;
   const int total_pages = batch > 0 ? kv[batch] : 0;
   if (total_pages > 0 && !pages) {
     err = "pages must be non-null";
     return FE_ERR_INVALID_ARGUMENT;
   }
-  std::vector<SeqInfo> seqs(batch);
-  std::vector<Unit> key_units, row_units_causal, row_units_full;
-  int64_t kv_tokens = 0;
+  seqs.resize(batch);
   for (int b = 0; b < batch; ++b) {
     const int q0 = qo[b], q1 = qo[b + 1];
     const int p0 = kv[b], p1 = kv[b + 1];
@@ -424,6 +408,24 @@ int build_plan(const PlanConfig& cfg, const int32_t* qo, const int32_t* kv, cons
         return FE_ERR_INVALID_ARGUMENT;
       }
     seqs[b] = SeqInfo{q0, qrows, static_cast<int32_t>(length), p0};
+  }
+  return FE_OK;
+}
+
+int build_plan(const PlanConfig& cfg, const int32_t* qo, const int32_t* kv, const int32_t* pages,
+               const int32_t* last, int batch, int rows, bool fixed_grid, PlanResult& out,
+               std::string& err) {
+  out = PlanResult{};
+  std::vector<SeqInfo> seqs;
+  const int bad = read_step(cfg, qo, kv, pages, last, batch, rows, seqs, err);
+  if (bad != FE_OK) return bad;
+  const int G = cfg.hq / cfg.hkv;
+  const int total_pages = batch > 0 ? kv[batch] : 0;
+  std::vector<Unit> key_units, row_units_causal, row_units_full;
+  int64_t kv_tokens = 0;
+  for (int b = 0; b < batch; ++b) {
+    const int qrows = seqs[b].qrows;
+    const int64_t length = seqs[b].length;
     kv_tokens += length;
     if (qrows == 0) continue;
     const int P = qrows * G;

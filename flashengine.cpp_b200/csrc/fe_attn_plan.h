@@ -70,7 +70,8 @@ struct SplitGroup {  // 32 bytes
 struct MetaHeader {  // 128 bytes
   int32_t n_items[3], n_groups[3], grid[3], cta_off_off[3], items_off[3], groups_off[3];
   int32_t batch, rows, seqs_off, pages_off, total_bytes, chunk_tiles, dec_heads;
-  int32_t pad[7];
+  // shared-prefix and scored plans (fe_long_plan.h); 0 in others
+  int32_t sink_off, row_seq_off, merge_off, chunk_off, unit_off[2], n_chunks;
 };
 static_assert(sizeof(MetaHeader) == 128, "MetaHeader layout");
 

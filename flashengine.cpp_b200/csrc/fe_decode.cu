@@ -33,6 +33,9 @@ namespace fe {
 
 int decode_launch(int dtype, int dim, int heads, const CUtensorMap& kmap, const CUtensorMap& vmap,
                   bool per_head_tma, const void* args, int grid, cudaStream_t stream);
+int decode_ext_launch(int dtype, int dim, int heads, const CUtensorMap& kmap,
+                      const CUtensorMap& vmap, bool per_head_tma, const void* args, int grid,
+                      cudaStream_t stream);
 int decode_merge_launch(int dtype, int dim, int list, const void* args, int grid, int grid_rows,
                         cudaStream_t stream, bool pdl);
 
@@ -79,7 +82,20 @@ __device__ __forceinline__ __half to_elem<__half>(float x) {
   return __float2half_rn(x);
 }
 
-template <typename T, int H, int NT, bool kInlineMerge>
+// Where the raw scores of item tile `jt` of head `hh` go (the scored form):
+// [KV head][key tile][16 keys][Pp columns] fp32 per sequence, Pp = the packed
+// rows rounded up to even.
+template <typename T>
+__device__ __forceinline__ float* score_tile(const AttnArgs<T>& a, const WorkItem& wi,
+                                             const SeqInfo& si, int hh, int jt, int cols) {
+  const MetaHeader* hdr = reinterpret_cast<const MetaHeader*>(a.meta);
+  const int64_t* off = reinterpret_cast<const int64_t*>(a.meta + hdr->sink_off);
+  const int tiles = (si.length + kTileTokens - 1) / kTileTokens;
+  return a.sink + off[wi.seq] +
+         (static_cast<int64_t>(wi.kvh + hh) * tiles + wi.kt0 + jt) * (kTileTokens * cols);
+}
+
+template <typename T, int H, int NT, bool kInlineMerge, bool kExt = false>
 __device__ __forceinline__ void decode_item(const AttnArgs<T>& a, const WorkItem& wi,
                                             const SeqInfo& si, const SplitGroup* groups,
                                             uint8_t* stages, uint64_t* full, uint64_t* empty,
@@ -90,7 +106,8 @@ __device__ __forceinline__ void decode_item(const AttnArgs<T>& a, const WorkItem
   const int G = a.G;
   const int P = si.qrows * G;
   const int head0 = (wi.kvh + hh) * G;
-  const bool causal = a.view == 1;
+  // kExt: items of a shared prefix (key_mode 2) are seen whole by every row
+  const bool causal = a.view == 1 && (!kExt || wi.key_mode == 1);
   KeyState<T, NT> ks;
   ks.init(a.q, a.hq, si.q_row0, si.qrows, si.length, head0, G, causal, lane);
 
@@ -106,7 +123,13 @@ __device__ __forceinline__ void decode_item(const AttnArgs<T>& a, const WorkItem
     TileAddr t;
     t.k = base + (2 * hh) * kHalfBytes;
     t.v = t.k + C::kKBytes;
-    ks.tile(t, (wi.kt0 + jt) * kTileTokens, si.length, a.scale_log2, lane);
+    if (kExt && a.sink) {
+      const int cols = (P + 1) & ~1;
+      ks.template tile<true>(t, (wi.kt0 + jt) * kTileTokens, si.length, a.scale_log2, lane,
+                             score_tile(a, wi, si, hh, jt, cols), cols, cols);
+    } else {
+      ks.tile(t, (wi.kt0 + jt) * kTileTokens, si.length, a.scale_log2, lane);
+    }
     __syncwarp();
     if (lane == 0) mbar_arrive_cnt(&empty[s], C::kWh);
   }
@@ -225,7 +248,7 @@ __device__ __forceinline__ void decode_item(const AttnArgs<T>& a, const WorkItem
 // a group take alternate tiles, then fold their states pairwise (round `step`:
 // warps step..2*step-1 of the group stash, warps 0..step-1 absorb), so the
 // group's first warp ends with the item's whole key range.
-template <typename T, int H>
+template <typename T, int H, bool kExt = false>
 __device__ __forceinline__ void decode_item_d256(const AttnArgs<T>& a, const WorkItem& wi,
                                                  const SeqInfo& si, uint8_t* stages,
                                                  uint64_t* full, uint64_t* empty,
@@ -241,7 +264,7 @@ __device__ __forceinline__ void decode_item_d256(const AttnArgs<T>& a, const Wor
   const int grp = w % groups, sub = w / groups;
   const int hh = grp % H, ch = grp / H;
   const int head0 = (wi.kvh + hh) * G;
-  const bool causal = a.view == 1;
+  const bool causal = a.view == 1 && (!kExt || wi.key_mode == 1);
   KeyState<T, 1, D> ks;
   ks.init(a.q, a.hq, si.q_row0, si.qrows, si.length, head0, G, causal, lane, ch * 8);
 
@@ -257,7 +280,13 @@ __device__ __forceinline__ void decode_item_d256(const AttnArgs<T>& a, const Wor
     TileAddr t;
     t.k = base + (C::kQ * hh) * kHalfBytes;
     t.v = t.k + C::kKBytes;
-    ks.tile(t, (wi.kt0 + jt) * kTileTokens, si.length, a.scale_log2, lane);
+    if (kExt && a.sink) {
+      const int cols = (P + 1) & ~1;
+      ks.template tile<true>(t, (wi.kt0 + jt) * kTileTokens, si.length, a.scale_log2, lane,
+                             score_tile(a, wi, si, hh, jt, cols) + ch * 8, cols, cols - ch * 8);
+    } else {
+      ks.tile(t, (wi.kt0 + jt) * kTileTokens, si.length, a.scale_log2, lane);
+    }
     __syncwarp();
     if (lane == 0) mbar_arrive_cnt(&empty[s], kwh);
   }
@@ -303,7 +332,9 @@ __device__ __forceinline__ void decode_item_d256(const AttnArgs<T>& a, const Wor
   }
 }
 
-template <typename T, int H, int D>
+// kExt: the lists of shared-prefix and scored plans (items that every row
+// sees whole, raw scores stored when a.sink is set).
+template <typename T, int H, int D, bool kExt>
 __global__ void __launch_bounds__(kDecThreads, 1)
     paged_decode_kernel(const __grid_constant__ CUtensorMap kmap,
                         const __grid_constant__ CUtensorMap vmap, const AttnArgs<T> a,
@@ -323,14 +354,22 @@ __global__ void __launch_bounds__(kDecThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const MetaHeader* hdr = reinterpret_cast<const MetaHeader*>(a.meta);
   constexpr int kView = 2;  // decode work list
-  if (static_cast<int>(blockIdx.x) >= hdr->grid[kView]) return;
+  // (kExt: a CTA without work waits for the grid before its own too, so that the
+  // kernel after this one finds the records of both)
+  if (static_cast<int>(blockIdx.x) >= hdr->grid[kView]) {
+    if (kExt) pdl_wait();
+    return;
+  }
   const int32_t* cta_off = reinterpret_cast<const int32_t*>(a.meta + hdr->cta_off_off[kView]);
   const WorkItem* items = reinterpret_cast<const WorkItem*>(a.meta + hdr->items_off[kView]);
   const SplitGroup* groups = reinterpret_cast<const SplitGroup*>(a.meta + hdr->groups_off[kView]);
   const SeqInfo* seqs = reinterpret_cast<const SeqInfo*>(a.meta + hdr->seqs_off);
   const int32_t* pages = reinterpret_cast<const int32_t*>(a.meta + hdr->pages_off);
   const int it0 = cta_off[blockIdx.x], it1 = cta_off[blockIdx.x + 1];
-  if (it0 >= it1) return;
+  if (it0 >= it1) {
+    if (kExt) pdl_wait();
+    return;
+  }
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kStages; ++s) {
@@ -426,29 +465,29 @@ __global__ void __launch_bounds__(kDecThreads, 1)
     const WorkItem wi = items[it];
     const SeqInfo si = seqs[wi.seq];
     if constexpr (D != kHeadDim)
-      decode_item_d256<T, H>(a, wi, si, stages, full, empty, flags, comb, warp, lane, g, aborted);
+      decode_item_d256<T, H, kExt>(a, wi, si, stages, full, empty, flags, comb, warp, lane, g, aborted);
     else if (si.qrows * a.G <= 8)
-      decode_item<T, H, 1, false>(a, wi, si, groups, stages, full, empty, flags, comb, warp, lane,
-                                  g, aborted);
+      decode_item<T, H, 1, false, kExt>(a, wi, si, groups, stages, full, empty, flags, comb, warp,
+                                        lane, g, aborted);
     else
-      decode_item<T, H, 2, false>(a, wi, si, groups, stages, full, empty, flags, comb, warp, lane,
-                                  g, aborted);
+      decode_item<T, H, 2, false, kExt>(a, wi, si, groups, stages, full, empty, flags, comb, warp,
+                                        lane, g, aborted);
   }
   if (aborted && lane == 0) raise_device_error(a.err, FE_DEVERR_TIMEOUT);
 }
 
-template <typename T, int H, int D = kHeadDim>
+template <typename T, int H, int D = kHeadDim, bool kExt = false>
 int launch_t(const CUtensorMap& kmap, const CUtensorMap& vmap, bool per_head_tma,
              const AttnArgs<T>& args, int grid, cudaStream_t stream) {
   using C = DecCfg<H, D>;
   static std::once_flag once;
   static cudaError_t attr_err = cudaSuccess;
   std::call_once(once, [] {
-    attr_err = cudaFuncSetAttribute(paged_decode_kernel<T, H, D>,
+    attr_err = cudaFuncSetAttribute(paged_decode_kernel<T, H, D, kExt>,
                                     cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
   });
   if (attr_err != cudaSuccess) return cuda_fail(attr_err, "paged_decode_kernel attribute");
-  FE_CUDA_TRY(launch_pdl(paged_decode_kernel<T, H, D>, dim3(grid), dim3(kDecThreads), C::kSmem,
+  FE_CUDA_TRY(launch_pdl(paged_decode_kernel<T, H, D, kExt>, dim3(grid), dim3(kDecThreads), C::kSmem,
                          stream, kmap, vmap, args, per_head_tma ? 1 : 0));
   return FE_OK;
 }
@@ -646,31 +685,39 @@ int decode_merge_launch(int dtype, int dim, int list, const void* args, int grid
   return launch_merge_t(*static_cast<const AttnArgs<__half>*>(args), dim, list, g, stream, pdl);
 }
 
+namespace {
+
+template <typename T, bool kExt>
+int launch_heads(int dim, int heads, const CUtensorMap& kmap, const CUtensorMap& vmap,
+                 bool per_head_tma, const void* args, int grid, cudaStream_t stream) {
+  const auto& a = *static_cast<const AttnArgs<T>*>(args);
+  if (dim == kWideHeadDim)
+    return heads == 2
+               ? launch_t<T, 2, kWideHeadDim, kExt>(kmap, vmap, per_head_tma, a, grid, stream)
+               : launch_t<T, 1, kWideHeadDim, kExt>(kmap, vmap, per_head_tma, a, grid, stream);
+  switch (heads) {
+    case 8: return launch_t<T, 8, kHeadDim, kExt>(kmap, vmap, per_head_tma, a, grid, stream);
+    case 4: return launch_t<T, 4, kHeadDim, kExt>(kmap, vmap, per_head_tma, a, grid, stream);
+    case 2: return launch_t<T, 2, kHeadDim, kExt>(kmap, vmap, per_head_tma, a, grid, stream);
+    default: return launch_t<T, 1, kHeadDim, kExt>(kmap, vmap, per_head_tma, a, grid, stream);
+  }
+}
+
+}  // namespace
+
 int decode_launch(int dtype, int dim, int heads, const CUtensorMap& kmap, const CUtensorMap& vmap,
                   bool per_head_tma, const void* args, int grid, cudaStream_t stream) {
-  if (dtype == FE_DTYPE_BF16) {
-    const auto& a = *static_cast<const AttnArgs<__nv_bfloat16>*>(args);
-    if (dim == kWideHeadDim)
-      return heads == 2
-                 ? launch_t<__nv_bfloat16, 2, kWideHeadDim>(kmap, vmap, per_head_tma, a, grid, stream)
-                 : launch_t<__nv_bfloat16, 1, kWideHeadDim>(kmap, vmap, per_head_tma, a, grid, stream);
-    switch (heads) {
-      case 8: return launch_t<__nv_bfloat16, 8>(kmap, vmap, per_head_tma, a, grid, stream);
-      case 4: return launch_t<__nv_bfloat16, 4>(kmap, vmap, per_head_tma, a, grid, stream);
-      case 2: return launch_t<__nv_bfloat16, 2>(kmap, vmap, per_head_tma, a, grid, stream);
-      default: return launch_t<__nv_bfloat16, 1>(kmap, vmap, per_head_tma, a, grid, stream);
-    }
-  }
-  const auto& a = *static_cast<const AttnArgs<__half>*>(args);
-  if (dim == kWideHeadDim)
-    return heads == 2 ? launch_t<__half, 2, kWideHeadDim>(kmap, vmap, per_head_tma, a, grid, stream)
-                      : launch_t<__half, 1, kWideHeadDim>(kmap, vmap, per_head_tma, a, grid, stream);
-  switch (heads) {
-    case 8: return launch_t<__half, 8>(kmap, vmap, per_head_tma, a, grid, stream);
-    case 4: return launch_t<__half, 4>(kmap, vmap, per_head_tma, a, grid, stream);
-    case 2: return launch_t<__half, 2>(kmap, vmap, per_head_tma, a, grid, stream);
-    default: return launch_t<__half, 1>(kmap, vmap, per_head_tma, a, grid, stream);
-  }
+  auto run = dtype == FE_DTYPE_BF16 ? launch_heads<__nv_bfloat16, false>
+                                    : launch_heads<__half, false>;
+  return run(dim, heads, kmap, vmap, per_head_tma, args, grid, stream);
+}
+
+int decode_ext_launch(int dtype, int dim, int heads, const CUtensorMap& kmap,
+                      const CUtensorMap& vmap, bool per_head_tma, const void* args, int grid,
+                      cudaStream_t stream) {
+  auto run = dtype == FE_DTYPE_BF16 ? launch_heads<__nv_bfloat16, true>
+                                    : launch_heads<__half, true>;
+  return run(dim, heads, kmap, vmap, per_head_tma, args, grid, stream);
 }
 
 }  // namespace fe

@@ -1,5 +1,5 @@
-// Copy lists for forked sequences (fe_kv_fork_copies, fe_kv.h). Host code
-// only: no device memory is touched, so it runs on a host without a GPU.
+// Copy lists for forked sequences and the prefixes that sequences share
+// (fe_kv_fork_copies, fe_kv_shared_prefixes, fe_kv.h). Host code only: no device memory is touched, so it runs on a host without a GPU.
 //
 // The reference's BlockManager shares only whole published pages between
 // sequences and never writes a published page (src/scheduler.cpp:6-29, the
@@ -79,5 +79,40 @@ extern "C" int fe_kv_fork_copies(int num_forks, const int32_t* parent_tables,
                         " past the fork belongs to the parent");
   }
   *num_copies = n;
+  return FE_OK;
+}
+
+extern "C" int fe_kv_shared_prefixes(const int32_t* kv, const int32_t* pages, int batch,
+                                     int min_pages, int32_t* group_off, int32_t* shared,
+                                     int* num_groups) {
+  using fe::fail;
+  if (num_groups) *num_groups = 0;
+  if (batch < 0 || min_pages < 1 || !num_groups)
+    return fail(FE_ERR_INVALID_ARGUMENT, "fe_kv_shared_prefixes: bad sizes");
+  if (!group_off || (batch > 0 && (!kv || !pages || !shared)))
+    return fail(FE_ERR_INVALID_ARGUMENT, "fe_kv_shared_prefixes: null pointer");
+  group_off[0] = 0;
+  int n = 0;
+  for (int b = 0; b < batch;) {
+    const int32_t* head = pages + kv[b];
+    int64_t common = int64_t(kv[b + 1]) - kv[b];
+    if (common < 0)
+      return fail(FE_ERR_INVALID_ARGUMENT, "fe_kv_shared_prefixes: kv decreases (b=" +
+                                               std::to_string(b) + ")");
+    int end = b + 1;
+    for (; end < batch; ++end) {
+      const int64_t len = int64_t(kv[end + 1]) - kv[end];
+      int64_t same = 0;
+      while (same < common && same < len && head[same] == pages[kv[end] + same]) ++same;
+      // the first neighbour sets what the group shares; one that shares less than
+      // half of it begins a group of its own
+      if (same < min_pages || (end > b + 1 && 2 * same < common)) break;
+      common = same;
+    }
+    shared[n] = end > b + 1 ? static_cast<int32_t>(common) : 0;
+    group_off[++n] = end;
+    b = end;
+  }
+  *num_groups = n;
   return FE_OK;
 }

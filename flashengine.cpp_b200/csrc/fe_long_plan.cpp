@@ -1,0 +1,319 @@
+// Host planners of the shared-prefix and the scored plans (see fe_long_plan.h).
+#include "fe_long_plan.h"
+
+#include <algorithm>
+#include <cstring>
+
+#include "fe_kv.h"
+#include "fe_plan_lists.h"
+
+namespace fe {
+namespace {
+
+constexpr int kRowItem = 128;  // packed rows of a row-kernel item
+
+// Saved key tiles (x KV heads) from which a prefix is shared: by the decode
+// kernel, whose records cost a merge at most, and by the row kernel, which is
+// one more launch.
+constexpr int64_t kShareDecode = 64;
+constexpr int64_t kShareRows = 1024;
+
+struct Tables {
+  std::vector<SeqInfo> seqs;
+  std::vector<MergeSeq> merge;  // one per sequence of the step (or row block)
+  std::vector<int32_t> row_seq;
+  std::vector<ScoreChunk> chunks;
+  std::vector<int64_t> sink;
+};
+
+// views: 0 and 1 the row list without and with the mask, 2 the decode list.
+// Offsets the decode list's records past the row lists' and packs everything.
+int pack(const PlanConfig& cfg, View (&views)[3], const Tables& t, const int32_t* pages,
+         int total_pages, int batch, int rows, LongResult& out, std::string& err) {
+  const int64_t row_floats = std::max(views[0].partial_floats, views[1].partial_floats);
+  out.partial_floats = row_floats + views[2].partial_floats;
+  if (out.partial_floats > cfg.partial_capacity || out.partial_floats > int64_t(INT32_MAX)) {
+    err = "attention work exceeds the plan's split-workspace capacity";
+    return FE_ERR_CAPACITY;
+  }
+  for (auto& it : views[2].items)
+    if (it.group >= 0) it.part += static_cast<int32_t>(row_floats);
+  for (auto& g : views[2].groups) g.part0 += static_cast<int32_t>(row_floats);
+
+  MetaHeader h{};
+  std::vector<uint8_t> meta(align16(sizeof(MetaHeader)));
+  size_t over = 0;
+  auto put = [&](const auto& v) -> int32_t {
+    const size_t at = meta.size(), bytes = sizeof(v[0]) * v.size();
+    if (at + bytes > size_t(INT32_MAX)) over = at + bytes;
+    if (over) return 0;
+    meta.resize(align16(at + bytes));
+    if (bytes) std::memcpy(meta.data() + at, v.data(), bytes);
+    return static_cast<int32_t>(at);
+  };
+  for (int c = 0; c < 3; ++c) {
+    const View& v = views[c];
+    h.n_items[c] = static_cast<int32_t>(v.items.size());
+    h.n_groups[c] = static_cast<int32_t>(v.groups.size());
+    h.grid[c] = out.grid[c] = v.grid;
+    h.cta_off_off[c] = put(v.cta_off);
+    h.items_off[c] = put(v.items);
+    h.groups_off[c] = put(v.groups);
+  }
+  for (int c = 0; c < 2; ++c) {
+    std::vector<int32_t> unit = views[c].unit_group;
+    unit.insert(unit.end(), views[2].unit_group.begin(), views[2].unit_group.end());
+    for (int32_t g : unit) out.merge[c] |= g >= 0;
+    h.unit_off[c] = put(unit);
+  }
+  h.seqs_off = put(t.seqs);
+  h.merge_off = put(t.merge);
+  h.row_seq_off = put(t.row_seq);
+  h.chunk_off = put(t.chunks);
+  h.sink_off = put(t.sink);
+  h.n_chunks = out.n_chunks = static_cast<int32_t>(t.chunks.size());
+  h.pages_off = put(std::vector<int32_t>(pages, pages + total_pages));
+  if (over) {
+    err = "metadata too large";
+    return FE_ERR_CAPACITY;
+  }
+  h.batch = batch;
+  h.rows = out.rows = rows;
+  h.total_bytes = static_cast<int32_t>(meta.size());
+  h.dec_heads = cfg.dec_heads;
+  h.chunk_tiles = static_cast<int32_t>(views[1].unit_group.size());  // here: row units
+  std::memcpy(meta.data(), &h, sizeof(h));
+  out.meta.swap(meta);
+  return FE_OK;
+}
+
+// Which sequence a query row belongs to, in entries of `merge`.
+void fill_rows(Tables& t, int rows) {
+  t.row_seq.assign(rows, 0);
+  for (size_t i = 0; i < t.merge.size(); ++i)
+    for (int r = 0; r < t.merge[i].qrows; ++r)
+      t.row_seq[t.merge[i].q_row0 + r] = static_cast<int32_t>(i);
+}
+
+struct Group {
+  int first, end;  // sequences
+  int pages;       // shared, as far as sharing them pays
+  int rows;        // query rows of the members
+};
+
+// One layout of the step; `share` off leaves every sequence whole.
+int layout(const PlanConfig& cfg, const std::vector<SeqInfo>& step, const std::vector<Group>& gs,
+           const int32_t* pages, int total_pages, int rows, bool share, bool fixed_grid,
+           LongResult& out, std::string& err) {
+  out = LongResult{};
+  const int G = cfg.hq / cfg.hkv, H = cfg.dec_heads, batch = static_cast<int>(step.size());
+  Tables t;
+  t.seqs = step;
+  t.merge.assign(batch, MergeSeq{0, 0, -1, 0, -1, 0, 0, 0});
+  std::vector<Unit> key, full, causal;
+  std::vector<int> key_refs;  // entries of `merge` whose units' numbers lie in the decode list
+  auto add_rows = [&](int seq, int mode, int P, int qrows, int64_t length, bool record) {
+    for (int h = 0; h < cfg.hkv; ++h)
+      for (int p0 = 0; p0 < P; p0 += kRowItem) {
+        const int n = std::min(kRowItem, P - p0);
+        const int64_t limit = mode == 2 ? length : length - qrows + (p0 + n - 1) / G + 1;
+        Unit u{seq, h, mode, p0 / kRowBlock, ceil_div(n, kRowBlock), ceil_div(length, kTileTokens),
+               n, record};
+        full.push_back(u);
+        u.tiles = ceil_div(limit, kTileTokens);
+        causal.push_back(u);
+      }
+  };
+  auto add_key = [&](int seq, int mode, int P, int64_t length, bool record) {
+    for (int h = 0; h < cfg.hkv; h += H)
+      key.push_back(Unit{seq, h, mode, 0, 1, ceil_div(length, kTileTokens), H * P, record});
+  };
+  for (const Group& g : gs) {
+    const int shared = share ? g.pages : 0;
+    const int64_t plen = int64_t(shared) * cfg.page;
+    int pre_unit = -1, pre_blocks = 0;
+    const int PP = g.rows * G;
+    if (shared > 0) {
+      const SeqInfo& s0 = step[g.first];
+      const int at = static_cast<int>(t.seqs.size());
+      t.seqs.push_back(SeqInfo{s0.q_row0, g.rows, static_cast<int32_t>(plen), s0.page_off});
+      ++out.groups_shared;
+      if (PP <= kRowBlock) {
+        pre_unit = static_cast<int>(key.size());
+        add_key(at, 2, PP, plen, true);
+      } else {
+        pre_unit = static_cast<int>(full.size());
+        pre_blocks = ceil_div(PP, kRowItem);
+        add_rows(at, 2, PP, g.rows, plen, true);
+      }
+    }
+    for (int b = g.first; b < g.end; ++b) {
+      SeqInfo& s = t.seqs[b];
+      if (s.qrows == 0) continue;
+      s.length -= static_cast<int32_t>(plen);
+      s.page_off += shared;
+      MergeSeq& m = t.merge[b];
+      const int P = s.qrows * G;
+      m.q_row0 = s.q_row0;
+      m.qrows = s.qrows;
+      m.pre_unit = pre_unit;
+      m.pre_blocks = pre_blocks;
+      m.pre_row0 = (s.q_row0 - step[g.first].q_row0) * G;
+      m.pre_rows = PP;
+      if (P <= kRowBlock) {
+        m.own_unit = static_cast<int>(key.size());
+        add_key(b, 1, P, s.length, shared > 0);
+      } else {
+        m.own_unit = static_cast<int>(full.size());
+        m.own_blocks = ceil_div(P, kRowItem);
+        add_rows(b, 0, P, s.qrows, s.length, shared > 0);
+      }
+    }
+  }
+  const int row_units = static_cast<int>(full.size());
+  for (MergeSeq& m : t.merge) {
+    if (m.own_unit >= 0 && m.own_blocks == 0) m.own_unit += row_units;
+    if (m.pre_unit >= 0 && m.pre_blocks == 0) m.pre_unit += row_units;
+  }
+  View views[3];
+  int rc = build_cost_view(cfg, full, cfg.grid_cap, fixed_grid, views[0], err);
+  if (rc == FE_OK) rc = build_cost_view(cfg, causal, cfg.grid_cap, fixed_grid, views[1], err);
+  if (rc == FE_OK)
+    rc = build_cut_view(cfg, key, cfg.dec_grid_cap, cfg.dec_min_tiles, fixed_grid, views[2], err);
+  if (rc != FE_OK) return rc;
+  fill_rows(t, rows);
+  return pack(cfg, views, t, pages, total_pages, batch, rows, out, err);
+}
+
+}  // namespace
+
+int build_shared_plan(const PlanConfig& cfg, const int32_t* qo, const int32_t* kv,
+                      const int32_t* pages, const int32_t* last, const int32_t* group_off,
+                      const int32_t* shared, int groups, int batch, int rows, bool fixed_grid,
+                      LongResult& out, std::string& err) {
+  std::vector<SeqInfo> step;
+  int rc = read_step(cfg, qo, kv, pages, last, batch, rows, step, err);
+  if (rc != FE_OK) return rc;
+  if (int64_t(rows) * cfg.hq > INT32_MAX / 2) {
+    err = "too many query rows";
+    return FE_ERR_CAPACITY;
+  }
+  if (groups < 0 || (groups > 0 && (!group_off || !shared))) {
+    err = "groups need group_off and shared";
+    return FE_ERR_INVALID_ARGUMENT;
+  }
+  std::vector<Group> gs;
+  if (groups == 0) {
+    for (int b = 0; b < batch; ++b) gs.push_back(Group{b, b + 1, 0, step[b].qrows});
+  } else if (group_off[0] != 0 || group_off[groups] != batch) {
+    err = "group_off must run from 0 to the batch";
+    return FE_ERR_INVALID_ARGUMENT;
+  }
+  const int G = cfg.hq / cfg.hkv;
+  int64_t saved_total = 0;
+  for (int g = 0; g < groups; ++g) {
+    const int first = group_off[g], end = group_off[g + 1];
+    if (end < first || end > batch || shared[g] < 0) {
+      err = "group_off must be non-decreasing and shared non-negative (g=" + std::to_string(g) +
+            ")";
+      return FE_ERR_INVALID_ARGUMENT;
+    }
+    Group x{first, end, shared[g], 0};
+    int64_t blocks = 0;  // items that read the prefix when it is not shared
+    int members = 0;
+    for (int b = first; b < end; ++b) {
+      if (shared[g] > kv[b + 1] - kv[b] ||
+          std::memcmp(pages + kv[first], pages + kv[b], sizeof(int32_t) * size_t(shared[g]))) {
+        err = "sequence does not begin with its group's shared pages (b=" + std::to_string(b) + ")";
+        return FE_ERR_INVALID_ARGUMENT;
+      }
+      const SeqInfo& s = step[b];
+      x.rows += s.qrows;
+      if (s.qrows == 0) continue;
+      // a causal row sees the whole prefix: the query rows' own keys (one at
+      // least) stay out
+      x.pages = std::min(x.pages, (s.length - s.qrows) / cfg.page);
+      ++members;
+      blocks += ceil_div(int64_t(s.qrows) * G, kRowItem);
+    }
+    const int64_t PP = int64_t(x.rows) * G;
+    const int64_t saved = (blocks - ceil_div(PP, kRowItem)) * x.pages *
+                          (cfg.page / kTileTokens) * cfg.hkv;
+    if (members < 2 || saved < (PP <= kRowBlock ? kShareDecode : kShareRows))
+      x.pages = 0;
+    else
+      saved_total += saved;
+    gs.push_back(x);
+  }
+  const int total_pages = batch > 0 ? kv[batch] : 0;
+  rc = layout(cfg, step, gs, pages, total_pages, rows, true, fixed_grid, out, err);
+  // where the records of the shared parts do not fit, every sequence stays whole
+  if (rc == FE_ERR_CAPACITY && saved_total > 0) {
+    saved_total = 0;
+    rc = layout(cfg, step, gs, pages, total_pages, rows, false, fixed_grid, out, err);
+  }
+  out.shared_tiles = saved_total;
+  return rc;
+}
+
+int build_scored_plan(const PlanConfig& cfg, const int32_t* qo, const int32_t* kv,
+                      const int32_t* pages, const int32_t* last, const int32_t* fresh, int batch,
+                      int rows, bool fixed_grid, int64_t sink_capacity, LongResult& out,
+                      std::string& err) {
+  out = LongResult{};
+  std::vector<SeqInfo> step;
+  int rc = read_step(cfg, qo, kv, pages, last, batch, rows, step, err);
+  if (rc != FE_OK) return rc;
+  if (int64_t(rows) * cfg.hq > INT32_MAX / 2) {
+    err = "too many query rows";
+    return FE_ERR_CAPACITY;
+  }
+  const int G = cfg.hq / cfg.hkv, H = cfg.dec_heads;
+  const int per = kRowBlock / G;  // query rows of a block
+  Tables t;
+  std::vector<Unit> key;
+  std::vector<uint8_t> used(size_t(cfg.num_blocks) + 1, 0);
+  for (int b = 0; b < batch; ++b) {
+    const SeqInfo& s = step[b];
+    if (s.qrows == 0) continue;
+    for (int i = kv[b]; i < kv[b + 1]; ++i) {
+      if (used[pages[i]]++) {
+        err = "page " + std::to_string(pages[i]) +
+              " is listed twice: its scores would be added to by two CTAs";
+        return FE_ERR_INVALID_ARGUMENT;
+      }
+    }
+    const int f = fresh ? fresh[b] : s.qrows;
+    if (f < 0 || f > s.length) {
+      err = "fresh[b] must be in [0, length] (b=" + std::to_string(b) + ")";
+      return FE_ERR_INVALID_ARGUMENT;
+    }
+    const int block0 = static_cast<int>(t.seqs.size());
+    for (int i = 0; i < s.qrows; i += per) {
+      const int n = std::min(per, s.qrows - i), P = n * G;
+      // up to the last key that the block's last row sees
+      const int length = s.length - s.qrows + i + n;
+      const int tiles = ceil_div(length, kTileTokens);
+      t.merge.push_back(MergeSeq{s.q_row0 + i, n, static_cast<int>(key.size()), 0, -1, 0, 0, 0});
+      t.seqs.push_back(SeqInfo{s.q_row0 + i, n, length, s.page_off});
+      t.sink.push_back(out.sink_floats);
+      out.sink_floats += int64_t(cfg.hkv) * tiles * kTileTokens * ((P + 1) & ~1);
+      for (int h = 0; h < cfg.hkv; h += H)
+        key.push_back(Unit{static_cast<int>(t.seqs.size()) - 1, h, 1, 0, 1, tiles, H * P, true});
+    }
+    const int blocks = static_cast<int>(t.seqs.size()) - block0;
+    for (int t0 = 0; t0 < s.length; t0 += kScoreChunk)
+      t.chunks.push_back(ScoreChunk{block0, blocks, s.length, s.page_off, s.length - f, t0, {0, 0}});
+  }
+  if (out.sink_floats > sink_capacity) {
+    err = "query rows x keys exceed the plan's max_keys";
+    return FE_ERR_CAPACITY;
+  }
+  View views[3];
+  rc = build_cut_view(cfg, key, cfg.dec_grid_cap, cfg.dec_min_tiles, fixed_grid, views[2], err);
+  if (rc != FE_OK) return rc;
+  fill_rows(t, rows);
+  return pack(cfg, views, t, pages, batch > 0 ? kv[batch] : 0, batch, rows, out, err);
+}
+
+}  // namespace fe

@@ -1,0 +1,71 @@
+// Host planners of the shared-prefix and the scored plans: work lists for the
+// decode and row kernels (fe_attn_plan.h) whose items write partial records,
+// and the tables by which the kernels of fe_long_attn.cu join them. Pure C++.
+//
+// Shared-prefix plans: the sequences of a group begin with the same pages. The
+// group's prefix becomes one more sequence of the lists, with the query rows of
+// all its members and a mask that hides nothing (key_mode 2); each member keeps
+// its own keys, those after the prefix. A query row's result is the joined
+// softmax of its records from both.
+//
+// Scored plans: the query rows of a sequence are cut into blocks of at most 16
+// packed rows, each a sequence of the decode list, whose raw scores the decode
+// kernel stores beside the records.
+#pragma once
+
+#include <stdint.h>
+
+#include <string>
+#include <vector>
+
+#include "fe_attn_plan.h"
+
+namespace fe {
+
+// Where the records of a sequence's query rows lie. Units are numbered through
+// both lists, row units first; unit_off maps them to split groups (-1: the unit
+// writes its output itself).
+struct MergeSeq {  // 32 bytes
+  int32_t q_row0, qrows;
+  int32_t own_unit;    // first unit of its own keys, -1: no query rows
+  int32_t own_blocks;  // 128-row blocks a KV head; 0: units of the decode list
+  int32_t pre_unit;    // the same of its prefix, -1: none
+  int32_t pre_blocks;
+  int32_t pre_row0;    // its first packed row among the prefix's
+  int32_t pre_rows;    // packed rows of the prefix (a KV head)
+};
+
+// A stretch of keys whose scores one CTA and KV head update.
+struct ScoreChunk {  // 32 bytes
+  int32_t block0, blocks;  // the sequence's row blocks (sequences of the lists)
+  int32_t length, page_off;
+  int32_t fresh;  // first key whose score is set and not added to
+  int32_t t0;
+  int32_t pad[2];
+};
+constexpr int kScoreChunk = 512;  // keys
+
+struct LongResult {
+  std::vector<uint8_t> meta;
+  int grid[3] = {0, 0, 0};
+  bool merge[2] = {false, false};  // by mask: some unit writes records
+  int rows = 0, groups_shared = 0, n_chunks = 0;
+  int64_t shared_tiles = 0;   // key tiles that the sharing saves
+  int64_t partial_floats = 0, sink_floats = 0;
+};
+
+// group_off [groups + 1]: runs of consecutive sequences, all of them;
+// shared [groups]: pages that the members of each have in common at the start.
+int build_shared_plan(const PlanConfig& cfg, const int32_t* qo, const int32_t* kv,
+                      const int32_t* pages, const int32_t* last, const int32_t* group_off,
+                      const int32_t* shared, int groups, int batch, int rows, bool fixed_grid,
+                      LongResult& out, std::string& err);
+
+// fresh [batch]: keys at each sequence's end whose score is set (null: the
+// query rows). sink_capacity: floats of raw scores.
+int build_scored_plan(const PlanConfig& cfg, const int32_t* qo, const int32_t* kv,
+                      const int32_t* pages, const int32_t* last, const int32_t* fresh, int batch,
+                      int rows, bool fixed_grid, int64_t sink_capacity, LongResult& out,
+                      std::string& err);
+
+}  // namespace fe

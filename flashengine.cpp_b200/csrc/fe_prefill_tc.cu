@@ -58,6 +58,9 @@ namespace fe {
 
 int prefill_tc_launch(int dtype, int dim, const CUtensorMap& kmap, const CUtensorMap& vmap,
                       const CUtensorMap& qmap, const void* args, int grid, cudaStream_t stream);
+int prefill_tc_ext_launch(int dtype, int dim, const CUtensorMap& kmap, const CUtensorMap& vmap,
+                          const CUtensorMap& qmap, const void* args, int grid,
+                          cudaStream_t stream);
 
 namespace {
 
@@ -159,7 +162,9 @@ __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, volati
   return !aborted;
 }
 
-template <typename T, int D>
+// kExt: the lists of shared-prefix plans (items that every row sees whole,
+// split at any head_dim).
+template <typename T, int D, bool kExt>
 __global__ void __launch_bounds__(kTcThreads, 1)
     paged_prefill_tc_kernel(const __grid_constant__ CUtensorMap kmap,
                             const __grid_constant__ CUtensorMap vmap,
@@ -169,7 +174,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   constexpr int kPiecesPerTile = C::kPiecesPerTile;
   constexpr int kSlots = kSlotsTc, kKStages = C::kKStages, kVStages = C::kVStages;
   constexpr uint32_t kOCol = C::kOCol;
-  constexpr bool kSplits = D != kHeadDim;  // the planner splits head_dim 256 row items only
+  // the planner splits row items of head_dim 256 and of shared-prefix plans only
+  constexpr bool kSplits = D != kHeadDim || kExt;
   // declared 16-byte aligned so that the 1 KiB check below is not folded away
   extern __shared__ __align__(16) uint8_t smem[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
@@ -199,13 +205,20 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const MetaHeader* hdr = reinterpret_cast<const MetaHeader*>(a.meta);
   const int view = a.view;
-  if (static_cast<int>(blockIdx.x) >= hdr->grid[view]) return;
+  // (kExt: a CTA without work waits for the grid before its own too)
+  if (static_cast<int>(blockIdx.x) >= hdr->grid[view]) {
+    if (kExt) pdl_wait();
+    return;
+  }
   const int32_t* cta_off = reinterpret_cast<const int32_t*>(a.meta + hdr->cta_off_off[view]);
   const WorkItem* items = reinterpret_cast<const WorkItem*>(a.meta + hdr->items_off[view]);
   const SeqInfo* seqs = reinterpret_cast<const SeqInfo*>(a.meta + hdr->seqs_off);
   const int32_t* pages = reinterpret_cast<const int32_t*>(a.meta + hdr->pages_off);
   const int it0 = cta_off[blockIdx.x], it1 = cta_off[blockIdx.x + 1];
-  if (it0 >= it1) return;
+  if (it0 >= it1) {
+    if (kExt) pdl_wait();
+    return;
+  }
   if (smem_u32(smem) & 1023u) {
     if (threadIdx.x == 0) raise_device_error(a.err, FE_DEVERR_SMEM_ALIGN);
     return;
@@ -492,7 +505,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       // keys this row sees in this item: the mask's, cut at the end of the
       // item's pieces (a split item covers part of the range; head_dim 128
       // items are never split)
-      int lim = (causal && row_valid) ? si.length - si.qrows + p / G + 1 : si.length;
+      int lim = (causal && row_valid && (!kExt || w.key_mode == 0)) ? si.length - si.qrows + p / G + 1 : si.length;
       if constexpr (kSplits) lim = min(lim, w.kt1 * kTileTokens);
       // m_used stays -inf until the first unmasked key (its weights are 0)
       float m_used = -INFINITY, l = 0.f;
@@ -696,36 +709,42 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   }
 }
 
-template <typename T, int D>
+template <typename T, int D, bool kExt>
 int launch_t(const CUtensorMap& kmap, const CUtensorMap& vmap, const CUtensorMap& qmap,
              const AttnArgs<T>& args, int grid, cudaStream_t stream) {
   static std::once_flag once;
   static cudaError_t attr_err = cudaSuccess;
   std::call_once(once, [] {
-    attr_err = cudaFuncSetAttribute(paged_prefill_tc_kernel<T, D>,
+    attr_err = cudaFuncSetAttribute(paged_prefill_tc_kernel<T, D, kExt>,
                                     cudaFuncAttributeMaxDynamicSharedMemorySize, TcCfg<D>::kSmem);
   });
   if (attr_err != cudaSuccess) return cuda_fail(attr_err, "paged_prefill_tc_kernel attribute");
-  FE_CUDA_TRY(launch_pdl(paged_prefill_tc_kernel<T, D>, dim3(grid), dim3(kTcThreads),
+  FE_CUDA_TRY(launch_pdl(paged_prefill_tc_kernel<T, D, kExt>, dim3(grid), dim3(kTcThreads),
                          TcCfg<D>::kSmem, stream, kmap, vmap, qmap, args));
   return FE_OK;
 }
 
-template <typename T>
+template <typename T, bool kExt>
 int launch_dim(int dim, const CUtensorMap& kmap, const CUtensorMap& vmap, const CUtensorMap& qmap,
                const void* args, int grid, cudaStream_t stream) {
   const auto& a = *static_cast<const AttnArgs<T>*>(args);
-  if (dim == kWideHeadDim) return launch_t<T, kWideHeadDim>(kmap, vmap, qmap, a, grid, stream);
-  return launch_t<T, kHeadDim>(kmap, vmap, qmap, a, grid, stream);
+  if (dim == kWideHeadDim) return launch_t<T, kWideHeadDim, kExt>(kmap, vmap, qmap, a, grid, stream);
+  return launch_t<T, kHeadDim, kExt>(kmap, vmap, qmap, a, grid, stream);
 }
 
 }  // namespace
 
 int prefill_tc_launch(int dtype, int dim, const CUtensorMap& kmap, const CUtensorMap& vmap,
                       const CUtensorMap& qmap, const void* args, int grid, cudaStream_t stream) {
-  if (dtype == FE_DTYPE_BF16)
-    return launch_dim<__nv_bfloat16>(dim, kmap, vmap, qmap, args, grid, stream);
-  return launch_dim<__half>(dim, kmap, vmap, qmap, args, grid, stream);
+  auto run = dtype == FE_DTYPE_BF16 ? launch_dim<__nv_bfloat16, false> : launch_dim<__half, false>;
+  return run(dim, kmap, vmap, qmap, args, grid, stream);
+}
+
+int prefill_tc_ext_launch(int dtype, int dim, const CUtensorMap& kmap, const CUtensorMap& vmap,
+                          const CUtensorMap& qmap, const void* args, int grid,
+                          cudaStream_t stream) {
+  auto run = dtype == FE_DTYPE_BF16 ? launch_dim<__nv_bfloat16, true> : launch_dim<__half, true>;
+  return run(dim, kmap, vmap, qmap, args, grid, stream);
 }
 
 }  // namespace fe

@@ -81,6 +81,17 @@ SIGNATURES = {
     "fe_accept": (_I, [_P, _P, _P, _I, _I, _P]),
     "fe_rope_axes": (_I, [_P, _P, _P, _I, _P, _P] + [_I] * 7 + [_P]),
     "fe_rope_axes_append": (_I, [_P] * 8 + [_I, _P, _P] + [_I] * 7 + [_I64, _P]),
+    "fe_long_plan_destroy": (_I, [_P]),
+    "fe_long_plan_create_host": (_I, [_I] * 9 + [_I64, _I, ctypes.POINTER(_P)]),
+    "fe_long_plan_debug_meta": (_I, [_P, _P, _I64, ctypes.POINTER(_I64)]),
+    "fe_long_plan_get_info": (_I, [_P, _P]),
+    "fe_shared_plan_create": (_I, [_I] * 8 + [ctypes.POINTER(_P)]),
+    "fe_shared_plan_prepare": (_I, [_P] * 7 + [_I] * 4 + [_P]),
+    "fe_shared_attn_run": (_I, [_P] * 5 + [_I, _P]),
+    "fe_kv_shared_prefixes": (_I, [_P, _P, _I, _I, _P, _P, ctypes.POINTER(_I)]),
+    "fe_scored_plan_create": (_I, [_I] * 8 + [_I64, ctypes.POINTER(_P)]),
+    "fe_scored_plan_prepare": (_I, [_P] * 6 + [_I] * 3 + [_P]),
+    "fe_scored_attn_run": (_I, [_P] * 7),
     "fe_kv_select": (_I, [_P] * 3 + [_I] + [_P] * 2 + [_I] * 7 + [_I64, _P]),
     "fe_kv_compact": (_I, [_P] * 6 + [_I] + [_P] * 3 + [_I] * 7 + [_I64, _P]),
 }
@@ -98,6 +109,11 @@ class PlanInfo(ctypes.Structure):
     _fields_ = [("batch", _I), ("rows", _I), ("decode_items", _I), ("prefill_items", _I),
                 ("split_sequences", _I), ("chunk_tiles", _I), ("grid_ctas", _I),
                 ("kv_tokens", _I64)]
+
+
+class LongPlanInfo(ctypes.Structure):
+    _fields_ = [("rows", _I), ("shared_groups", _I), ("row_ctas", _I), ("decode_ctas", _I),
+                ("shared_tiles", _I64), ("partial_floats", _I64), ("weight_floats", _I64)]
 
 
 _lib = None

@@ -576,8 +576,9 @@ class Kv8Plan(AttentionPlan):
 
 
 # ---------------------------------------------------------------------------
-# Long shared prompts: rotary positions with several axes, and eviction by
-# accumulated attention weight (no reference counterpart). Checks as for the
+# Long shared prompts: rotary positions with several axes, attention over
+# shared prefixes and with scores of the keys, and eviction by those scores (no
+# reference counterpart). Checks as for the
 # 8-bit calls: each tensor attribute is read once.
 # ---------------------------------------------------------------------------
 
@@ -753,6 +754,167 @@ def compact_tokens(k_pool, v_pool, scores, kept, kv, pages, last, page, dst_kv=N
         check(rc, "compact_tokens")
 
 
+def shared_prefixes(kv, pages, min_pages=1):
+    """The groups of a batch whose sequences begin with the same pages (host
+    only): group_off (the first sequence of each group, then the batch) and
+    shared (pages in common), for SharedPlan.prepare."""
+    kv, pages = _host_i32(kv), _host_i32(pages)
+    batch = kv.shape[0] - 1
+    if batch < 0 or (batch and pages.shape[0] < kv[batch]):
+        raise ValueError(f"{pages.shape[0]} pages, kv counts {kv[-1] if batch >= 0 else 0}")
+    off, shared = np.zeros(batch + 1, np.int32), np.zeros(max(batch, 1), np.int32)
+    n = ctypes.c_int(0)
+    check(_lib.load().fe_kv_shared_prefixes(kv.ctypes.data, pages.ctypes.data, batch,
+                                            int(min_pages), off.ctypes.data, shared.ctypes.data,
+                                            ctypes.byref(n)), "shared_prefixes")
+    return off[:n.value + 1].copy(), shared[:n.value].copy()
+
+
+class _LongPlan:
+    """What SharedPlan and ScoredPlan have in common: the handle, its shapes,
+    and the checks of a run."""
+
+    def _own(self, handle, hq, hkv, dim, page, bf16, blocks):
+        torch = _torch()
+        self.handle = handle
+        self.hq, self.hkv, self.dim, self.page = int(hq), int(hkv), int(dim), int(page)
+        self.slots = (int(blocks) + 1) * self.page
+        self.dtype = torch.bfloat16 if bf16 else torch.float16
+        self.rows = 0  # query rows of the last prepare
+        self.index = _kv8_device()
+
+    def _device(self):
+        device = _kv8_device()
+        if self.index != device:
+            raise ValueError(f"the plan is for cuda:{self.index}, the current device is "
+                             f"cuda:{device}")
+        return device
+
+    def _step(self, qo, kv, pages, last, batch, rows):
+        qo, kv, pages, last = _host_i32(qo), _host_i32(kv), _host_i32(pages), _host_i32(last)
+        batch = kv.shape[0] - 1 if batch is None else int(batch)
+        _kv8_metadata(qo, kv, last, batch)
+        if pages.shape[0] < kv[batch]:
+            raise ValueError(f"{pages.shape[0]} pages, kv counts {kv[batch]}")
+        return qo, kv, pages, last, batch, int(qo[batch]) if rows is None else int(rows)
+
+    def _buffers(self, q, k, v, out, device):
+        """Addresses of q and out [rows, hq, dim] and of the pools."""
+        if q.dim() != 3 or q.shape[0] < self.rows:
+            raise ValueError(f"q {tuple(q.shape)}: the plan was prepared for {self.rows} rows")
+        shape = (q.shape[0], self.hq, self.dim)
+        width = self.hkv * self.dim
+        kp, ks = _pool16("k", k, self.dtype, width, device)
+        vp, vs = _pool16("v", v, self.dtype, width, device)
+        if ks != self.slots or vs != self.slots:
+            raise ValueError(f"pools of {ks} and {vs} slots: the plan is for {self.slots}")
+        return (_kv8_rows("q", q, self.dtype, shape, device), kp, vp,
+                _kv8_rows("out", out, self.dtype, shape, device))
+
+    def info(self) -> dict:
+        inf = _lib.LongPlanInfo()
+        check(self.lib.fe_long_plan_get_info(self.handle, ctypes.byref(inf)), "plan_info")
+        return {name: getattr(inf, name) for name, _ in _lib.LongPlanInfo._fields_}
+
+    def close(self):
+        if getattr(self, "handle", None):
+            self.lib.fe_long_plan_destroy(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class SharedPlan(_LongPlan):
+    """Attention for sequences that begin with the same pages: as an
+    AttentionPlan's over the full page lists, with the keys and values of a
+    shared prefix read once for the whole group."""
+
+    def __init__(self, hq, hkv, dim, page, max_batch, max_pages, bf16, blocks):
+        self.lib = _lib.load()
+        h = _P()
+        check(self.lib.fe_shared_plan_create(int(hq), int(hkv), int(dim), int(page),
+                                             int(max_batch), int(max_pages),
+                                             FE_DTYPE_BF16 if bf16 else FE_DTYPE_F16, int(blocks),
+                                             ctypes.byref(h)), "create_shared_plan")
+        self._own(h, hq, hkv, dim, page, bf16, blocks)
+
+    def prepare(self, qo, kv, pages, last, groups=None, batch=None, rows=None, graph=False,
+                stream=None):
+        """Host metadata as AttentionPlan.prepare (full page lists). groups:
+        (group_off, shared) as shared_prefixes() gives, which is asked when it
+        is None."""
+        device = self._device()
+        qo, kv, pages, last, batch, rows = self._step(qo, kv, pages, last, batch, rows)
+        off, shared = shared_prefixes(kv[:batch + 1], pages) if groups is None else groups
+        off, shared = _host_i32(off), _host_i32(shared)
+        if off.shape != (shared.shape[0] + 1,):
+            raise ValueError("group_off must have one entry more than shared")
+        check(self.lib.fe_shared_plan_prepare(self.handle, qo.ctypes.data, kv.ctypes.data,
+                                              pages.ctypes.data, last.ctypes.data,
+                                              off.ctypes.data, shared.ctypes.data,
+                                              shared.shape[0], batch, rows, int(bool(graph)),
+                                              _kv8_stream(stream, device)), "prepare_plan")
+        self.rows = rows
+
+    def attention(self, q, k, v, out, causal=True, stream=None):
+        """q, out [rows, hq, dim]; k, v: pools [cache_slots, hkv, dim]."""
+        device = self._device()
+        qp, kp, vp, op = self._buffers(q, k, v, out, device)
+        rc = self.lib.fe_shared_attn_run(self.handle, qp, kp, vp, op, 1 if causal else 0,
+                                         _kv8_stream(stream, device))
+        if rc:
+            check(rc, "attention")
+
+
+class ScoredPlan(_LongPlan):
+    """Causal attention that adds each cached key's softmax weights to its
+    score, fp32 [hkv, cache_slots]. max_keys: the most query rows x keys of a
+    step (each sequence's keys rounded up to 16), summed over the sequences."""
+
+    def __init__(self, hq, hkv, dim, page, max_batch, max_pages, bf16, blocks, max_keys):
+        self.lib = _lib.load()
+        h = _P()
+        check(self.lib.fe_scored_plan_create(int(hq), int(hkv), int(dim), int(page),
+                                             int(max_batch), int(max_pages),
+                                             FE_DTYPE_BF16 if bf16 else FE_DTYPE_F16, int(blocks),
+                                             int(max_keys), ctypes.byref(h)), "create_scored_plan")
+        self._own(h, hq, hkv, dim, page, bf16, blocks)
+
+    def prepare(self, qo, kv, pages, last, fresh=None, batch=None, rows=None, graph=False,
+                stream=None):
+        """Host metadata as AttentionPlan.prepare. fresh [batch]: the keys at
+        each sequence's end whose score is set and not added to (None: as many
+        as it has query rows)."""
+        device = self._device()
+        qo, kv, pages, last, batch, rows = self._step(qo, kv, pages, last, batch, rows)
+        fp = None
+        if fresh is not None:
+            fresh = _host_i32(fresh)
+            if fresh.shape[0] < batch:
+                raise ValueError(f"{batch} sequences, {fresh.shape[0]} entries of fresh")
+            fp = fresh.ctypes.data
+        check(self.lib.fe_scored_plan_prepare(self.handle, qo.ctypes.data, kv.ctypes.data,
+                                              pages.ctypes.data, last.ctypes.data, fp, batch,
+                                              rows, int(bool(graph)),
+                                              _kv8_stream(stream, device)), "prepare_plan")
+        self.rows = rows
+
+    def attention(self, q, k, v, scores, out, stream=None):
+        """q, out [rows, hq, dim]; k, v: pools [cache_slots, hkv, dim]; scores:
+        fp32 [hkv, cache_slots], updated in place."""
+        device = self._device()
+        qp, kp, vp, op = self._buffers(q, k, v, out, device)
+        sp = _kv8_rows("scores", scores, _torch().float32, (self.hkv, self.slots), device)
+        rc = self.lib.fe_scored_attn_run(self.handle, qp, kp, vp, sp, op,
+                                         _kv8_stream(stream, device))
+        if rc:
+            check(rc, "attention")
+
+
 def create_plan(hq, hkv, dim, page, max_batch, max_pages, bf16, blocks) -> AttentionPlan:
     return AttentionPlan(hq, hkv, dim, page, max_batch, max_pages, bf16, blocks)
 
@@ -869,7 +1031,7 @@ class HostKv8Plan(HostPlan):
     _create = "fe_kv8_plan_create_host"
 
 
-__all__ = ["rope_sections", "rope_axes", "rope_axes_append", "select_tokens", "compact_tokens",
+__all__ = ["SharedPlan", "ScoredPlan", "shared_prefixes", "rope_sections", "rope_axes", "rope_axes_append", "select_tokens", "compact_tokens",
            "Kv8Pool", "Kv8Plan", "HostKv8Plan", "append_kv8", "gather_kv8", "copy_blocks_kv8",
            "store", "copy_blocks", "paged_decode_noalloc", "clear_pages", "gather", "device_errors", "AttentionPlan",
            "create_plan", "destroy_plan", "prepare_plan", "attention", "HostPlan", "FeError",

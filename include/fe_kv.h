@@ -434,6 +434,74 @@ int fe_kv8_attn_run(fe_attn_plan* plan, const void* q, const uint8_t* k_codes,
                     int causal, void* stream);
 
 /* ------------------------------------------------------------------------
+ * Attention for long shared prompts (no reference counterpart: the reference
+ * reads every sequence's pages by itself, src/flashinfer_attention.cu:35-44).
+ * Two kinds of plans over the 16-bit pools, of one handle type; head_dim, heads,
+ * pages and capacities as for fe_attn_plan_create, metadata (HOST) and `graph` as
+ * for fe_attn_plan_prepare. Prepare uploads to fixed buffers with one async copy
+ * on `stream`: a graph that captured a run replays for later prepares of the same
+ * batch and rows. A plan has one workspace (256 MiB of partial records): its runs
+ * must not overlap on the GPU. Scale 1/sqrt(dim), fp32 softmax and accumulation,
+ * softmax weights of about 16 bits in the second product, output rounded to
+ * nearest even, as fe_attn_run.
+ * ------------------------------------------------------------------------ */
+typedef struct fe_long_plan fe_long_plan;
+int fe_long_plan_destroy(fe_long_plan* plan);
+
+/* Shared prefixes. Sequences group_off[g] .. group_off[g+1]-1 (HOST, runs of
+ * consecutive sequences that cover the batch) begin with the same shared[g]
+ * pages: prepare checks that they do (FE_ERR_INVALID_ARGUMENT). The result is
+ * fe_attn_run's over the full lists (causal as there); K and V of the prefix
+ * are read once for the rows of the whole group. groups = 0: nothing is
+ * shared. A prefix is taken as far as it is whole pages before every member's
+ * query rows, and not at all where sharing it saves too little (a single
+ * member, a short prefix, members whose query rows fill the row kernel's tiles by
+ * themselves). */
+int fe_shared_plan_create(int hq, int hkv, int dim, int page, int max_batch, int max_pages,
+                          int dtype, int num_blocks, fe_long_plan** plan_out);
+int fe_shared_plan_prepare(fe_long_plan* plan, const int32_t* qo, const int32_t* kv,
+                           const int32_t* pages, const int32_t* last, const int32_t* group_off,
+                           const int32_t* shared, int groups, int batch, int rows, int graph,
+                           void* stream);
+int fe_shared_attn_run(fe_long_plan* plan, const void* q, const void* k_pool, const void* v_pool,
+                       void* out, int causal, void* stream);
+/* The groups of a batch from its page lists (HOST memory only, needs no GPU):
+ * neighbours whose first min_pages pages or more are the same, as long as the
+ * group goes on sharing half of what its first two members do. group_off
+ * [batch+1] and shared [batch] receive the *num_groups groups. */
+int fe_kv_shared_prefixes(const int32_t* kv, const int32_t* pages, int batch, int min_pages,
+                          int32_t* group_off, int32_t* shared, int* num_groups);
+
+/* Scored attention: causal attention as fe_attn_run's, and for every key t that
+ * a sequence's query rows see, scores[h, slot(t)] (fp32 [hkv, cache_slots], on
+ * the device) grows by the softmax weights that KV head h's query heads gave it,
+ * summed in fp32 in a fixed order. The last fresh[b] keys of sequence b (HOST,
+ * NULL: as many as it has query rows, those that this step appended) have no
+ * score yet: theirs is set instead. A page may be listed once only
+ * (FE_ERR_INVALID_ARGUMENT: scores of a shared page would be added to by two
+ * CTAs). max_keys, at creation: the most query rows x keys of a step, each
+ * sequence's keys rounded up to a multiple of 16, summed over the sequences; the
+ * plan holds hkv * (hq / hkv rounded up to even) fp32 raw scores for each. A
+ * step beyond it fails with FE_ERR_CAPACITY. A query row with an infinity or NaN
+ * gives its keys NaN. */
+int fe_scored_plan_create(int hq, int hkv, int dim, int page, int max_batch, int max_pages,
+                          int dtype, int num_blocks, int64_t max_keys, fe_long_plan** plan_out);
+int fe_scored_plan_prepare(fe_long_plan* plan, const int32_t* qo, const int32_t* kv,
+                           const int32_t* pages, const int32_t* last, const int32_t* fresh,
+                           int batch, int rows, int graph, void* stream);
+int fe_scored_attn_run(fe_long_plan* plan, const void* q, const void* k_pool, const void* v_pool,
+                       float* scores, void* out, void* stream);
+
+/* Host-side numbers of the last prepare. */
+typedef struct fe_long_plan_info {
+  int rows, shared_groups;   /* groups whose prefix is read once */
+  int row_ctas, decode_ctas; /* CTAs of the two kernels (causal) */
+  int64_t shared_tiles;      /* 16-key tiles (x KV heads) that sharing saves */
+  int64_t partial_floats, weight_floats;
+} fe_long_plan_info;
+int fe_long_plan_get_info(const fe_long_plan* plan, fe_long_plan_info* info);
+
+/* ------------------------------------------------------------------------
  * Device-side step preparation (no reference counterpart: replaces the host
  * loops of CudaModel::prepare, src/cuda_model.cpp:131-142, and the host
  * planning plus pageable H2D copies of prepare_plan,
@@ -492,6 +560,10 @@ int fe_attn_plan_create_host(int hq, int hkv, int dim, int page, int max_batch, 
                              int dtype, int num_blocks, int grid_cap, fe_attn_plan** plan_out);
 int fe_kv8_plan_create_host(int hq, int hkv, int dim, int page, int max_batch, int max_pages,
                             int dtype, int num_blocks, int grid_cap, fe_attn_plan** plan_out);
+int fe_long_plan_create_host(int hq, int hkv, int dim, int page, int max_batch, int max_pages,
+                             int dtype, int num_blocks, int scored, int64_t max_keys, int grid_cap,
+                             fe_long_plan** plan_out);
+int fe_long_plan_debug_meta(const fe_long_plan* plan, void* dst, int64_t cap, int64_t* bytes);
 /* Copy the packed work-list metadata of the last prepare into `dst` (at most
  * `cap` bytes); *bytes receives its full size. Layout: fe_attn_plan.h. */
 int fe_attn_plan_debug_meta(const fe_attn_plan* plan, void* dst, int64_t cap, int64_t* bytes);
