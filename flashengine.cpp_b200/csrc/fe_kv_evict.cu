@@ -16,6 +16,7 @@ namespace fe {
 namespace {
 
 constexpr int kSelThreads = 512;
+constexpr int kSelList = 2048;
 constexpr int kSelWarps = kSelThreads / 32;
 constexpr int kBins = 2048;
 constexpr int kSelKeys = 48 << 10;  // keys that fit in shared memory beside the histogram
@@ -78,25 +79,58 @@ __device__ __forceinline__ int block_scan(int v, int* warp_sums, int& total) {
   return before + x - v;
 }
 
+// The bin from the top in which the left-th key lies: (bin, keys still wanted
+// of it), for the whole block. hist holds kBins bins.
+__device__ __forceinline__ int2 find_bin(const int* hist, int left, int* warp_sums, int* found) {
+  constexpr int kPer = kBins / kSelThreads;
+  const int tid = threadIdx.x;
+  int mine[kPer], sum = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    mine[i] = hist[kBins - 1 - (tid * kPer + i)];
+    sum += mine[i];
+  }
+  int total;
+  int above = block_scan(sum, warp_sums, total);
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    if (above < left && left <= above + mine[i]) {
+      found[0] = kBins - 1 - (tid * kPer + i);
+      found[1] = left - above;
+    }
+    above += mine[i];
+  }
+  __syncthreads();
+  const int2 r = make_int2(found[0], found[1]);
+  __syncthreads();  // hist and found may be written again
+  return r;
+}
+
 // One CTA per (sequence, KV head). The `want` best of the tokens between sink
-// and the recent ones are found by a radix select over their ordered scores
-// (11, 11 and 10 bits: histogram, then the bin in which the want-th lies),
-// which gives the threshold and how many of the tokens equal to it are kept,
-// the lowest indexes first; then the kept tokens are written in order.
-// The keys of a sequence of up to `room` tokens stay in shared memory between
-// the passes; a longer one's scores are read again by each.
+// and the recent ones are found by a radix select over their ordered scores:
+// a histogram of the first 11 bits gives the bin in which the want-th key lies,
+// the keys of that bin are listed, and two more histograms (11 and 10 bits)
+// over the list give the threshold and how many of the tokens equal to it are
+// kept, the lowest indexes first; then the kept tokens are written in order.
+// Scores are read four tokens at a time (pages are multiples of 16), the first
+// histogram on the way. The keys of a sequence of up to `room` tokens stay in
+// shared memory; a longer one's scores are read again by each pass, and so are
+// all keys where the bin has more than kSelList (equal or close scores).
 __global__ void __launch_bounds__(kSelThreads)
     select_kernel(const float* __restrict__ scores, const SeqTable table,
                   int32_t* __restrict__ kept, int hkv, int budget, int sink, int recent, int room,
                   unsigned int* err) {
   extern __shared__ uint32_t keys[];
   __shared__ int hist[kBins];
+  __shared__ uint32_t list[kSelList];
   __shared__ int warp_sums[kSelWarps];
-  __shared__ int found[2];
+  __shared__ int found[2], listed;
   pdl_trigger();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0;
+  if (tid == 0) listed = 0;
   pdl_wait();  // the scores come from, and the lists may come from, earlier kernels
   const int b = blockIdx.x / hkv, h = blockIdx.x % hkv;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int32_t* out = kept + static_cast<int64_t>(blockIdx.x) * budget;
   int p0, n;
   if (!sequence(table, b, p0, n)) {
@@ -113,56 +147,81 @@ __global__ void __launch_bounds__(kSelThreads)
   for (int i = tid; i < recent; i += kSelThreads) out[budget - recent + i] = end + i;
   if (want == 0) return;
   const float* sc = scores + static_cast<int64_t>(h) * table.cache_slots;
-  auto load = [&](int t) -> uint32_t {
-    const int64_t slot = slot_of(table, p0, t);
+  const bool cached = n <= room;
+  // the keys of tokens 4g .. 4g + 3 (whose slots are adjacent)
+  auto load4 = [&](int g) -> uint4 {
+    const int64_t slot = slot_of(table, p0, 4 * g);
     if (slot < 0) {
       raise_device_error(err, FE_DEVERR_PAGE_RANGE);
-      return 0;
+      return make_uint4(0, 0, 0, 0);
     }
-    return ordered(__ldg(sc + slot));
+    const float4 x = __ldg(reinterpret_cast<const float4*>(sc + slot));
+    return make_uint4(ordered(x.x), ordered(x.y), ordered(x.z), ordered(x.w));
   };
-  const bool cached = n <= room;
-  if (cached)
-    for (int t = sink + tid; t < end; t += kSelThreads) keys[t] = load(t);
-  auto key = [&](int t) -> uint32_t { return cached ? keys[t] : load(t); };
-  // ---- the want-th largest key: `prefix` holds its bits above `shift`
-  uint32_t prefix = 0;
-  int left = want;  // of the keys that begin with prefix
-#pragma unroll 1
-  for (int pass = 0; pass < 3; ++pass) {
-    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
-    const int bits = pass == 2 ? 10 : 11;
-    for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0;
-    __syncthreads();
-    const uint32_t mask = pass == 0 ? 0u : ~0u << (shift + bits);
+  auto key = [&](int t) -> uint32_t {
+    if (cached) return keys[t];
+    const int64_t slot = slot_of(table, p0, t);
+    return slot < 0 ? 0 : ordered(__ldg(sc + slot));
+  };
+  __syncthreads();
+  {
+    constexpr int kAhead = 4;
+    const int g1 = (end + 3) / 4;
+    for (int g0 = sink / 4 + tid; g0 < g1; g0 += kAhead * kSelThreads) {
+      uint4 x[kAhead];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int g = g0 + u * kSelThreads;
+        if (g < g1) x[u] = load4(g);
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int g = g0 + u * kSelThreads;
+        if (g >= g1) break;
+        if (cached) reinterpret_cast<uint4*>(keys)[g] = x[u];
+        const uint32_t v[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (4 * g + i >= sink && 4 * g + i < end) atomicAdd(&hist[v[i] >> 21], 1);
+      }
+    }
+  }
+  __syncthreads();
+  int2 at = find_bin(hist, want, warp_sums, found);
+  uint32_t prefix = static_cast<uint32_t>(at.x) << 21;
+  int left = at.y;  // of the keys that begin with prefix
+  // ---- the rest of the threshold's bits, over the keys of its bin
+  for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0;
+  __syncthreads();
+  for (int t = sink + tid; t < end; t += kSelThreads) {
+    const uint32_t x = key(t);
+    if ((x >> 21) == (prefix >> 21)) {
+      atomicAdd(&hist[(x >> 10) & 2047], 1);
+      const int i = atomicAdd(&listed, 1);
+      if (i < kSelList) list[i] = x;
+    }
+  }
+  __syncthreads();
+  const bool whole = listed <= kSelList;  // the list holds the bin
+  const int count = min(listed, kSelList);
+  at = find_bin(hist, left, warp_sums, found);
+  prefix |= static_cast<uint32_t>(at.x) << 10;
+  left = at.y;
+  for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0;
+  __syncthreads();
+  if (whole) {
+    for (int i = tid; i < count; i += kSelThreads)
+      if ((list[i] >> 10) == (prefix >> 10)) atomicAdd(&hist[list[i] & 1023], 1);
+  } else {
     for (int t = sink + tid; t < end; t += kSelThreads) {
       const uint32_t x = key(t);
-      if ((x & mask) == prefix) atomicAdd(&hist[(x >> shift) & ((1u << bits) - 1)], 1);
+      if ((x >> 10) == (prefix >> 10)) atomicAdd(&hist[x & 1023], 1);
     }
-    __syncthreads();
-    // bins from the largest down, a few a thread
-    constexpr int kPer = kBins / kSelThreads;
-    int mine[kPer], sum = 0;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      mine[i] = hist[kBins - 1 - (tid * kPer + i)];
-      sum += mine[i];
-    }
-    int total;
-    int above = block_scan(sum, warp_sums, total);
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      if (above < left && left <= above + mine[i]) {
-        found[0] = kBins - 1 - (tid * kPer + i);
-        found[1] = left - above;
-      }
-      above += mine[i];
-    }
-    __syncthreads();
-    prefix |= static_cast<uint32_t>(found[0]) << shift;
-    left = found[1];
-    __syncthreads();
   }
+  __syncthreads();
+  at = find_bin(hist, left, warp_sums, found);
+  prefix |= static_cast<uint32_t>(at.x);
+  left = at.y;
   // ---- kept tokens in order: a warp owns a stretch of the tokens
   const int span = end - sink;
   const int per = ((span + kSelWarps - 1) / kSelWarps + 31) / 32 * 32;
@@ -201,13 +260,16 @@ __global__ void __launch_bounds__(kSelThreads)
 // compaction: for every sequence and KV head, the K and V rows and the score
 // of token kept[j] move to token j. A CTA walks the list of one (sequence,
 // head) in order, for one slice of the row's 16-byte chunks (slices give one
-// sequence's move more CTAs). Each step moves kMoveRows tokens: all of them are
-// read before any is written, and the sources of later steps lie at or past
-// their own index (kept[j] >= j, checked), which no earlier step writes; so the
-// move works in place.
+// sequence's move more CTAs). A table of the source and destination slots of
+// kTableTokens tokens is made first, so that the moves wait for no index. Each
+// step moves rows * kMoveUnroll tokens: all of them are read before any is
+// written, and the sources of later steps lie at or past their own index
+// (kept[j] >= j, checked), which no earlier step writes; so the move works in
+// place.
 // ---------------------------------------------------------------------------
 constexpr int kMoveThreads = 256;
 constexpr int kMoveUnroll = 4;
+constexpr int kTableTokens = kMoveThreads;
 
 struct MoveArgs {
   uint4* k;
@@ -222,6 +284,7 @@ struct MoveArgs {
 };
 
 __global__ void __launch_bounds__(kMoveThreads) compact_kernel(const MoveArgs a) {
+  __shared__ int2 table[2][kTableTokens];  // source and destination slot, -1: no move
   pdl_trigger();
   pdl_wait();
   const int b = blockIdx.x / a.hkv, h = blockIdx.x % a.hkv;
@@ -231,9 +294,10 @@ __global__ void __launch_bounds__(kMoveThreads) compact_kernel(const MoveArgs a)
   const bool idle = row >= rows;  // threads left over where lanes does not divide the block
   const bool is_v = c >= a.slice;
   const int chunk = blockIdx.y * a.slice + (is_v ? c - a.slice : c);
-  const bool first = blockIdx.y == 0 && c == 0;
-  uint4* pool = is_v ? a.v : a.k;
-  float* sc = a.scores ? a.scores + static_cast<int64_t>(h) * a.src.cache_slots : nullptr;
+  const bool scoring = blockIdx.y == 0 && c == 0 && a.scores != nullptr;
+  uint4* pool = (is_v ? a.v : a.k) + h * a.chunks + chunk;
+  const int64_t slot_chunks = static_cast<int64_t>(a.hkv) * a.chunks;
+  float* sc = a.scores + (a.scores ? static_cast<int64_t>(h) * a.src.cache_slots : 0);
   int p0, n, d0, dn;
   bool good = sequence(a.src, b, p0, n);
   if (a.in_place) {
@@ -253,35 +317,49 @@ __global__ void __launch_bounds__(kMoveThreads) compact_kernel(const MoveArgs a)
     return;
   }
   const int32_t* kept = a.kept + static_cast<int64_t>(blockIdx.x) * a.budget;
-  for (int j0 = 0; j0 < a.budget; j0 += rows * kMoveUnroll) {
-    int64_t to[kMoveUnroll];
-    uint4 x[kMoveUnroll];
-    float s[kMoveUnroll];
-#pragma unroll
-    for (int u = 0; u < kMoveUnroll; ++u) {
-      const int j = j0 + u * rows + row;
-      to[u] = -1;
-      const int t = !idle && j < a.budget ? __ldg(kept + j) : -1;
-      if (t < 0 || (a.in_place && t == j)) continue;
-      int64_t from = -1;
-      if (t < n && j < dn && (!a.in_place || t > j)) {
-        from = slot_of(a.src, p0, t);
-        to[u] = slot_of(a.in_place ? a.src : a.dst, d0, j);
+  int next = static_cast<int>(threadIdx.x) < a.budget ? __ldg(kept + threadIdx.x) : -1;
+  int buf = 0;
+  for (int base = 0; base < a.budget; base += kTableTokens, buf ^= 1) {
+    {
+      const int j = base + threadIdx.x, t = next;
+      const int jn = j + kTableTokens;
+      next = jn < a.budget ? __ldg(kept + jn) : -1;
+      int2 e = make_int2(-1, -1);
+      if (t >= 0 && !(a.in_place && t == j)) {
+        if (t < n && j < dn && (!a.in_place || t > j)) {
+          e.x = static_cast<int>(slot_of(a.src, p0, t));
+          e.y = static_cast<int>(slot_of(a.in_place ? a.src : a.dst, d0, j));
+        }
+        if (e.x < 0 || e.y < 0) {
+          if (blockIdx.y == 0) raise_device_error(a.err, FE_DEVERR_PAGE_RANGE);
+          e = make_int2(-1, -1);
+        }
       }
-      if (from < 0 || to[u] < 0) {
-        if (first) raise_device_error(a.err, FE_DEVERR_PAGE_RANGE);
-        to[u] = -1;
-        continue;
-      }
-      x[u] = pool[(from * a.hkv + h) * a.chunks + chunk];
-      if (first && sc) s[u] = sc[from];
+      table[buf][threadIdx.x] = e;
     }
-    __syncthreads();  // everything of this step has been read
+    // nothing of these tokens moves: a prefix that stays, the end of the list.
+    // (Two buffers: this barrier also keeps the table before the last in use.)
+    if (!__syncthreads_or(table[buf][threadIdx.x].x >= 0)) continue;
+    const int count = min(kTableTokens, a.budget - base);
+    for (int j0 = 0; j0 < count; j0 += rows * kMoveUnroll) {
+      int2 e[kMoveUnroll];
+      uint4 x[kMoveUnroll];
+      float s[kMoveUnroll];
 #pragma unroll
-    for (int u = 0; u < kMoveUnroll; ++u) {
-      if (to[u] < 0) continue;
-      pool[(to[u] * a.hkv + h) * a.chunks + chunk] = x[u];
-      if (first && sc) sc[to[u]] = s[u];
+      for (int u = 0; u < kMoveUnroll; ++u) {
+        const int j = j0 + u * rows + row;
+        e[u] = !idle && j < count ? table[buf][j] : make_int2(-1, -1);
+        if (e[u].x < 0) continue;
+        x[u] = pool[e[u].x * slot_chunks];
+        if (scoring) s[u] = sc[e[u].x];
+      }
+      __syncthreads();  // everything of this step has been read
+#pragma unroll
+      for (int u = 0; u < kMoveUnroll; ++u) {
+        if (e[u].x < 0) continue;
+        pool[e[u].y * slot_chunks] = x[u];
+        if (scoring) sc[e[u].y] = s[u];
+      }
     }
   }
 }
@@ -322,6 +400,8 @@ int fe_kv_select(const float* scores, const int32_t* kv, const int32_t* pages, i
   if (max_len < 0) return fail(FE_ERR_INVALID_ARGUMENT, "fe_kv_select: max_len < 0");
   if (batch == 0 || budget == 0) return FE_OK;
   if (!scores || !kept) return fail(FE_ERR_INVALID_ARGUMENT, "fe_kv_select: null pointer");
+  if (!aligned16(scores))
+    return fail(FE_ERR_INVALID_ARGUMENT, "fe_kv_select: scores must be 16-byte aligned");
   const SeqTable table{kv, pages, last, num_pages, page, cache_slots};
   auto s = static_cast<cudaStream_t>(stream);
   const int room = max_len <= kSelKeys ? max_len : 0;
@@ -333,7 +413,7 @@ int fe_kv_select(const float* scores, const int32_t* kv, const int32_t* pages, i
   });
   if (attr != cudaSuccess) return cuda_fail(attr, "fe_kv_select: shared memory attribute");
   FE_CUDA_TRY(launch_pdl(select_kernel, dim3(batch * hkv), dim3(kSelThreads),
-                         sizeof(uint32_t) * room, s, scores, table, kept, hkv, budget, sink,
+                         (sizeof(uint32_t) * room + 15) / 16 * 16, s, scores, table, kept, hkv, budget, sink,
                          recent, room, device_error_word()));
   return FE_OK;
 }

@@ -10,6 +10,7 @@
 //
 // HBM-bound: 4 bytes of q and 8 of k and v per element (in and out) and one
 // cos / sin row a token.
+#include <algorithm>
 #include <string>
 
 #include "fe_rope_common.cuh"
@@ -122,10 +123,14 @@ __global__ void __launch_bounds__(kAxesThreads)
 // 16-byte aligned buffers. A head is `units` units: unit u < rot/16 owns the
 // eight pairs 8u .. 8u+7 (two 16-byte chunks), the others an unrotated chunk.
 // A thread keeps its unit and walks the heads hl, hl + hl_count, ... two at a
-// time, so that a row's cos / sin are read once for all of its heads.
-// kWhole: the eight pairs of every unit turn by one axis (sections that are
-// multiples of 8), and their cos / sin are whole vectors.
-template <typename T, bool kWhole>
+// time. The row's cos / sin, each pair's from the cache row of its own axis, are
+// gathered into shared memory by asynchronous copies one row ahead (three
+// buffers: the barrier before a row's use also ends the use of the row before
+// the last), so that a pair's axis costs one 4-byte copy a row and not one load
+// a head.
+constexpr int kRowBufs = 3;
+
+template <typename T>
 __global__ void __launch_bounds__(kAxesThreads)
     rope_axes_vec_kernel(T* __restrict__ q, const T* k, const T* __restrict__ v, T* k_out,
                          T* __restrict__ kc, T* __restrict__ vc, const AxesArgs a,
@@ -135,27 +140,39 @@ __global__ void __launch_bounds__(kAxesThreads)
     uint4 u;
     V v[4];
   };
+  extern __shared__ __align__(16) float turns[];  // [kRowBufs][rot]: cos, then sin
   pdl_trigger();
   pdl_wait();  // q, k, v come from, and the pools are read by, earlier kernels
   const int heads = a.hq + a.hkv;
   const int hl = threadIdx.x / units, u = threadIdx.x - hl * units;
-  if (hl >= hl_count) return;
+  const bool idle = hl >= hl_count;
   const int rot_units = a.rot / 16, r = a.rot / 2;
   const bool rotating = u < rot_units;
   const int e0 = rotating ? 8 * u : a.rot + 8 * (u - rot_units);
   const int e1 = e0 + r;  // the partners (rotating)
   const int first = blockIdx.x * hl_count + hl, step = gridDim.x * hl_count;
+  auto gather = [&](int row, int buf) {
+    for (int i = threadIdx.x; i < a.rot; i += blockDim.x) {
+      const int j = i < r ? i : i - r;
+      const int64_t p = __ldg(a.pos + static_cast<int64_t>(map.axis[j]) * a.rows + row);
+      // a row that is out of range is skipped below; its copies stay in bounds
+      const float* src = a.cache + (p >= 0 && p < a.max_positions ? p : 0) * a.rot + i;
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(turns + buf * a.rot + i)),
+                   "l"(src)
+                   : "memory");
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  int buf = 0;
+  if (static_cast<int>(blockIdx.y) < a.rows) gather(blockIdx.y, 0);
   for (int row = blockIdx.y; row < a.rows; row += gridDim.y) {
-    float2 c[4], s[4];
-    bool known = false, good = true;
-    int64_t slot = -1;
-    for (int h0 = first; h0 < heads; h0 += 2 * step) {
-      // every load that does not depend on the position first
-      Chunk lo[2], hi[2], vlo[2], vhi[2];
+    const int ahead = buf == kRowBufs - 1 ? 0 : buf + 1;
+    Chunk lo[2], hi[2], vlo[2], vhi[2];
+    auto load = [&](int h0) {
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         const int head = h0 + x * step;
-        if (head >= heads || (head < a.hq && !rotating)) continue;
+        if (idle || head >= heads || (head < a.hq && !rotating)) continue;
         const T* src = head < a.hq ? q + (static_cast<int64_t>(row) * a.hq + head) * a.dim
                                    : k + (static_cast<int64_t>(row) * a.hkv + head - a.hq) * a.dim;
         lo[x].u = *reinterpret_cast<const uint4*>(src + e0);
@@ -166,52 +183,45 @@ __global__ void __launch_bounds__(kAxesThreads)
           if (rotating) vhi[x].u = *reinterpret_cast<const uint4*>(vs + e1);
         }
       }
-      if (!known) {
-        known = true;
-        if (kc) slot = __ldg(a.slots + row);
-        int p[kMaxAxes];
-        good = row_positions(a, row, p, threadIdx.x == 0 && blockIdx.x == 0);
-        if (slot >= a.cache_slots) {
-          if (threadIdx.x == 0 && blockIdx.x == 0 && good)
-            raise_device_error(a.err, FE_DEVERR_SLOT_RANGE);
-          slot = -1;
-        }
-        if (good && rotating) {
-          if constexpr (kWhole) {
-            const float* base =
-                a.cache + static_cast<int64_t>(pick(p, map.axis[8 * u])) * a.rot + 8 * u;
-            const float4* cp = reinterpret_cast<const float4*>(base);
-            const float4* sp = reinterpret_cast<const float4*>(base + r);
-            const float4 c0 = __ldg(cp), c1 = __ldg(cp + 1), s0 = __ldg(sp), s1 = __ldg(sp + 1);
-            c[0] = make_float2(c0.x, c0.y);
-            c[1] = make_float2(c0.z, c0.w);
-            c[2] = make_float2(c1.x, c1.y);
-            c[3] = make_float2(c1.z, c1.w);
-            s[0] = make_float2(s0.x, s0.y);
-            s[1] = make_float2(s0.z, s0.w);
-            s[2] = make_float2(s1.x, s1.y);
-            s[3] = make_float2(s1.z, s1.w);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int j = 8 * u + 2 * i;
-              const float* c0 = a.cache + static_cast<int64_t>(pick(p, map.axis[j])) * a.rot + j;
-              const float* c1 =
-                  a.cache + static_cast<int64_t>(pick(p, map.axis[j + 1])) * a.rot + j + 1;
-              c[i] = make_float2(__ldg(c0), __ldg(c1));
-              s[i] = make_float2(__ldg(c0 + r), __ldg(c1 + r));
-            }
-          }
-        }
-      }
-      if (!good) break;
+    };
+    load(first);
+    int p[kMaxAxes];
+    const bool good = row_positions(a, row, p, threadIdx.x == 0 && blockIdx.x == 0);
+    int64_t slot = kc ? __ldg(a.slots + row) : -1;
+    if (slot >= a.cache_slots) {
+      if (threadIdx.x == 0 && blockIdx.x == 0 && good)
+        raise_device_error(a.err, FE_DEVERR_SLOT_RANGE);
+      slot = -1;
+    }
+    if (row + static_cast<int>(gridDim.y) < a.rows)
+      gather(row + gridDim.y, ahead);
+    else
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    __syncthreads();
+    const float* cs = turns + buf * a.rot + 8 * u;
+    buf = ahead;
+    if (!good) continue;
+    float4 c[2], s[2];
+    if (rotating) {
+      c[0] = *reinterpret_cast<const float4*>(cs);
+      c[1] = *reinterpret_cast<const float4*>(cs + 4);
+      s[0] = *reinterpret_cast<const float4*>(cs + r);
+      s[1] = *reinterpret_cast<const float4*>(cs + r + 4);
+    }
+    for (int h0 = first;;) {
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         const int head = h0 + x * step;
-        if (head >= heads || (head < a.hq && !rotating)) continue;
+        if (idle || head >= heads || (head < a.hq && !rotating)) continue;
         if (rotating)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) rotate<T>(lo[x].v[i], hi[x].v[i], c[i], s[i]);
+          for (int i = 0; i < 4; ++i) {
+            const float4 cc = c[i >> 1], ss = s[i >> 1];
+            rotate<T>(lo[x].v[i], hi[x].v[i],
+                      i & 1 ? make_float2(cc.z, cc.w) : make_float2(cc.x, cc.y),
+                      i & 1 ? make_float2(ss.z, ss.w) : make_float2(ss.x, ss.y));
+          }
         if (head < a.hq) {
           T* dst = q + (static_cast<int64_t>(row) * a.hq + head) * a.dim;
           *reinterpret_cast<uint4*>(dst + e0) = lo[x].u;
@@ -224,7 +234,7 @@ __global__ void __launch_bounds__(kAxesThreads)
           *reinterpret_cast<uint4*>(k_out + off + e0) = lo[x].u;
           if (rotating) *reinterpret_cast<uint4*>(k_out + off + e1) = hi[x].u;
         }
-        if (!kc || slot < 0) continue;
+        if (slot < 0) continue;
         const int64_t dst = (slot * a.hkv + h) * a.dim;
         *reinterpret_cast<uint4*>(kc + dst + e0) = lo[x].u;
         *reinterpret_cast<uint4*>(vc + dst + e0) = vlo[x].u;
@@ -233,6 +243,9 @@ __global__ void __launch_bounds__(kAxesThreads)
           *reinterpret_cast<uint4*>(vc + dst + e1) = vhi[x].u;
         }
       }
+      h0 += 2 * step;
+      if (h0 >= heads) break;
+      load(h0);
     }
   }
 }
@@ -249,16 +262,18 @@ int launch_axes(void* q, const void* k, const void* v, void* k_out, void* kc, vo
   if (a.rot % 16 == 0 && a.dim % 8 == 0 && aligned16(q) && aligned16(k) && aligned16(v) &&
       aligned16(k_out) && aligned16(kc) && aligned16(vc) && aligned16(a.cache) &&
       units <= kAxesThreads) {
-    bool whole = true;
-    for (int j = 0; j < a.rot / 2; ++j) whole &= map.axis[j] == map.axis[j & ~7];
     // heads of a row over as few blocks as fit, evenly
     const int most = kAxesThreads / units;
     const int passes = (heads + most - 1) / most;
     const int hl = (heads + passes - 1) / passes;
     const int threads = (hl * units + 31) / 32 * 32;
-    const dim3 grid(a.rows < 1024 ? passes : (passes + 1) / 2, a.rows < 65535 ? a.rows : 65535);
-    auto kernel = whole ? rope_axes_vec_kernel<T, true> : rope_axes_vec_kernel<T, false>;
-    FE_CUDA_TRY(launch_pdl(kernel, grid, dim3(threads), 0, stream, tq, tk, tv, to, tkc, tvc, a,
+    const int gx = a.rows < 1024 ? passes : (passes + 1) / 2;
+    // a row a block while there are few; then blocks that walk the rows, as many
+    // as are resident
+    const int resident = 148 * std::max(1, 65536 / (80 * threads));  // by registers
+    const int gy = a.rows < 1024 ? a.rows : std::min(a.rows, std::max(1, resident / gx));
+    FE_CUDA_TRY(launch_pdl(rope_axes_vec_kernel<T>, dim3(gx, gy), dim3(threads),
+                           sizeof(float) * kRowBufs * a.rot, stream, tq, tk, tv, to, tkc, tvc, a,
                            map, units, hl));
     return FE_OK;
   }

@@ -160,7 +160,7 @@ int fe_kv_gather(const void* pool, void* out, const int32_t* kv, const int32_t* 
  * may be among the source pages of any sequence of the call: the source keeps
  * its tokens. A page that is written belongs to one sequence. Entries that break
  * these bounds are skipped and raise FE_DEVERR_PAGE_RANGE. dim a multiple of 8,
- * at most 512; pools 16-byte aligned; cache_slots whole pages.
+ * at most 512; pools and scores 16-byte aligned; cache_slots whole pages.
  * ------------------------------------------------------------------------ */
 int fe_kv_select(const float* scores, const int32_t* kv, const int32_t* pages, int num_pages,
                  const int32_t* last, int32_t* kept, int batch, int max_len, int hkv, int page,
