@@ -34,7 +34,8 @@ CXX_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-Wall", "-Wextra"]
 
 KV_SOURCES = ["fe_kv_ops.cu", "fe_attn.cu", "fe_decode.cu", "fe_prefill_tc.cu", "fe_rope_accept.cu",
               "fe_plan_device.cu", "fe_kv8_ops.cu", "fe_kv8_decode.cu", "fe_kv8_rows.cu",
-              "fe_rope_axes.cu", "fe_kv_evict.cu", "fe_long_attn.cu", "fe_long_plan.cpp",
+              "fe_rope_axes.cu", "fe_kv_evict.cu", "fe_long_attn.cu", "fe_rows2_tc.cu", "fe_keys.cu",
+              "fe_long_plan.cpp",
               "fe_attn_plan.cpp", "fe_kv_fork.cpp"]
 SHIM_SOURCES = ["fe_native_cuda_shim.cpp"]
 HEADERS = ["fe_common.cuh", "fe_attn_common.cuh", "fe_attn_plan.h", "fe_tcgen05.cuh",

@@ -221,23 +221,27 @@ int build_cut_view(const PlanConfig& cfg, const std::vector<Unit>& units, int gr
 // CTAs of a step's many short items far more time than the others (a mixed
 // step took 314 us where this cut takes a third). The units are laid end to end
 // and cut into at most grid_cap pieces of equal cost, at whole tiles, in pieces
-// of at least kMinPiece tiles.
+// of at least cfg.row_min_piece tiles.
 int build_cost_view(const PlanConfig& cfg, const std::vector<Unit>& units, int grid_cap_in,
                     bool fixed_grid, View& v, std::string& err) {
-  constexpr int64_t kMinPiece = 4;
+  const int64_t kMinPiece = cfg.row_min_piece;
   v = View{};
   if (units.empty()) return FE_OK;
   const int64_t ov = cfg.row_item_tiles;
   const int grid_cap = std::max(1, grid_cap_in);
   auto big = [&](const Unit& u) -> int64_t { return ceil_div(u.tiles, cfg.row_tile); };
+  auto weight = [&](const Unit& u) -> int64_t {  // cost of a tile
+    return cfg.row_pair_blocks > 0 && u.nrb > cfg.row_pair_blocks ? 2 : 1;
+  };
   // Cut for CTAs of cost `budget`; emit(unit, first tile, tiles, cta). Returns
   // the CTAs used.
   auto cut = [&](int64_t budget, auto&& emit) -> int64_t {
     int64_t cta = 0, room = budget;
     for (size_t i = 0; i < units.size(); ++i) {
       int64_t at = 0, left = big(units[i]);
+      const int64_t wt = weight(units[i]);
       while (left > 0) {
-        int64_t take = std::min(left, room - ov);
+        int64_t take = room <= ov ? 0 : std::min(left, (room - ov) / wt);
         if (take < left) {  // a piece: both sides long enough, or none here
           if (left - take < kMinPiece) take = left - kMinPiece;
           if (take < kMinPiece) take = 0;
@@ -253,18 +257,19 @@ int build_cost_view(const PlanConfig& cfg, const std::vector<Unit>& units, int g
         emit(i, at, take, cta);
         at += take;
         left -= take;
-        room -= take + ov;
+        room -= take * wt + ov;
       }
     }
     return cta + 1;
   };
   int64_t total = 0, most = 0;
   for (const auto& u : units) {
-    total += big(u) + ov;
-    most = std::max(most, big(u) + ov);
+    const int64_t cost = big(u) * weight(u) + ov;
+    total += cost;
+    most = std::max(most, cost);
   }
   // (below ov + kMinPiece no unit can be cut, and every budget would do)
-  int64_t lo = std::max<int64_t>(ov + kMinPiece, (total + grid_cap - 1) / grid_cap), hi = total + most;
+  int64_t lo = std::max<int64_t>(ov + kMinPiece * (cfg.row_pair_blocks > 0 ? 2 : 1), (total + grid_cap - 1) / grid_cap), hi = total + most;
   auto none = [](size_t, int64_t, int64_t, int64_t) {};
   while (lo < hi) {
     const int64_t mid = (lo + hi) / 2;

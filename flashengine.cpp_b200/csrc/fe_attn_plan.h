@@ -71,7 +71,7 @@ struct MetaHeader {  // 128 bytes
   int32_t n_items[3], n_groups[3], grid[3], cta_off_off[3], items_off[3], groups_off[3];
   int32_t batch, rows, seqs_off, pages_off, total_bytes, chunk_tiles, dec_heads;
   // shared-prefix and scored plans (fe_long_plan.h); 0 in others
-  int32_t sink_off, row_seq_off, merge_off, chunk_off, unit_off[2], n_chunks;
+  int32_t sink_off, row_info_off, chunk_off, unit_off[2], n_chunks, key_items_off;
 };
 static_assert(sizeof(MetaHeader) == 128, "MetaHeader layout");
 
@@ -85,6 +85,8 @@ struct PlanConfig {
   bool cut_rows;              // row items' key ranges are cut across CTAs (head_dim 256, 8-bit)
   int row_tile;               // 8-bit row lists: 16-key pieces per tile of the kernel,
   int row_item_tiles;         // and an item's fixed cost in tiles (0: cut by keys alone)
+  int row_pair_blocks;        // items of more 16-row blocks cost two tiles a tile (0: none do)
+  int row_min_piece;          // fewest tiles of a piece
   int elem_bytes;             // bytes of a cached element
   int dec_min_tiles;          // fewest key tiles per CTA of the decode list, while CTAs are left
   int max_items;              // work-item capacity

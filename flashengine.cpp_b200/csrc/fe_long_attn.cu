@@ -5,7 +5,8 @@
 // (Cambridgebit/FlashEngine.cpp src/flashinfer_attention.cu:35-44).
 //
 // Both run the decode kernel (fe_decode.cu) and the row kernel
-// (fe_prefill_tc.cu) over the lists of fe_long_plan.h. A record holds, for each
+// (fe_rows2_tc.cu, fe_prefill_tc.cu at
+// head_dim 256) over the lists of fe_long_plan.h. A record holds, for each
 // of its rows, m = the largest base-2 score of its keys, l = sum 2^(s - m) and
 // O = sum 2^(s - m) v; records of disjoint keys join as
 //   m = max m_i, l = sum l_i 2^(m_i - m), out = sum O_i 2^(m_i - m) / l.
@@ -24,6 +25,10 @@ namespace fe {
 int decode_ext_launch(int dtype, int dim, int heads, const CUtensorMap& kmap,
                       const CUtensorMap& vmap, bool per_head_tma, const void* args, int grid,
                       cudaStream_t stream);
+int keys_launch(int dtype, const CUtensorMap& kmap, const CUtensorMap& vmap, const void* args,
+                int grid, cudaStream_t stream);
+int rows2_launch(int dtype, const CUtensorMap& kmap, const CUtensorMap& vmap,
+                 const CUtensorMap& qmap, const void* args, int grid, cudaStream_t stream);
 int prefill_tc_ext_launch(int dtype, int dim, const CUtensorMap& kmap, const CUtensorMap& vmap,
                           const CUtensorMap& qmap, const void* args, int grid,
                           cudaStream_t stream);
@@ -33,45 +38,26 @@ namespace {
 constexpr int kJoinThreads = 256;
 constexpr int kJoinWarps = kJoinThreads / 32;
 
-// The records of one row: nsplit of them, rec_floats apart.
+// The records of one row: n of them, rec_floats apart.
 struct Records {
-  const float* first;  // split 0's record
+  const float* first;
   int n, rec_floats, rows, row;
 };
 
-__device__ __forceinline__ const SplitGroup* group_of(const MetaHeader* hdr, const uint8_t* meta,
-                                                      int view, int unit, int row_units) {
-  const int g = reinterpret_cast<const int32_t*>(meta + hdr->unit_off[view])[unit];
-  if (g < 0) return nullptr;
-  return reinterpret_cast<const SplitGroup*>(
-             meta + hdr->groups_off[unit < row_units ? view : 2]) + g;
+// Unit and record row of packed row p (of P a KV head) for KV head h.
+template <int D>
+__device__ __forceinline__ int unit_of(int unit, int blocks, int p, int P, int h, int H,
+                                       int& row) {
+  if (blocks > 0) {
+    row = p % row_item_rows(D);
+    return unit + h * blocks + p / row_item_rows(D);
+  }
+  row = (h % H) * P + p;
+  return unit + h / H;
 }
 
-// Records of packed row p (of P) of KV head h in the units that start at
-// `unit`; n = 0 where the unit wrote its output itself.
-__device__ __forceinline__ Records records_of(const MetaHeader* hdr, const uint8_t* meta,
-                                              const float* partials, int view, int unit,
-                                              int blocks, int p, int P, int h) {
-  Records r{nullptr, 0, 0, 0, 0};
-  if (unit < 0) return r;
-  const int H = hdr->dec_heads;
-  int row;
-  if (blocks > 0) {
-    unit += h * blocks + p / 128;
-    row = p % 128;
-  } else {
-    unit += h / H;
-    row = (h % H) * P + p;
-  }
-  const int row_units = hdr->chunk_tiles;
-  const SplitGroup* g = group_of(hdr, meta, view, unit, row_units);
-  if (!g) return r;
-  r.first = partials + g->part0;
-  r.n = g->nsplit;
-  r.rec_floats = g->rec_floats;
-  r.rows = g->rows;
-  r.row = row;
-  return r;
+__device__ __forceinline__ Records records_of(const UnitRec& u, const float* partials, int row) {
+  return Records{partials + u.part0, u.n, u.rec_floats, u.rows, row};
 }
 
 template <int D>
@@ -84,35 +70,45 @@ __device__ __forceinline__ const float* record(const Records& a, const Records& 
                 : a.first + static_cast<int64_t>(i) * a.rec_floats;
 }
 
-// One warp joins the records of one row and stores its 16-bit output.
+// One warp joins the records of one row and stores its 16-bit output. What
+// bounds it is the way to the L2 and back, so the loads of kStep records, their
+// (m, l) among them, go out together.
 template <typename T, int D>
-__device__ __forceinline__ void join_row(const Records& a, const Records& b, int lane, T* out) {
-  constexpr int kV = D / 128;  // float4 vectors per lane
+__device__ __forceinline__ void join_row(const Records& a, const Records& b, int lane, T* out,
+                                         float* lse) {
+  constexpr int kV = D / 128;         // float4 vectors per lane
+  constexpr int kStep = 8 / kV;
   const int n = a.n + b.n;
   float4 acc[kV];
 #pragma unroll
   for (int v = 0; v < kV; ++v) acc[v] = make_float4(0.f, 0.f, 0.f, 0.f);
   float M = -INFINITY, L = 0.f;
-  for (int s0 = 0; s0 < n; s0 += 32) {
-    float m = -INFINITY, l = 0.f;
-    if (s0 + lane < n) {
-      int rows, row;
-      const float* rec = record<D>(a, b, s0 + lane, rows, row);
-      m = __ldcg(rec + rows * D + row);
-      l = __ldcg(rec + rows * (D + 1) + row);
+  for (int s0 = 0; s0 < n; s0 += kStep) {
+    float m[kStep], l[kStep];
+    float4 x[kStep][kV];
+#pragma unroll
+    for (int j = 0; j < kStep; ++j) {
+      m[j] = -INFINITY;
+      l[j] = 0.f;
+#pragma unroll
+      for (int v = 0; v < kV; ++v) x[j][v] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (s0 + j < n) {
+        int rows, row;
+        const float* rec = record<D>(a, b, s0 + j, rows, row);
+        m[j] = __ldcg(rec + rows * D + row);
+        l[j] = __ldcg(rec + rows * (D + 1) + row);
+#pragma unroll
+        for (int v = 0; v < kV; ++v)
+          x[j][v] = __ldcg(reinterpret_cast<const float4*>(rec + row * D + v * 128 + lane * 4));
+      }
     }
-    float mc = m;
+    float top = M;
 #pragma unroll
-    for (int o = 16; o; o >>= 1) mc = fmaxf(mc, __shfl_xor_sync(0xffffffffu, mc, o));
-    const float M_new = fmaxf(M, mc);
-    const float base = M_new == -INFINITY ? 0.f : M_new;
+    for (int j = 0; j < kStep; ++j) top = fmaxf(top, m[j]);
+    const float base = top == -INFINITY ? 0.f : top;
     const float resc = M == -INFINITY ? 0.f : fast_exp2(M - base);
-    M = M_new;
-    const float w = s0 + lane < n ? fast_exp2(m - base) : 0.f;
-    float lw = l * w;
-#pragma unroll
-    for (int o = 16; o; o >>= 1) lw += __shfl_xor_sync(0xffffffffu, lw, o);
-    L = L * resc + lw;
+    M = top;
+    L *= resc;
 #pragma unroll
     for (int v = 0; v < kV; ++v) {
       acc[v].x *= resc;
@@ -120,20 +116,17 @@ __device__ __forceinline__ void join_row(const Records& a, const Records& b, int
       acc[v].z *= resc;
       acc[v].w *= resc;
     }
-    const int c = min(32, n - s0);
-#pragma unroll 4
-    for (int j = 0; j < c; ++j) {
-      int rows, row;
-      const float* rec = record<D>(a, b, s0 + j, rows, row);
-      const float wj = __shfl_sync(0xffffffffu, w, j);
+#pragma unroll
+    for (int j = 0; j < kStep; ++j) {
+      if (s0 + j >= n) break;
+      const float w = fast_exp2(m[j] - base);
+      L = fmaf(l[j], w, L);
 #pragma unroll
       for (int v = 0; v < kV; ++v) {
-        const float4 x =
-            __ldcg(reinterpret_cast<const float4*>(rec + row * D + v * 128 + lane * 4));
-        acc[v].x = fmaf(x.x, wj, acc[v].x);
-        acc[v].y = fmaf(x.y, wj, acc[v].y);
-        acc[v].z = fmaf(x.z, wj, acc[v].z);
-        acc[v].w = fmaf(x.w, wj, acc[v].w);
+        acc[v].x = fmaf(x[j][v].x, w, acc[v].x);
+        acc[v].y = fmaf(x[j][v].y, w, acc[v].y);
+        acc[v].z = fmaf(x[j][v].z, w, acc[v].z);
+        acc[v].w = fmaf(x[j][v].w, w, acc[v].w);
       }
     }
   }
@@ -142,112 +135,118 @@ __device__ __forceinline__ void join_row(const Records& a, const Records& b, int
   for (int v = 0; v < kV; ++v)
     store4<T>(out + v * 128 + lane * 4, acc[v].x * inv, acc[v].y * inv, acc[v].z * inv,
               acc[v].w * inv);
+  if (lse && lane == 0) *lse = M + log2f(L);
 }
 
-// Warp `w` of the joining warps: query row w / hq, head w % hq.
+// Warp `w` of the joining warps: query row w / hq, head w % hq. Everything up to
+// pdl_wait() is the plan's metadata, complete before the kernels ahead began.
 template <typename T, int D>
-__device__ __forceinline__ void join_warp(const AttnArgs<T>& a, int64_t w, int lane) {
+__device__ __forceinline__ void join_warp(const AttnArgs<T>& a, float* lse, int64_t w, int lane) {
   const MetaHeader* hdr = reinterpret_cast<const MetaHeader*>(a.meta);
   const int r = static_cast<int>(w / a.hq), head = static_cast<int>(w % a.hq);
-  if (r >= hdr->rows) return;
-  const int s = reinterpret_cast<const int32_t*>(a.meta + hdr->row_seq_off)[r];
-  const MergeSeq m = reinterpret_cast<const MergeSeq*>(a.meta + hdr->merge_off)[s];
-  const int h = head / a.G, p = (r - m.q_row0) * a.G + head % a.G;
-  const Records own = records_of(hdr, a.meta, a.partials, a.view, m.own_unit, m.own_blocks, p,
-                                 m.qrows * a.G, h);
+  const int H = hdr->dec_heads, h = head / a.G;
+  Records own{nullptr, 0, 0, 0, 0}, pre = own;
+  if (r < hdr->rows) {
+    const RowInfo x = reinterpret_cast<const RowInfo*>(a.meta + hdr->row_info_off)[r];
+    const UnitRec* units = reinterpret_cast<const UnitRec*>(a.meta + hdr->unit_off[a.view]);
+    int row;
+    if (x.own_unit >= 0) {
+      const int u = unit_of<D>(x.own_unit, x.own_blocks, x.own_p + head % a.G, x.own_rows, h, H,
+                               row);
+      own = records_of(units[u], a.partials, row);
+    }
+    if (x.pre_unit >= 0) {
+      const int u = unit_of<D>(x.pre_unit, x.pre_blocks, x.pre_p + head % a.G, x.pre_rows, h, H,
+                               row);
+      pre = records_of(units[u], a.partials, row);
+    }
+  }
+  pdl_wait();
   if (own.n == 0) return;  // written by its unit
-  const Records pre = records_of(hdr, a.meta, a.partials, a.view, m.pre_unit, m.pre_blocks,
-                                 m.pre_row0 + p, m.pre_rows, h);
-  join_row<T, D>(own, pre, lane, a.out + (static_cast<int64_t>(r) * a.hq + head) * D);
+  join_row<T, D>(own, pre, lane, a.out + w * D, lse ? lse + w : nullptr);
 }
 
-// Shared-prefix plans: one warp per query row and head.
+// One warp per query row and head; lse (scored plans): where m + log2 l of each
+// goes, fp32 [rows, hq].
 template <typename T, int D>
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttnArgs<T> a) {
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttnArgs<T> a, float* lse) {
   pdl_trigger();
-  pdl_wait();
-  join_warp<T, D>(a, static_cast<int64_t>(blockIdx.x) * kJoinWarps + (threadIdx.x >> 5),
+  join_warp<T, D>(a, lse, static_cast<int64_t>(blockIdx.x) * kJoinWarps + (threadIdx.x >> 5),
                   threadIdx.x & 31);
 }
 
-// Scored plans: the first `join_ctas` CTAs join rows as above, the others give
-// the weights of kScoreChunk keys of one KV head at a time to the scores.
-template <typename T, int D>
+// Scored plans, behind the join: the weights of kScoreChunk keys of one KV head
+// at a time, 2^(raw score - lse) summed over the packed rows in order, go to the
+// keys' scores.
 __global__ void __launch_bounds__(kJoinThreads)
-    score_kernel(const AttnArgs<T> a, float* __restrict__ scores, int hkv, int64_t cache_slots,
-                 int join_ctas) {
+    score_kernel(const uint8_t* __restrict__ meta, const float* __restrict__ raw_scores,
+                 const float* __restrict__ lse, float* __restrict__ scores, int hq, int hkv,
+                 int page, int64_t cache_slots) {
   constexpr int kPer = kScoreChunk / kJoinThreads;  // keys a thread
-  __shared__ float lse[kRowBlock];
   pdl_trigger();
-  pdl_wait();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  if (static_cast<int>(blockIdx.x) < join_ctas) {
-    join_warp<T, D>(a, static_cast<int64_t>(blockIdx.x) * kJoinWarps + warp, lane);
-    return;
-  }
-  const MetaHeader* hdr = reinterpret_cast<const MetaHeader*>(a.meta);
-  const ScoreChunk* chunks = reinterpret_cast<const ScoreChunk*>(a.meta + hdr->chunk_off);
-  const SeqInfo* seqs = reinterpret_cast<const SeqInfo*>(a.meta + hdr->seqs_off);
-  const MergeSeq* merge = reinterpret_cast<const MergeSeq*>(a.meta + hdr->merge_off);
-  const int64_t* sink = reinterpret_cast<const int64_t*>(a.meta + hdr->sink_off);
-  const int32_t* pages = reinterpret_cast<const int32_t*>(a.meta + hdr->pages_off);
+  const MetaHeader* hdr = reinterpret_cast<const MetaHeader*>(meta);
+  const ScoreChunk* chunks = reinterpret_cast<const ScoreChunk*>(meta + hdr->chunk_off);
+  const SeqInfo* seqs = reinterpret_cast<const SeqInfo*>(meta + hdr->seqs_off);
+  const int64_t* sink = reinterpret_cast<const int64_t*>(meta + hdr->sink_off);
+  const int32_t* pages = reinterpret_cast<const int32_t*>(meta + hdr->pages_off);
   const int64_t total = static_cast<int64_t>(hdr->n_chunks) * hkv;
-  for (int64_t e = blockIdx.x - join_ctas; e < total; e += gridDim.x - join_ctas) {
+  const int G = hq / hkv;
+  bool waited = false;
+  for (int64_t e = blockIdx.x; e < total; e += gridDim.x) {
     const ScoreChunk c = chunks[e / hkv];
     const int h = static_cast<int>(e % hkv);
     float w[kPer];
+    int64_t at[kPer];
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) w[i] = 0.f;
-    for (int j = c.block0; j < c.block0 + c.blocks; ++j) {
-      const SeqInfo si = seqs[j];
-      if (c.t0 >= si.length) continue;  // the block's rows do not see this far
-      const int P = si.qrows * a.G, cols = (P + 1) & ~1;
-      __syncthreads();  // the last block's sums have been read
-      for (int p = warp; p < P; p += kJoinWarps) {
-        const Records r =
-            records_of(hdr, a.meta, a.partials, a.view, merge[j].own_unit, 0, p, P, h);
-        float M = -INFINITY, L = 0.f;
-        for (int s = lane; s < r.n; s += 32) {
-          const float* rec = r.first + static_cast<int64_t>(s) * r.rec_floats;
-          const float m = __ldcg(rec + r.rows * D + r.row);
-          const float l = __ldcg(rec + r.rows * (D + 1) + r.row);
-          const float mn = fmaxf(M, m), base = mn == -INFINITY ? 0.f : mn;
-          L = L * fast_exp2(M - base) + l * fast_exp2(m - base);
-          M = mn;
-        }
-        float top = M;
-#pragma unroll
-        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        L *= fast_exp2(M - (top == -INFINITY ? 0.f : top));
-#pragma unroll
-        for (int o = 16; o; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-        if (lane == 0) lse[p] = top + log2f(L);
-      }
-      __syncthreads();
-      const int tiles = (si.length + kTileTokens - 1) / kTileTokens;
-      const float* raw = a.sink + sink[j] + static_cast<int64_t>(h) * tiles * kTileTokens * cols;
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        const int t = c.t0 + i * kJoinThreads + threadIdx.x;
-        if (t >= si.length) continue;
-        const float2* s2 = reinterpret_cast<const float2*>(raw + static_cast<int64_t>(t) * cols);
-        for (int p = 0; p < P; p += 2) {
-          const float2 s = __ldcg(s2 + p / 2);
-          w[i] += fast_exp2(s.x - lse[p]);
-          if (p + 1 < P) w[i] += fast_exp2(s.y - lse[p + 1]);
-        }
-      }
+    for (int i = 0; i < kPer; ++i) {
+      w[i] = 0.f;
+      const int t = c.t0 + i * kJoinThreads + threadIdx.x;
+      at[i] = t < c.length ? h * cache_slots +
+                                 static_cast<int64_t>(__ldg(pages + c.page_off + t / page)) * page +
+                                 t % page
+                           : -1;
     }
+    SeqInfo si = seqs[c.block0];
+    int64_t raw0 = sink[c.block0];
+    if (!waited) pdl_wait();
+    waited = true;
+    float old[kPer];
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       const int t = c.t0 + i * kJoinThreads + threadIdx.x;
-      if (t >= c.length) continue;
-      const int64_t slot =
-          static_cast<int64_t>(__ldg(pages + c.page_off + t / a.page)) * a.page + t % a.page;
-      float* at = scores + h * cache_slots + slot;
-      *at = t >= c.fresh ? w[i] : *at + w[i];
+      old[i] = at[i] >= 0 && t < c.fresh ? scores[at[i]] : 0.f;
     }
+    for (int j = 0;;) {
+      if (c.t0 < si.length) {  // else the block's rows do not see this far
+        const int P = si.qrows * G, cols = (P + 1) & ~1;
+        const int tiles = (si.length + kTileTokens - 1) / kTileTokens;
+        const float* raw = raw_scores + raw0 + static_cast<int64_t>(h) * tiles * kTileTokens * cols;
+        const float* row = lse + static_cast<int64_t>(si.q_row0) * hq + h * G;
+        for (int p = 0; p < P; p += 2) {
+          const float l0 = __ldcg(row + static_cast<int64_t>(p / G) * hq + p % G);
+          const float l1 = p + 1 < P
+                               ? __ldcg(row + static_cast<int64_t>((p + 1) / G) * hq + (p + 1) % G)
+                               : INFINITY;
+#pragma unroll
+          for (int i = 0; i < kPer; ++i) {
+            const int t = c.t0 + i * kJoinThreads + threadIdx.x;
+            if (t >= si.length) continue;
+            const float2 s = __ldcg(
+                reinterpret_cast<const float2*>(raw + static_cast<int64_t>(t) * cols + p));
+            w[i] += fast_exp2(s.x - l0);
+            if (p + 1 < P) w[i] += fast_exp2(s.y - l1);
+          }
+        }
+      }
+      if (++j >= c.blocks) break;
+      si = seqs[c.block0 + j];
+      raw0 = sink[c.block0 + j];
+    }
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (at[i] >= 0) scores[at[i]] = old[i] + w[i];
   }
+  if (!waited) pdl_wait();
 }
 
 }  // namespace
@@ -259,14 +258,18 @@ struct fe_long_plan {
   PlanConfig cfg{};
   int dtype = 0;
   bool scored = false, host_only = false;
+  bool keys = false;  // the decode list is the key kernel's
   int device = -1;
   uint8_t* d_meta = nullptr;
   size_t meta_cap = 0;
   float* d_partials = nullptr;
   float* d_sink = nullptr;
+  float* d_lse = nullptr;  // scored plans: m + log2 l of each query row and head
+  int64_t max_rows = 0;
   int64_t sink_floats = 0;
   // pinned staging, double-buffered
   uint8_t* h_meta[2] = {nullptr, nullptr};
+  size_t h_cap[2] = {0, 0};
   cudaEvent_t h_ev[2] = {nullptr, nullptr};
   bool h_used[2] = {false, false};
   int h_idx = 0;
@@ -282,6 +285,7 @@ struct fe_long_plan {
 
 namespace {
 
+constexpr int kKeyWarps = 8;  // CTAs (of one warp) of the key kernel an SM
 constexpr int64_t kLongPartialFloats = int64_t(64) << 20;  // 256 MiB
 
 void destroy_long(fe_long_plan* p) {
@@ -297,6 +301,7 @@ void destroy_long(fe_long_plan* p) {
     if (p->d_meta) cudaFree(p->d_meta);
     if (p->d_partials) cudaFree(p->d_partials);
     if (p->d_sink) cudaFree(p->d_sink);
+    if (p->d_lse) cudaFree(p->d_lse);
   }
   delete p;
 }
@@ -350,11 +355,18 @@ int create_long(const char* what, int hq, int hkv, int dim, int page, int max_ba
   c.dec_heads = 8;
   while (hkv % c.dec_heads) c.dec_heads >>= 1;
   if (dim == kWideHeadDim) c.dec_heads = hkv % 2 == 0 ? 2 : 1;
+  p->keys = dim == kHeadDim;
+  if (p->keys) {
+    c.dec_heads = 1;
+    c.dec_grid_cap = kKeyWarps * sms;
+  }
   c.row_group_blocks = 8;
   c.row_tile = dim == kWideHeadDim ? 4 : 8;
   c.row_item_tiles = 2;
+  c.row_pair_blocks = dim == kHeadDim ? 8 : 0;
+  c.row_min_piece = 2;
   c.elem_bytes = 2;
-  c.dec_min_tiles = 8;
+  c.dec_min_tiles = p->keys ? 4 : 8;
   c.max_items = c.max_groups = static_cast<int>(std::min<int64_t>(
       std::max<int64_t>(int64_t(max_batch) * hkv * 64, 8192), 1 << 20));
   c.partial_capacity = kLongPartialFloats;
@@ -363,9 +375,9 @@ int create_long(const char* what, int hq, int hkv, int dim, int page, int max_ba
   // lists (cta offsets, items, groups) three times, units twice, row blocks and
   // their tables, query rows, chunks, pages
   const size_t n = c.max_items;
-  p->meta_cap = 3 * (n * (sizeof(WorkItem) + sizeof(SplitGroup)) + 4 * size_t(sms + 1) + 64) +
-                2 * 4 * n + n * (sizeof(SeqInfo) + sizeof(MergeSeq) + 8) + 4 * 16 * n +
-                2 * size_t(max_batch) * (sizeof(SeqInfo) + sizeof(MergeSeq)) +
+  p->meta_cap = n * sizeof(KeyItem) + 3 * (n * (sizeof(WorkItem) + sizeof(SplitGroup)) + 4 * size_t(c.dec_grid_cap + 1) + 64) +
+                2 * sizeof(UnitRec) * n + n * (sizeof(SeqInfo) + 8) + sizeof(RowInfo) * 16 * n +
+                2 * size_t(max_batch) * sizeof(SeqInfo) +
                 sizeof(ScoreChunk) * size_t(max_batch) *
                     (size_t(max_pages) * page / kScoreChunk + 1) +
                 4 * size_t(max_batch) * max_pages + 4096;
@@ -376,8 +388,14 @@ int create_long(const char* what, int hq, int hkv, int dim, int page, int max_ba
   if (e == cudaSuccess) e = cudaMemset(p->d_meta, 0, sizeof(MetaHeader));
   if (e == cudaSuccess && p->sink_floats > 0)
     e = cudaMalloc(&p->d_sink, sizeof(float) * p->sink_floats);
+  // a step has no more query rows than row blocks' rows, nor than max_keys / 16
+  // keys (each row sees one block of 16 at least)
+  p->max_rows = scored ? max_keys / kTileTokens : 0;
+  if (e == cudaSuccess && p->max_rows > 0)
+    e = cudaMalloc(&p->d_lse, sizeof(float) * p->max_rows * hq);
   for (int i = 0; i < 2 && e == cudaSuccess; ++i) {
-    e = cudaMallocHost(&p->h_meta[i], p->meta_cap);
+    p->h_cap[i] = std::min<size_t>(p->meta_cap, size_t(256) << 10);  // grows with the steps
+    e = cudaMallocHost(&p->h_meta[i], p->h_cap[i]);
     if (e == cudaSuccess) e = cudaEventCreateWithFlags(&p->h_ev[i], cudaEventDisableTiming);
   }
   if (e == cudaSuccess) e = cudaDeviceSynchronize();
@@ -398,6 +416,14 @@ int install(fe_long_plan* p, LongResult& res, int batch, int rows, int graph,
     auto s = static_cast<cudaStream_t>(stream);
     const int i = p->h_idx;
     if (p->h_used[i]) FE_CUDA_TRY(cudaEventSynchronize(p->h_ev[i]));
+    if (res.meta.size() > p->h_cap[i]) {
+      uint8_t* more = nullptr;
+      const size_t cap = std::min(p->meta_cap, 2 * res.meta.size());
+      FE_CUDA_TRY(cudaMallocHost(&more, cap));
+      cudaFreeHost(p->h_meta[i]);
+      p->h_meta[i] = more;
+      p->h_cap[i] = cap;
+    }
     std::memcpy(p->h_meta[i], res.meta.data(), res.meta.size());
     FE_CUDA_TRY(
         cudaMemcpyAsync(p->d_meta, p->h_meta[i], res.meta.size(), cudaMemcpyHostToDevice, s));
@@ -459,6 +485,7 @@ int maps(fe_long_plan* p, const void* k_pool, const void* v_pool) {
           FE_OK ||
       encode_decode_map(&p->vmap_dec, v_pool, p->dtype, c.hkv, c.dim, c.dec_heads, slots) !=
           FE_OK) {
+    if (p->keys) return FE_ERR_CUDA;
     p->per_head_tma = true;
     int rc = encode_pool_map(&p->kmap_dec, k_pool, p->dtype, c.hkv, c.dim, slots);
     if (rc == FE_OK) rc = encode_pool_map(&p->vmap_dec, v_pool, p->dtype, c.hkv, c.dim, slots);
@@ -494,6 +521,12 @@ int join_ctas(const fe_long_plan* p) {
   return static_cast<int>((int64_t(p->last.rows) * p->cfg.hq + kJoinWarps - 1) / kJoinWarps);
 }
 
+int launch_decode(fe_long_plan* p, const void* args, int grid, cudaStream_t s) {
+  if (p->keys) return keys_launch(p->dtype, p->kmap_dec, p->vmap_dec, args, grid, s);
+  return decode_ext_launch(p->dtype, p->cfg.dim, p->cfg.dec_heads, p->kmap_dec, p->vmap_dec,
+                           p->per_head_tma, args, grid, s);
+}
+
 template <typename T>
 int run_shared(fe_long_plan* p, const void* q, void* out, int view, cudaStream_t s) {
   const PlanConfig& c = p->cfg;
@@ -510,17 +543,20 @@ int run_shared(fe_long_plan* p, const void* q, void* out, int view, cudaStream_t
   }
   const AttnArgs<T> a = long_args<T>(p, q, out, view, q_map_rows);
   if (grid_rows > 0) {
-    int rc = prefill_tc_ext_launch(p->dtype, c.dim, p->kmap_tc, p->vmap_tc, qmap, &a, grid_rows, s);
+    int rc = c.dim == kHeadDim
+                 ? rows2_launch(p->dtype, p->kmap_tc, p->vmap_tc, qmap, &a, grid_rows, s)
+                 : prefill_tc_ext_launch(p->dtype, c.dim, p->kmap_tc, p->vmap_tc, qmap, &a,
+                                         grid_rows, s);
     if (rc != FE_OK) return rc;
   }
   if (grid_dec > 0) {
-    int rc = decode_ext_launch(p->dtype, c.dim, c.dec_heads, p->kmap_dec, p->vmap_dec,
-                               p->per_head_tma, &a, grid_dec, s);
+    int rc = launch_decode(p, &a, grid_dec, s);
     if (rc != FE_OK) return rc;
   }
   if (p->fixed_grid || p->last.merge[view]) {
     auto kernel = c.dim == kWideHeadDim ? join_kernel<T, kWideHeadDim> : join_kernel<T, kHeadDim>;
-    FE_CUDA_TRY(launch_pdl(kernel, dim3(join_ctas(p)), dim3(kJoinThreads), 0, s, a));
+    FE_CUDA_TRY(launch_pdl(kernel, dim3(join_ctas(p)), dim3(kJoinThreads), 0, s, a,
+                           static_cast<float*>(nullptr)));
   }
   return FE_OK;
 }
@@ -530,17 +566,20 @@ int run_scored(fe_long_plan* p, const void* q, float* scores, void* out, cudaStr
   const PlanConfig& c = p->cfg;
   const int grid_dec = p->fixed_grid ? c.dec_grid_cap : p->last.grid[2];
   const AttnArgs<T> a = long_args<T>(p, q, out, 1, 0);
-  int rc = decode_ext_launch(p->dtype, c.dim, c.dec_heads, p->kmap_dec, p->vmap_dec,
-                             p->per_head_tma, &a, grid_dec, s);
+  int rc = launch_decode(p, &a, grid_dec, s);
   if (rc != FE_OK) return rc;
-  const int joins = join_ctas(p);
+  auto join = c.dim == kWideHeadDim ? join_kernel<T, kWideHeadDim> : join_kernel<T, kHeadDim>;
+  FE_CUDA_TRY(
+      launch_pdl(join, dim3(join_ctas(p)), dim3(kJoinThreads), 0, s, a, p->d_lse));
   // a graph's launch has to do for later steps of more keys: the CTAs stride
   const int64_t most = int64_t(8) * c.grid_cap;
   const int64_t work = int64_t(p->last.n_chunks) * c.hkv;
-  const int more = static_cast<int>(p->fixed_grid ? most : std::min(work, most));
-  auto kernel = c.dim == kWideHeadDim ? score_kernel<T, kWideHeadDim> : score_kernel<T, kHeadDim>;
-  FE_CUDA_TRY(launch_pdl(kernel, dim3(joins + more), dim3(kJoinThreads), 0, s, a, scores, c.hkv,
-                         int64_t(c.num_blocks + 1) * c.page, joins));
+  const int grid = static_cast<int>(p->fixed_grid ? most : std::min(work, most));
+  FE_CUDA_TRY(launch_pdl(score_kernel, dim3(grid), dim3(kJoinThreads), 0, s,
+                         static_cast<const uint8_t*>(p->d_meta),
+                         static_cast<const float*>(p->d_sink),
+                         static_cast<const float*>(p->d_lse), scores, c.hq, c.hkv, c.page,
+                         int64_t(c.num_blocks + 1) * c.page));
   return FE_OK;
 }
 
@@ -583,7 +622,7 @@ int fe_shared_plan_prepare(fe_long_plan* p, const int32_t* qo, const int32_t* kv
   LongResult res;
   std::string err;
   try {
-    rc = build_shared_plan(p->cfg, qo, kv, pages, last, group_off, shared, groups, batch, rows,
+    rc = build_shared_plan(p->cfg, p->keys, qo, kv, pages, last, group_off, shared, groups, batch, rows,
                            graph != 0, res, err);
   } catch (const std::bad_alloc&) {
     return fail(FE_ERR_CAPACITY, name + ": out of host memory");
@@ -598,10 +637,12 @@ int fe_scored_plan_prepare(fe_long_plan* p, const int32_t* qo, const int32_t* kv
   const std::string name = "fe_scored_plan_prepare";
   int rc = check_prepare(p, true, batch, rows, graph, name);
   if (rc != FE_OK) return rc;
+  if (!p->host_only && rows > p->max_rows)
+    return fail(FE_ERR_CAPACITY, name + ": query rows x keys exceed the plan's max_keys");
   LongResult res;
   std::string err;
   try {
-    rc = build_scored_plan(p->cfg, qo, kv, pages, last, fresh, batch, rows, graph != 0,
+    rc = build_scored_plan(p->cfg, p->keys, qo, kv, pages, last, fresh, batch, rows, graph != 0,
                            p->sink_floats, res, err);
   } catch (const std::bad_alloc&) {
     return fail(FE_ERR_CAPACITY, name + ": out of host memory");

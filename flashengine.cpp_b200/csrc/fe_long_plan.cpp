@@ -10,7 +10,7 @@
 namespace fe {
 namespace {
 
-constexpr int kRowItem = 128;  // packed rows of a row-kernel item
+constexpr int kRowTile = 128;  // packed rows of a tile of the row kernels
 
 // Saved key tiles (x KV heads) from which a prefix is shared: by the decode
 // kernel, whose records cost a merge at most, and by the row kernel, which is
@@ -18,18 +18,45 @@ constexpr int kRowItem = 128;  // packed rows of a row-kernel item
 constexpr int64_t kShareDecode = 64;
 constexpr int64_t kShareRows = 1024;
 
+// Where the records of a sequence's (or row block's) query rows lie; unit
+// numbers as in RowInfo.
+struct MergeSeq {
+  int q_row0 = 0, qrows = 0;
+  int own_unit = -1, own_blocks = 0;
+  int pre_unit = -1, pre_blocks = 0;
+  int pre_row0 = 0;  // its first packed row among the prefix's
+  int pre_rows = 0;  // packed rows of the prefix (a KV head)
+};
+
 struct Tables {
   std::vector<SeqInfo> seqs;
   std::vector<MergeSeq> merge;  // one per sequence of the step (or row block)
-  std::vector<int32_t> row_seq;
+  std::vector<RowInfo> rows;
   std::vector<ScoreChunk> chunks;
   std::vector<int64_t> sink;
 };
 
+// The decode list: for the key kernel cut by cost, a piece of a unit costing its
+// tiles and about kKeyItem more (its queries, first loads and record), else
+// evenly by tiles.
+constexpr int kKeyItem = 4;
+int decode_view(const PlanConfig& cfg, bool keys, const std::vector<Unit>& units, bool fixed_grid,
+                View& v, std::string& err) {
+  if (!keys)
+    return build_cut_view(cfg, units, cfg.dec_grid_cap, cfg.dec_min_tiles, fixed_grid, v, err);
+  PlanConfig c = cfg;
+  c.row_tile = 1;
+  c.row_item_tiles = kKeyItem;
+  c.row_pair_blocks = 0;
+  c.row_min_piece = cfg.dec_min_tiles;
+  return build_cost_view(c, units, cfg.dec_grid_cap, fixed_grid, v, err);
+}
+
 // views: 0 and 1 the row list without and with the mask, 2 the decode list.
 // Offsets the decode list's records past the row lists' and packs everything.
-int pack(const PlanConfig& cfg, View (&views)[3], const Tables& t, const int32_t* pages,
-         int total_pages, int batch, int rows, LongResult& out, std::string& err) {
+int pack(const PlanConfig& cfg, bool keys, View (&views)[3], const Tables& t,
+         const int32_t* pages, int total_pages, int batch, int rows, LongResult& out,
+         std::string& err) {
   const int64_t row_floats = std::max(views[0].partial_floats, views[1].partial_floats);
   out.partial_floats = row_floats + views[2].partial_floats;
   if (out.partial_floats > cfg.partial_capacity || out.partial_floats > int64_t(INT32_MAX)) {
@@ -61,14 +88,30 @@ int pack(const PlanConfig& cfg, View (&views)[3], const Tables& t, const int32_t
     h.groups_off[c] = put(v.groups);
   }
   for (int c = 0; c < 2; ++c) {
-    std::vector<int32_t> unit = views[c].unit_group;
-    unit.insert(unit.end(), views[2].unit_group.begin(), views[2].unit_group.end());
-    for (int32_t g : unit) out.merge[c] |= g >= 0;
+    std::vector<UnitRec> unit;
+    for (const View* v : {&views[c], &views[2]})
+      for (int32_t g : v->unit_group) {
+        UnitRec u{0, 0, 0, 0};
+        if (g >= 0) {
+          const SplitGroup& sg = v->groups[g];
+          u = UnitRec{sg.part0, sg.nsplit, sg.rec_floats, sg.rows};
+          out.merge[c] = true;
+        }
+        unit.push_back(u);
+      }
     h.unit_off[c] = put(unit);
   }
+  if (keys) {
+    std::vector<KeyItem> items;
+    for (const WorkItem& w : views[2].items) {
+      const SeqInfo& s = t.seqs[w.seq];
+      items.push_back(KeyItem{s.q_row0, s.qrows, s.length, s.page_off, w.kvh, w.key_mode, w.kt0,
+                              w.kt1, w.part, w.group, w.seq, 0});
+    }
+    h.key_items_off = put(items);
+  }
   h.seqs_off = put(t.seqs);
-  h.merge_off = put(t.merge);
-  h.row_seq_off = put(t.row_seq);
+  h.row_info_off = put(t.rows);
   h.chunk_off = put(t.chunks);
   h.sink_off = put(t.sink);
   h.n_chunks = out.n_chunks = static_cast<int32_t>(t.chunks.size());
@@ -81,18 +124,17 @@ int pack(const PlanConfig& cfg, View (&views)[3], const Tables& t, const int32_t
   h.rows = out.rows = rows;
   h.total_bytes = static_cast<int32_t>(meta.size());
   h.dec_heads = cfg.dec_heads;
-  h.chunk_tiles = static_cast<int32_t>(views[1].unit_group.size());  // here: row units
   std::memcpy(meta.data(), &h, sizeof(h));
   out.meta.swap(meta);
   return FE_OK;
 }
 
-// Which sequence a query row belongs to, in entries of `merge`.
-void fill_rows(Tables& t, int rows) {
-  t.row_seq.assign(rows, 0);
-  for (size_t i = 0; i < t.merge.size(); ++i)
-    for (int r = 0; r < t.merge[i].qrows; ++r)
-      t.row_seq[t.merge[i].q_row0 + r] = static_cast<int32_t>(i);
+void fill_rows(Tables& t, int rows, int G) {
+  t.rows.assign(rows, RowInfo{-1, 0, 0, 0, -1, 0, 0, 0});
+  for (const MergeSeq& m : t.merge)
+    for (int i = 0; i < m.qrows; ++i)
+      t.rows[m.q_row0 + i] = RowInfo{m.own_unit,  m.own_blocks, m.qrows * G, i * G,
+                                     m.pre_unit,  m.pre_blocks, m.pre_rows,  m.pre_row0 + i * G};
 }
 
 struct Group {
@@ -102,16 +144,16 @@ struct Group {
 };
 
 // One layout of the step; `share` off leaves every sequence whole.
-int layout(const PlanConfig& cfg, const std::vector<SeqInfo>& step, const std::vector<Group>& gs,
+int layout(const PlanConfig& cfg, bool keys, const std::vector<SeqInfo>& step, const std::vector<Group>& gs,
            const int32_t* pages, int total_pages, int rows, bool share, bool fixed_grid,
            LongResult& out, std::string& err) {
   out = LongResult{};
   const int G = cfg.hq / cfg.hkv, H = cfg.dec_heads, batch = static_cast<int>(step.size());
+  const int kRowItem = row_item_rows(cfg.dim);
   Tables t;
   t.seqs = step;
-  t.merge.assign(batch, MergeSeq{0, 0, -1, 0, -1, 0, 0, 0});
+  t.merge.assign(batch, MergeSeq{});
   std::vector<Unit> key, full, causal;
-  std::vector<int> key_refs;  // entries of `merge` whose units' numbers lie in the decode list
   auto add_rows = [&](int seq, int mode, int P, int qrows, int64_t length, bool record) {
     for (int h = 0; h < cfg.hkv; ++h)
       for (int p0 = 0; p0 < P; p0 += kRowItem) {
@@ -179,15 +221,15 @@ int layout(const PlanConfig& cfg, const std::vector<SeqInfo>& step, const std::v
   int rc = build_cost_view(cfg, full, cfg.grid_cap, fixed_grid, views[0], err);
   if (rc == FE_OK) rc = build_cost_view(cfg, causal, cfg.grid_cap, fixed_grid, views[1], err);
   if (rc == FE_OK)
-    rc = build_cut_view(cfg, key, cfg.dec_grid_cap, cfg.dec_min_tiles, fixed_grid, views[2], err);
+    rc = decode_view(cfg, keys, key, fixed_grid, views[2], err);
   if (rc != FE_OK) return rc;
-  fill_rows(t, rows);
-  return pack(cfg, views, t, pages, total_pages, batch, rows, out, err);
+  fill_rows(t, rows, G);
+  return pack(cfg, keys, views, t, pages, total_pages, batch, rows, out, err);
 }
 
 }  // namespace
 
-int build_shared_plan(const PlanConfig& cfg, const int32_t* qo, const int32_t* kv,
+int build_shared_plan(const PlanConfig& cfg, bool keys, const int32_t* qo, const int32_t* kv,
                       const int32_t* pages, const int32_t* last, const int32_t* group_off,
                       const int32_t* shared, int groups, int batch, int rows, bool fixed_grid,
                       LongResult& out, std::string& err) {
@@ -234,10 +276,10 @@ int build_shared_plan(const PlanConfig& cfg, const int32_t* qo, const int32_t* k
       // least) stay out
       x.pages = std::min(x.pages, (s.length - s.qrows) / cfg.page);
       ++members;
-      blocks += ceil_div(int64_t(s.qrows) * G, kRowItem);
+      blocks += ceil_div(int64_t(s.qrows) * G, kRowTile);
     }
     const int64_t PP = int64_t(x.rows) * G;
-    const int64_t saved = (blocks - ceil_div(PP, kRowItem)) * x.pages *
+    const int64_t saved = (blocks - ceil_div(PP, kRowTile)) * x.pages *
                           (cfg.page / kTileTokens) * cfg.hkv;
     if (members < 2 || saved < (PP <= kRowBlock ? kShareDecode : kShareRows))
       x.pages = 0;
@@ -246,17 +288,17 @@ int build_shared_plan(const PlanConfig& cfg, const int32_t* qo, const int32_t* k
     gs.push_back(x);
   }
   const int total_pages = batch > 0 ? kv[batch] : 0;
-  rc = layout(cfg, step, gs, pages, total_pages, rows, true, fixed_grid, out, err);
+  rc = layout(cfg, keys, step, gs, pages, total_pages, rows, true, fixed_grid, out, err);
   // where the records of the shared parts do not fit, every sequence stays whole
   if (rc == FE_ERR_CAPACITY && saved_total > 0) {
     saved_total = 0;
-    rc = layout(cfg, step, gs, pages, total_pages, rows, false, fixed_grid, out, err);
+    rc = layout(cfg, keys, step, gs, pages, total_pages, rows, false, fixed_grid, out, err);
   }
   out.shared_tiles = saved_total;
   return rc;
 }
 
-int build_scored_plan(const PlanConfig& cfg, const int32_t* qo, const int32_t* kv,
+int build_scored_plan(const PlanConfig& cfg, bool keys, const int32_t* qo, const int32_t* kv,
                       const int32_t* pages, const int32_t* last, const int32_t* fresh, int batch,
                       int rows, bool fixed_grid, int64_t sink_capacity, LongResult& out,
                       std::string& err) {
@@ -288,13 +330,17 @@ int build_scored_plan(const PlanConfig& cfg, const int32_t* qo, const int32_t* k
       err = "fresh[b] must be in [0, length] (b=" + std::to_string(b) + ")";
       return FE_ERR_INVALID_ARGUMENT;
     }
-    const int block0 = static_cast<int>(t.seqs.size());
+    const int block0 = static_cast<int>(t.seqs.size()), unit0 = static_cast<int>(key.size());
     for (int i = 0; i < s.qrows; i += per) {
       const int n = std::min(per, s.qrows - i), P = n * G;
       // up to the last key that the block's last row sees
       const int length = s.length - s.qrows + i + n;
       const int tiles = ceil_div(length, kTileTokens);
-      t.merge.push_back(MergeSeq{s.q_row0 + i, n, static_cast<int>(key.size()), 0, -1, 0, 0, 0});
+      MergeSeq m;
+      m.q_row0 = s.q_row0 + i;
+      m.qrows = n;
+      m.own_unit = static_cast<int>(key.size());
+      t.merge.push_back(m);
       t.seqs.push_back(SeqInfo{s.q_row0 + i, n, length, s.page_off});
       t.sink.push_back(out.sink_floats);
       out.sink_floats += int64_t(cfg.hkv) * tiles * kTileTokens * ((P + 1) & ~1);
@@ -303,17 +349,18 @@ int build_scored_plan(const PlanConfig& cfg, const int32_t* qo, const int32_t* k
     }
     const int blocks = static_cast<int>(t.seqs.size()) - block0;
     for (int t0 = 0; t0 < s.length; t0 += kScoreChunk)
-      t.chunks.push_back(ScoreChunk{block0, blocks, s.length, s.page_off, s.length - f, t0, {0, 0}});
+      t.chunks.push_back(
+          ScoreChunk{block0, blocks, s.length, s.page_off, s.length - f, t0, unit0, 0});
   }
   if (out.sink_floats > sink_capacity) {
     err = "query rows x keys exceed the plan's max_keys";
     return FE_ERR_CAPACITY;
   }
   View views[3];
-  rc = build_cut_view(cfg, key, cfg.dec_grid_cap, cfg.dec_min_tiles, fixed_grid, views[2], err);
+  rc = decode_view(cfg, keys, key, fixed_grid, views[2], err);
   if (rc != FE_OK) return rc;
-  fill_rows(t, rows);
-  return pack(cfg, views, t, pages, batch > 0 ? kv[batch] : 0, batch, rows, out, err);
+  fill_rows(t, rows, G);
+  return pack(cfg, keys, views, t, pages, batch > 0 ? kv[batch] : 0, batch, rows, out, err);
 }
 
 }  // namespace fe

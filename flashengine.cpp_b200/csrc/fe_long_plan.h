@@ -22,17 +22,36 @@
 
 namespace fe {
 
-// Where the records of a sequence's query rows lie. Units are numbered through
-// both lists, row units first; unit_off maps them to split groups (-1: the unit
-// writes its output itself).
-struct MergeSeq {  // 32 bytes
-  int32_t q_row0, qrows;
-  int32_t own_unit;    // first unit of its own keys, -1: no query rows
-  int32_t own_blocks;  // 128-row blocks a KV head; 0: units of the decode list
-  int32_t pre_unit;    // the same of its prefix, -1: none
-  int32_t pre_blocks;
-  int32_t pre_row0;    // its first packed row among the prefix's
-  int32_t pre_rows;    // packed rows of the prefix (a KV head)
+// The records of a unit (one sequence, KV head or heads, and block of rows):
+// `n` of them, rec_floats apart. Units are numbered through both lists, row
+// units first; n = 0: the unit writes its output itself.
+struct UnitRec {  // 16 bytes
+  int32_t part0, n, rec_floats, rows;
+};
+
+// Where the records of a query row lie: packed rows own_p .. own_p + G - 1 of
+// the units from own_unit on, and the same of the prefix (pre_unit -1: none).
+struct RowInfo {  // 32 bytes
+  int32_t own_unit;
+  int32_t own_blocks;  // row blocks (row_item_rows) a KV head; 0: units of the decode list
+  int32_t own_rows;    // packed rows a KV head
+  int32_t own_p;
+  int32_t pre_unit, pre_blocks, pre_rows, pre_p;
+};
+
+// Packed rows of a row-kernel item: two tiles of the two-stream kernel, or one of
+// the head_dim 256 kernel.
+#ifdef __CUDACC__
+__host__ __device__
+#endif
+constexpr int row_item_rows(int dim) { return dim == kHeadDim ? 256 : 128; }
+
+// An item of the key kernel (fe_keys.cu): a WorkItem of the decode list with what
+// it needs of its sequence.
+struct KeyItem {  // 48 bytes
+  int32_t q_row0, qrows, length, page_off;
+  int32_t kvh, key_mode, kt0, kt1;
+  int32_t part, group, seq, pad;
 };
 
 // A stretch of keys whose scores one CTA and KV head update.
@@ -41,7 +60,8 @@ struct ScoreChunk {  // 32 bytes
   int32_t length, page_off;
   int32_t fresh;  // first key whose score is set and not added to
   int32_t t0;
-  int32_t pad[2];
+  int32_t unit0;  // first unit of block0; a block has hkv / dec_heads
+  int32_t pad;
 };
 constexpr int kScoreChunk = 512;  // keys
 
@@ -56,14 +76,15 @@ struct LongResult {
 
 // group_off [groups + 1]: runs of consecutive sequences, all of them;
 // shared [groups]: pages that the members of each have in common at the start.
-int build_shared_plan(const PlanConfig& cfg, const int32_t* qo, const int32_t* kv,
+// keys: the decode list is the key kernel's (one KV head an item, cut by cost).
+int build_shared_plan(const PlanConfig& cfg, bool keys, const int32_t* qo, const int32_t* kv,
                       const int32_t* pages, const int32_t* last, const int32_t* group_off,
                       const int32_t* shared, int groups, int batch, int rows, bool fixed_grid,
                       LongResult& out, std::string& err);
 
 // fresh [batch]: keys at each sequence's end whose score is set (null: the
 // query rows). sink_capacity: floats of raw scores.
-int build_scored_plan(const PlanConfig& cfg, const int32_t* qo, const int32_t* kv,
+int build_scored_plan(const PlanConfig& cfg, bool keys, const int32_t* qo, const int32_t* kv,
                       const int32_t* pages, const int32_t* last, const int32_t* fresh, int batch,
                       int rows, bool fixed_grid, int64_t sink_capacity, LongResult& out,
                       std::string& err);

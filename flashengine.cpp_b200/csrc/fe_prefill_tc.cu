@@ -162,8 +162,8 @@ __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, volati
   return !aborted;
 }
 
-// kExt: the lists of shared-prefix plans (items that every row sees whole,
-// split at any head_dim).
+// kExt: the lists of shared-prefix plans (items that every row sees whole) at
+// head_dim 256.
 template <typename T, int D, bool kExt>
 __global__ void __launch_bounds__(kTcThreads, 1)
     paged_prefill_tc_kernel(const __grid_constant__ CUtensorMap kmap,
@@ -174,8 +174,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   constexpr int kPiecesPerTile = C::kPiecesPerTile;
   constexpr int kSlots = kSlotsTc, kKStages = C::kKStages, kVStages = C::kVStages;
   constexpr uint32_t kOCol = C::kOCol;
-  // the planner splits row items of head_dim 256 and of shared-prefix plans only
-  constexpr bool kSplits = D != kHeadDim || kExt;
+  constexpr bool kSplits = D != kHeadDim;  // the planner splits head_dim 256 row items only
   // declared 16-byte aligned so that the 1 KiB check below is not folded away
   extern __shared__ __align__(16) uint8_t smem[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
@@ -724,27 +723,31 @@ int launch_t(const CUtensorMap& kmap, const CUtensorMap& vmap, const CUtensorMap
   return FE_OK;
 }
 
-template <typename T, bool kExt>
+template <typename T>
 int launch_dim(int dim, const CUtensorMap& kmap, const CUtensorMap& vmap, const CUtensorMap& qmap,
                const void* args, int grid, cudaStream_t stream) {
   const auto& a = *static_cast<const AttnArgs<T>*>(args);
-  if (dim == kWideHeadDim) return launch_t<T, kWideHeadDim, kExt>(kmap, vmap, qmap, a, grid, stream);
-  return launch_t<T, kHeadDim, kExt>(kmap, vmap, qmap, a, grid, stream);
+  if (dim == kWideHeadDim) return launch_t<T, kWideHeadDim, false>(kmap, vmap, qmap, a, grid, stream);
+  return launch_t<T, kHeadDim, false>(kmap, vmap, qmap, a, grid, stream);
 }
 
 }  // namespace
 
 int prefill_tc_launch(int dtype, int dim, const CUtensorMap& kmap, const CUtensorMap& vmap,
                       const CUtensorMap& qmap, const void* args, int grid, cudaStream_t stream) {
-  auto run = dtype == FE_DTYPE_BF16 ? launch_dim<__nv_bfloat16, false> : launch_dim<__half, false>;
+  auto run = dtype == FE_DTYPE_BF16 ? launch_dim<__nv_bfloat16> : launch_dim<__half>;
   return run(dim, kmap, vmap, qmap, args, grid, stream);
 }
 
 int prefill_tc_ext_launch(int dtype, int dim, const CUtensorMap& kmap, const CUtensorMap& vmap,
                           const CUtensorMap& qmap, const void* args, int grid,
                           cudaStream_t stream) {
-  auto run = dtype == FE_DTYPE_BF16 ? launch_dim<__nv_bfloat16, true> : launch_dim<__half, true>;
-  return run(dim, kmap, vmap, qmap, args, grid, stream);
+  if (dim != kWideHeadDim) return fail(FE_ERR_UNSUPPORTED, "row kernel of shared-prefix plans: dim");
+  if (dtype == FE_DTYPE_BF16)
+    return launch_t<__nv_bfloat16, kWideHeadDim, true>(
+        kmap, vmap, qmap, *static_cast<const AttnArgs<__nv_bfloat16>*>(args), grid, stream);
+  return launch_t<__half, kWideHeadDim, true>(
+      kmap, vmap, qmap, *static_cast<const AttnArgs<__half>*>(args), grid, stream);
 }
 
 }  // namespace fe

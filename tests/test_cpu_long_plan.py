@@ -9,10 +9,13 @@ import fekv
 from fekv import _lib
 from fekv.ops import GROUP_DTYPE, ITEM_DTYPE, SEQ_DTYPE, FeError, check
 
-MERGE = np.dtype([(n, "<i4") for n in ("q_row0", "qrows", "own_unit", "own_blocks", "pre_unit",
-                                       "pre_blocks", "pre_row0", "pre_rows")])
+ROW = np.dtype([(n, "<i4") for n in ("own_unit", "own_blocks", "own_rows", "own_p", "pre_unit",
+                                     "pre_blocks", "pre_rows", "pre_p")])
+UNIT = np.dtype([(n, "<i4") for n in ("part0", "n", "rec_floats", "rows")])
+KEY = np.dtype([(n, "<i4") for n in ("q_row0", "qrows", "length", "page_off", "kvh", "key_mode",
+                                     "kt0", "kt1", "part", "group", "seq", "pad")])
 CHUNK = np.dtype([(n, "<i4") for n in ("block0", "blocks", "length", "page_off", "fresh", "t0",
-                                       "a", "b")])
+                                       "unit0", "pad")])
 
 
 class Host:
@@ -20,7 +23,8 @@ class Host:
                  ctas=148):
         self.lib = _lib.load()
         self.h = ctypes.c_void_p()
-        self.hq, self.hkv, self.page, self.scored = hq, hkv, page, scored
+        self.hq, self.hkv, self.dim, self.page, self.scored = hq, hkv, dim, page, scored
+        self.item = 256 if dim == 128 else 128  # packed rows of a row item
         check(self.lib.fe_long_plan_create_host(hq, hkv, dim, page, batch, pages, 1, blocks,
                                                 int(scored), max_keys, ctas, ctypes.byref(self.h)),
               "create")
@@ -59,15 +63,23 @@ class Meta:
             n, g, grid = int(h[c]), int(h[3 + c]), int(h[6 + c])
             self.lists.append((take(h[9 + c], grid + 1, "<i4") if grid else np.zeros(1, int),
                                take(h[12 + c], n, ITEM_DTYPE), take(h[15 + c], g, GROUP_DTYPE)))
-        self.batch, self.rows, self.H, self.row_units = (int(h[i]) for i in (18, 19, 24, 23))
-        self.sink_off, self.row_seq_off, merge, chunk, u0, u1, n_chunks = (int(x) for x in h[25:32])
-        self.row_seq = take(self.row_seq_off, self.rows, "<i4")
-        n_merge = (self.row_seq_off - merge) // MERGE.itemsize
-        self.merge = take(merge, n_merge, MERGE)
-        self.seqs = take(h[20], (merge - int(h[20])) // SEQ_DTYPE.itemsize, SEQ_DTYPE)
-        key_units = (u1 - u0) // 4  # at least; trimmed by use
-        self.units = [take(o, key_units, "<i4") for o in (u0, u1)]
+        self.batch, self.rows, self.H = (int(h[i]) for i in (18, 19, 24))
+        sink, info, chunk, u0, u1, n_chunks, key = (int(x) for x in h[25:32])
+        seqs = int(h[20])
+        self.info = take(info, self.rows, ROW)
+        self.units = [take(u0, (u1 - u0) // UNIT.itemsize, UNIT),
+                      take(u1, ((key or seqs) - u1) // UNIT.itemsize, UNIT)]
+        self.seqs = take(seqs, (info - seqs) // SEQ_DTYPE.itemsize, SEQ_DTYPE)
+        if key:  # the key kernel's items say the same
+            k = take(key, int(h[2]), KEY)
+            w = self.lists[2][1]
+            for n in ("kvh", "key_mode", "kt0", "kt1", "part", "group", "seq"):
+                np.testing.assert_array_equal(k[n], w[n])
+            for n, of in (("q_row0", "q_row0"), ("qrows", "qrows"), ("length", "length"),
+                          ("page_off", "page_off")):
+                np.testing.assert_array_equal(k[n], self.seqs[w["seq"]][of])
         self.chunks = take(chunk, n_chunks, CHUNK)
+        self.sink = buf[sink:int(h[21])].view("<i8")
         self.pages = buf[int(h[21]):].view("<i4")
 
 
@@ -94,20 +106,28 @@ def coverage(m, host, view):
     spans.sort()
     assert all(a[1] <= b[0] for a, b in zip(spans, spans[1:]))
 
-    def keys(unit, blocks, p, kvh, qrow, causal):
-        u = unit + (kvh * blocks + p // 128 if blocks else kvh // H)
-        g = m.units[view][u]
-        c = view if u < m.row_units else 2
-        if g < 0:
+    first = {}  # records' pieces by where they begin
+    for c in (view, 2):
+        for g, x in enumerate(m.lists[c][2]):
+            first[int(x["part0"])] = (c, g)
+
+    def keys(unit, blocks, p, P, kvh, qrow, causal):
+        u = m.units[view][unit + (kvh * blocks + p // host.item if blocks else kvh // H)]
+        if u["n"] == 0:
             return None
+        c, g = first[int(u["part0"])]
+        x = m.lists[c][2][g]
+        assert (u["n"], u["rec_floats"], u["rows"]) == (x["nsplit"], x["rec_floats"], x["rows"])
+        row = p % host.item if blocks else kvh % H * P + p
+        assert row + G <= u["rows"] and u["rows"] * (host.dim + 2) <= u["rec_floats"]
         out = []
-        for it in pieces[(c, int(g))]:
+        for it in pieces[(c, g)]:
             s = m.seqs[it["seq"]]
             assert it["kvh"] <= kvh < it["kvh"] + (1 if blocks else H)
             if blocks:
-                assert it["rb0"] * 16 == p // 128 * 128
+                assert it["rb0"] * 16 == p // host.item * host.item
             i = qrow - s["q_row0"]
-            assert 0 <= i < s["qrows"]
+            assert 0 <= i < s["qrows"] and P == s["qrows"] * G
             hides = causal and it["key_mode"] != 2
             limit = s["length"] - s["qrows"] + i + 1 if hides else s["length"]
             t = np.arange(it["kt0"] * 16, min(it["kt1"] * 16, limit))
@@ -121,16 +141,14 @@ def coverage(m, host, view):
                 direct.setdefault((c, int(it["seq"])), []).append(it)
     seen = []
     for r in range(m.rows):
-        x = m.merge[m.row_seq[r]]
-        assert x["q_row0"] <= r < x["q_row0"] + x["qrows"]
-        p = (r - x["q_row0"]) * G
+        x = m.info[r]
         for kvh in range(host.hkv):
-            own = keys(x["own_unit"], x["own_blocks"], p, kvh, r, view == 1)
+            own = keys(x["own_unit"], x["own_blocks"], x["own_p"], x["own_rows"], kvh, r, view == 1)
             if own is None:
                 seen.append(None)
                 continue
-            pre = keys(x["pre_unit"], x["pre_blocks"], x["pre_row0"] + p, kvh, r, view == 1) \
-                if x["pre_unit"] >= 0 else np.zeros(0, int)
+            pre = keys(x["pre_unit"], x["pre_blocks"], x["pre_p"], x["pre_rows"], kvh, r,
+                       view == 1) if x["pre_unit"] >= 0 else np.zeros(0, int)
             seen.append(np.sort(np.concatenate([own, pre])))
     return seen, direct
 
@@ -216,6 +234,9 @@ def test_scored_blocks_cover_rows_and_keys(shape):
             mine = [c for c in m.chunks if c["page_off"] == meta[1][b]]
             assert [c["t0"] for c in mine] == list(range(0, n, 512))
             assert all(c["length"] == n and c["fresh"] == n - fresh[b] for c in mine)
+            for j in range(mine[0]["blocks"]):  # units of its row blocks
+                r0 = int(m.seqs[mine[0]["block0"] + j]["q_row0"])
+                assert mine[0]["unit0"] + j * (hkv // m.H) == m.info[r0]["own_unit"]
             s = m.seqs[mine[0]["block0"]:mine[0]["block0"] + mine[0]["blocks"]]
             assert s["qrows"].sum() == r and (s["qrows"] * (hq // hkv) <= 16).all()
             assert s["length"][-1] == n
@@ -226,6 +247,7 @@ def test_scored_blocks_cover_rows_and_keys(shape):
     for s in spans:
         P = s["qrows"] * G
         sink.append(sink[-1] + hkv * -(-s["length"] // 16) * 16 * (P + P % 2))
+    np.testing.assert_array_equal(m.sink[:len(spans)], sink[:-1])
     assert sink[-1] <= cap * hkv * (G + G % 2)
 
 
