@@ -29,10 +29,8 @@
 //  warps 0-3, 4-7  softmax of stream 0 and 1;
 //  warps 8 / 11    producers of K (and Q) / of V: eight 16-token page pieces a
 //                  tile, one TMA box each, into 3 K and 2 V stages of 32 KiB;
-//  warp 9          MMA issue (one thread) and TMEM owner. MMAs of one thread
-//                  execute in order: S of a tile may overwrite the P that the
-//                  product issued before it reads, and the commit behind S also
-//                  tells that product's end.
+//  warps 9 / 10    issue of a stream's S and P V products (one elected thread
+//                  each); warp 9 owns the TMEM.
 // All hand-offs are mbarriers; every wait is bounded.
 #include <mutex>
 
@@ -53,7 +51,7 @@ constexpr int kHalf = kN / 2;
 constexpr int kPieces = kN / kTileTokens;
 constexpr int kKStages = 3, kVStages = 2, kQBufs = 2;
 constexpr int kThreads = 12 * 32;
-constexpr int kKWarp = 8, kMmaWarp = 9, kVWarp = 11;
+constexpr int kKWarp = 8, kMmaWarp = 9, kVWarp = 11;  // MMA: 9 and 10, a stream each
 constexpr int kBoxes = kD / 64;
 constexpr int kQBox = kM * 128;            // 128 rows x 64 dims
 constexpr int kQBytes = kBoxes * kQBox;    // 32 KiB
@@ -65,8 +63,8 @@ constexpr int kOffV = kOffK + kKStages * kTile;
 constexpr int kOffX = kOffV + kVStages * kTile;  // [stream][m, l][row]
 constexpr int kOffBar = kOffX + 2 * 2 * kM * 4;
 // q_full[2], q_empty[2], k_full[3], k_empty[3], v_full[2], v_empty[2],
-// s_full[2], p_full[2][2], o_full[2], o_free[2], x_full, drain
-constexpr int kBars = 4 + 2 * kKStages + 2 * kVStages + 10 + 2;
+// s_full[2][2], pv_done[2][2], p_full[2][2], o_full[2], o_free[2], x_full, drain
+constexpr int kBars = 4 + 2 * kKStages + 2 * kVStages + 16 + 2;
 constexpr int kSmem = kOffBar + kBars * 8 + 32;
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kOCol = 2 * kN;  // O of stream i at kOCol + i * 128
@@ -110,6 +108,16 @@ __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, volati
   return !aborted;
 }
 
+// The same value in every lane, known as such to the compiler.
+__device__ __forceinline__ int uniform(int x) { return __reduce_max_sync(0xffffffffu, x); }
+
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+               : "=r"(p));
+  return p != 0;
+}
+
 // What all roles derive from an item.
 struct Shape {
   int pieces, tiles;
@@ -138,8 +146,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* k_empty = k_full + kKStages;
   uint64_t* v_full = k_empty + kKStages;
   uint64_t* v_empty = v_full + kVStages;
-  uint64_t* s_full = v_empty + kVStages;  // [stream]: S written, the P V before it done
-  uint64_t* p_full = s_full + 2;          // [stream * 2 + half]: P written, O rescaled
+  // [stream * 2 + half of the tile]
+  uint64_t* s_full = v_empty + kVStages;  // S written
+  uint64_t* pv_done = s_full + 4;         // P V done
+  uint64_t* p_full = pv_done + 4;          // P written, O rescaled
   uint64_t* o_full = p_full + 4;          // [stream]: the item's last P V done
   uint64_t* o_free = o_full + 2;          // [stream]: O read
   uint64_t* x_full = o_free + 2;          // both streams' (m, l) written
@@ -173,23 +183,25 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) {
     for (int b = 0; b < 2; ++b) {
       mbar_init(&q_full[b], 1);
-      mbar_init(&q_empty[b], 1);
-      mbar_init(&s_full[b], 1);
-      mbar_init(&p_full[2 * b], 4);  // one arrival per warp of the group
-      mbar_init(&p_full[2 * b + 1], 4);
+      mbar_init(&q_empty[b], 2);  // as k_empty and v_empty: see the issuers
+      for (int h = 2 * b; h < 2 * b + 2; ++h) {
+        mbar_init(&s_full[h], 1);
+        mbar_init(&pv_done[h], 1);
+        mbar_init(&p_full[h], 4);  // one arrival per warp of the group
+      }
       mbar_init(&o_full[b], 1);
       mbar_init(&o_free[b], 8);  // eight warps, or four that arrive twice
     }
     for (int s = 0; s < kKStages; ++s) {
       mbar_init(&k_full[s], 1);
-      mbar_init(&k_empty[s], 1);
+      mbar_init(&k_empty[s], 2);
     }
     for (int s = 0; s < kVStages; ++s) {
       mbar_init(&v_full[s], 1);
-      mbar_init(&v_empty[s], 1);
+      mbar_init(&v_empty[s], 2);
     }
     mbar_init(x_full, 256);
-    mbar_init(drain, 1);
+    mbar_init(drain, 2);  // one commit per issuing warp
     flags[0] = 0;
     flags[1] = 0;
     fence_barrier_init();
@@ -322,9 +334,17 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (uint32_t t = qn > kQBufs ? qn - kQBufs : 0; t < qn; ++t)
             wait_bounded_short(&q_full[t % kQBufs], (t / kQBufs) & 1u, flags + 1);
       }
-    } else if (warp == kMmaWarp && lane == 0) {
-      // ------------------------------------------------------ MMA issuer
-      constexpr uint32_t idesc_s = tc::idesc_f16(Fmt<T>::v, false, false, kM, kN);
+    } else {
+      // ------------------------------------------- MMA issuers, one a stream
+      // A warp walks its stream's schedule whole and one elected thread issues:
+      // descriptors and counters then stay in uniform registers (issued by one thread
+      // under `lane == 0`, eight products took 700 to 1200 cycles of moving
+      // descriptors where they run for 512). A step is the P V product of a half tile
+      // and the S of the same half of the next tile behind it, whose slot it frees:
+      // MMAs of one thread execute in order. All that a step waits for is polled at
+      // once, a barrier a lane.
+      const int i = warp - kMmaWarp;
+      constexpr uint32_t idesc_s = tc::idesc_f16(Fmt<T>::v, false, false, kM, kHalf);
       constexpr uint32_t idesc_o = tc::idesc_f16(Fmt<T>::v, false, true, kM, kD);
       // Descriptors of the first buffers; the 14-bit start-address field (address >>
       // 4) is advanced by plain addition. K: K-major, 8-key groups kGroupBytes
@@ -333,83 +353,96 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint64_t q_desc0 = tc::smem_desc_sw128(smem_u32(smem), 16, 1024);
       const uint64_t k_desc0 = tc::smem_desc_sw128(smem_u32(smem + kOffK), 16, kGroupBytes);
       const uint64_t v_desc0 = tc::smem_desc_sw128(smem_u32(smem + kOffV), 1024, kGroupBytes);
-      uint32_t base = 0, qn = 0;       // tiles and Q tiles of earlier items
-      uint32_t np[2] = {0, 0};         // P tiles consumed, by stream
+      const uint32_t tm = uniform(tmem);
+      const uint32_t s_col = tm + i * kN, o_col = tm + kOCol + i * kD;
+      const int i0 = uniform(it0), i1 = uniform(it1);
+      uint32_t base = 0, qn = 0, done = 0;  // tiles, Q tiles and tiles of the stream before the item
       int unit = 0;
-      for (int it = it0; it < it1 && !aborted; ++it, ++unit) {
-        const Shape sh(items[it]);
-        const int q_tiles = sh.pair ? 2 : 1;
-        // S of the stream's tile j; the K stage is free behind its last reader
-        auto issue_s = [&](int i, int j) -> bool {
-          const uint32_t qt = qn + (sh.pair ? i : 0);
-          const uint32_t kg = base + sh.key_tile(i, j);
-          const int st = kg % kKStages;
-          if (j == 0 &&
-              !wait_or_abort(&q_full[qt % kQBufs], (qt / kQBufs) & 1u, flags, aborted))
-            return false;
-          if (!wait_or_abort(&k_full[st], (kg / kKStages) & 1u, flags, aborted)) return false;
+      for (int it = i0; it < i1 && !aborted; ++it, ++unit) {
+        const Shape loaded(items[it]);
+        const int tiles = uniform(loaded.tiles);
+        const bool pair = uniform(loaded.pair ? 1 : 0) != 0;
+        const int n = pair ? tiles : (tiles + 1 - i) / 2;
+        const uint32_t qt = qn + (pair ? i : 0), qb = qt % kQBufs;
+        const uint64_t q_desc = q_desc0 + uint64_t((qb * kQBytes) >> 4);
+        // K and V stages are free behind both streams' products, or this one's twice; a Q
+        // tile behind the last S of the one stream or of both
+        const int arrivals = pair ? 1 : 2, q_arrivals = pair || tiles == 1 ? 2 : 1;
+#pragma unroll 1
+        for (int step = -2; step < 2 * n; ++step) {
+          if (n == 0) break;
+          const int half = step & 1, j = step < 0 ? -1 : step >> 1;
+          const bool next = j + 1 < n;
+          const uint32_t vg = base + (pair ? j : 2 * j + i), vst = vg % kVStages;
+          const uint32_t kg = base + (pair ? j + 1 : 2 * (j + 1) + i), kst = kg % kKStages;
+          uint64_t* bar;
+          uint32_t parity;
+          if (j < 0) {  // the item's first S
+            bar = lane == 1 ? &q_full[qb] : &k_full[kst];
+            parity = lane == 1 ? (qt / kQBufs) & 1u : (kg / kKStages) & 1u;
+          } else {
+            bar = &p_full[2 * i + half];
+            parity = (done + j) & 1u;
+            if (lane == 1) {
+              bar = &v_full[vst];
+              parity = (vg / kVStages) & 1u;
+            } else if (lane == 2 && next) {
+              bar = &k_full[kst];
+              parity = (kg / kKStages) & 1u;
+            } else if (lane == 3 && unit > 0) {
+              // O belongs to the softmax groups until they have stored the last item
+              bar = &o_free[i];
+              parity = (unit - 1) & 1u;
+            }
+          }
+          if (!wait_warp(bar, parity, flags, aborted)) break;
           tc::fence_after_sync();
-          const uint64_t q_desc = q_desc0 + uint64_t(((qt % kQBufs) * kQBytes) >> 4);
-          const uint64_t k_desc = k_desc0 + uint64_t((st * kTile) >> 4);
-#pragma unroll
-          for (int kk = 0; kk < kD / 16; ++kk) {
-            const int box = kk >> 2, ko = (kk & 3) * 32;
-            tc::mma_f16(tmem + i * kN, q_desc + uint64_t((box * kQBox + ko) >> 4),
-                        k_desc + uint64_t((box * 1024 + ko) >> 4), idesc_s, kk > 0 ? 1u : 0u);
-          }
-          tc::commit(&s_full[i]);
-          if (!sh.pair || i == 1) tc::commit(&k_empty[st]);
-          // the Q tile is free behind its last S: the stream's own, or the item's
-          const bool last = sh.pair ? j + 1 == sh.tiles : sh.key_tile(i, j) + 1 == sh.tiles;
-          if (last) tc::commit(&q_empty[qt % kQBufs]);
-          return true;
-        };
-        const int n[2] = {sh.count(0), sh.count(1)};
-        bool ok = true;
-#pragma unroll 1
-        for (int step = 0; step < 2 * (n[0] + 1) && ok; ++step) {
-          const int i = step & 1, j = (step >> 1) - 1;
-          if (j >= n[i]) continue;
-          if (step == 2 && unit > 0) {
-            // both O's belong to the softmax groups until they have stored the last item
-            ok = wait_or_abort(&o_free[0], (unit - 1) & 1u, flags, aborted) &&
-                 wait_or_abort(&o_free[1], (unit - 1) & 1u, flags, aborted);
-            if (!ok) break;
-          }
-          if (j >= 0) {  // O += P V of the stream's tile j
-            const uint32_t vg = base + sh.key_tile(i, j);
-            const int st = vg % kVStages;
-            ok = wait_or_abort(&v_full[st], (vg / kVStages) & 1u, flags, aborted);
-            const uint64_t v_desc = v_desc0 + uint64_t((st * kTile) >> 4);
-            // keys 64-127 first, as the softmax writes them
-#pragma unroll 1
-            for (int half = 1; half >= 0 && ok; --half) {
-              ok = wait_or_abort(&p_full[2 * i + half], np[i] & 1u, flags, aborted);
-              if (!ok) break;
-              tc::fence_after_sync();
-              const uint32_t p_col = tmem + i * kN + half * (kN / 2);
-              const uint64_t vh = v_desc + uint64_t((half * (kPieces / 2) * kPieceBytes) >> 4);
+          const uint32_t p_col = s_col + half * kHalf;
+          const uint64_t vh =
+              v_desc0 + uint64_t((vst * kTile + half * (kPieces / 2) * kPieceBytes) >> 4);
+          const uint64_t kh =
+              k_desc0 + uint64_t((kst * kTile + half * (kPieces / 2) * kPieceBytes) >> 4);
+          const uint32_t more = step > 0 ? 1u : 0u;
+          if (elect_one()) {
+            if (j >= 0) {  // O += P V of the half
 #pragma unroll
               for (int part = 0; part < 2; ++part)
 #pragma unroll
-                for (int kk = 0; kk < kN / 32; ++kk)
-                  tc::mma_f16_ts(tmem + kOCol + i * kD, p_col + part * (kN / 4) + kk * 8,
+                for (int kk = 0; kk < kHalf / 16; ++kk)
+                  tc::mma_f16_ts(o_col, p_col + part * (kHalf / 2) + kk * 8,
                                  vh + uint64_t((kk * kPieceBytes) >> 4), idesc_o,
-                                 j == 0 && half == 1 && part == 0 && kk == 0 ? 0u : 1u);
+                                 part + kk == 0 ? more : 1u);
+              tc::commit(&pv_done[2 * i + half]);
+              if (half == 1) {
+                for (int x = 0; x < arrivals; ++x) tc::commit(&v_empty[vst]);
+                if (!next) tc::commit(&o_full[i]);
+              }
             }
-            if (!ok) break;
-            ++np[i];
-            if (!sh.pair || i == 1) tc::commit(&v_empty[st]);
-            if (j + 1 == n[i]) tc::commit(&o_full[i]);
+            if (next) {  // S of the half of the next tile
+#pragma unroll
+              for (int kk = 0; kk < kD / 16; ++kk) {
+                const int box = kk >> 2, ko = (kk & 3) * 32;
+                tc::mma_f16(p_col, q_desc + uint64_t((box * kQBox + ko) >> 4),
+                            kh + uint64_t((box * 1024 + ko) >> 4), idesc_s, kk > 0 ? 1u : 0u);
+              }
+              tc::commit(&s_full[2 * i + half]);
+              if (half == 1) {
+                for (int x = 0; x < arrivals; ++x) tc::commit(&k_empty[kst]);
+                if (j + 2 == n)
+                  for (int x = 0; x < q_arrivals; ++x) tc::commit(&q_empty[qb]);
+              }
+            }
           }
-          if (j + 1 < n[i]) ok = issue_s(i, j + 1);
+          __syncwarp();
         }
-        base += sh.tiles;
-        qn += q_tiles;
+        base += tiles;
+        qn += pair ? 2 : 1;
+        done += n;
       }
-      if (aborted) raise_device_error(a.err, FE_DEVERR_TIMEOUT);
+      if (aborted && lane == 0) raise_device_error(a.err, FE_DEVERR_TIMEOUT);
       // TMEM is released only after every MMA issued here has completed.
-      tc::commit(drain);
+      if (elect_one()) tc::commit(drain);
+      __syncwarp();
       wait_bounded_short(drain, 0, flags + 1);
     }
   } else {
@@ -421,7 +454,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t s_addr = lane_addr + gi * kN;
     const uint32_t o_addr = lane_addr + kOCol + gi * kD;
     const int G = a.G;
-    uint32_t base = 0, ns = 0;           // tiles of earlier items, S tiles of the stream
+    uint32_t base = 0, ns = 0;           // tiles of earlier items, of the stream's
     uint32_t no[2] = {0, 0}, nx = 0;     // items that used each O, that joined the streams
     for (int it = it0; it < it1 && !aborted; ++it) {
       const WorkItem w = items[it];
@@ -439,120 +472,111 @@ __global__ void __launch_bounds__(kThreads, 1)
       // m stays -inf until the first unmasked key (its weights are 0)
       float m = -INFINITY, l = 0.f;
       const int n = sh.count(gi);
-      for (int j = 0; j < n; ++j, ++ns) {
-        const int kt = sh.key_tile(gi, j);
-        const int tkey = (w.kt0 + kPieces * kt) * kTileTokens;
-        if (!wait_warp(&s_full[gi], ns & 1u, flags, aborted)) break;
+#pragma unroll 1
+      for (int step = 0; step < 2 * n; ++step) {
+        const int half = step & 1, kt = sh.key_tile(gi, step >> 1);
+        const uint32_t c = ns + (step >> 1);  // the stream's tile
+        const int t0 = (w.kt0 + kPieces * kt) * kTileTokens + half * kHalf;
+        if (!wait_warp(&s_full[2 * gi + half], c & 1u, flags, aborted)) break;
         tc::fence_after_sync();
-        // Three passes over half of the keys, one copy of the code (it has to stay in the
-        // instruction cache beside the other roles'): the maximum of the first half, of
-        // the second, whose weights follow from registers, and the first half's weights.
-        float mx = -INFINITY;
+        const uint32_t half_addr = s_addr + half * kHalf;
+        float s[kHalf];
+#pragma unroll
+        for (int x = 0; x < kHalf; x += 32)
+          tc::ld_32x32b_x32(half_addr + x, *reinterpret_cast<uint32_t(*)[32]>(&s[x]));
+        tc::wait_ld();
+        const int room = lim - t0;  // keys that the row sees here
+        if (room < kHalf) {
+#pragma unroll
+          for (int x = 0; x < kHalf; ++x)
+            if (x >= room) s[x] = -INFINITY;
+        }
+        float mx8[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) mx8[e] = fmax3(s[e], s[8 + e], s[16 + e]);
+#pragma unroll
+        for (int x = 24; x < kHalf - 8; x += 16)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) mx8[e] = fmax3(mx8[e], s[x + e], s[x + 8 + e]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) mx8[e] = fmaxf(mx8[e], s[kHalf - 8 + e]);
+        const float mx = fmaxf(fmax3(mx8[0], mx8[1], mx8[2]),
+                               fmax3(fmax3(mx8[3], mx8[4], mx8[5]), mx8[6], mx8[7]));
+        const float m_new = fmaxf(m, mx * a.scale_log2);
+        // lazily: O and l keep the old maximum until it grew by 2^8 (true for a row's
+        // first finite maximum too)
+        const bool grow = m_new > m + kRescaleThreshold;
+        if (__any_sync(0xffffffffu, grow)) {
+          const float alpha = grow ? fast_exp2(m - m_new) : 1.f;
+          if (step > 0) {
+            // the P V before this one has completed (its slot's earlier one had before this
+            // slot's S: the barrier is at most one phase short)
+            const uint32_t cp = half ? c : c - 1;
+            if (!wait_warp(&pv_done[2 * gi + (half ^ 1)], cp & 1u, flags, aborted)) break;
+            tc::fence_after_sync();
+#pragma unroll 1
+            for (int c2 = 0; c2 < kD / 16; ++c2) {
+              float ov[16];
+              tc::ld_32x32b_x16(o_addr + c2 * 16, *reinterpret_cast<uint32_t(*)[16]>(&ov[0]));
+              tc::wait_ld();
+#pragma unroll
+              for (int x = 0; x < 16; ++x) ov[x] *= alpha;
+              tc::st_32x32b_x16(o_addr + c2 * 16, *reinterpret_cast<uint32_t(*)[16]>(&ov[0]));
+            }
+          }
+          l *= alpha;
+          if (grow) m = m_new;
+        }
+        const float m_sub = m == -INFINITY ? 0.f : m;
+        // V rows of this half past the sequence end or past the loaded pieces are zeroed
+        // (the pool may hold NaN there; unloaded rows hold an older tile). The stage's
+        // earlier tile landed before the P V that made room for this S, so its full
+        // barrier is at most one phase short of this tile's.
+        const int valid = min(si.length - t0, (sh.pieces - kPieces * kt) * kTileTokens - half * kHalf);
+        if (valid < kHalf) {
+          const uint32_t vg = base + kt;
+          const int st = vg % kVStages;
+          if (!wait_warp(&v_full[st], (vg / kVStages) & 1u, flags, aborted)) break;
+          uint8_t* vb = smem + kOffV + st * kTile;
+          const int r0 = max(valid, 0), nch = (kHalf - r0) * 8;  // 16-byte chunks per box
+#pragma unroll 1
+          for (int i = r; i < kBoxes * nch; i += kM) {
+            const int box = i / nch, rem = i % nch;
+            const int row = half * kHalf + r0 + rem / 8, ch = rem % 8;
+            *reinterpret_cast<uint4*>(vb + (row >> 3) * kGroupBytes + box * 1024 +
+                                      (row & 7) * 128 + (ch << 4)) = make_uint4(0, 0, 0, 0);
+          }
+          tc::fence_proxy_async_smem();
+        }
+        // P = exp2(S * scale - m) over its own S columns: the 16-bit high part in the
+        // first 32, the residual in the others
         float2 l4[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f),
                         make_float2(0.f, 0.f)};
-        float2 nm2 = make_float2(0.f, 0.f);
         const float2 sc2 = make_float2(a.scale_log2, a.scale_log2);
-#pragma unroll 1
-        for (int pass = 0; pass < 3; ++pass) {
-          const int half = pass & 1;
-          float s[kHalf];
+        const float2 nm2 = make_float2(-m_sub, -m_sub);
 #pragma unroll
-          for (int c = 0; c < kHalf; c += 32)
-            tc::ld_32x32b_x32(s_addr + half * kHalf + c,
-                              *reinterpret_cast<uint32_t(*)[32]>(&s[c]));
-          tc::wait_ld();
-          const int room = lim - (tkey + half * kHalf);  // keys that the row sees here
-          if (room < kHalf) {
+        for (int h = 0; h < kHalf / 32; ++h) {  // 32 keys -> 16 high + 16 residual columns
+          uint32_t hi[16], lo[16];
 #pragma unroll
-            for (int c = 0; c < kHalf; ++c)
-              if (c >= room) s[c] = -INFINITY;
+          for (int e = 0; e < 16; ++e) {
+            const float2 x = fma2(make_float2(s[32 * h + 2 * e], s[32 * h + 2 * e + 1]), sc2, nm2);
+            const float2 pp = make_float2(fast_exp2(x.x), fast_exp2(x.y));
+            l4[e & 3] = add2(l4[e & 3], pp);
+            hi[e] = pack2<T>(pp.x, pp.y);
+            const float2 res = sub2(pp, hi_as_float<T>(hi[e]));
+            lo[e] = pack2<T>(res.x, res.y);
           }
-          if (pass < 2) {
-            float mx8[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) mx8[e] = fmax3(s[e], s[8 + e], s[16 + e]);
-#pragma unroll
-            for (int c = 24; c < kHalf - 8; c += 16)
-#pragma unroll
-              for (int e = 0; e < 8; ++e) mx8[e] = fmax3(mx8[e], s[c + e], s[c + 8 + e]);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) mx8[e] = fmaxf(mx8[e], s[kHalf - 8 + e]);
-            mx = fmaxf(mx, fmaxf(fmax3(mx8[0], mx8[1], mx8[2]),
-                                 fmax3(fmax3(mx8[3], mx8[4], mx8[5]), mx8[6], mx8[7])));
-            if (pass == 0) continue;
-            const float m_new = fmaxf(m, mx * a.scale_log2);
-            // lazily: O and l keep the old maximum until it grew by 2^8 (true for a
-            // row's first finite maximum too)
-            const bool grow = m_new > m + kRescaleThreshold;
-            if (__any_sync(0xffffffffu, grow)) {
-              const float alpha = grow ? fast_exp2(m - m_new) : 1.f;
-              if (j > 0) {  // the P V before this S has completed
-#pragma unroll 1
-                for (int c2 = 0; c2 < kD / 16; ++c2) {
-                  float ov[16];
-                  tc::ld_32x32b_x16(o_addr + c2 * 16,
-                                    *reinterpret_cast<uint32_t(*)[16]>(&ov[0]));
-                  tc::wait_ld();
-#pragma unroll
-                  for (int c = 0; c < 16; ++c) ov[c] *= alpha;
-                  tc::st_32x32b_x16(o_addr + c2 * 16,
-                                    *reinterpret_cast<uint32_t(*)[16]>(&ov[0]));
-                }
-              }
-              l *= alpha;
-              if (grow) m = m_new;
-            }
-            const float m_sub = m == -INFINITY ? 0.f : m;
-            nm2 = make_float2(-m_sub, -m_sub);
-            // V rows past the sequence end or past the loaded pieces are zeroed (the pool
-            // may hold NaN there; unloaded rows hold an older tile). The stage's earlier
-            // tile landed before the P V that preceded this S, so its full barrier is at
-            // most one phase short of this tile's.
-            const int valid = min(si.length - tkey, (sh.pieces - kPieces * kt) * kTileTokens);
-            if (valid < kN) {
-              const uint32_t vg = base + kt;
-              const int st = vg % kVStages;
-              if (!wait_warp(&v_full[st], (vg / kVStages) & 1u, flags, aborted)) break;
-              uint8_t* vb = smem + kOffV + st * kTile;
-              const int nch = (kN - valid) * 8;  // 16-byte chunks per 64-dim box
-#pragma unroll 1
-              for (int i = r; i < kBoxes * nch; i += kM) {
-                const int box = i / nch, rem = i % nch;
-                const int row = valid + rem / 8, ch = rem % 8;
-                *reinterpret_cast<uint4*>(vb + (row >> 3) * kGroupBytes + box * 1024 +
-                                          (row & 7) * 128 + (ch << 4)) = make_uint4(0, 0, 0, 0);
-              }
-              tc::fence_proxy_async_smem();
-            }
-          }
-          // P = exp2(S * scale - m) of a half over its own S columns: the 16-bit high
-          // part in the first 32, the residual in the others. The second half goes
-          // first (its S is in registers), and its product starts meanwhile.
-#pragma unroll
-          for (int h = 0; h < kHalf / 32; ++h) {  // 32 keys -> 16 high + 16 residual columns
-            uint32_t hi[16], lo[16];
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const float2 x =
-                  fma2(make_float2(s[32 * h + 2 * e], s[32 * h + 2 * e + 1]), sc2, nm2);
-              const float2 pp = make_float2(fast_exp2(x.x), fast_exp2(x.y));
-              l4[e & 3] = add2(l4[e & 3], pp);
-              hi[e] = pack2<T>(pp.x, pp.y);
-              const float2 res = sub2(pp, hi_as_float<T>(hi[e]));
-              lo[e] = pack2<T>(res.x, res.y);
-            }
-            tc::st_32x32b_x16(s_addr + half * kHalf + 16 * h, hi);
-            tc::st_32x32b_x16(s_addr + half * kHalf + kHalf / 2 + 16 * h, lo);
-          }
-          tc::wait_st();
-          tc::fence_before_sync();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&p_full[2 * gi + half]);
+          tc::st_32x32b_x16(half_addr + 16 * h, hi);
+          tc::st_32x32b_x16(half_addr + kHalf / 2 + 16 * h, lo);
         }
-        if (aborted) break;
+        tc::wait_st();
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[2 * gi + half]);
         l += ((l4[0].x + l4[0].y) + (l4[1].x + l4[1].y)) +
              ((l4[2].x + l4[2].y) + (l4[3].x + l4[3].y));
       }
+      ns += n;
       if (aborted) break;
       base += sh.tiles;
       const int rows_rec = min(P - p0, w.nrb * kRowBlock);
