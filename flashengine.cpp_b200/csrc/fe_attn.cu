@@ -277,6 +277,7 @@ PlanConfig make_config(int hq, int hkv, int dim, int page, int max_batch, int ma
   c.row_tile = dim == kWideHeadDim ? 4 : 8;
   c.row_item_tiles = kv8 ? 4 : 0;
   c.row_min_piece = 4;
+  c.row_weight[0] = c.row_weight[1] = 1;
   // a step of the 8-bit decode kernel is two tiles: two steps, where a short
   // batch leaves SMs idle, cost less than four in a row and their merge
   c.dec_min_tiles = kv8 ? 4 : 8;

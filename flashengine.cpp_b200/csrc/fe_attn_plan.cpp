@@ -231,7 +231,7 @@ int build_cost_view(const PlanConfig& cfg, const std::vector<Unit>& units, int g
   const int grid_cap = std::max(1, grid_cap_in);
   auto big = [&](const Unit& u) -> int64_t { return ceil_div(u.tiles, cfg.row_tile); };
   auto weight = [&](const Unit& u) -> int64_t {  // cost of a tile
-    return cfg.row_pair_blocks > 0 && u.nrb > cfg.row_pair_blocks ? 2 : 1;
+    return cfg.row_weight[cfg.row_pair_blocks > 0 && u.nrb > cfg.row_pair_blocks];
   };
   // Cut for CTAs of cost `budget`; emit(unit, first tile, tiles, cta). Returns
   // the CTAs used.
@@ -269,7 +269,9 @@ int build_cost_view(const PlanConfig& cfg, const std::vector<Unit>& units, int g
     most = std::max(most, cost);
   }
   // (below ov + kMinPiece no unit can be cut, and every budget would do)
-  int64_t lo = std::max<int64_t>(ov + kMinPiece * (cfg.row_pair_blocks > 0 ? 2 : 1), (total + grid_cap - 1) / grid_cap), hi = total + most;
+  const int64_t heavy = std::max(cfg.row_weight[0], cfg.row_pair_blocks > 0 ? cfg.row_weight[1] : 0);
+  int64_t lo = std::max<int64_t>(ov + kMinPiece * heavy, (total + grid_cap - 1) / grid_cap);
+  int64_t hi = total + most;
   auto none = [](size_t, int64_t, int64_t, int64_t) {};
   while (lo < hi) {
     const int64_t mid = (lo + hi) / 2;

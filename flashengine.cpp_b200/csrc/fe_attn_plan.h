@@ -85,7 +85,8 @@ struct PlanConfig {
   bool cut_rows;              // row items' key ranges are cut across CTAs (head_dim 256, 8-bit)
   int row_tile;               // 8-bit row lists: 16-key pieces per tile of the kernel,
   int row_item_tiles;         // and an item's fixed cost in tiles (0: cut by keys alone)
-  int row_pair_blocks;        // items of more 16-row blocks cost two tiles a tile (0: none do)
+  int row_weight[2];          // cost of a tile, in the fixed cost's units, of items of up to
+  int row_pair_blocks;        // row_pair_blocks 16-row blocks and of more (0: none)
   int row_min_piece;          // fewest tiles of a piece
   int elem_bytes;             // bytes of a cached element
   int dec_min_tiles;          // fewest key tiles per CTA of the decode list, while CTAs are left

@@ -22,7 +22,7 @@
 namespace fe {
 
 int keys_launch(int dtype, const CUtensorMap& kmap, const CUtensorMap& vmap, const void* args,
-                int grid, cudaStream_t stream);
+                int grid, bool beside, cudaStream_t stream);
 
 namespace {
 
@@ -40,6 +40,11 @@ __device__ __forceinline__ __nv_bfloat16 to_elem<__nv_bfloat16>(float x) {
 template <>
 __device__ __forceinline__ __half to_elem<__half>(float x) {
   return __float2half_rn(x);
+}
+
+// Past the L1, as TMA reads K and V: nothing here depends on its being clean.
+__device__ __forceinline__ uint32_t ld_l2(const void* p) {
+  return __ldcg(reinterpret_cast<const uint32_t*>(p));
 }
 
 // D += A B on one 16 x 8 x 16 product; no side effects, so that the compiler
@@ -89,8 +94,8 @@ struct RowState {
                           : nullptr;
 #pragma unroll
       for (int kk = 0; kk < 8; ++kk) {
-        qb[nt][kk][0] = qp ? ldg32(qp + kk * 16 + 2 * cq) : 0u;
-        qb[nt][kk][1] = qp ? ldg32(qp + kk * 16 + 8 + 2 * cq) : 0u;
+        qb[nt][kk][0] = qp ? ld_l2(qp + kk * 16 + 2 * cq) : 0u;
+        qb[nt][kk][1] = qp ? ld_l2(qp + kk * 16 + 8 + 2 * cq) : 0u;
       }
     }
     lim_min = si.length;
@@ -389,7 +394,7 @@ __device__ __forceinline__ bool piece(const AttnArgs<T>& a, const KeyItem& wi, R
 template <typename T>
 __global__ void __launch_bounds__(32)
     paged_keys_kernel(const __grid_constant__ CUtensorMap kmap,
-                      const __grid_constant__ CUtensorMap vmap, const AttnArgs<T> a) {
+                      const __grid_constant__ CUtensorMap vmap, const AttnArgs<T> a, int beside) {
   extern __shared__ __align__(16) uint8_t smem[];
   pdl_trigger();
   const int lane = threadIdx.x;
@@ -400,8 +405,8 @@ __global__ void __launch_bounds__(32)
     it0 = cta_off[blockIdx.x];
     it1 = cta_off[blockIdx.x + 1];
   }
-  if (it0 >= it1) {  // nothing to do, but not before the grid ahead is done
-    pdl_wait();
+  if (it0 >= it1) {  // nothing to do, but the grid does not end before the one ahead
+    if (!beside || blockIdx.x == 0) pdl_wait();
     return;
   }
   if (smem_u32(smem) & 1023u) {  // the swizzle's atoms
@@ -429,7 +434,11 @@ __global__ void __launch_bounds__(32)
   }
   __syncwarp();
   ring.open(it0, lane);
-  pdl_wait();  // q, the pools and the records belong to earlier kernels until here
+  // q, the pools and the records belong to earlier kernels until here. `beside`: the
+  // grid ahead is the row kernel, which lets this one start once it has waited for
+  // those itself, and which shares nothing with it but the kernel that joins their
+  // records; that one waits for this grid, so the row kernel's end is awaited last.
+  if (!beside) pdl_wait();
   for (int s = 0; s < kStages; ++s) ring.issue(lane);
   uint32_t g = 0;
   bool ok = true;
@@ -439,6 +448,7 @@ __global__ void __launch_bounds__(32)
                              : piece<T, 2>(a, wi, ring, g, flag, lane);
     ok = __all_sync(0xffffffffu, ok);
   }
+  if (beside) pdl_wait();
   if (!ok) {
     if (lane == 0) raise_device_error(a.err, FE_DEVERR_TIMEOUT);
     // what was fetched has landed before the CTA exits (bounded)
@@ -450,7 +460,7 @@ __global__ void __launch_bounds__(32)
 
 template <typename T>
 int launch_t(const CUtensorMap& kmap, const CUtensorMap& vmap, const void* args, int grid,
-             cudaStream_t stream) {
+             bool beside, cudaStream_t stream) {
   static std::once_flag once;
   static cudaError_t attr_err = cudaSuccess;
   std::call_once(once, [] {
@@ -459,16 +469,16 @@ int launch_t(const CUtensorMap& kmap, const CUtensorMap& vmap, const void* args,
   });
   if (attr_err != cudaSuccess) return cuda_fail(attr_err, "paged_keys_kernel attribute");
   FE_CUDA_TRY(launch_pdl(paged_keys_kernel<T>, dim3(grid), dim3(32), kSmem, stream, kmap, vmap,
-                         *static_cast<const AttnArgs<T>*>(args)));
+                         *static_cast<const AttnArgs<T>*>(args), beside ? 1 : 0));
   return FE_OK;
 }
 
 }  // namespace
 
 int keys_launch(int dtype, const CUtensorMap& kmap, const CUtensorMap& vmap, const void* args,
-                int grid, cudaStream_t stream) {
-  return dtype == FE_DTYPE_BF16 ? launch_t<__nv_bfloat16>(kmap, vmap, args, grid, stream)
-                                : launch_t<__half>(kmap, vmap, args, grid, stream);
+                int grid, bool beside, cudaStream_t stream) {
+  return dtype == FE_DTYPE_BF16 ? launch_t<__nv_bfloat16>(kmap, vmap, args, grid, beside, stream)
+                                : launch_t<__half>(kmap, vmap, args, grid, beside, stream);
 }
 
 }  // namespace fe

@@ -26,7 +26,7 @@ int decode_ext_launch(int dtype, int dim, int heads, const CUtensorMap& kmap,
                       const CUtensorMap& vmap, bool per_head_tma, const void* args, int grid,
                       cudaStream_t stream);
 int keys_launch(int dtype, const CUtensorMap& kmap, const CUtensorMap& vmap, const void* args,
-                int grid, cudaStream_t stream);
+                int grid, bool beside, cudaStream_t stream);
 int rows2_launch(int dtype, const CUtensorMap& kmap, const CUtensorMap& vmap,
                  const CUtensorMap& qmap, const void* args, int grid, cudaStream_t stream);
 int prefill_tc_ext_launch(int dtype, int dim, const CUtensorMap& kmap, const CUtensorMap& vmap,
@@ -362,7 +362,11 @@ int create_long(const char* what, int hq, int hkv, int dim, int page, int max_ba
   }
   c.row_group_blocks = 8;
   c.row_tile = dim == kWideHeadDim ? 4 : 8;
-  c.row_item_tiles = 2;
+  // measured: a 128-key tile of the two-stream kernel 2.0 us for 256 rows, 1.4 us for
+  // 128; of the head_dim 256 kernel (64 keys) 1.6 us; an item about 4 us more
+  c.row_weight[0] = dim == kHeadDim ? 10 : 8;
+  c.row_weight[1] = 10;
+  c.row_item_tiles = 20;  // in fifths of a microsecond, as the weights
   c.row_pair_blocks = dim == kHeadDim ? 8 : 0;
   c.row_min_piece = 2;
   c.elem_bytes = 2;
@@ -521,8 +525,8 @@ int join_ctas(const fe_long_plan* p) {
   return static_cast<int>((int64_t(p->last.rows) * p->cfg.hq + kJoinWarps - 1) / kJoinWarps);
 }
 
-int launch_decode(fe_long_plan* p, const void* args, int grid, cudaStream_t s) {
-  if (p->keys) return keys_launch(p->dtype, p->kmap_dec, p->vmap_dec, args, grid, s);
+int launch_decode(fe_long_plan* p, const void* args, int grid, bool beside, cudaStream_t s) {
+  if (p->keys) return keys_launch(p->dtype, p->kmap_dec, p->vmap_dec, args, grid, beside, s);
   return decode_ext_launch(p->dtype, p->cfg.dim, p->cfg.dec_heads, p->kmap_dec, p->vmap_dec,
                            p->per_head_tma, args, grid, s);
 }
@@ -550,7 +554,7 @@ int run_shared(fe_long_plan* p, const void* q, void* out, int view, cudaStream_t
     if (rc != FE_OK) return rc;
   }
   if (grid_dec > 0) {
-    int rc = launch_decode(p, &a, grid_dec, s);
+    int rc = launch_decode(p, &a, grid_dec, grid_rows > 0, s);
     if (rc != FE_OK) return rc;
   }
   if (p->fixed_grid || p->last.merge[view]) {
@@ -566,7 +570,7 @@ int run_scored(fe_long_plan* p, const void* q, float* scores, void* out, cudaStr
   const PlanConfig& c = p->cfg;
   const int grid_dec = p->fixed_grid ? c.dec_grid_cap : p->last.grid[2];
   const AttnArgs<T> a = long_args<T>(p, q, out, 1, 0);
-  int rc = launch_decode(p, &a, grid_dec, s);
+  int rc = launch_decode(p, &a, grid_dec, false, s);
   if (rc != FE_OK) return rc;
   auto join = c.dim == kWideHeadDim ? join_kernel<T, kWideHeadDim> : join_kernel<T, kHeadDim>;
   FE_CUDA_TRY(

@@ -10,13 +10,23 @@
 namespace fe {
 namespace {
 
-constexpr int kRowTile = 128;  // packed rows of a tile of the row kernels
-
-// Saved key tiles (x KV heads) from which a prefix is shared: by the decode
-// kernel, whose records cost a merge at most, and by the row kernel, which is
-// one more launch.
-constexpr int64_t kShareDecode = 64;
-constexpr int64_t kShareRows = 1024;
+// Costs, as measured on B200, in microseconds of one SM. A 128-key tile of the row
+// kernels: the weights of the row lists (fifths of a microsecond). The same keys
+// in the key or decode kernel: their bytes at an SM's share of the memory rate. A
+// record's bytes, written and read through the L2; one more launch on all SMs.
+double tile_us(const PlanConfig& cfg, int64_t P) {
+  if (P <= kRowBlock) return 1.75 * cfg.dim / kHeadDim;
+  const int rows = row_item_rows(cfg.dim);
+  const double per_key = 128.0 / (kTileTokens * cfg.row_tile) / 5.0;
+  const int64_t full = P / rows, rest = P % rows;
+  const double last = rest == 0 ? 0 : rest > 128 ? cfg.row_weight[1] : cfg.row_weight[0];
+  return (full * (rows > 128 ? cfg.row_weight[1] : cfg.row_weight[0]) + last) * per_key;
+}
+constexpr double kRecordGbs = 27;  // per SM
+constexpr double kLaunchUs = 2;
+// A 16-key tile and an item of a warp of the key kernel that memory does not hold up
+constexpr double kKeyTileUs = 0.65, kKeyItemUs = 2.5;
+constexpr double kHbmGbs = 6000;
 
 // Where the records of a sequence's (or row block's) query rows lie; unit
 // numbers as in RowInfo.
@@ -40,16 +50,15 @@ struct Tables {
 // tiles and about kKeyItem more (its queries, first loads and record), else
 // evenly by tiles.
 constexpr int kKeyItem = 4;
-int decode_view(const PlanConfig& cfg, bool keys, const std::vector<Unit>& units, bool fixed_grid,
-                View& v, std::string& err) {
-  if (!keys)
-    return build_cut_view(cfg, units, cfg.dec_grid_cap, cfg.dec_min_tiles, fixed_grid, v, err);
+int decode_view(const PlanConfig& cfg, bool keys, const std::vector<Unit>& units, int ctas,
+                bool fixed_grid, View& v, std::string& err) {
+  if (!keys) return build_cut_view(cfg, units, ctas, cfg.dec_min_tiles, fixed_grid, v, err);
   PlanConfig c = cfg;
-  c.row_tile = 1;
+  c.row_tile = c.row_weight[0] = 1;
   c.row_item_tiles = kKeyItem;
   c.row_pair_blocks = 0;
   c.row_min_piece = cfg.dec_min_tiles;
-  return build_cost_view(c, units, cfg.dec_grid_cap, fixed_grid, v, err);
+  return build_cost_view(c, units, ctas, fixed_grid, v, err);
 }
 
 // views: 0 and 1 the row list without and with the mask, 2 the decode list.
@@ -217,11 +226,36 @@ int layout(const PlanConfig& cfg, bool keys, const std::vector<SeqInfo>& step, c
     if (m.own_unit >= 0 && m.own_blocks == 0) m.own_unit += row_units;
     if (m.pre_unit >= 0 && m.pre_blocks == 0) m.pre_unit += row_units;
   }
+  // Both kinds of work: the kernels run side by side, each on SMs of its own, the
+  // row list's on as many as let both end together (it is bound by the tensor
+  // pipe, the key kernel by memory, which a part of the SMs fills too).
+  int row_sms = cfg.grid_cap, key_ctas = cfg.dec_grid_cap;
+  if (keys && !full.empty() && !key.empty() && cfg.grid_cap > 1) {
+    double row_us = 0, key_us = 0, key_bytes = 0;
+    for (const Unit& u : full)
+      row_us += (ceil_div(u.tiles, cfg.row_tile) *
+                     cfg.row_weight[u.nrb > cfg.row_pair_blocks] + cfg.row_item_tiles) / 5.0;
+    for (const Unit& u : key) {
+      key_us += u.tiles * kKeyTileUs + kKeyItemUs;
+      key_bytes += double(u.tiles) * kTileTokens * cfg.dim * 4;
+    }
+    const int per_sm = cfg.dec_grid_cap / cfg.grid_cap;
+    double best = 1e30;
+    for (int n = 1; n < cfg.grid_cap; ++n) {
+      const int m = cfg.grid_cap - n;
+      const double t = std::max(
+          row_us / n, std::max(key_us / (m * per_sm), key_bytes / (kHbmGbs * 1e3)));
+      if (t < best) {
+        best = t;
+        row_sms = n;
+        key_ctas = m * per_sm;
+      }
+    }
+  }
   View views[3];
-  int rc = build_cost_view(cfg, full, cfg.grid_cap, fixed_grid, views[0], err);
-  if (rc == FE_OK) rc = build_cost_view(cfg, causal, cfg.grid_cap, fixed_grid, views[1], err);
-  if (rc == FE_OK)
-    rc = decode_view(cfg, keys, key, fixed_grid, views[2], err);
+  int rc = build_cost_view(cfg, full, row_sms, fixed_grid, views[0], err);
+  if (rc == FE_OK) rc = build_cost_view(cfg, causal, row_sms, fixed_grid, views[1], err);
+  if (rc == FE_OK) rc = decode_view(cfg, keys, key, key_ctas, fixed_grid, views[2], err);
   if (rc != FE_OK) return rc;
   fill_rows(t, rows, G);
   return pack(cfg, keys, views, t, pages, total_pages, batch, rows, out, err);
@@ -261,7 +295,7 @@ int build_shared_plan(const PlanConfig& cfg, bool keys, const int32_t* qo, const
       return FE_ERR_INVALID_ARGUMENT;
     }
     Group x{first, end, shared[g], 0};
-    int64_t blocks = 0;  // items that read the prefix when it is not shared
+    double apart = 0;  // a tile of the prefix when it is not shared
     int members = 0;
     for (int b = first; b < end; ++b) {
       if (shared[g] > kv[b + 1] - kv[b] ||
@@ -276,15 +310,16 @@ int build_shared_plan(const PlanConfig& cfg, bool keys, const int32_t* qo, const
       // least) stay out
       x.pages = std::min(x.pages, (s.length - s.qrows) / cfg.page);
       ++members;
-      blocks += ceil_div(int64_t(s.qrows) * G, kRowTile);
+      apart += tile_us(cfg, int64_t(s.qrows) * G);
     }
     const int64_t PP = int64_t(x.rows) * G;
-    const int64_t saved = (blocks - ceil_div(PP, kRowTile)) * x.pages *
-                          (cfg.page / kTileTokens) * cfg.hkv;
-    if (members < 2 || saved < (PP <= kRowBlock ? kShareDecode : kShareRows))
+    const double tiles = double(x.pages) * cfg.page / 128 * cfg.hkv;
+    const double records = 4.0 * PP * cfg.hkv * cfg.dim * sizeof(float) / (kRecordGbs * 1e3);
+    const double launch = PP > kRowBlock ? kLaunchUs * cfg.grid_cap : 0;
+    if (members < 2 || tile_us(cfg, PP) * tiles + records + launch >= apart * tiles)
       x.pages = 0;
     else
-      saved_total += saved;
+      saved_total += int64_t(members - 1) * x.pages * (cfg.page / kTileTokens) * cfg.hkv;
     gs.push_back(x);
   }
   const int total_pages = batch > 0 ? kv[batch] : 0;
@@ -357,7 +392,7 @@ int build_scored_plan(const PlanConfig& cfg, bool keys, const int32_t* qo, const
     return FE_ERR_CAPACITY;
   }
   View views[3];
-  rc = decode_view(cfg, keys, key, fixed_grid, views[2], err);
+  rc = decode_view(cfg, keys, key, cfg.dec_grid_cap, fixed_grid, views[2], err);
   if (rc != FE_OK) return rc;
   fill_rows(t, rows, G);
   return pack(cfg, keys, views, t, pages, batch > 0 ? kv[batch] : 0, batch, rows, out, err);

@@ -17,9 +17,10 @@
 // so that one group exponentiates while the other's products run.
 //  * An item of more than 128 rows (up to 256) gives each stream 128 of them;
 //    every K and V tile is loaded once for both.
-//  * An item of up to 128 rows gives both streams the same rows and alternate
-//    key tiles; at its end the streams' states are joined: both groups read both
-//    O's (warps q and q + 4 own the same TMEM lanes), each half of the dims.
+//  * An item of up to 128 rows gives both streams the same rows and each half of
+//    every tile's keys; at its end the streams' states are joined: both groups
+//    read both O's (warps q and q + 4 own the same TMEM lanes), each half of the
+//    dims.
 // A 256-row item's 128-key tile costs 2 S and 4 P V products of 128 x 128 x 128,
 // about 3100 cycles of the tensor pipe; a group's softmax of a tile (16384
 // exponentials on one SM's 16 a cycle, packed arithmetic beside them) hides
@@ -118,19 +119,14 @@ __device__ __forceinline__ bool elect_one() {
   return p != 0;
 }
 
-// What all roles derive from an item.
+// What all roles derive from an item. A stream walks it in steps of 64 keys: both
+// halves of every tile of a pair, else the stream's half of every tile.
 struct Shape {
   int pieces, tiles;
-  bool pair;  // two row tiles (else one, its key tiles dealt to the streams)
+  bool pair;  // two row tiles
   __device__ __forceinline__ explicit Shape(const WorkItem& w)
       : pieces(w.kt1 - w.kt0), tiles((pieces + kPieces - 1) / kPieces),
         pair(w.nrb * kRowBlock > kM) {}
-  __device__ __forceinline__ int count(int stream) const {  // key tiles of a stream
-    return pair ? tiles : (tiles + 1 - stream) / 2;
-  }
-  __device__ __forceinline__ int key_tile(int stream, int j) const {
-    return pair ? j : 2 * j + stream;
-  }
 };
 
 template <typename T>
@@ -146,7 +142,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* k_empty = k_full + kKStages;
   uint64_t* v_full = k_empty + kKStages;
   uint64_t* v_empty = v_full + kVStages;
-  // [stream * 2 + half of the tile]
+  // [stream * 2 + slot]: a stream's steps take its two slots in turn
   uint64_t* s_full = v_empty + kVStages;  // S written
   uint64_t* pv_done = s_full + 4;         // P V done
   uint64_t* p_full = pv_done + 4;          // P written, O rescaled
@@ -157,7 +153,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kBars);
   volatile int* flags = reinterpret_cast<volatile int*>(tmem_slot + 2);
 
-  pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const MetaHeader* hdr = reinterpret_cast<const MetaHeader*>(a.meta);
   const int view = a.view;
@@ -183,7 +178,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) {
     for (int b = 0; b < 2; ++b) {
       mbar_init(&q_full[b], 1);
-      mbar_init(&q_empty[b], 2);  // as k_empty and v_empty: see the issuers
+      mbar_init(&q_empty[b], 2);  // as k_empty and v_empty: one commit per stream
       for (int h = 2 * b; h < 2 * b + 2; ++h) {
         mbar_init(&s_full[h], 1);
         mbar_init(&pv_done[h], 1);
@@ -216,6 +211,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = *tmem_slot;
   bool aborted = false;
   pdl_wait();  // q and the pools belong to earlier kernels until here
+  // Only now: the key kernel, launched behind this one, starts beside it on the SMs
+  // that this grid leaves free, and so behind whatever this grid has waited for.
+  pdl_trigger();
 
   if (warp >= 8) {
     if (warp == kKWarp || warp == kVWarp) {
@@ -339,10 +337,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       // A warp walks its stream's schedule whole and one elected thread issues:
       // descriptors and counters then stay in uniform registers (issued by one thread
       // under `lane == 0`, eight products took 700 to 1200 cycles of moving
-      // descriptors where they run for 512). A step is the P V product of a half tile
-      // and the S of the same half of the next tile behind it, whose slot it frees:
-      // MMAs of one thread execute in order. All that a step waits for is polled at
-      // once, a barrier a lane.
+      // descriptors where they run for 512). An event is the P V product of a step and,
+      // behind it, the S of the step after the next, in the slot that it frees: MMAs of
+      // one thread execute in order. All that an event waits for is polled at once, a
+      // barrier a lane. Both streams wait for every Q, K and V tile and both release
+      // it, whoever reads it: a barrier that a warp waits for is then never more than
+      // one phase ahead of or behind it, which a wait by parity needs.
       const int i = warp - kMmaWarp;
       constexpr uint32_t idesc_s = tc::idesc_f16(Fmt<T>::v, false, false, kM, kHalf);
       constexpr uint32_t idesc_o = tc::idesc_f16(Fmt<T>::v, false, true, kM, kD);
@@ -356,55 +356,52 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t tm = uniform(tmem);
       const uint32_t s_col = tm + i * kN, o_col = tm + kOCol + i * kD;
       const int i0 = uniform(it0), i1 = uniform(it1);
-      uint32_t base = 0, qn = 0, done = 0;  // tiles, Q tiles and tiles of the stream before the item
+      uint32_t base = 0, qn = 0, gs = 0;  // tiles, Q tiles and steps before the item
       int unit = 0;
       for (int it = i0; it < i1 && !aborted; ++it, ++unit) {
         const Shape loaded(items[it]);
         const int tiles = uniform(loaded.tiles);
-        const bool pair = uniform(loaded.pair ? 1 : 0) != 0;
-        const int n = pair ? tiles : (tiles + 1 - i) / 2;
-        const uint32_t qt = qn + (pair ? i : 0), qb = qt % kQBufs;
+        const int pair = uniform(loaded.pair ? 1 : 0);
+        const int steps = tiles << pair;
+        const uint32_t qb = (qn + (pair ? i : 0)) % kQBufs;
         const uint64_t q_desc = q_desc0 + uint64_t((qb * kQBytes) >> 4);
-        // K and V stages are free behind both streams' products, or this one's twice; a Q
-        // tile behind the last S of the one stream or of both
-        const int arrivals = pair ? 1 : 2, q_arrivals = pair || tiles == 1 ? 2 : 1;
 #pragma unroll 1
-        for (int step = -2; step < 2 * n; ++step) {
-          if (n == 0) break;
-          const int half = step & 1, j = step < 0 ? -1 : step >> 1;
-          const bool next = j + 1 < n;
-          const uint32_t vg = base + (pair ? j : 2 * j + i), vst = vg % kVStages;
-          const uint32_t kg = base + (pair ? j + 1 : 2 * (j + 1) + i), kst = kg % kKStages;
-          uint64_t* bar;
-          uint32_t parity;
-          if (j < 0) {  // the item's first S
-            bar = lane == 1 ? &q_full[qb] : &k_full[kst];
-            parity = lane == 1 ? (qt / kQBufs) & 1u : (kg / kKStages) & 1u;
-          } else {
-            bar = &p_full[2 * i + half];
-            parity = (done + j) & 1u;
-            if (lane == 1) {
-              bar = &v_full[vst];
-              parity = (vg / kVStages) & 1u;
-            } else if (lane == 2 && next) {
-              bar = &k_full[kst];
-              parity = (kg / kKStages) & 1u;
-            } else if (lane == 3 && unit > 0) {
-              // O belongs to the softmax groups until they have stored the last item
-              bar = &o_free[i];
-              parity = (unit - 1) & 1u;
+        for (int e = -2; e < steps; ++e) {
+          const bool next = e + 2 < steps;
+          const uint32_t g = gs + e + 2, slot = g & 1u;  // of the step e + 2, and of e
+          const uint32_t vg = base + (e >> pair), vst = vg % kVStages;
+          const uint32_t kg = base + ((e + 2) >> pair), kst = kg % kKStages;
+          const int vhalf = pair ? e & 1 : i;  // a pair's steps e and e + 2: the same half
+          uint64_t* bar = &k_full[kst];
+          uint32_t parity = (kg / kKStages) & 1u;
+          if (e < 0) {  // the item's first two S
+            if (!next) continue;
+            if (lane >= 1 && lane <= 1 + pair) {
+              const uint32_t qt = qn + lane - 1;
+              bar = &q_full[qt % kQBufs];
+              parity = (qt / kQBufs) & 1u;
             }
+          } else if (lane == 1) {
+            bar = &v_full[vst];
+            parity = (vg / kVStages) & 1u;
+          } else if (lane == 2 && unit > 0) {
+            // O belongs to the softmax groups until they have stored the last item
+            bar = &o_free[i];
+            parity = (unit - 1) & 1u;
+          } else if (lane != 3 || !next) {
+            bar = &p_full[2 * i + slot];
+            parity = ((g - 2) >> 1) & 1u;
           }
           if (!wait_warp(bar, parity, flags, aborted)) break;
           tc::fence_after_sync();
-          const uint32_t p_col = s_col + half * kHalf;
+          const uint32_t p_col = s_col + slot * kHalf;
           const uint64_t vh =
-              v_desc0 + uint64_t((vst * kTile + half * (kPieces / 2) * kPieceBytes) >> 4);
+              v_desc0 + uint64_t((vst * kTile + vhalf * (kPieces / 2) * kPieceBytes) >> 4);
           const uint64_t kh =
-              k_desc0 + uint64_t((kst * kTile + half * (kPieces / 2) * kPieceBytes) >> 4);
-          const uint32_t more = step > 0 ? 1u : 0u;
+              k_desc0 + uint64_t((kst * kTile + vhalf * (kPieces / 2) * kPieceBytes) >> 4);
+          const uint32_t more = e > 0 ? 1u : 0u;
           if (elect_one()) {
-            if (j >= 0) {  // O += P V of the half
+            if (e >= 0) {  // O += P V of the step
 #pragma unroll
               for (int part = 0; part < 2; ++part)
 #pragma unroll
@@ -412,32 +409,30 @@ __global__ void __launch_bounds__(kThreads, 1)
                   tc::mma_f16_ts(o_col, p_col + part * (kHalf / 2) + kk * 8,
                                  vh + uint64_t((kk * kPieceBytes) >> 4), idesc_o,
                                  part + kk == 0 ? more : 1u);
-              tc::commit(&pv_done[2 * i + half]);
-              if (half == 1) {
-                for (int x = 0; x < arrivals; ++x) tc::commit(&v_empty[vst]);
-                if (!next) tc::commit(&o_full[i]);
-              }
+              tc::commit(&pv_done[2 * i + slot]);
+              if (!pair || vhalf) tc::commit(&v_empty[vst]);
+              if (e + 1 == steps) tc::commit(&o_full[i]);
             }
-            if (next) {  // S of the half of the next tile
+            if (next) {  // S of the step after the next
 #pragma unroll
               for (int kk = 0; kk < kD / 16; ++kk) {
                 const int box = kk >> 2, ko = (kk & 3) * 32;
                 tc::mma_f16(p_col, q_desc + uint64_t((box * kQBox + ko) >> 4),
                             kh + uint64_t((box * 1024 + ko) >> 4), idesc_s, kk > 0 ? 1u : 0u);
               }
-              tc::commit(&s_full[2 * i + half]);
-              if (half == 1) {
-                for (int x = 0; x < arrivals; ++x) tc::commit(&k_empty[kst]);
-                if (j + 2 == n)
-                  for (int x = 0; x < q_arrivals; ++x) tc::commit(&q_empty[qb]);
+              tc::commit(&s_full[2 * i + slot]);
+              if (!pair || vhalf) tc::commit(&k_empty[kst]);
+              if (e + 3 == steps) {
+                tc::commit(&q_empty[qn % kQBufs]);
+                if (pair) tc::commit(&q_empty[(qn + 1) % kQBufs]);
               }
             }
           }
           __syncwarp();
         }
         base += tiles;
-        qn += pair ? 2 : 1;
-        done += n;
+        qn += 1 + pair;
+        gs += steps;
       }
       if (aborted && lane == 0) raise_device_error(a.err, FE_DEVERR_TIMEOUT);
       // TMEM is released only after every MMA issued here has completed.
@@ -454,9 +449,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t s_addr = lane_addr + gi * kN;
     const uint32_t o_addr = lane_addr + kOCol + gi * kD;
     const int G = a.G;
-    uint32_t base = 0, ns = 0;           // tiles of earlier items, of the stream's
-    uint32_t no[2] = {0, 0}, nx = 0;     // items that used each O, that joined the streams
-    for (int it = it0; it < it1 && !aborted; ++it) {
+    uint32_t base = 0, gs = 0, nx = 0;  // tiles, steps and joined items before this one
+    int unit = 0;
+    for (int it = it0; it < it1 && !aborted; ++it, ++unit) {
       const WorkItem w = items[it];
       const SeqInfo si = seqs[w.seq];
       const Shape sh(w);
@@ -471,15 +466,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       lim = min(lim, w.kt1 * kTileTokens);
       // m stays -inf until the first unmasked key (its weights are 0)
       float m = -INFINITY, l = 0.f;
-      const int n = sh.count(gi);
+      const int steps = sh.tiles << (sh.pair ? 1 : 0);
 #pragma unroll 1
-      for (int step = 0; step < 2 * n; ++step) {
-        const int half = step & 1, kt = sh.key_tile(gi, step >> 1);
-        const uint32_t c = ns + (step >> 1);  // the stream's tile
+      for (int step = 0; step < steps; ++step) {
+        const uint32_t g = gs + step, slot = g & 1u;
+        const int kt = sh.pair ? step >> 1 : step, half = sh.pair ? step & 1 : gi;
         const int t0 = (w.kt0 + kPieces * kt) * kTileTokens + half * kHalf;
-        if (!wait_warp(&s_full[2 * gi + half], c & 1u, flags, aborted)) break;
+        if (!wait_warp(&s_full[2 * gi + slot], (g >> 1) & 1u, flags, aborted)) break;
         tc::fence_after_sync();
-        const uint32_t half_addr = s_addr + half * kHalf;
+        const uint32_t half_addr = s_addr + slot * kHalf;
         float s[kHalf];
 #pragma unroll
         for (int x = 0; x < kHalf; x += 32)
@@ -511,8 +506,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (step > 0) {
             // the P V before this one has completed (its slot's earlier one had before this
             // slot's S: the barrier is at most one phase short)
-            const uint32_t cp = half ? c : c - 1;
-            if (!wait_warp(&pv_done[2 * gi + (half ^ 1)], cp & 1u, flags, aborted)) break;
+            if (!wait_warp(&pv_done[2 * gi + (slot ^ 1)], ((g - 1) >> 1) & 1u, flags, aborted))
+              break;
             tc::fence_after_sync();
 #pragma unroll 1
             for (int c2 = 0; c2 < kD / 16; ++c2) {
@@ -572,11 +567,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc::wait_st();
         tc::fence_before_sync();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[2 * gi + half]);
+        if (lane == 0) mbar_arrive(&p_full[2 * gi + slot]);
         l += ((l4[0].x + l4[0].y) + (l4[1].x + l4[1].y)) +
              ((l4[2].x + l4[2].y) + (l4[3].x + l4[3].y));
       }
-      ns += n;
+      gs += steps;
       if (aborted) break;
       base += sh.tiles;
       const int rows_rec = min(P - p0, w.nrb * kRowBlock);
@@ -604,9 +599,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       };
       if (sh.pair) {
-        if (!wait_warp(&o_full[gi], no[gi] & 1u, flags, aborted)) break;
-        ++no[0];
-        ++no[1];
+        if (!wait_warp(&o_full[gi], unit & 1u, flags, aborted)) break;
         tc::fence_after_sync();
         if (rec && row_valid) {
           rec[rows_rec * kD + (p - p0)] = m;
@@ -626,13 +619,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       } else {
         // join the streams: (m, l) through shared memory, then each group half of the
         // dims of both O's
-        const bool two = sh.tiles > 1;
-        if (!wait_warp(&o_full[0], no[0] & 1u, flags, aborted)) break;
-        ++no[0];
-        if (two) {
-          if (!wait_warp(&o_full[1], no[1] & 1u, flags, aborted)) break;
-          ++no[1];
-        }
+        if (!wait_warp(&o_full[gi], unit & 1u, flags, aborted)) break;
         // (the next item's write comes behind its o_full, which comes behind both
         // groups' o_free of this item: nobody still reads)
         float* x = reinterpret_cast<float*>(smem + kOffX);
@@ -641,11 +628,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_arrive(x_full);
         if (!wait_warp(x_full, nx & 1u, flags, aborted)) break;
         ++nx;
+        // (the other group has seen its stream's end: the phase is complete)
+        if (!wait_warp(&o_full[gi ^ 1], unit & 1u, flags, aborted)) break;
         tc::fence_after_sync();
         const float m0 = x[r], l0 = x[kM + r], m1 = x[2 * kM + r], l1 = x[3 * kM + r];
         const float mj = fmaxf(m0, m1), mb = mj == -INFINITY ? 0.f : mj;
-        const float f0 = fast_exp2(m0 - mb), f1 = two ? fast_exp2(m1 - mb) : 0.f;
-        const float lj = l0 * f0 + (two ? l1 * f1 : 0.f);
+        const float f0 = fast_exp2(m0 - mb), f1 = fast_exp2(m1 - mb);
+        const float lj = l0 * f0 + l1 * f1;
         if (rec && row_valid && gi == 0) {
           rec[rows_rec * kD + r] = mj;
           rec[rows_rec * (kD + 1) + r] = lj;
@@ -657,16 +646,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           float o[32];
           tc::ld_32x32b_x32(lane_addr + kOCol + dim0, *reinterpret_cast<uint32_t(*)[32]>(&o[0]));
           tc::wait_ld();
+          float o1[32];
+          tc::ld_32x32b_x32(lane_addr + kOCol + kD + dim0,
+                            *reinterpret_cast<uint32_t(*)[32]>(&o1[0]));
+          tc::wait_ld();
 #pragma unroll
-          for (int c = 0; c < 32; ++c) o[c] *= f0;
-          if (two) {
-            float o1[32];
-            tc::ld_32x32b_x32(lane_addr + kOCol + kD + dim0,
-                              *reinterpret_cast<uint32_t(*)[32]>(&o1[0]));
-            tc::wait_ld();
-#pragma unroll
-            for (int c = 0; c < 32; ++c) o[c] = fmaf(o1[c], f1, o[c]);
-          }
+          for (int c = 0; c < 32; ++c) o[c] = o[c] * f0 + o1[c] * f1;
           store32(dim0, o, inv);
         }
         tc::fence_before_sync();

@@ -496,7 +496,7 @@ int fe_scored_attn_run(fe_long_plan* plan, const void* q, const void* k_pool, co
 typedef struct fe_long_plan_info {
   int rows, shared_groups;   /* groups whose prefix is read once */
   int row_ctas, decode_ctas; /* CTAs of the two kernels (causal) */
-  int64_t shared_tiles;      /* 16-key tiles (x KV heads) that sharing saves */
+  int64_t shared_tiles;      /* 16-key tiles (x KV heads) that sharing saves reading */
   int64_t partial_floats, weight_floats;
 } fe_long_plan_info;
 int fe_long_plan_get_info(const fe_long_plan* plan, fe_long_plan_info* info);

@@ -66,6 +66,11 @@ LAYOUTS = {
     "three": [(20, ones(*[7] * 40)), (40, ones(*range(3, 40))), (1, ones(2, 9))],
     # draft blocks of several rows, some of them long; one member without rows
     "drafts": [(30, [(4, 4)] * 9 + [(20, 3), (3, 0), (16, 16)] + [(5, 5)] * 8)],
+    # verification blocks: items of one and of two row tiles, of one and of several
+    # key tiles, one behind the other on an SM
+    "blocks": [(70, [(16 + 23 * i % 300, 16) for i in range(40)]),
+               (0, [(200, 40), (333, 9), (90, 20), (17, 17)]),
+               (33, [(64 + i, 33) for i in range(0, 300, 17)])],
     # a prefill chunk over the prefix beside decode rows
     "chunk": [(26, [(300, 300)] + ones(*range(1, 30)))],
 }
