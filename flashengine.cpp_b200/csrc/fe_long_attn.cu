@@ -364,8 +364,8 @@ int create_long(const char* what, int hq, int hkv, int dim, int page, int max_ba
   c.row_tile = dim == kWideHeadDim ? 4 : 8;
   // measured: a 128-key tile of the two-stream kernel 2.0 us for 256 rows, 1.4 us for
   // 128; of the head_dim 256 kernel (64 keys) 1.6 us; an item about 4 us more
-  c.row_weight[0] = dim == kHeadDim ? 10 : 8;
-  c.row_weight[1] = 10;
+  c.row_weight[0] = dim == kHeadDim ? 6 : 8;
+  c.row_weight[1] = 12;
   c.row_item_tiles = 20;  // in fifths of a microsecond, as the weights
   c.row_pair_blocks = dim == kHeadDim ? 8 : 0;
   c.row_min_piece = 2;

@@ -29,7 +29,8 @@
 // One persistent CTA per SM, three warpgroups:
 //  warps 0-3, 4-7  softmax of stream 0 and 1;
 //  warps 8 / 11    producers of K (and Q) / of V: eight 16-token page pieces a
-//                  tile, one TMA box each, into 3 K and 2 V stages of 32 KiB;
+//                  tile, one TMA box each, into 2 K and 2 V stages of 32 KiB (S runs two steps
+//                  ahead, so that a K stage is refilled two before it is read);
 //  warps 9 / 10    issue of a stream's S and P V products (one elected thread
 //                  each); warp 9 owns the TMEM.
 // All hand-offs are mbarriers; every wait is bounded.
@@ -50,7 +51,7 @@ constexpr int kM = 128;  // rows of a stream
 constexpr int kN = 128;  // keys of a tile
 constexpr int kHalf = kN / 2;
 constexpr int kPieces = kN / kTileTokens;
-constexpr int kKStages = 3, kVStages = 2, kQBufs = 2;
+constexpr int kKStages = 2, kVStages = 2, kQBufs = 2;
 constexpr int kThreads = 12 * 32;
 constexpr int kKWarp = 8, kMmaWarp = 9, kVWarp = 11;  // MMA: 9 and 10, a stream each
 constexpr int kBoxes = kD / 64;
@@ -61,7 +62,8 @@ constexpr int kGroupBytes = 8 * kD * 2;
 constexpr int kTile = kPieces * kPieceBytes;  // 32 KiB
 constexpr int kOffK = kQBufs * kQBytes;
 constexpr int kOffV = kOffK + kKStages * kTile;
-constexpr int kOffX = kOffV + kVStages * kTile;  // [stream][m, l][row]
+constexpr int kOffOut = kOffV + kVStages * kTile;  // [softmax warp][32 rows][128 B]
+constexpr int kOffX = kOffOut + 8 * 4096;         // [stream][m, l][row]
 constexpr int kOffBar = kOffX + 2 * 2 * kM * 4;
 // q_full[2], q_empty[2], k_full[3], k_empty[3], v_full[2], v_empty[2],
 // s_full[2][2], pv_done[2][2], p_full[2][2], o_full[2], o_free[2], x_full, drain
@@ -94,18 +96,47 @@ __device__ __forceinline__ float2 hi_as_float<__half>(uint32_t h) {
   return unpack2<__half>(h);
 }
 
+// Bounded wait of a whole warp, a barrier a lane (shared-memory addresses):
+// false when one did not complete within kWaitLimitNs, or another warp gave up,
+// so that every warp of the CTA winds down. Time is looked at every 4096 polls
+// only: a poll that fails suspends the warp for a while anyway.
+__device__ __forceinline__ bool poll(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
+__device__ __noinline__ bool give_up(uint64_t& since, volatile int* flags) {
+  const uint64_t now = global_ns();
+  if (since == 0) since = now;
+  if (now - since > kWaitLimitNs) *flags = 1;
+  return __any_sync(0xffffffffu, *flags != 0);
+}
+
+__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, volatile int* flags,
+                                          bool& aborted) {
+  uint64_t since = 0;
+  uint32_t n = 0;
+  while (!__all_sync(0xffffffffu, poll(bar, parity))) {
+    if ((++n & 4095u) == 0 && give_up(since, flags)) {
+      aborted = true;
+      return false;
+    }
+  }
+  return true;
+}
+
+// Bounded wait of one thread.
 __device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, volatile int* flags,
                                               bool& aborted) {
   if (aborted) return false;
   if (!wait_bounded_short(bar, parity, flags)) aborted = true;
-  return !aborted;
-}
-
-// Warp-uniform wait (the tcgen05.ld / st that follow need the whole warp).
-__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, volatile int* flags,
-                                          bool& aborted) {
-  wait_or_abort(bar, parity, flags, aborted);
-  if (__any_sync(0xffffffffu, aborted)) aborted = true;
   return !aborted;
 }
 
@@ -152,6 +183,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* drain = x_full + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kBars);
   volatile int* flags = reinterpret_cast<volatile int*>(tmem_slot + 2);
+  auto at = [&](const uint64_t* bar) { return smem_u32(bar); };
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const MetaHeader* hdr = reinterpret_cast<const MetaHeader*>(a.meta);
@@ -355,6 +387,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint64_t v_desc0 = tc::smem_desc_sw128(smem_u32(smem + kOffV), 1024, kGroupBytes);
       const uint32_t tm = uniform(tmem);
       const uint32_t s_col = tm + i * kN, o_col = tm + kOCol + i * kD;
+      const uint32_t b_qf = at(q_full), b_kf = at(k_full), b_vf = at(v_full),
+                     b_of = at(o_free + i), b_pf = at(p_full + 2 * i);
       const int i0 = uniform(it0), i1 = uniform(it1);
       uint32_t base = 0, qn = 0, gs = 0;  // tiles, Q tiles and steps before the item
       int unit = 0;
@@ -372,24 +406,24 @@ __global__ void __launch_bounds__(kThreads, 1)
           const uint32_t vg = base + (e >> pair), vst = vg % kVStages;
           const uint32_t kg = base + ((e + 2) >> pair), kst = kg % kKStages;
           const int vhalf = pair ? e & 1 : i;  // a pair's steps e and e + 2: the same half
-          uint64_t* bar = &k_full[kst];
+          uint32_t bar = b_kf + 8 * kst;
           uint32_t parity = (kg / kKStages) & 1u;
           if (e < 0) {  // the item's first two S
             if (!next) continue;
             if (lane >= 1 && lane <= 1 + pair) {
               const uint32_t qt = qn + lane - 1;
-              bar = &q_full[qt % kQBufs];
+              bar = b_qf + 8 * (qt % kQBufs);
               parity = (qt / kQBufs) & 1u;
             }
           } else if (lane == 1) {
-            bar = &v_full[vst];
+            bar = b_vf + 8 * vst;
             parity = (vg / kVStages) & 1u;
           } else if (lane == 2 && unit > 0) {
             // O belongs to the softmax groups until they have stored the last item
-            bar = &o_free[i];
+            bar = b_of;
             parity = (unit - 1) & 1u;
           } else if (lane != 3 || !next) {
-            bar = &p_full[2 * i + slot];
+            bar = b_pf + 8 * slot;
             parity = ((g - 2) >> 1) & 1u;
           }
           if (!wait_warp(bar, parity, flags, aborted)) break;
@@ -472,7 +506,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t g = gs + step, slot = g & 1u;
         const int kt = sh.pair ? step >> 1 : step, half = sh.pair ? step & 1 : gi;
         const int t0 = (w.kt0 + kPieces * kt) * kTileTokens + half * kHalf;
-        if (!wait_warp(&s_full[2 * gi + slot], (g >> 1) & 1u, flags, aborted)) break;
+        if (!wait_warp(at(&s_full[2 * gi + slot]), (g >> 1) & 1u, flags, aborted)) break;
         tc::fence_after_sync();
         const uint32_t half_addr = s_addr + slot * kHalf;
         float s[kHalf];
@@ -506,7 +540,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (step > 0) {
             // the P V before this one has completed (its slot's earlier one had before this
             // slot's S: the barrier is at most one phase short)
-            if (!wait_warp(&pv_done[2 * gi + (slot ^ 1)], ((g - 1) >> 1) & 1u, flags, aborted))
+            if (!wait_warp(at(&pv_done[2 * gi + (slot ^ 1)]), ((g - 1) >> 1) & 1u, flags, aborted))
               break;
             tc::fence_after_sync();
 #pragma unroll 1
@@ -531,7 +565,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (valid < kHalf) {
           const uint32_t vg = base + kt;
           const int st = vg % kVStages;
-          if (!wait_warp(&v_full[st], (vg / kVStages) & 1u, flags, aborted)) break;
+          if (!wait_warp(at(&v_full[st]), (vg / kVStages) & 1u, flags, aborted)) break;
           uint8_t* vb = smem + kOffV + st * kTile;
           const int r0 = max(valid, 0), nch = (kHalf - r0) * 8;  // 16-byte chunks per box
 #pragma unroll 1
@@ -576,30 +610,59 @@ __global__ void __launch_bounds__(kThreads, 1)
       base += sh.tiles;
       const int rows_rec = min(P - p0, w.nrb * kRowBlock);
       float* rec = w.part >= 0 ? a.partials + w.part : nullptr;
-      T* out_row = a.out + (static_cast<int64_t>(si.q_row0 + p / G) * a.hq + w.kvh * G + p % G) * kD;
-      // 32 dims of this row: to the output (times `f`) or, unscaled, to the record
-      auto store32 = [&](int dim0, const float (&o)[32], float f) {
-        if (!row_valid) return;
-        if (rec) {
-          float* dst = rec + static_cast<int64_t>(p - p0) * kD + dim0;
+      // What a thread holds of its row, 128 bytes at `x`, goes through shared memory (16-
+      // byte chunks swizzled by the row), so that a store of the warp covers whole
+      // lines of four rows and not a piece of 32 (5 us an item before). `dst` is row 0's
+      // place of the warp; rows [0, live) are stored.
+      uint8_t* stage = smem + kOffOut + warp * 4096;
+      const int wrow0 = p0 + (sh.pair ? gi * kM : 0) + quad * 32;  // the warp's first packed row
+      const int live = min(32, P - wrow0);
+      auto put = [&](const uint4 (&x)[8], auto&& dst) {
+        __syncwarp();
 #pragma unroll
-          for (int v = 0; v < 8; ++v)
-            *reinterpret_cast<float4*>(dst + 4 * v) =
-                make_float4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
-          return;
+        for (int v = 0; v < 8; ++v)
+          *reinterpret_cast<uint4*>(stage + lane * 128 + ((v ^ (lane & 7)) << 4)) = x[v];
+        __syncwarp();
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          const int row = 4 * q + (lane >> 3), c = lane & 7;
+          const uint4 y =
+              *reinterpret_cast<const uint4*>(stage + row * 128 + ((c ^ (row & 7)) << 4));
+          if (row < live) *reinterpret_cast<uint4*>(dst(row) + c * 16) = y;
         }
+      };
+      // Dims dim0 .. +31, unscaled, to the record.
+      auto put_record = [&](int dim0, const float (&o)[32]) {
+        uint4 x[8];
+#pragma unroll
+        for (int v = 0; v < 8; ++v)
+          x[v] = make_uint4(__float_as_uint(o[4 * v]), __float_as_uint(o[4 * v + 1]),
+                            __float_as_uint(o[4 * v + 2]), __float_as_uint(o[4 * v + 3]));
+        put(x, [&](int row) {
+          return reinterpret_cast<uint8_t*>(
+              rec + static_cast<int64_t>(wrow0 - p0 + row) * kD + dim0);
+        });
+      };
+      // Dims dim0 .. +63 in 16 bits to the output.
+      auto put_out = [&](int dim0, const uint4 (&x)[8]) {
+        put(x, [&](int row) {
+          const int pr = wrow0 + row;
+          return reinterpret_cast<uint8_t*>(
+              a.out + (static_cast<int64_t>(si.q_row0 + pr / G) * a.hq + w.kvh * G + pr % G) * kD +
+              dim0);
+        });
+      };
+      auto pack32 = [&](const float (&o)[32], float f, uint4* x) {
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
-          uint4 pk;
-          pk.x = pack2<T>(o[8 * v + 0] * f, o[8 * v + 1] * f);
-          pk.y = pack2<T>(o[8 * v + 2] * f, o[8 * v + 3] * f);
-          pk.z = pack2<T>(o[8 * v + 4] * f, o[8 * v + 5] * f);
-          pk.w = pack2<T>(o[8 * v + 6] * f, o[8 * v + 7] * f);
-          *reinterpret_cast<uint4*>(out_row + dim0 + 8 * v) = pk;
+          x[v].x = pack2<T>(o[8 * v + 0] * f, o[8 * v + 1] * f);
+          x[v].y = pack2<T>(o[8 * v + 2] * f, o[8 * v + 3] * f);
+          x[v].z = pack2<T>(o[8 * v + 4] * f, o[8 * v + 5] * f);
+          x[v].w = pack2<T>(o[8 * v + 6] * f, o[8 * v + 7] * f);
         }
       };
       if (sh.pair) {
-        if (!wait_warp(&o_full[gi], unit & 1u, flags, aborted)) break;
+        if (!wait_warp(at(&o_full[gi]), unit & 1u, flags, aborted)) break;
         tc::fence_after_sync();
         if (rec && row_valid) {
           rec[rows_rec * kD + (p - p0)] = m;
@@ -607,11 +670,20 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         const float inv = 1.f / l;
 #pragma unroll 1
-        for (int c2 = 0; c2 < kD / 32; ++c2) {
-          float o[32];
-          tc::ld_32x32b_x32(o_addr + c2 * 32, *reinterpret_cast<uint32_t(*)[32]>(&o[0]));
-          tc::wait_ld();
-          store32(c2 * 32, o, inv);
+        for (int c2 = 0; c2 < kD / 64; ++c2) {
+          uint4 x[8];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float o[32];
+            tc::ld_32x32b_x32(o_addr + c2 * 64 + h * 32,
+                              *reinterpret_cast<uint32_t(*)[32]>(&o[0]));
+            tc::wait_ld();
+            if (rec)
+              put_record(c2 * 64 + h * 32, o);
+            else
+              pack32(o, inv, x + 4 * h);
+          }
+          if (!rec) put_out(c2 * 64, x);
         }
         tc::fence_before_sync();
         __syncwarp();
@@ -619,17 +691,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       } else {
         // join the streams: (m, l) through shared memory, then each group half of the
         // dims of both O's
-        if (!wait_warp(&o_full[gi], unit & 1u, flags, aborted)) break;
+        if (!wait_warp(at(&o_full[gi]), unit & 1u, flags, aborted)) break;
         // (the next item's write comes behind its o_full, which comes behind both
         // groups' o_free of this item: nobody still reads)
         float* x = reinterpret_cast<float*>(smem + kOffX);
         x[gi * 2 * kM + r] = m;
         x[gi * 2 * kM + kM + r] = l;
         mbar_arrive(x_full);
-        if (!wait_warp(x_full, nx & 1u, flags, aborted)) break;
+        if (!wait_warp(at(x_full), nx & 1u, flags, aborted)) break;
         ++nx;
         // (the other group has seen its stream's end: the phase is complete)
-        if (!wait_warp(&o_full[gi ^ 1], unit & 1u, flags, aborted)) break;
+        if (!wait_warp(at(&o_full[gi ^ 1]), unit & 1u, flags, aborted)) break;
         tc::fence_after_sync();
         const float m0 = x[r], l0 = x[kM + r], m1 = x[2 * kM + r], l1 = x[3 * kM + r];
         const float mj = fmaxf(m0, m1), mb = mj == -INFINITY ? 0.f : mj;
@@ -640,20 +712,23 @@ __global__ void __launch_bounds__(kThreads, 1)
           rec[rows_rec * (kD + 1) + r] = lj;
         }
         const float inv = 1.f / lj;
-#pragma unroll 1
+        uint4 y[8];
+#pragma unroll
         for (int c2 = 0; c2 < 2; ++c2) {
           const int dim0 = gi * 64 + c2 * 32;
-          float o[32];
+          float o[32], o1[32];
           tc::ld_32x32b_x32(lane_addr + kOCol + dim0, *reinterpret_cast<uint32_t(*)[32]>(&o[0]));
-          tc::wait_ld();
-          float o1[32];
           tc::ld_32x32b_x32(lane_addr + kOCol + kD + dim0,
                             *reinterpret_cast<uint32_t(*)[32]>(&o1[0]));
           tc::wait_ld();
 #pragma unroll
           for (int c = 0; c < 32; ++c) o[c] = o[c] * f0 + o1[c] * f1;
-          store32(dim0, o, inv);
+          if (rec)
+            put_record(dim0, o);
+          else
+            pack32(o, inv, y + 4 * c2);
         }
+        if (!rec) put_out(gi * 64, y);
         tc::fence_before_sync();
         __syncwarp();
         if (lane == 0) {
