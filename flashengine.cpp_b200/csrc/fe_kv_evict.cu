@@ -19,13 +19,12 @@ constexpr int kSelThreads = 512;
 constexpr int kSelList = 2048;
 constexpr int kSelWarps = kSelThreads / 32;
 constexpr int kBins = 2048;
-constexpr int kSelKeys = 48 << 10;  // keys that fit in shared memory beside the histogram
+constexpr int kSelRoom = 128 << 10;  // tokens whose classes fit in shared memory
 
 // A score as an unsigned number of the same order; NaN below everything.
 __device__ __forceinline__ uint32_t ordered(float x) {
-  if (x != x) return 0;
-  const uint32_t b = __float_as_uint(x == 0.f ? 0.f : x);  // -0 and +0 tie
-  return b & 0x80000000u ? ~b : b | 0x80000000u;
+  const int b = __float_as_int(x + 0.f);  // -0 and +0 tie
+  return x != x ? 0u : static_cast<uint32_t>(b ^ ((b >> 31) | static_cast<int>(0x80000000u)));
 }
 
 struct SeqTable {
@@ -108,21 +107,24 @@ __device__ __forceinline__ int2 find_bin(const int* hist, int left, int* warp_su
 
 // One CTA per (sequence, KV head). The `want` best of the tokens between sink
 // and the recent ones are found by a radix select over their ordered scores:
-// a histogram of the first 11 bits gives the bin in which the want-th key lies,
-// the keys of that bin are listed, and two more histograms (11 and 10 bits)
-// over the list give the threshold and how many of the tokens equal to it are
-// kept, the lowest indexes first; then the kept tokens are written in order.
-// Scores are read four tokens at a time (pages are multiples of 16), the first
-// histogram on the way. The keys of a sequence of up to `room` tokens stay in
-// shared memory; a longer one's scores are read again by each pass, and so are
-// all keys where the bin has more than kSelList (equal or close scores).
-__global__ void __launch_bounds__(kSelThreads)
+// a histogram of the first 11 bits gives the bin in which the want-th key lies;
+// a second sweep over the scores notes for every token whether it is above that
+// bin and lists the keys within; two more histograms (11 and 10 bits) over the
+// list give the threshold and how many of the tokens equal to it are kept, the
+// lowest indexes first; then the kept tokens are written in order from the notes.
+// Scores are read four tokens at a time (pages are multiples of 16), each twice;
+// a note is a byte per four tokens (above the threshold, at it). A sequence of
+// more than `room` tokens is read again for the output, and so is one whose bin
+// has more than kSelList keys (equal or close scores). 64 sequences of up to 32k
+// tokens, 8 heads: 52 us, two thirds of it the longest lists' own time (75 us with
+// all keys in shared memory and one CTA an SM; with 256 or 1024 threads 79, 65).
+__global__ void __launch_bounds__(kSelThreads, 3)
     select_kernel(const float* __restrict__ scores, const SeqTable table,
                   int32_t* __restrict__ kept, int hkv, int budget, int sink, int recent, int room,
                   unsigned int* err) {
-  extern __shared__ uint32_t keys[];
+  extern __shared__ uint32_t notes32[];  // notes, four a word
   __shared__ int hist[kBins];
-  __shared__ uint32_t list[kSelList];
+  __shared__ uint2 list[kSelList];  // key, token
   __shared__ int warp_sums[kSelWarps];
   __shared__ int found[2], listed;
   pdl_trigger();
@@ -147,60 +149,73 @@ __global__ void __launch_bounds__(kSelThreads)
   for (int i = tid; i < recent; i += kSelThreads) out[budget - recent + i] = end + i;
   if (want == 0) return;
   const float* sc = scores + static_cast<int64_t>(h) * table.cache_slots;
-  const bool cached = n <= room;
+  uint8_t* notes = reinterpret_cast<uint8_t*>(notes32);
+  const bool noted = n <= room;
+  const int per16 = table.page / 16;
   // the keys of tokens 4g .. 4g + 3 (whose slots are adjacent)
   auto load4 = [&](int g) -> uint4 {
-    const int64_t slot = slot_of(table, p0, 4 * g);
-    if (slot < 0) {
+    const int blk = g >> 2, pi = per16 == 1 ? blk : blk / per16;
+    const int pg = __ldg(table.pages + p0 + pi);
+    const int64_t first = static_cast<int64_t>(pg) * table.page;
+    if (pg < 0 || first + table.page > table.cache_slots) {
       raise_device_error(err, FE_DEVERR_PAGE_RANGE);
       return make_uint4(0, 0, 0, 0);
     }
-    const float4 x = __ldg(reinterpret_cast<const float4*>(sc + slot));
+    const float4 x = __ldg(reinterpret_cast<const float4*>(sc + first + (4 * g - pi * table.page)));
     return make_uint4(ordered(x.x), ordered(x.y), ordered(x.z), ordered(x.w));
   };
-  auto key = [&](int t) -> uint32_t {
-    if (cached) return keys[t];
-    const int64_t slot = slot_of(table, p0, t);
-    return slot < 0 ? 0 : ordered(__ldg(sc + slot));
+  const int ga = sink / 4, gb = (end + 3) / 4;
+  // f(i, key) for the tokens 4g + i of a group that lie between sink and end
+  auto each = [&](int g, const uint4& x, auto&& f) {
+    const uint32_t v[4] = {x.x, x.y, x.z, x.w};
+    // (the first and the last group may lie across the bounds)
+    const int from = max(sink - 4 * g, 0), to = min(end - 4 * g, 4);
+    if (to - from == 4) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f(i, v[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (i >= from && i < to) f(i, v[i]);
+    }
   };
-  __syncthreads();
-  {
-    constexpr int kAhead = 4;
-    const int g1 = (end + 3) / 4;
-    for (int g0 = sink / 4 + tid; g0 < g1; g0 += kAhead * kSelThreads) {
+  constexpr int kAhead = 2;  // groups in flight a thread
+  auto sweep = [&](auto&& f) {
+    for (int g0 = ga + tid; g0 < gb; g0 += kAhead * kSelThreads) {
       uint4 x[kAhead];
 #pragma unroll
-      for (int u = 0; u < kAhead; ++u) {
-        const int g = g0 + u * kSelThreads;
-        if (g < g1) x[u] = load4(g);
-      }
+      for (int u = 0; u < kAhead; ++u)
+        if (g0 + u * kSelThreads < gb) x[u] = load4(g0 + u * kSelThreads);
 #pragma unroll
-      for (int u = 0; u < kAhead; ++u) {
-        const int g = g0 + u * kSelThreads;
-        if (g >= g1) break;
-        if (cached) reinterpret_cast<uint4*>(keys)[g] = x[u];
-        const uint32_t v[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (4 * g + i >= sink && 4 * g + i < end) atomicAdd(&hist[v[i] >> 21], 1);
-      }
+      for (int u = 0; u < kAhead; ++u)
+        if (g0 + u * kSelThreads < gb) f(g0 + u * kSelThreads, x[u]);
     }
-  }
+  };
+  __syncthreads();
+  sweep([&](int g, const uint4& x) {
+    each(g, x, [&](int, uint32_t k) { atomicAdd(&hist[k >> 21], 1); });
+  });
   __syncthreads();
   int2 at = find_bin(hist, want, warp_sums, found);
   uint32_t prefix = static_cast<uint32_t>(at.x) << 21;
   int left = at.y;  // of the keys that begin with prefix
+  const uint32_t bin_end = prefix | ((1u << 21) - 1);
   // ---- the rest of the threshold's bits, over the keys of its bin
   for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0;
   __syncthreads();
-  for (int t = sink + tid; t < end; t += kSelThreads) {
-    const uint32_t x = key(t);
-    if ((x >> 21) == (prefix >> 21)) {
-      atomicAdd(&hist[(x >> 10) & 2047], 1);
-      const int i = atomicAdd(&listed, 1);
-      if (i < kSelList) list[i] = x;
-    }
-  }
+  sweep([&](int g, const uint4& x) {
+    uint32_t note = 0;
+    each(g, x, [&](int i, uint32_t k) {
+      if (k > bin_end) {
+        note |= 1u << i;
+      } else if (k >= prefix) {
+        atomicAdd(&hist[(k >> 10) & 2047], 1);
+        const int at = atomicAdd(&listed, 1);
+        if (at < kSelList) list[at] = make_uint2(k, 4 * g + i);
+      }
+    });
+    if (noted) notes[g] = note;
+  });
   __syncthreads();
   const bool whole = listed <= kSelList;  // the list holds the bin
   const int count = min(listed, kSelList);
@@ -211,26 +226,46 @@ __global__ void __launch_bounds__(kSelThreads)
   __syncthreads();
   if (whole) {
     for (int i = tid; i < count; i += kSelThreads)
-      if ((list[i] >> 10) == (prefix >> 10)) atomicAdd(&hist[list[i] & 1023], 1);
+      if ((list[i].x >> 10) == (prefix >> 10)) atomicAdd(&hist[list[i].x & 1023], 1);
   } else {
-    for (int t = sink + tid; t < end; t += kSelThreads) {
-      const uint32_t x = key(t);
-      if ((x >> 10) == (prefix >> 10)) atomicAdd(&hist[x & 1023], 1);
-    }
+    sweep([&](int g, const uint4& x) {
+      each(g, x, [&](int, uint32_t k) {
+        if ((k >> 10) == (prefix >> 10)) atomicAdd(&hist[k & 1023], 1);
+      });
+    });
   }
   __syncthreads();
   at = find_bin(hist, left, warp_sums, found);
   prefix |= static_cast<uint32_t>(at.x);
   left = at.y;
-  // ---- kept tokens in order: a warp owns a stretch of the tokens
-  const int span = end - sink;
-  const int per = ((span + kSelWarps - 1) / kSelWarps + 31) / 32 * 32;
-  const int t0 = min(end, sink + warp * per), t1 = min(end, t0 + per);
+  // ---- the notes against the threshold itself: bits 0-3 above it, 4-7 at it
+  auto judge = [&](int g, const uint4& x) -> uint32_t {
+    uint32_t note = 0;
+    each(g, x, [&](int i, uint32_t k) {
+      note |= (k > prefix ? 1u : k == prefix ? 16u : 0u) << i;
+    });
+    return note;
+  };
+  if (noted && whole) {
+    for (int i = tid; i < count; i += kSelThreads) {
+      const uint2 e = list[i];
+      const uint32_t bit = (e.x > prefix ? 1u : e.x == prefix ? 16u : 0u) << (e.y & 3);
+      const int g = static_cast<int>(e.y) >> 2;
+      if (bit) atomicOr(&notes32[g >> 2], bit << (8 * (g & 3)));
+    }
+  } else if (noted) {
+    sweep([&](int g, const uint4& x) { notes[g] = judge(g, x); });
+  }
+  __syncthreads();
+  auto note_of = [&](int g) -> uint32_t { return noted ? notes[g] : judge(g, load4(g)); };
+  // ---- kept tokens in order: a warp owns a stretch of the groups
+  const int per = ((gb - ga + kSelWarps - 1) / kSelWarps + 31) / 32 * 32;
+  const int g0 = min(gb, ga + warp * per), g1 = min(gb, g0 + per);
   int gt = 0, eq = 0;
-  for (int t = t0 + lane; t < t1; t += 32) {
-    const uint32_t x = key(t);
-    gt += x > prefix;
-    eq += x == prefix;
+  for (int g = g0 + lane; g < g1; g += 32) {
+    const uint32_t note = note_of(g);
+    gt += __popc(note & 15u);
+    eq += __popc(note >> 4);
   }
 #pragma unroll
   for (int o = 16; o; o >>= 1) {
@@ -242,17 +277,30 @@ __global__ void __launch_bounds__(kSelThreads)
   int eq0 = block_scan(lane == 0 ? eq : 0, warp_sums, total);
   gt0 = __shfl_sync(0xffffffffu, gt0, 0);
   eq0 = __shfl_sync(0xffffffffu, eq0, 0);
-  const uint32_t below = (1u << lane) - 1;
-  for (int tb = t0; tb < t1; tb += 32) {
-    const int t = tb + lane;
-    const uint32_t x = t < t1 ? key(t) : 0;
-    const uint32_t mg = __ballot_sync(0xffffffffu, t < t1 && x > prefix);
-    const uint32_t me = __ballot_sync(0xffffffffu, t < t1 && x == prefix);
-    const int g = gt0 + __popc(mg & below), e = eq0 + __popc(me & below);
-    const bool keep = (mg >> lane & 1) || ((me >> lane & 1) && e < left);
-    if (keep) out[sink + g + min(e, left)] = t;
-    gt0 += __popc(mg);
-    eq0 += __popc(me);
+  for (int gbase = g0; gbase < g1; gbase += 32) {
+    const int g = gbase + lane;
+    const uint32_t note = g < g1 ? note_of(g) : 0;
+    const uint32_t mg = note & 15u, me = note >> 4;  // of this lane's four tokens
+    // counts of the lanes before: both in one sum (128 of each at most)
+    const int mine = __popc(mg) | __popc(me) << 16;
+    int before = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, before, o);
+      if (lane >= o) before += y;
+    }
+    const int all = __shfl_sync(0xffffffffu, before, 31);
+    before -= mine;
+    int at_g = gt0 + (before & 0xffff), at_e = eq0 + (before >> 16);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const bool above = mg >> i & 1, same = me >> i & 1;
+      if (above || (same && at_e < left)) out[sink + at_g + min(at_e, left)] = 4 * g + i;
+      at_g += above;
+      at_e += same;
+    }
+    gt0 += all & 0xffff;
+    eq0 += all >> 16;
   }
 }
 
@@ -404,17 +452,17 @@ int fe_kv_select(const float* scores, const int32_t* kv, const int32_t* pages, i
     return fail(FE_ERR_INVALID_ARGUMENT, "fe_kv_select: scores must be 16-byte aligned");
   const SeqTable table{kv, pages, last, num_pages, page, cache_slots};
   auto s = static_cast<cudaStream_t>(stream);
-  const int room = max_len <= kSelKeys ? max_len : 0;
+  const int room = std::min(max_len, kSelRoom);
   static std::once_flag once;
   static cudaError_t attr = cudaSuccess;
   std::call_once(once, [] {
     attr = cudaFuncSetAttribute(select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                kSelKeys * 4);
+                                kSelRoom / 4);
   });
   if (attr != cudaSuccess) return cuda_fail(attr, "fe_kv_select: shared memory attribute");
   FE_CUDA_TRY(launch_pdl(select_kernel, dim3(batch * hkv), dim3(kSelThreads),
-                         (sizeof(uint32_t) * room + 15) / 16 * 16, s, scores, table, kept, hkv, budget, sink,
-                         recent, room, device_error_word()));
+                         static_cast<size_t>(room + 15) / 16 * 4, s, scores, table, kept, hkv,
+                         budget, sink, recent, room, device_error_word()));
   return FE_OK;
 }
 

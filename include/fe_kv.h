@@ -148,7 +148,7 @@ int fe_kv_gather(const void* pool, void* out, const int32_t* kv, const int32_t* 
  * in all; of equal scores (-0 and +0 are equal) the lowest token indexes win,
  * NaN is below every number. A shorter sequence keeps all of its tokens, and -1
  * fills the rest. max_len sizes the launch: sequences of up to max_len tokens
- * (and up to 49152) are read once, longer ones several times. A page that lies
+ * (and up to 131072) are read twice, longer ones several times. A page that lies
  * outside the pool counts as NaN.
  *
  * fe_kv_compact: for each KV head, the K and V row and (scores not NULL) the
