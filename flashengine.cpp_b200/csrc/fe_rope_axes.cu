@@ -11,8 +11,10 @@
 // HBM-bound: 4 bytes of q and 8 of k and v per element (in and out) and one
 // cos / sin row a token.
 #include <algorithm>
+#include <mutex>
 #include <string>
 
+#include "fe_attn_common.cuh"
 #include "fe_rope_common.cuh"
 
 namespace fe {
@@ -129,6 +131,7 @@ __global__ void __launch_bounds__(kAxesThreads)
 // the last), so that a pair's axis costs one 4-byte copy a row and not one load
 // a head.
 constexpr int kRowBufs = 3;
+constexpr int kBulkRows = 2048;  // rows from which the ring of bulk copies is used
 
 template <typename T>
 __global__ void __launch_bounds__(kAxesThreads)
@@ -250,6 +253,187 @@ __global__ void __launch_bounds__(kAxesThreads)
   }
 }
 
+// Many rows: a CTA walks rows through a ring of shared-memory stages. A stage
+// holds a row's q, k and v, brought by bulk copies several rows ahead; the threads
+// turn q and k in place, and bulk copies take q back, k and v to their pool rows (and
+// k to k_out), while the next rows are already there. Loads and stores are then
+// in flight all the time, where a thread that loads, turns and stores its row
+// itself keeps the memory waiting (64k rows of 32 + 8 heads: 426 us so). The cos /
+// sin come as in the kernel above.
+constexpr int kBulkThreads = 256;
+constexpr int kMaxStages = 6;
+constexpr int kMetaBufs = 8;
+
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes,
+                                          uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+          smem_u32(dst)),
+      "l"(src), "r"(bytes), "r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ void bulk_store(void* dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst),
+               "r"(smem_u32(src)), "r"(bytes)
+               : "memory");
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kBulkThreads)
+    rope_axes_bulk_kernel(T* __restrict__ q, const T* k, const T* __restrict__ v, T* k_out,
+                          T* __restrict__ kc, T* __restrict__ vc, const AxesArgs a,
+                          const AxisMap map, int stages) {
+  using V = typename Pair2<T>::V;
+  union Chunk {
+    uint4 u;
+    V v[4];
+  };
+  extern __shared__ __align__(128) uint8_t ring[];
+  pdl_trigger();
+  const uint32_t qb = a.hq * a.dim * 2, kb = a.hkv * a.dim * 2;
+  const uint32_t stage_bytes = qb + kb + (kc ? kb : 0);
+  uint64_t* full = reinterpret_cast<uint64_t*>(ring + stages * stage_bytes);
+  volatile int* flag = reinterpret_cast<volatile int*>(full + kMaxStages);
+  int64_t* meta = reinterpret_cast<int64_t*>(full + kMaxStages + 2);
+  float* turns = reinterpret_cast<float*>(meta + kMetaBufs * (kMaxAxes + 1));  // [kRowBufs][rot]
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < stages; ++s) mbar_init(&full[s], 1);
+    *flag = 0;
+    fence_barrier_init();
+  }
+  __syncthreads();
+  pdl_wait();  // q, k, v come from, and the pools are read by, earlier kernels
+  const int rot_units = a.rot / 16, r = a.rot / 2, heads = a.hq + a.hkv;
+  auto fetch = [&](int64_t row, int s) {  // one thread
+    uint8_t* st = ring + s * stage_bytes;
+    mbar_arrive_expect_tx(&full[s], stage_bytes);
+    if (qb) bulk_load(st, q + row * a.hq * a.dim, qb, &full[s]);
+    bulk_load(st + qb, k + row * a.hkv * a.dim, kb, &full[s]);
+    if (kc) bulk_load(st + qb + kb, v + row * a.hkv * a.dim, kb, &full[s]);
+  };
+  // positions and slot of a row, four rows ahead: [row % kMetaBufs][kMaxAxes + 1]
+  auto meta_ahead = [&](int64_t row, uint32_t n) {
+    if (threadIdx.x <= kMaxAxes && row < a.rows) {
+      const int64_t* src = nullptr;
+      if (static_cast<int>(threadIdx.x) < a.axes)
+        src = a.pos + static_cast<int64_t>(threadIdx.x) * a.rows + row;
+      else if (threadIdx.x == kMaxAxes && kc)
+        src = a.slots + row;
+      if (src)
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(
+                         smem_u32(meta + n % kMetaBufs * (kMaxAxes + 1) + threadIdx.x)),
+                     "l"(src)
+                     : "memory");
+    }
+  };
+  auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
+  // its cos / sin, two rows ahead
+  auto gather = [&](int64_t row, uint32_t n) {
+    if (row >= a.rows) return;
+    const int64_t* m = meta + n % kMetaBufs * (kMaxAxes + 1);
+    float* dst = turns + n % kRowBufs * a.rot;
+    for (int i = threadIdx.x; i < a.rot; i += kBulkThreads) {
+      const int64_t p = m[map.axis[i < r ? i : i - r]];
+      // a row that is out of range is skipped below; its copies stay in bounds
+      const float* src = a.cache + (p >= 0 && p < a.max_positions ? p : 0) * a.rot + i;
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst + i)), "l"(src)
+                   : "memory");
+    }
+  };
+  const int64_t step = gridDim.x;
+  const int lag = stages > 3 ? 2 : 1;  // rows whose stores may still read their stage
+  int64_t fetched = blockIdx.x;        // next row to fetch (thread 0)
+  uint32_t nf = 0, n = 0;              // rows fetched, rows done
+  if (threadIdx.x == 0)
+    for (; static_cast<int>(nf) < stages - lag && fetched < a.rows; fetched += step, ++nf)
+      fetch(fetched, nf);
+  for (uint32_t i = 0; i < 4; ++i) meta_ahead(blockIdx.x + i * step, i);
+  commit();
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  __syncthreads();
+  for (uint32_t i = 0; i < 2; ++i) {
+    gather(blockIdx.x + i * step, i);
+    commit();
+  }
+  bool ok = true;
+  for (int64_t row = blockIdx.x; row < a.rows; row += step, ++n) {
+    const int s = n % stages;
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    ok = wait_bounded(&full[s], (n / stages) & 1u, flag);
+    if (!__syncthreads_and(ok)) {  // (and what came by cp.async is there for everyone)
+      ok = false;
+      break;
+    }
+    gather(row + 2 * step, n + 2);
+    meta_ahead(row + 4 * step, n + 4);
+    commit();
+    const int64_t* m = meta + n % kMetaBufs * (kMaxAxes + 1);
+    bool good = true;
+    for (int i = 0; i < a.axes; ++i) good &= m[i] >= 0 && m[i] < a.max_positions;
+    const float* cs = turns + n % kRowBufs * a.rot;
+    uint8_t* st = ring + s * stage_bytes;
+    if (good) {
+      for (int t = threadIdx.x; t < heads * rot_units; t += kBulkThreads) {
+        const int head = t / rot_units, u = t - head * rot_units;
+        uint4* x = reinterpret_cast<uint4*>(st + head * a.dim * 2) + u;
+        uint4* y = x + r / 8;
+        const float* c = cs + 8 * u;
+        Chunk lo, hi;
+        lo.u = *x;
+        hi.u = *y;
+        const float4 c0 = *reinterpret_cast<const float4*>(c);
+        const float4 c1 = *reinterpret_cast<const float4*>(c + 4);
+        const float4 s0 = *reinterpret_cast<const float4*>(c + r);
+        const float4 s1 = *reinterpret_cast<const float4*>(c + r + 4);
+        rotate<T>(lo.v[0], hi.v[0], make_float2(c0.x, c0.y), make_float2(s0.x, s0.y));
+        rotate<T>(lo.v[1], hi.v[1], make_float2(c0.z, c0.w), make_float2(s0.z, s0.w));
+        rotate<T>(lo.v[2], hi.v[2], make_float2(c1.x, c1.y), make_float2(s1.x, s1.y));
+        rotate<T>(lo.v[3], hi.v[3], make_float2(c1.z, c1.w), make_float2(s1.z, s1.w));
+        *x = lo.u;
+        *y = hi.u;
+      }
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      int64_t slot = kc ? m[kMaxAxes] : -1;
+      if (!good) raise_device_error(a.err, FE_DEVERR_POS_RANGE);
+      if (good && slot >= a.cache_slots) {
+        raise_device_error(a.err, FE_DEVERR_SLOT_RANGE);
+        slot = -1;
+      }
+      if (good) {
+        if (qb) bulk_store(q + row * a.hq * a.dim, st, qb);
+        if (k_out) bulk_store(k_out + row * a.hkv * a.dim, st + qb, kb);
+        if (slot >= 0) {
+          bulk_store(kc + slot * a.hkv * a.dim, st + qb, kb);
+          bulk_store(vc + slot * a.hkv * a.dim, st + qb + kb, kb);
+        }
+      }
+      asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+      // the stage of the row `lag` before this one is free once its stores have read it
+      if (fetched < a.rows) {
+        if (lag == 2)
+          asm volatile("cp.async.bulk.wait_group.read 2;" ::: "memory");
+        else
+          asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+        fetch(fetched, nf % stages);
+        fetched += step;
+        ++nf;
+      }
+    }
+  }
+  if (threadIdx.x == 0) {
+    if (!ok) {
+      raise_device_error(a.err, FE_DEVERR_TIMEOUT);
+      volatile int never = 0;
+      for (uint32_t t = n; t < nf; ++t)  // what was fetched has landed (bounded)
+        (void)wait_bounded(&full[t % stages], (t / stages) & 1u, &never);
+    }
+    asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  }
+}
+
 template <typename T>
 int launch_axes(void* q, const void* k, const void* v, void* k_out, void* kc, void* vc,
                 const AxesArgs& a, const AxisMap& map, cudaStream_t stream) {
@@ -267,6 +451,26 @@ int launch_axes(void* q, const void* k, const void* v, void* k_out, void* kc, vo
     const int passes = (heads + most - 1) / most;
     const int hl = (heads + passes - 1) / passes;
     const int threads = (hl * units + 31) / 32 * 32;
+    const int stage = (heads + (kc ? a.hkv : 0)) * a.dim * 2;
+    const int extra =
+        8 * (kMaxStages + 2 + kMetaBufs * (kMaxAxes + 1)) + 4 * kRowBufs * a.rot;
+    // stages of about 72 KiB a CTA, three CTAs an SM; at least three stages
+    const int stages = std::min(kMaxStages, std::max(3, (72 * 1024 - extra) / stage));
+    const int smem = stages * stage + extra;
+    if (a.rows >= kBulkRows && smem <= 112 * 1024) {
+      static std::once_flag once;
+      static cudaError_t attr = cudaSuccess;
+      std::call_once(once, [] {
+        attr = cudaFuncSetAttribute(rope_axes_bulk_kernel<T>,
+                                    cudaFuncAttributeMaxDynamicSharedMemorySize, 112 * 1024);
+      });
+      if (attr != cudaSuccess) return cuda_fail(attr, "fe_rope_axes: shared memory attribute");
+      const int per_sm = std::max(1, 225 * 1024 / (smem + 1024));
+      FE_CUDA_TRY(launch_pdl(rope_axes_bulk_kernel<T>, dim3(std::min(a.rows, 148 * per_sm)),
+                             dim3(kBulkThreads), smem, stream, tq, tk, tv, to, tkc, tvc, a, map,
+                             stages));
+      return FE_OK;
+    }
     const int gx = a.rows < 1024 ? passes : (passes + 1) / 2;
     // a row a block while there are few; then blocks that walk the rows, as many
     // as are resident

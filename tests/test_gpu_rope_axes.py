@@ -50,7 +50,8 @@ def same(got, want):
 
 CASES = [(1, 16, 8, 128, 128), (64, 32, 8, 128, 128), (37, 6, 3, 128, 64), (5, 40, 8, 128, 128),
          (3, 16, 2, 256, 256), (9, 5, 5, 256, 128), (130, 8, 1, 128, 128), (7, 3, 1, 44, 20),
-         (6, 2, 2, 128, 0), (1500, 12, 4, 128, 128)]
+         (6, 2, 2, 128, 0), (1500, 12, 4, 128, 128),
+         (2500, 12, 4, 128, 128), (2049, 0, 2, 128, 64), (2300, 40, 8, 256, 128)]
 
 
 @pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
