@@ -131,7 +131,12 @@ __global__ void __launch_bounds__(kAxesThreads)
 // the last), so that a pair's axis costs one 4-byte copy a row and not one load
 // a head.
 constexpr int kRowBufs = 3;
-constexpr int kBulkRows = 2048;  // rows from which the ring of bulk copies is used
+// From this many rows of this many bytes the ring of bulk copies is used: 4096 rows
+// of 8 + 2 heads of 128 (3 KiB) took 10.1 us by threads and 13.5 by the ring, 16 + 4
+// heads 17.7 and 16.3, 32 + 8 heads 22.5 and 20.4; 2048 rows of those 9.4 and 9.5,
+// 11.4 and 12.3.
+constexpr int kBulkRows = 4096;
+constexpr int kBulkRowBytes = 4096;
 
 template <typename T>
 __global__ void __launch_bounds__(kAxesThreads)
@@ -258,11 +263,17 @@ __global__ void __launch_bounds__(kAxesThreads)
 // turn q and k in place, and bulk copies take q back, k and v to their pool rows (and
 // k to k_out), while the next rows are already there. Loads and stores are then
 // in flight all the time, where a thread that loads, turns and stores its row
-// itself keeps the memory waiting (64k rows of 32 + 8 heads: 426 us so). The cos /
-// sin come as in the kernel above.
-constexpr int kBulkThreads = 256;
-constexpr int kMaxStages = 6;
+// itself keeps the memory waiting. The cos / sin come as in the kernel above, two
+// rows ahead, and their positions and the slot four rows ahead. 64k rows of 32 + 8
+// heads of 128, 1.6 GB: 258 us, 6.4 TB/s (426 us by the kernel above). A row's
+// steps follow one another behind two barriers, so it is the CTAs of an SM that
+// overlap: five of 64 threads and three stages, where three of 256 threads and
+// five stages took 328 us, two with eight stages 437 us.
+constexpr int kBulkThreads = 64;
+constexpr int kMaxStages = 10;
 constexpr int kMetaBufs = 8;
+// (what lies between the stages and `turns`, which is read 16 bytes at a time)
+static_assert((kMaxStages + 2 + kMetaBufs * (kMaxAxes + 1)) % 2 == 0, "turns: 16-byte aligned");
 
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes,
                                           uint64_t* bar) {
@@ -454,10 +465,10 @@ int launch_axes(void* q, const void* k, const void* v, void* k_out, void* kc, vo
     const int stage = (heads + (kc ? a.hkv : 0)) * a.dim * 2;
     const int extra =
         8 * (kMaxStages + 2 + kMetaBufs * (kMaxAxes + 1)) + 4 * kRowBufs * a.rot;
-    // stages of about 72 KiB a CTA, three CTAs an SM; at least three stages
-    const int stages = std::min(kMaxStages, std::max(3, (72 * 1024 - extra) / stage));
+    // at least three stages; many small CTAs rather than few large ones
+    const int stages = std::min(kMaxStages, std::max(3, (38 * 1024 - extra) / stage));
     const int smem = stages * stage + extra;
-    if (a.rows >= kBulkRows && smem <= 112 * 1024) {
+    if (a.rows >= kBulkRows && stage >= kBulkRowBytes && smem <= 112 * 1024) {
       static std::once_flag once;
       static cudaError_t attr = cudaSuccess;
       std::call_once(once, [] {

@@ -51,7 +51,7 @@ def same(got, want):
 CASES = [(1, 16, 8, 128, 128), (64, 32, 8, 128, 128), (37, 6, 3, 128, 64), (5, 40, 8, 128, 128),
          (3, 16, 2, 256, 256), (9, 5, 5, 256, 128), (130, 8, 1, 128, 128), (7, 3, 1, 44, 20),
          (6, 2, 2, 128, 0), (1500, 12, 4, 128, 128),
-         (2500, 12, 4, 128, 128), (2049, 0, 2, 128, 64), (2300, 40, 8, 256, 128)]
+         (2500, 12, 4, 128, 128), (4097, 0, 8, 128, 64), (4100, 20, 4, 256, 128), (4500, 32, 8, 128, 128)]
 
 
 @pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
@@ -110,12 +110,13 @@ def test_one_position_gives_rope(turns):
     same(t["k"], k.cpu())
 
 
-def test_rows_out_of_range_are_skipped_and_flagged():
+@pytest.mark.parametrize("rows", [20, 4200])
+def test_rows_out_of_range_are_skipped_and_flagged(rows):
     import fekv
     import torch
     from fekv import _lib
     pairs = fekv.rope_sections((24, 20, 20), True)
-    t = make(20, 8, 4, 128, 128, 3, torch.float16, 9)
+    t = make(rows, 8, 4, 128, 128, 3, torch.float16, 9)
     t["pos"][1, 4] = 700
     t["pos"][2, 7] = -1
     t["slots"][11] = t["kc"].shape[0]
@@ -129,7 +130,7 @@ def test_rows_out_of_range_are_skipped_and_flagged():
     bad = [4, 7]
     q[bad] = t["q"][bad]
     kc, vc = t["kc"].clone(), t["vc"].clone()
-    live = [i for i in range(20) if i not in (4, 7, 11)]
+    live = [i for i in range(rows) if i not in (4, 7, 11)]
     kc[t["slots"][live]] = k[live]
     vc[t["slots"][live]] = t["v"][live]
     same(d["q"], q)
