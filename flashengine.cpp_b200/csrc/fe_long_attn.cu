@@ -37,6 +37,7 @@ namespace {
 
 constexpr int kJoinThreads = 256;
 constexpr int kJoinWarps = kJoinThreads / 32;
+constexpr int kScoreThreads = 128;
 
 // The records of one row: n of them, rec_floats apart.
 struct Records {
@@ -73,11 +74,10 @@ __device__ __forceinline__ const float* record(const Records& a, const Records& 
 // One warp joins the records of one row and stores its 16-bit output. What
 // bounds it is the way to the L2 and back, so the loads of kStep records, their
 // (m, l) among them, go out together.
-template <typename T, int D>
+template <typename T, int D, int kStep>
 __device__ __forceinline__ void join_row(const Records& a, const Records& b, int lane, T* out,
                                          float* lse) {
-  constexpr int kV = D / 128;         // float4 vectors per lane
-  constexpr int kStep = 8 / kV;
+  constexpr int kV = D / 128;  // float4 vectors per lane
   const int n = a.n + b.n;
   float4 acc[kV];
 #pragma unroll
@@ -138,72 +138,93 @@ __device__ __forceinline__ void join_row(const Records& a, const Records& b, int
   if (lse && lane == 0) *lse = M + log2f(L);
 }
 
-// Warp `w` of the joining warps: query row w / hq, head w % hq. Everything up to
-// pdl_wait() is the plan's metadata, complete before the kernels ahead began.
+// The records of query row w / hq, head w % hq: the plan's metadata alone, complete
+// before the kernels ahead began.
 template <typename T, int D>
-__device__ __forceinline__ void join_warp(const AttnArgs<T>& a, float* lse, int64_t w, int lane) {
+__device__ __forceinline__ void find_records(const AttnArgs<T>& a, int64_t w, Records& own,
+                                             Records& pre) {
   const MetaHeader* hdr = reinterpret_cast<const MetaHeader*>(a.meta);
   const int r = static_cast<int>(w / a.hq), head = static_cast<int>(w % a.hq);
   const int H = hdr->dec_heads, h = head / a.G;
-  Records own{nullptr, 0, 0, 0, 0}, pre = own;
-  if (r < hdr->rows) {
-    const RowInfo x = reinterpret_cast<const RowInfo*>(a.meta + hdr->row_info_off)[r];
-    const UnitRec* units = reinterpret_cast<const UnitRec*>(a.meta + hdr->unit_off[a.view]);
-    int row;
-    if (x.own_unit >= 0) {
-      const int u = unit_of<D>(x.own_unit, x.own_blocks, x.own_p + head % a.G, x.own_rows, h, H,
-                               row);
-      own = records_of(units[u], a.partials, row);
-    }
-    if (x.pre_unit >= 0) {
-      const int u = unit_of<D>(x.pre_unit, x.pre_blocks, x.pre_p + head % a.G, x.pre_rows, h, H,
-                               row);
-      pre = records_of(units[u], a.partials, row);
-    }
+  own = pre = Records{nullptr, 0, 0, 0, 0};
+  if (r >= hdr->rows) return;
+  const RowInfo x = reinterpret_cast<const RowInfo*>(a.meta + hdr->row_info_off)[r];
+  const UnitRec* units = reinterpret_cast<const UnitRec*>(a.meta + hdr->unit_off[a.view]);
+  int row;
+  if (x.own_unit >= 0) {
+    const int u = unit_of<D>(x.own_unit, x.own_blocks, x.own_p + head % a.G, x.own_rows, h, H,
+                             row);
+    own = records_of(units[u], a.partials, row);
   }
-  pdl_wait();
-  if (own.n == 0) return;  // written by its unit
-  join_row<T, D>(own, pre, lane, a.out + w * D, lse ? lse + w : nullptr);
+  if (x.pre_unit >= 0) {
+    const int u = unit_of<D>(x.pre_unit, x.pre_blocks, x.pre_p + head % a.G, x.pre_rows, h, H,
+                             row);
+    pre = records_of(units[u], a.partials, row);
+  }
 }
 
 // One warp per query row and head; lse (scored plans): where m + log2 l of each
-// goes, fp32 [rows, hq].
-template <typename T, int D>
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttnArgs<T> a, float* lse) {
+// goes, fp32 [rows, hq]. Few pairs: all records of one in flight. Many: what counts
+// are loads in flight an SM, so two records a warp and more warps (2048 rows of
+// 32 heads, 60 % with two records: 7 us less; 64 rows of 64 heads 2 us more).
+constexpr int kManyPairs = 148 * 48;
+
+template <typename T, int D, int kStep>
+__global__ void __launch_bounds__(kJoinThreads, kStep == 2 && D == kHeadDim ? 5 : 3)
+    join_kernel(const AttnArgs<T> a, float* lse) {
   pdl_trigger();
-  join_warp<T, D>(a, lse, static_cast<int64_t>(blockIdx.x) * kJoinWarps + (threadIdx.x >> 5),
-                  threadIdx.x & 31);
+  const int lane = threadIdx.x & 31;
+  const int64_t w = static_cast<int64_t>(blockIdx.x) * kJoinWarps + (threadIdx.x >> 5);
+  Records own, pre;
+  find_records<T, D>(a, w, own, pre);
+  pdl_wait();
+  if (own.n > 0)  // else written by its unit
+    join_row<T, D, kStep>(own, pre, lane, a.out + w * D, lse ? lse + w : nullptr);
+}
+
+template <typename T, int D>
+int launch_join(const AttnArgs<T>& a, int rows, float* lse, cudaStream_t s) {
+  const int64_t pairs = int64_t(rows) * a.hq;
+  const int grid = static_cast<int>((pairs + kJoinWarps - 1) / kJoinWarps);
+  auto kernel = pairs > kManyPairs ? join_kernel<T, D, 2> : join_kernel<T, D, 8 * kHeadDim / D>;
+  FE_CUDA_TRY(launch_pdl(kernel, dim3(grid), dim3(kJoinThreads), 0, s, a, lse));
+  return FE_OK;
+}
+
+template <typename T>
+int launch_join(const AttnArgs<T>& a, int dim, int rows, float* lse, cudaStream_t s) {
+  return dim == kWideHeadDim ? launch_join<T, kWideHeadDim>(a, rows, lse, s)
+                             : launch_join<T, kHeadDim>(a, rows, lse, s);
 }
 
 // Scored plans, behind the join: the weights of kScoreChunk keys of one KV head
 // at a time, 2^(raw score - lse) summed over the packed rows in order, go to the
-// keys' scores.
-__global__ void __launch_bounds__(kJoinThreads)
+// keys' scores. Grid: chunks x KV heads.
+__global__ void __launch_bounds__(kScoreThreads, 8)
     score_kernel(const uint8_t* __restrict__ meta, const float* __restrict__ raw_scores,
                  const float* __restrict__ lse, float* __restrict__ scores, int hq, int hkv,
                  int page, int64_t cache_slots) {
-  constexpr int kPer = kScoreChunk / kJoinThreads;  // keys a thread
+  constexpr int kPer = kScoreChunk / kScoreThreads;  // keys a thread
   pdl_trigger();
   const MetaHeader* hdr = reinterpret_cast<const MetaHeader*>(meta);
   const ScoreChunk* chunks = reinterpret_cast<const ScoreChunk*>(meta + hdr->chunk_off);
   const SeqInfo* seqs = reinterpret_cast<const SeqInfo*>(meta + hdr->seqs_off);
   const int64_t* sink = reinterpret_cast<const int64_t*>(meta + hdr->sink_off);
   const int32_t* pages = reinterpret_cast<const int32_t*>(meta + hdr->pages_off);
-  const int64_t total = static_cast<int64_t>(hdr->n_chunks) * hkv;
-  const int G = hq / hkv;
+  const int total = hdr->n_chunks, G = hq / hkv, h = blockIdx.y;
+  float* out = scores + h * cache_slots;
   bool waited = false;
-  for (int64_t e = blockIdx.x; e < total; e += gridDim.x) {
-    const ScoreChunk c = chunks[e / hkv];
-    const int h = static_cast<int>(e % hkv);
+  for (int e = blockIdx.x; e < total; e += gridDim.x) {
+    const ScoreChunk c = chunks[e];
     float w[kPer];
     int64_t at[kPer];
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       w[i] = 0.f;
-      const int t = c.t0 + i * kJoinThreads + threadIdx.x;
-      at[i] = t < c.length ? h * cache_slots +
-                                 static_cast<int64_t>(__ldg(pages + c.page_off + t / page)) * page +
-                                 t % page
+      const int t = c.t0 + i * kScoreThreads + threadIdx.x;
+      const unsigned pg = static_cast<unsigned>(t) / static_cast<unsigned>(page);
+      at[i] = t < c.length ? static_cast<int64_t>(__ldg(pages + c.page_off + pg)) * page +
+                                 (t - static_cast<int>(pg) * page)
                            : -1;
     }
     SeqInfo si = seqs[c.block0];
@@ -213,8 +234,8 @@ __global__ void __launch_bounds__(kJoinThreads)
     float old[kPer];
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      const int t = c.t0 + i * kJoinThreads + threadIdx.x;
-      old[i] = at[i] >= 0 && t < c.fresh ? scores[at[i]] : 0.f;
+      const int t = c.t0 + i * kScoreThreads + threadIdx.x;
+      old[i] = at[i] >= 0 && t < c.fresh ? out[at[i]] : 0.f;
     }
     for (int j = 0;;) {
       if (c.t0 < si.length) {  // else the block's rows do not see this far
@@ -222,19 +243,35 @@ __global__ void __launch_bounds__(kJoinThreads)
         const int tiles = (si.length + kTileTokens - 1) / kTileTokens;
         const float* raw = raw_scores + raw0 + static_cast<int64_t>(h) * tiles * kTileTokens * cols;
         const float* row = lse + static_cast<int64_t>(si.q_row0) * hq + h * G;
-        for (int p = 0; p < P; p += 2) {
-          const float l0 = __ldcg(row + static_cast<int64_t>(p / G) * hq + p % G);
-          const float l1 = p + 1 < P
-                               ? __ldcg(row + static_cast<int64_t>((p + 1) / G) * hq + (p + 1) % G)
-                               : INFINITY;
+        const float* at_key = raw + static_cast<int64_t>(c.t0 + threadIdx.x) * cols;
+        const int stride = kScoreThreads * cols;
+        int g = 0;  // packed row p is head g of the query row that `row` points at
+        for (int p = 0; p < P; p += 4, at_key += 4) {  // four rows' scores of a key at once
+          float l[4];
+          float2 s0[kPer], s1[kPer];
 #pragma unroll
           for (int i = 0; i < kPer; ++i) {
-            const int t = c.t0 + i * kJoinThreads + threadIdx.x;
-            if (t >= si.length) continue;
-            const float2 s = __ldcg(
-                reinterpret_cast<const float2*>(raw + static_cast<int64_t>(t) * cols + p));
-            w[i] += fast_exp2(s.x - l0);
-            if (p + 1 < P) w[i] += fast_exp2(s.y - l1);
+            s0[i] = s1[i] = make_float2(-INFINITY, -INFINITY);
+            if (c.t0 + i * kScoreThreads + static_cast<int>(threadIdx.x) < si.length) {
+              const float2* x = reinterpret_cast<const float2*>(at_key + i * stride);
+              s0[i] = __ldcg(x);
+              if (p + 2 < P) s1[i] = __ldcg(x + 1);
+            }
+          }
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            l[r] = p + r < P ? __ldcg(row + g) : INFINITY;
+            if (++g == G) {
+              g = 0;
+              row += hq;
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < kPer; ++i) {
+            w[i] += fast_exp2(s0[i].x - l[0]);
+            if (p + 1 < P) w[i] += fast_exp2(s0[i].y - l[1]);
+            if (p + 2 < P) w[i] += fast_exp2(s1[i].x - l[2]);
+            if (p + 3 < P) w[i] += fast_exp2(s1[i].y - l[3]);
           }
         }
       }
@@ -244,7 +281,7 @@ __global__ void __launch_bounds__(kJoinThreads)
     }
 #pragma unroll
     for (int i = 0; i < kPer; ++i)
-      if (at[i] >= 0) scores[at[i]] = old[i] + w[i];
+      if (at[i] >= 0) out[at[i]] = old[i] + w[i];
   }
   if (!waited) pdl_wait();
 }
@@ -521,10 +558,6 @@ AttnArgs<T> long_args(const fe_long_plan* p, const void* q, void* out, int view,
   return a;
 }
 
-int join_ctas(const fe_long_plan* p) {
-  return static_cast<int>((int64_t(p->last.rows) * p->cfg.hq + kJoinWarps - 1) / kJoinWarps);
-}
-
 int launch_decode(fe_long_plan* p, const void* args, int grid, bool beside, cudaStream_t s) {
   if (p->keys) return keys_launch(p->dtype, p->kmap_dec, p->vmap_dec, args, grid, beside, s);
   return decode_ext_launch(p->dtype, p->cfg.dim, p->cfg.dec_heads, p->kmap_dec, p->vmap_dec,
@@ -557,11 +590,8 @@ int run_shared(fe_long_plan* p, const void* q, void* out, int view, cudaStream_t
     int rc = launch_decode(p, &a, grid_dec, grid_rows > 0, s);
     if (rc != FE_OK) return rc;
   }
-  if (p->fixed_grid || p->last.merge[view]) {
-    auto kernel = c.dim == kWideHeadDim ? join_kernel<T, kWideHeadDim> : join_kernel<T, kHeadDim>;
-    FE_CUDA_TRY(launch_pdl(kernel, dim3(join_ctas(p)), dim3(kJoinThreads), 0, s, a,
-                           static_cast<float*>(nullptr)));
-  }
+  if (p->fixed_grid || p->last.merge[view])
+    return launch_join<T>(a, c.dim, p->last.rows, nullptr, s);
   return FE_OK;
 }
 
@@ -572,14 +602,12 @@ int run_scored(fe_long_plan* p, const void* q, float* scores, void* out, cudaStr
   const AttnArgs<T> a = long_args<T>(p, q, out, 1, 0);
   int rc = launch_decode(p, &a, grid_dec, false, s);
   if (rc != FE_OK) return rc;
-  auto join = c.dim == kWideHeadDim ? join_kernel<T, kWideHeadDim> : join_kernel<T, kHeadDim>;
-  FE_CUDA_TRY(
-      launch_pdl(join, dim3(join_ctas(p)), dim3(kJoinThreads), 0, s, a, p->d_lse));
+  rc = launch_join<T>(a, c.dim, p->last.rows, p->d_lse, s);
+  if (rc != FE_OK) return rc;
   // a graph's launch has to do for later steps of more keys: the CTAs stride
-  const int64_t most = int64_t(8) * c.grid_cap;
-  const int64_t work = int64_t(p->last.n_chunks) * c.hkv;
-  const int grid = static_cast<int>(p->fixed_grid ? most : std::min(work, most));
-  FE_CUDA_TRY(launch_pdl(score_kernel, dim3(grid), dim3(kJoinThreads), 0, s,
+  const int most = std::max(1, 16 * c.grid_cap / c.hkv);
+  const dim3 grid(p->fixed_grid ? most : std::max(1, std::min(p->last.n_chunks, most)), c.hkv);
+  FE_CUDA_TRY(launch_pdl(score_kernel, grid, dim3(kScoreThreads), 0, s,
                          static_cast<const uint8_t*>(p->d_meta),
                          static_cast<const float*>(p->d_sink),
                          static_cast<const float*>(p->d_lse), scores, c.hq, c.hkv, c.page,
