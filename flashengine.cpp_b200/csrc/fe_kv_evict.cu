@@ -19,6 +19,7 @@ constexpr int kSelThreads = 512;
 constexpr int kSelList = 2048;
 constexpr int kSelWarps = kSelThreads / 32;
 constexpr int kBins = 2048;
+constexpr int kRankBatch = 128;  // sequences that are taken longest first
 constexpr int kSelRoom = 128 << 10;  // tokens whose classes fit in shared memory
 
 // A score as an unsigned number of the same order; NaN below everything.
@@ -121,20 +122,37 @@ __device__ __forceinline__ int2 find_bin(const int* hist, int left, int* warp_su
 __global__ void __launch_bounds__(kSelThreads, 3)
     select_kernel(const float* __restrict__ scores, const SeqTable table,
                   int32_t* __restrict__ kept, int hkv, int budget, int sink, int recent, int room,
-                  unsigned int* err) {
+                  bool ranked, unsigned int* err) {
   extern __shared__ uint32_t notes32[];  // notes, four a word
   __shared__ int hist[kBins];
   __shared__ uint2 list[kSelList];  // key, token
   __shared__ int warp_sums[kSelWarps];
-  __shared__ int found[2], listed;
+  __shared__ int found[2], listed, ranks[kRankBatch];
   pdl_trigger();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0;
   if (tid == 0) listed = 0;
   pdl_wait();  // the scores come from, and the lists may come from, earlier kernels
-  const int b = blockIdx.x / hkv, h = blockIdx.x % hkv;
-  int32_t* out = kept + static_cast<int64_t>(blockIdx.x) * budget;
-  int p0, n;
+  int b = blockIdx.x / hkv, p0, n;
+  const int h = blockIdx.x % hkv;
+  if (ranked) {  // the b-th longest sequence
+    const int batch = gridDim.x / hkv;
+    if (tid < kRankBatch) {
+      int len = -1;
+      if (tid < batch && !sequence(table, tid, p0, len)) len = 0;
+      ranks[tid] = len;
+    }
+    __syncthreads();
+    if (tid < batch) {
+      const int len = ranks[tid];
+      int longer = 0;
+      for (int j = 0; j < batch; ++j) longer += ranks[j] > len || (ranks[j] == len && j < tid);
+      if (longer == b) found[0] = tid;
+    }
+    __syncthreads();
+    b = found[0];
+  }
+  int32_t* out = kept + (static_cast<int64_t>(b) * hkv + h) * budget;
   if (!sequence(table, b, p0, n)) {
     if (tid == 0 && h == 0) raise_device_error(err, FE_DEVERR_PAGE_RANGE);
     for (int i = tid; i < budget; i += kSelThreads) out[i] = -1;
@@ -152,19 +170,28 @@ __global__ void __launch_bounds__(kSelThreads, 3)
   uint8_t* notes = reinterpret_cast<uint8_t*>(notes32);
   const bool noted = n <= room;
   const int per16 = table.page / 16;
-  // the keys of tokens 4g .. 4g + 3 (whose slots are adjacent)
-  auto load4 = [&](int g) -> uint4 {
-    const int blk = g >> 2, pi = per16 == 1 ? blk : blk / per16;
-    const int pg = __ldg(table.pages + p0 + pi);
-    const int64_t first = static_cast<int64_t>(pg) * table.page;
-    if (pg < 0 || first + table.page > table.cache_slots) {
+  // the page of tokens 4g .. 4g + 3, whose slots are adjacent, and their scores
+  const int num_pages = static_cast<int>(table.cache_slots / table.page);
+  auto page_of = [&](int g) {
+    return __ldg(table.pages + p0 + (per16 == 1 ? g >> 2 : (g >> 2) / per16));
+  };
+  auto load4 = [&](int g, int pg) -> float4 {
+    if (static_cast<unsigned>(pg) >= static_cast<unsigned>(num_pages)) {
       raise_device_error(err, FE_DEVERR_PAGE_RANGE);
-      return make_uint4(0, 0, 0, 0);
+      const float least = __uint_as_float(0xffffffffu);
+      return make_float4(least, least, least, least);
     }
-    const float4 x = __ldg(reinterpret_cast<const float4*>(sc + first + (4 * g - pi * table.page)));
+    const int in = per16 == 1 ? g & 3 : g - (g >> 2) / per16 * per16 * 4;
+    return __ldg(reinterpret_cast<const float4*>(sc + static_cast<int64_t>(pg) * table.page) + in);
+  };
+  auto keys = [&](const float4& x) {
     return make_uint4(ordered(x.x), ordered(x.y), ordered(x.z), ordered(x.w));
   };
   const int ga = sink / 4, gb = (end + 3) / 4;
+  if (noted && tid == 0) {  // (the sweeps write the notes of [ga, gb) only)
+    notes32[ga / 4] = 0;
+    notes32[(gb - 1) / 4] = 0;
+  }
   // f(i, key) for the tokens 4g + i of a group that lie between sink and end
   auto each = [&](int g, const uint4& x, auto&& f) {
     const uint32_t v[4] = {x.x, x.y, x.z, x.w};
@@ -179,16 +206,27 @@ __global__ void __launch_bounds__(kSelThreads, 3)
         if (i >= from && i < to) f(i, v[i]);
     }
   };
-  constexpr int kAhead = 2;  // groups in flight a thread
+  // groups in flight a thread; the pages of the next ones are there by then
+  constexpr int kAhead = 2;
   auto sweep = [&](auto&& f) {
-    for (int g0 = ga + tid; g0 < gb; g0 += kAhead * kSelThreads) {
-      uint4 x[kAhead];
+    int pg[kAhead];
+    int g0 = ga + tid;
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      pg[u] = g0 + u * kSelThreads < gb ? page_of(g0 + u * kSelThreads) : 0;
+    for (; g0 < gb; g0 += kAhead * kSelThreads) {
+      float4 x[kAhead];
 #pragma unroll
       for (int u = 0; u < kAhead; ++u)
-        if (g0 + u * kSelThreads < gb) x[u] = load4(g0 + u * kSelThreads);
+        if (g0 + u * kSelThreads < gb) x[u] = load4(g0 + u * kSelThreads, pg[u]);
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int g = g0 + (kAhead + u) * kSelThreads;
+        if (g < gb) pg[u] = page_of(g);
+      }
 #pragma unroll
       for (int u = 0; u < kAhead; ++u)
-        if (g0 + u * kSelThreads < gb) f(g0 + u * kSelThreads, x[u]);
+        if (g0 + u * kSelThreads < gb) f(g0 + u * kSelThreads, keys(x[u]));
     }
   };
   __syncthreads();
@@ -206,15 +244,21 @@ __global__ void __launch_bounds__(kSelThreads, 3)
   sweep([&](int g, const uint4& x) {
     uint32_t note = 0;
     each(g, x, [&](int i, uint32_t k) {
-      if (k > bin_end) {
-        note |= 1u << i;
-      } else if (k >= prefix) {
-        atomicAdd(&hist[(k >> 10) & 2047], 1);
-        const int at = atomicAdd(&listed, 1);
-        if (at < kSelList) list[at] = make_uint2(k, 4 * g + i);
-      }
+      note |= (k > bin_end ? 1u : k >= prefix ? 16u : 0u) << i;
     });
-    if (noted) notes[g] = note;
+    const uint32_t in_bin = note >> 4;
+    if (noted) notes[g] = note & 15u;
+    if (in_bin) {
+      int at = atomicAdd(&listed, __popc(in_bin));
+      const uint32_t v[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (!(in_bin >> i & 1)) continue;
+        atomicAdd(&hist[(v[i] >> 10) & 2047], 1);
+        if (at < kSelList) list[at] = make_uint2(v[i], 4 * g + i);
+        ++at;
+      }
+    }
   });
   __syncthreads();
   const bool whole = listed <= kSelList;  // the list holds the bin
@@ -257,15 +301,36 @@ __global__ void __launch_bounds__(kSelThreads, 3)
     sweep([&](int g, const uint4& x) { notes[g] = judge(g, x); });
   }
   __syncthreads();
-  auto note_of = [&](int g) -> uint32_t { return noted ? notes[g] : judge(g, load4(g)); };
-  // ---- kept tokens in order: a warp owns a stretch of the groups
-  const int per = ((gb - ga + kSelWarps - 1) / kSelWarps + 31) / 32 * 32;
-  const int g0 = min(gb, ga + warp * per), g1 = min(gb, g0 + per);
+  // ---- kept tokens in order: a warp owns a stretch of the groups, a lane four of
+  // them at a time: sixteen tokens, bit t of `mg` / `me` token t above / at it
+  const int wa = ga / 4, wb = (gb + 3) / 4;
+  const int per = ((wb - wa + kSelWarps - 1) / kSelWarps + 31) / 32 * 32;
+  const int w0 = min(wb, wa + warp * per), w1 = min(wb, w0 + per);
+  auto word = [&](int w, uint32_t& mg, uint32_t& me) {
+    uint32_t x = 0;
+    if (noted) {
+      x = notes32[w];
+    } else {
+#pragma unroll 1
+      for (int i = 0; i < 4; ++i) {
+        const int g = 4 * w + i;
+        if (g >= ga && g < gb) x |= judge(g, keys(load4(g, page_of(g)))) << (8 * i);
+      }
+    }
+    auto nibbles = [](uint32_t y) {  // the low half of each byte, packed
+      y &= 0x0f0f0f0fu;
+      y |= y >> 4;
+      return (y & 0xffu) | (y >> 8 & 0xff00u);
+    };
+    mg = nibbles(x);
+    me = nibbles(x >> 4);
+  };
   int gt = 0, eq = 0;
-  for (int g = g0 + lane; g < g1; g += 32) {
-    const uint32_t note = note_of(g);
-    gt += __popc(note & 15u);
-    eq += __popc(note >> 4);
+  for (int w = w0 + lane; w < w1; w += 32) {
+    uint32_t mg, me;
+    word(w, mg, me);
+    gt += __popc(mg);
+    eq += __popc(me);
   }
 #pragma unroll
   for (int o = 16; o; o >>= 1) {
@@ -277,11 +342,11 @@ __global__ void __launch_bounds__(kSelThreads, 3)
   int eq0 = block_scan(lane == 0 ? eq : 0, warp_sums, total);
   gt0 = __shfl_sync(0xffffffffu, gt0, 0);
   eq0 = __shfl_sync(0xffffffffu, eq0, 0);
-  for (int gbase = g0; gbase < g1; gbase += 32) {
-    const int g = gbase + lane;
-    const uint32_t note = g < g1 ? note_of(g) : 0;
-    const uint32_t mg = note & 15u, me = note >> 4;  // of this lane's four tokens
-    // counts of the lanes before: both in one sum (128 of each at most)
+  for (int wbase = w0; wbase < w1; wbase += 32) {
+    const int w = wbase + lane;
+    uint32_t mg = 0, me = 0;
+    if (w < w1) word(w, mg, me);
+    // counts of the lanes before: both in one sum (512 of each at most)
     const int mine = __popc(mg) | __popc(me) << 16;
     int before = mine;
 #pragma unroll
@@ -292,11 +357,11 @@ __global__ void __launch_bounds__(kSelThreads, 3)
     const int all = __shfl_sync(0xffffffffu, before, 31);
     before -= mine;
     int at_g = gt0 + (before & 0xffff), at_e = eq0 + (before >> 16);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const bool above = mg >> i & 1, same = me >> i & 1;
-      if (above || (same && at_e < left)) out[sink + at_g + min(at_e, left)] = 4 * g + i;
-      at_g += above;
+    for (uint32_t m = mg | me; m; m &= m - 1) {
+      const int t = __ffs(m) - 1;
+      const bool same = me >> t & 1;
+      if (!same || at_e < left) out[sink + at_g + min(at_e, left)] = 16 * w + t;
+      at_g += !same;
       at_e += same;
     }
     gt0 += all & 0xffff;
@@ -460,9 +525,12 @@ int fe_kv_select(const float* scores, const int32_t* kv, const int32_t* pages, i
                                 kSelRoom / 4);
   });
   if (attr != cudaSuccess) return cuda_fail(attr, "fe_kv_select: shared memory attribute");
+  // more lists than SMs: the longest first, so that the last to end are short. Not
+  // for large batches, where a CTA's look at all lengths costs more than it gives.
+  const bool ranked = batch <= kRankBatch && batch * hkv > 148;
   FE_CUDA_TRY(launch_pdl(select_kernel, dim3(batch * hkv), dim3(kSelThreads),
                          static_cast<size_t>(room + 15) / 16 * 4, s, scores, table, kept, hkv,
-                         budget, sink, recent, room, device_error_word()));
+                         budget, sink, recent, room, ranked, device_error_word()));
   return FE_OK;
 }
 
