@@ -19,6 +19,7 @@ constexpr int kSelThreads = 512;
 constexpr int kSelList = 2048;
 constexpr int kSelWarps = kSelThreads / 32;
 constexpr int kBins = 2048;
+constexpr int kSelCluster = 8, kSelCtas = 296, kSelPart = 4096;
 constexpr int kRankBatch = 128;  // sequences that are taken longest first
 constexpr int kSelRoom = 128 << 10;  // tokens whose classes fit in shared memory
 
@@ -44,7 +45,7 @@ __device__ __forceinline__ bool sequence(const SeqTable& t, int b, int& p0, int&
   n = 0;
   if (p0 < 0 || p1 <= p0 || p1 > t.num_pages || ln < 1 || ln > t.page) return false;
   const int64_t len = static_cast<int64_t>(p1 - p0 - 1) * t.page + ln;
-  if (len > INT32_MAX) return false;
+  if (len > INT32_MAX - 127) return false;  // (room for rounding up)
   n = static_cast<int>(len);
   return true;
 }
@@ -79,19 +80,56 @@ __device__ __forceinline__ int block_scan(int v, int* warp_sums, int& total) {
   return before + x - v;
 }
 
-// The bin from the top in which the left-th key lies: (bin, keys still wanted
-// of it), for the whole block. hist holds kBins bins.
-__device__ __forceinline__ int2 find_bin(const int* hist, int left, int* warp_sums, int* found) {
-  constexpr int kPer = kBins / kSelThreads;
-  const int tid = threadIdx.x;
-  int mine[kPer], sum = 0;
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    mine[i] = hist[kBins - 1 - (tid * kPer + i)];
-    sum += mine[i];
+// The CTAs of a cluster share a list: rank, size, a barrier of all their threads, and
+// loads from another CTA's shared memory.
+struct Cluster {
+  uint32_t rank, size;
+  __device__ __forceinline__ Cluster() {
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(size));
   }
+  __device__ __forceinline__ void sync() const {
+    if (size == 1) {
+      __syncthreads();
+    } else {
+      asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+      asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    }
+  }
+  __device__ __forceinline__ static uint32_t at(const void* p, uint32_t r) {
+    uint32_t addr;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(smem_u32(p)), "r"(r));
+    return addr;
+  }
+};
+
+// The bin from the top in which the left-th key lies: (bin, keys still wanted
+// of it), for the whole cluster. hist holds kBins bins in each of its CTAs, all
+// written before a cluster barrier.
+__device__ __forceinline__ int2 find_bin(const Cluster& cl, const int* hist, int left,
+                                         int* warp_sums, int* found) {
+  constexpr int kPer = kBins / kSelThreads;
+  static_assert(kPer == 4, "a thread reads its bins as one vector");
+  const int tid = threadIdx.x;
+  const int4* at = reinterpret_cast<const int4*>(hist) + (kSelThreads - 1 - tid);
+  int4 x = *at;
+  if (cl.size > 1) {
+    for (uint32_t r = 1; r < cl.size; ++r) {  // the others, each CTA from its own neighbour on
+      uint32_t other = cl.rank + r;
+      if (other >= cl.size) other -= cl.size;
+      int4 y;
+      asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(y.x), "=r"(y.y), "=r"(y.z), "=r"(y.w)
+                   : "r"(Cluster::at(at, other)));
+      x.x += y.x;
+      x.y += y.y;
+      x.z += y.z;
+      x.w += y.w;
+    }
+  }
+  const int mine[kPer] = {x.w, x.z, x.y, x.x};
   int total;
-  int above = block_scan(sum, warp_sums, total);
+  int above = block_scan(x.x + x.y + x.z + x.w, warp_sums, total);
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     if (above < left && left <= above + mine[i]) {
@@ -102,11 +140,11 @@ __device__ __forceinline__ int2 find_bin(const int* hist, int left, int* warp_su
   }
   __syncthreads();
   const int2 r = make_int2(found[0], found[1]);
-  __syncthreads();  // hist and found may be written again
+  __syncthreads();  // found may be written again
   return r;
 }
 
-// One CTA per (sequence, KV head). The `want` best of the tokens between sink
+// One CTA, or a cluster of them, per (sequence, KV head). The `want` best of the tokens between sink
 // and the recent ones are found by a radix select over their ordered scores:
 // a histogram of the first 11 bits gives the bin in which the want-th key lies;
 // a second sweep over the scores notes for every token whether it is above that
@@ -117,26 +155,29 @@ __device__ __forceinline__ int2 find_bin(const int* hist, int left, int* warp_su
 // a note is a byte per four tokens (above the threshold, at it). A sequence of
 // more than `room` tokens is read again for the output, and so is one whose bin
 // has more than kSelList keys (equal or close scores). 64 sequences of up to 32k
-// tokens, 8 heads: 52 us, two thirds of it the longest lists' own time (75 us with
-// all keys in shared memory and one CTA an SM; with 256 or 1024 threads 79, 65).
+// tokens, 8 heads: 40 us, bound by the instructions of the two sweeps, some forty a
+// token (75 us with all keys in shared memory and one CTA an SM; 52 with a byte's
+// tokens written at a time and a branch a token). With 256 threads 79, with 1024 65.
 __global__ void __launch_bounds__(kSelThreads, 3)
     select_kernel(const float* __restrict__ scores, const SeqTable table,
-                  int32_t* __restrict__ kept, int hkv, int budget, int sink, int recent, int room,
-                  bool ranked, unsigned int* err) {
+                  int32_t* __restrict__ kept, int batch, int hkv, int budget, int sink,
+                  int recent, int room, bool ranked, unsigned int* err) {
   extern __shared__ uint32_t notes32[];  // notes, four a word
-  __shared__ int hist[kBins];
+  __shared__ __align__(16) int hist[kBins], hist1[kBins], hist2[kBins];
   __shared__ uint2 list[kSelList];  // key, token
   __shared__ int warp_sums[kSelWarps];
+  __shared__ __align__(8) int counts[2];
   __shared__ int found[2], listed, ranks[kRankBatch];
   pdl_trigger();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0;
+  for (int i = tid; i < kBins; i += kSelThreads) hist[i] = hist1[i] = hist2[i] = 0;
   if (tid == 0) listed = 0;
+  const Cluster cl;
+  const int lists_at = blockIdx.x / cl.size;
   pdl_wait();  // the scores come from, and the lists may come from, earlier kernels
-  int b = blockIdx.x / hkv, p0, n;
-  const int h = blockIdx.x % hkv;
+  int b = lists_at / hkv, p0, n;
+  const int h = lists_at % hkv;
   if (ranked) {  // the b-th longest sequence
-    const int batch = gridDim.x / hkv;
     if (tid < kRankBatch) {
       int len = -1;
       if (tid < batch && !sequence(table, tid, p0, len)) len = 0;
@@ -153,25 +194,25 @@ __global__ void __launch_bounds__(kSelThreads, 3)
     b = found[0];
   }
   int32_t* out = kept + (static_cast<int64_t>(b) * hkv + h) * budget;
+  const int all_tid = cl.rank * kSelThreads + tid, all_threads = cl.size * kSelThreads;
   if (!sequence(table, b, p0, n)) {
     if (tid == 0 && h == 0) raise_device_error(err, FE_DEVERR_PAGE_RANGE);
-    for (int i = tid; i < budget; i += kSelThreads) out[i] = -1;
+    for (int i = all_tid; i < budget; i += all_threads) out[i] = -1;
     return;
   }
   if (n <= budget) {
-    for (int i = tid; i < budget; i += kSelThreads) out[i] = i < n ? i : -1;
+    for (int i = all_tid; i < budget; i += all_threads) out[i] = i < n ? i : -1;
     return;
   }
   const int end = n - recent, want = budget - sink - recent;
-  for (int i = tid; i < sink; i += kSelThreads) out[i] = i;
-  for (int i = tid; i < recent; i += kSelThreads) out[budget - recent + i] = end + i;
+  for (int i = all_tid; i < sink; i += all_threads) out[i] = i;
+  for (int i = all_tid; i < recent; i += all_threads) out[budget - recent + i] = end + i;
   if (want == 0) return;
   const float* sc = scores + static_cast<int64_t>(h) * table.cache_slots;
-  uint8_t* notes = reinterpret_cast<uint8_t*>(notes32);
-  const bool noted = n <= room;
   const int per16 = table.page / 16;
   // the page of tokens 4g .. 4g + 3, whose slots are adjacent, and their scores
   const int num_pages = static_cast<int>(table.cache_slots / table.page);
+  uint8_t* notes = reinterpret_cast<uint8_t*>(notes32);  // of group 4 * wa on
   auto page_of = [&](int g) {
     return __ldg(table.pages + p0 + (per16 == 1 ? g >> 2 : (g >> 2) / per16));
   };
@@ -187,10 +228,16 @@ __global__ void __launch_bounds__(kSelThreads, 3)
   auto keys = [&](const float4& x) {
     return make_uint4(ordered(x.x), ordered(x.y), ordered(x.z), ordered(x.w));
   };
-  const int ga = sink / 4, gb = (end + 3) / 4;
-  if (noted && tid == 0) {  // (the sweeps write the notes of [ga, gb) only)
-    notes32[ga / 4] = 0;
-    notes32[(gb - 1) / 4] = 0;
+  // this CTA's stretch of groups, in whole words of notes: [ga, gb), words from wa on
+  const int first_word = sink / 16, end_word = (end + 15) / 16;
+  const int part = (end_word - first_word + cl.size - 1) / cl.size;
+  const int wa = min(end_word, first_word + static_cast<int>(cl.rank) * part);
+  const int wb = min(end_word, wa + part);
+  const int ga = max(4 * wa, sink / 4), gb = min(4 * wb, (end + 3) / 4);
+  const bool noted = (wb - wa) * 16 <= room;
+  if (noted && tid == 0 && wa < wb) {  // (the sweeps write the notes of [ga, gb) only)
+    notes32[0] = 0;
+    notes32[wb - 1 - wa] = 0;
   }
   // f(i, key) for the tokens 4g + i of a group that lie between sink and end
   auto each = [&](int g, const uint4& x, auto&& f) {
@@ -233,53 +280,49 @@ __global__ void __launch_bounds__(kSelThreads, 3)
   sweep([&](int g, const uint4& x) {
     each(g, x, [&](int, uint32_t k) { atomicAdd(&hist[k >> 21], 1); });
   });
-  __syncthreads();
-  int2 at = find_bin(hist, want, warp_sums, found);
+  cl.sync();
+  int2 at = find_bin(cl, hist, want, warp_sums, found);
   uint32_t prefix = static_cast<uint32_t>(at.x) << 21;
   int left = at.y;  // of the keys that begin with prefix
   const uint32_t bin_end = prefix | ((1u << 21) - 1);
   // ---- the rest of the threshold's bits, over the keys of its bin
-  for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0;
-  __syncthreads();
   sweep([&](int g, const uint4& x) {
     uint32_t note = 0;
     each(g, x, [&](int i, uint32_t k) {
       note |= (k > bin_end ? 1u : k >= prefix ? 16u : 0u) << i;
     });
     const uint32_t in_bin = note >> 4;
-    if (noted) notes[g] = note & 15u;
+    if (noted) notes[g - 4 * wa] = note & 15u;
     if (in_bin) {
       int at = atomicAdd(&listed, __popc(in_bin));
       const uint32_t v[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         if (!(in_bin >> i & 1)) continue;
-        atomicAdd(&hist[(v[i] >> 10) & 2047], 1);
+        atomicAdd(&hist1[(v[i] >> 10) & 2047], 1);
         if (at < kSelList) list[at] = make_uint2(v[i], 4 * g + i);
         ++at;
       }
     }
   });
-  __syncthreads();
+  cl.sync();
   const bool whole = listed <= kSelList;  // the list holds the bin
   const int count = min(listed, kSelList);
-  at = find_bin(hist, left, warp_sums, found);
+  at = find_bin(cl, hist1, left, warp_sums, found);
   prefix |= static_cast<uint32_t>(at.x) << 10;
   left = at.y;
-  for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0;
-  __syncthreads();
   if (whole) {
     for (int i = tid; i < count; i += kSelThreads)
-      if ((list[i].x >> 10) == (prefix >> 10)) atomicAdd(&hist[list[i].x & 1023], 1);
+      if ((list[i].x >> 10) == (prefix >> 10)) atomicAdd(&hist2[list[i].x & 1023], 1);
   } else {
     sweep([&](int g, const uint4& x) {
       each(g, x, [&](int, uint32_t k) {
-        if ((k >> 10) == (prefix >> 10)) atomicAdd(&hist[k & 1023], 1);
+        if ((k >> 10) == (prefix >> 10)) atomicAdd(&hist2[k & 1023], 1);
       });
     });
   }
-  __syncthreads();
-  at = find_bin(hist, left, warp_sums, found);
+  cl.sync();
+  at = find_bin(cl, hist2, left, warp_sums, found);
   prefix |= static_cast<uint32_t>(at.x);
   left = at.y;
   // ---- the notes against the threshold itself: bits 0-3 above it, 4-7 at it
@@ -294,22 +337,21 @@ __global__ void __launch_bounds__(kSelThreads, 3)
     for (int i = tid; i < count; i += kSelThreads) {
       const uint2 e = list[i];
       const uint32_t bit = (e.x > prefix ? 1u : e.x == prefix ? 16u : 0u) << (e.y & 3);
-      const int g = static_cast<int>(e.y) >> 2;
+      const int g = (static_cast<int>(e.y) >> 2) - 4 * wa;
       if (bit) atomicOr(&notes32[g >> 2], bit << (8 * (g & 3)));
     }
   } else if (noted) {
-    sweep([&](int g, const uint4& x) { notes[g] = judge(g, x); });
+    sweep([&](int g, const uint4& x) { notes[g - 4 * wa] = judge(g, x); });
   }
   __syncthreads();
   // ---- kept tokens in order: a warp owns a stretch of the groups, a lane four of
   // them at a time: sixteen tokens, bit t of `mg` / `me` token t above / at it
-  const int wa = ga / 4, wb = (gb + 3) / 4;
   const int per = ((wb - wa + kSelWarps - 1) / kSelWarps + 31) / 32 * 32;
   const int w0 = min(wb, wa + warp * per), w1 = min(wb, w0 + per);
   auto word = [&](int w, uint32_t& mg, uint32_t& me) {
     uint32_t x = 0;
     if (noted) {
-      x = notes32[w];
+      x = notes32[w - wa];
     } else {
 #pragma unroll 1
       for (int i = 0; i < 4; ++i) {
@@ -337,11 +379,24 @@ __global__ void __launch_bounds__(kSelThreads, 3)
     gt += __shfl_xor_sync(0xffffffffu, gt, o);
     eq += __shfl_xor_sync(0xffffffffu, eq, o);
   }
-  int total;
-  int gt0 = block_scan(lane == 0 ? gt : 0, warp_sums, total);
+  int total_gt, total;
+  int gt0 = block_scan(lane == 0 ? gt : 0, warp_sums, total_gt);
   int eq0 = block_scan(lane == 0 ? eq : 0, warp_sums, total);
   gt0 = __shfl_sync(0xffffffffu, gt0, 0);
   eq0 = __shfl_sync(0xffffffffu, eq0, 0);
+  if (cl.size > 1) {  // what the CTAs before this one keep
+    if (tid == 0) counts[0] = total_gt;
+    if (tid == 0) counts[1] = total;
+    cl.sync();
+    for (uint32_t r = 0; r < cl.rank; ++r) {
+      int x, y;
+      asm volatile("ld.shared::cluster.v2.s32 {%0, %1}, [%2];"
+                   : "=r"(x), "=r"(y)
+                   : "r"(Cluster::at(counts, r)));
+      gt0 += x;
+      eq0 += y;
+    }
+  }
   for (int wbase = w0; wbase < w1; wbase += 32) {
     const int w = wbase + lane;
     uint32_t mg = 0, me = 0;
@@ -367,6 +422,7 @@ __global__ void __launch_bounds__(kSelThreads, 3)
     gt0 += all & 0xffff;
     eq0 += all >> 16;
   }
+  if (cl.size > 1) cl.sync();  // the others have read this CTA's shared memory
 }
 
 // ---------------------------------------------------------------------------
@@ -517,7 +573,6 @@ int fe_kv_select(const float* scores, const int32_t* kv, const int32_t* pages, i
     return fail(FE_ERR_INVALID_ARGUMENT, "fe_kv_select: scores must be 16-byte aligned");
   const SeqTable table{kv, pages, last, num_pages, page, cache_slots};
   auto s = static_cast<cudaStream_t>(stream);
-  const int room = std::min(max_len, kSelRoom);
   static std::once_flag once;
   static cudaError_t attr = cudaSuccess;
   std::call_once(once, [] {
@@ -527,10 +582,31 @@ int fe_kv_select(const float* scores, const int32_t* kv, const int32_t* pages, i
   if (attr != cudaSuccess) return cuda_fail(attr, "fe_kv_select: shared memory attribute");
   // more lists than SMs: the longest first, so that the last to end are short. Not
   // for large batches, where a CTA's look at all lengths costs more than it gives.
-  const bool ranked = batch <= kRankBatch && batch * hkv > 148;
-  FE_CUDA_TRY(launch_pdl(select_kernel, dim3(batch * hkv), dim3(kSelThreads),
-                         static_cast<size_t>(room + 15) / 16 * 4, s, scores, table, kept, hkv,
-                         budget, sink, recent, room, ranked, device_error_word()));
+  const int lists = batch * hkv;
+  const bool ranked = batch <= kRankBatch && lists > 148;
+  // few long lists: a cluster of CTAs each, of at least kSelPart tokens a CTA (8 lists
+  // of 32k tokens 25.7 us with one CTA each, 16.6 with eight; of 8k 11.0 with one,
+  // 11.7 with four, 16.1 with eight; 512 lists 40 us with one, 53 with two)
+  int cluster = 1;
+  while (cluster < kSelCluster && lists * cluster * 2 <= kSelCtas &&
+         max_len >= 2 * cluster * kSelPart)
+    cluster *= 2;
+  const int room = std::min(max_len / cluster + 32, kSelRoom);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(lists * cluster);
+  cfg.blockDim = dim3(kSelThreads);
+  cfg.dynamicSmemBytes = static_cast<size_t>(room + 15) / 16 * 4;
+  cfg.stream = s;
+  cudaLaunchAttribute attrs[2];
+  attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attrs[0].val.programmaticStreamSerializationAllowed = 1;
+  attrs[1].id = cudaLaunchAttributeClusterDimension;
+  attrs[1].val.clusterDim.x = cluster;
+  attrs[1].val.clusterDim.y = attrs[1].val.clusterDim.z = 1;
+  cfg.attrs = attrs;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  FE_CUDA_TRY(cudaLaunchKernelEx(&cfg, select_kernel, scores, table, kept, batch, hkv, budget,
+                                 sink, recent, room, ranked, device_error_word()));
   return FE_OK;
 }
 

@@ -41,7 +41,10 @@ SELECT = [  # lens, page, hkv, budget, sink, recent
     ([1], 16, 1, 1, 0, 0), ([2, 1, 16, 17], 16, 3, 1, 0, 1), ([5], 16, 2, 3, 0, 0),
     ([33, 700, 64], 32, 8, 64, 4, 16), ([1000] * 4, 16, 8, 384, 4, 64),
     ([513, 512, 511], 48, 5, 512, 0, 512), ([4097], 64, 4, 100, 100, 0),
-    ([20000, 37], 16, 2, 1024, 4, 128), ([50000], 16, 1, 300, 4, 10), ([3000], 16, 4, 2999, 1, 1)]
+    ([20000, 37], 16, 2, 1024, 4, 128), ([50000], 16, 1, 300, 4, 10), ([3000], 16, 4, 2999, 1, 1),
+    ([70000, 300, 9000, 70000], 16, 2, 5000, 20, 333), ([40001] * 3, 48, 3, 39000, 17, 19),
+    ([37 * i % 900 + 1 for i in range(40)], 16, 5, 200, 3, 30),
+    ([53 * i % 400 + 1 for i in range(130)], 16, 2, 100, 0, 9)]
 
 
 @pytest.mark.parametrize("case", SELECT)
