@@ -33,9 +33,8 @@ namespace fe {
 
 int decode_launch(int dtype, int dim, int heads, const CUtensorMap& kmap, const CUtensorMap& vmap,
                   bool per_head_tma, const void* args, int grid, cudaStream_t stream);
-int decode_ext_launch(int dtype, int dim, int heads, const CUtensorMap& kmap,
-                      const CUtensorMap& vmap, bool per_head_tma, const void* args, int grid,
-                      cudaStream_t stream);
+int decode_ext_launch(int dtype, int heads, const CUtensorMap& kmap, const CUtensorMap& vmap,
+                      bool per_head_tma, const void* args, int grid, cudaStream_t stream);
 int decode_merge_launch(int dtype, int dim, int list, const void* args, int grid, int grid_rows,
                         cudaStream_t stream, bool pdl);
 
@@ -82,20 +81,7 @@ __device__ __forceinline__ __half to_elem<__half>(float x) {
   return __float2half_rn(x);
 }
 
-// Where the raw scores of item tile `jt` of head `hh` go (the scored form):
-// [KV head][key tile][16 keys][Pp columns] fp32 per sequence, Pp = the packed
-// rows rounded up to even.
-template <typename T>
-__device__ __forceinline__ float* score_tile(const AttnArgs<T>& a, const WorkItem& wi,
-                                             const SeqInfo& si, int hh, int jt, int cols) {
-  const MetaHeader* hdr = reinterpret_cast<const MetaHeader*>(a.meta);
-  const int64_t* off = reinterpret_cast<const int64_t*>(a.meta + hdr->sink_off);
-  const int tiles = (si.length + kTileTokens - 1) / kTileTokens;
-  return a.sink + off[wi.seq] +
-         (static_cast<int64_t>(wi.kvh + hh) * tiles + wi.kt0 + jt) * (kTileTokens * cols);
-}
-
-template <typename T, int H, int NT, bool kInlineMerge, bool kExt = false>
+template <typename T, int H, int NT, bool kInlineMerge>
 __device__ __forceinline__ void decode_item(const AttnArgs<T>& a, const WorkItem& wi,
                                             const SeqInfo& si, const SplitGroup* groups,
                                             uint8_t* stages, uint64_t* full, uint64_t* empty,
@@ -106,8 +92,7 @@ __device__ __forceinline__ void decode_item(const AttnArgs<T>& a, const WorkItem
   const int G = a.G;
   const int P = si.qrows * G;
   const int head0 = (wi.kvh + hh) * G;
-  // kExt: items of a shared prefix (key_mode 2) are seen whole by every row
-  const bool causal = a.view == 1 && (!kExt || wi.key_mode == 1);
+  const bool causal = a.view == 1;
   KeyState<T, NT> ks;
   ks.init(a.q, a.hq, si.q_row0, si.qrows, si.length, head0, G, causal, lane);
 
@@ -123,13 +108,7 @@ __device__ __forceinline__ void decode_item(const AttnArgs<T>& a, const WorkItem
     TileAddr t;
     t.k = base + (2 * hh) * kHalfBytes;
     t.v = t.k + C::kKBytes;
-    if (kExt && a.sink) {
-      const int cols = (P + 1) & ~1;
-      ks.template tile<true>(t, (wi.kt0 + jt) * kTileTokens, si.length, a.scale_log2, lane,
-                             score_tile(a, wi, si, hh, jt, cols), cols, cols);
-    } else {
-      ks.tile(t, (wi.kt0 + jt) * kTileTokens, si.length, a.scale_log2, lane);
-    }
+    ks.tile(t, (wi.kt0 + jt) * kTileTokens, si.length, a.scale_log2, lane);
     __syncwarp();
     if (lane == 0) mbar_arrive_cnt(&empty[s], C::kWh);
   }
@@ -243,12 +222,25 @@ __device__ __forceinline__ void decode_item(const AttnArgs<T>& a, const WorkItem
   }
 }
 
+// Where the raw scores of item tile `jt` of head `hh` go (the scored form):
+// [KV head][key tile][16 keys][Pp columns] fp32 per sequence, Pp = the packed
+// rows rounded up to even.
+template <typename T>
+__device__ __forceinline__ float* score_tile(const AttnArgs<T>& a, const WorkItem& wi,
+                                             const SeqInfo& si, int hh, int jt, int cols) {
+  const MetaHeader* hdr = reinterpret_cast<const MetaHeader*>(a.meta);
+  const int64_t* off = reinterpret_cast<const int64_t*>(a.meta + hdr->sink_off);
+  const int tiles = (si.length + kTileTokens - 1) / kTileTokens;
+  return a.sink + off[wi.seq] +
+         (static_cast<int64_t>(wi.kvh + hh) * tiles + wi.kt0 + jt) * (kTileTokens * cols);
+}
+
 // head_dim 256: warp w serves group w % (H*C) = (head hh, column half ch),
 // C = 2 when the item has more than 8 packed rows; the kWh = 8/(H*C) warps of
 // a group take alternate tiles, then fold their states pairwise (round `step`:
 // warps step..2*step-1 of the group stash, warps 0..step-1 absorb), so the
 // group's first warp ends with the item's whole key range.
-template <typename T, int H, bool kExt = false>
+template <typename T, int H, bool kExt>
 __device__ __forceinline__ void decode_item_d256(const AttnArgs<T>& a, const WorkItem& wi,
                                                  const SeqInfo& si, uint8_t* stages,
                                                  uint64_t* full, uint64_t* empty,
@@ -264,6 +256,7 @@ __device__ __forceinline__ void decode_item_d256(const AttnArgs<T>& a, const Wor
   const int grp = w % groups, sub = w / groups;
   const int hh = grp % H, ch = grp / H;
   const int head0 = (wi.kvh + hh) * G;
+  // kExt: items of a shared prefix (key_mode 2) are seen whole by every row
   const bool causal = a.view == 1 && (!kExt || wi.key_mode == 1);
   KeyState<T, 1, D> ks;
   ks.init(a.q, a.hq, si.q_row0, si.qrows, si.length, head0, G, causal, lane, ch * 8);
@@ -332,8 +325,9 @@ __device__ __forceinline__ void decode_item_d256(const AttnArgs<T>& a, const Wor
   }
 }
 
-// kExt: the lists of shared-prefix and scored plans (items that every row
-// sees whole, raw scores stored when a.sink is set).
+// kExt: the lists of shared-prefix and scored plans at head_dim 256 (items that
+// every row sees whole, raw scores stored when a.sink is set); at 128 their lists
+// are the key kernel's.
 template <typename T, int H, int D, bool kExt>
 __global__ void __launch_bounds__(kDecThreads, 1)
     paged_decode_kernel(const __grid_constant__ CUtensorMap kmap,
@@ -465,13 +459,14 @@ __global__ void __launch_bounds__(kDecThreads, 1)
     const WorkItem wi = items[it];
     const SeqInfo si = seqs[wi.seq];
     if constexpr (D != kHeadDim)
-      decode_item_d256<T, H, kExt>(a, wi, si, stages, full, empty, flags, comb, warp, lane, g, aborted);
+      decode_item_d256<T, H, kExt>(a, wi, si, stages, full, empty, flags, comb, warp, lane, g,
+                                   aborted);
     else if (si.qrows * a.G <= 8)
-      decode_item<T, H, 1, false, kExt>(a, wi, si, groups, stages, full, empty, flags, comb, warp,
-                                        lane, g, aborted);
+      decode_item<T, H, 1, false>(a, wi, si, groups, stages, full, empty, flags, comb, warp, lane,
+                                  g, aborted);
     else
-      decode_item<T, H, 2, false, kExt>(a, wi, si, groups, stages, full, empty, flags, comb, warp,
-                                        lane, g, aborted);
+      decode_item<T, H, 2, false>(a, wi, si, groups, stages, full, empty, flags, comb, warp, lane,
+                                  g, aborted);
   }
   if (aborted && lane == 0) raise_device_error(a.err, FE_DEVERR_TIMEOUT);
 }
@@ -487,8 +482,8 @@ int launch_t(const CUtensorMap& kmap, const CUtensorMap& vmap, bool per_head_tma
                                     cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
   });
   if (attr_err != cudaSuccess) return cuda_fail(attr_err, "paged_decode_kernel attribute");
-  FE_CUDA_TRY(launch_pdl(paged_decode_kernel<T, H, D, kExt>, dim3(grid), dim3(kDecThreads), C::kSmem,
-                         stream, kmap, vmap, args, per_head_tma ? 1 : 0));
+  FE_CUDA_TRY(launch_pdl(paged_decode_kernel<T, H, D, kExt>, dim3(grid), dim3(kDecThreads),
+                         C::kSmem, stream, kmap, vmap, args, per_head_tma ? 1 : 0));
   return FE_OK;
 }
 
@@ -688,18 +683,23 @@ int decode_merge_launch(int dtype, int dim, int list, const void* args, int grid
 namespace {
 
 template <typename T, bool kExt>
-int launch_heads(int dim, int heads, const CUtensorMap& kmap, const CUtensorMap& vmap,
-                 bool per_head_tma, const void* args, int grid, cudaStream_t stream) {
+int launch_wide(int heads, const CUtensorMap& kmap, const CUtensorMap& vmap, bool per_head_tma,
+                const void* args, int grid, cudaStream_t stream) {
   const auto& a = *static_cast<const AttnArgs<T>*>(args);
-  if (dim == kWideHeadDim)
-    return heads == 2
-               ? launch_t<T, 2, kWideHeadDim, kExt>(kmap, vmap, per_head_tma, a, grid, stream)
-               : launch_t<T, 1, kWideHeadDim, kExt>(kmap, vmap, per_head_tma, a, grid, stream);
+  return heads == 2
+             ? launch_t<T, 2, kWideHeadDim, kExt>(kmap, vmap, per_head_tma, a, grid, stream)
+             : launch_t<T, 1, kWideHeadDim, kExt>(kmap, vmap, per_head_tma, a, grid, stream);
+}
+
+template <typename T>
+int launch_heads(int heads, const CUtensorMap& kmap, const CUtensorMap& vmap, bool per_head_tma,
+                 const void* args, int grid, cudaStream_t stream) {
+  const auto& a = *static_cast<const AttnArgs<T>*>(args);
   switch (heads) {
-    case 8: return launch_t<T, 8, kHeadDim, kExt>(kmap, vmap, per_head_tma, a, grid, stream);
-    case 4: return launch_t<T, 4, kHeadDim, kExt>(kmap, vmap, per_head_tma, a, grid, stream);
-    case 2: return launch_t<T, 2, kHeadDim, kExt>(kmap, vmap, per_head_tma, a, grid, stream);
-    default: return launch_t<T, 1, kHeadDim, kExt>(kmap, vmap, per_head_tma, a, grid, stream);
+    case 8: return launch_t<T, 8>(kmap, vmap, per_head_tma, a, grid, stream);
+    case 4: return launch_t<T, 4>(kmap, vmap, per_head_tma, a, grid, stream);
+    case 2: return launch_t<T, 2>(kmap, vmap, per_head_tma, a, grid, stream);
+    default: return launch_t<T, 1>(kmap, vmap, per_head_tma, a, grid, stream);
   }
 }
 
@@ -707,17 +707,19 @@ int launch_heads(int dim, int heads, const CUtensorMap& kmap, const CUtensorMap&
 
 int decode_launch(int dtype, int dim, int heads, const CUtensorMap& kmap, const CUtensorMap& vmap,
                   bool per_head_tma, const void* args, int grid, cudaStream_t stream) {
-  auto run = dtype == FE_DTYPE_BF16 ? launch_heads<__nv_bfloat16, false>
-                                    : launch_heads<__half, false>;
-  return run(dim, heads, kmap, vmap, per_head_tma, args, grid, stream);
+  const bool bf16 = dtype == FE_DTYPE_BF16;
+  if (dim == kWideHeadDim) {
+    auto run = bf16 ? launch_wide<__nv_bfloat16, false> : launch_wide<__half, false>;
+    return run(heads, kmap, vmap, per_head_tma, args, grid, stream);
+  }
+  auto run = bf16 ? launch_heads<__nv_bfloat16> : launch_heads<__half>;
+  return run(heads, kmap, vmap, per_head_tma, args, grid, stream);
 }
 
-int decode_ext_launch(int dtype, int dim, int heads, const CUtensorMap& kmap,
-                      const CUtensorMap& vmap, bool per_head_tma, const void* args, int grid,
-                      cudaStream_t stream) {
-  auto run = dtype == FE_DTYPE_BF16 ? launch_heads<__nv_bfloat16, true>
-                                    : launch_heads<__half, true>;
-  return run(dim, heads, kmap, vmap, per_head_tma, args, grid, stream);
+int decode_ext_launch(int dtype, int heads, const CUtensorMap& kmap, const CUtensorMap& vmap,
+                      bool per_head_tma, const void* args, int grid, cudaStream_t stream) {
+  auto run = dtype == FE_DTYPE_BF16 ? launch_wide<__nv_bfloat16, true> : launch_wide<__half, true>;
+  return run(heads, kmap, vmap, per_head_tma, args, grid, stream);
 }
 
 }  // namespace fe

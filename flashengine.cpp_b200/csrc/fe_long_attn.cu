@@ -22,14 +22,13 @@
 
 namespace fe {
 
-int decode_ext_launch(int dtype, int dim, int heads, const CUtensorMap& kmap,
-                      const CUtensorMap& vmap, bool per_head_tma, const void* args, int grid,
-                      cudaStream_t stream);
+int decode_ext_launch(int dtype, int heads, const CUtensorMap& kmap, const CUtensorMap& vmap,
+                      bool per_head_tma, const void* args, int grid, cudaStream_t stream);
 int keys_launch(int dtype, const CUtensorMap& kmap, const CUtensorMap& vmap, const void* args,
                 int grid, bool beside, cudaStream_t stream);
 int rows2_launch(int dtype, const CUtensorMap& kmap, const CUtensorMap& vmap,
                  const CUtensorMap& qmap, const void* args, int grid, cudaStream_t stream);
-int prefill_tc_ext_launch(int dtype, int dim, const CUtensorMap& kmap, const CUtensorMap& vmap,
+int prefill_tc_ext_launch(int dtype, const CUtensorMap& kmap, const CUtensorMap& vmap,
                           const CUtensorMap& qmap, const void* args, int grid,
                           cudaStream_t stream);
 
@@ -560,8 +559,8 @@ AttnArgs<T> long_args(const fe_long_plan* p, const void* q, void* out, int view,
 
 int launch_decode(fe_long_plan* p, const void* args, int grid, bool beside, cudaStream_t s) {
   if (p->keys) return keys_launch(p->dtype, p->kmap_dec, p->vmap_dec, args, grid, beside, s);
-  return decode_ext_launch(p->dtype, p->cfg.dim, p->cfg.dec_heads, p->kmap_dec, p->vmap_dec,
-                           p->per_head_tma, args, grid, s);
+  return decode_ext_launch(p->dtype, p->cfg.dec_heads, p->kmap_dec, p->vmap_dec, p->per_head_tma,
+                           args, grid, s);
 }
 
 template <typename T>
@@ -582,8 +581,8 @@ int run_shared(fe_long_plan* p, const void* q, void* out, int view, cudaStream_t
   if (grid_rows > 0) {
     int rc = c.dim == kHeadDim
                  ? rows2_launch(p->dtype, p->kmap_tc, p->vmap_tc, qmap, &a, grid_rows, s)
-                 : prefill_tc_ext_launch(p->dtype, c.dim, p->kmap_tc, p->vmap_tc, qmap, &a,
-                                         grid_rows, s);
+                 : prefill_tc_ext_launch(p->dtype, p->kmap_tc, p->vmap_tc, qmap, &a, grid_rows,
+                                         s);
     if (rc != FE_OK) return rc;
   }
   if (grid_dec > 0) {

@@ -365,7 +365,7 @@ int build_scored_plan(const PlanConfig& cfg, bool keys, const int32_t* qo, const
       err = "fresh[b] must be in [0, length] (b=" + std::to_string(b) + ")";
       return FE_ERR_INVALID_ARGUMENT;
     }
-    const int block0 = static_cast<int>(t.seqs.size()), unit0 = static_cast<int>(key.size());
+    const int block0 = static_cast<int>(t.seqs.size());
     for (int i = 0; i < s.qrows; i += per) {
       const int n = std::min(per, s.qrows - i), P = n * G;
       // up to the last key that the block's last row sees
@@ -384,8 +384,7 @@ int build_scored_plan(const PlanConfig& cfg, bool keys, const int32_t* qo, const
     }
     const int blocks = static_cast<int>(t.seqs.size()) - block0;
     for (int t0 = 0; t0 < s.length; t0 += kScoreChunk)
-      t.chunks.push_back(
-          ScoreChunk{block0, blocks, s.length, s.page_off, s.length - f, t0, unit0, 0});
+      t.chunks.push_back(ScoreChunk{block0, blocks, s.length, s.page_off, s.length - f, t0});
   }
   if (out.sink_floats > sink_capacity) {
     err = "query rows x keys exceed the plan's max_keys";

@@ -55,13 +55,11 @@ struct KeyItem {  // 48 bytes
 };
 
 // A stretch of keys whose scores one CTA and KV head update.
-struct ScoreChunk {  // 32 bytes
+struct ScoreChunk {  // 24 bytes
   int32_t block0, blocks;  // the sequence's row blocks (sequences of the lists)
   int32_t length, page_off;
   int32_t fresh;  // first key whose score is set and not added to
   int32_t t0;
-  int32_t unit0;  // first unit of block0; a block has hkv / dec_heads
-  int32_t pad;
 };
 constexpr int kScoreChunk = 512;  // keys
 

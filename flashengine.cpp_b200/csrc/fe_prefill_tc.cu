@@ -58,7 +58,7 @@ namespace fe {
 
 int prefill_tc_launch(int dtype, int dim, const CUtensorMap& kmap, const CUtensorMap& vmap,
                       const CUtensorMap& qmap, const void* args, int grid, cudaStream_t stream);
-int prefill_tc_ext_launch(int dtype, int dim, const CUtensorMap& kmap, const CUtensorMap& vmap,
+int prefill_tc_ext_launch(int dtype, const CUtensorMap& kmap, const CUtensorMap& vmap,
                           const CUtensorMap& qmap, const void* args, int grid,
                           cudaStream_t stream);
 
@@ -504,7 +504,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       // keys this row sees in this item: the mask's, cut at the end of the
       // item's pieces (a split item covers part of the range; head_dim 128
       // items are never split)
-      int lim = (causal && row_valid && (!kExt || w.key_mode == 0)) ? si.length - si.qrows + p / G + 1 : si.length;
+      int lim = (causal && row_valid && (!kExt || w.key_mode == 0))
+                    ? si.length - si.qrows + p / G + 1
+                    : si.length;
       if constexpr (kSplits) lim = min(lim, w.kt1 * kTileTokens);
       // m_used stays -inf until the first unmasked key (its weights are 0)
       float m_used = -INFINITY, l = 0.f;
@@ -727,7 +729,8 @@ template <typename T>
 int launch_dim(int dim, const CUtensorMap& kmap, const CUtensorMap& vmap, const CUtensorMap& qmap,
                const void* args, int grid, cudaStream_t stream) {
   const auto& a = *static_cast<const AttnArgs<T>*>(args);
-  if (dim == kWideHeadDim) return launch_t<T, kWideHeadDim, false>(kmap, vmap, qmap, a, grid, stream);
+  if (dim == kWideHeadDim)
+    return launch_t<T, kWideHeadDim, false>(kmap, vmap, qmap, a, grid, stream);
   return launch_t<T, kHeadDim, false>(kmap, vmap, qmap, a, grid, stream);
 }
 
@@ -739,10 +742,9 @@ int prefill_tc_launch(int dtype, int dim, const CUtensorMap& kmap, const CUtenso
   return run(dim, kmap, vmap, qmap, args, grid, stream);
 }
 
-int prefill_tc_ext_launch(int dtype, int dim, const CUtensorMap& kmap, const CUtensorMap& vmap,
+int prefill_tc_ext_launch(int dtype, const CUtensorMap& kmap, const CUtensorMap& vmap,
                           const CUtensorMap& qmap, const void* args, int grid,
                           cudaStream_t stream) {
-  if (dim != kWideHeadDim) return fail(FE_ERR_UNSUPPORTED, "row kernel of shared-prefix plans: dim");
   if (dtype == FE_DTYPE_BF16)
     return launch_t<__nv_bfloat16, kWideHeadDim, true>(
         kmap, vmap, qmap, *static_cast<const AttnArgs<__nv_bfloat16>*>(args), grid, stream);

@@ -514,6 +514,9 @@ int run_axes(const char* what, void* q, const void* k, const void* v, void* k_ou
   if (dim % 4 != 0 || rot < 0 || rot > dim || rot % 4 != 0 || rot > 2 * kMaxPairs)
     return fail(FE_ERR_UNSUPPORTED, name + ": dim and rotary_dim must be multiples of 4, "
                                            "rotary_dim <= dim and <= 512");
+  // (row and element indexes of a step ahead stay within 31 bits)
+  if (rows > (1 << 30) || (int64_t(hq) + hkv) * dim > (1 << 24))
+    return fail(FE_ERR_CAPACITY, name + ": at most 2^30 rows of 2^24 elements");
   if (rot > 0 && !pair_axis) return fail(FE_ERR_INVALID_ARGUMENT, name + ": pair_axis is null");
   AxisMap map{};
   for (int j = 0; j < rot / 2; ++j) {
@@ -533,6 +536,8 @@ int run_axes(const char* what, void* q, const void* k, const void* v, void* k_ou
                         static_cast<const void*>(cache)})
     if (reinterpret_cast<uintptr_t>(p) & 3u)
       return fail(FE_ERR_INVALID_ARGUMENT, name + ": buffers must be 4-byte aligned");
+  if ((reinterpret_cast<uintptr_t>(pos) | reinterpret_cast<uintptr_t>(slots)) & 7u)
+    return fail(FE_ERR_INVALID_ARGUMENT, name + ": pos and slots must be 8-byte aligned");
   const AxesArgs a{slots, pos, cache, device_error_word(), cache_slots, rows, axes, hq, hkv, dim,
                    rot, max_positions};
   auto s = static_cast<cudaStream_t>(stream);

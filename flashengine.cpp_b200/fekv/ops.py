@@ -1031,7 +1031,8 @@ class HostKv8Plan(HostPlan):
     _create = "fe_kv8_plan_create_host"
 
 
-__all__ = ["SharedPlan", "ScoredPlan", "shared_prefixes", "rope_sections", "rope_axes", "rope_axes_append", "select_tokens", "compact_tokens",
+__all__ = ["SharedPlan", "ScoredPlan", "shared_prefixes", "rope_sections", "rope_axes",
+           "rope_axes_append", "select_tokens", "compact_tokens",
            "Kv8Pool", "Kv8Plan", "HostKv8Plan", "append_kv8", "gather_kv8", "copy_blocks_kv8",
            "store", "copy_blocks", "paged_decode_noalloc", "clear_pages", "gather", "device_errors", "AttentionPlan",
            "create_plan", "destroy_plan", "prepare_plan", "attention", "HostPlan", "FeError",

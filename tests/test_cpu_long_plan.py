@@ -14,8 +14,7 @@ ROW = np.dtype([(n, "<i4") for n in ("own_unit", "own_blocks", "own_rows", "own_
 UNIT = np.dtype([(n, "<i4") for n in ("part0", "n", "rec_floats", "rows")])
 KEY = np.dtype([(n, "<i4") for n in ("q_row0", "qrows", "length", "page_off", "kvh", "key_mode",
                                      "kt0", "kt1", "part", "group", "seq", "pad")])
-CHUNK = np.dtype([(n, "<i4") for n in ("block0", "blocks", "length", "page_off", "fresh", "t0",
-                                       "unit0", "pad")])
+CHUNK = np.dtype([(n, "<i4") for n in ("block0", "blocks", "length", "page_off", "fresh", "t0")])
 
 
 class Host:
@@ -234,9 +233,9 @@ def test_scored_blocks_cover_rows_and_keys(shape):
             mine = [c for c in m.chunks if c["page_off"] == meta[1][b]]
             assert [c["t0"] for c in mine] == list(range(0, n, 512))
             assert all(c["length"] == n and c["fresh"] == n - fresh[b] for c in mine)
-            for j in range(mine[0]["blocks"]):  # units of its row blocks
-                r0 = int(m.seqs[mine[0]["block0"] + j]["q_row0"])
-                assert mine[0]["unit0"] + j * (hkv // m.H) == m.info[r0]["own_unit"]
+            units = [m.info[int(m.seqs[mine[0]["block0"] + j]["q_row0"])]["own_unit"]
+                     for j in range(mine[0]["blocks"])]  # of its row blocks
+            assert np.array_equal(np.diff(units), [hkv // m.H] * (len(units) - 1))
             s = m.seqs[mine[0]["block0"]:mine[0]["block0"] + mine[0]["blocks"]]
             assert s["qrows"].sum() == r and (s["qrows"] * (hq // hkv) <= 16).all()
             assert s["length"][-1] == n
