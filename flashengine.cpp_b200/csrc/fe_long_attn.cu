@@ -163,13 +163,14 @@ __device__ __forceinline__ void find_records(const AttnArgs<T>& a, int64_t w, Re
 }
 
 // One warp per query row and head; lse (scored plans): where m + log2 l of each
-// goes, fp32 [rows, hq]. Few pairs: all records of one in flight. Many: what counts
+// goes, fp32 [rows, hq]. Few pairs: four records of one in flight (eight: 2 us more
+// for 64 rows of 64 heads, whose warps are then not all resident). Many: what counts
 // are loads in flight an SM, so two records a warp and more warps (2048 rows of
 // 32 heads, 60 % with two records: 7 us less; 64 rows of 64 heads 2 us more).
 constexpr int kManyPairs = 148 * 48;
 
 template <typename T, int D, int kStep>
-__global__ void __launch_bounds__(kJoinThreads, kStep == 2 && D == kHeadDim ? 5 : 3)
+__global__ void __launch_bounds__(kJoinThreads, kStep == 2 && D == kHeadDim ? 5 : 4)
     join_kernel(const AttnArgs<T> a, float* lse) {
   pdl_trigger();
   const int lane = threadIdx.x & 31;
@@ -185,7 +186,7 @@ template <typename T, int D>
 int launch_join(const AttnArgs<T>& a, int rows, float* lse, cudaStream_t s) {
   const int64_t pairs = int64_t(rows) * a.hq;
   const int grid = static_cast<int>((pairs + kJoinWarps - 1) / kJoinWarps);
-  auto kernel = pairs > kManyPairs ? join_kernel<T, D, 2> : join_kernel<T, D, 8 * kHeadDim / D>;
+  auto kernel = pairs > kManyPairs ? join_kernel<T, D, 2> : join_kernel<T, D, 4 * kHeadDim / D>;
   FE_CUDA_TRY(launch_pdl(kernel, dim3(grid), dim3(kJoinThreads), 0, s, a, lse));
   return FE_OK;
 }
