@@ -407,7 +407,7 @@ int create_long(const char* what, int hq, int hkv, int dim, int page, int max_ba
   c.row_pair_blocks = dim == kHeadDim ? 8 : 0;
   c.row_min_piece = 2;
   c.elem_bytes = 2;
-  c.dec_min_tiles = p->keys ? 4 : 8;
+  c.dec_min_tiles = 4;
   c.max_items = c.max_groups = static_cast<int>(std::min<int64_t>(
       std::max<int64_t>(int64_t(max_batch) * hkv * 64, 8192), 1 << 20));
   c.partial_capacity = kLongPartialFloats;

@@ -46,13 +46,13 @@ struct Tables {
   std::vector<int64_t> sink;
 };
 
-// The decode list: for the key kernel cut by cost, a piece of a unit costing its
-// tiles and about kKeyItem more (its queries, first loads and record), else
-// evenly by tiles.
+// The decode list, cut by cost: a piece of a unit costs its tiles and about kKeyItem
+// more (its queries, first loads and record). Cut by tiles alone the short
+// sequences of a step fall to a few CTAs (three of 24 keys at head_dim 256: six
+// items to one CTA, 25 us).
 constexpr int kKeyItem = 4;
-int decode_view(const PlanConfig& cfg, bool keys, const std::vector<Unit>& units, int ctas,
-                bool fixed_grid, View& v, std::string& err) {
-  if (!keys) return build_cut_view(cfg, units, ctas, cfg.dec_min_tiles, fixed_grid, v, err);
+int decode_view(const PlanConfig& cfg, const std::vector<Unit>& units, int ctas, bool fixed_grid,
+                View& v, std::string& err) {
   PlanConfig c = cfg;
   c.row_tile = c.row_weight[0] = 1;
   c.row_item_tiles = kKeyItem;
@@ -255,7 +255,7 @@ int layout(const PlanConfig& cfg, bool keys, const std::vector<SeqInfo>& step, c
   View views[3];
   int rc = build_cost_view(cfg, full, row_sms, fixed_grid, views[0], err);
   if (rc == FE_OK) rc = build_cost_view(cfg, causal, row_sms, fixed_grid, views[1], err);
-  if (rc == FE_OK) rc = decode_view(cfg, keys, key, key_ctas, fixed_grid, views[2], err);
+  if (rc == FE_OK) rc = decode_view(cfg, key, key_ctas, fixed_grid, views[2], err);
   if (rc != FE_OK) return rc;
   fill_rows(t, rows, G);
   return pack(cfg, keys, views, t, pages, total_pages, batch, rows, out, err);
@@ -391,7 +391,7 @@ int build_scored_plan(const PlanConfig& cfg, bool keys, const int32_t* qo, const
     return FE_ERR_CAPACITY;
   }
   View views[3];
-  rc = decode_view(cfg, keys, key, cfg.dec_grid_cap, fixed_grid, views[2], err);
+  rc = decode_view(cfg, key, cfg.dec_grid_cap, fixed_grid, views[2], err);
   if (rc != FE_OK) return rc;
   fill_rows(t, rows, G);
   return pack(cfg, keys, views, t, pages, batch > 0 ? kv[batch] : 0, batch, rows, out, err);

@@ -131,12 +131,12 @@ __global__ void __launch_bounds__(kAxesThreads)
 // the last), so that a pair's axis costs one 4-byte copy a row and not one load
 // a head.
 constexpr int kRowBufs = 3;
-// From this many rows of this many bytes the ring of bulk copies is used: 4096 rows
-// of 8 + 2 heads of 128 (3 KiB) took 10.1 us by threads and 13.5 by the ring, 16 + 4
-// heads 17.7 and 16.3, 32 + 8 heads 22.5 and 20.4; 2048 rows of those 9.4 and 9.5,
-// 11.4 and 12.3.
+// From this many rows the ring of bulk copies is used (us by threads and by the
+// ring, head_dim 128): 4096 rows of 4 + 1 heads 8.7 and 9.9, of 16 + 1 heads 17.8 and
+// 13.0, of 32 + 8 heads 23.0 and 20.3; 2048 rows of those 5.4 and 8.0, 9.3 and 8.6,
+// 11.5 and 12.2; 32k rows of 4 + 1 heads 50.7 and 46.1, of 16 + 1 heads 170 and 69.
 constexpr int kBulkRows = 4096;
-constexpr int kBulkRowBytes = 4096;
+constexpr int kBulkSmem = 112 * 1024;
 
 template <typename T>
 __global__ void __launch_bounds__(kAxesThreads)
@@ -267,13 +267,14 @@ __global__ void __launch_bounds__(kAxesThreads)
 // rows ahead, and their positions and the slot four rows ahead. 64k rows of 32 + 8
 // heads of 128, 1.6 GB: 258 us, 6.4 TB/s (426 us by the kernel above). A row's
 // steps follow one another behind two barriers, so it is the CTAs of an SM that
-// overlap: five of 64 threads and three stages, where three of 256 threads and
-// five stages took 328 us, two with eight stages 437 us.
-constexpr int kBulkThreads = 64;
-constexpr int kMaxStages = 10;
+// overlap, as many as their stages leave room for: five of 64 threads and three
+// stages, where three of 256 threads and five stages took 328 us, two with eight
+// stages 437 us. Short rows take a warp a CTA (16 + 1 heads: 69 us, 75 with two
+// warps), long ones four (64 + 8 heads: 213 us, 248 with two).
+constexpr uint32_t kStages = 3;
 constexpr int kMetaBufs = 8;
 // (what lies between the stages and `turns`, which is read 16 bytes at a time)
-static_assert((kMaxStages + 2 + kMetaBufs * (kMaxAxes + 1)) % 2 == 0, "turns: 16-byte aligned");
+static_assert((kStages + 1 + kMetaBufs * (kMaxAxes + 1)) % 2 == 0, "turns: 16-byte aligned");
 
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes,
                                           uint64_t* bar) {
@@ -289,11 +290,11 @@ __device__ __forceinline__ void bulk_store(void* dst, const void* src, uint32_t 
                : "memory");
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kBulkThreads)
+template <typename T, int kThreads>
+__global__ void __launch_bounds__(kThreads)
     rope_axes_bulk_kernel(T* __restrict__ q, const T* k, const T* __restrict__ v, T* k_out,
                           T* __restrict__ kc, T* __restrict__ vc, const AxesArgs a,
-                          const AxisMap map, int stages) {
+                          const AxisMap map, uint32_t stages) {
   using V = typename Pair2<T>::V;
   union Chunk {
     uint4 u;
@@ -304,11 +305,11 @@ __global__ void __launch_bounds__(kBulkThreads)
   const uint32_t qb = a.hq * a.dim * 2, kb = a.hkv * a.dim * 2;
   const uint32_t stage_bytes = qb + kb + (kc ? kb : 0);
   uint64_t* full = reinterpret_cast<uint64_t*>(ring + stages * stage_bytes);
-  volatile int* flag = reinterpret_cast<volatile int*>(full + kMaxStages);
-  int64_t* meta = reinterpret_cast<int64_t*>(full + kMaxStages + 2);
+  volatile int* flag = reinterpret_cast<volatile int*>(full + kStages);
+  int64_t* meta = reinterpret_cast<int64_t*>(full + kStages + 1);
   float* turns = reinterpret_cast<float*>(meta + kMetaBufs * (kMaxAxes + 1));  // [kRowBufs][rot]
   if (threadIdx.x == 0) {
-    for (int s = 0; s < stages; ++s) mbar_init(&full[s], 1);
+    for (int s = 0; s < static_cast<int>(stages); ++s) mbar_init(&full[s], 1);
     *flag = 0;
     fence_barrier_init();
   }
@@ -343,7 +344,7 @@ __global__ void __launch_bounds__(kBulkThreads)
     if (row >= a.rows) return;
     const int64_t* m = meta + n % kMetaBufs * (kMaxAxes + 1);
     float* dst = turns + n % kRowBufs * a.rot;
-    for (int i = threadIdx.x; i < a.rot; i += kBulkThreads) {
+    for (int i = threadIdx.x; i < a.rot; i += kThreads) {
       const int64_t p = m[map.axis[i < r ? i : i - r]];
       // a row that is out of range is skipped below; its copies stay in bounds
       const float* src = a.cache + (p >= 0 && p < a.max_positions ? p : 0) * a.rot + i;
@@ -352,11 +353,10 @@ __global__ void __launch_bounds__(kBulkThreads)
     }
   };
   const int64_t step = gridDim.x;
-  const int lag = stages > 3 ? 2 : 1;  // rows whose stores may still read their stage
   int64_t fetched = blockIdx.x;        // next row to fetch (thread 0)
   uint32_t nf = 0, n = 0;              // rows fetched, rows done
   if (threadIdx.x == 0)
-    for (; static_cast<int>(nf) < stages - lag && fetched < a.rows; fetched += step, ++nf)
+    for (; nf < stages - 1 && fetched < a.rows; fetched += step, ++nf)
       fetch(fetched, nf);
   for (uint32_t i = 0; i < 4; ++i) meta_ahead(blockIdx.x + i * step, i);
   commit();
@@ -368,7 +368,7 @@ __global__ void __launch_bounds__(kBulkThreads)
   }
   bool ok = true;
   for (int64_t row = blockIdx.x; row < a.rows; row += step, ++n) {
-    const int s = n % stages;
+    const uint32_t s = n % stages;
     asm volatile("cp.async.wait_group 1;" ::: "memory");
     ok = wait_bounded(&full[s], (n / stages) & 1u, flag);
     if (!__syncthreads_and(ok)) {  // (and what came by cp.async is there for everyone)
@@ -384,7 +384,7 @@ __global__ void __launch_bounds__(kBulkThreads)
     const float* cs = turns + n % kRowBufs * a.rot;
     uint8_t* st = ring + s * stage_bytes;
     if (good) {
-      for (int t = threadIdx.x; t < heads * rot_units; t += kBulkThreads) {
+      for (int t = threadIdx.x; t < heads * rot_units; t += kThreads) {
         const int head = t / rot_units, u = t - head * rot_units;
         uint4* x = reinterpret_cast<uint4*>(st + head * a.dim * 2) + u;
         uint4* y = x + r / 8;
@@ -422,12 +422,9 @@ __global__ void __launch_bounds__(kBulkThreads)
         }
       }
       asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-      // the stage of the row `lag` before this one is free once its stores have read it
+      // the stage of the row before this one is free once its stores have read it
       if (fetched < a.rows) {
-        if (lag == 2)
-          asm volatile("cp.async.bulk.wait_group.read 2;" ::: "memory");
-        else
-          asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+        asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
         fetch(fetched, nf % stages);
         fetched += step;
         ++nf;
@@ -461,33 +458,36 @@ int launch_axes(void* q, const void* k, const void* v, void* k_out, void* kc, vo
     const int most = kAxesThreads / units;
     const int passes = (heads + most - 1) / most;
     const int hl = (heads + passes - 1) / passes;
-    const int threads = (hl * units + 31) / 32 * 32;
+    const int vec_threads = (hl * units + 31) / 32 * 32;
     const int stage = (heads + (kc ? a.hkv : 0)) * a.dim * 2;
-    const int extra =
-        8 * (kMaxStages + 2 + kMetaBufs * (kMaxAxes + 1)) + 4 * kRowBufs * a.rot;
-    // at least three stages; many small CTAs rather than few large ones
-    const int stages = std::min(kMaxStages, std::max(3, (38 * 1024 - extra) / stage));
-    const int smem = stages * stage + extra;
-    if (a.rows >= kBulkRows && stage >= kBulkRowBytes && smem <= 112 * 1024) {
+    const int smem = static_cast<int>(kStages) * stage +
+                     8 * (kStages + 1 + kMetaBufs * (kMaxAxes + 1)) + 4 * kRowBufs * a.rot;
+    if (a.rows >= kBulkRows && smem <= kBulkSmem) {
+      const int ring_threads = stage <= 5120 ? 32 : stage <= 14336 ? 64 : 128;
+      auto kernel = ring_threads == 32   ? rope_axes_bulk_kernel<T, 32>
+                    : ring_threads == 64 ? rope_axes_bulk_kernel<T, 64>
+                                         : rope_axes_bulk_kernel<T, 128>;
       static std::once_flag once;
       static cudaError_t attr = cudaSuccess;
       std::call_once(once, [] {
-        attr = cudaFuncSetAttribute(rope_axes_bulk_kernel<T>,
-                                    cudaFuncAttributeMaxDynamicSharedMemorySize, 112 * 1024);
+        for (auto f : {rope_axes_bulk_kernel<T, 32>, rope_axes_bulk_kernel<T, 64>,
+                       rope_axes_bulk_kernel<T, 128>})
+          if (attr == cudaSuccess)
+            attr = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, kBulkSmem);
       });
       if (attr != cudaSuccess) return cuda_fail(attr, "fe_rope_axes: shared memory attribute");
-      const int per_sm = std::max(1, 225 * 1024 / (smem + 1024));
-      FE_CUDA_TRY(launch_pdl(rope_axes_bulk_kernel<T>, dim3(std::min(a.rows, 148 * per_sm)),
-                             dim3(kBulkThreads), smem, stream, tq, tk, tv, to, tkc, tvc, a, map,
-                             stages));
+      const int per_sm = std::min(40, 225 * 1024 / (smem + 1024));
+      FE_CUDA_TRY(launch_pdl(kernel, dim3(std::min(a.rows, 148 * per_sm)),
+                             dim3(ring_threads), smem, stream, tq, tk, tv, to, tkc, tvc, a, map,
+                             kStages));
       return FE_OK;
     }
     const int gx = a.rows < 1024 ? passes : (passes + 1) / 2;
     // a row a block while there are few; then blocks that walk the rows, as many
     // as are resident
-    const int resident = 148 * std::max(1, 65536 / (80 * threads));  // by registers
+    const int resident = 148 * std::max(1, 65536 / (80 * vec_threads));  // by registers
     const int gy = a.rows < 1024 ? a.rows : std::min(a.rows, std::max(1, resident / gx));
-    FE_CUDA_TRY(launch_pdl(rope_axes_vec_kernel<T>, dim3(gx, gy), dim3(threads),
+    FE_CUDA_TRY(launch_pdl(rope_axes_vec_kernel<T>, dim3(gx, gy), dim3(vec_threads),
                            sizeof(float) * kRowBufs * a.rot, stream, tq, tk, tv, to, tkc, tvc, a,
                            map, units, hl));
     return FE_OK;

@@ -51,7 +51,9 @@ def same(got, want):
 CASES = [(1, 16, 8, 128, 128), (64, 32, 8, 128, 128), (37, 6, 3, 128, 64), (5, 40, 8, 128, 128),
          (3, 16, 2, 256, 256), (9, 5, 5, 256, 128), (130, 8, 1, 128, 128), (7, 3, 1, 44, 20),
          (6, 2, 2, 128, 0), (1500, 12, 4, 128, 128),
-         (2500, 12, 4, 128, 128), (4097, 0, 8, 128, 64), (4100, 20, 4, 256, 128), (4500, 32, 8, 128, 128)]
+         (2500, 12, 4, 128, 128), (4097, 0, 8, 128, 64), (4100, 20, 4, 256, 128),
+         (4500, 32, 8, 128, 128),
+         (4099, 4, 1, 128, 128), (4097, 64, 8, 128, 128)]
 
 
 @pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
