@@ -14,8 +14,6 @@
 // own, does their products and writes a partial record. Eight such warps, each a
 // CTA, fit an SM; a step's tiles are cut evenly across all of them, so that short
 // pieces run side by side and long streams keep 192 KiB an SM in flight.
-#include <mutex>
-
 #include "fe_attn_common.cuh"
 #include "fe_long_plan.h"
 
@@ -461,13 +459,8 @@ __global__ void __launch_bounds__(32)
 template <typename T>
 int launch_t(const CUtensorMap& kmap, const CUtensorMap& vmap, const void* args, int grid,
              bool beside, cudaStream_t stream) {
-  static std::once_flag once;
-  static cudaError_t attr_err = cudaSuccess;
-  std::call_once(once, [] {
-    attr_err = cudaFuncSetAttribute(paged_keys_kernel<T>,
-                                    cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
-  });
-  if (attr_err != cudaSuccess) return cuda_fail(attr_err, "paged_keys_kernel attribute");
+  static std::atomic<uint64_t> done{0};
+  FE_CUDA_TRY(allow_smem(paged_keys_kernel<T>, kSmem, done));
   FE_CUDA_TRY(launch_pdl(paged_keys_kernel<T>, dim3(grid), dim3(32), kSmem, stream, kmap, vmap,
                          *static_cast<const AttnArgs<T>*>(args), beside ? 1 : 0));
   return FE_OK;

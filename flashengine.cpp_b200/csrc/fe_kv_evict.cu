@@ -7,7 +7,6 @@
 // steps) and check what they read of it: a sequence or token that reaches past
 // its lists or the pool is skipped and flagged.
 #include <algorithm>
-#include <mutex>
 #include <string>
 
 #include "fe_common.cuh"
@@ -573,13 +572,8 @@ int fe_kv_select(const float* scores, const int32_t* kv, const int32_t* pages, i
     return fail(FE_ERR_INVALID_ARGUMENT, "fe_kv_select: scores must be 16-byte aligned");
   const SeqTable table{kv, pages, last, num_pages, page, cache_slots};
   auto s = static_cast<cudaStream_t>(stream);
-  static std::once_flag once;
-  static cudaError_t attr = cudaSuccess;
-  std::call_once(once, [] {
-    attr = cudaFuncSetAttribute(select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                kSelRoom / 4);
-  });
-  if (attr != cudaSuccess) return cuda_fail(attr, "fe_kv_select: shared memory attribute");
+  static std::atomic<uint64_t> done{0};
+  FE_CUDA_TRY(allow_smem(select_kernel, kSelRoom / 4, done));
   // more lists than SMs: the longest first, so that the last to end are short. Not
   // for large batches, where a CTA's look at all lengths costs more than it gives.
   const int lists = batch * hkv;

@@ -11,7 +11,6 @@
 // HBM-bound: 4 bytes of q and 8 of k and v per element (in and out) and one
 // cos / sin row a token.
 #include <algorithm>
-#include <mutex>
 #include <string>
 
 #include "fe_attn_common.cuh"
@@ -463,23 +462,15 @@ int launch_axes(void* q, const void* k, const void* v, void* k_out, void* kc, vo
     const int smem = static_cast<int>(kStages) * stage +
                      8 * (kStages + 1 + kMetaBufs * (kMaxAxes + 1)) + 4 * kRowBufs * a.rot;
     if (a.rows >= kBulkRows && smem <= kBulkSmem) {
-      const int ring_threads = stage <= 5120 ? 32 : stage <= 14336 ? 64 : 128;
-      auto kernel = ring_threads == 32   ? rope_axes_bulk_kernel<T, 32>
-                    : ring_threads == 64 ? rope_axes_bulk_kernel<T, 64>
-                                         : rope_axes_bulk_kernel<T, 128>;
-      static std::once_flag once;
-      static cudaError_t attr = cudaSuccess;
-      std::call_once(once, [] {
-        for (auto f : {rope_axes_bulk_kernel<T, 32>, rope_axes_bulk_kernel<T, 64>,
-                       rope_axes_bulk_kernel<T, 128>})
-          if (attr == cudaSuccess)
-            attr = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, kBulkSmem);
-      });
-      if (attr != cudaSuccess) return cuda_fail(attr, "fe_rope_axes: shared memory attribute");
+      static std::atomic<uint64_t> done[3];
+      const int i = stage <= 5120 ? 0 : stage <= 14336 ? 1 : 2;
+      auto kernel = i == 0   ? rope_axes_bulk_kernel<T, 32>
+                    : i == 1 ? rope_axes_bulk_kernel<T, 64>
+                             : rope_axes_bulk_kernel<T, 128>;
+      FE_CUDA_TRY(allow_smem(kernel, kBulkSmem, done[i]));
       const int per_sm = std::min(40, 225 * 1024 / (smem + 1024));
-      FE_CUDA_TRY(launch_pdl(kernel, dim3(std::min(a.rows, 148 * per_sm)),
-                             dim3(ring_threads), smem, stream, tq, tk, tv, to, tkc, tvc, a, map,
-                             kStages));
+      FE_CUDA_TRY(launch_pdl(kernel, dim3(std::min(a.rows, 148 * per_sm)), dim3(32 << i), smem,
+                             stream, tq, tk, tv, to, tkc, tvc, a, map, kStages));
       return FE_OK;
     }
     const int gx = a.rows < 1024 ? passes : (passes + 1) / 2;

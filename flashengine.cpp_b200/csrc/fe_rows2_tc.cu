@@ -34,8 +34,6 @@
 //  warps 9 / 10    issue of a stream's S and P V products (one elected thread
 //                  each); warp 9 owns the TMEM.
 // All hand-offs are mbarriers; every wait is bounded.
-#include <mutex>
-
 #include "fe_attn_common.cuh"
 #include "fe_tcgen05.cuh"
 
@@ -751,13 +749,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 template <typename T>
 int launch_t(const CUtensorMap& kmap, const CUtensorMap& vmap, const CUtensorMap& qmap,
              const void* args, int grid, cudaStream_t stream) {
-  static std::once_flag once;
-  static cudaError_t attr_err = cudaSuccess;
-  std::call_once(once, [] {
-    attr_err = cudaFuncSetAttribute(paged_rows2_kernel<T>,
-                                    cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
-  });
-  if (attr_err != cudaSuccess) return cuda_fail(attr_err, "paged_rows2_kernel attribute");
+  static std::atomic<uint64_t> done{0};
+  FE_CUDA_TRY(allow_smem(paged_rows2_kernel<T>, kSmem, done));
   FE_CUDA_TRY(launch_pdl(paged_rows2_kernel<T>, dim3(grid), dim3(kThreads), kSmem, stream, kmap,
                          vmap, qmap, *static_cast<const AttnArgs<T>*>(args)));
   return FE_OK;
