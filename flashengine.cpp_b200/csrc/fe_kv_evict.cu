@@ -18,6 +18,7 @@ constexpr int kSelThreads = 512;
 constexpr int kSelList = 2048;
 constexpr int kSelWarps = kSelThreads / 32;
 constexpr int kBins = 2048;
+// most CTAs a list, most CTAs for which lists are divided, fewest tokens a CTA
 constexpr int kSelCluster = 8, kSelCtas = 296, kSelPart = 4096;
 constexpr int kRankBatch = 128;  // sequences that are taken longest first
 constexpr int kSelRoom = 128 << 10;  // tokens whose classes fit in shared memory
@@ -143,8 +144,8 @@ __device__ __forceinline__ int2 find_bin(const Cluster& cl, const int* hist, int
   return r;
 }
 
-// One CTA, or a cluster of them, per (sequence, KV head). The `want` best of the tokens between sink
-// and the recent ones are found by a radix select over their ordered scores:
+// One CTA, or a cluster of them, per (sequence, KV head). The `want` best of the
+// tokens between sink and the recent ones are found by a radix select over their ordered scores:
 // a histogram of the first 11 bits gives the bin in which the want-th key lies;
 // a second sweep over the scores notes for every token whether it is above that
 // bin and lists the keys within; two more histograms (11 and 10 bits) over the

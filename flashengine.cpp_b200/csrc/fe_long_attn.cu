@@ -416,7 +416,9 @@ int create_long(const char* what, int hq, int hkv, int dim, int page, int max_ba
   // lists (cta offsets, items, groups) three times, units twice, row blocks and
   // their tables, query rows, chunks, pages
   const size_t n = c.max_items;
-  p->meta_cap = n * sizeof(KeyItem) + 3 * (n * (sizeof(WorkItem) + sizeof(SplitGroup)) + 4 * size_t(c.dec_grid_cap + 1) + 64) +
+  p->meta_cap = n * sizeof(KeyItem) +
+                3 * (n * (sizeof(WorkItem) + sizeof(SplitGroup)) +
+                     4 * size_t(c.dec_grid_cap + 1) + 64) +
                 2 * sizeof(UnitRec) * n + n * (sizeof(SeqInfo) + 8) + sizeof(RowInfo) * 16 * n +
                 2 * size_t(max_batch) * sizeof(SeqInfo) +
                 sizeof(ScoreChunk) * size_t(max_batch) *
@@ -654,8 +656,8 @@ int fe_shared_plan_prepare(fe_long_plan* p, const int32_t* qo, const int32_t* kv
   LongResult res;
   std::string err;
   try {
-    rc = build_shared_plan(p->cfg, p->keys, qo, kv, pages, last, group_off, shared, groups, batch, rows,
-                           graph != 0, res, err);
+    rc = build_shared_plan(p->cfg, p->keys, qo, kv, pages, last, group_off, shared, groups, batch,
+                           rows, graph != 0, res, err);
   } catch (const std::bad_alloc&) {
     return fail(FE_ERR_CAPACITY, name + ": out of host memory");
   }

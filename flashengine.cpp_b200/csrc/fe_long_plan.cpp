@@ -153,7 +153,8 @@ struct Group {
 };
 
 // One layout of the step; `share` off leaves every sequence whole.
-int layout(const PlanConfig& cfg, bool keys, const std::vector<SeqInfo>& step, const std::vector<Group>& gs,
+int layout(const PlanConfig& cfg, bool keys, const std::vector<SeqInfo>& step,
+           const std::vector<Group>& gs,
            const int32_t* pages, int total_pages, int rows, bool share, bool fixed_grid,
            LongResult& out, std::string& err) {
   out = LongResult{};

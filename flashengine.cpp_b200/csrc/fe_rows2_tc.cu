@@ -29,8 +29,9 @@
 // One persistent CTA per SM, three warpgroups:
 //  warps 0-3, 4-7  softmax of stream 0 and 1;
 //  warps 8 / 11    producers of K (and Q) / of V: eight 16-token page pieces a
-//                  tile, one TMA box each, into 2 K and 2 V stages of 32 KiB (S runs two steps
-//                  ahead, so that a K stage is refilled two before it is read);
+//                  tile, one TMA box each, into 2 K and 2 V stages of 32 KiB
+//                  (S runs two steps ahead, so that a K stage is refilled two
+//                  before it is read);
 //  warps 9 / 10    issue of a stream's S and P V products (one elected thread
 //                  each); warp 9 owns the TMEM.
 // All hand-offs are mbarriers; every wait is bounded.
@@ -63,7 +64,7 @@ constexpr int kOffV = kOffK + kKStages * kTile;
 constexpr int kOffOut = kOffV + kVStages * kTile;  // [softmax warp][32 rows][128 B]
 constexpr int kOffX = kOffOut + 8 * 4096;         // [stream][m, l][row]
 constexpr int kOffBar = kOffX + 2 * 2 * kM * 4;
-// q_full[2], q_empty[2], k_full[3], k_empty[3], v_full[2], v_empty[2],
+// q_full[2], q_empty[2], k_full[2], k_empty[2], v_full[2], v_empty[2],
 // s_full[2][2], pv_done[2][2], p_full[2][2], o_full[2], o_free[2], x_full, drain
 constexpr int kBars = 4 + 2 * kKStages + 2 * kVStages + 16 + 2;
 constexpr int kSmem = kOffBar + kBars * 8 + 32;

@@ -164,33 +164,39 @@ def compact(**kw):
 
 
 PYTHON = [
-    (rope, dict(), None), (rope, dict(q=None), None),
-    (rope, dict(q=t(5, 4, 64)), "q"), (rope, dict(q=t(4, 4, 128)), "q"),
-    (rope, dict(q=t(5, 4, 128, dtype=torch.float16)), "q"), (rope, dict(q=t(5, 512)), "q"),
-    (rope, dict(q=t(5, 4, 128, where=1)), "q"), (rope, dict(k=t(5, 2, 128, where=1)), "k"),
+    (rope, dict(), None), (rope, dict(q=None), None), (rope, dict(q=t(5, 4, 64)), "q"),
+    (rope, dict(q=t(4, 4, 128)), "q"), (rope, dict(q=t(5, 4, 128, dtype=torch.float16)), "q"),
+    (rope, dict(q=t(5, 512)), "q"), (rope, dict(q=t(5, 4, 128, where=1)), "q"),
+    (rope, dict(k=t(5, 2, 128, where=1)), "k"),
     (rope, dict(k=t(5, 2, 128, dtype=torch.float32), q=None), "float16 or bfloat16"),
     (rope, dict(k=strided(t(5, 2, 128))), "k"), (rope, dict(q=strided(t(5, 4, 128))), "q"),
-    (rope, dict(pos=t(5, dtype=torch.int64)), "pos"), (rope, dict(pos=t(3, 4, dtype=torch.int64)), "pos"),
+    (rope, dict(pos=t(5, dtype=torch.int64)), "pos"),
+    (rope, dict(pos=t(3, 4, dtype=torch.int64)), "pos"),
     (rope, dict(pos=t(3, 5, dtype=torch.int32)), "pos"), (rope, dict(pairs=bytes(31)), "pair_axis"),
     (rope, dict(pairs=[0] * 32), "pair_axis"),
-    (rope, dict(cache=t(9, 64, dtype=torch.bfloat16)), "cache"),
-    (append, dict(), None), (append, dict(k_out=None, q=None), None),
-    (append, dict(v=t(5, 2, 64)), "v"), (append, dict(v=t(5, 2, 128, where=1)), "v"),
-    (append, dict(k_out=t(4, 2, 128)), "k_out"), (append, dict(slots=t(4, dtype=torch.int64)), "slots"),
+    (rope, dict(cache=t(9, 64, dtype=torch.bfloat16)), "cache"), (append, dict(), None),
+    (append, dict(k_out=None, q=None), None), (append, dict(v=t(5, 2, 64)), "v"),
+    (append, dict(v=t(5, 2, 128, where=1)), "v"), (append, dict(k_out=t(4, 2, 128)), "k_out"),
+    (append, dict(slots=t(4, dtype=torch.int64)), "slots"),
     (append, dict(slots=t(5, dtype=torch.int32)), "slots"), (append, dict(kc=t(31, 2, 128)), "kc"),
-    (append, dict(vc=t(32, 2, 128, where=1)), "vc"), (append, dict(kc=strided(t(32, 2, 128))), "kc"),
-    (append, dict(kc=t(32, 2, 128, dtype=torch.float16)), "kc"),
-    (select, dict(), None), (select, dict(scores=t(64, dtype=torch.float32)), "scores"),
-    (select, dict(scores=t(2, 64)), "scores"), (select, dict(scores=t(2, 64, dtype=torch.float32, where=1)), "scores"),
-    (select, dict(kept=t(1, 2, 8, dtype=torch.int64)), "kept"), (select, dict(kept=t(1, 3, 8, dtype=torch.int32)), "kept"),
+    (append, dict(vc=t(32, 2, 128, where=1)), "vc"),
+    (append, dict(kc=strided(t(32, 2, 128))), "kc"),
+    (append, dict(kc=t(32, 2, 128, dtype=torch.float16)), "kc"), (select, dict(), None),
+    (select, dict(scores=t(64, dtype=torch.float32)), "scores"),
+    (select, dict(scores=t(2, 64)), "scores"),
+    (select, dict(scores=t(2, 64, dtype=torch.float32, where=1)), "scores"),
+    (select, dict(kept=t(1, 2, 8, dtype=torch.int64)), "kept"),
+    (select, dict(kept=t(1, 3, 8, dtype=torch.int32)), "kept"),
     (select, dict(kept=t(2, 8, dtype=torch.int32)), "kept"), (select, dict(kv=i32(0, 1, 2)), "kv"),
-    (select, dict(last=i32(5, where=1)), ""), (select, dict(pages=t(2, dtype=torch.int64)), ""),
+    (select, dict(last=i32(5, where=1)), "."), (select, dict(pages=t(2, dtype=torch.int64)), "."),
     (compact, dict(), None), (compact, dict(scores=None, dst_kv=None, dst_pages=None), None),
-    (compact, dict(v=t(64, 2, 64)), "pools"), (compact, dict(v=t(64, 2, 128, dtype=torch.float16)), "v_pool"),
-    (compact, dict(k=t(64, 2, 128, where=1)), "k_pool"), (compact, dict(scores=t(2, 48, dtype=torch.float32)), "scores"),
+    (compact, dict(v=t(64, 2, 64)), "pools"),
+    (compact, dict(v=t(64, 2, 128, dtype=torch.float16)), "v_pool"),
+    (compact, dict(k=t(64, 2, 128, where=1)), "k_pool"),
+    (compact, dict(scores=t(2, 48, dtype=torch.float32)), "scores"),
     (compact, dict(kept=t(1, 2, 8)), "kept"), (compact, dict(dst_kv=i32(0, 1, 1)), "dst_kv"),
-    (compact, dict(dst_pages=None), ""), (compact, dict(dst_kv=None), ""),
-    (compact, dict(dst_pages=i32(2, where=1)), "")]
+    (compact, dict(dst_pages=None), "."), (compact, dict(dst_kv=None), "."),
+    (compact, dict(dst_pages=i32(2, where=1)), "."),]
 
 
 @pytest.mark.parametrize("n", range(len(PYTHON)))
