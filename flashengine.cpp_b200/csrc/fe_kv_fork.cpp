@@ -1,5 +1,6 @@
 // Copy lists for forked sequences and the prefixes that sequences share
-// (fe_kv_fork_copies, fe_kv_shared_prefixes, fe_kv.h). Host code only: no device memory is touched, so it runs on a host without a GPU.
+// (fe_kv_fork_copies, fe_kv_shared_prefixes, fe_kv.h). Host code only: no device
+// memory is touched, so it runs on a host without a GPU.
 //
 // The reference's BlockManager shares only whole published pages between
 // sequences and never writes a published page (src/scheduler.cpp:6-29, the
@@ -91,14 +92,18 @@ extern "C" int fe_kv_shared_prefixes(const int32_t* kv, const int32_t* pages, in
     return fail(FE_ERR_INVALID_ARGUMENT, "fe_kv_shared_prefixes: bad sizes");
   if (!group_off || (batch > 0 && (!kv || !pages || !shared)))
     return fail(FE_ERR_INVALID_ARGUMENT, "fe_kv_shared_prefixes: null pointer");
+  // before any page is read: every list lies within the first kv[batch] pages
+  if (batch > 0 && kv[0] != 0)
+    return fail(FE_ERR_INVALID_ARGUMENT, "fe_kv_shared_prefixes: kv[0] must be 0");
+  for (int b = 0; b < batch; ++b)
+    if (kv[b + 1] < kv[b])
+      return fail(FE_ERR_INVALID_ARGUMENT, "fe_kv_shared_prefixes: kv decreases (b=" +
+                                               std::to_string(b) + ")");
   group_off[0] = 0;
   int n = 0;
   for (int b = 0; b < batch;) {
     const int32_t* head = pages + kv[b];
     int64_t common = int64_t(kv[b + 1]) - kv[b];
-    if (common < 0)
-      return fail(FE_ERR_INVALID_ARGUMENT, "fe_kv_shared_prefixes: kv decreases (b=" +
-                                               std::to_string(b) + ")");
     int end = b + 1;
     for (; end < batch; ++end) {
       const int64_t len = int64_t(kv[end + 1]) - kv[end];
