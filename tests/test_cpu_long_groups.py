@@ -47,7 +47,7 @@ def test_offsets_are_refused_by_prepare(lib, kv, monkeypatch):  # noqa: F811
     real = fekv.load()
     plan = fekv.SharedPlan(8, 2, 128, 16, 4, 4, True, 3)
     before = lib.count
-    for name in ("fe_kv_shared_prefixes", "fe_last_error"):
+    for name in ("fe_kv_shared_prefixes", "fe_last_error", "fe_status_string"):
         monkeypatch.setattr(lib, name, getattr(real, name), raising=False)
     with pytest.raises((FeError, ValueError)):
         plan.prepare(np.array([0, 1, 2, 3]), np.array(kv), np.array([1, 2, 3]),
