@@ -475,13 +475,8 @@ template <typename T, int H, int D = kHeadDim, bool kExt = false>
 int launch_t(const CUtensorMap& kmap, const CUtensorMap& vmap, bool per_head_tma,
              const AttnArgs<T>& args, int grid, cudaStream_t stream) {
   using C = DecCfg<H, D>;
-  static std::once_flag once;
-  static cudaError_t attr_err = cudaSuccess;
-  std::call_once(once, [] {
-    attr_err = cudaFuncSetAttribute(paged_decode_kernel<T, H, D, kExt>,
-                                    cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
-  });
-  if (attr_err != cudaSuccess) return cuda_fail(attr_err, "paged_decode_kernel attribute");
+  static std::atomic<uint64_t> done{0};
+  FE_CUDA_TRY(allow_smem(paged_decode_kernel<T, H, D, kExt>, C::kSmem, done));
   FE_CUDA_TRY(launch_pdl(paged_decode_kernel<T, H, D, kExt>, dim3(grid), dim3(kDecThreads),
                          C::kSmem, stream, kmap, vmap, args, per_head_tma ? 1 : 0));
   return FE_OK;

@@ -44,7 +44,6 @@
 // Nine warps leave 168 registers a thread, of which ptxas spills 96 to 112
 // bytes at 128 dims, 72 at 256.
 #include <algorithm>
-#include <mutex>
 #include <type_traits>
 
 #include "fe_attn_common.cuh"
@@ -655,13 +654,8 @@ template <typename T, int H, int D>
 int launch(const CUtensorMap& kmap, const CUtensorMap& vmap, const Kv8Args<T>& args, int grid,
            cudaStream_t stream) {
   using C = Cfg<H, D>;
-  static std::once_flag once;
-  static cudaError_t attr_err = cudaSuccess;
-  std::call_once(once, [] {
-    attr_err = cudaFuncSetAttribute(kv8_decode_kernel<T, H, D>,
-                                    cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
-  });
-  if (attr_err != cudaSuccess) return cuda_fail(attr_err, "kv8_decode_kernel attribute");
+  static std::atomic<uint64_t> done{0};
+  FE_CUDA_TRY(allow_smem(kv8_decode_kernel<T, H, D>, C::kSmem, done));
   FE_CUDA_TRY(launch_pdl(kv8_decode_kernel<T, H, D>, dim3(grid), dim3(kThreads), C::kSmem, stream,
                          kmap, vmap, args));
   return FE_OK;

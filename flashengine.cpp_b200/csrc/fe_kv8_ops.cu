@@ -4,7 +4,6 @@
 // reference, whose pools are 16-bit (src/cuda_model.cpp:60); slot semantics,
 // rotation and roundings follow fe_kv_append / fe_rope.
 #include <cstring>
-#include <mutex>
 #include <string>
 
 #include "fe_kv8_common.cuh"
@@ -622,19 +621,11 @@ int launch_append(AppendArgs& a, cudaStream_t stream) {
   a.kv_blocks = static_cast<int>(kvb);
   const dim3 grid(static_cast<unsigned>(kvb + qb));
   constexpr int kSmem = kWarps * 2 * Stage<D>::kBytes;
-  static std::once_flag once;
-  static cudaError_t attr_err = cudaSuccess;
-  std::call_once(once, [] {
-    for (auto kernel : {kv8_append_kernel<T, D, 16>, kv8_append_kernel<T, D, 4>,
-                        kv8_append_kernel<T, D, 1>})
-      if (attr_err == cudaSuccess)
-        attr_err =
-            cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
-  });
-  if (attr_err != cudaSuccess) return cuda_fail(attr_err, "kv8_append_kernel attribute");
+  static std::atomic<uint64_t> done[3];
   auto kernel = w == 16  ? kv8_append_kernel<T, D, 16>
                 : w == 4 ? kv8_append_kernel<T, D, 4>
                          : kv8_append_kernel<T, D, 1>;
+  FE_CUDA_TRY(allow_smem(kernel, kSmem, done[w == 16 ? 0 : w == 4 ? 1 : 2]));
   FE_CUDA_TRY(launch_pdl(kernel, grid, dim3(kThreads), a.apart ? kSmem / 2 : kSmem, stream, a));
   return FE_OK;
 }

@@ -64,7 +64,6 @@
 // or both, 2 to 5 % slower; one pass over the scores with the maximum of the
 // group's tile before (and corrections where it is exceeded), three softmax
 // groups, items' descriptions in shared memory: no change.
-#include <mutex>
 #include <type_traits>
 
 #include "fe_attn_common.cuh"
@@ -807,14 +806,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 template <typename T, int D>
 int launch(const CUtensorMap& kmap, const CUtensorMap& vmap, const Kv8Args<T>& args, int grid,
            cudaStream_t stream) {
-  static std::once_flag once;
-  static cudaError_t attr_err = cudaSuccess;
-  std::call_once(once, [] {
-    attr_err = cudaFuncSetAttribute(kv8_rows_kernel<T, D>,
-                                    cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<T, D>::kSmem);
-  });
-  if (attr_err != cudaSuccess) return cuda_fail(attr_err, "kv8_rows_kernel attribute");
+  static std::atomic<uint64_t> done{0};
   constexpr int kSmem = Cfg<T, D>::kSmem;
+  FE_CUDA_TRY(allow_smem(kv8_rows_kernel<T, D>, kSmem, done));
   FE_CUDA_TRY(launch_pdl(kv8_rows_kernel<T, D>, dim3(grid), dim3(kThreads), kSmem, stream, kmap,
                          vmap, args));
   return FE_OK;

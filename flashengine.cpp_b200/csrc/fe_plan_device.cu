@@ -515,10 +515,8 @@ int plan_device_launch(const DevPlanArgs& a, cudaStream_t stream) {
   // A plain launch (no programmatic serialization): the planner starts only
   // after every earlier kernel of the stream has completed, since the
   // previous step's attention still reads the lists it rewrites.
-  static const cudaError_t attr = cudaFuncSetAttribute(
-      plan_device_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-      int(sizeof(uint64_t) * kMaxRowUnits));
-  FE_CUDA_TRY(attr);
+  static std::atomic<uint64_t> done{0};
+  FE_CUDA_TRY(allow_smem(plan_device_kernel, int(sizeof(uint64_t) * kMaxRowUnits), done));
   plan_device_kernel<<<1, kPlanThreads, sizeof(uint64_t) * kMaxRowUnits, stream>>>(a);
   FE_CUDA_TRY(cudaGetLastError());
   return FE_OK;

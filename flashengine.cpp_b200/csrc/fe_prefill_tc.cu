@@ -49,7 +49,6 @@
 // (few 128-row items, as DFlash draft blocks give): a piece stores its
 // unnormalised O with the row's (m, l) into a partial record, and
 // decode_merge_kernel combines them.
-#include <mutex>
 
 #include "fe_attn_common.cuh"
 #include "fe_tcgen05.cuh"
@@ -713,13 +712,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 template <typename T, int D, bool kExt>
 int launch_t(const CUtensorMap& kmap, const CUtensorMap& vmap, const CUtensorMap& qmap,
              const AttnArgs<T>& args, int grid, cudaStream_t stream) {
-  static std::once_flag once;
-  static cudaError_t attr_err = cudaSuccess;
-  std::call_once(once, [] {
-    attr_err = cudaFuncSetAttribute(paged_prefill_tc_kernel<T, D, kExt>,
-                                    cudaFuncAttributeMaxDynamicSharedMemorySize, TcCfg<D>::kSmem);
-  });
-  if (attr_err != cudaSuccess) return cuda_fail(attr_err, "paged_prefill_tc_kernel attribute");
+  static std::atomic<uint64_t> done{0};
+  FE_CUDA_TRY(allow_smem(paged_prefill_tc_kernel<T, D, kExt>, TcCfg<D>::kSmem, done));
   FE_CUDA_TRY(launch_pdl(paged_prefill_tc_kernel<T, D, kExt>, dim3(grid), dim3(kTcThreads),
                          TcCfg<D>::kSmem, stream, kmap, vmap, qmap, args));
   return FE_OK;
