@@ -153,7 +153,9 @@ struct KeyState {
 
   // One 16-token tile starting at token `tbase` of a sequence of `length` keys.
   // kSink: the scaled scores (base 2, -inf where masked) are also stored to
-  // sink[key * stride + column], for this state's columns below `cols`.
+  // sink[key * stride + column], for this state's columns below `cols`; they are
+  // rounded before the difference from the maximum, so that l is the sum of the
+  // weights that the stored scores give.
   template <bool kSink = false>
   __device__ __forceinline__ void tile(const TileAddr& t, int tbase, int length, float scale_log2,
                                        int lane, float* sink = nullptr, int stride = 0,
@@ -188,14 +190,16 @@ struct KeyState {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         const int col = nt * 8 + 2 * cq;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sc[nt][e] = __fmul_rn(sc[nt][e], scale_log2);
         if (col < cols) {
-          *reinterpret_cast<float2*>(sink + r8 * stride + col) =
-              make_float2(sc[nt][0] * scale_log2, sc[nt][1] * scale_log2);
+          *reinterpret_cast<float2*>(sink + r8 * stride + col) = make_float2(sc[nt][0], sc[nt][1]);
           *reinterpret_cast<float2*>(sink + (r8 + 8) * stride + col) =
-              make_float2(sc[nt][2] * scale_log2, sc[nt][3] * scale_log2);
+              make_float2(sc[nt][2], sc[nt][3]);
         }
       }
     }
+    const float scale = kSink ? 1.f : scale_log2;
     // ---- online softmax per column; the 8 lanes sharing lane%4 hold a column
     float al[NT][2];
 #pragma unroll
@@ -206,12 +210,12 @@ struct KeyState {
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-        const float mn = fmaxf(m[nt][e], mx * scale_log2);
+        const float mn = fmaxf(m[nt][e], mx * scale);
         const float base = mn == -INFINITY ? 0.f : mn;
         al[nt][e] = fast_exp2(m[nt][e] - base);
         m[nt][e] = mn;
-        const float p0 = fast_exp2(fmaf(sc[nt][e], scale_log2, -base));
-        const float p1 = fast_exp2(fmaf(sc[nt][2 + e], scale_log2, -base));
+        const float p0 = fast_exp2(fmaf(sc[nt][e], scale, -base));
+        const float p1 = fast_exp2(fmaf(sc[nt][2 + e], scale, -base));
         sc[nt][e] = p0;
         sc[nt][2 + e] = p1;
         l[nt][e] = fmaf(l[nt][e], al[nt][e], p0 + p1);

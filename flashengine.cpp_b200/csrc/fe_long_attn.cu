@@ -10,7 +10,9 @@
 // of its rows, m = the largest base-2 score of its keys, l = sum 2^(s - m) and
 // O = sum 2^(s - m) v; records of disjoint keys join as
 //   m = max m_i, l = sum l_i 2^(m_i - m), out = sum O_i 2^(m_i - m) / l.
-// The weight of a key with score s is then 2^(s - m - log2 l).
+// The weight of a key with score s is then 2^(s - m) / l. (2^(s - (m + log2 l)) loses
+// log2 l to the rounding of m + log2 l where scores are large: with |m| = 2^23 the
+// weights of equal keys are up to 4 % off, with 2^28 each of 700 weighs 1.)
 #include <algorithm>
 #include <cstring>
 #include <new>
@@ -75,7 +77,7 @@ __device__ __forceinline__ const float* record(const Records& a, const Records& 
 // (m, l) among them, go out together.
 template <typename T, int D, int kStep>
 __device__ __forceinline__ void join_row(const Records& a, const Records& b, int lane, T* out,
-                                         float* lse) {
+                                         float2* norm) {
   constexpr int kV = D / 128;  // float4 vectors per lane
   const int n = a.n + b.n;
   float4 acc[kV];
@@ -134,7 +136,7 @@ __device__ __forceinline__ void join_row(const Records& a, const Records& b, int
   for (int v = 0; v < kV; ++v)
     store4<T>(out + v * 128 + lane * 4, acc[v].x * inv, acc[v].y * inv, acc[v].z * inv,
               acc[v].w * inv);
-  if (lse && lane == 0) *lse = M + log2f(L);
+  if (norm && lane == 0) *norm = make_float2(M, inv);
 }
 
 // The records of query row w / hq, head w % hq: the plan's metadata alone, complete
@@ -162,8 +164,8 @@ __device__ __forceinline__ void find_records(const AttnArgs<T>& a, int64_t w, Re
   }
 }
 
-// One warp per query row and head; lse (scored plans): where m + log2 l of each
-// goes, fp32 [rows, hq]. Few pairs: four records of one in flight (eight: 2 us more
+// One warp per query row and head; norms (scored plans): where (m, 1 / l) of each
+// goes, [rows, hq]. Few pairs: four records of one in flight (eight: 2 us more
 // for 64 rows of 64 heads, whose warps are then not all resident). Many: what counts
 // are loads in flight an SM, so two records a warp and more warps (2048 rows of
 // 32 heads, 60 % with two records: 7 us less; 64 rows of 64 heads 2 us more).
@@ -171,7 +173,7 @@ constexpr int kManyPairs = 148 * 48;
 
 template <typename T, int D, int kStep>
 __global__ void __launch_bounds__(kJoinThreads, kStep == 2 && D == kHeadDim ? 5 : 4)
-    join_kernel(const AttnArgs<T> a, float* lse) {
+    join_kernel(const AttnArgs<T> a, float2* norms) {
   pdl_trigger();
   const int lane = threadIdx.x & 31;
   const int64_t w = static_cast<int64_t>(blockIdx.x) * kJoinWarps + (threadIdx.x >> 5);
@@ -179,30 +181,30 @@ __global__ void __launch_bounds__(kJoinThreads, kStep == 2 && D == kHeadDim ? 5 
   find_records<T, D>(a, w, own, pre);
   pdl_wait();
   if (own.n > 0)  // else written by its unit
-    join_row<T, D, kStep>(own, pre, lane, a.out + w * D, lse ? lse + w : nullptr);
+    join_row<T, D, kStep>(own, pre, lane, a.out + w * D, norms ? norms + w : nullptr);
 }
 
 template <typename T, int D>
-int launch_join(const AttnArgs<T>& a, int rows, float* lse, cudaStream_t s) {
+int launch_join(const AttnArgs<T>& a, int rows, float2* norms, cudaStream_t s) {
   const int64_t pairs = int64_t(rows) * a.hq;
   const int grid = static_cast<int>((pairs + kJoinWarps - 1) / kJoinWarps);
   auto kernel = pairs > kManyPairs ? join_kernel<T, D, 2> : join_kernel<T, D, 4 * kHeadDim / D>;
-  FE_CUDA_TRY(launch_pdl(kernel, dim3(grid), dim3(kJoinThreads), 0, s, a, lse));
+  FE_CUDA_TRY(launch_pdl(kernel, dim3(grid), dim3(kJoinThreads), 0, s, a, norms));
   return FE_OK;
 }
 
 template <typename T>
-int launch_join(const AttnArgs<T>& a, int dim, int rows, float* lse, cudaStream_t s) {
-  return dim == kWideHeadDim ? launch_join<T, kWideHeadDim>(a, rows, lse, s)
-                             : launch_join<T, kHeadDim>(a, rows, lse, s);
+int launch_join(const AttnArgs<T>& a, int dim, int rows, float2* norms, cudaStream_t s) {
+  return dim == kWideHeadDim ? launch_join<T, kWideHeadDim>(a, rows, norms, s)
+                             : launch_join<T, kHeadDim>(a, rows, norms, s);
 }
 
 // Scored plans, behind the join: the weights of kScoreChunk keys of one KV head
-// at a time, 2^(raw score - lse) summed over the packed rows in order, go to the
+// at a time, 2^(raw score - m) / l summed over the packed rows in order, go to the
 // keys' scores. Grid: chunks x KV heads.
 __global__ void __launch_bounds__(kScoreThreads, 8)
     score_kernel(const uint8_t* __restrict__ meta, const float* __restrict__ raw_scores,
-                 const float* __restrict__ lse, float* __restrict__ scores, int hq, int hkv,
+                 const float2* __restrict__ norms, float* __restrict__ scores, int hq, int hkv,
                  int page, int64_t cache_slots) {
   constexpr int kPer = kScoreChunk / kScoreThreads;  // keys a thread
   pdl_trigger();
@@ -242,12 +244,12 @@ __global__ void __launch_bounds__(kScoreThreads, 8)
         const int P = si.qrows * G, cols = (P + 1) & ~1;
         const int tiles = (si.length + kTileTokens - 1) / kTileTokens;
         const float* raw = raw_scores + raw0 + static_cast<int64_t>(h) * tiles * kTileTokens * cols;
-        const float* row = lse + static_cast<int64_t>(si.q_row0) * hq + h * G;
+        const float2* row = norms + static_cast<int64_t>(si.q_row0) * hq + h * G;
         const float* at_key = raw + static_cast<int64_t>(c.t0 + threadIdx.x) * cols;
         const int stride = kScoreThreads * cols;
         int g = 0;  // packed row p is head g of the query row that `row` points at
         for (int p = 0; p < P; p += 4, at_key += 4) {  // four rows' scores of a key at once
-          float l[4];
+          float2 c4[4];  // (m, 1 / l) of the four rows
           float2 s0[kPer], s1[kPer];
 #pragma unroll
           for (int i = 0; i < kPer; ++i) {
@@ -260,7 +262,7 @@ __global__ void __launch_bounds__(kScoreThreads, 8)
           }
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            l[r] = p + r < P ? __ldcg(row + g) : INFINITY;
+            c4[r] = p + r < P ? __ldcg(row + g) : make_float2(INFINITY, 0.f);
             if (++g == G) {
               g = 0;
               row += hq;
@@ -268,10 +270,10 @@ __global__ void __launch_bounds__(kScoreThreads, 8)
           }
 #pragma unroll
           for (int i = 0; i < kPer; ++i) {
-            w[i] += fast_exp2(s0[i].x - l[0]);
-            if (p + 1 < P) w[i] += fast_exp2(s0[i].y - l[1]);
-            if (p + 2 < P) w[i] += fast_exp2(s1[i].x - l[2]);
-            if (p + 3 < P) w[i] += fast_exp2(s1[i].y - l[3]);
+            w[i] = fmaf(fast_exp2(s0[i].x - c4[0].x), c4[0].y, w[i]);
+            if (p + 1 < P) w[i] = fmaf(fast_exp2(s0[i].y - c4[1].x), c4[1].y, w[i]);
+            if (p + 2 < P) w[i] = fmaf(fast_exp2(s1[i].x - c4[2].x), c4[2].y, w[i]);
+            if (p + 3 < P) w[i] = fmaf(fast_exp2(s1[i].y - c4[3].x), c4[3].y, w[i]);
           }
         }
       }
@@ -301,7 +303,7 @@ struct fe_long_plan {
   size_t meta_cap = 0;
   float* d_partials = nullptr;
   float* d_sink = nullptr;
-  float* d_lse = nullptr;  // scored plans: m + log2 l of each query row and head
+  float2* d_norms = nullptr;  // scored plans: (m, 1 / l) of each query row and head
   int64_t max_rows = 0;
   int64_t sink_floats = 0;
   // pinned staging, double-buffered
@@ -338,7 +340,7 @@ void destroy_long(fe_long_plan* p) {
     if (p->d_meta) cudaFree(p->d_meta);
     if (p->d_partials) cudaFree(p->d_partials);
     if (p->d_sink) cudaFree(p->d_sink);
-    if (p->d_lse) cudaFree(p->d_lse);
+    if (p->d_norms) cudaFree(p->d_norms);
   }
   delete p;
 }
@@ -435,7 +437,7 @@ int create_long(const char* what, int hq, int hkv, int dim, int page, int max_ba
   // keys (each row sees one block of 16 at least)
   p->max_rows = scored ? max_keys / kTileTokens : 0;
   if (e == cudaSuccess && p->max_rows > 0)
-    e = cudaMalloc(&p->d_lse, sizeof(float) * p->max_rows * hq);
+    e = cudaMalloc(&p->d_norms, sizeof(float2) * p->max_rows * hq);
   for (int i = 0; i < 2 && e == cudaSuccess; ++i) {
     p->h_cap[i] = std::min<size_t>(p->meta_cap, size_t(256) << 10);  // grows with the steps
     e = cudaMallocHost(&p->h_meta[i], p->h_cap[i]);
@@ -604,7 +606,7 @@ int run_scored(fe_long_plan* p, const void* q, float* scores, void* out, cudaStr
   const AttnArgs<T> a = long_args<T>(p, q, out, 1, 0);
   int rc = launch_decode(p, &a, grid_dec, false, s);
   if (rc != FE_OK) return rc;
-  rc = launch_join<T>(a, c.dim, p->last.rows, p->d_lse, s);
+  rc = launch_join<T>(a, c.dim, p->last.rows, p->d_norms, s);
   if (rc != FE_OK) return rc;
   // a graph's launch has to do for later steps of more keys: the CTAs stride
   const int most = std::max(1, 16 * c.grid_cap / c.hkv);
@@ -612,7 +614,7 @@ int run_scored(fe_long_plan* p, const void* q, float* scores, void* out, cudaStr
   FE_CUDA_TRY(launch_pdl(score_kernel, grid, dim3(kScoreThreads), 0, s,
                          static_cast<const uint8_t*>(p->d_meta),
                          static_cast<const float*>(p->d_sink),
-                         static_cast<const float*>(p->d_lse), scores, c.hq, c.hkv, c.page,
+                         static_cast<const float2*>(p->d_norms), scores, c.hq, c.hkv, c.page,
                          int64_t(c.num_blocks + 1) * c.page));
   return FE_OK;
 }
