@@ -14,9 +14,11 @@
 // log2 l to the rounding of m + log2 l where scores are large: with |m| = 2^23 the
 // weights of equal keys are up to 4 % off, with 2^28 each of 700 weighs 1.)
 #include <algorithm>
+#include <cmath>
 #include <cstring>
 #include <new>
 #include <string>
+#include <vector>
 
 #include "fe_attn_common.cuh"
 #include "fe_long_plan.h"
@@ -302,6 +304,8 @@ struct fe_long_plan {
   uint8_t* d_meta = nullptr;
   size_t meta_cap = 0;
   float* d_partials = nullptr;
+  int64_t partial_floats = 0;
+  std::vector<float*> outgrown;  // earlier, smaller d_partials: a captured run may hold them
   float* d_sink = nullptr;
   float2* d_norms = nullptr;  // scored plans: (m, 1 / l) of each query row and head
   int64_t max_rows = 0;
@@ -339,6 +343,7 @@ void destroy_long(fe_long_plan* p) {
     }
     if (p->d_meta) cudaFree(p->d_meta);
     if (p->d_partials) cudaFree(p->d_partials);
+    for (float* x : p->outgrown) cudaFree(x);
     if (p->d_sink) cudaFree(p->d_sink);
     if (p->d_norms) cudaFree(p->d_norms);
   }
@@ -410,32 +415,50 @@ int create_long(const char* what, int hq, int hkv, int dim, int page, int max_ba
   c.row_min_piece = 2;
   c.elem_bytes = 2;
   c.dec_min_tiles = 4;
-  c.max_items = c.max_groups = static_cast<int>(std::min<int64_t>(
-      std::max<int64_t>(int64_t(max_batch) * hkv * 64, 8192), 1 << 20));
-  c.partial_capacity = kLongPartialFloats;
-  // every query row of a key or score is rounded up to an even number of columns
-  p->sink_floats = scored ? max_keys * hkv * (G + (G & 1)) : 0;
-  // lists (cta offsets, items, groups) three times, units twice, row blocks and
-  // their tables, query rows, chunks, pages
-  const size_t n = c.max_items;
-  p->meta_cap = n * sizeof(KeyItem) +
-                3 * (n * (sizeof(WorkItem) + sizeof(SplitGroup)) +
-                     4 * size_t(c.dec_grid_cap + 1) + 64) +
-                2 * sizeof(UnitRec) * n + n * (sizeof(SeqInfo) + 8) + sizeof(RowInfo) * 16 * n +
-                2 * size_t(max_batch) * sizeof(SeqInfo) +
-                sizeof(ScoreChunk) * size_t(max_batch) *
-                    (size_t(max_pages) * page / kScoreChunk + 1) +
-                4 * size_t(max_batch) * max_pages + 4096;
+  const size_t list_heads = 3 * (4 * size_t(c.dec_grid_cap + 1) + 64) + 4096;
+  if (scored) {
+    // every query row of a key or score is rounded up to an even number of columns
+    p->sink_floats = max_keys * hkv * (G + (G & 1));
+    // What max_keys lets a step have. Query rows: each sees a block of 16 keys at
+    // least, and the i-th of a sequence i keys, so that R rows of B sequences have
+    // R^2 / 2 B of them. Row blocks: full ones, and one more a sequence. Items: a
+    // block's KV heads, and a cut at the end of each CTA's share.
+    const double pairs = double(max_keys) * (G + (G & 1)) / G;
+    p->max_rows = std::min<int64_t>(max_keys / kTileTokens,
+                                    int64_t(std::sqrt(2.0 * max_batch * pairs)) + 1);
+    const int64_t blocks = std::min(p->max_rows, p->max_rows / (kRowBlock / G) + max_batch);
+    const int64_t units = std::min<int64_t>(blocks * (hkv / c.dec_heads), 1 << 28);
+    c.max_groups = static_cast<int>(units);
+    c.max_items = static_cast<int>(units + c.dec_grid_cap);
+    c.partial_capacity = INT32_MAX;  // offsets of records; the workspace grows (hold_records)
+    // decode list, units twice, row blocks, query rows, chunks, pages
+    p->meta_cap = size_t(c.max_items) * (sizeof(WorkItem) + sizeof(KeyItem)) +
+                  size_t(units) * (sizeof(SplitGroup) + 2 * sizeof(UnitRec)) +
+                  size_t(blocks) * (sizeof(SeqInfo) + 8) + size_t(p->max_rows) * sizeof(RowInfo) +
+                  sizeof(ScoreChunk) * size_t(max_batch) *
+                      (size_t(max_pages) * page / kScoreChunk + 1) +
+                  4 * size_t(max_batch) * max_pages + list_heads;
+    p->meta_cap = std::min(p->meta_cap, size_t(INT32_MAX));  // offsets within it
+  } else {
+    c.max_items = c.max_groups = static_cast<int>(std::min<int64_t>(
+        std::max<int64_t>(int64_t(max_batch) * hkv * 64, 8192), 1 << 20));
+    c.partial_capacity = kLongPartialFloats;
+    // lists (cta offsets, items, groups) three times, units twice, sequences and
+    // prefixes, query rows, pages
+    const size_t n = c.max_items;
+    p->meta_cap = n * sizeof(KeyItem) + 3 * n * (sizeof(WorkItem) + sizeof(SplitGroup)) +
+                  2 * sizeof(UnitRec) * n + n * (sizeof(SeqInfo) + 8) + sizeof(RowInfo) * 16 * n +
+                  2 * size_t(max_batch) * sizeof(SeqInfo) + 4 * size_t(max_batch) * max_pages +
+                  list_heads;
+  }
   *plan_out = p;
   if (p->host_only) return FE_OK;
-  cudaError_t e = cudaMalloc(&p->d_partials, sizeof(float) * c.partial_capacity);
+  p->partial_floats = kLongPartialFloats;
+  cudaError_t e = cudaMalloc(&p->d_partials, sizeof(float) * p->partial_floats);
   if (e == cudaSuccess) e = cudaMalloc(&p->d_meta, p->meta_cap);
   if (e == cudaSuccess) e = cudaMemset(p->d_meta, 0, sizeof(MetaHeader));
   if (e == cudaSuccess && p->sink_floats > 0)
     e = cudaMalloc(&p->d_sink, sizeof(float) * p->sink_floats);
-  // a step has no more query rows than row blocks' rows, nor than max_keys / 16
-  // keys (each row sees one block of 16 at least)
-  p->max_rows = scored ? max_keys / kTileTokens : 0;
   if (e == cudaSuccess && p->max_rows > 0)
     e = cudaMalloc(&p->d_norms, sizeof(float2) * p->max_rows * hq);
   for (int i = 0; i < 2 && e == cudaSuccess; ++i) {
@@ -449,6 +472,35 @@ int create_long(const char* what, int hq, int hkv, int dim, int page, int max_ba
     *plan_out = nullptr;
     return cuda_fail(e, (name + ": workspace allocation").c_str());
   }
+  return FE_OK;
+}
+
+// The records of a step with more query rows than the workspace holds at first. A
+// graph's later steps have as many rows, so their records (cut in other places)
+// fit too; the smaller workspace stays for runs that are in flight or captured.
+int hold_records(fe_long_plan* p, const LongResult& res, int batch, int rows, int graph,
+                 const std::string& name) {
+  const PlanConfig& c = p->cfg;
+  int64_t need = res.partial_floats;
+  if (graph) {
+    const int64_t per = kRowBlock / (c.hq / c.hkv), H = c.dec_heads;
+    const int64_t units = std::min<int64_t>(rows, rows / per + batch) * (c.hkv / H);
+    need = int64_t(rows) * c.hq * (c.dim + 2) + 3 * (units + c.dec_grid_cap) +
+           int64_t(c.dec_grid_cap) * H * kRowBlock * (c.dim + 2);
+  }
+  need = std::min<int64_t>(need, INT32_MAX);
+  if (need <= p->partial_floats) return FE_OK;
+  need = std::min<int64_t>(std::max(need, 2 * p->partial_floats), INT32_MAX);
+  p->outgrown.reserve(p->outgrown.size() + 1);
+  float* more = nullptr;
+  const cudaError_t e = cudaMalloc(&more, sizeof(float) * need);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return cuda_fail(e, (name + ": workspace of more query rows").c_str());
+  }
+  p->outgrown.push_back(p->d_partials);
+  p->d_partials = more;
+  p->partial_floats = need;
   return FE_OK;
 }
 
@@ -673,13 +725,17 @@ int fe_scored_plan_prepare(fe_long_plan* p, const int32_t* qo, const int32_t* kv
   const std::string name = "fe_scored_plan_prepare";
   int rc = check_prepare(p, true, batch, rows, graph, name);
   if (rc != FE_OK) return rc;
-  if (!p->host_only && rows > p->max_rows)
+  if (rows > p->max_rows)
     return fail(FE_ERR_CAPACITY, name + ": query rows x keys exceed the plan's max_keys");
   LongResult res;
   std::string err;
   try {
     rc = build_scored_plan(p->cfg, p->keys, qo, kv, pages, last, fresh, batch, rows, graph != 0,
                            p->sink_floats, res, err);
+    if (rc == FE_OK && !p->host_only) {
+      rc = hold_records(p, res, batch, rows, graph, name);
+      if (rc != FE_OK) return rc;
+    }
   } catch (const std::bad_alloc&) {
     return fail(FE_ERR_CAPACITY, name + ": out of host memory");
   }

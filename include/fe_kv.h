@@ -440,8 +440,8 @@ int fe_kv8_attn_run(fe_attn_plan* plan, const void* q, const uint8_t* k_codes,
  * pages and capacities as for fe_attn_plan_create, metadata (HOST) and `graph` as
  * for fe_attn_plan_prepare. Prepare uploads to fixed buffers with one async copy
  * on `stream`: a graph that captured a run replays for later prepares of the same
- * batch and rows. A plan has one workspace (256 MiB of partial records): its runs
- * must not overlap on the GPU. Scale 1/sqrt(dim), fp32 softmax and accumulation,
+ * batch and rows. A plan has one workspace (256 MiB of partial records, more in a
+ * scored plan whose steps need it): its runs must not overlap on the GPU. Scale 1/sqrt(dim), fp32 softmax and accumulation,
  * softmax weights of about 16 bits in the second product, output rounded to
  * nearest even, as fe_attn_run.
  * ------------------------------------------------------------------------ */
@@ -483,8 +483,11 @@ int fe_kv_shared_prefixes(const int32_t* kv, const int32_t* pages, int batch, in
  * (FE_ERR_INVALID_ARGUMENT: scores of a shared page would be added to by two
  * CTAs). max_keys, at creation: the most query rows x keys of a step, each
  * sequence's keys rounded up to a multiple of 16, summed over the sequences; the
- * plan holds hkv * (hq / hkv rounded up to even) fp32 raw scores for each. A
- * step beyond it fails with FE_ERR_CAPACITY. A query row with an infinity or NaN
+ * plan holds hkv * (hq / hkv rounded up to even) fp32 raw scores for each. A step
+ * within it is served, whatever its rows: the first with more than 2^26 / (hq *
+ * (dim + 2)) of them, or such a graph prepare, allocates a larger workspace
+ * (records of 2^31 floats are the most). A step beyond it fails with
+ * FE_ERR_CAPACITY. A query row with an infinity or NaN
  * gives its keys NaN. */
 int fe_scored_plan_create(int hq, int hkv, int dim, int page, int max_batch, int max_pages,
                           int dtype, int num_blocks, int64_t max_keys, fe_long_plan** plan_out);
