@@ -12,8 +12,11 @@
 // rejects tables that would let one sequence write a page the other reads.
 #include <stdint.h>
 
+#include <algorithm>
+#include <new>
 #include <string>
 #include <unordered_set>
+#include <vector>
 
 #include "fe_kv.h"
 
@@ -83,6 +86,68 @@ extern "C" int fe_kv_fork_copies(int num_forks, const int32_t* parent_tables,
   return FE_OK;
 }
 
+namespace fe {
+namespace {
+
+// Cuts the batch into groups of neighbours so that sharing saves the most: a group
+// [a, e) reads its common pages once and not e - a times. With same[b] the pages in
+// common of sequences b - 1 and b, it saves (e - a - 1) * min same[a + 1 .. e - 1];
+// best[x] is the most that the sequences before begin[x] can save. Where same[] does
+// not change a cut saves no more than at either end of the stretch, so that groups
+// begin at those ends only: a batch over few prefixes has few of them. Among equals
+// the larger last group is taken. Returns the groups.
+int share(const int32_t* kv, const int32_t* pages, int batch, int min_pages, int32_t* group_off,
+          int32_t* shared) {
+  std::vector<int32_t> same(size_t(batch) + 1, 0);
+  for (int b = 1; b < batch; ++b) {
+    const int32_t *x = pages + kv[b - 1], *y = pages + kv[b];
+    const int32_t most = std::min(kv[b] - kv[b - 1], kv[b + 1] - kv[b]);
+    int32_t n = 0;
+    while (n < most && x[n] == y[n]) ++n;
+    same[b] = n >= min_pages ? n : 0;
+  }
+  std::vector<int> begin{0};
+  for (int b = 1; b < batch; ++b)
+    if (same[b] == 0 || b == 1 || b + 1 == batch || same[b] != same[b - 1] ||
+        same[b] != same[b + 1])
+      begin.push_back(b);
+  if (batch > 0) begin.push_back(batch);
+  const int ends = static_cast<int>(begin.size());
+  std::vector<int64_t> best(ends, 0);
+  std::vector<int> from(ends, 0);          // the last group begins at begin[from]
+  std::vector<int32_t> common(ends, 0);    // and has so many pages in common
+  for (int x = 1; x < ends; ++x) {
+    const int end = begin[x];
+    int32_t low = INT32_MAX;  // pages in common of the sequences from `a` on
+    best[x] = -1;
+    for (int y = x - 1; y >= 0; --y) {
+      const int a = begin[y];
+      if (begin[y + 1] - a > 1) low = std::min(low, same[a + 1]);
+      if (y + 1 < x) low = std::min(low, same[begin[y + 1]]);
+      if (low == 0) break;
+      // no group that begins before can save more
+      if (end - a > 1 && best[y] + int64_t(end - 1) * low < best[x]) break;
+      const int64_t saved = best[y] + (end - a > 1 ? int64_t(end - a - 1) * low : 0);
+      if (saved >= best[x]) {
+        best[x] = saved;
+        from[x] = y;
+        common[x] = end - a > 1 ? low : 0;
+      }
+    }
+  }
+  int groups = 0;
+  for (int x = ends - 1; x > 0; x = from[x]) ++groups;
+  group_off[0] = 0;
+  for (int x = ends - 1, g = groups; x > 0; x = from[x]) {
+    group_off[g] = begin[x];
+    shared[--g] = common[x];
+  }
+  return groups;
+}
+
+}  // namespace
+}  // namespace fe
+
 extern "C" int fe_kv_shared_prefixes(const int32_t* kv, const int32_t* pages, int batch,
                                      int min_pages, int32_t* group_off, int32_t* shared,
                                      int* num_groups) {
@@ -99,25 +164,10 @@ extern "C" int fe_kv_shared_prefixes(const int32_t* kv, const int32_t* pages, in
     if (kv[b + 1] < kv[b])
       return fail(FE_ERR_INVALID_ARGUMENT, "fe_kv_shared_prefixes: kv decreases (b=" +
                                                std::to_string(b) + ")");
-  group_off[0] = 0;
-  int n = 0;
-  for (int b = 0; b < batch;) {
-    const int32_t* head = pages + kv[b];
-    int64_t common = int64_t(kv[b + 1]) - kv[b];
-    int end = b + 1;
-    for (; end < batch; ++end) {
-      const int64_t len = int64_t(kv[end + 1]) - kv[end];
-      int64_t same = 0;
-      while (same < common && same < len && head[same] == pages[kv[end] + same]) ++same;
-      // the first neighbour sets what the group shares; one that shares less than
-      // half of it begins a group of its own
-      if (same < min_pages || (end > b + 1 && 2 * same < common)) break;
-      common = same;
-    }
-    shared[n] = end > b + 1 ? static_cast<int32_t>(common) : 0;
-    group_off[++n] = end;
-    b = end;
+  try {
+    *num_groups = fe::share(kv, pages, batch, min_pages, group_off, shared);
+  } catch (const std::bad_alloc&) {
+    return fail(FE_ERR_CAPACITY, "fe_kv_shared_prefixes: out of host memory");
   }
-  *num_groups = n;
   return FE_OK;
 }

@@ -756,8 +756,9 @@ def compact_tokens(k_pool, v_pool, scores, kept, kv, pages, last, page, dst_kv=N
 
 def shared_prefixes(kv, pages, min_pages=1):
     """The groups of a batch whose sequences begin with the same pages (host
-    only): group_off (the first sequence of each group, then the batch) and
-    shared (pages in common), for SharedPlan.prepare."""
+    only), cut so that sharing saves the most: group_off (the first sequence of
+    each group, then the batch) and shared (pages in common), for
+    SharedPlan.prepare."""
     kv, pages = _host_i32(kv), _host_i32(pages)
     batch = kv.shape[0] - 1
     if batch < 0 or (batch and pages.shape[0] < kv[batch]):

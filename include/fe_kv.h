@@ -466,11 +466,12 @@ int fe_shared_plan_prepare(fe_long_plan* plan, const int32_t* qo, const int32_t*
 int fe_shared_attn_run(fe_long_plan* plan, const void* q, const void* k_pool, const void* v_pool,
                        void* out, int causal, void* stream);
 /* The groups of a batch from its page lists (HOST memory only, needs no GPU):
- * neighbours whose first min_pages pages or more are the same, as long as the
- * group goes on sharing half of what its first two members do. kv [batch+1] has to
- * begin with 0 and not to decrease (FE_ERR_INVALID_ARGUMENT), and pages to hold
- * kv[batch] entries. group_off [batch+1] and shared [batch] receive the
- * *num_groups groups. */
+ * neighbours whose first min_pages pages or more are the same. Of all ways to cut
+ * the batch into such groups the one that saves the most is taken, the sum of
+ * (members - 1) x pages in common: a sequence that has little in common with its
+ * neighbours stays out of their groups. kv [batch+1] has to begin with 0 and not to
+ * decrease (FE_ERR_INVALID_ARGUMENT), and pages to hold kv[batch] entries.
+ * group_off [batch+1] and shared [batch] receive the *num_groups groups. */
 int fe_kv_shared_prefixes(const int32_t* kv, const int32_t* pages, int batch, int min_pages,
                           int32_t* group_off, int32_t* shared, int* num_groups);
 
