@@ -454,6 +454,7 @@ struct MoveArgs {
 
 __global__ void __launch_bounds__(kMoveThreads) compact_kernel(const MoveArgs a) {
   __shared__ int2 table[2][kTableTokens];  // source and destination slot, -1: no move
+  __shared__ int ends[2][kMoveThreads / 32];  // a warp's first entry below 0
   pdl_trigger();
   pdl_wait();
   const int b = blockIdx.x / a.hkv, h = blockIdx.x % a.hkv;
@@ -489,8 +490,10 @@ __global__ void __launch_bounds__(kMoveThreads) compact_kernel(const MoveArgs a)
   int next = static_cast<int>(threadIdx.x) < a.budget ? __ldg(kept + threadIdx.x) : -1;
   int buf = 0;
   for (int base = 0; base < a.budget; base += kTableTokens, buf ^= 1) {
+    const int j = base + threadIdx.x;
+    bool bad = false;
     {
-      const int j = base + threadIdx.x, t = next;
+      const int t = next;
       const int jn = j + kTableTokens;
       next = jn < a.budget ? __ldg(kept + jn) : -1;
       int2 e = make_int2(-1, -1);
@@ -499,17 +502,22 @@ __global__ void __launch_bounds__(kMoveThreads) compact_kernel(const MoveArgs a)
           e.x = static_cast<int>(slot_of(a.src, p0, t));
           e.y = static_cast<int>(slot_of(a.in_place ? a.src : a.dst, d0, j));
         }
-        if (e.x < 0 || e.y < 0) {
-          if (blockIdx.y == 0) raise_device_error(a.err, FE_DEVERR_PAGE_RANGE);
-          e = make_int2(-1, -1);
-        }
+        bad = e.x < 0 || e.y < 0;
+        if (bad) e = make_int2(-1, -1);
       }
       table[buf][threadIdx.x] = e;
+      const unsigned none = __ballot_sync(0xffffffffu, t < 0);  // (also past the budget)
+      if ((threadIdx.x & 31) == 0)
+        ends[buf][threadIdx.x >> 5] = none ? j + __ffs(none) - 1 : INT32_MAX;
     }
-    // nothing of these tokens moves: a prefix that stays, the end of the list.
     // (Two buffers: this barrier also keeps the table before the last in use.)
-    if (!__syncthreads_or(table[buf][threadIdx.x].x >= 0)) continue;
-    const int count = min(kTableTokens, a.budget - base);
+    const bool moves = __syncthreads_or(table[buf][threadIdx.x].x >= 0);
+    int end = INT32_MAX;  // the list ends at its first entry below 0
+#pragma unroll
+    for (int w = 0; w < kMoveThreads / 32; ++w) end = min(end, ends[buf][w]);
+    if (bad && j < end && blockIdx.y == 0) raise_device_error(a.err, FE_DEVERR_PAGE_RANGE);
+    // where nothing of these tokens moves: a prefix that stays
+    const int count = moves ? min(kTableTokens, end - base) : 0;
     for (int j0 = 0; j0 < count; j0 += rows * kMoveUnroll) {
       int2 e[kMoveUnroll];
       uint4 x[kMoveUnroll];
@@ -530,6 +538,7 @@ __global__ void __launch_bounds__(kMoveThreads) compact_kernel(const MoveArgs a)
         if (scoring) sc[e[u].y] = s[u];
       }
     }
+    if (end < base + kTableTokens) break;
   }
 }
 
