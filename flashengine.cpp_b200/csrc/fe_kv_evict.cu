@@ -554,6 +554,8 @@ int check_lists(const char* what, const int32_t* kv, const int32_t* pages, const
                 name + ": cache_slots must be whole pages, below 2^31");
   if (int64_t(batch) * hkv > INT32_MAX)
     return fail(FE_ERR_CAPACITY, name + ": batch x hkv too large");
+  // (the kernels' indexes of an entry go a block's threads past the last)
+  if (budget > (1 << 30)) return fail(FE_ERR_CAPACITY, name + ": budget above 2^30");
   if (batch > 0 && budget > 0 && (!kv || !pages || !last))
     return fail(FE_ERR_INVALID_ARGUMENT, name + ": null pointer");
   return FE_OK;

@@ -140,7 +140,7 @@ int fe_kv_gather(const void* pool, void* out, const int32_t* kv, const int32_t* 
  * metadata: kv [batch+1], pages [num_pages] (kv[batch] of them are used) and
  * last [batch] as in fe_attn_plan_prepare. A sequence that reaches past the
  * page list, or a page past the pool, is skipped (its kept entries are -1) and
- * raises FE_DEVERR_PAGE_RANGE.
+ * raises FE_DEVERR_PAGE_RANGE. A budget of at most 2^30 tokens.
  *
  * fe_kv_select: the tokens to keep, int32 kept [batch, hkv, budget], ascending.
  * Of a sequence of more than `budget` tokens each KV head keeps the first `sink`,
