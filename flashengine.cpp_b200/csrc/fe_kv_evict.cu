@@ -597,7 +597,7 @@ int fe_kv_select(const float* scores, const int32_t* kv, const int32_t* pages, i
   while (cluster < kSelCluster && lists * cluster * 2 <= kSelCtas &&
          max_len >= 2 * cluster * kSelPart)
     cluster *= 2;
-  const int room = std::min(max_len / cluster + 32, kSelRoom);
+  const int room = std::min(std::min(max_len / cluster, kSelRoom) + 32, kSelRoom);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(lists * cluster);
   cfg.blockDim = dim3(kSelThreads);
