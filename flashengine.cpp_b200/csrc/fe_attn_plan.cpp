@@ -385,15 +385,17 @@ int read_step(const PlanConfig& cfg, const int32_t* qo, const int32_t* kv, const
     err = "pages must be non-null";
     return FE_ERR_INVALID_ARGUMENT;
   }
-  seqs.resize(batch);
-  for (int b = 0; b < batch; ++b) {
-    const int q0 = qo[b], q1 = qo[b + 1];
-    const int p0 = kv[b], p1 = kv[b + 1];
-    if (q1 < q0 || p1 <= p0) {
+  // before any page is read: every list lies within the first kv[batch] pages
+  for (int b = 0; b < batch; ++b)
+    if (qo[b + 1] < qo[b] || kv[b + 1] <= kv[b]) {
       err = "qo must be non-decreasing and every sequence must own at least one page (b=" +
             std::to_string(b) + ")";
       return FE_ERR_INVALID_ARGUMENT;
     }
+  seqs.resize(batch);
+  for (int b = 0; b < batch; ++b) {
+    const int q0 = qo[b], q1 = qo[b + 1];
+    const int p0 = kv[b], p1 = kv[b + 1];
     if (last[b] < 1 || last[b] > cfg.page) {
       err = "last[b] must be in [1, page] (b=" + std::to_string(b) + ")";
       return FE_ERR_INVALID_ARGUMENT;
