@@ -110,8 +110,6 @@ int build_view(const PlanConfig& cfg, const std::vector<Unit>& units, int grid_c
   return FE_OK;
 }
 
-}  // namespace
-
 // Decode lists (and head_dim 256 row lists) cost in proportion to key
 // tiles, so they are balanced exactly: the units' tile ranges are laid end to
 // end and cut into `grid` equal contiguous pieces, one per CTA. A unit cut
@@ -149,7 +147,7 @@ int build_cut_view(const PlanConfig& cfg, const std::vector<Unit>& units, int gr
   // pass 2: emit items CTA by CTA
   std::vector<int> group_of(units.size(), -1), part0_of(units.size(), -1), next_split(units.size(), 0);
   for (size_t i = 0; i < units.size(); ++i) {
-    if (pieces[i] > 1 || units[i].record) {
+    if (pieces[i] > 1) {
       const Unit& u = units[i];
       const int rec = partial_rec_floats(u.rows, cfg.dim);
       group_of[i] = static_cast<int>(v.groups.size());
@@ -163,7 +161,6 @@ int build_cut_view(const PlanConfig& cfg, const std::vector<Unit>& units, int gr
       ++v.split_units;
     }
   }
-  v.unit_group = group_of;
   v.cta_off.clear();
   int64_t room = per;
   int cta = 0;
@@ -215,13 +212,17 @@ int build_cut_view(const PlanConfig& cfg, const std::vector<Unit>& units, int gr
   return FE_OK;
 }
 
-// Row lists of the 8-bit cache. The kernel's time for an item is its key tiles
-// (of cfg.row_tile 16-key pieces) plus a fixed cost worth cfg.row_item_tiles of
-// them (queries, first scores, epilogue), so a cut by tiles alone gives the
-// CTAs of a step's many short items far more time than the others (a mixed
-// step took 314 us where this cut takes a third). The units are laid end to end
-// and cut into at most grid_cap pieces of equal cost, at whole tiles, in pieces
-// of at least cfg.row_min_piece tiles.
+}  // namespace
+
+// Row lists of the 8-bit cache, and both lists of the plans for long shared prompts
+// (whose units may ask for a record although they are not cut). A kernel's time
+// for an item is its key tiles (of cfg.row_tile 16-key pieces, each worth
+// cfg.row_weight) plus a fixed cost of cfg.row_item_tiles (queries, first scores,
+// epilogue), so a cut by tiles alone gives the CTAs of a step's many short items
+// far more time than the others (a mixed step over the 8-bit cache took 314 us
+// where this cut takes a third). The units are laid end to end and cut into at
+// most grid_cap pieces of equal cost, at whole tiles, in pieces of at least
+// cfg.row_min_piece tiles.
 int build_cost_view(const PlanConfig& cfg, const std::vector<Unit>& units, int grid_cap_in,
                     bool fixed_grid, View& v, std::string& err) {
   const int64_t kMinPiece = cfg.row_min_piece;

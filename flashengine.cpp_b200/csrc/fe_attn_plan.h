@@ -83,7 +83,7 @@ struct PlanConfig {
   int row_group_blocks;       // 16-row blocks per row-mode item (8 = one 128-row tcgen05 tile)
   bool row_split;             // row-mode key ranges may be split across CTAs
   bool cut_rows;              // row items' key ranges are cut across CTAs (head_dim 256, 8-bit)
-  int row_tile;               // 8-bit row lists: 16-key pieces per tile of the kernel,
+  int row_tile;               // lists cut by cost: 16-key pieces per tile of the kernel,
   int row_item_tiles;         // and an item's fixed cost in tiles (0: cut by keys alone)
   int row_weight[2];          // cost of a tile, in the fixed cost's units, of items of up to
   int row_pair_blocks;        // row_pair_blocks 16-row blocks and of more (0: none)

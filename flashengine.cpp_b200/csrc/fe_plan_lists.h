@@ -12,14 +12,14 @@ namespace fe {
 // One (sequence, KV head or heads, query-row block) against its key tiles.
 struct Unit {
   int seq, kvh, key_mode, rb0, nrb, tiles, rows;
-  bool record = false;  // writes partial records even when it is not split
+  bool record = false;  // lists cut by cost: a record even when it is not cut
 };
 
 struct View {
   std::vector<int32_t> cta_off;
   std::vector<WorkItem> items;
   std::vector<SplitGroup> groups;
-  std::vector<int> unit_group;  // cut lists: group of each unit, -1 for none
+  std::vector<int> unit_group;  // lists cut by cost: group of each unit, -1 for none
   int grid = 0, chunk = 0, decode_items = 0, prefill_items = 0, split_units = 0;
   int64_t partial_floats = 0;
 };
@@ -31,9 +31,6 @@ inline size_t align16(size_t n) { return (n + 15) & ~size_t(15); }
 int read_step(const PlanConfig& cfg, const int32_t* qo, const int32_t* kv, const int32_t* pages,
               const int32_t* last, int batch, int rows, std::vector<SeqInfo>& seqs,
               std::string& err);
-
-int build_cut_view(const PlanConfig& cfg, const std::vector<Unit>& units, int grid_cap,
-                   int min_tiles_per_cta, bool fixed_grid, View& v, std::string& err);
 
 int build_cost_view(const PlanConfig& cfg, const std::vector<Unit>& units, int grid_cap,
                     bool fixed_grid, View& v, std::string& err);
