@@ -295,17 +295,27 @@ __global__ void __launch_bounds__(kScoreThreads, 8)
 
 using namespace fe;
 
+// What a step's kernels read and write of the plan: its lists, and records of up to
+// `floats`.
+struct LongSpace {
+  uint8_t* meta = nullptr;
+  float* partials = nullptr;
+  int64_t floats = 0;
+};
+
 struct fe_long_plan {
   PlanConfig cfg{};
   int dtype = 0;
   bool scored = false, host_only = false;
   bool keys = false;  // the decode list is the key kernel's
   int device = -1;
-  uint8_t* d_meta = nullptr;
+  // The first serves most steps; later, larger ones the steps with more query rows.
+  // None is freed before the plan, as a captured run keeps the one that it was
+  // captured with, and a step takes the first that it fits, so that a graph's later
+  // steps come to the same one.
+  std::vector<LongSpace> spaces;
+  size_t space = 0;  // of the last prepare
   size_t meta_cap = 0;
-  float* d_partials = nullptr;
-  int64_t partial_floats = 0;
-  std::vector<float*> outgrown;  // earlier, smaller d_partials: a captured run may hold them
   float* d_sink = nullptr;
   float2* d_norms = nullptr;  // scored plans: (m, 1 / l) of each query row and head
   int64_t max_rows = 0;
@@ -341,13 +351,31 @@ void destroy_long(fe_long_plan* p) {
       }
       if (p->h_meta[i]) cudaFreeHost(p->h_meta[i]);
     }
-    if (p->d_meta) cudaFree(p->d_meta);
-    if (p->d_partials) cudaFree(p->d_partials);
-    for (float* x : p->outgrown) cudaFree(x);
+    for (const LongSpace& x : p->spaces) {
+      if (x.meta) cudaFree(x.meta);
+      if (x.partials) cudaFree(x.partials);
+    }
     if (p->d_sink) cudaFree(p->d_sink);
     if (p->d_norms) cudaFree(p->d_norms);
   }
   delete p;
+}
+
+cudaError_t add_space(fe_long_plan* p, int64_t floats) {
+  LongSpace x;
+  x.floats = floats;
+  cudaError_t e = cudaMalloc(&x.partials, sizeof(float) * floats);
+  if (e == cudaSuccess) e = cudaMalloc(&x.meta, p->meta_cap);
+  if (e == cudaSuccess) try {
+      p->spaces.push_back(x);
+      return e;
+    } catch (const std::bad_alloc&) {
+      e = cudaErrorMemoryAllocation;
+    }
+  if (x.meta) cudaFree(x.meta);
+  if (x.partials) cudaFree(x.partials);
+  cudaGetLastError();
+  return e;
 }
 
 int create_long(const char* what, int hq, int hkv, int dim, int page, int max_batch,
@@ -453,10 +481,8 @@ int create_long(const char* what, int hq, int hkv, int dim, int page, int max_ba
   }
   *plan_out = p;
   if (p->host_only) return FE_OK;
-  p->partial_floats = kLongPartialFloats;
-  cudaError_t e = cudaMalloc(&p->d_partials, sizeof(float) * p->partial_floats);
-  if (e == cudaSuccess) e = cudaMalloc(&p->d_meta, p->meta_cap);
-  if (e == cudaSuccess) e = cudaMemset(p->d_meta, 0, sizeof(MetaHeader));
+  cudaError_t e = add_space(p, kLongPartialFloats);
+  if (e == cudaSuccess) e = cudaMemset(p->spaces[0].meta, 0, sizeof(MetaHeader));
   if (e == cudaSuccess && p->sink_floats > 0)
     e = cudaMalloc(&p->d_sink, sizeof(float) * p->sink_floats);
   if (e == cudaSuccess && p->max_rows > 0)
@@ -475,11 +501,11 @@ int create_long(const char* what, int hq, int hkv, int dim, int page, int max_ba
   return FE_OK;
 }
 
-// The records of a step with more query rows than the workspace holds at first. A
-// graph's later steps have as many rows, so their records (cut in other places)
-// fit too; the smaller workspace stays for runs that are in flight or captured.
-int hold_records(fe_long_plan* p, const LongResult& res, int batch, int rows, int graph,
-                 const std::string& name) {
+// The space for a step: by the records that it needs, those of a graph's later steps
+// (as many query rows, cut in other places) among them. Nothing of the plan's
+// current step changes.
+int find_space(fe_long_plan* p, const LongResult& res, int batch, int rows, int graph,
+               const std::string& name, size_t& space) {
   const PlanConfig& c = p->cfg;
   int64_t need = res.partial_floats;
   if (graph) {
@@ -487,25 +513,18 @@ int hold_records(fe_long_plan* p, const LongResult& res, int batch, int rows, in
     const int64_t units = std::min<int64_t>(rows, rows / per + batch) * (c.hkv / H);
     need = int64_t(rows) * c.hq * (c.dim + 2) + 3 * (units + c.dec_grid_cap) +
            int64_t(c.dec_grid_cap) * H * kRowBlock * (c.dim + 2);
+    need = std::min<int64_t>(need, INT32_MAX);
   }
-  need = std::min<int64_t>(need, INT32_MAX);
-  if (need <= p->partial_floats) return FE_OK;
-  need = std::min<int64_t>(std::max(need, 2 * p->partial_floats), INT32_MAX);
-  p->outgrown.reserve(p->outgrown.size() + 1);
-  float* more = nullptr;
-  const cudaError_t e = cudaMalloc(&more, sizeof(float) * need);
-  if (e != cudaSuccess) {
-    cudaGetLastError();
-    return cuda_fail(e, (name + ": workspace of more query rows").c_str());
-  }
-  p->outgrown.push_back(p->d_partials);
-  p->d_partials = more;
-  p->partial_floats = need;
+  for (space = 0; space < p->spaces.size(); ++space)
+    if (need <= p->spaces[space].floats) return FE_OK;
+  const cudaError_t e = add_space(
+      p, std::min<int64_t>(std::max(need, 2 * p->spaces.back().floats), INT32_MAX));
+  if (e != cudaSuccess) return cuda_fail(e, (name + ": workspace of more query rows").c_str());
   return FE_OK;
 }
 
 // Upload a step's metadata and take it as the plan's current one.
-int install(fe_long_plan* p, LongResult& res, int batch, int rows, int graph,
+int install(fe_long_plan* p, LongResult& res, size_t space, int batch, int rows, int graph,
             const std::string& name, void* stream) {
   if (res.meta.size() > p->meta_cap)
     return fail(FE_ERR_CAPACITY, name + ": metadata exceeds workspace");
@@ -522,13 +541,14 @@ int install(fe_long_plan* p, LongResult& res, int batch, int rows, int graph,
       p->h_cap[i] = cap;
     }
     std::memcpy(p->h_meta[i], res.meta.data(), res.meta.size());
-    FE_CUDA_TRY(
-        cudaMemcpyAsync(p->d_meta, p->h_meta[i], res.meta.size(), cudaMemcpyHostToDevice, s));
+    FE_CUDA_TRY(cudaMemcpyAsync(p->spaces[space].meta, p->h_meta[i], res.meta.size(),
+                                cudaMemcpyHostToDevice, s));
     FE_CUDA_TRY(cudaEventRecord(p->h_ev[i], s));
     p->h_used[i] = true;
     p->h_idx ^= 1;
   }
   p->last = std::move(res);
+  p->space = space;
   p->prepared = true;
   p->fixed_grid = graph != 0;
   if (graph) {
@@ -599,10 +619,10 @@ int maps(fe_long_plan* p, const void* k_pool, const void* v_pool) {
 template <typename T>
 AttnArgs<T> long_args(const fe_long_plan* p, const void* q, void* out, int view, int q_map_rows) {
   AttnArgs<T> a{};
-  a.meta = p->d_meta;
+  a.meta = p->spaces[p->space].meta;
   a.q = static_cast<const T*>(q);
   a.out = static_cast<T*>(out);
-  a.partials = p->d_partials;
+  a.partials = p->spaces[p->space].partials;
   a.err = device_error_word();
   a.hq = p->cfg.hq;
   a.G = p->cfg.hq / p->cfg.hkv;
@@ -664,7 +684,7 @@ int run_scored(fe_long_plan* p, const void* q, float* scores, void* out, cudaStr
   const int most = std::max(1, 16 * c.grid_cap / c.hkv);
   const dim3 grid(p->fixed_grid ? most : std::max(1, std::min(p->last.n_chunks, most)), c.hkv);
   FE_CUDA_TRY(launch_pdl(score_kernel, grid, dim3(kScoreThreads), 0, s,
-                         static_cast<const uint8_t*>(p->d_meta),
+                         static_cast<const uint8_t*>(a.meta),
                          static_cast<const float*>(p->d_sink),
                          static_cast<const float2*>(p->d_norms), scores, c.hq, c.hkv, c.page,
                          int64_t(c.num_blocks + 1) * c.page));
@@ -716,7 +736,7 @@ int fe_shared_plan_prepare(fe_long_plan* p, const int32_t* qo, const int32_t* kv
     return fail(FE_ERR_CAPACITY, name + ": out of host memory");
   }
   if (rc != FE_OK) return fail(rc, name + ": " + err);
-  return install(p, res, batch, rows, graph, name, stream);
+  return install(p, res, 0, batch, rows, graph, name, stream);
 }
 
 int fe_scored_plan_prepare(fe_long_plan* p, const int32_t* qo, const int32_t* kv,
@@ -728,19 +748,20 @@ int fe_scored_plan_prepare(fe_long_plan* p, const int32_t* qo, const int32_t* kv
   if (rows > p->max_rows)
     return fail(FE_ERR_CAPACITY, name + ": query rows x keys exceed the plan's max_keys");
   LongResult res;
+  size_t space = 0;
   std::string err;
   try {
     rc = build_scored_plan(p->cfg, p->keys, qo, kv, pages, last, fresh, batch, rows, graph != 0,
                            p->sink_floats, res, err);
     if (rc == FE_OK && !p->host_only) {
-      rc = hold_records(p, res, batch, rows, graph, name);
+      rc = find_space(p, res, batch, rows, graph, name, space);
       if (rc != FE_OK) return rc;
     }
   } catch (const std::bad_alloc&) {
     return fail(FE_ERR_CAPACITY, name + ": out of host memory");
   }
   if (rc != FE_OK) return fail(rc, name + ": " + err);
-  return install(p, res, batch, rows, graph, name, stream);
+  return install(p, res, space, batch, rows, graph, name, stream);
 }
 
 int fe_shared_attn_run(fe_long_plan* p, const void* q, const void* k_pool, const void* v_pool,

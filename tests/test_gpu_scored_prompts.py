@@ -30,7 +30,7 @@ def test_prompt_of_one_sequence(shape, n):
 def test_workspace_grows_and_captured_runs_stay():
     """128 heads, 1030 query rows of each of four sequences: 2^26 floats hold the
     records of 4032. A run captured before keeps the workspace that it was
-    captured with."""
+    captured with, lists and records: steps of other workspaces do not reach it."""
     import fekv
     import torch
     big = Step([(0, [(1030, 1030)] * 4)], 128, 8, 128, 16, "bfloat16")
@@ -51,8 +51,9 @@ def test_workspace_grows_and_captured_runs_stay():
         plan.attention(small.q, small.k, small.v, scores, out)
     run(big, plan)
     assert plan.info()["partial_floats"] > 1 << 26
-    for _ in range(2):
-        plan.prepare(*small.meta(), graph=True)
+    for again in (False, True, True):
+        if again:
+            plan.prepare(*small.meta(), graph=True)
         scores.copy_(before)
         out.zero_()
         g.replay()
