@@ -29,7 +29,7 @@ struct AttnArgs {
   int hq, G, page, view;
   float scale_log2;
   int q_map_rows;  // query rows the row kernel's Q tensor map covers (0: none)
-  float* sink;     // scored plans: where the decode kernel stores raw scores
+  float* sink;     // scored plans: where the key or decode kernel stores raw scores
 };
 
 __device__ __forceinline__ uint64_t global_ns() {

@@ -154,10 +154,15 @@ __device__ __forceinline__ int2 find_bin(const Cluster& cl, const int* hist, int
 // Scores are read four tokens at a time (pages are multiples of 16), each twice;
 // a note is a byte per four tokens (above the threshold, at it). A sequence of
 // more than `room` tokens is read again for the output, and so is one whose bin
-// has more than kSelList keys (equal or close scores). 64 sequences of up to 32k
-// tokens, 8 heads: 40 us, bound by the instructions of the two sweeps, some forty a
-// token (75 us with all keys in shared memory and one CTA an SM; 52 with a byte's
-// tokens written at a time and a branch a token). With 256 threads 79, with 1024 65.
+// has more than kSelList keys (equal or close scores). 64 sequences of 4 to 36 Ki
+// tokens, 8 heads: 43 us (40 where the L2 holds the scores already). That is latency
+// before all: a CTA's sweeps follow one another behind barriers, each load of
+// scores behind that of its page, with three CTAs an SM, and eight lists of 32k tokens
+// on an empty GPU take 26 us with a CTA each. Warps issue in 46 % of the slots
+// (24.5 M instructions, 115 a token counting all lanes and phases), 57 % on the SM
+// with the most. Measured before: 75 us with all keys in shared memory and one CTA an
+// SM, 52 with a byte's tokens written at a time and a branch a token, 79 with 256
+// threads, 65 with 1024.
 __global__ void __launch_bounds__(kSelThreads, 3)
     select_kernel(const float* __restrict__ scores, const SeqTable table,
                   int32_t* __restrict__ kept, int batch, int hkv, int budget, int sink,
@@ -427,11 +432,11 @@ __global__ void __launch_bounds__(kSelThreads, 3)
 
 // ---------------------------------------------------------------------------
 // compaction: for every sequence and KV head, the K and V rows and the score
-// of token kept[j] move to token j. A CTA walks the list of one (sequence,
-// head) in order, for one slice of the row's 16-byte chunks (slices give one
-// sequence's move more CTAs). A table of the source and destination slots of
-// kTableTokens tokens is made first, so that the moves wait for no index. Each
-// step moves rows * kMoveUnroll tokens: all of them are read before any is
+// of token kept[j] move to token j, for every j before the list's first entry
+// below 0. A CTA walks the list of one (sequence, head) in order, for one slice
+// of the row's 16-byte chunks (slices give one sequence's move more CTAs). A
+// table of the source and destination slots of kTableTokens tokens is made
+// first, so that the moves wait for no index. Each step moves rows * kMoveUnroll tokens: all of them are read before any is
 // written, and the sources of later steps lie at or past their own index
 // (kept[j] >= j, checked), which no earlier step writes; so the move works in
 // place.

@@ -4,10 +4,11 @@
 // reference, whose attention reads each sequence's pages by itself
 // (Cambridgebit/FlashEngine.cpp src/flashinfer_attention.cu:35-44).
 //
-// Both run the decode kernel (fe_decode.cu) and the row kernel
-// (fe_rows2_tc.cu, fe_prefill_tc.cu at
-// head_dim 256) over the lists of fe_long_plan.h. A record holds, for each
-// of its rows, m = the largest base-2 score of its keys, l = sum 2^(s - m) and
+// Both run over the lists of fe_long_plan.h: up to 16 packed rows by the key kernel
+// (fe_keys.cu; at head_dim 256 the decode kernel, fe_decode.cu), more rows of the
+// shared plans by a row kernel (fe_rows2_tc.cu; at 256 fe_prefill_tc.cu). Scored plans
+// cut their rows into blocks of 16 and run no row kernel. A record holds, for each of
+// its rows, m = the largest base-2 score of its keys, l = sum 2^(s - m) and
 // O = sum 2^(s - m) v; records of disjoint keys join as
 //   m = max m_i, l = sum l_i 2^(m_i - m), out = sum O_i 2^(m_i - m) / l.
 // The weight of a key with score s is then 2^(s - m) / l. (2^(s - (m + log2 l)) loses
@@ -167,10 +168,12 @@ __device__ __forceinline__ void find_records(const AttnArgs<T>& a, int64_t w, Re
 }
 
 // One warp per query row and head; norms (scored plans): where (m, 1 / l) of each
-// goes, [rows, hq]. Few pairs: four records of one in flight (eight: 2 us more
-// for 64 rows of 64 heads, whose warps are then not all resident). Many: what counts
-// are loads in flight an SM, so two records a warp and more warps (2048 rows of
-// 32 heads, 60 % with two records: 7 us less; 64 rows of 64 heads 2 us more).
+// goes, [rows, hq]. A warp has kStep records in flight: with few pairs of row and
+// head all warps are resident and four shorten each one's chain of loads; with many
+// what counts are loads in flight an SM, and two leave registers for more warps.
+// Whole calls in us with four and with two at head_dim 128: 4 rows of 16 heads 7.2
+// and 7.8, 128 rows of 32 heads 21.6 and 22.6, 64 rows of 64 heads 68.0 and 68.3,
+// 2048 rows of 32 heads (many pairs) 113.1 and 111.5.
 constexpr int kManyPairs = 148 * 48;
 
 template <typename T, int D, int kStep>

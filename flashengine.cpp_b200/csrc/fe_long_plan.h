@@ -1,6 +1,8 @@
-// Host planners of the shared-prefix and the scored plans: work lists for the
-// decode and row kernels (fe_attn_plan.h) whose items write partial records,
-// and the tables by which the kernels of fe_long_attn.cu join them. Pure C++.
+// Host planners of the shared-prefix and the scored plans: work lists for the key
+// kernel (at head_dim 256 the decode kernel) and the row kernels whose items write
+// partial records, and the tables by which the kernels of fe_long_attn.cu join
+// them. "Decode list" below is list 2 of fe_attn_plan.h, whichever kernel serves
+// it. Pure C++.
 //
 // Shared-prefix plans: the sequences of a group begin with the same pages. The
 // group's prefix becomes one more sequence of the lists, with the query rows of
@@ -9,8 +11,8 @@
 // softmax of its records from both.
 //
 // Scored plans: the query rows of a sequence are cut into blocks of at most 16
-// packed rows, each a sequence of the decode list, whose raw scores the decode
-// kernel stores beside the records.
+// packed rows, each a sequence of the decode list, whose raw scores the kernel
+// stores beside the records.
 #pragma once
 
 #include <stdint.h>

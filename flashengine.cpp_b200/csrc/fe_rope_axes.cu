@@ -131,9 +131,13 @@ __global__ void __launch_bounds__(kAxesThreads)
 // a head.
 constexpr int kRowBufs = 3;
 // From this many rows the ring of bulk copies is used (us by threads and by the
-// ring, head_dim 128): 4096 rows of 4 + 1 heads 8.7 and 9.9, of 16 + 1 heads 17.8 and
-// 13.0, of 32 + 8 heads 23.0 and 20.3; 2048 rows of those 5.4 and 8.0, 9.3 and 8.6,
-// 11.5 and 12.2; 32k rows of 4 + 1 heads 50.7 and 46.1, of 16 + 1 heads 170 and 69.
+// ring, head_dim 128, all dims rotated): 4096 rows of 4 + 1 heads 8.7 and 9.9, of
+// 16 + 1 heads 17.8 and 13.0, of 32 + 8 heads 23.0 and 20.3; 2048 rows of those 5.4 and
+// 8.0, 9.3 and 8.6, 11.5 and 12.2; 32k rows of 4 + 1 heads 50.7 and 46.1, of 16 + 1
+// heads 170 and 69. With fewer dims rotated the ring moves the rest of q as well,
+// which the threads skip, and is the faster one all the same: 64k rows of 32 + 8 heads
+// of 128 with 64 rotated 365 and 284, with 32 rotated 559 and 282, of 16 + 2 heads of
+// 256 with 64 rotated 352 and 240.
 constexpr int kBulkRows = 4096;
 constexpr int kBulkSmem = 112 * 1024;
 
