@@ -41,6 +41,9 @@ int fail(int status, const std::string& msg) {
 }
 
 int cuda_fail(cudaError_t rc, const char* what) {
+  // the caller learns of it by the status: as the thread's last error it would be
+  // reported again by whatever checks that next
+  cudaGetLastError();
   t_error = std::string(what) + ": " + cudaGetErrorName(rc) + " (" + cudaGetErrorString(rc) + ")";
   return FE_ERR_CUDA;
 }

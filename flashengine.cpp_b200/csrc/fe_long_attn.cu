@@ -377,7 +377,6 @@ cudaError_t add_space(fe_long_plan* p, int64_t floats) {
     }
   if (x.meta) cudaFree(x.meta);
   if (x.partials) cudaFree(x.partials);
-  cudaGetLastError();
   return e;
 }
 
