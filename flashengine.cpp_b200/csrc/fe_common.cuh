@@ -84,6 +84,7 @@ __device__ __forceinline__ void raise_device_error(unsigned int* word, unsigned 
 }
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+inline bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
 
 // ---- element traits ------------------------------------------------------
 

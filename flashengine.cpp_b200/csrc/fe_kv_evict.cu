@@ -587,6 +587,8 @@ int fe_kv_select(const float* scores, const int32_t* kv, const int32_t* pages, i
   if (!scores || !kept) return fail(FE_ERR_INVALID_ARGUMENT, "fe_kv_select: null pointer");
   if (!aligned16(scores))
     return fail(FE_ERR_INVALID_ARGUMENT, "fe_kv_select: scores must be 16-byte aligned");
+  if (!aligned4(kept))
+    return fail(FE_ERR_INVALID_ARGUMENT, "fe_kv_select: kept must be 4-byte aligned");
   const SeqTable table{kv, pages, last, num_pages, page, cache_slots};
   auto s = static_cast<cudaStream_t>(stream);
   static std::atomic<uint64_t> done{0};
@@ -639,6 +641,8 @@ int fe_kv_compact(void* k_pool, void* v_pool, float* scores, const int32_t* kept
     return fail(FE_ERR_INVALID_ARGUMENT, "fe_kv_compact: null pointer");
   if (!aligned16(k_pool) || !aligned16(v_pool))
     return fail(FE_ERR_INVALID_ARGUMENT, "fe_kv_compact: pools must be 16-byte aligned");
+  if (!aligned4(scores) || !aligned4(kept))
+    return fail(FE_ERR_INVALID_ARGUMENT, "fe_kv_compact: scores and kept must be 4-byte aligned");
   MoveArgs a{};
   a.k = static_cast<uint4*>(k_pool);
   a.v = static_cast<uint4*>(v_pool);

@@ -787,6 +787,8 @@ int fe_scored_attn_run(fe_long_plan* p, const void* q, const void* k_pool, const
   rc = check_buffers(q, k_pool, v_pool, out, name);
   if (rc != FE_OK) return rc;
   if (!scores) return fail(FE_ERR_INVALID_ARGUMENT, name + ": null pointer");
+  if (!aligned4(scores))
+    return fail(FE_ERR_INVALID_ARGUMENT, name + ": scores must be 4-byte aligned");
   rc = maps(p, k_pool, v_pool);
   if (rc != FE_OK) return rc;
   auto s = static_cast<cudaStream_t>(stream);
