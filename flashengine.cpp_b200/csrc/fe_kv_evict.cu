@@ -436,10 +436,10 @@ __global__ void __launch_bounds__(kSelThreads, 3)
 // below 0. A CTA walks the list of one (sequence, head) in order, for one slice
 // of the row's 16-byte chunks (slices give one sequence's move more CTAs). A
 // table of the source and destination slots of kTableTokens tokens is made
-// first, so that the moves wait for no index. Each step moves rows * kMoveUnroll tokens: all of them are read before any is
-// written, and the sources of later steps lie at or past their own index
-// (kept[j] >= j, checked), which no earlier step writes; so the move works in
-// place.
+// first, so that the moves wait for no index. Each step moves rows *
+// kMoveUnroll tokens: all of them are read before any is written, and the
+// sources of later steps lie at or past their own index (kept[j] >= j, checked),
+// which no earlier step writes; so the move works in place.
 // ---------------------------------------------------------------------------
 constexpr int kMoveThreads = 256;
 constexpr int kMoveUnroll = 4;

@@ -440,10 +440,11 @@ int fe_kv8_attn_run(fe_attn_plan* plan, const void* q, const uint8_t* k_codes,
  * pages and capacities as for fe_attn_plan_create, metadata (HOST) and `graph` as
  * for fe_attn_plan_prepare. Prepare uploads to fixed buffers with one async copy
  * on `stream`: a graph that captured a run replays for later prepares of the same
- * batch and rows. A plan has one workspace (256 MiB of partial records, more in a
- * scored plan whose steps need it): its runs must not overlap on the GPU. Scale 1/sqrt(dim), fp32 softmax and accumulation,
- * softmax weights of about 16 bits in the second product, output rounded to
- * nearest even, as fe_attn_run.
+ * batch and rows. A plan has one workspace (256 MiB of partial records; a scored
+ * plan's steps of many rows may get a larger one of their own): its runs must not
+ * overlap on the GPU. Scale 1/sqrt(dim), fp32 softmax and accumulation, softmax
+ * weights of about 16 bits in the second product, output rounded to nearest even,
+ * as fe_attn_run.
  * ------------------------------------------------------------------------ */
 typedef struct fe_long_plan fe_long_plan;
 int fe_long_plan_destroy(fe_long_plan* plan);
