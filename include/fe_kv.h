@@ -443,8 +443,9 @@ int fe_kv8_attn_run(fe_attn_plan* plan, const void* q, const uint8_t* k_codes,
  * batch and rows. A plan has one workspace (256 MiB of partial records; a scored
  * plan's steps of many rows may get a larger one of their own): its runs must not
  * overlap on the GPU. Scale 1/sqrt(dim), fp32 softmax and accumulation, softmax
- * weights of about 16 bits in the second product, output rounded to nearest even,
- * as fe_attn_run.
+ * weights of about 16 bits in the second product (in f16, whose numbers end at
+ * 2^-24, to 2^-25 of a row's largest weight), output rounded to nearest even, as
+ * fe_attn_run.
  * ------------------------------------------------------------------------ */
 typedef struct fe_long_plan fe_long_plan;
 int fe_long_plan_destroy(fe_long_plan* plan);
